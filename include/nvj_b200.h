@@ -73,6 +73,25 @@ int nvj_compute_slot_mapping(const int32_t* positions, const int32_t* block_tabl
                              int table_rows, int table_width, int block_size,
                              int32_t* slot_mapping, nvj_stream_t stream);
 
+/*
+ * The layout of a packed step made on the device from its rows' lengths (the host builds the same in the reference,
+ * nanovllm_jax/engine/scheduler.py:734-1098).  Row r has cached_lens[r] tokens in the cache and gets new_lens[r] more:
+ *   need[r] = ceil((cached + new) / bs) - ceil(cached / bs) blocks are taken from free_blocks, in row order, from
+ *   free_head[0] on, and entered into block_tables[r] behind its ceil(cached / bs) entries;
+ *   seq_lens[r] = cached + new; query_start_loc [rows + 1] = running sum of new_lens; free_head_out[0] = free_head[0] + sum of need;
+ *   token i of row r: positions[i], token_row_ids[i] = r, slot_mapping[i] = entry * bs + position % bs; tokens of the bucket behind
+ *   the last row's get position 0, row 0 and slot -1.
+ * A row with a negative length, or more tokens than its table has room for, is flagged NVJ_DEV_BAD_LENGTH and gets no new tokens; tokens
+ * beyond the bucket are flagged the same way and left out (query_start_loc counts them).  Entries beyond the end of the free list
+ * become -1, and their tokens' slots, flagged NVJ_DEV_BAD_BLOCK_ID.  free_head_out may not be free_head.  At most 16384 rows, and
+ * rows * table_width * block_size below 2^31; NVJ_ERR_TOO_LARGE beyond.
+ */
+int nvj_build_packed_layout(const int32_t* cached_lens, const int32_t* new_lens, int rows, int32_t* block_tables,
+                            int table_width, int block_size, const int32_t* free_blocks, int free_count,
+                            const int32_t* free_head, int token_bucket, int32_t* positions, int32_t* token_row_ids,
+                            int32_t* slot_mapping, int32_t* query_start_loc, int32_t* seq_lens, int32_t* free_head_out,
+                            int32_t* status, nvj_stream_t stream);
+
 /* ------------------------------------------------------------------ append */
 
 /*
@@ -421,6 +440,68 @@ int nvj_paged_prefill_packed_counted(const void* q, int q_dtype,
                                      float* out, int32_t* status,
                                      void* workspace, size_t workspace_bytes, int variant,
                                      int part, int tile_pairs, nvj_stream_t stream);
+
+/* ---------------------------------------------------------- 8-bit cache */
+
+/*
+ * The paged cache held in 8 bits (no counterpart in the reference, whose cache types are bf16, f16 and f32).  One layer of K and of
+ * V: e4m3 numbers [num_blocks, block_size, num_kv_heads, head_dim] and a scale per block and kv head, f32
+ * [num_blocks, num_kv_heads]; a value is number * scale.  Scales are powers of two between 2^-117 and 2^119.  head_dim 64, 128 or
+ * 256, block_size 16, 32, 48 or 64, otherwise NVJ_ERR_UNSUPPORTED; data pointers 16-byte aligned.
+ */
+
+/*
+ * Append of new rows.  new_k / new_v [n_rows, n_cols, num_kv_heads, head_dim] bf16, f16 or f32; token i stands at positions[i] of its row
+ * (token_row_ids given: a packed batch of one row of n_cols tokens, token i of table row token_row_ids[i]; else row
+ * i / n_cols) and is written where the row's block table says.  A token counts under nvj_kv_append's rule for
+ * query_start_loc, and, with seq_lens given, if seq_lens[row] > 0.
+ *
+ * The tokens of a call that fall into one block have to stand together in the batch (any order among them); a row's
+ * consecutive positions do.  A block that two runs of tokens write in one call (two rows that share it) ends as either leaves it, or
+ * as a mixture.  For each run and kv head, K and V apart: a = the largest finite magnitude, e = the least integer with
+ * a <= 448 * 2^e.  If one of the tokens is the block's first (offset 0) the block begins anew with scale 2^e; otherwise its scale
+ * becomes max(scale, 2^e), and if it grows the numbers of the block's other rows are rescaled, rounded to nearest even.  New
+ * numbers are value / scale rounded to nearest even; magnitudes over 448 * scale (infinities among them) are held there, NaN is kept.
+ * A position outside the block table is flagged NVJ_DEV_BAD_LENGTH, a block id or table row outside its range
+ * NVJ_DEV_BAD_BLOCK_ID, and skipped.  Other blocks, and the other rows of a block whose scale stays, are left as they were.
+ */
+int nvj_kv_append_quantized(const void* new_k, const void* new_v, int src_dtype, const int32_t* positions,
+                            const int32_t* block_tables, const int32_t* token_row_ids, int table_rows, int table_width,
+                            const int32_t* query_start_loc, int qsl_rows, const int32_t* seq_lens, int n_rows, int n_cols,
+                            void* k_cache_layer, void* v_cache_layer, float* k_scale, float* v_scale, int64_t num_blocks,
+                            int block_size, int num_kv_heads, int head_dim, int32_t* status, nvj_stream_t stream);
+
+/*
+ * Attention for rows of `width` query tokens over the 8-bit cache: q [rows, width, num_q_heads, head_dim] bf16, f16 or f32; token t of row b
+ * attends keys p < seq_lens[b] and, with positions given ([rows, width]), p <= positions[b, t].  out as q, float32; a token that
+ * sees no key gets zeros.  Meant for few query tokens per row (one kernel serves width * num_q_heads / num_kv_heads <= 16 columns
+ * per pass over a row's keys); any width is taken.  query_start_loc given (width 1): q, positions and out are those of a packed batch, and
+ * the rows that hold exactly one token are served, nothing else is written.  The scale may be any number.
+ * A length beyond the block table is flagged and clipped, a block id outside the pool flagged and its keys left out.
+ */
+int nvj_paged_decode_quantized(const void* q, int q_dtype, const void* k_cache_layer, const void* v_cache_layer,
+                               const float* k_scale, const float* v_scale, int64_t num_blocks, int block_size,
+                               int num_kv_heads, int head_dim, int num_q_heads, const int32_t* block_tables, int table_width,
+                               const int32_t* seq_lens, const int32_t* positions, const int32_t* query_start_loc, int rows,
+                               int width, float scale, float* out, int32_t* status, nvj_stream_t stream);
+
+/*
+ * Ragged packed prefill attention over the 8-bit cache: masks, layout and padding as nvj_paged_prefill_packed.
+ *
+ *   single_rows  0: no row holds a single query token; otherwise such rows, if there are any, are served by the decode kernel
+ *   tile_pairs   as for nvj_paged_prefill_packed_counted (-1: not counted)
+ *   workspace    nullable scratch of nvj_paged_prefill_quantized_workspace_bytes(...): with it, bf16 queries of the model's
+ *                shape go to the tcgen05 tiles over bf16 pages that are written there; everything else, and a
+ *                call without it, to mma.sync tiles over the 8-bit blocks.  The size is 0 for calls that have no use for one.
+ */
+size_t nvj_paged_prefill_quantized_workspace_bytes(int q_dtype, int rows, int table_width, int block_size, int num_kv_heads,
+                                                   int head_dim, int num_q_heads, float scale);
+int nvj_paged_prefill_quantized(const void* q, int q_dtype, const void* k_cache_layer, const void* v_cache_layer,
+                                const float* k_scale, const float* v_scale, int64_t num_blocks, int block_size,
+                                int num_kv_heads, int head_dim, int num_q_heads, const int32_t* block_tables, int table_width,
+                                const int32_t* kv_lens, const int32_t* positions, const int32_t* query_start_loc, int rows,
+                                int token_bucket, float scale, float* out, int32_t* status, void* workspace,
+                                size_t workspace_bytes, int single_rows, int tile_pairs, nvj_stream_t stream);
 
 /* ------------------------------------------------------------------ copies */
 

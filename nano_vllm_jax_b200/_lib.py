@@ -75,6 +75,18 @@ SIGNATURES = {
                                                  c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p,
                                                  c_void_p, c_int, c_int, c_float, c_void_p, c_void_p,
                                                  c_void_p, c_size_t, c_int, c_int, c_int, c_void_p]),
+    "nvj_build_packed_layout": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_int,
+                                        c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "nvj_kv_append_quantized": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int,
+                                        c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int,
+                                        c_int, c_void_p, c_void_p]),
+    "nvj_paged_decode_quantized": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_int,
+                                           c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_float, c_void_p,
+                                           c_void_p, c_void_p]),
+    "nvj_paged_prefill_quantized_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float]),
+    "nvj_paged_prefill_quantized": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_int,
+                                            c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_float, c_void_p,
+                                            c_void_p, c_void_p, c_size_t, c_int, c_int, c_void_p]),
     "nvj_copy_blocks": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p,
                                 c_void_p, c_int, c_void_p, c_void_p]),
     "nvj_hybrid_snapshot": (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int64,

@@ -24,13 +24,14 @@ import torch
 
 from . import kv_cache as kvc
 from .kernels import paged_kv as _k
-from .kv_cache import AttentionMetadata, KVCacheSpec, KVCacheStorage
+from .kernels import quantized_kv as _q
+from .kv_cache import AttentionMetadata, KVCacheSpec, KVCacheStorage, QuantizedKVCacheStorage
 
 B200_IMPL = "b200"
 
 _CACHE_DTYPES = {"default": None, "bf16": torch.bfloat16, "bfloat16": torch.bfloat16,
                  "fp16": torch.float16, "float16": torch.float16, "fp32": torch.float32,
-                 "float32": torch.float32}
+                 "float32": torch.float32, "fp8": torch.float8_e4m3fn, "float8_e4m3fn": torch.float8_e4m3fn}
 
 
 def normalize_full_attention_impl(value: Optional[str]) -> str:
@@ -46,7 +47,7 @@ _OFF_VALUES = {"", "0", "false", "no", "off", "none"}
 
 
 def full_attention_kv_cache_dtype(default_dtype, config=None):
-    """`full_attention_kv_cache_dtype` override (backends.py:100-118): default | bf16 | fp16 | fp32 | off.
+    """`full_attention_kv_cache_dtype` override (backends.py:100-118): default | bf16 | fp16 | fp32 | off, and fp8 here.
 
     As in the reference (backends.py:74-80) the environment variable
     NANO_VLLM_JAX_FULL_ATTN_KV_CACHE_DTYPE wins over the config attribute.
@@ -61,7 +62,7 @@ def full_attention_kv_cache_dtype(default_dtype, config=None):
     if name == "default" or name in _OFF_VALUES:
         return default_dtype
     if name not in _CACHE_DTYPES:
-        raise ValueError(f"Unknown {_CACHE_DTYPE_ENV}={name!r}; expected fp32, bf16, fp16, default, or off")
+        raise ValueError(f"Unknown {_CACHE_DTYPE_ENV}={name!r}; expected fp32, bf16, fp16, default, or off; fp8 for an 8-bit cache")
     return _CACHE_DTYPES[name]
 
 
@@ -82,6 +83,8 @@ class B200Backend:
     def allocate_kv_cache(self, spec: KVCacheSpec, max_seqs: int, max_blocks_per_seq: int) -> KVCacheStorage:
         dtype = full_attention_kv_cache_dtype(spec.dtype, self.config)
         capped = replace(spec, dtype=dtype)
+        if dtype == torch.float8_e4m3fn:
+            return kvc.init_quantized_kv_cache(capped, device=self.device)
         capped = replace(capped, num_blocks=kvc.cap_num_kv_cache_blocks(capped))
         state = kvc.init_kv_cache(capped.num_blocks, capped.block_size, capped.num_kv_heads, capped.head_dim,
                                   max_seqs, max_blocks_per_seq, num_layers=capped.num_layers, dtype=dtype,
@@ -192,6 +195,8 @@ class B200Backend:
 
     # ---- append (backends.py:980-1067)
     def write_kv(self, layer_id, k, v, cache: KVCacheStorage, metadata: AttentionMetadata) -> KVCacheStorage:
+        if type(cache) is QuantizedKVCacheStorage:
+            return self._write_quantized(layer_id, k, v, cache, metadata)
         unread = metadata.__dict__["slot_mapping"]
         if type(unread) is kvc.SlotsFromTables:
             done = _k.host().append(k, v, cache.k_cache, cache.v_cache, layer_id, None, unread.positions, unread.block_tables,
@@ -212,6 +217,8 @@ class B200Backend:
     # ---- attention (backends.py:1069-1250)
     def attention(self, layer_id, query, cache: KVCacheStorage, metadata: AttentionMetadata, block_size,
                   scale, num_key_value_groups, is_prefill):
+        if type(cache) is QuantizedKVCacheStorage:
+            return self._attend_quantized(layer_id, query, cache, metadata, block_size, scale, num_key_value_groups, is_prefill)
         f32 = torch.float32
         if is_prefill:
             if metadata.token_row_ids is not None:
@@ -250,6 +257,9 @@ class B200Backend:
     # ---- fused boundary (backends.py:1252-1461)
     def write_kv_and_attention(self, layer_id, query, k, v, cache: KVCacheStorage, metadata: AttentionMetadata,
                                block_size, scale, num_key_value_groups, is_prefill):
+        if type(cache) is QuantizedKVCacheStorage:
+            self._write_quantized(layer_id, k, v, cache, metadata)
+            return cache, self._attend_quantized(layer_id, query, cache, metadata, block_size, scale, num_key_value_groups, is_prefill)
         if not is_prefill and metadata.positions is not None:  # one token per row on the 5-D cache; anything else comes back as None
             out = _k.host().fused_decode(query, k, v, cache.k_cache, cache.v_cache, metadata.block_tables, metadata.seq_lens,
                                          metadata.positions, layer_id, block_size, scale, num_key_value_groups, 0, None, None)
@@ -266,6 +276,44 @@ class B200Backend:
         storage = self.write_kv(layer_id, k, v, cache, metadata)
         out = self.attention(layer_id, query, storage, metadata, block_size, scale, num_key_value_groups, is_prefill)
         return storage, out
+
+
+    # ---- the same over a cache held in 8 bits (kernels/quantized_kv.py); blocks are written by position, so positions are required
+    def _write_quantized(self, layer_id, k, v, cache: QuantizedKVCacheStorage, metadata: AttentionMetadata) -> KVCacheStorage:
+        if metadata.positions is None:
+            raise ValueError("metadata.positions is required for an append to an 8-bit cache")
+        i32 = torch.int32
+        ids = None if metadata.token_row_ids is None else metadata.token_row_ids.to(i32)
+        _q.kv_append_quantized(k, v, *cache.layer(layer_id), metadata.positions.to(i32), metadata.block_tables.to(i32),
+                               query_start_loc=metadata.query_start_loc.to(i32), token_row_ids=ids, seq_lens=metadata.seq_lens.to(i32))
+        return cache
+
+    def _attend_quantized(self, layer_id, query, cache: QuantizedKVCacheStorage, metadata: AttentionMetadata, block_size, scale,
+                          num_key_value_groups, is_prefill):
+        if metadata.positions is None:
+            raise ValueError("metadata.positions is required for attention over an 8-bit cache")
+        i32 = torch.int32
+        tables, lens, positions = metadata.block_tables.to(i32), metadata.seq_lens.to(i32), metadata.positions.to(i32)
+        layer = cache.layer(layer_id)
+        if block_size != layer[0].shape[1] or query.shape[2] != layer[0].shape[2] * num_key_value_groups:
+            raise ValueError("query / cache shapes do not agree")
+        if metadata.token_row_ids is not None:
+            return _q.packed_paged_prefill_attention_quantized(
+                query, *layer, tables, lens, positions, metadata.query_start_loc.to(i32), block_size, scale, num_key_value_groups,
+                num_decode_rows=metadata.single_token_rows, query_tile_pairs=metadata.query_tile_pairs)
+        batch, width = query.shape[:2]
+        if positions.shape[0] != tables.shape[0]:
+            raise ValueError("positions and block_tables batch dimensions must match")
+        if metadata.max_kv_len is not None and metadata.max_kv_len < tables.shape[1] * block_size:
+            lens = lens.clamp(max=int(metadata.max_kv_len))
+        if is_prefill and width * num_key_value_groups > _q.DECODE_COLUMNS:
+            # a rectangular batch is a packed batch with rows of equal width
+            qsl = torch.arange(batch + 1, dtype=i32, device=query.device) * width
+            out = _q.packed_paged_prefill_attention_quantized(
+                query.reshape(1, batch * width, *query.shape[2:]), *layer, tables, lens, positions.reshape(1, -1), qsl, block_size, scale,
+                num_key_value_groups, num_decode_rows=0)
+            return out.reshape(batch, width, -1)
+        return _q.paged_decode_attention_quantized(query, *layer, tables, lens, scale, positions=positions)
 
 
 def select_backend(name: Optional[str] = None, config=None, device="cuda") -> B200Backend:

@@ -1,0 +1,232 @@
+// Append of new K/V rows to the 8-bit paged cache (quantized_kv.cuh).
+//
+// A block's tokens share a scale per kv head, so the unit of work is not a token but a run: the tokens of one call that stand
+// together in the batch and fall into one block.  One warp takes a run's rows of K, or of V, of one kv head: it finds their largest
+// magnitude in registers, settles the block's scale, rescales the rows that were there if the scale has to grow, and stores the new
+// ones.  K and V, and the heads, are warps of their own; nothing is shared between warps, so there are no atomics and no
+// second pass over memory.  bytes = tokens * kv_heads * head_dim * 2 * (source size + 1), bound by HBM for prompts, by the chain
+// positions -> block id -> scale -> store for a decode step.
+
+#include "quantized_kv.cuh"
+
+namespace nvj {
+
+struct QAppendParams {
+  const void* new_k;
+  const void* new_v;
+  uint8_t* k_cache;
+  uint8_t* v_cache;
+  float* k_scale;
+  float* v_scale;
+  const int32_t* positions;
+  const int32_t* block_tables;
+  const int32_t* token_row_ids;    // packed batches
+  const int32_t* query_start_loc;  // nullable
+  const int32_t* seq_lens;         // nullable: rows with seq_lens[r] <= 0 are skipped
+  int32_t* status;
+  long long num_blocks;
+  int qsl_rows, packed, n_tokens, n_cols, table_rows, table_width, block_size, num_kv_heads;
+};
+
+// What a lane knows about one token of the batch: its row's place in the block table, or -1 for a token that is not written.
+struct QToken {
+  long long entry;  // row * table_width + block of the row
+  int offset;       // within the block
+};
+
+__device__ __forceinline__ QToken q_token(const QAppendParams& p, int i) {
+  QToken t{-1, 0};
+  if (i < 0 || i >= p.n_tokens) return t;
+  const int pos = p.positions[i];
+  int row = p.packed ? p.token_row_ids[i] : i / p.n_cols;
+  if (p.query_start_loc) {
+    if (p.packed) {
+      if (i >= p.query_start_loc[p.qsl_rows]) return t;
+    } else {
+      if (row >= p.qsl_rows || i - row * p.n_cols >= p.query_start_loc[row + 1] - p.query_start_loc[row]) return t;
+    }
+  }
+  if (row < 0 || row >= p.table_rows) {
+    atomicOr(p.status, NVJ_DEV_BAD_BLOCK_ID);
+    return t;
+  }
+  if (p.seq_lens && p.seq_lens[row] <= 0) return t;
+  if (pos < 0 || pos / p.block_size >= p.table_width) {
+    atomicOr(p.status, NVJ_DEV_BAD_LENGTH);
+    return t;
+  }
+  t.entry = (long long)row * p.table_width + pos / p.block_size;
+  t.offset = pos % p.block_size;
+  return t;
+}
+
+// One run: `n` tokens from `first` on, offsets[] as q_token gives them.  kLanes lanes hold a row of 8 * kLanes elements.
+template <typename T, int kD>
+__device__ void q_append_run(const QAppendParams& p, int first, int n, long long entry, int head, bool is_v, int lane) {
+  constexpr int kLanes = kD / 8, kRows = 32 / kLanes;  // lanes of a row, rows of a step
+  constexpr int kHold = sizeof(T) == 4 ? 8 : 16;       // steps whose rows stay in registers between the two looks at them
+  const int col = (lane % kLanes) * 8, sub = lane / kLanes;
+  const long long token_stride = (long long)p.num_kv_heads * kD;
+  const T* src = static_cast<const T*>(is_v ? p.new_v : p.new_k) + (long long)first * token_stride + (long long)head * kD + col;
+  const int id = p.block_tables[entry];
+  const int steps = (n + kRows - 1) / kRows;
+  QRaw<T> held[kHold];
+#pragma unroll
+  for (int s = 0; s < kHold; ++s)
+    if (s < steps && s * kRows + sub < n) held[s] = q_load8(src + (long long)(s * kRows + sub) * token_stride);
+  if (id < 0 || id >= p.num_blocks) {
+    if (lane == 0) atomicOr(p.status, NVJ_DEV_BAD_BLOCK_ID);
+    return;
+  }
+  float* scale_at = (is_v ? p.v_scale : p.k_scale) + (long long)id * p.num_kv_heads + head;
+  const float before = *scale_at;
+  // the offsets of up to 32 tokens at a time, one per lane; whether the block begins here, and which of its rows are new
+  bool begins = false;
+  unsigned fresh[2] = {0u, 0u};  // offsets 0 - 31 and 32 - 63
+  for (int c = 0; c < n; c += 32) {
+    const int o = c + lane < n ? p.positions[first + c + lane] % p.block_size : -1;
+    begins |= __any_sync(kFullMask, o == 0);
+    fresh[0] |= __reduce_or_sync(kFullMask, o >= 0 && o < 32 ? 1u << o : 0u);
+    fresh[1] |= __reduce_or_sync(kFullMask, o >= 32 ? 1u << (o - 32) : 0u);
+  }
+  float largest = 0.f, x[8];
+#pragma unroll
+  for (int s = 0; s < kHold; ++s)
+    if (s < steps && s * kRows + sub < n) {
+      q_floats(held[s], x);
+      largest = q_largest(largest, x);
+    }
+  for (int s = kHold; s < steps; ++s)
+    if (s * kRows + sub < n) {
+      q_floats(q_load8(src + (long long)(s * kRows + sub) * token_stride), x);
+      largest = q_largest(largest, x);
+    }
+  largest = __int_as_float(__reduce_max_sync(kFullMask, __float_as_int(largest)));
+  const float wanted = q_scale_for(largest);
+  const float scale = begins ? wanted : fmaxf(wanted, before);
+  uint8_t* base = (is_v ? p.v_cache : p.k_cache) + ((long long)id * p.block_size * p.num_kv_heads + head) * kD + col;
+  if (scale != before && lane == 0) *scale_at = scale;
+  if (!begins && scale > before) {  // the rows that were there, in the new unit
+    const float ratio = before / scale;
+    for (int o = sub; o < p.block_size; o += kRows) {
+      if (fresh[o >> 5] >> (o & 31) & 1) continue;
+      uint2* at = reinterpret_cast<uint2*>(base + (long long)o * token_stride);
+      const uint2 w = *at;
+      const float2 a = q_float2(q_half2(w.x)), b = q_float2(q_half2_high(w.x)), c = q_float2(q_half2(w.y)), d = q_float2(q_half2_high(w.y));
+      *at = make_uint2(q_pack2(a.x * ratio, a.y * ratio) | q_pack2(b.x * ratio, b.y * ratio) << 16,
+                       q_pack2(c.x * ratio, c.y * ratio) | q_pack2(d.x * ratio, d.y * ratio) << 16);
+    }
+  }
+  const float inverse = 1.f / scale;
+  auto store = [&](int r, const QRaw<T>& raw) {
+    q_floats(raw, x);
+    const int o = p.positions[first + r] % p.block_size;
+    *reinterpret_cast<uint2*>(base + (long long)o * token_stride) =
+        make_uint2(q_pack2(x[0] * inverse, x[1] * inverse) | q_pack2(x[2] * inverse, x[3] * inverse) << 16,
+                   q_pack2(x[4] * inverse, x[5] * inverse) | q_pack2(x[6] * inverse, x[7] * inverse) << 16);
+  };
+#pragma unroll
+  for (int s = 0; s < kHold; ++s)
+    if (s < steps && s * kRows + sub < n) store(s * kRows + sub, held[s]);
+  for (int s = kHold; s < steps; ++s)
+    if (s * kRows + sub < n) store(s * kRows + sub, q_load8(src + (long long)(s * kRows + sub) * token_stride));
+}
+
+// Grid x: windows of `window` tokens; grid y: 2 * num_kv_heads (K, V of each head).  A window's warps take the runs that begin in it
+// in turn.
+constexpr int kQAppendWarps = 4;
+template <typename T, int kD>
+__global__ void __launch_bounds__(32 * kQAppendWarps) quantized_append_kernel(QAppendParams p, int window) {
+  pdl_wait();
+  pdl_release();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int task = window == 1 ? blockIdx.x * kQAppendWarps + warp : blockIdx.x;
+  const int base = task * window;  // first token of the window
+  if (base >= p.n_tokens) return;
+  const int head = blockIdx.y >> 1;
+  const bool is_v = blockIdx.y & 1;
+  // lane l looks at token base - 1 + l: the one in front tells whether the window's first token begins a run
+  const QToken t = q_token(p, base - 1 + lane);
+  const long long in_front = __shfl_up_sync(kFullMask, t.entry, 1);
+  const bool same = lane > 0 && t.entry >= 0 && t.entry == in_front;
+  const unsigned chain = __ballot_sync(kFullMask, same);
+  unsigned starts = __ballot_sync(kFullMask, lane > 0 && lane <= window && t.entry >= 0 && !same);
+  for (int k = 0; starts; ++k, starts &= starts - 1) {
+    if (window > 1 && k % kQAppendWarps != warp) continue;
+    const int at = __ffs(starts) - 1;  // lane of the run's first token
+    const long long entry = __shfl_sync(kFullMask, t.entry, at);
+    const int first = base - 1 + at;
+    const unsigned follow = at == 31 ? 0u : ~(chain >> (at + 1));  // bit j clear: token first + 1 + j is of the run
+    int n = 1 + (follow ? __ffs(follow) - 1 : 32);
+    if (at + n > 31) {  // the run may go on behind what the lanes have seen
+      n = 32 - at;
+      for (;;) {
+        const unsigned more = __ballot_sync(kFullMask, q_token(p, first + n + lane).entry == entry);
+        const int add = more == kFullMask ? 32 : __ffs(~more) - 1;
+        n += add;
+        if (add < 32) break;
+      }
+    }
+    q_append_run<T, kD>(p, first, n, entry, head, is_v, lane);
+  }
+}
+
+template <typename T>
+static int launch_quantized_append(const QAppendParams& p, int head_dim, cudaStream_t stream) {
+  // A token per warp while the warps find a place at once, 16 tokens per CTA beyond: see the launch below.
+  const int window = (long long)p.n_tokens * p.num_kv_heads * 2 <= 148LL * 64 ? 1 : 16;
+  const int per = window == 1 ? kQAppendWarps : window;
+  const dim3 grid((p.n_tokens + per - 1) / per, 2 * p.num_kv_heads);
+  auto go = [&](auto* kernel) {
+    return launch_after(kernel, grid, dim3(32 * kQAppendWarps), 0, stream, p, window) == cudaSuccess ? NVJ_OK : NVJ_ERR_LAUNCH;
+  };
+  if (head_dim == 256) return go(quantized_append_kernel<T, 256>);
+  if (head_dim == 128) return go(quantized_append_kernel<T, 128>);
+  return go(quantized_append_kernel<T, 64>);
+}
+
+}  // namespace nvj
+
+extern "C" int nvj_kv_append_quantized(const void* new_k, const void* new_v, int src_dtype, const int32_t* positions,
+                                       const int32_t* block_tables, const int32_t* token_row_ids, int table_rows, int table_width,
+                                       const int32_t* query_start_loc, int qsl_rows, const int32_t* seq_lens, int n_rows, int n_cols,
+                                       void* k_cache_layer, void* v_cache_layer, float* k_scale, float* v_scale, int64_t num_blocks,
+                                       int block_size, int num_kv_heads, int head_dim, int32_t* status, nvj_stream_t stream) {
+  using namespace nvj;
+  if (n_rows < 0 || n_cols < 0 || table_rows < 0 || table_width < 0 || qsl_rows < 0 || num_blocks < 0) return NVJ_ERR_INVALID_ARGUMENT;
+  if (src_dtype < NVJ_BF16 || src_dtype > NVJ_F32 || !quantized_cache_shape_ok(block_size, num_kv_heads, head_dim)) return NVJ_ERR_UNSUPPORTED;
+  const long long n = (long long)n_rows * n_cols;
+  if (n == 0) return NVJ_OK;
+  if (n > 0x7fffffffLL - 64) return NVJ_ERR_TOO_LARGE;
+  if (!new_k || !new_v || !positions || !block_tables || !k_cache_layer || !v_cache_layer || !k_scale || !v_scale || !status)
+    return NVJ_ERR_INVALID_ARGUMENT;
+  if (!aligned16(new_k) || !aligned16(new_v) || !aligned16(k_cache_layer) || !aligned16(v_cache_layer)) return NVJ_ERR_INVALID_ARGUMENT;
+  if (table_rows == 0 || table_width == 0 || num_blocks == 0) return NVJ_ERR_INVALID_ARGUMENT;
+  if (token_row_ids && n_rows != 1) return NVJ_ERR_INVALID_ARGUMENT;
+  QAppendParams p{};
+  p.new_k = new_k;
+  p.new_v = new_v;
+  p.k_cache = static_cast<uint8_t*>(k_cache_layer);
+  p.v_cache = static_cast<uint8_t*>(v_cache_layer);
+  p.k_scale = k_scale;
+  p.v_scale = v_scale;
+  p.positions = positions;
+  p.block_tables = block_tables;
+  p.token_row_ids = token_row_ids;
+  p.query_start_loc = query_start_loc;
+  p.seq_lens = seq_lens;
+  p.status = status;
+  p.num_blocks = num_blocks;
+  p.qsl_rows = qsl_rows;
+  p.packed = token_row_ids != nullptr;
+  p.n_tokens = (int)n;
+  p.n_cols = n_cols;
+  p.table_rows = table_rows;
+  p.table_width = table_width;
+  p.block_size = block_size;
+  p.num_kv_heads = num_kv_heads;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (src_dtype == NVJ_BF16) return launch_quantized_append<__nv_bfloat16>(p, head_dim, s);
+  if (src_dtype == NVJ_F16) return launch_quantized_append<__half>(p, head_dim, s);
+  return launch_quantized_append<float>(p, head_dim, s);
+}

@@ -1,0 +1,555 @@
+// Paged attention over the 8-bit cache (quantized_kv.cuh) for rows of few query tokens: decode and verification of speculated tokens.
+//
+//   out[t, h] = sum_p w_p v_p / sum_p w_p,  w_p = exp(scale * q[t, h] . k_p),  p < len and p <= position[t]
+//
+// Bound by the bytes of K and V: 2 * kv_heads * head_dim per key, half of the bf16 cache's.  At the same byte rate an SM meets twice
+// as many numbers per second as over bf16, so what a number costs in instructions decides:
+//   * one thread-block cluster per (row, kv head, tile of query columns), a warp per 16-key tile, tiles dealt to the
+//     cluster's warps in turn: no scan of the lengths, no workspace, no counter; warps merge through shared memory, CTAs through
+//     distributed shared memory;
+//   * K and V go from global memory to registers in 16-byte pieces and nowhere else: both products are taken transposed
+//     (S^T = K Q^T, O^T = V^T P^T), and since the order of a contraction is free, the 16 bytes that a lane holds of a
+//     row ARE its operands, permuted the same way on the other side.  No shared memory, no ldmatrix on the way;
+//   * e4m3 becomes f16 exactly, two numbers per instruction; V takes one byte permute per two numbers besides, which pairs its keys;
+//   * f16 queries times a power of two per column (exact for bf16 and f16; f32 queries go as a high and a low term), weights as
+//     a high and a low f16 term: products as good as in f32.  With up to four columns the two terms of the weights are the
+//     two halves of the eight columns of one mma.sync, with more they are two of them;
+//   * the K scale of a block multiplies its scores, the V scale goes into the exponent of the weights: a running maximum of
+//     its own for the weighted sum keeps blocks of any scale apart from the sum of the weights.
+// Maxima are lazy: only a score that passes its column's maximum by 2^8 (one vote per tile) rescales the sums.
+
+#include "cluster.cuh"
+#include "quantized_kv.cuh"
+
+namespace nvj {
+
+struct QDecodeParams {
+  const void* q;
+  const uint8_t* k_cache;
+  const uint8_t* v_cache;
+  const float* k_scale;
+  const float* v_scale;
+  const int32_t* block_tables;
+  const int32_t* seq_lens;
+  const int32_t* positions;        // nullable: [rows, width], packed: per token
+  const int32_t* query_start_loc;  // packed: the rows of one query token are served, the others left alone
+  float* out;
+  int32_t* status;
+  long long num_blocks;
+  int rows, width, table_width, block_size, num_kv_heads, groups;
+  int column_tiles;  // tiles of query columns of a row and kv head
+  float scale_log2;  // scale * log2(e)
+};
+
+constexpr int kQdWarps = 4, kQdThreads = 32 * kQdWarps;
+constexpr float kQdNone = -3e38f;  // a maximum that no score has touched
+constexpr float kQdSlack = 8.f;    // weights may reach 2^8 before the sums are rescaled
+
+// Shared memory: the queries as f16 while the tiles are walked, then each warp's sums.
+// kTiles: mma column tiles of 8.  kPack: at most four columns, the low term of the weights in columns 4 - 7.  kF32: f32 queries.
+template <int kD, int kTiles, bool kPack, bool kF32>
+struct QdShape {
+  static constexpr int kCols = kPack ? 4 : 8 * kTiles;  // query columns
+  static constexpr int kQCols = 8 * kTiles;             // columns of the operand
+  static constexpr int kQPitch = kD + 8;                // f16 elements; two columns' pieces fall into different banks
+  static constexpr int kQTerms = kF32 && !kPack ? 2 : 1;
+  static constexpr int kQBytes = kQTerms * kQCols * kQPitch * 2;
+  static constexpr int kAccPitch = kD + 4;  // floats
+  static constexpr int kAccBytes = kQdWarps * kCols * kAccPitch * 4;
+  static constexpr int kBytes = kQBytes > kAccBytes ? kQBytes : kAccBytes;
+};
+
+template <typename T, int kD, int kTiles, bool kPack>
+__global__ void __launch_bounds__(kQdThreads, kPack && kD == 256 ? 3 : 1) quantized_decode_kernel(QDecodeParams p, int ctas) {
+  constexpr bool kF32 = std::is_same<T, float>::value;
+  using S = QdShape<kD, kTiles, kPack, kF32>;
+  constexpr int kCols = S::kCols, kParts = kD / 64;  // parts of 64 dims: one 16-byte piece per lane and key row
+  constexpr int kVHalves = kD >= 128 ? kD / 128 : 1;  // parts of 128 dims of V (64: 8-byte pieces)
+  constexpr int kVWords = kD >= 128 ? 4 : 2;          // words of a V piece
+  constexpr int kMTiles = kD / 16;
+  extern __shared__ __align__(16) char qd_smem[];
+  __shared__ float qd_factor[S::kQCols];                  // what the products of a column are to be multiplied by
+  __shared__ float2 qd_ml[kQdWarps][kCols];               // a warp's maximum and sum
+  __shared__ float qd_mv[kQdWarps][kCols];                // ... and the reference of its weighted sums
+  __shared__ float2 qd_ML[kCols];                         // the CTA's
+  __half* qs = reinterpret_cast<__half*>(qd_smem);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int rank = ctas > 1 ? (int)cl_rank() : 0;
+  const int row = blockIdx.x / ctas;
+  const int head = blockIdx.y / p.column_tiles, ct = blockIdx.y % p.column_tiles;
+  const int hq = p.num_kv_heads * p.groups;
+  pdl_wait();
+  pdl_release();
+
+  // the row's first query token and how many it has; a packed batch's rows of several tokens are not ours
+  int token = row * p.width, width = p.width, live = 1;
+  if (p.query_start_loc) {
+    token = p.query_start_loc[row];
+    width = 1;
+    live = p.query_start_loc[row + 1] - token == 1;
+  }
+  const int columns = width * p.groups;  // of the row and kv head: column c = (token c / groups, head c % groups)
+  int len = p.seq_lens[row];
+  const int step = ctas * kQdWarps;
+  int tile = rank * kQdWarps + warp;  // this warp's tiles: tile, tile + step, ..
+  const int per_block = p.block_size >> 4;
+  const int32_t* table = p.block_tables + (long long)row * p.table_width;
+  // ids of this warp's next 32 tiles, one per lane (a table entry exists whatever the length is)
+  auto fetch_id = [&](int first) {
+    const int b = (first + lane * step) / per_block;
+    return b < p.table_width ? table[b] : -1;
+  };
+  int id = fetch_id(tile);
+  if (!live) len = 0;
+  if (len > p.table_width * (long long)p.block_size) {
+    if (threadIdx.x == 0 && rank == 0) atomicOr(p.status, NVJ_DEV_BAD_LENGTH);
+    len = p.table_width * p.block_size;
+  }
+  const int tiles = (len + 15) >> 4;
+  float ks = 0.f, lv = 0.f;  // scales of this lane's tile: of K, and log2 of V's
+  auto fetch_scales = [&](int first) {
+    const bool used = first + lane * step < tiles;
+    if (used && (id < 0 || id >= p.num_blocks)) {
+      atomicOr(p.status, NVJ_DEV_BAD_BLOCK_ID);
+      id = -1;
+    }
+    if (used && id >= 0) {
+      ks = p.k_scale[(long long)id * p.num_kv_heads + head];
+      lv = p.v_scale[(long long)id * p.num_kv_heads + head];
+    }
+  };
+  const long long key_stride = (long long)p.num_kv_heads * kD;
+  uint4 kr[kParts][2];                // keys g and g + 8: dims 64 part + 16 t ..
+  uint4 vr[kVHalves][4];              // keys 2t, 2t + 1, 2t + 8, 2t + 9: dims 128 half + 16 g .. (64 dims: 8 g ..)
+  auto load_k = [&](int tile_id, int which) {
+    if (tile_id < 0) {
+#pragma unroll
+      for (int s = 0; s < kParts; ++s) kr[s][0] = kr[s][1] = make_uint4(0, 0, 0, 0);
+      return;
+    }
+    const uint8_t* at = p.k_cache + (((long long)tile_id * p.block_size + (which % per_block) * 16 + g) * p.num_kv_heads + head) * kD + 16 * t;
+#pragma unroll
+    for (int s = 0; s < kParts; ++s) {
+      kr[s][0] = ld_stream_u4(at + 64 * s);
+      kr[s][1] = ld_stream_u4(at + 8 * key_stride + 64 * s);
+    }
+  };
+  auto load_v = [&](int tile_id, int which) {
+    const int first = which * 16 + 2 * t;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int key = (k & 1) + 8 * (k >> 1);  // behind 2t
+      // keys behind the row's last one hold anything: they must not reach a product
+      const bool ok = tile_id >= 0 && first + key < len;
+      const uint8_t* at = p.v_cache + (((long long)tile_id * p.block_size + (which % per_block) * 16 + 2 * t + key) * p.num_kv_heads + head) * kD;
+#pragma unroll
+      for (int h = 0; h < kVHalves; ++h) {
+        vr[h][k] = make_uint4(0, 0, 0, 0);
+        if (ok) {
+          if constexpr (kD >= 128) {
+            vr[h][k] = ld_stream_u4(at + 128 * h + 16 * g);
+          } else {
+            const uint2 w = *reinterpret_cast<const uint2*>(at + 8 * g);
+            vr[h][k].x = w.x;
+            vr[h][k].y = w.y;
+          }
+        }
+      }
+    }
+  };
+
+  int slot = 0;  // lane that holds the current tile's id and scales
+  if (tile < tiles) {
+    fetch_scales(tile);
+    const int first_id = __shfl_sync(kFullMask, id, 0);
+    load_k(first_id, tile);
+    load_v(first_id, tile);
+  }
+
+  // queries into shared memory: a warp a column at a time, lane l the dims 8 l .. (f16 after a power of two that brings the largest
+  // magnitude next to 2^14, so that numbers down to 2^-28 of it keep 11 bits)
+  for (int c = warp; c < S::kQCols; c += kQdWarps) {
+    const int col = kPack ? (c & 3) : c;
+    const int at = ct * kCols + col;
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = 0.f;
+    if (live && at < columns && lane < kD / 8)
+      q_floats(q_load8(static_cast<const T*>(p.q) + ((long long)(token + at / p.groups) * hq + head * p.groups + at % p.groups) * kD + 8 * lane), x);
+    float largest = 0.f;
+    largest = q_largest(largest, x);
+    const int bits = __reduce_max_sync(kFullMask, __float_as_int(largest));
+    int e = (bits >> 23) - 127 - 14;  // largest = 2^(e + 14) * [1, 2)
+    e = bits == 0 ? 0 : (e < -126 ? -126 : e);
+    const float down = q_pow2(-e > 126 ? 126 : -e);
+    if (lane == 0) qd_factor[c] = q_pow2(e) * p.scale_log2;
+    if (lane < kD / 8) {
+      uint32_t w[4], low[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float a = x[2 * i] * down, b = x[2 * i + 1] * down;
+        w[i] = q_pair(a, b);
+        low[i] = q_pair_rest(a, b, w[i]);
+      }
+      const bool second = kF32 && kPack && c >= 4;  // packed f32 queries: columns 4 - 7 hold the low terms
+      uint4* at4 = reinterpret_cast<uint4*>(qs + c * S::kQPitch + 8 * lane);
+      *at4 = second ? make_uint4(low[0], low[1], low[2], low[3]) : make_uint4(w[0], w[1], w[2], w[3]);
+      if constexpr (S::kQTerms == 2)
+        *reinterpret_cast<uint4*>(qs + (S::kQCols + c) * S::kQPitch + 8 * lane) = make_uint4(low[0], low[1], low[2], low[3]);
+    }
+  }
+  __syncthreads();
+
+  // this lane's columns 2t, 2t + 1 of each column tile
+  float factor[kTiles][2], m[kTiles][2], mv[kTiles][2], l[kTiles][2];
+  int limit[kTiles][2];
+#pragma unroll
+  for (int j = 0; j < kTiles; ++j)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int c = 8 * j + 2 * t + i, at = ct * kCols + (kPack ? (c & 3) : c);
+      factor[j][i] = qd_factor[c];
+      m[j][i] = mv[j][i] = kQdNone;
+      l[j][i] = 0.f;
+      limit[j][i] = len;
+      if (p.positions && at < columns) {
+        const int last = p.positions[token + at / p.groups];
+        limit[j][i] = last < len ? last + 1 : len;
+      }
+    }
+  float acc[kTiles][kMTiles][4];
+#pragma unroll
+  for (int j = 0; j < kTiles; ++j)
+#pragma unroll
+    for (int i = 0; i < kMTiles; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) acc[j][i][k] = 0.f;
+
+  while (tile < tiles) {
+    const float k_unit = __shfl_sync(kFullMask, ks, slot), v_log = __log2f(__shfl_sync(kFullMask, lv, slot));
+    const bool usable = __shfl_sync(kFullMask, id, slot) >= 0;
+    // S^T = K Q^T: rows keys, columns queries
+    float s[kTiles][4];
+#pragma unroll
+    for (int j = 0; j < kTiles; ++j)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) s[j][k] = 0.f;
+#pragma unroll
+    for (int part = 0; part < kParts; ++part) {
+      const uint32_t lo[4] = {kr[part][0].x, kr[part][0].y, kr[part][0].z, kr[part][0].w};
+      const uint32_t hi[4] = {kr[part][1].x, kr[part][1].y, kr[part][1].z, kr[part][1].w};
+#pragma unroll
+      for (int j = 0; j < kTiles; ++j)
+#pragma unroll
+        for (int term = 0; term < S::kQTerms; ++term) {
+          const uint4* b4 = reinterpret_cast<const uint4*>(qs + ((term * kTiles + j) * 8 + g) * S::kQPitch + 64 * part + 16 * t);
+          const uint4 b0 = b4[0], b1 = b4[1];
+          const uint32_t b[8] = {b0.x, b0.y, b0.z, b0.w, b1.x, b1.y, b1.z, b1.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            q_mma(s[j], q_half2(lo[k]), q_half2(hi[k]), q_half2_high(lo[k]), q_half2_high(hi[k]), b[2 * k], b[2 * k + 1]);
+        }
+    }
+    // the next tile's K rows
+    const int this_tile = tile;
+    tile += step;
+    if (++slot == 32) {
+      slot = 0;
+      if (tile < tiles) {
+        id = fetch_id(tile);
+        fetch_scales(tile);
+      }
+    }
+    const int next_id = __shfl_sync(kFullMask, id, slot);
+    if (tile < tiles) load_k(next_id, tile);
+
+    // scores in log2 units; whether one passes its maximum by more than the slack
+    bool over = false;
+#pragma unroll
+    for (int j = 0; j < kTiles; ++j)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if constexpr (kF32 && kPack) s[j][k] += __shfl_xor_sync(kFullMask, s[j][k], 2);  // the low terms' columns are two lanes away
+        const int i = k & 1, key = this_tile * 16 + g + 8 * (k >> 1);
+        s[j][k] = key < limit[j][i] && usable ? s[j][k] * (factor[j][i] * k_unit) : -INFINITY;
+        over |= s[j][k] > m[j][i] + kQdSlack || s[j][k] + v_log > mv[j][i] + kQdSlack;
+      }
+    if (__any_sync(kFullMask, over)) {
+#pragma unroll
+      for (int j = 0; j < kTiles; ++j)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float top = fmaxf(s[j][i], s[j][i + 2]);
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, o));
+          const float now = fmaxf(m[j][i], top), now_v = fmaxf(mv[j][i], top + v_log);
+          l[j][i] *= ex2_approx(m[j][i] - now);
+          const float f = ex2_approx(mv[j][i] - now_v);
+          m[j][i] = now;
+          mv[j][i] = now_v;
+#pragma unroll
+          for (int a = 0; a < kMTiles; ++a) {
+            acc[j][a][i] *= f;
+            acc[j][a][i + 2] *= f;
+          }
+        }
+    }
+    // weights: their sum, and P^T as high and low f16 terms
+    uint32_t high[kTiles][2], low[kTiles][2];
+#pragma unroll
+    for (int j = 0; j < kTiles; ++j) {
+      float w[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int i = k & 1;
+        l[j][i] += ex2_approx(s[j][k] - m[j][i]);
+        w[k] = ex2_approx(s[j][k] + v_log - mv[j][i]);
+      }
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const uint32_t h = q_pair(w[2 * r], w[2 * r + 1]);
+        const uint32_t rest = q_pair_rest(w[2 * r], w[2 * r + 1], h);
+        if constexpr (kPack) {
+          high[j][r] = q_transpose(t < 2 ? h : rest);
+        } else {
+          high[j][r] = q_transpose(h);
+          low[j][r] = q_transpose(rest);
+        }
+      }
+    }
+    // O^T += V^T P^T: rows dims 16 g + 2 i and 16 g + 2 i + 1 of a part of 128 (64: 8 g + ..)
+#pragma unroll
+    for (int h = 0; h < kVHalves; ++h) {
+#pragma unroll
+      for (int w = 0; w < kVWords; ++w) {
+        auto word = [&](int k) { return w == 0 ? vr[h][k].x : w == 1 ? vr[h][k].y : w == 2 ? vr[h][k].z : vr[h][k].w; };
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {  // bytes 2b, 2b + 1 of the word
+          const uint32_t near = __byte_perm(word(0), word(1), b ? 0x7362 : 0x5140);  // keys 2t, 2t + 1
+          const uint32_t far = __byte_perm(word(2), word(3), b ? 0x7362 : 0x5140);   // keys 2t + 8, 2t + 9
+          const uint32_t a0 = q_half2(near), a1 = q_half2_high(near), a2 = q_half2(far), a3 = q_half2_high(far);
+          const int at = (h * kVWords + w) * 2 + b;
+#pragma unroll
+          for (int j = 0; j < kTiles; ++j) {
+            q_mma(acc[j][at], a0, a1, a2, a3, high[j][0], high[j][1]);
+            if constexpr (!kPack) q_mma(acc[j][at], a0, a1, a2, a3, low[j][0], low[j][1]);
+          }
+        }
+      }
+    }
+    if (tile < tiles) load_v(next_id, tile);
+  }
+
+  // the warps' sums into shared memory (the queries are no longer needed)
+#pragma unroll
+  for (int j = 0; j < kTiles; ++j)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) l[j][i] += __shfl_xor_sync(kFullMask, l[j][i], o);
+    }
+  __syncthreads();
+  float* sums = reinterpret_cast<float*>(qd_smem) + warp * kCols * S::kAccPitch;
+#pragma unroll
+  for (int j = 0; j < kTiles; ++j) {
+    const int c = 8 * j + 2 * t;
+#pragma unroll
+    for (int a = 0; a < kMTiles; ++a) {
+      if constexpr (kPack) {  // the low terms' share of a column is two lanes away
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc[j][a][k] += __shfl_xor_sync(kFullMask, acc[j][a][k], 2);
+      }
+      const int d = kD >= 128 ? (a / 8) * 128 + 16 * g + 2 * (a % 8) : 8 * g + 2 * a;
+      if (!kPack || t < 2) {
+        *reinterpret_cast<float2*>(sums + c * S::kAccPitch + d) = make_float2(acc[j][a][0], acc[j][a][2]);
+        *reinterpret_cast<float2*>(sums + (c + 1) * S::kAccPitch + d) = make_float2(acc[j][a][1], acc[j][a][3]);
+      }
+    }
+    if (g == 0 && (!kPack || t < 2)) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        qd_ml[warp][c + i] = make_float2(m[j][i], l[j][i]);
+        qd_mv[warp][c + i] = mv[j][i];
+      }
+    }
+  }
+  __syncthreads();
+  // ... and into one, in the first warp's place: relative to the largest maximum of the scores
+  float* all = reinterpret_cast<float*>(qd_smem);
+  for (int i = threadIdx.x; i < kCols * (kD / 4); i += kQdThreads) {
+    const int c = i / (kD / 4), d = i % (kD / 4) * 4;
+    float top = kQdNone, sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kQdWarps; ++w) top = fmaxf(top, qd_ml[w][c].x);
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kQdWarps; ++w) {
+      const float2 ml = qd_ml[w][c];
+      sum = fmaf(ml.y, ex2_approx(ml.x - top), sum);
+      const float f = ml.y == 0.f ? 0.f : ex2_approx(qd_mv[w][c] - top);
+      const float4 x = *reinterpret_cast<const float4*>(all + (w * kCols + c) * S::kAccPitch + d);
+      y.x = fmaf(x.x, f, y.x);
+      y.y = fmaf(x.y, f, y.y);
+      y.z = fmaf(x.z, f, y.z);
+      y.w = fmaf(x.w, f, y.w);
+    }
+    *reinterpret_cast<float4*>(all + c * S::kAccPitch + d) = y;  // (read above by this thread alone)
+    if (d == 0) qd_ML[c] = make_float2(top, sum);
+  }
+  auto place = [&](int c, int d) {  // of column c's dims d .. d + 3 in the output
+    const int at = ct * kCols + c;
+    return p.out + ((long long)(token + at / p.groups) * hq + head * p.groups + at % p.groups) * kD + d;
+  };
+  const int used = live ? min(kCols, columns - ct * kCols) : 0;
+  if (ctas == 1) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < used * (kD / 4); i += kQdThreads) {
+      const int c = i / (kD / 4), d = i % (kD / 4) * 4;
+      const float sum = qd_ML[c].y, inverse = sum == 0.f ? 0.f : 1.f / sum;
+      const float4 y = *reinterpret_cast<const float4*>(all + c * S::kAccPitch + d);
+      *reinterpret_cast<float4*>(place(c, d)) = make_float4(y.x * inverse, y.y * inverse, y.z * inverse, y.w * inverse);
+    }
+    return;
+  }
+  cl_sync();
+  bool odd = false;
+  const int pieces = used * (kD / 4), per = (pieces + ctas - 1) / ctas;
+  for (int i = threadIdx.x; i < per; i += kQdThreads) {
+    const int piece = rank * per + i;
+    if (piece >= pieces) break;
+    const int c = piece / (kD / 4), d = piece % (kD / 4) * 4;
+    float top = kQdNone, sum = 0.f;
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int first = 0; first < ctas; first += 4) {  // four CTAs' shares in flight
+      float2 e[4];
+      float4 x[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int from = first + k < ctas ? first + k : first;
+        e[k] = cl_ld2(cl_map(&qd_ML[c], from));
+        x[k] = cl_ld4(cl_map(all + c * S::kAccPitch + d, from));
+        if (first + k >= ctas) e[k] = make_float2(kQdNone, 0.f), x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      float now = top;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) now = fmaxf(now, e[k].x);
+      const float f = ex2_approx(top - now);
+      sum *= f;
+      y = make_float4(y.x * f, y.y * f, y.z * f, y.w * f);
+      top = now;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float f = ex2_approx(e[k].x - top);
+        sum = fmaf(e[k].y, f, sum);
+        y.x = fmaf(x[k].x, f, y.x);
+        y.y = fmaf(x[k].y, f, y.y);
+        y.z = fmaf(x[k].z, f, y.z);
+        y.w = fmaf(x[k].w, f, y.w);
+      }
+    }
+    const float inverse = sum == 0.f ? 0.f : 1.f / sum;
+    y = make_float4(y.x * inverse, y.y * inverse, y.z * inverse, y.w * inverse);
+    odd |= cl_not_finite(y) || !(sum - sum == 0.f);
+    *reinterpret_cast<float4*>(place(c, d)) = y;
+  }
+  cl_sync_read(odd);  // no CTA goes while another reads its sums
+}
+
+// CTAs per cluster: as many as give every SM its three resident CTAs, up to 16, and no more than one per four tiles of the widest
+// row; at least four in batches of long rows, so that the last CTAs to finish are short ones.
+static int quantized_decode_ctas(long long units, long long tiles, int sms) {
+  long long c = (3LL * sms + units / 2) / units;
+  if (c < 4 && tiles > 128) c = 4;
+  const long long useful = (tiles + kQdWarps - 1) / kQdWarps;
+  c = c < useful ? c : useful;
+  return (int)(c < 1 ? 1 : (c > 16 ? 16 : c));
+}
+
+template <typename T, int kD, int kTiles, bool kPack>
+static int launch_quantized_decode(QDecodeParams p, cudaStream_t stream) {
+  using S = QdShape<kD, kTiles, kPack, std::is_same<T, float>::value>;
+  auto* kernel = quantized_decode_kernel<T, kD, kTiles, kPack>;
+  static PerDeviceFlags ready;
+  if (!once_per_device(ready, [&](int) {
+        return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes) == cudaSuccess &&
+               cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess;
+      }))
+    return NVJ_ERR_LAUNCH;
+  p.column_tiles = (p.width * p.groups + S::kCols - 1) / S::kCols;
+  const long long units = (long long)p.rows * p.num_kv_heads * p.column_tiles;
+  const int ctas = quantized_decode_ctas(units, (long long)p.table_width * p.block_size / 16, 148);
+  if ((long long)ctas * p.rows > 0x7fffffffLL || (long long)p.num_kv_heads * p.column_tiles > 65535) return NVJ_ERR_TOO_LARGE;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)ctas * (unsigned)p.rows, p.num_kv_heads * p.column_tiles, 1);
+  cfg.blockDim = dim3(kQdThreads, 1, 1);
+  cfg.dynamicSmemBytes = S::kBytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = ctas;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = ctas > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, p, ctas) == cudaSuccess ? NVJ_OK : NVJ_ERR_LAUNCH;
+}
+
+template <typename T, int kD>
+static int launch_quantized_decode_columns(const QDecodeParams& p, cudaStream_t stream) {
+  const long long columns = (long long)p.width * p.groups;
+  if (columns <= 4) return launch_quantized_decode<T, kD, 1, true>(p, stream);
+  if (columns <= 8) return launch_quantized_decode<T, kD, 1, false>(p, stream);
+  return launch_quantized_decode<T, kD, 2, false>(p, stream);
+}
+template <typename T>
+static int launch_quantized_decode_dims(const QDecodeParams& p, int head_dim, cudaStream_t stream) {
+  if (head_dim == 256) return launch_quantized_decode_columns<T, 256>(p, stream);
+  if (head_dim == 128) return launch_quantized_decode_columns<T, 128>(p, stream);
+  return launch_quantized_decode_columns<T, 64>(p, stream);
+}
+
+}  // namespace nvj
+
+extern "C" int nvj_paged_decode_quantized(const void* q, int q_dtype, const void* k_cache_layer, const void* v_cache_layer,
+                                          const float* k_scale, const float* v_scale, int64_t num_blocks, int block_size,
+                                          int num_kv_heads, int head_dim, int num_q_heads, const int32_t* block_tables, int table_width,
+                                          const int32_t* seq_lens, const int32_t* positions, const int32_t* query_start_loc, int rows,
+                                          int width, float scale, float* out, int32_t* status, nvj_stream_t stream) {
+  using namespace nvj;
+  if (rows < 0 || width < 0 || table_width < 0 || num_blocks < 0) return NVJ_ERR_INVALID_ARGUMENT;
+  if (q_dtype < NVJ_BF16 || q_dtype > NVJ_F32 || !quantized_cache_shape_ok(block_size, num_kv_heads, head_dim)) return NVJ_ERR_UNSUPPORTED;
+  if (num_q_heads <= 0 || num_q_heads % num_kv_heads != 0) return NVJ_ERR_INVALID_ARGUMENT;
+  if (rows == 0 || width == 0) return NVJ_OK;
+  if (query_start_loc && (width != 1 || !positions)) return NVJ_ERR_INVALID_ARGUMENT;
+  if (!q || !k_cache_layer || !v_cache_layer || !k_scale || !v_scale || !seq_lens || !out || !status) return NVJ_ERR_INVALID_ARGUMENT;
+  if (table_width > 0 && !block_tables) return NVJ_ERR_INVALID_ARGUMENT;
+  if (!aligned16(q) || !aligned16(out) || !aligned16(k_cache_layer) || !aligned16(v_cache_layer)) return NVJ_ERR_INVALID_ARGUMENT;
+  if ((long long)table_width * block_size > 0x7fffffffLL - 65536) return NVJ_ERR_TOO_LARGE;
+  if ((long long)width * (num_q_heads / num_kv_heads) > 0xffff || (long long)rows * width > 0x7fffffffLL) return NVJ_ERR_TOO_LARGE;
+  QDecodeParams p{};
+  p.q = q;
+  p.k_cache = static_cast<const uint8_t*>(k_cache_layer);
+  p.v_cache = static_cast<const uint8_t*>(v_cache_layer);
+  p.k_scale = k_scale;
+  p.v_scale = v_scale;
+  p.block_tables = block_tables;
+  p.seq_lens = seq_lens;
+  p.positions = positions;
+  p.query_start_loc = query_start_loc;
+  p.out = out;
+  p.status = status;
+  p.num_blocks = num_blocks;
+  p.rows = rows;
+  p.width = width;
+  p.table_width = table_width;
+  p.block_size = block_size;
+  p.num_kv_heads = num_kv_heads;
+  p.groups = num_q_heads / num_kv_heads;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (q_dtype == NVJ_BF16) return launch_quantized_decode_dims<__nv_bfloat16>(p, head_dim, s);
+  if (q_dtype == NVJ_F16) return launch_quantized_decode_dims<__half>(p, head_dim, s);
+  return launch_quantized_decode_dims<float>(p, head_dim, s);
+}

@@ -112,6 +112,11 @@ class ResidentDecodeMetadata:
             raise ValueError("row or block index outside the resident block table")
         self.block_tables[row, index] = int(block_id)
 
+    def reserve(self, pool) -> None:
+        """Room for the next token of every active row out of a `device_blocks.DeviceBlockPool`: what `set_block` does for the rows that
+        reach a new block, without the host knowing which."""
+        pool.extend(self.block_tables, self.seq_lens, (self.seq_lens > 0).to(torch.int32), self.rows)
+
     def advance(self) -> None:
         """positions <- seq_lens, seq_lens += 1 for every active row; no host involvement."""
         lib = _lib.load()

@@ -24,7 +24,7 @@ from __future__ import annotations
 import ctypes
 import os
 import threading
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -253,6 +253,57 @@ def compute_slot_mapping(positions, block_table, block_size, token_row_ids=None)
                                        int(block_size), _ptr(out), _stream(positions.device)),
           "nvj_compute_slot_mapping")
     return out
+
+
+class PackedLayout(NamedTuple):
+    """A packed step's arrays as `build_packed_layout` makes them: `[1, T]`, `[1, T]`, `[1, T]`, `[rows + 1]`, `[rows]`, `[1]`, int32."""
+
+    positions: torch.Tensor
+    token_row_ids: torch.Tensor
+    slot_mapping: torch.Tensor
+    query_start_loc: torch.Tensor
+    seq_lens: torch.Tensor
+    free_head: torch.Tensor
+
+
+def build_packed_layout(cached_lens, new_lens, block_tables, free_blocks, free_head, block_size, token_bucket) -> PackedLayout:
+    """Lay out a packed step on the device: row r, with `cached_lens[r]` tokens in the cache, gets `new_lens[r]` more (0: none).
+
+    The blocks that the new tokens need come from `free_blocks` (int32 ids) from `free_head` (int32 `[1]`) on, in row order, and are entered
+    into `block_tables` `[rows, W]` in place; the result holds the step's arrays over a bucket of `token_bucket` tokens (padding:
+    position 0, row 0, slot -1) and the list's new head.  Nothing is read back: the caller knows from its own lengths that the
+    list suffices, and a list that ends too early, a row without room or a bucket too small is flagged on the device
+    (`check_device_status`).
+    """
+    named = (("cached_lens", cached_lens), ("new_lens", new_lens), ("block_tables", block_tables), ("free_blocks", free_blocks),
+             ("free_head", free_head))
+    for name, t in named:
+        if _cuda(name, t).dtype != torch.int32 or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous int32 tensor")
+        if t.device != block_tables.device:
+            raise ValueError(f"{name} must be on the device of block_tables")
+    if block_tables.ndim != 2 or cached_lens.shape != (block_tables.shape[0],) or new_lens.shape != cached_lens.shape:
+        raise ValueError("block_tables must be [rows, W], cached_lens and new_lens [rows]")
+    if free_blocks.ndim != 1 or free_head.shape != (1,):
+        raise ValueError("free_blocks must be [n] and free_head [1]")
+    block_size, bucket = int(block_size), int(token_bucket)
+    if block_size <= 0 or bucket < 0:
+        raise ValueError("block_size must be positive and token_bucket not negative")
+    rows, width = block_tables.shape
+    device = block_tables.device
+    # one allocation: the three token arrays, then head, lengths and query_start_loc
+    flat = torch.empty(3 * bucket + 2 * rows + 2, dtype=torch.int32, device=device)
+    positions, ids, slots, rest = flat.split((bucket, bucket, bucket, 2 * rows + 2))
+    head, lens, qsl = rest.split((1, rows, rows + 1))
+    with torch.cuda.device(device):
+        st = _status_word(device)
+        check(_lib.load().nvj_build_packed_layout(
+            cached_lens.data_ptr(), new_lens.data_ptr(), rows, block_tables.data_ptr(), width, block_size, free_blocks.data_ptr(),
+            free_blocks.numel(), free_head.data_ptr(), bucket, positions.data_ptr(), ids.data_ptr(), slots.data_ptr(), qsl.data_ptr(),
+            lens.data_ptr(), head.data_ptr(), st.data_ptr(), _stream(device)), "nvj_build_packed_layout")
+        if _strict():
+            _check_word(st, "nvj_build_packed_layout")
+    return PackedLayout(positions[None], ids[None], slots[None], qsl, lens, head)
 
 
 # --------------------------------------------------------------------------- append

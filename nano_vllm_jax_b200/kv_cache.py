@@ -47,6 +47,20 @@ class KVCacheStorage:
 
 
 @dataclass
+class QuantizedKVCacheStorage(KVCacheStorage):
+    """The cache held in 8 bits: `torch.float8_e4m3fn` arrays and a float32 scale per layer, block and kv head
+    `[num_layers, num_blocks, num_kv_heads]` of K and of V; a value is number * scale (not in the reference)."""
+
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+
+    def layer(self, layer_id: int):
+        """(k, v, k_scale, v_scale) of one layer, as the kernels of `kernels/quantized_kv.py` take them."""
+        return tuple(_resolve_kv_layer(t, layer_id)[0] if t.ndim == 5 else t[layer_id]
+                     for t in (self.k_cache, self.v_cache, self.k_scale, self.v_scale))
+
+
+@dataclass
 class AttentionMetadata:
     """Per-step paged/ragged attention metadata (kv_cache.py:51-64).
 
@@ -162,9 +176,10 @@ def _itemsize(dtype) -> int:
 
 
 def estimate_kv_cache_bytes(spec: KVCacheSpec) -> int:
-    """Total bytes of the K and V arrays (kv_cache.py:142-152)."""
+    """Total bytes of the K and V arrays (kv_cache.py:142-152), and of the scales of an 8-bit cache."""
     n = spec.num_layers * spec.num_blocks * spec.block_size * spec.num_kv_heads * spec.head_dim
-    return int(n * _itemsize(spec.dtype) * 2)
+    scales = spec.num_layers * spec.num_blocks * spec.num_kv_heads * 4 if spec.dtype == torch.float8_e4m3fn else 0
+    return int((n * _itemsize(spec.dtype) + scales) * 2)
 
 
 def cap_num_kv_cache_blocks(spec: KVCacheSpec) -> int:
@@ -194,6 +209,20 @@ def init_kv_cache(num_blocks, block_size, num_kv_heads, head_dim, max_seqs, max_
         kv_lens=torch.zeros(max_seqs, dtype=torch.int32, device=device),
         slot_mapping=torch.zeros((max_seqs, 1), dtype=torch.int32, device=device),
     )
+
+
+def init_quantized_kv_cache(spec: KVCacheSpec, device="cuda") -> QuantizedKVCacheStorage:
+    """Zero-filled 8-bit cache of as many blocks as `spec` allows, every scale the smallest there is (a block's first append sets its own)."""
+    from .kernels.quantized_kv import HEAD_DIMS, PAGE_SIZES, quantized_cache_supported
+    spec = replace(spec, dtype=torch.float8_e4m3fn)
+    if not quantized_cache_supported(spec.block_size, spec.head_dim):
+        raise ValueError(f"an 8-bit cache has head_dim in {HEAD_DIMS} and block_size in {PAGE_SIZES}, not {spec.head_dim} and "
+                         f"{spec.block_size}")
+    nb = cap_num_kv_cache_blocks(spec)
+    shape = (spec.num_layers, nb, spec.block_size, spec.num_kv_heads, spec.head_dim)
+    scales = (spec.num_layers, nb, spec.num_kv_heads)
+    numbers = [torch.zeros(shape, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn) for _ in range(2)]
+    return QuantizedKVCacheStorage(*numbers, *[torch.full(scales, 2.0 ** -117, dtype=torch.float32, device=device) for _ in range(2)])
 
 
 def init_hybrid_state(config, batch_size: int = 1, dtype=None, device="cuda") -> HybridLayerState:
