@@ -474,16 +474,23 @@ int nvj_kv_append_quantized(const void* new_k, const void* new_v, int src_dtype,
 /*
  * Attention for rows of `width` query tokens over the 8-bit cache: q [rows, width, num_q_heads, head_dim] bf16, f16 or f32; token t of row b
  * attends keys p < seq_lens[b] and, with positions given ([rows, width]), p <= positions[b, t].  out as q, float32; a token that
- * sees no key gets zeros.  Meant for few query tokens per row (one kernel serves width * num_q_heads / num_kv_heads <= 16 columns
- * per pass over a row's keys); any width is taken.  query_start_loc given (width 1): q, positions and out are those of a packed batch, and
+ * sees no key gets zeros.  Meant for few query tokens per row; any width is taken.  query_start_loc given (width 1): q, positions and out are those of a packed batch, and
  * the rows that hold exactly one token are served, nothing else is written.  The scale may be any number.
  * A length beyond the block table is flagged and clipped, a block id outside the pool flagged and its keys left out.
+ *
+ *   form       0 automatic, 1 mma.sync tiles on thread-block clusters (width * num_q_heads / num_kv_heads <= 16 columns per pass over a
+ *              row's keys), 2 tcgen05 tiles (24 columns; head_dim 128 or 256, else NVJ_ERR_UNSUPPORTED)
+ *   workspace  nullable scratch of nvj_paged_decode_quantized_workspace_bytes(..., form) bytes (0: the call has no use for one), 16-byte
+ *              aligned, nothing kept in it between calls; without one the automatic choice is form 1
  */
+size_t nvj_paged_decode_quantized_workspace_bytes(int rows, int width, int table_width, int block_size, int num_kv_heads,
+                                                  int head_dim, int num_q_heads, int form);
 int nvj_paged_decode_quantized(const void* q, int q_dtype, const void* k_cache_layer, const void* v_cache_layer,
                                const float* k_scale, const float* v_scale, int64_t num_blocks, int block_size,
                                int num_kv_heads, int head_dim, int num_q_heads, const int32_t* block_tables, int table_width,
                                const int32_t* seq_lens, const int32_t* positions, const int32_t* query_start_loc, int rows,
-                               int width, float scale, float* out, int32_t* status, nvj_stream_t stream);
+                               int width, float scale, float* out, int32_t* status, void* workspace,
+                               size_t workspace_bytes, int form, nvj_stream_t stream);
 
 /*
  * Ragged packed prefill attention over the 8-bit cache: masks, layout and padding as nvj_paged_prefill_packed.

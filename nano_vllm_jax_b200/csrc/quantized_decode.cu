@@ -19,7 +19,10 @@
 // Maxima are lazy: only a score that passes its column's maximum by 2^8 (one vote per tile) rescales the sums.
 
 #include "cluster.cuh"
+#include "decode_parts.cuh"
 #include "quantized_kv.cuh"
+#include "quantized_umma_params.cuh"
+#include "umma.cuh"
 
 namespace nvj {
 
@@ -510,14 +513,182 @@ static int launch_quantized_decode_dims(const QDecodeParams& p, int head_dim, cu
   return launch_quantized_decode_columns<T, 64>(p, stream);
 }
 
+// ---- the tcgen05 form (quantized_umma.cuh): its tensor maps, workspace, launch and fold ------------------------------------------
+typedef CUresult (*QuEncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                    const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static QuEncodeTiledFn qu_encode_fn() {
+  static QuEncodeTiledFn fn = [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult res;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &res) != cudaSuccess || res != cudaDriverEntryPointSuccess)
+      ptr = nullptr;
+    return reinterpret_cast<QuEncodeTiledFn>(ptr);
+  }();
+  return fn;
+}
+// A layer [token, kv head, head_dim] of bytes seen as {128 dims, token of a group of 8, 128-dim chunk, group, kv head}: a box is 16 keys of
+// one kv head and lands as [group][chunk][8 keys][128 B] with the 128-byte swizzle.  `extent` = (tokens << 12) | kv heads << 1 | head_dim 256.
+static bool qu_make_map(CUtensorMap* map, const void* base, uint64_t extent) {
+  const cuuint64_t tokens = extent >> 12, heads = (extent >> 1) & 0x7ff, dim = extent & 1 ? 256 : 128;
+  const cuuint64_t dims[5] = {128, 8, dim / 128, tokens / 8, heads};
+  const cuuint64_t strides[4] = {heads * dim, 128, 8 * heads * dim, dim};
+  const cuuint32_t box[5] = {128, 8, (cuuint32_t)(dim / 128), 2, 1};
+  const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  return qu_encode_fn()(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 5, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+constexpr int kQuMapKind = 6;  // (tensor_map_cached)
+
+// How a call is cut: column tiles, ranges, and where its partials lie in the workspace.
+struct QuPlan {
+  int column_tiles, tile_columns, hcts, ranges;
+  size_t acc_bytes, ml_bytes, cut_bytes;
+  size_t bytes() const { return acc_bytes + ml_bytes + cut_bytes; }
+};
+static QuPlan qu_plan(int columns, int num_kv_heads, int head_dim, int sms) {
+  QuPlan w{};
+  w.column_tiles = (columns + 23) / 24;
+  const int each = (columns + w.column_tiles - 1) / w.column_tiles;
+  w.tile_columns = each <= 4 ? 4 : each <= 8 ? 8 : each <= 16 ? 16 : 24;
+  w.hcts = num_kv_heads * w.column_tiles;
+  w.ranges = sms / w.hcts > 1 ? sms / w.hcts : 1;
+  const size_t slots = w.ranges > 1 ? (size_t)2 * w.ranges * w.hcts * w.tile_columns : 0;
+  w.acc_bytes = ws_round(slots * head_dim * sizeof(float));
+  w.ml_bytes = ws_round(slots * 2 * sizeof(float));
+  w.cut_bytes = ws_round((size_t)w.ranges * sizeof(UmmaCut));
+  return w;
+}
+
+// One CTA per (boundary between two ranges, kv head and column tile): the first boundary that cuts a row folds the row's columns from the
+// ranges' partials.  Thread = (column, 4 dims) in turn.
+__global__ void __launch_bounds__(256) quantized_umma_fold_kernel(QuParams a, int head_dim) {
+  const int hct = blockIdx.y, head = hct / a.column_tiles, ct = hct % a.column_tiles;
+  pdl_wait();
+  pdl_release();
+  const UmmaCut cut = a.cuts[blockIdx.x + 1];
+  if (cut.b < 0) return;
+  const int parts = cut.last - cut.first + 1, pieces = head_dim / 4;
+  const int columns = min(a.columns - ct * a.tile_columns, a.tile_columns);
+  const long long token = a.query_start_loc ? (long long)a.query_start_loc[cut.b] : (long long)cut.b * a.width;
+  for (int i = threadIdx.x; i < columns * pieces; i += 256) {
+    const int c = i / pieces, d = i % pieces * 4;
+    float top = -3e38f, sum = 0.f;
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k0 = 0; k0 < parts; k0 += 8) {  // eight parts in flight
+      float2 e[8];
+      float4 x[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int part = cut.first + (k0 + k < parts ? k0 + k : 0);
+        const long long slot = ((long long)partial_slot(part, part == cut.first) * a.hcts + hct) * a.tile_columns + c;
+        e[k] = __ldcg(reinterpret_cast<const float2*>(a.part_ml + slot * 2));
+        x[k] = __ldcg(reinterpret_cast<const float4*>(a.part_acc + slot * head_dim + d));
+        if (k0 + k >= parts) e[k] = make_float2(-3e38f, 0.f), x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      float now = top;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) now = fmaxf(now, e[k].x);
+      const float f = ex2_approx(top - now);
+      sum *= f;
+      y = make_float4(y.x * f, y.y * f, y.z * f, y.w * f);
+      top = now;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float w = ex2_approx(e[k].x - top);
+        sum = fmaf(e[k].y, w, sum);
+        y.x = fmaf(x[k].x, w, y.x);
+        y.y = fmaf(x[k].y, w, y.y);
+        y.z = fmaf(x[k].z, w, y.z);
+        y.w = fmaf(x[k].w, w, y.w);
+      }
+    }
+    const float inverse = sum == 0.f ? 0.f : 1.f / sum;
+    const int at = ct * a.tile_columns + c;
+    *reinterpret_cast<float4*>(a.out + ((token + at / a.groups) * a.num_q_heads + head * a.groups + at % a.groups) * head_dim + d) =
+        make_float4(y.x * inverse, y.y * inverse, y.z * inverse, y.w * inverse);
+  }
+}
+
+// What a row's end costs a CTA, in units of 16 keys (decode_parts.cuh).
+constexpr int kQuRowEndCost = 8;
+
+static int run_quantized_umma(const QDecodeParams& q, int q_dtype, int head_dim, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
+  const int sms = decode_wide_num_ctas();
+  if (sms <= 0) return NVJ_ERR_LAUNCH;
+  if (head_dim < 128 || !qu_encode_fn()) return NVJ_ERR_UNSUPPORTED;
+  if (q.num_blocks < 1 || q.num_blocks * (q.block_size / 8) >= 0x7fffffffLL) return NVJ_ERR_UNSUPPORTED;
+  const int columns = q.width * q.groups;
+  const QuPlan w = qu_plan(columns, q.num_kv_heads, head_dim, sms);
+  if (!workspace || !aligned16(workspace) || workspace_bytes < w.bytes()) return NVJ_ERR_WORKSPACE;
+  CUtensorMap k_map, v_map;
+  const uint64_t extent = (uint64_t)q.num_blocks * q.block_size << 12 | (uint64_t)q.num_kv_heads << 1 | (head_dim == 256 ? 1u : 0u);
+  if (!tensor_map_cached(&k_map, kQuMapKind, q.k_cache, extent, qu_make_map) || !tensor_map_cached(&v_map, kQuMapKind, q.v_cache, extent, qu_make_map))
+    return NVJ_ERR_UNSUPPORTED;
+  char* at = static_cast<char*>(workspace);
+  QuParams a{};
+  a.q = q.q;
+  a.k_scale = q.k_scale;
+  a.v_scale = q.v_scale;
+  a.positions = q.positions;
+  a.query_start_loc = q.query_start_loc;
+  a.out = q.out;
+  a.part_acc = reinterpret_cast<float*>(at);
+  a.part_ml = reinterpret_cast<float*>(at + w.acc_bytes);
+  a.cuts = reinterpret_cast<UmmaCut*>(at + w.acc_bytes + w.ml_bytes);
+  a.width = q.width;
+  a.columns = columns;
+  a.groups = q.groups;
+  a.num_q_heads = q.groups * q.num_kv_heads;
+  a.num_kv_heads = q.num_kv_heads;
+  a.column_tiles = w.column_tiles;
+  a.tile_columns = w.tile_columns;
+  a.hcts = w.hcts;
+  a.scale_log2 = q.scale_log2;
+  DecodeParams p{};
+  p.block_tables = q.block_tables;
+  p.seq_lens = q.seq_lens;
+  p.query_start_loc = q.query_start_loc;
+  p.query_positions = q.positions;
+  p.packed_rows = q.query_start_loc != nullptr;
+  p.status = q.status;
+  p.num_blocks = q.num_blocks;
+  p.batch = q.rows;
+  p.table_width = q.table_width;
+  p.block_size = q.block_size;
+  p.row_end_cost = kQuRowEndCost;
+  const auto launch = q_dtype == NVJ_BF16 ? launch_quantized_umma_bf16 : q_dtype == NVJ_F16 ? launch_quantized_umma_f16 : launch_quantized_umma_f32;
+  const int rc = launch(k_map, v_map, a, p, head_dim, w.ranges, stream);
+  if (rc != NVJ_OK || w.ranges < 2) return rc;
+  return launch_after(quantized_umma_fold_kernel, dim3(w.ranges - 1, w.hcts), dim3(256), 0, stream, a, head_dim) == cudaSuccess ? NVJ_OK : NVJ_ERR_LAUNCH;
+}
+
+// Whether a call goes to the tcgen05 form.
+static bool quantized_umma_pays(int rows, int width, int table_width, int block_size, int num_kv_heads, int head_dim, int groups) {
+  return head_dim >= 128 && (long long)rows * table_width * block_size / 16 * num_kv_heads * head_dim >= 1024LL * 512;
+}
+
 }  // namespace nvj
+
+extern "C" size_t nvj_paged_decode_quantized_workspace_bytes(int rows, int width, int table_width, int block_size, int num_kv_heads,
+                                                              int head_dim, int num_q_heads, int form) {
+  using namespace nvj;
+  if (rows <= 0 || width <= 0 || table_width <= 0 || !quantized_cache_shape_ok(block_size, num_kv_heads, head_dim) || num_q_heads <= 0 ||
+      num_q_heads % num_kv_heads != 0 || head_dim < 128 || form < 0 || form == 1)
+    return 0;
+  const int groups = num_q_heads / num_kv_heads, sms = decode_wide_num_ctas();
+  if (sms <= 0 || (long long)width * groups > 0xffff) return 0;
+  if (form == 0 && !quantized_umma_pays(rows, width, table_width, block_size, num_kv_heads, head_dim, groups)) return 0;
+  return qu_plan(width * groups, num_kv_heads, head_dim, sms).bytes();
+}
 
 extern "C" int nvj_paged_decode_quantized(const void* q, int q_dtype, const void* k_cache_layer, const void* v_cache_layer,
                                           const float* k_scale, const float* v_scale, int64_t num_blocks, int block_size,
                                           int num_kv_heads, int head_dim, int num_q_heads, const int32_t* block_tables, int table_width,
                                           const int32_t* seq_lens, const int32_t* positions, const int32_t* query_start_loc, int rows,
-                                          int width, float scale, float* out, int32_t* status, nvj_stream_t stream) {
+                                          int width, float scale, float* out, int32_t* status, void* workspace,
+                                          size_t workspace_bytes, int form, nvj_stream_t stream) {
   using namespace nvj;
+  if (form < 0 || form > 2) return NVJ_ERR_INVALID_ARGUMENT;
   if (rows < 0 || width < 0 || table_width < 0 || num_blocks < 0) return NVJ_ERR_INVALID_ARGUMENT;
   if (q_dtype < NVJ_BF16 || q_dtype > NVJ_F32 || !quantized_cache_shape_ok(block_size, num_kv_heads, head_dim)) return NVJ_ERR_UNSUPPORTED;
   if (num_q_heads <= 0 || num_q_heads % num_kv_heads != 0) return NVJ_ERR_INVALID_ARGUMENT;
@@ -549,6 +720,10 @@ extern "C" int nvj_paged_decode_quantized(const void* q, int q_dtype, const void
   p.groups = num_q_heads / num_kv_heads;
   p.scale_log2 = scale * 1.4426950408889634f;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (form == 2 || (form == 0 && workspace && quantized_umma_pays(rows, width, table_width, block_size, num_kv_heads, head_dim, p.groups))) {
+    const int rc = run_quantized_umma(p, q_dtype, head_dim, workspace, workspace_bytes, s);
+    if (form == 2 || (rc != NVJ_ERR_UNSUPPORTED && rc != NVJ_ERR_WORKSPACE)) return rc;
+  }
   if (q_dtype == NVJ_BF16) return launch_quantized_decode_dims<__nv_bfloat16>(p, head_dim, s);
   if (q_dtype == NVJ_F16) return launch_quantized_decode_dims<__half>(p, head_dim, s);
   return launch_quantized_decode_dims<float>(p, head_dim, s);

@@ -465,10 +465,11 @@ extern "C" int nvj_paged_prefill_quantized(const void* q, int q_dtype, const voi
     return NVJ_ERR_TOO_LARGE;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int skip_single = single_rows != 0;
+  // the workspace is used twice, one launch behind the other: by the decode kernel's partials and then for the pages
   if (skip_single && rows > 0) {
     const int rc = nvj_paged_decode_quantized(q, q_dtype, k_cache_layer, v_cache_layer, k_scale, v_scale, num_blocks, block_size, num_kv_heads,
                                               head_dim, num_q_heads, block_tables, table_width, kv_lens, positions, query_start_loc, rows, 1,
-                                              scale, out, status, stream);
+                                              scale, out, status, workspace, workspace_bytes, 0, stream);
     if (rc != NVJ_OK) return rc;
   }
   const size_t needed =

@@ -129,11 +129,12 @@ def kv_append_quantized(new_k, new_v, k_cache_layer, v_cache_layer, k_scale, v_s
     return k_cache_layer, v_cache_layer, k_scale, v_scale
 
 
-def paged_decode_attention_quantized(q, k_cache_layer, v_cache_layer, k_scale, v_scale, block_table, seq_lens, scale, *, positions=None):
+def paged_decode_attention_quantized(q, k_cache_layer, v_cache_layer, k_scale, v_scale, block_table, seq_lens, scale, *, positions=None, form=0):
     """Decode attention over one layer of the 8-bit cache, for rows of one query token or a few.
 
     q `[B, Hq, D]` -> float32 `[B, Hq, D]`, or `[B, T, Hq, D]` -> `[B, T, Hq * D]`.  Token t of row b sees the keys p < seq_lens[b] and,
-    with `positions` `[B, T]`, p <= positions[b, t]; one that sees none gives zeros.
+    with `positions` `[B, T]`, p <= positions[b, t]; one that sees none gives zeros.  `form`: 0 automatic, 1 mma.sync tiles on
+    thread-block clusters, 2 tcgen05 tiles (head_dim 128 or 256).
     """
     pages, page_size, hkv, d = _cache(k_cache_layer, v_cache_layer, k_scale, v_scale)
     device = k_cache_layer.device
@@ -160,12 +161,16 @@ def paged_decode_attention_quantized(q, k_cache_layer, v_cache_layer, k_scale, v
         return out
     if _k._poison():
         out.fill_(float("nan"))
+    lib = _lib.load()
     with _on(device):
+        nbytes = lib.nvj_paged_decode_quantized_workspace_bytes(batch, width, block_table.shape[1], page_size, hkv, d, hq, int(form))
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
         st = _k._status_word(device)
-        check(_lib.load().nvj_paged_decode_quantized(
+        check(lib.nvj_paged_decode_quantized(
             q.data_ptr(), _k._dt(q), k_cache_layer.data_ptr(), v_cache_layer.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pages,
             page_size, hkv, d, hq, block_table.data_ptr(), block_table.shape[1], seq_lens.data_ptr(), _k._ptr(positions), None, batch,
-            width, float(scale), out.data_ptr(), st.data_ptr(), _k._stream(device)), "nvj_paged_decode_quantized")
+            width, float(scale), out.data_ptr(), st.data_ptr(), _k._ptr(scratch), nbytes, int(form), _k._stream(device)),
+            "nvj_paged_decode_quantized")
         if _k._strict():
             _k._check_word(st, "nvj_paged_decode_quantized")
     return out

@@ -12,6 +12,7 @@ pytestmark = pytest.mark.gpu
 
 BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
 # query heads, kv heads, head_dim, block size
+FORMS = (1, 2)  # mma.sync tiles on clusters, tcgen05 tiles
 SHAPES = [(8, 2, 256, 16), (32, 8, 128, 16), (16, 2, 64, 32), (6, 6, 64, 48), (24, 2, 128, 64), (16, 1, 256, 16), (5, 1, 128, 32), (2, 2, 256, 64)]
 
 
@@ -207,6 +208,10 @@ def _check(out, q, state, tables, lens, limits, scale, term_bits=22):
         assert np.isfinite(out[r]).all() and off <= R.tolerance(q[r], k, v, scale, term_bits), (r, n, off)
 
 
+def _forms(shape):
+    return FORMS if shape[2] >= 128 else (1,)
+
+
 def _queries(rng, shape, dtype):
     q = torch.from_numpy(rng.standard_normal(shape)).to(dtype)
     return q.cuda(), _f64(q)
@@ -225,13 +230,14 @@ def test_decode(shape, dtype):
     _poison_behind(state, tables, LENGTHS, bs)
     q, q64 = _queries(rng, (len(LENGTHS), hq, d), dtype)
     (k, ks), (v, vs) = (_gpu(*s) for s in state)
-    out = Q.paged_decode_attention_quantized(q, k, v, ks, vs, _i32(tables), _i32(LENGTHS), d ** -0.5)
-    assert out.dtype == F32 and out.shape == q.shape
-    _check(_f64(out)[:, None], q64[:, None], state, tables, LENGTHS, [[n] for n in LENGTHS], d ** -0.5)
-    # the same rows one at a time (clusters of other sizes)
-    for r in (1, 9, 15):
-        one = Q.paged_decode_attention_quantized(q[r: r + 1], k, v, ks, vs, _i32(tables[r: r + 1]), _i32(LENGTHS[r: r + 1]), d ** -0.5)
-        _check(_f64(one)[:, None], q64[r: r + 1, None], state, tables[r: r + 1], LENGTHS[r: r + 1], [LENGTHS[r: r + 1]], d ** -0.5)
+    for form in _forms(shape):
+        out = Q.paged_decode_attention_quantized(q, k, v, ks, vs, _i32(tables), _i32(LENGTHS), d ** -0.5, form=form)
+        assert out.dtype == F32 and out.shape == q.shape
+        _check(_f64(out)[:, None], q64[:, None], state, tables, LENGTHS, [[n] for n in LENGTHS], d ** -0.5)
+        # the same rows one at a time (clusters of other sizes, other ranges)
+        for r in (1, 9, 15):
+            one = Q.paged_decode_attention_quantized(q[r: r + 1], k, v, ks, vs, _i32(tables[r: r + 1]), _i32(LENGTHS[r: r + 1]), d ** -0.5, form=form)
+            _check(_f64(one)[:, None], q64[r: r + 1, None], state, tables[r: r + 1], LENGTHS[r: r + 1], [LENGTHS[r: r + 1]], d ** -0.5)
 
 
 @pytest.mark.parametrize("width", [2, 3, 5, 9, 17])
@@ -248,16 +254,18 @@ def test_rows_of_several_tokens(shape, dtype, width):
     limits = rng.integers(-2, 40, (len(lens), width)) + np.array(lens)[:, None] - 20  # some see nothing, some more than there is
     limits[3] = 33
     args = (q, k, v, ks, vs, _i32(tables), _i32(lens), d ** -0.5)
-    out = Q.paged_decode_attention_quantized(*args, positions=_i32(limits - 1))
-    assert out.shape == (len(lens), width, hq * d)
-    _check(_f64(out).reshape(q64.shape), q64, state, tables, lens, limits, d ** -0.5)
-    free = Q.paged_decode_attention_quantized(*args)
-    _check(_f64(free).reshape(q64.shape), q64, state, tables, lens, [[n] * width for n in lens], d ** -0.5)
+    for form in _forms(shape):
+        out = Q.paged_decode_attention_quantized(*args, positions=_i32(limits - 1), form=form)
+        assert out.shape == (len(lens), width, hq * d)
+        _check(_f64(out).reshape(q64.shape), q64, state, tables, lens, limits, d ** -0.5)
+        free = Q.paged_decode_attention_quantized(*args, form=form)
+        _check(_f64(free).reshape(q64.shape), q64, state, tables, lens, [[n] * width for n in lens], d ** -0.5)
 
 
+@pytest.mark.parametrize("form", FORMS)
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("scale", [0.0, -0.07, 1.5])
-def test_any_scale_of_the_scores(scale, dtype):
+def test_any_scale_of_the_scores(scale, dtype, form):
     # 1.5: scores of tens, a softmax that is nearly one-hot, maxima that move
     hq, hkv, d, bs = shape = SHAPES[1]
     rng = np.random.default_rng(11)
@@ -266,11 +274,11 @@ def test_any_scale_of_the_scores(scale, dtype):
     state = [_pool(rng, 60, shape, spread=1) for _ in range(2)]
     q, q64 = _queries(rng, (3, hq, d), dtype)
     (k, ks), (v, vs) = (_gpu(*s) for s in state)
-    out = Q.paged_decode_attention_quantized(q, k, v, ks, vs, _i32(tables), _i32(lens), scale)
+    out = Q.paged_decode_attention_quantized(q, k, v, ks, vs, _i32(tables), _i32(lens), scale, form=form)
     _check(_f64(out)[:, None], q64[:, None], state, tables, lens, [[n] for n in lens], scale)
 
 
-@pytest.mark.parametrize("route", ["decode", "prefill"])
+@pytest.mark.parametrize("route", [1, 2, "prefill"])
 def test_blocks_of_very_different_scales(route):
     # V: one block in four 2^100 as loud, and one row of quiet blocks alone; K: the loud ones' scores are -1000s, so that the quiet blocks decide
     hq, hkv, d, bs = shape = SHAPES[1]
@@ -292,8 +300,8 @@ def test_blocks_of_very_different_scales(route):
     q64 = _f64(qg)
     (k, ks), (v, vs) = (_gpu(*s) for s in state)
     args = (k, v, ks, vs, _i32(tables), _i32(lens))
-    if route == "decode":
-        out = Q.paged_decode_attention_quantized(qg, *args, d ** -0.5)
+    if route != "prefill":
+        out = Q.paged_decode_attention_quantized(qg, *args, d ** -0.5, form=route)
     else:
         out = Q.packed_paged_prefill_attention_quantized(qg[None], *args, _i32([[159, 159, 89]]), _i32([0, 1, 2, 3]), bs, d ** -0.5, hq // hkv,
                                                          num_decode_rows=0)
@@ -307,8 +315,9 @@ def test_blocks_of_very_different_scales(route):
         assert np.abs(out[r] - want).max() <= within
 
 
+@pytest.mark.parametrize("form", FORMS)
 @pytest.mark.parametrize("queries", [2.0 ** 40, 2.0 ** -40, 0.0])
-def test_queries_of_any_size(queries):
+def test_queries_of_any_size(queries, form):
     hq, hkv, d, bs = shape = SHAPES[0]
     rng = np.random.default_rng(13)
     lens = [50, 20]
@@ -318,11 +327,12 @@ def test_queries_of_any_size(queries):
     (k, ks), (v, vs) = (_gpu(*s) for s in state)
     for dtype in (BF16, F32):
         q = torch.from_numpy(rng.standard_normal((2, hq, d)) * queries).to(dtype).cuda()
-        out = Q.paged_decode_attention_quantized(q, k, v, ks, vs, _i32(tables), _i32(lens), 1 / 16)
+        out = Q.paged_decode_attention_quantized(q, k, v, ks, vs, _i32(tables), _i32(lens), 1 / 16, form=form)
         _check(_f64(out)[:, None], _f64(q)[:, None], state, tables, lens, [[n] for n in lens], 1 / 16)
 
 
-def test_nan_and_infinite_queries_stay_in_their_row_and_head():
+@pytest.mark.parametrize("form", FORMS)
+def test_nan_and_infinite_queries_stay_in_their_row_and_head(form):
     hq, hkv, d, bs = shape = SHAPES[0]
     rng = np.random.default_rng(14)
     lens = [50, 40]
@@ -330,9 +340,9 @@ def test_nan_and_infinite_queries_stay_in_their_row_and_head():
     state = [_pool(rng, 10, shape) for _ in range(2)]
     (k, ks), (v, vs) = (_gpu(*s) for s in state)
     q = torch.from_numpy(rng.standard_normal((2, hq, d))).to(BF16).cuda()
-    clean = Q.paged_decode_attention_quantized(q, k, v, ks, vs, _i32(tables), _i32(lens), 1 / 16)
+    clean = Q.paged_decode_attention_quantized(q, k, v, ks, vs, _i32(tables), _i32(lens), 1 / 16, form=form)
     q[0, 3, 7], q[1, 6, 0] = float("nan"), float("inf")
-    out = Q.paged_decode_attention_quantized(q, k, v, ks, vs, _i32(tables), _i32(lens), 1 / 16)
+    out = Q.paged_decode_attention_quantized(q, k, v, ks, vs, _i32(tables), _i32(lens), 1 / 16, form=form)
     assert torch.isnan(out[0, 3]).all() and torch.isnan(out[1, 6]).all()
     out[0, 3], out[1, 6] = clean[0, 3], clean[1, 6]
     assert torch.equal(out, clean)
@@ -346,22 +356,23 @@ def test_what_lies_outside_the_pool_or_the_table_is_flagged(monkeypatch):
     q, q64 = _queries(rng, (2, hq, d), BF16)
     monkeypatch.setenv("NVJ_CHECK_STATUS", "0")
     tables = np.array([[1, 8, 3], [4, 5, -7]])
-    for prefill in (False, True):
-        if prefill:
+    for form in (None, 1, 2):
+        if form is None:
             out = Q.packed_paged_prefill_attention_quantized(q[None], k, v, ks, vs, _i32(tables), _i32([48, 40]), _i32([[47, 39]]), _i32([0, 1, 2]), bs,
                                                              d ** -0.5, hq // hkv, num_decode_rows=0)[0].view(2, hq, d)
         else:
-            out = Q.paged_decode_attention_quantized(q, k, v, ks, vs, _i32(tables), _i32([48, 40]), d ** -0.5)
+            out = Q.paged_decode_attention_quantized(q, k, v, ks, vs, _i32(tables), _i32([48, 40]), d ** -0.5, form=form)
         for r, good in ((0, [0, 2]), (1, [0, 1])):  # the other blocks' keys alone
             kk, vv = (R.gather(codes, s, tables[r][good], 32) for codes, s in state)
             want = R.attend(q64[r: r + 1], kk, vv, np.ones((1, 32), bool), d ** -0.5)[0]
             assert np.abs(_f64(out[r]) - want).max() <= R.tolerance(q64[r: r + 1], kk, vv, d ** -0.5)
         with pytest.raises(K.DeviceStatusError, match="device status 2 "):
             K.check_device_status()
-    long = Q.paged_decode_attention_quantized(q, k, v, ks, vs, _i32([[1, 2], [3, 4]]), _i32([33, 1 << 30]), d ** -0.5)
-    with pytest.raises(K.DeviceStatusError, match="device status 4 "):
-        K.check_device_status()
-    assert torch.equal(long, Q.paged_decode_attention_quantized(q, k, v, ks, vs, _i32([[1, 2], [3, 4]]), _i32([32, 32]), d ** -0.5))
+    for form in FORMS:
+        long = Q.paged_decode_attention_quantized(q, k, v, ks, vs, _i32([[1, 2], [3, 4]]), _i32([33, 1 << 30]), d ** -0.5, form=form)
+        with pytest.raises(K.DeviceStatusError, match="device status 4 "):
+            K.check_device_status()
+        assert torch.equal(long, Q.paged_decode_attention_quantized(q, k, v, ks, vs, _i32([[1, 2], [3, 4]]), _i32([32, 32]), d ** -0.5, form=form))
 
 
 def test_blocks_beyond_four_gigabytes():
@@ -386,23 +397,25 @@ def test_blocks_beyond_four_gigabytes():
         R.append(codes, scale, _f64(new)[:, 0], [(2, 8), (5, 15)], bs)
     _same([(n.view(torch.uint8)[far].view(torch.float8_e4m3fn), s[far]) for n, s in big], state)
     q, q64 = _queries(rng, (2, hq, d), BF16)
-    out = Q.paged_decode_attention_quantized(q, big[0][0], big[1][0], big[0][1], big[1][1], _i32(far[local]), _i32([41, 48]), 1 / 16)
-    _check(_f64(out)[:, None], q64[:, None], state, local, [41, 48], [[41], [48]], 1 / 16)
+    for form in FORMS:
+        out = Q.paged_decode_attention_quantized(q, big[0][0], big[1][0], big[0][1], big[1][1], _i32(far[local]), _i32([41, 48]), 1 / 16, form=form)
+        _check(_f64(out)[:, None], q64[:, None], state, local, [41, 48], [[41], [48]], 1 / 16)
     for dtype in (BF16, F32):
         out = Q.packed_paged_prefill_attention_quantized(q.to(dtype)[None], big[0][0], big[1][0], big[0][1], big[1][1], _i32(far[local]), _i32([41, 48]),
                                                          _i32([[40, 47]]), _i32([0, 1, 2]), bs, 1 / 16, 4, num_decode_rows=0)
         _check(_f64(out).reshape(2, 1, hq, d), q64[:, None], state, local, [41, 48], [[41], [48]], 1 / 16, 16)
 
 
-def test_more_rows_than_a_grid_dimension_holds():
-    hq, hkv, d, bs = shape = SHAPES[3]
+@pytest.mark.parametrize("shape,form", [(SHAPES[3], 1), (SHAPES[6], 2)])
+def test_more_rows_than_a_grid_dimension_holds(shape, form):
+    hq, hkv, d, bs = shape
     rows = 65536 + 5
     rng = np.random.default_rng(17)
     state = [_pool(rng, 30, shape) for _ in range(2)]
     (k, ks), (v, vs) = (_gpu(*s) for s in state)
     tables, lens = rng.integers(0, 30, (rows, 1)), rng.integers(0, bs + 1, rows)
     q = torch.randn((rows, hq, d), device="cuda").to(BF16)
-    out = Q.paged_decode_attention_quantized(q, k, v, ks, vs, _i32(tables), _i32(lens), d ** -0.5)
+    out = Q.paged_decode_attention_quantized(q, k, v, ks, vs, _i32(tables), _i32(lens), d ** -0.5, form=form)
     assert torch.isfinite(out).all()
     pick = [0, 1, 40000, 65534, 65535, 65536, rows - 1]
     _check(_f64(out[pick])[:, None], _f64(q[pick])[:, None], state, tables[pick], lens[pick], [[n] for n in lens[pick]], d ** -0.5)
@@ -600,6 +613,22 @@ def test_the_same_inputs_give_the_same_bits():
     state = [_pool(rng, 260, shape) for _ in range(2)]
     (k, ks), (v, vs) = (_gpu(*s) for s in state)
     q, _ = _queries(rng, (3, hq, d), BF16)
-    first = Q.paged_decode_attention_quantized(q, k, v, ks, vs, _i32(tables), _i32(lens), 1 / 16)
-    for _ in range(5):
-        assert torch.equal(first, Q.paged_decode_attention_quantized(q, k, v, ks, vs, _i32(tables), _i32(lens), 1 / 16))
+    for form in FORMS:
+        first = Q.paged_decode_attention_quantized(q, k, v, ks, vs, _i32(tables), _i32(lens), 1 / 16, form=form)
+        for _ in range(5):
+            assert torch.equal(first, Q.paged_decode_attention_quantized(q, k, v, ks, vs, _i32(tables), _i32(lens), 1 / 16, form=form))
+
+
+@pytest.mark.parametrize("shape,dtype,rows,hi", [(SHAPES[0], BF16, 300, 700), (SHAPES[1], F16, 40, 1500), (SHAPES[4], F32, 9, 2500), (SHAPES[6], BF16, 1, 9000)])
+def test_rows_cut_over_many_ranges_of_the_tcgen05_tiles(shape, dtype, rows, hi):
+    hq, hkv, d, bs = shape
+    rng = np.random.default_rng(rows)
+    lens = rng.integers(0, hi + 1, rows)
+    lens[0] = hi
+    tables = _tables(rng, lens, bs, int((-(-lens // bs)).sum()))
+    state = [_pool(rng, int(tables.max()) + 1, shape) for _ in range(2)]
+    _poison_behind(state, tables, lens, bs)
+    q, q64 = _queries(rng, (rows, hq, d), dtype)
+    (k, ks), (v, vs) = (_gpu(*s) for s in state)
+    out = Q.paged_decode_attention_quantized(q, k, v, ks, vs, _i32(tables), _i32(lens), d ** -0.5, form=2)
+    _check(_f64(out)[:, None], q64[:, None], state, tables, lens, [[n] for n in lens], d ** -0.5)

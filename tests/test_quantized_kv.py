@@ -22,7 +22,7 @@ def _append(**change):
 
 def _decode(**change):
     a = dict(q=P, dtype=0, k=P, v=P, ks=P, vs=P, blocks=8, bs=16, hkv=2, d=256, hq=8, tables=P, width=4, lens=P, pos=None, qsl=None, rows=2,
-             tokens=1, scale=1.0, out=P, status=P) | change
+             tokens=1, scale=1.0, out=P, status=P, ws=None, nbytes=0, form=0) | change
     return _lib.load().nvj_paged_decode_quantized(*a.values(), None)
 
 
@@ -57,7 +57,7 @@ def test_appends_that_are_refused(change, code):
 @pytest.mark.parametrize("change,code", [
     ({"hq": 9}, INVALID), ({"hq": 0}, INVALID), ({"q": P + 2}, INVALID), ({"out": P + 4}, INVALID), ({"lens": None}, INVALID),
     ({"qsl": P, "tokens": 2}, INVALID), ({"qsl": P, "pos": None}, INVALID), ({"width": 1 << 27}, TOO_LARGE),
-    ({"tokens": 1 << 15}, TOO_LARGE)])
+    ({"tokens": 1 << 15}, TOO_LARGE), ({"form": 3}, INVALID), ({"form": -1}, INVALID)])
 def test_decode_calls_that_are_refused(change, code):
     assert _decode(**change) == code
 
