@@ -13,14 +13,17 @@
 //
 // Work split: CTA = (range, kv head and column tile).  The 16-key units of all rows form one sequence that is cut into equal ranges
 // (decode_parts.cuh); rows cut over ranges leave partials, folded by a second small launch.
-//   warps 0 - 3  softmax, thread = key: scores from tensor memory, times the K scale of the key's block; weights
-//                exp2(s + log2 V scale - reference) as e4m3 terms into shared memory; their sum without the V scale under a
-//                reference of its own.  References move only when a score passes one by 2^8 (weights up to 2^8 <= 448).  Thread = dim when
-//                a row's segment ends.
-//   warp 4       MMA issue.
-//   warp 5       TMA producer: 16-key boxes [8-key group][128-byte chunk][8 keys][128 B], 128-byte swizzle, into a ring of tiles of K
-//                and V in turn (160 KiB).
-//   warps 6, 7   the next segment's queries: scaled to 2^7 - 2^8 by a power of two per column, split into terms.
+//   warps 0 - 7   softmax, thread = key, in two groups of four warps.  Up to eight columns the groups take the tiles in turn, each with
+//                 references, sums and accumulators of its own (a tile's chain of waits, from its scores to its weights, is longer than
+//                 its bytes: one group alone took 1.85 us per tile of 64 KiB); with 16 or 24 they take half of the columns each.
+//                 Scores from tensor memory, times the K scale of the key's block; weights exp2(s + log2 V scale - reference) as
+//                 e4m3 terms into shared memory; their sum without the V scale under a reference of its own.  A reference is set 2^4 above
+//                 the largest score and moves when a score passes it by 2^8 (weights up to 2^8 <= 448).  Thread = dim when a
+//                 row's segment ends.
+//   warp 8        MMA issue: the scores of the next tile in front of the weighted sum of this one.
+//   warp 9        TMA producer: 16-key boxes [8-key group][128-byte chunk][8 keys][128 B], 128-byte swizzle, into a ring of tiles of K
+//                 and V in turn (160 KiB).
+//   warps 10, 11  the queries, up to two segments ahead: scaled to 2^7 - 2^8 by a power of two per column, split into terms.
 // Every wait is bounded; after a timeout (NVJ_DEV_TIMEOUT) the kernel stops issuing, lets copies land and frees its tensor
 // memory.  A block id outside the pool is flagged, fetched from beyond the tensor (zeros) and its keys are left out.
 #pragma once
@@ -38,41 +41,50 @@ constexpr int kQuTile = 128;    // keys per tile
 constexpr int kQuUnit = 16;     // keys per box
 constexpr int kQuUnits = kQuTile / kQuUnit;
 constexpr int kQuPTerms = 5;
-constexpr float kQuNone = -3e38f, kQuSlack = 8.f;
+constexpr int kQuThreads = 384;
+constexpr float kQuNone = -3e38f, kQuSlack = 8.f, kQuHead = 4.f;
 
 template <typename T>
 constexpr int quq_terms() {
   return sizeof(T) == 4 ? 5 : std::is_same<T, __half>::value ? 3 : 2;
 }
 
-template <typename T, int kDim, int kC>
+// kCg: columns of a softmax thread; kByTiles: the two groups take the tiles in turn, else half of the columns each.
+template <typename T, int kDim, int kCg, bool kByTiles>
 struct QuLayout {
+  static constexpr int kC = kByTiles ? kCg : 2 * kCg;  // columns of the CTA
+  static constexpr int kRegions = kByTiles ? 1 : 2;    // of a row of query terms or weights: one per group that shares a tile
   static constexpr int kQTerms = quq_terms<T>();
   static constexpr int kChunks = kDim / 128;
-  static constexpr int kNS = (kQTerms * kC + 15) / 16 * 16;   // columns of S (N of an MMA: multiples of 16)
-  static constexpr int kNO = (kQuPTerms * kC + 15) / 16 * 16;  // columns of O
-  static constexpr int kSets0 = (512 - kNS) / (kNO * kChunks);
-  static constexpr int kSets = kSets0 < 1 ? 1 : (kSets0 > 3 ? 3 : kSets0);  // accumulators that take the tiles in turn: shorter sums
-  static constexpr int kColO = kNS;
-  static constexpr int kTileBytes = kQuTile * kDim;           // of K (or V)
+  static constexpr int kSRegion = kQTerms * kCg;                        // columns of S: [region][term][kCg]
+  static constexpr int kORegion = (kQuPTerms * kCg + 15) / 16 * 16;     // columns of O: [region][term][kCg], padded
+  static constexpr int kNS = (kRegions * kSRegion + 15) / 16 * 16;      // (N of an MMA: multiples of 16)
+  static constexpr int kNO = kRegions * kORegion;
+  static constexpr int kSets0 = (512 - 2 * kNS) / (kNO * kChunks);      // accumulators that take the tiles in turn: shorter sums
+  static constexpr int kSets = kByTiles ? (kSets0 < 4 ? 2 : 4) : (kSets0 < 2 ? 1 : 2);
+  static constexpr int kColO = 2 * kNS;                                 // S twice, then the sets
+  static constexpr int kTileBytes = kQuTile * kDim;                     // of K (or V)
   static constexpr int kUnitBytes = kQuUnit * kDim;
-  static constexpr int kSlots = 160 * 1024 / kTileBytes;
-  static constexpr int kQChunk = kNS * 128;                   // bytes of a chunk of the query terms
+  static constexpr int kQChunk = kNS * 128;                             // bytes of a chunk of the query terms
+  static constexpr int kQBytes = kChunks * kQChunk, kWBytes = kQuTile * 128;
+  static constexpr int kFit = (232448 - 1024 - 6144 - 2 * kQBytes - 2 * kWBytes) / kTileBytes;
+  static constexpr int kSlots = kFit < 160 * 1024 / kTileBytes ? kFit : 160 * 1024 / kTileBytes;
   static_assert(kNO <= 128 && kNS <= 256, "a row of weights is 128 bytes");
-  static_assert(kNS + kSets * kChunks * kNO <= 512, "tensor memory");
+  static_assert(kColO + kSets * kChunks * kNO <= 512, "tensor memory");
+  static_assert(kSlots >= 3, "a tile of K and of V, and one on its way");
 };
 
-template <typename T, int kDim, int kC>
+template <class L>
 struct QuSmem {
-  using L = QuLayout<T, kDim, kC>;
   alignas(1024) char slot[L::kSlots][L::kTileBytes];
-  alignas(1024) char q[L::kChunks][L::kQChunk];  // [chunk][term * kC + column][128 B]
-  alignas(1024) char w[kQuTile * 128];           // weights' terms [key][128 B]
-  alignas(8) unsigned long long full[L::kSlots], empty[L::kSlots], q_full, q_free, s_full, p_full, o_full, o_free;
-  alignas(16) float factor[2][kC];  // by segment parity: what a column's products are multiplied by, and the keys it may see
-  alignas(16) int limit[2][kC];
-  alignas(16) float red[4][kC], red_v[4][kC];
-  alignas(16) float m[kC], mv[kC], f[kC], fv[kC];
+  alignas(1024) char q[2][L::kChunks][L::kQChunk];  // by segment parity: [chunk][region, term, column][128 B]
+  alignas(1024) char w[2][L::kWBytes];              // by tile parity: weights' terms [key][128 B]
+  alignas(8) unsigned long long full[L::kSlots], empty[L::kSlots], q_full[2], q_free[2], s_full[2], p_full[2], pv_done[2], o_full, o_free;
+  alignas(16) float factor[4][L::kC];  // by segment: what a column's products are multiplied by, and the keys it may see
+  alignas(16) int limit[4][L::kC];
+  alignas(16) float red[2][4][12], red_v[2][4][12];  // per group and warp
+  alignas(16) float m[2][12], mv[2][12], f[2][12], fv[2][12];
+  alignas(16) float out_f[2][L::kC];  // what a group's sums are multiplied by at the end
   int scan[16];
   int start_b, start_j, abort_flag;
   uint32_t tmem_base;
@@ -104,19 +116,41 @@ __device__ __forceinline__ void qu_tmem_st8(uint32_t taddr, const float (&v)[8])
 __device__ __forceinline__ void qu_sts4(uint32_t at, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
-// Whether `mine` holds in any thread of the softmax warps, which meet here.
-__device__ __forceinline__ bool qu_meet_any(bool mine) {
+// Whether `mine` holds in any of the `threads` threads that meet at barrier `id`.
+template <int kThreads>
+__device__ __forceinline__ bool qu_meet_any(int id, bool mine) {
   uint32_t any;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
-      "barrier.cta.red.or.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-      : "=r"(any) : "r"((uint32_t)mine) : "memory");
+      "barrier.cta.red.or.pred q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(any) : "r"((uint32_t)mine), "r"(id), "n"(kThreads) : "memory");
   return any != 0;
 }
 // The warp's largest x (order-preserving integers; a NaN with a clear sign counts as the largest).
 __device__ __forceinline__ float qu_warp_max(float x) {
   const int i = __float_as_int(x), k = __reduce_max_sync(kFullMask, i ^ ((i >> 31) & 0x7fffffff));
   return __int_as_float(k ^ ((k >> 31) & 0x7fffffff));
+}
+// Inclusive scan of one int per thread over the CTA.
+__device__ __forceinline__ int qu_inclusive_scan(int v, int* warp_sums, int& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int n = __shfl_up_sync(kFullMask, v, o);
+    if (lane >= o) v += n;
+  }
+  __syncthreads();
+  if (lane == 31) warp_sums[warp] = v;
+  __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kQuThreads / 32; ++w) {
+    const int x = warp_sums[w];
+    if (w < warp) before += x;
+    all += x;
+  }
+  total = all;
+  return v + before;
 }
 
 // A place in the ring: K and V of a tile follow one another.
@@ -146,11 +180,10 @@ struct QuWalk {
   }
 };
 
-// ---- warp 5: TMA loads ------------------------------------------------------------------------------------------------------------
-template <typename T, int kDim, int kC>
-__device__ __forceinline__ void qu_producer(const CUtensorMap* k_map, const CUtensorMap* v_map, const QuParams& a, const DecodeParams& p,
-                                            QuSmem<T, kDim, kC>& sm, int head, QuWalk walk, int lane) {
-  using L = QuLayout<T, kDim, kC>;
+// ---- warp 9: TMA loads ------------------------------------------------------------------------------------------------------------
+template <class L>
+__device__ __forceinline__ void qu_producer(const CUtensorMap* k_map, const CUtensorMap* v_map, const DecodeParams& p, QuSmem<L>& sm, int head,
+                                            QuWalk walk, int lane) {
   const int per_block = p.block_size / kQuUnit;
   const int oob = (int)(p.num_blocks * (p.block_size / 8));  // a box that starts here is filled with zeros
   uint64_t policy;  // every block is read once
@@ -198,62 +231,89 @@ __device__ __forceinline__ void qu_producer(const CUtensorMap* k_map, const CUte
   }
 }
 
-// ---- warp 4: MMA issue ------------------------------------------------------------------------------------------------------------
-template <typename T, int kDim, int kC>
-__device__ __forceinline__ void qu_mma_warp(QuSmem<T, kDim, kC>& sm, const DecodeParams& p, uint32_t tmem, QuWalk walk) {
-  using L = QuLayout<T, kDim, kC>;
+// ---- warp 8: MMA issue ------------------------------------------------------------------------------------------------------------
+// S(n + 1), then O += V(n)^T P(n).  S(n) is issued behind the weighted sum of tile n - 2, which has waited for its weights: the scores
+// of tile n - 2 have been read by then, and their place is S(n)'s.
+template <class L>
+__device__ __forceinline__ void qu_mma_warp(QuSmem<L>& sm, const DecodeParams& p, uint32_t tmem, QuWalk walk) {
   constexpr uint32_t idesc_s = qu_idesc(L::kNS, false, false), idesc_o = qu_idesc(L::kNO, true, true);
-  const uint64_t k_desc0 = umma_desc(smem_u32(sm.slot[0]), 16, L::kChunks * 1024);  // keys are rows: groups of 8
+  const uint64_t k_desc0 = umma_desc(smem_u32(sm.slot[0]), 16, L::kChunks * 1024);    // keys are rows: groups of 8
   const uint64_t v_desc0 = umma_desc(smem_u32(sm.slot[0]), 1024, L::kChunks * 1024);  // dims are rows, a chunk at a time; keys in groups of 8
-  const uint64_t q_desc = umma_desc(smem_u32(sm.q[0]), 16, 1024);
-  const uint64_t w_desc = umma_desc(smem_u32(sm.w), 1024, 1024);
-  QuRing<L::kSlots> at;
-  QuSeg s;
-  uint32_t tile = 0;
+  const uint64_t q_desc0 = umma_desc(smem_u32(sm.q[0][0]), 16, 1024);
+  const uint64_t w_desc0 = umma_desc(smem_u32(sm.w[0]), 1024, 1024);
+  QuWalk ahead = walk;  // of the scores
+  QuSeg sa, s;
+  QuRing<L::kSlots> k_at, v_at;  // K slots and V slots: every other place of the ring, from 0 and from 1
+  v_at.step();
+  int ta = 0;
+  uint32_t na = 0, seg_a = 0;
+  bool more = ahead.next(p, sa);
+  auto scores = [&]() -> bool {  // of the next tile, if there is one
+    if (!more) return true;
+    const uint32_t qb = seg_a & 1u;
+    if (ta == 0 && !um_wait(&sm.q_full[qb], (seg_a >> 1) & 1u, &sm.abort_flag, p.status)) return false;
+    if (!um_wait(&sm.full[k_at.at], k_at.phase, &sm.abort_flag, p.status)) return false;
+    tc_fence_after_sync();
+    const bool last = ta == sa.tiles() - 1;
+    if (um_elect_one()) {
+      // (rows of keys that the tile does not have are computed from whatever lies there, and masked)
+      const uint64_t k_desc = k_desc0 + (uint64_t)((k_at.at * L::kTileBytes) >> 4), q_desc = q_desc0 + (uint64_t)((qb * L::kQBytes) >> 4);
+#pragma unroll
+      for (int ks = 0; ks < L::kChunks * 4; ++ks)
+        qu_mma(tmem + (na & 1u) * L::kNS, k_desc + (uint64_t)(((ks >> 2) * 1024 + (ks & 3) * 32) >> 4),
+               q_desc + (uint64_t)(((ks >> 2) * L::kQChunk + (ks & 3) * 32) >> 4), idesc_s, ks > 0 ? 1u : 0u);
+      umma_commit(smem_u32(&sm.s_full[na & 1u]));
+      umma_commit(smem_u32(&sm.empty[k_at.at]));
+      if (last) umma_commit(smem_u32(&sm.q_free[qb]));
+    }
+    __syncwarp();
+    k_at.step();
+    k_at.step();
+    ++na;
+    if (last) {
+      ta = 0;
+      ++seg_a;
+      more = ahead.next(p, sa);
+    } else {
+      ++ta;
+    }
+    return true;
+  };
+  if (!scores()) return;
+  uint32_t n = 0;
   for (uint32_t seg = 0; walk.next(p, s); ++seg) {
     const int nt = s.tiles();
-    for (int t = 0; t < nt; ++t, ++tile) {
-      // (rows of keys that the tile does not have are computed from whatever lies there, and masked)
-      if (t == 0 && !um_wait(&sm.q_full, seg & 1u, &sm.abort_flag, p.status)) return;
-      if (!um_wait(&sm.full[at.at], at.phase, &sm.abort_flag, p.status)) return;
-      tc_fence_after_sync();
-      if (um_elect_one()) {
-        const uint64_t k_desc = k_desc0 + (uint64_t)((at.at * L::kTileBytes) >> 4);
-#pragma unroll
-        for (int ks = 0; ks < kDim / 32; ++ks)
-          qu_mma(tmem, k_desc + (uint64_t)(((ks >> 2) * 1024 + (ks & 3) * 32) >> 4), q_desc + (uint64_t)(((ks >> 2) * L::kQChunk + (ks & 3) * 32) >> 4),
-                 idesc_s, ks > 0 ? 1u : 0u);
-        umma_commit(smem_u32(&sm.s_full));
-        umma_commit(smem_u32(&sm.empty[at.at]));
-        if (t == nt - 1) umma_commit(smem_u32(&sm.q_free));
-      }
-      __syncwarp();
-      at.step();
-      if (!um_wait(&sm.full[at.at], at.phase, &sm.abort_flag, p.status)) return;
-      if (!um_wait(&sm.p_full, tile & 1u, &sm.abort_flag, p.status)) return;
-      // the first weighted sum of a segment overwrites O: the segment before must have been read out
+    const uint32_t n0 = n;
+    for (int t = 0; t < nt; ++t, ++n) {
+      if (!scores()) return;
+      if (!um_wait(&sm.full[v_at.at], v_at.phase, &sm.abort_flag, p.status)) return;
+      if (!um_wait(&sm.p_full[n & 1u], (n >> 1) & 1u, &sm.abort_flag, p.status)) return;
+      // the first weighted sums of a segment overwrite O: the segment before must have been read out
       if (t == 0 && seg > 0 && !um_wait(&sm.o_free, (seg - 1) & 1u, &sm.abort_flag, p.status)) return;
       tc_fence_after_sync();
       if (um_elect_one()) {
         const int steps = (s.tile_units(t) + 1) / 2;
-        const uint32_t o = tmem + L::kColO + (t % L::kSets) * (L::kChunks * L::kNO);
-        const uint64_t v_desc = v_desc0 + (uint64_t)((at.at * L::kTileBytes) >> 4);
+        const uint32_t o = tmem + L::kColO + ((n0 & 1u) + t) % L::kSets * (L::kChunks * L::kNO);
+        const uint64_t v_desc = v_desc0 + (uint64_t)((v_at.at * L::kTileBytes) >> 4), w_desc = w_desc0 + (uint64_t)(((n & 1u) * L::kWBytes) >> 4);
         for (int i = 0; i < steps; ++i) {  // 32 keys, four groups of 8
-          const uint32_t more = (t >= L::kSets || i > 0) ? 1u : 0u;
+          const uint32_t accumulate = (t >= L::kSets || i > 0) ? 1u : 0u;
           const uint64_t wd = w_desc + (uint64_t)((i * 32 * 128) >> 4), vd = v_desc + (uint64_t)((i * 2 * L::kUnitBytes) >> 4);
 #pragma unroll
-          for (int h = 0; h < L::kChunks; ++h) qu_mma(o + h * L::kNO, vd + (uint64_t)((h * 1024) >> 4), wd, idesc_o, more);
+          for (int h = 0; h < L::kChunks; ++h) qu_mma(o + h * L::kNO, vd + (uint64_t)((h * 1024) >> 4), wd, idesc_o, accumulate);
         }
-        umma_commit(smem_u32(&sm.empty[at.at]));
+        umma_commit(smem_u32(&sm.pv_done[n & 1u]));
+        umma_commit(smem_u32(&sm.empty[v_at.at]));
         if (t == nt - 1) umma_commit(smem_u32(&sm.o_full));
       }
       __syncwarp();
-      at.step();
+      v_at.step();
+      v_at.step();
     }
   }
 }
 
-// Scales of the CTA's tiles, one tile ahead: thread = key.  `id` belongs to the tile behind `k_unit` and `v_unit`.
+// Scales of a group's tiles, one tile ahead: thread = key.  `id` belongs to the tile behind the one whose scales were given out last.
+template <bool kByTiles>
 struct QuScales {
   QuWalk walk;
   QuSeg s;
@@ -261,18 +321,25 @@ struct QuScales {
   bool have;
   int id;
 
+  __device__ __forceinline__ void one_on(const DecodeParams& p) {
+    if (have && ++t == s.tiles()) {
+      t = 0;
+      have = walk.next(p, s);
+    }
+  }
   __device__ __forceinline__ void fetch_id(const DecodeParams& p, int key) {
     id = -1;
     const int u = t * kQuUnits + key / kQuUnit;
     if (have && u < s.n) id = p.block_tables[(long long)s.b * p.table_width + (s.j0 + u) / (p.block_size / kQuUnit)];
   }
-  __device__ __forceinline__ void begin(const DecodeParams& p, const QuWalk& w, int key) {
+  __device__ __forceinline__ void begin(const DecodeParams& p, const QuWalk& w, int key, int group) {
     walk = w;
     t = 0;
     have = walk.next(p, s);
+    if (kByTiles && group == 1) one_on(p);
     fetch_id(p, key);
   }
-  // the scales of the tile whose id is here (of -1: no key), and the id of the one behind it
+  // the scales of the tile whose id is here (V's -1: no key), and the id of the group's next one
   __device__ __forceinline__ void step(const QuParams& a, const DecodeParams& p, int key, int head, float& k_unit, float& v_unit) {
     k_unit = 0.f;
     v_unit = -1.f;
@@ -280,129 +347,150 @@ struct QuScales {
       k_unit = a.k_scale[(long long)id * a.num_kv_heads + head];
       v_unit = a.v_scale[(long long)id * a.num_kv_heads + head];
     }
-    if (have && ++t == s.tiles()) {
-      t = 0;
-      have = walk.next(p, s);
-    }
+    one_on(p);
+    if (kByTiles) one_on(p);
     fetch_id(p, key);
   }
 };
 
-// ---- warps 0 - 3: softmax and output.  Thread = key of the tile, then dim of the output ---------------------------------------
-// (A wait that runs out does so for one warp and perhaps not for the next: they leave together, behind a meeting.)
-template <typename T, int kDim, int kC>
-__device__ __forceinline__ void qu_softmax_warps(QuSmem<T, kDim, kC>& sm, const QuParams& a, const DecodeParams& p, uint32_t tmem, int head, int hct,
-                                                 int ct, QuWalk walk, int range, int warp, int lane) {
-  using L = QuLayout<T, kDim, kC>;
-  constexpr int kSRead = (L::kQTerms * kC + 7) / 8, kORead = (kQuPTerms * kC + 7) / 8;  // pieces of 8 columns
-  const int key = warp * 32 + lane;
-  const uint32_t w_row = smem_u32(sm.w) + key * 128;
+// ---- warps 0 - 7: softmax and output.  Thread = key of the tile, then dim of the output ---------------------------------------
+// (A wait that runs out does so for one warp and perhaps not for the next: a group's warps leave together, behind a meeting.)
+template <class L, int kCg, bool kByTiles>
+__device__ __forceinline__ void qu_softmax_warps(QuSmem<L>& sm, const QuParams& a, const DecodeParams& p, uint32_t tmem, int head, int hct, int ct,
+                                                 QuWalk walk, int range, int group, int warp, int lane) {
+  constexpr int kSRead = (L::kSRegion + 7) / 8, kORead = (kQuPTerms * kCg + 7) / 8;  // pieces of 8 columns
+  constexpr int kDim = L::kChunks * 128, kWords = L::kORegion / 4;
+  const int key = warp * 32 + lane, region = kByTiles ? 0 : group, first_col = kByTiles ? 0 : group * kCg, bar = 1 + group;
   tmem += (uint32_t)(warp * 32) << 16;
-  QuScales scales;
-  scales.begin(p, walk, key);
+  // a group that leaves early meets the other one, which waits at a segment's end or leaves as well
+  auto give_up = [] { qu_meet_any<256>(3, true); };
+  float(&gm)[12] = sm.m[group];
+  float(&gmv)[12] = sm.mv[group];
+  QuScales<kByTiles> scales;
+  scales.begin(p, walk, key, group);
   float next_k, next_v;
   scales.step(a, p, key, head, next_k, next_v);
   QuRing<L::kSlots> at;
   QuSeg s;
-  uint32_t tile = 0;
+  uint32_t n = 0;
   for (uint32_t seg = 0; walk.next(p, s); ++seg) {
-    const float* factor = sm.factor[seg & 1u];
-    const int* limit = sm.limit[seg & 1u];
-    float l[kC];
+    const float* factor = sm.factor[seg & 3u] + first_col;
+    const int* limit = sm.limit[seg & 3u] + first_col;
+    const uint32_t n0 = n;
+    bool begun = false;  // the group has had a tile of this segment
+    float l[kCg];
 #pragma unroll
-    for (int c = 0; c < kC; ++c) l[c] = 0.f;
+    for (int c = 0; c < kCg; ++c) l[c] = 0.f;
     const int nt = s.tiles();
-    for (int t = 0; t < nt; ++t, ++tile) {
+    for (int t = 0; t < nt; ++t, ++n) {
       at.step();  // V's slot
+      if (kByTiles && (int)(n & 1u) != group) {
+        at.step();
+        continue;
+      }
       const int cnt = s.tile_units(t);
+      const uint32_t buf = n & 1u, phase = (n >> 1) & 1u;
       // this thread's key; one that the tile does not have is behind everybody's last one
       const int at_key = (key >> 4) < cnt ? (s.j0 + t * kQuUnits) * kQuUnit + key : 0x7fffffff;
       const float k_unit = next_k, v_unit = next_v;
       scales.step(a, p, key, head, next_k, next_v);
       const bool there = v_unit >= 0.f;
       const float v_log = there ? __log2f(v_unit) : 0.f;
-      const bool ok = um_wait(&sm.s_full, tile & 1u, &sm.abort_flag, p.status);
+      const bool ok = um_wait(&sm.s_full[buf], phase, &sm.abort_flag, p.status);
       tc_fence_after_sync();
-      float sc[kC];
+      float sc[kCg];
       {
         float x[kSRead][8];
 #pragma unroll
-        for (int i = 0; i < kSRead; ++i) tmem_ld8(tmem + 8 * i, x[i]);
+        for (int i = 0; i < kSRead; ++i) tmem_ld8(tmem + buf * L::kNS + region * L::kSRegion + 8 * i, x[i]);
         tmem_ld_wait();
 #pragma unroll
         for (int i = 0; i < kSRead; ++i) tmem_loaded(x[i]);
 #pragma unroll
-        for (int c = 0; c < kC; ++c) {
-          float y = x[((L::kQTerms - 1) * kC + c) / 8][((L::kQTerms - 1) * kC + c) % 8];
+        for (int c = 0; c < kCg; ++c) {
+          float y = x[((L::kQTerms - 1) * kCg + c) / 8][((L::kQTerms - 1) * kCg + c) % 8];
 #pragma unroll
-          for (int j = L::kQTerms - 2; j >= 0; --j) y = fmaf(y, 0.0625f, x[(j * kC + c) / 8][(j * kC + c) % 8]);
+          for (int j = L::kQTerms - 2; j >= 0; --j) y = fmaf(y, 0.0625f, x[(j * kCg + c) / 8][(j * kCg + c) % 8]);
           sc[c] = there && at_key < limit[c] ? y * (factor[c] * k_unit) : -INFINITY;
         }
       }
-      bool above = false;
-      if (t > 0) {
+      bool above = !begun;
+      if (begun) {
 #pragma unroll
-        for (int c = 0; c < kC; ++c) above |= sc[c] > sm.m[c] + kQuSlack || sc[c] + v_log > sm.mv[c] + kQuSlack;
+        for (int c = 0; c < kCg; ++c) above |= sc[c] > gm[c] + kQuSlack || sc[c] + v_log > gmv[c] + kQuSlack;
       }
-      if (qu_meet_any(!ok || t == 0 || above)) {
+      if (qu_meet_any<128>(bar, !ok || above)) {
         // the first tile, or rarely a later one: the tile's maxima; what has been summed so far is brought to the new references
 #pragma unroll
-        for (int c = 0; c < kC; ++c) {
+        for (int c = 0; c < kCg; ++c) {
           const float x = qu_warp_max(sc[c]), y = qu_warp_max(sc[c] + v_log);
           if (lane == 0) {
-            sm.red[warp][c] = x;
-            sm.red_v[warp][c] = y;
+            sm.red[group][warp][c] = x;
+            sm.red_v[group][warp][c] = y;
           }
         }
-        if (qu_meet_any(!ok)) return;
-        if (key < kC) {
-          const float x = fmaxf(fmaxf(sm.red[0][key], sm.red[1][key]), fmaxf(sm.red[2][key], sm.red[3][key]));
-          const float y = fmaxf(fmaxf(sm.red_v[0][key], sm.red_v[1][key]), fmaxf(sm.red_v[2][key], sm.red_v[3][key]));
-          const float old = t == 0 ? kQuNone : sm.m[key], old_v = t == 0 ? kQuNone : sm.mv[key];
-          const float now = fmaxf(old, x), now_v = fmaxf(old_v, y);
-          sm.f[key] = ex2_approx(old - now);
-          sm.fv[key] = ex2_approx(old_v - now_v);
-          sm.m[key] = now;
-          sm.mv[key] = now_v;
+        if (qu_meet_any<128>(bar, !ok)) return give_up();
+        if (key < kCg) {
+          const float x = fmaxf(fmaxf(sm.red[group][0][key], sm.red[group][1][key]), fmaxf(sm.red[group][2][key], sm.red[group][3][key]));
+          const float y = fmaxf(fmaxf(sm.red_v[group][0][key], sm.red_v[group][1][key]), fmaxf(sm.red_v[group][2][key], sm.red_v[group][3][key]));
+          const float old = begun ? gm[key] : kQuNone, old_v = begun ? gmv[key] : kQuNone;
+          // (a column whose scores stay under its reference keeps it)
+          const float now = !begun || x > old + kQuSlack ? fmaxf(old, x + kQuHead) : old;
+          const float now_v = !begun || y > old_v + kQuSlack ? fmaxf(old_v, y + kQuHead) : old_v;
+          sm.f[group][key] = ex2_approx(old - now);
+          sm.fv[group][key] = ex2_approx(old_v - now_v);
+          gm[key] = now;
+          gmv[key] = now_v;
         }
-        qu_meet_any(false);
-        if (t > 0) {  // (the weighted sums so far are complete: S of this tile was issued behind them)
+        qu_meet_any<128>(bar, false);
+        if (begun) {
+          // the sums of the group's tile before have to be complete: by tiles S of this one was issued behind them
+          if (!kByTiles && qu_meet_any<128>(bar, !um_wait(&sm.pv_done[buf ^ 1u], ((n - 1) >> 1) & 1u, &sm.abort_flag, p.status))) return give_up();
+          tc_fence_after_sync();
 #pragma unroll
-          for (int c = 0; c < kC; ++c) l[c] *= sm.f[c];
-          const int sets = t < L::kSets ? t : L::kSets;
+          for (int c = 0; c < kCg; ++c) l[c] *= sm.f[group][c];
 #pragma unroll 1
-          for (int i = 0; i < sets * L::kChunks; ++i) {
+          for (int k = 0; k < L::kSets; ++k) {
+            const int since = (k - (int)(n0 & 1u) + L::kSets) % L::kSets;  // the set's first tile in this segment
+            if (since >= t || (kByTiles && (k & 1) != group)) continue;
+#pragma unroll 1
+            for (int h = 0; h < L::kChunks; ++h) {
+              float o[kORead][8];
+              const uint32_t from = tmem + L::kColO + (k * L::kChunks + h) * L::kNO + region * L::kORegion;
 #pragma unroll
-            for (int c8 = 0; c8 < kORead; ++c8) {
-              float o[8];
-              tmem_ld8(tmem + L::kColO + i * L::kNO + 8 * c8, o);
+              for (int i = 0; i < kORead; ++i) tmem_ld8(from + 8 * i, o[i]);
               tmem_ld_wait();
-              tmem_loaded(o);
 #pragma unroll
-              for (int k = 0; k < 8; ++k) o[k] *= sm.fv[(8 * c8 + k) % kC];
-              qu_tmem_st8(tmem + L::kColO + i * L::kNO + 8 * c8, o);
+              for (int i = 0; i < kORead; ++i) {
+                tmem_loaded(o[i]);
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                  if (8 * i + e < kQuPTerms * kCg) o[i][e] *= sm.fv[group][(8 * i + e) % kCg];
+                qu_tmem_st8(from + 8 * i, o[i]);
+              }
             }
           }
           tmem_st_wait();
         }
+        begun = true;
       }
-      // weights as e4m3 terms: byte term * kC + column of the key's row
+      // weights as e4m3 terms: byte term * kCg + column of the group's region of the key's row
       {
-        float r[kC];
+        float r[kCg];
 #pragma unroll
-        for (int c = 0; c < kC; ++c) {
-          l[c] += ex2_approx(sc[c] - sm.m[c]);
-          r[c] = ex2_approx(sc[c] + v_log - sm.mv[c]);
+        for (int c = 0; c < kCg; ++c) {
+          l[c] += ex2_approx(sc[c] - gm[c]);
+          r[c] = ex2_approx(sc[c] + v_log - gmv[c]);
         }
-        uint32_t bytes[(kQuPTerms * kC / 4 + 3) / 4 * 4];
+        uint32_t bytes[kWords];
 #pragma unroll
-        for (int i = 0; i < (kQuPTerms * kC / 4 + 3) / 4 * 4; ++i) bytes[i] = 0u;
+        for (int i = kQuPTerms * kCg / 4; i < kWords; ++i) bytes[i] = 0u;
 #pragma unroll
         for (int j = 0; j < kQuPTerms; ++j)
 #pragma unroll
-          for (int c = 0; c < kC; c += 4) {
+          for (int c = 0; c < kCg; c += 4) {
             const uint32_t x = q_pack2(r[c], r[c + 1]), y = q_pack2(r[c + 2], r[c + 3]);
-            bytes[(j * kC + c) / 4] = x | y << 16;
+            bytes[(j * kCg + c) / 4] = x | y << 16;
             if (j + 1 < kQuPTerms) {
               const float2 b0 = q_float2(q_half2(x)), b1 = q_float2(q_half2(y));
               r[c] = (r[c] - b0.x) * 16.f;
@@ -411,13 +499,14 @@ __device__ __forceinline__ void qu_softmax_warps(QuSmem<T, kDim, kC>& sm, const 
               r[c + 3] = (r[c + 3] - b1.y) * 16.f;
             }
           }
+        const uint32_t w_row = smem_u32(sm.w[buf]) + key * 128;
 #pragma unroll
-        for (int i = 0; i < (kQuPTerms * kC / 4 + 3) / 4; ++i)
-          qu_sts4(w_row + ((i ^ (key & 7)) << 4), bytes[4 * i], bytes[4 * i + 1], bytes[4 * i + 2], bytes[4 * i + 3]);
+        for (int i = 0; i < kWords / 4; ++i)
+          qu_sts4(w_row + (((region * (kWords / 4) + i) ^ (key & 7)) << 4), bytes[4 * i], bytes[4 * i + 1], bytes[4 * i + 2], bytes[4 * i + 3]);
       }
       // V rows of keys that are not there weigh nothing, but may hold anything: 0 x NaN is not 0
-      if (t == nt - 1 && ((cnt & 1) || (s.j0 + s.n == s.nb && (s.len & (kQuUnit - 1))))) {
-        if (qu_meet_any(!um_wait(&sm.full[at.at], at.phase, &sm.abort_flag, p.status))) return;
+      if (t == nt - 1 && (kByTiles || group == 0) && ((cnt & 1) || (s.j0 + s.n == s.nb && (s.len & (kQuUnit - 1))))) {
+        if (qu_meet_any<128>(bar, !um_wait(&sm.full[at.at], at.phase, &sm.abort_flag, p.status))) return give_up();
         if (key < ((cnt + 1) / 2) * 32 && (at_key == 0x7fffffff || at_key >= s.len)) {
           const uint32_t v_row = smem_u32(sm.slot[at.at]) + (key >> 3) * (8 * kDim) + (key & 7) * 128;
 #pragma unroll
@@ -426,64 +515,76 @@ __device__ __forceinline__ void qu_softmax_warps(QuSmem<T, kDim, kC>& sm, const 
       }
       fence_proxy_async_smem();
       tc_fence_before_sync();
-      mbar_arrive(smem_u32(&sm.p_full));
+      mbar_arrive(smem_u32(&sm.p_full[buf]));
       at.step();
     }
     // ---- end of the segment: sums over the keys, then the output or the partial
 #pragma unroll
-    for (int c = 0; c < kC; ++c) {
+    for (int c = 0; c < kCg; ++c) {
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) l[c] += __shfl_xor_sync(kFullMask, l[c], o);
-      if (lane == 0) sm.red[warp][c] = l[c];
+      if (lane == 0) sm.red[group][warp][c] = l[c];
     }
-    if (qu_meet_any(!um_wait(&sm.o_full, seg & 1u, &sm.abort_flag, p.status))) return;
+    if (!begun && key < kCg) gm[key] = gmv[key] = kQuNone;
+    if (qu_meet_any<256>(3, !um_wait(&sm.o_full, seg & 1u, &sm.abort_flag, p.status))) return;
     const bool final_row = s.whole();
     const long long slot = (long long)partial_slot(range, s.j0 == 0) * a.hcts + hct;
-    if (key < kC) {
-      const float sum = (sm.red[0][key] + sm.red[1][key]) + (sm.red[2][key] + sm.red[3][key]);
-      const float up = ex2_approx(sm.mv[key] - sm.m[key]);
-      sm.f[key] = sum == 0.f ? 0.f : final_row ? up / sum : up;
-      if (!final_row) *reinterpret_cast<float2*>(a.part_ml + (slot * kC + key) * 2) = make_float2(sm.m[key], sum);
+    const int tid = group * 128 + key;
+    if (tid < L::kC) {
+      auto sum_of = [&](int g, int c) { return (sm.red[g][0][c] + sm.red[g][1][c]) + (sm.red[g][2][c] + sm.red[g][3][c]); };
+      if constexpr (kByTiles) {
+        const float s0 = sum_of(0, tid), s1 = sum_of(1, tid), top = fmaxf(sm.m[0][tid], sm.m[1][tid]);
+        const float sum = s0 * ex2_approx(sm.m[0][tid] - top) + s1 * ex2_approx(sm.m[1][tid] - top);
+        const float f = sum == 0.f ? 0.f : final_row ? 1.f / sum : 1.f;
+        sm.out_f[0][tid] = s0 == 0.f ? 0.f : f * ex2_approx(sm.mv[0][tid] - top);
+        sm.out_f[1][tid] = s1 == 0.f ? 0.f : f * ex2_approx(sm.mv[1][tid] - top);
+        if (!final_row) *reinterpret_cast<float2*>(a.part_ml + (slot * L::kC + tid) * 2) = make_float2(top, sum);
+      } else {
+        const int g = tid / kCg, c = tid % kCg;
+        const float sum = sum_of(g, c);
+        sm.out_f[0][tid] = sum == 0.f ? 0.f : ex2_approx(sm.mv[g][c] - sm.m[g][c]) * (final_row ? 1.f / sum : 1.f);
+        if (!final_row) *reinterpret_cast<float2*>(a.part_ml + (slot * L::kC + tid) * 2) = make_float2(sm.m[g][c], sum);
+      }
     }
-    qu_meet_any(false);
+    qu_meet_any<256>(3, false);
     tc_fence_after_sync();
-    const int sets = nt < L::kSets ? nt : L::kSets;
-    const int columns = min(a.columns - ct * kC, kC);
+    const int columns = min(a.columns - ct * L::kC, L::kC);
     const long long token = a.query_start_loc ? (long long)a.query_start_loc[s.b] : (long long)s.b * a.width;
+    // head_dim 256: a group a chunk of the dims; 128: half of the columns
+    const int h = L::kChunks == 2 ? group : 0;
 #pragma unroll 1
-    for (int h = 0; h < L::kChunks; ++h) {
-      float y[kC];
+    for (int r = 0; r < L::kRegions; ++r) {
+      if (L::kChunks == 1 && L::kRegions == 2 && r != group) continue;
+      float y[kCg];
 #pragma unroll
-      for (int c = 0; c < kC; ++c) y[c] = 0.f;
+      for (int c = 0; c < kCg; ++c) y[c] = 0.f;
 #pragma unroll 1
-      for (int k = 0; k < sets; ++k) {
-        float part[kC];  // high terms last: small numbers are added first
+      for (int k = 0; k < L::kSets; ++k) {
+        if ((k - (int)(n0 & 1u) + L::kSets) % L::kSets >= nt) continue;  // no tile of this segment
+        float o[kORead][8], part[kCg];  // high terms last: small numbers are added first
+        const uint32_t from = tmem + L::kColO + (k * L::kChunks + h) * L::kNO + r * L::kORegion;
 #pragma unroll
-        for (int c = 0; c < kC; ++c) part[c] = 0.f;
+        for (int i = 0; i < kORead; ++i) tmem_ld8(from + 8 * i, o[i]);
+        tmem_ld_wait();
 #pragma unroll
-        for (int i = kORead - 1; i >= 0; --i) {
-          float o[8];
-          tmem_ld8(tmem + L::kColO + (k * L::kChunks + h) * L::kNO + 8 * i, o);
-          tmem_ld_wait();
-          tmem_loaded(o);
+        for (int i = 0; i < kORead; ++i) tmem_loaded(o[i]);
 #pragma unroll
-          for (int e = 7; e >= 0; --e) {
-            const int n = 8 * i + e;
-            if (n < kQuPTerms * kC) part[n % kC] = fmaf(part[n % kC], 0.0625f, o[e]);
-          }
+        for (int c = 0; c < kCg; ++c) {
+          part[c] = o[((kQuPTerms - 1) * kCg + c) / 8][((kQuPTerms - 1) * kCg + c) % 8];
+#pragma unroll
+          for (int j = kQuPTerms - 2; j >= 0; --j) part[c] = fmaf(part[c], 0.0625f, o[(j * kCg + c) / 8][(j * kCg + c) % 8]);
+          const float f = sm.out_f[kByTiles ? k & 1 : 0][r * kCg + c];
+          if (!(f == 0.f)) y[c] = fmaf(part[c], f, y[c]);
         }
-#pragma unroll
-        for (int c = 0; c < kC; ++c) y[c] += part[c];
       }
 #pragma unroll
-      for (int c = 0; c < kC; ++c) {
-        if (c < columns) {
-          const int at_col = ct * kC + c;
-          float* to = final_row ? a.out + ((token + at_col / a.groups) * a.num_q_heads + head * a.groups + at_col % a.groups) * kDim
-                                : a.part_acc + (slot * kC + c) * kDim;
-          const float f = sm.f[c];
-          to[h * 128 + key] = f == 0.f ? 0.f : y[c] * f;
-        }
+      for (int c = 0; c < kCg; ++c) {
+        const int col = r * kCg + c;
+        if (col >= columns || (L::kChunks == 1 && L::kRegions == 1 && c / (kCg / 2) != group)) continue;
+        const int at_col = ct * L::kC + col;
+        float* to = final_row ? a.out + ((token + at_col / a.groups) * a.num_q_heads + head * a.groups + at_col % a.groups) * kDim
+                              : a.part_acc + (slot * L::kC + col) * kDim;
+        to[h * 128 + key] = y[c];
       }
     }
     tc_fence_before_sync();  // the next segment's first weighted sums overwrite what was just read
@@ -491,23 +592,22 @@ __device__ __forceinline__ void qu_softmax_warps(QuSmem<T, kDim, kC>& sm, const 
   }
 }
 
-// ---- warps 6 and 7: a segment's queries as e4m3 terms -------------------------------------------------------------------------
-template <typename T, int kDim, int kC>
-__device__ __forceinline__ void qu_query_warps(QuSmem<T, kDim, kC>& sm, const QuParams& a, const DecodeParams& p, int head, int ct, QuWalk walk, int tid) {
-  using L = QuLayout<T, kDim, kC>;
-  constexpr int kFly = kC / 2 < 4 ? kC / 2 : 4;  // columns of a warp in flight
+// ---- warps 10 and 11: a segment's queries as e4m3 terms -----------------------------------------------------------------------
+template <class L, typename T, int kCg>
+__device__ __forceinline__ void qu_query_warps(QuSmem<L>& sm, const QuParams& a, const DecodeParams& p, int head, int ct, QuWalk walk, int tid) {
+  constexpr int kDim = L::kChunks * 128, kFly = L::kC / 2 < 4 ? L::kC / 2 : 4;  // columns of a warp in flight
   const int half = tid >> 5, lane = tid & 31;
   const int d = 8 * lane;  // (head_dim 128: half of the lanes)
   QuSeg s;
   for (uint32_t seg = 0; walk.next(p, s); ++seg) {
     const long long token = a.query_start_loc ? (long long)a.query_start_loc[s.b] : (long long)s.b * a.width;
 #pragma unroll 1
-    for (int c0 = 0; c0 < kC; c0 += 2 * kFly) {
+    for (int c0 = 0; c0 < L::kC; c0 += 2 * kFly) {
       float x[kFly][8];
       int limit[kFly];
 #pragma unroll
       for (int i = 0; i < kFly; ++i) {
-        const int at = ct * kC + c0 + 2 * i + half;
+        const int at = ct * L::kC + c0 + 2 * i + half;
         limit[i] = 0;
 #pragma unroll
         for (int k = 0; k < 8; ++k) x[i][k] = 0.f;
@@ -518,7 +618,8 @@ __device__ __forceinline__ void qu_query_warps(QuSmem<T, kDim, kC>& sm, const Qu
           limit[i] = last < s.len ? last + 1 : s.len;
         }
       }
-      if (c0 == 0 && seg > 0 && !um_wait(&sm.q_free, (seg - 1) & 1u, &sm.abort_flag, p.status)) return;
+      // the scores of the segment two before have been computed
+      if (c0 == 0 && seg > 1 && !um_wait(&sm.q_free[seg & 1u], ((seg >> 1) - 1) & 1u, &sm.abort_flag, p.status)) return;
 #pragma unroll
       for (int i = 0; i < kFly; ++i) {
         const int c = c0 + 2 * i + half;
@@ -534,8 +635,8 @@ __device__ __forceinline__ void qu_query_warps(QuSmem<T, kDim, kC>& sm, const Qu
         }
         odd = __any_sync(kFullMask, odd);
         if (lane == 0) {
-          sm.factor[seg & 1u][c] = odd ? __int_as_float(0x7fffffff) : q_pow2(e) * a.scale_log2;
-          sm.limit[seg & 1u][c] = limit[i];
+          sm.factor[seg & 3u][c] = odd ? __int_as_float(0x7fffffff) : q_pow2(e) * a.scale_log2;
+          sm.limit[seg & 3u][c] = limit[i];
         }
 #pragma unroll
         for (int j = 0; j < L::kQTerms; ++j) {
@@ -547,24 +648,24 @@ __device__ __forceinline__ void qu_query_warps(QuSmem<T, kDim, kC>& sm, const Qu
             x[i][2 * k] = (x[i][2 * k] - y.x) * 16.f;
             x[i][2 * k + 1] = (x[i][2 * k + 1] - y.y) * 16.f;
           }
-          const int row = j * kC + c;
+          const int row = c / kCg * L::kSRegion + j * kCg + c % kCg;
           if (d < kDim)
-            *reinterpret_cast<uint2*>(sm.q[d / 128] + row * 128 + (((d % 128 / 16) ^ (row & 7)) << 4) + (d & 8)) =
+            *reinterpret_cast<uint2*>(sm.q[seg & 1u][d / 128] + row * 128 + (((d % 128 / 16) ^ (row & 7)) << 4) + (d & 8)) =
                 make_uint2(b[0] | b[1] << 16, b[2] | b[3] << 16);
         }
       }
     }
     fence_proxy_async_smem();
-    mbar_arrive(smem_u32(&sm.q_full));
+    mbar_arrive(smem_u32(&sm.q_full[seg & 1u]));
   }
 }
 
-template <typename T, int kDim, int kC>
-__global__ void __launch_bounds__(kDecodeThreads, 1)
+template <typename T, int kDim, int kCg, bool kByTiles>
+__global__ void __launch_bounds__(kQuThreads, 1)
 quantized_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const QuParams a, const DecodeParams p) {
-  using L = QuLayout<T, kDim, kC>;
+  using L = QuLayout<T, kDim, kCg, kByTiles>;
   extern __shared__ unsigned char qu_smem_raw[];
-  QuSmem<T, kDim, kC>& sm = *reinterpret_cast<QuSmem<T, kDim, kC>*>((reinterpret_cast<uintptr_t>(qu_smem_raw) + 1023) & ~(uintptr_t)1023);
+  QuSmem<L>& sm = *reinterpret_cast<QuSmem<L>*>((reinterpret_cast<uintptr_t>(qu_smem_raw) + 1023) & ~(uintptr_t)1023);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int hct = blockIdx.x % a.hcts, range = blockIdx.x / a.hcts, ranges = gridDim.x / a.hcts;
   const int head = hct / a.column_tiles, ct = hct % a.column_tiles;
@@ -577,23 +678,29 @@ quantized_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
       mbar_init(smem_u32(&sm.full[i]), 1);
       mbar_init(smem_u32(&sm.empty[i]), 1);
     }
-    mbar_init(smem_u32(&sm.q_full), 64);
-    mbar_init(smem_u32(&sm.q_free), 1);
-    mbar_init(smem_u32(&sm.s_full), 1);
-    mbar_init(smem_u32(&sm.p_full), 128);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&sm.q_full[i]), 64);
+      mbar_init(smem_u32(&sm.q_free[i]), 1);
+      mbar_init(smem_u32(&sm.s_full[i]), 1);
+      mbar_init(smem_u32(&sm.p_full[i]), kByTiles ? 128 : 256);
+      mbar_init(smem_u32(&sm.pv_done[i]), 1);
+    }
     mbar_init(smem_u32(&sm.o_full), 1);
-    mbar_init(smem_u32(&sm.o_free), 128);
+    mbar_init(smem_u32(&sm.o_free), 256);
     mbar_fence_init();
   }
+  // (rows of the query terms that no column fills: finite, and never read)
+  for (int i = threadIdx.x; i < (int)sizeof(sm.q) / 16; i += kQuThreads) reinterpret_cast<uint4*>(sm.q)[i] = make_uint4(0, 0, 0, 0);
+  fence_proxy_async_smem();
   pdl_wait();
   {  // this CTA's share of the block tables into the L2, while the lengths are on their way
     const long long lines = ((long long)p.batch * p.table_width * (long long)sizeof(int32_t) + 127) / 128;
-    const long long line = (long long)blockIdx.x * kDecodeThreads + threadIdx.x;
+    const long long line = (long long)blockIdx.x * kQuThreads + threadIdx.x;
     if (line < lines) asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const char*>(p.block_tables) + line * 128));
   }
   // ---- pass 1: total number of units; zero the output of rows without keys
   int mine = 0, first_n = 0;
-  for (int base = 0; base < p.batch; base += kDecodeThreads) {
+  for (int base = 0; base < p.batch; base += kQuThreads) {
     const int b = base + threadIdx.x;
     int len = 0;
     if (b < p.batch) len = decode_row_len(p, b);
@@ -605,16 +712,16 @@ quantized_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
     for (unsigned todo = __ballot_sync(kFullMask, ours); todo; todo &= todo - 1) {
       const int bb = base + (warp << 5) + (__ffs(todo) - 1);
       const long long token = a.query_start_loc ? (long long)a.query_start_loc[bb] : (long long)bb * a.width;
-      const int columns = min(a.columns - ct * kC, kC);
+      const int columns = min(a.columns - ct * L::kC, L::kC);
       for (int i = lane; i < columns * (kDim / 4); i += 32) {
-        const int at = ct * kC + i / (kDim / 4);
+        const int at = ct * L::kC + i / (kDim / 4);
         reinterpret_cast<float4*>(a.out + ((token + at / a.groups) * a.num_q_heads + head * a.groups + at % a.groups) * kDim)[i % (kDim / 4)] =
             make_float4(0.f, 0.f, 0.f, 0.f);
       }
     }
   }
   int total = 0;
-  const int incl = cta_inclusive_scan(mine, sm.scan, total);
+  const int incl = qu_inclusive_scan(mine, sm.scan, total);
   const Partition pt = make_partition(total > 0 ? total : 1, ranges);
   const long long g0 = pt.start(range), g1 = pt.start(range + 1);
   if (total == 0 || range >= pt.n || g0 == g1) {  // nothing for this CTA
@@ -623,26 +730,23 @@ quantized_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
   }
   // ---- pass 2: locate (row, unit) of g0
   long long carry = 0;
-  if (p.batch <= kDecodeThreads) {  // one row per thread: the scan of pass 1 has the answer already
+  if (p.batch <= kQuThreads) {  // one row per thread: the scan of pass 1 has the answer already
     const long long excl = incl - first_n;
     if (first_n > 0 && excl <= g0 && g0 < excl + first_n) { sm.start_b = threadIdx.x; sm.start_j = (int)(g0 - excl); }
     carry = g0 + 1;  // skips the loop below
   }
-  for (int base = 0; base < p.batch && carry <= g0; base += kDecodeThreads) {
+  for (int base = 0; base < p.batch && carry <= g0; base += kQuThreads) {
     const int b = base + threadIdx.x;
     int n = 0;
     if (b < p.batch) n = blocks_in_sequence(p, (decode_row_len(p, b) + kBlk - 1) / kBlk);
     int chunk_total = 0;
-    const long long excl = carry + cta_inclusive_scan(n, sm.scan, chunk_total) - n;
+    const long long excl = carry + qu_inclusive_scan(n, sm.scan, chunk_total) - n;
     if (n > 0 && excl <= g0 && g0 < excl + n) { sm.start_b = b; sm.start_j = (int)(g0 - excl); }
     carry += chunk_total;
   }
-  // (rows of the query terms that no column fills: finite, and never read)
-  for (int i = threadIdx.x; i < (int)sizeof(sm.q) / 16; i += kDecodeThreads) reinterpret_cast<uint4*>(sm.q)[i] = make_uint4(0, 0, 0, 0);
-  fence_proxy_async_smem();
   __syncthreads();
   const QuWalk walk{sm.start_b, sm.start_j, g0, g1};
-  if (warp == 4) {  // tensor memory between the wait and the release (umma.cuh)
+  if (warp == 8) {  // tensor memory between the wait and the release (umma.cuh)
     tmem_alloc(smem_u32(&sm.tmem_base), 512);
     if (lane == 0) pdl_release();
   }
@@ -651,14 +755,14 @@ quantized_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
   tc_fence_after_sync();
   const uint32_t tmem = sm.tmem_base;
 
-  if (warp < 4) qu_softmax_warps<T, kDim, kC>(sm, a, p, tmem, head, hct, ct, walk, range, warp, lane);
-  else if (warp == 4) {
+  if (warp < 8) qu_softmax_warps<L, kCg, kByTiles>(sm, a, p, tmem, head, hct, ct, walk, range, warp >> 2, warp & 3, lane);
+  else if (warp == 8) {
     if (hct == 0 && lane == 0) a.cuts[range] = umma_cut(p, pt, range, walk.b, walk.j, walk.g);
     __syncwarp();
-    qu_mma_warp<T, kDim, kC>(sm, p, tmem, walk);
+    qu_mma_warp<L>(sm, p, tmem, walk);
   }
-  else if (warp == 5) qu_producer<T, kDim, kC>(&k_map, &v_map, a, p, sm, head, walk, lane);
-  else qu_query_warps<T, kDim, kC>(sm, a, p, head, ct, walk, threadIdx.x - 192);
+  else if (warp == 9) qu_producer<L>(&k_map, &v_map, p, sm, head, walk, lane);
+  else qu_query_warps<L, T, kCg>(sm, a, p, head, ct, walk, threadIdx.x - 320);
 
   tc_fence_before_sync();
   __syncthreads();
@@ -667,20 +771,20 @@ quantized_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
     while (global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
     __syncthreads();
   }
-  if (warp == 4) tmem_dealloc(tmem, 512);
+  if (warp == 8) tmem_dealloc(tmem, 512);
 }
 
-template <typename T, int kDim, int kC>
+template <typename T, int kDim, int kCg, bool kByTiles>
 static int launch_quantized_umma(const CUtensorMap& k_map, const CUtensorMap& v_map, const QuParams& a, const DecodeParams& p, int ranges,
                                  cudaStream_t stream) {
-  constexpr int bytes = (int)sizeof(QuSmem<T, kDim, kC>) + 1024;
+  constexpr int bytes = (int)sizeof(QuSmem<QuLayout<T, kDim, kCg, kByTiles>>) + 1024;
   static_assert(bytes <= 232448, "the ring exceeds the shared memory of one CTA");
-  auto* kernel = quantized_umma_kernel<T, kDim, kC>;
+  auto* kernel = quantized_umma_kernel<T, kDim, kCg, kByTiles>;
   static PerDeviceFlags ready;
   if (!once_per_device(ready, [&](int) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess; }))
     return NVJ_ERR_LAUNCH;
-  return launch_after(kernel, dim3((unsigned)(ranges * a.hcts)), dim3(kDecodeThreads), bytes, stream, k_map, v_map, a, p) == cudaSuccess ? NVJ_OK
-                                                                                                                                 : NVJ_ERR_LAUNCH;
+  return launch_after(kernel, dim3((unsigned)(ranges * a.hcts)), dim3(kQuThreads), bytes, stream, k_map, v_map, a, p) == cudaSuccess ? NVJ_OK
+                                                                                                                             : NVJ_ERR_LAUNCH;
 }
 template <typename T>
 static int launch_quantized_umma_shape(const CUtensorMap& k_map, const CUtensorMap& v_map, const QuParams& a, const DecodeParams& p, int head_dim,
@@ -688,10 +792,10 @@ static int launch_quantized_umma_shape(const CUtensorMap& k_map, const CUtensorM
   auto columns = [&](auto dim) {
     constexpr int kDim = decltype(dim)::value;
     switch (a.tile_columns) {
-      case 4: return launch_quantized_umma<T, kDim, 4>(k_map, v_map, a, p, ranges, stream);
-      case 8: return launch_quantized_umma<T, kDim, 8>(k_map, v_map, a, p, ranges, stream);
-      case 16: return launch_quantized_umma<T, kDim, 16>(k_map, v_map, a, p, ranges, stream);
-      default: return launch_quantized_umma<T, kDim, 24>(k_map, v_map, a, p, ranges, stream);
+      case 4: return launch_quantized_umma<T, kDim, 4, true>(k_map, v_map, a, p, ranges, stream);
+      case 8: return launch_quantized_umma<T, kDim, 8, true>(k_map, v_map, a, p, ranges, stream);
+      case 16: return launch_quantized_umma<T, kDim, 8, false>(k_map, v_map, a, p, ranges, stream);
+      default: return launch_quantized_umma<T, kDim, 12, false>(k_map, v_map, a, p, ranges, stream);
     }
   };
   return head_dim == 256 ? columns(std::integral_constant<int, 256>{}) : columns(std::integral_constant<int, 128>{});
