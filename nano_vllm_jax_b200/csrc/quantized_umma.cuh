@@ -80,6 +80,7 @@ struct QuSmem {
   alignas(1024) char q[2][L::kChunks][L::kQChunk];  // by segment parity: [chunk][region, term, column][128 B]
   alignas(1024) char w[2][L::kWBytes];              // by tile parity: weights' terms [key][128 B]
   alignas(8) unsigned long long full[L::kSlots], empty[L::kSlots], q_full[2], q_free[2], s_full[2], p_full[2], pv_done[2], o_full, o_free;
+  alignas(16) float k_unit[8][kQuUnits], v_unit[8][kQuUnits];  // by tile: the scales of its units' blocks; V's -1: no such block
   alignas(16) float factor[4][L::kC];  // by segment: what a column's products are multiplied by, and the keys it may see
   alignas(16) int limit[4][L::kC];
   alignas(16) float red[2][4][12], red_v[2][4][12];  // per group and warp
@@ -115,6 +116,23 @@ __device__ __forceinline__ void qu_tmem_st8(uint32_t taddr, const float (&v)[8])
 }
 __device__ __forceinline__ void qu_sts4(uint32_t at, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+// N (a multiple of 4) numbers from a 16-byte boundary in shared memory on.
+template <int N>
+__device__ __forceinline__ void qu_lds(float (&v)[N], const float* from) {
+#pragma unroll
+  for (int i = 0; i < N; i += 4) {
+    const float4 x = *reinterpret_cast<const float4*>(from + i);
+    v[i] = x.x; v[i + 1] = x.y; v[i + 2] = x.z; v[i + 3] = x.w;
+  }
+}
+template <int N>
+__device__ __forceinline__ void qu_lds(int (&v)[N], const int* from) {
+#pragma unroll
+  for (int i = 0; i < N; i += 4) {
+    const int4 x = *reinterpret_cast<const int4*>(from + i);
+    v[i] = x.x; v[i + 1] = x.y; v[i + 2] = x.z; v[i + 3] = x.w;
+  }
 }
 // Whether `mine` holds in any of the `threads` threads that meet at barrier `id`.
 template <int kThreads>
@@ -182,8 +200,8 @@ struct QuWalk {
 
 // ---- warp 9: TMA loads ------------------------------------------------------------------------------------------------------------
 template <class L>
-__device__ __forceinline__ void qu_producer(const CUtensorMap* k_map, const CUtensorMap* v_map, const DecodeParams& p, QuSmem<L>& sm, int head,
-                                            QuWalk walk, int lane) {
+__device__ __forceinline__ void qu_producer(const CUtensorMap* k_map, const CUtensorMap* v_map, const QuParams& a, const DecodeParams& p, QuSmem<L>& sm,
+                                            int head, QuWalk walk, int lane) {
   const int per_block = p.block_size / kQuUnit;
   const int oob = (int)(p.num_blocks * (p.block_size / 8));  // a box that starts here is filled with zeros
   uint64_t policy;  // every block is read once
@@ -193,6 +211,7 @@ __device__ __forceinline__ void qu_producer(const CUtensorMap* k_map, const CUte
   };
   QuRing<L::kSlots> at;
   bool reuse = false;  // the slot has been used before
+  uint32_t tile = 0;
   QuSeg s, nxt;
   bool have = walk.next(p, s);
   int ids = have ? ids_at(s, 0) : 0;
@@ -207,10 +226,27 @@ __device__ __forceinline__ void qu_producer(const CUtensorMap* k_map, const CUte
       const int group = bad || lane >= n ? oob : ids * (p.block_size / 8) + (s.j0 + i0 + lane) % per_block * 2;
       for (int i = 0; i < n; i += kQuUnits) {
         const int cnt = min(n - i, kQuUnits), mine = __shfl_sync(kFullMask, group, (i + lane) & 31);  // a lane per unit
+        const int id = __shfl_sync(kFullMask, bad ? -1 : ids, (i + lane) & 31);
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
           if (reuse && !um_wait(&sm.empty[at.at], at.phase ^ 1u, &sm.abort_flag, p.status)) return;
           const uint32_t full = smem_u32(&sm.full[at.at]), dst = smem_u32(sm.slot[at.at]) + lane * L::kUnitBytes;
+          // The scales with K, counted on its barrier: eight tiles' places, so that the ones of tile n have been read before those
+          // of tile n + 8 come.  (Fetched by the softmax threads a tile ahead, each waited ~1100 cycles per tile for them: with the
+          // memory busy an access takes longer than two tiles.)
+          if (kv == 0 && lane < cnt) {
+            float *ku = &sm.k_unit[tile & 7u][lane], *vu = &sm.v_unit[tile & 7u][lane];
+            if (id >= 0) {
+              const long long entry = (long long)id * a.num_kv_heads + head;
+              asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(ku)), "l"(a.k_scale + entry) : "memory");
+              asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(vu)), "l"(a.v_scale + entry) : "memory");
+              asm volatile("cp.async.mbarrier.arrive.shared::cta.b64 [%0];" ::"r"(full) : "memory");
+            } else {
+              *ku = 0.f;
+              *vu = -1.f;
+            }
+          }
+          __syncwarp();
           if (lane == 0) mbar_arrive_expect_tx(full, (uint32_t)cnt * L::kUnitBytes);
           __syncwarp();
           if (lane < cnt) qu_load(dst, kv == 0 ? k_map : v_map, mine, head, full, policy);
@@ -218,6 +254,7 @@ __device__ __forceinline__ void qu_producer(const CUtensorMap* k_map, const CUte
           at.step();
           if (at.at == 0) reuse = true;
         }
+        ++tile;
       }
       ids = ahead;
       if (i0 == 0) {  // the row behind this one, once the first copies are on their way
@@ -312,47 +349,6 @@ __device__ __forceinline__ void qu_mma_warp(QuSmem<L>& sm, const DecodeParams& p
   }
 }
 
-// Scales of a group's tiles, one tile ahead: thread = key.  `id` belongs to the tile behind the one whose scales were given out last.
-template <bool kByTiles>
-struct QuScales {
-  QuWalk walk;
-  QuSeg s;
-  int t;
-  bool have;
-  int id;
-
-  __device__ __forceinline__ void one_on(const DecodeParams& p) {
-    if (have && ++t == s.tiles()) {
-      t = 0;
-      have = walk.next(p, s);
-    }
-  }
-  __device__ __forceinline__ void fetch_id(const DecodeParams& p, int key) {
-    id = -1;
-    const int u = t * kQuUnits + key / kQuUnit;
-    if (have && u < s.n) id = p.block_tables[(long long)s.b * p.table_width + (s.j0 + u) / (p.block_size / kQuUnit)];
-  }
-  __device__ __forceinline__ void begin(const DecodeParams& p, const QuWalk& w, int key, int group) {
-    walk = w;
-    t = 0;
-    have = walk.next(p, s);
-    if (kByTiles && group == 1) one_on(p);
-    fetch_id(p, key);
-  }
-  // the scales of the tile whose id is here (V's -1: no key), and the id of the group's next one
-  __device__ __forceinline__ void step(const QuParams& a, const DecodeParams& p, int key, int head, float& k_unit, float& v_unit) {
-    k_unit = 0.f;
-    v_unit = -1.f;
-    if (id >= 0 && id < p.num_blocks) {
-      k_unit = a.k_scale[(long long)id * a.num_kv_heads + head];
-      v_unit = a.v_scale[(long long)id * a.num_kv_heads + head];
-    }
-    one_on(p);
-    if (kByTiles) one_on(p);
-    fetch_id(p, key);
-  }
-};
-
 // ---- warps 0 - 7: softmax and output.  Thread = key of the tile, then dim of the output ---------------------------------------
 // (A wait that runs out does so for one warp and perhaps not for the next: a group's warps leave together, behind a meeting.)
 template <class L, int kCg, bool kByTiles>
@@ -366,10 +362,6 @@ __device__ __forceinline__ void qu_softmax_warps(QuSmem<L>& sm, const QuParams& 
   auto give_up = [] { qu_meet_any<256>(3, true); };
   float(&gm)[12] = sm.m[group];
   float(&gmv)[12] = sm.mv[group];
-  QuScales<kByTiles> scales;
-  scales.begin(p, walk, key, group);
-  float next_k, next_v;
-  scales.step(a, p, key, head, next_k, next_v);
   QuRing<L::kSlots> at;
   QuSeg s;
   uint32_t n = 0;
@@ -392,33 +384,37 @@ __device__ __forceinline__ void qu_softmax_warps(QuSmem<L>& sm, const QuParams& 
       const uint32_t buf = n & 1u, phase = (n >> 1) & 1u;
       // this thread's key; one that the tile does not have is behind everybody's last one
       const int at_key = (key >> 4) < cnt ? (s.j0 + t * kQuUnits) * kQuUnit + key : 0x7fffffff;
-      const float k_unit = next_k, v_unit = next_v;
-      scales.step(a, p, key, head, next_k, next_v);
-      const bool there = v_unit >= 0.f;
-      const float v_log = there ? __log2f(v_unit) : 0.f;
       const bool ok = um_wait(&sm.s_full[buf], phase, &sm.abort_flag, p.status);
       tc_fence_after_sync();
+      const float k_unit = sm.k_unit[n & 7u][key >> 4], v_unit = sm.v_unit[n & 7u][key >> 4];
       float sc[kCg];
       {
         float x[kSRead][8];
+        const bool there = v_unit >= 0.f;
 #pragma unroll
         for (int i = 0; i < kSRead; ++i) tmem_ld8(tmem + buf * L::kNS + region * L::kSRegion + 8 * i, x[i]);
         tmem_ld_wait();
 #pragma unroll
         for (int i = 0; i < kSRead; ++i) tmem_loaded(x[i]);
+        float by[kCg];
+        int seen[kCg];
+        qu_lds(by, factor);
+        qu_lds(seen, limit);
 #pragma unroll
         for (int c = 0; c < kCg; ++c) {
           float y = x[((L::kQTerms - 1) * kCg + c) / 8][((L::kQTerms - 1) * kCg + c) % 8];
 #pragma unroll
           for (int j = L::kQTerms - 2; j >= 0; --j) y = fmaf(y, 0.0625f, x[(j * kCg + c) / 8][(j * kCg + c) % 8]);
-          sc[c] = there && at_key < limit[c] ? y * (factor[c] * k_unit) : -INFINITY;
+          sc[c] = there && at_key < seen[c] ? y * (by[c] * k_unit) : -INFINITY;
         }
       }
+      const float v_log = v_unit >= 0.f ? __log2f(v_unit) : 0.f;
+      float m[kCg], mv[kCg];
+      qu_lds(m, gm);
+      qu_lds(mv, gmv);
       bool above = !begun;
-      if (begun) {
 #pragma unroll
-        for (int c = 0; c < kCg; ++c) above |= sc[c] > gm[c] + kQuSlack || sc[c] + v_log > gmv[c] + kQuSlack;
-      }
+      for (int c = 0; c < kCg; ++c) above |= sc[c] > m[c] + kQuSlack || sc[c] + v_log > mv[c] + kQuSlack;
       if (qu_meet_any<128>(bar, !ok || above)) {
         // the first tile, or rarely a later one: the tile's maxima; what has been summed so far is brought to the new references
 #pragma unroll
@@ -443,6 +439,8 @@ __device__ __forceinline__ void qu_softmax_warps(QuSmem<L>& sm, const QuParams& 
           gmv[key] = now_v;
         }
         qu_meet_any<128>(bar, false);
+        qu_lds(m, gm);
+        qu_lds(mv, gmv);
         if (begun) {
           // the sums of the group's tile before have to be complete: by tiles S of this one was issued behind them
           if (!kByTiles && qu_meet_any<128>(bar, !um_wait(&sm.pv_done[buf ^ 1u], ((n - 1) >> 1) & 1u, &sm.abort_flag, p.status))) return give_up();
@@ -479,8 +477,8 @@ __device__ __forceinline__ void qu_softmax_warps(QuSmem<L>& sm, const QuParams& 
         float r[kCg];
 #pragma unroll
         for (int c = 0; c < kCg; ++c) {
-          l[c] += ex2_approx(sc[c] - gm[c]);
-          r[c] = ex2_approx(sc[c] + v_log - gmv[c]);
+          l[c] += ex2_approx(sc[c] - m[c]);
+          r[c] = ex2_approx(sc[c] + v_log - mv[c]);
         }
         uint32_t bytes[kWords];
 #pragma unroll
@@ -761,7 +759,7 @@ quantized_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
     __syncwarp();
     qu_mma_warp<L>(sm, p, tmem, walk);
   }
-  else if (warp == 9) qu_producer<L>(&k_map, &v_map, p, sm, head, walk, lane);
+  else if (warp == 9) qu_producer<L>(&k_map, &v_map, a, p, sm, head, walk, lane);
   else qu_query_warps<L, T, kCg>(sm, a, p, head, ct, walk, threadIdx.x - 320);
 
   tc_fence_before_sync();
