@@ -20,10 +20,10 @@
 //                 e4m3 terms into shared memory; their sum without the V scale under a reference of its own.  A reference is set 2^4 above
 //                 the largest score and moves when a score passes it by 2^8 (weights up to 2^8 <= 448).  Thread = dim when a
 //                 row's segment ends.
-//   warp 8        MMA issue: the scores of the next tile in front of the weighted sum of this one.
-//   warp 9        TMA producer: 16-key boxes [8-key group][128-byte chunk][8 keys][128 B], 128-byte swizzle, into a ring of tiles of K
-//                 and V in turn (160 KiB).
-//   warps 10, 11  the queries, up to two segments ahead: scaled to 2^7 - 2^8 by a power of two per column, split into terms.
+//   warps 8, 9    MMA issue: the scores (up to two tiles ahead), the weighted sums.
+//   warp 10       TMA producer: 16-key boxes [8-key group][128-byte chunk][8 keys][128 B], 128-byte swizzle, into rings of tiles of K
+//                 and of V (160 KiB), and with K the scales of its blocks.
+//   warp 11       the queries, up to two segments ahead: scaled to 2^7 - 2^8 by a power of two per column, split into terms.
 // Every wait is bounded; after a timeout (NVJ_DEV_TIMEOUT) the kernel stops issuing, lets copies land and frees its tensor
 // memory.  A block id outside the pool is flagged, fetched from beyond the tensor (zeros) and its keys are left out.
 #pragma once
@@ -69,17 +69,19 @@ struct QuLayout {
   static constexpr int kQBytes = kChunks * kQChunk, kWBytes = kQuTile * 128;
   static constexpr int kFit = (232448 - 1024 - 6144 - 2 * kQBytes - 2 * kWBytes) / kTileBytes;
   static constexpr int kSlots = kFit < 160 * 1024 / kTileBytes ? kFit : 160 * 1024 / kTileBytes;
+  static constexpr int kKSlots = kSlots / 2, kVSlots = kSlots - kKSlots;  // a ring of tiles of K, one of V (which waits for its weights)
   static_assert(kNO <= 128 && kNS <= 256, "a row of weights is 128 bytes");
   static_assert(kColO + kSets * kChunks * kNO <= 512, "tensor memory");
-  static_assert(kSlots >= 3, "a tile of K and of V, and one on its way");
+  static_assert(kKSlots >= 1 && kVSlots >= 2, "the rings");
 };
 
 template <class L>
 struct QuSmem {
-  alignas(1024) char slot[L::kSlots][L::kTileBytes];
+  alignas(1024) char k[L::kKSlots][L::kTileBytes];
+  alignas(1024) char v[L::kVSlots][L::kTileBytes];
   alignas(1024) char q[2][L::kChunks][L::kQChunk];  // by segment parity: [chunk][region, term, column][128 B]
   alignas(1024) char w[2][L::kWBytes];              // by tile parity: weights' terms [key][128 B]
-  alignas(8) unsigned long long full[L::kSlots], empty[L::kSlots], q_full[2], q_free[2], s_full[2], p_full[2], pv_done[2], o_full, o_free;
+  alignas(8) unsigned long long k_full[L::kKSlots], k_empty[L::kKSlots], v_full[L::kVSlots], v_empty[L::kVSlots], q_full[2], q_free[2], s_full[2], p_full[2], pv_done[2], o_full, o_free;
   alignas(16) float k_unit[8][kQuUnits], v_unit[8][kQuUnits];  // by tile: the scales of its units' blocks; V's -1: no such block
   alignas(16) float factor[4][L::kC];  // by segment: what a column's products are multiplied by, and the keys it may see
   alignas(16) int limit[4][L::kC];
@@ -171,13 +173,15 @@ __device__ __forceinline__ int qu_inclusive_scan(int v, int* warp_sums, int& tot
   return v + before;
 }
 
-// A place in the ring: K and V of a tile follow one another.
+// A place in a ring.  (K and V have rings of their own: the barriers of a ring have to be waited on in the order of its uses, and the two
+// products are issued by a warp each.)
 template <int kSlots>
 struct QuRing {
   int at = 0;
   uint32_t phase = 0;
+  bool reuse = false;  // the place has been used before
   __device__ __forceinline__ void step() {
-    if (++at == kSlots) { at = 0; phase ^= 1u; }
+    if (++at == kSlots) { at = 0; phase ^= 1u; reuse = true; }
   }
 };
 // The CTA's segments: 16-key units [j0, j0 + n) of row b, which has nb of them and len keys.
@@ -198,7 +202,7 @@ struct QuWalk {
   }
 };
 
-// ---- warp 9: TMA loads ------------------------------------------------------------------------------------------------------------
+// ---- warp 10: TMA loads ------------------------------------------------------------------------------------------------------------
 template <class L>
 __device__ __forceinline__ void qu_producer(const CUtensorMap* k_map, const CUtensorMap* v_map, const QuParams& a, const DecodeParams& p, QuSmem<L>& sm,
                                             int head, QuWalk walk, int lane) {
@@ -209,8 +213,8 @@ __device__ __forceinline__ void qu_producer(const CUtensorMap* k_map, const CUte
   auto ids_at = [&](const QuSeg& s, int i) {
     return i + lane < s.n ? p.block_tables[(long long)s.b * p.table_width + (s.j0 + i + lane) / per_block] : 0;
   };
-  QuRing<L::kSlots> at;
-  bool reuse = false;  // the slot has been used before
+  QuRing<L::kKSlots> k_at;
+  QuRing<L::kVSlots> v_at;
   uint32_t tile = 0;
   QuSeg s, nxt;
   bool have = walk.next(p, s);
@@ -227,14 +231,13 @@ __device__ __forceinline__ void qu_producer(const CUtensorMap* k_map, const CUte
       for (int i = 0; i < n; i += kQuUnits) {
         const int cnt = min(n - i, kQuUnits), mine = __shfl_sync(kFullMask, group, (i + lane) & 31);  // a lane per unit
         const int id = __shfl_sync(kFullMask, bad ? -1 : ids, (i + lane) & 31);
-#pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-          if (reuse && !um_wait(&sm.empty[at.at], at.phase ^ 1u, &sm.abort_flag, p.status)) return;
-          const uint32_t full = smem_u32(&sm.full[at.at]), dst = smem_u32(sm.slot[at.at]) + lane * L::kUnitBytes;
+        {
+          if (k_at.reuse && !um_wait(&sm.k_empty[k_at.at], k_at.phase ^ 1u, &sm.abort_flag, p.status)) return;
+          const uint32_t full = smem_u32(&sm.k_full[k_at.at]);
           // The scales with K, counted on its barrier: eight tiles' places, so that the ones of tile n have been read before those
           // of tile n + 8 come.  (Fetched by the softmax threads a tile ahead, each waited ~1100 cycles per tile for them: with the
           // memory busy an access takes longer than two tiles.)
-          if (kv == 0 && lane < cnt) {
+          if (lane < cnt) {
             float *ku = &sm.k_unit[tile & 7u][lane], *vu = &sm.v_unit[tile & 7u][lane];
             if (id >= 0) {
               const long long entry = (long long)id * a.num_kv_heads + head;
@@ -249,10 +252,18 @@ __device__ __forceinline__ void qu_producer(const CUtensorMap* k_map, const CUte
           __syncwarp();
           if (lane == 0) mbar_arrive_expect_tx(full, (uint32_t)cnt * L::kUnitBytes);
           __syncwarp();
-          if (lane < cnt) qu_load(dst, kv == 0 ? k_map : v_map, mine, head, full, policy);
+          if (lane < cnt) qu_load(smem_u32(sm.k[k_at.at]) + lane * L::kUnitBytes, k_map, mine, head, full, policy);
           __syncwarp();
-          at.step();
-          if (at.at == 0) reuse = true;
+          k_at.step();
+        }
+        {
+          if (v_at.reuse && !um_wait(&sm.v_empty[v_at.at], v_at.phase ^ 1u, &sm.abort_flag, p.status)) return;
+          const uint32_t full = smem_u32(&sm.v_full[v_at.at]);
+          if (lane == 0) mbar_arrive_expect_tx(full, (uint32_t)cnt * L::kUnitBytes);
+          __syncwarp();
+          if (lane < cnt) qu_load(smem_u32(sm.v[v_at.at]) + lane * L::kUnitBytes, v_map, mine, head, full, policy);
+          __syncwarp();
+          v_at.step();
         }
         ++tile;
       }
@@ -268,62 +279,54 @@ __device__ __forceinline__ void qu_producer(const CUtensorMap* k_map, const CUte
   }
 }
 
-// ---- warp 8: MMA issue ------------------------------------------------------------------------------------------------------------
-// S(n + 1), then O += V(n)^T P(n).  S(n) is issued behind the weighted sum of tile n - 2, which has waited for its weights: the scores
-// of tile n - 2 have been read by then, and their place is S(n)'s.
+// ---- warps 8 and 9: MMA issue -------------------------------------------------------------------------------------------------
+// A warp for either product: a tile's ~ 500 cycles of waits, descriptors and commits on each side would otherwise add up to more than its
+// bytes take (head_dim 128).  S(n) takes the place of S(n - 2), which has been read when that tile's weights are there.
 template <class L>
-__device__ __forceinline__ void qu_mma_warp(QuSmem<L>& sm, const DecodeParams& p, uint32_t tmem, QuWalk walk) {
-  constexpr uint32_t idesc_s = qu_idesc(L::kNS, false, false), idesc_o = qu_idesc(L::kNO, true, true);
-  const uint64_t k_desc0 = umma_desc(smem_u32(sm.slot[0]), 16, L::kChunks * 1024);    // keys are rows: groups of 8
-  const uint64_t v_desc0 = umma_desc(smem_u32(sm.slot[0]), 1024, L::kChunks * 1024);  // dims are rows, a chunk at a time; keys in groups of 8
+__device__ __forceinline__ void qu_scores_warp(QuSmem<L>& sm, const DecodeParams& p, uint32_t tmem, QuWalk walk) {
+  constexpr uint32_t idesc = qu_idesc(L::kNS, false, false);
+  const uint64_t k_desc0 = umma_desc(smem_u32(sm.k[0]), 16, L::kChunks * 1024);  // keys are rows: groups of 8
   const uint64_t q_desc0 = umma_desc(smem_u32(sm.q[0][0]), 16, 1024);
-  const uint64_t w_desc0 = umma_desc(smem_u32(sm.w[0]), 1024, 1024);
-  QuWalk ahead = walk;  // of the scores
-  QuSeg sa, s;
-  QuRing<L::kSlots> k_at, v_at;  // K slots and V slots: every other place of the ring, from 0 and from 1
-  v_at.step();
-  int ta = 0;
-  uint32_t na = 0, seg_a = 0;
-  bool more = ahead.next(p, sa);
-  auto scores = [&]() -> bool {  // of the next tile, if there is one
-    if (!more) return true;
-    const uint32_t qb = seg_a & 1u;
-    if (ta == 0 && !um_wait(&sm.q_full[qb], (seg_a >> 1) & 1u, &sm.abort_flag, p.status)) return false;
-    if (!um_wait(&sm.full[k_at.at], k_at.phase, &sm.abort_flag, p.status)) return false;
-    tc_fence_after_sync();
-    const bool last = ta == sa.tiles() - 1;
-    if (um_elect_one()) {
-      // (rows of keys that the tile does not have are computed from whatever lies there, and masked)
-      const uint64_t k_desc = k_desc0 + (uint64_t)((k_at.at * L::kTileBytes) >> 4), q_desc = q_desc0 + (uint64_t)((qb * L::kQBytes) >> 4);
+  QuRing<L::kKSlots> at;
+  QuSeg s;
+  uint32_t n = 0;
+  for (uint32_t seg = 0; walk.next(p, s); ++seg) {
+    const uint32_t qb = seg & 1u;
+    const int nt = s.tiles();
+    for (int t = 0; t < nt; ++t, ++n) {
+      if (t == 0 && !um_wait(&sm.q_full[qb], (seg >> 1) & 1u, &sm.abort_flag, p.status)) return;
+      if (!um_wait(&sm.k_full[at.at], at.phase, &sm.abort_flag, p.status)) return;
+      if (n >= 2 && !um_wait(&sm.p_full[n & 1u], ((n >> 1) - 1) & 1u, &sm.abort_flag, p.status)) return;
+      tc_fence_after_sync();
+      if (um_elect_one()) {
+        // (rows of keys that the tile does not have are computed from whatever lies there, and masked)
+        const uint64_t k_desc = k_desc0 + (uint64_t)((at.at * L::kTileBytes) >> 4), q_desc = q_desc0 + (uint64_t)((qb * L::kQBytes) >> 4);
 #pragma unroll
-      for (int ks = 0; ks < L::kChunks * 4; ++ks)
-        qu_mma(tmem + (na & 1u) * L::kNS, k_desc + (uint64_t)(((ks >> 2) * 1024 + (ks & 3) * 32) >> 4),
-               q_desc + (uint64_t)(((ks >> 2) * L::kQChunk + (ks & 3) * 32) >> 4), idesc_s, ks > 0 ? 1u : 0u);
-      umma_commit(smem_u32(&sm.s_full[na & 1u]));
-      umma_commit(smem_u32(&sm.empty[k_at.at]));
-      if (last) umma_commit(smem_u32(&sm.q_free[qb]));
+        for (int ks = 0; ks < L::kChunks * 4; ++ks)
+          qu_mma(tmem + (n & 1u) * L::kNS, k_desc + (uint64_t)(((ks >> 2) * 1024 + (ks & 3) * 32) >> 4),
+                 q_desc + (uint64_t)(((ks >> 2) * L::kQChunk + (ks & 3) * 32) >> 4), idesc, ks > 0 ? 1u : 0u);
+        umma_commit(smem_u32(&sm.s_full[n & 1u]));
+        umma_commit(smem_u32(&sm.k_empty[at.at]));
+        if (t == nt - 1) umma_commit(smem_u32(&sm.q_free[qb]));
+      }
+      __syncwarp();
+      at.step();
     }
-    __syncwarp();
-    k_at.step();
-    k_at.step();
-    ++na;
-    if (last) {
-      ta = 0;
-      ++seg_a;
-      more = ahead.next(p, sa);
-    } else {
-      ++ta;
-    }
-    return true;
-  };
-  if (!scores()) return;
+  }
+}
+template <class L>
+__device__ __forceinline__ void qu_sums_warp(QuSmem<L>& sm, const DecodeParams& p, uint32_t tmem, QuWalk walk) {
+  constexpr uint32_t idesc = qu_idesc(L::kNO, true, true);
+  const uint64_t v_desc0 = umma_desc(smem_u32(sm.v[0]), 1024, L::kChunks * 1024);  // dims are rows, a chunk at a time; keys in groups of 8
+  const uint64_t w_desc0 = umma_desc(smem_u32(sm.w[0]), 1024, 1024);
+  QuRing<L::kVSlots> at;
+  QuSeg s;
   uint32_t n = 0;
   for (uint32_t seg = 0; walk.next(p, s); ++seg) {
     const int nt = s.tiles();
     const uint32_t n0 = n;
     for (int t = 0; t < nt; ++t, ++n) {
-      if (!scores()) return;
-      if (!um_wait(&sm.full[v_at.at], v_at.phase, &sm.abort_flag, p.status)) return;
+      if (!um_wait(&sm.v_full[at.at], at.phase, &sm.abort_flag, p.status)) return;
       if (!um_wait(&sm.p_full[n & 1u], (n >> 1) & 1u, &sm.abort_flag, p.status)) return;
       // the first weighted sums of a segment overwrite O: the segment before must have been read out
       if (t == 0 && seg > 0 && !um_wait(&sm.o_free, (seg - 1) & 1u, &sm.abort_flag, p.status)) return;
@@ -331,20 +334,19 @@ __device__ __forceinline__ void qu_mma_warp(QuSmem<L>& sm, const DecodeParams& p
       if (um_elect_one()) {
         const int steps = (s.tile_units(t) + 1) / 2;
         const uint32_t o = tmem + L::kColO + ((n0 & 1u) + t) % L::kSets * (L::kChunks * L::kNO);
-        const uint64_t v_desc = v_desc0 + (uint64_t)((v_at.at * L::kTileBytes) >> 4), w_desc = w_desc0 + (uint64_t)(((n & 1u) * L::kWBytes) >> 4);
+        const uint64_t v_desc = v_desc0 + (uint64_t)((at.at * L::kTileBytes) >> 4), w_desc = w_desc0 + (uint64_t)(((n & 1u) * L::kWBytes) >> 4);
         for (int i = 0; i < steps; ++i) {  // 32 keys, four groups of 8
           const uint32_t accumulate = (t >= L::kSets || i > 0) ? 1u : 0u;
           const uint64_t wd = w_desc + (uint64_t)((i * 32 * 128) >> 4), vd = v_desc + (uint64_t)((i * 2 * L::kUnitBytes) >> 4);
 #pragma unroll
-          for (int h = 0; h < L::kChunks; ++h) qu_mma(o + h * L::kNO, vd + (uint64_t)((h * 1024) >> 4), wd, idesc_o, accumulate);
+          for (int h = 0; h < L::kChunks; ++h) qu_mma(o + h * L::kNO, vd + (uint64_t)((h * 1024) >> 4), wd, idesc, accumulate);
         }
         umma_commit(smem_u32(&sm.pv_done[n & 1u]));
-        umma_commit(smem_u32(&sm.empty[v_at.at]));
+        umma_commit(smem_u32(&sm.v_empty[at.at]));
         if (t == nt - 1) umma_commit(smem_u32(&sm.o_full));
       }
       __syncwarp();
-      v_at.step();
-      v_at.step();
+      at.step();
     }
   }
 }
@@ -362,7 +364,7 @@ __device__ __forceinline__ void qu_softmax_warps(QuSmem<L>& sm, const QuParams& 
   auto give_up = [] { qu_meet_any<256>(3, true); };
   float(&gm)[12] = sm.m[group];
   float(&gmv)[12] = sm.mv[group];
-  QuRing<L::kSlots> at;
+  QuRing<L::kVSlots> at;  // V's slot of the tile at hand
   QuSeg s;
   uint32_t n = 0;
   for (uint32_t seg = 0; walk.next(p, s); ++seg) {
@@ -375,7 +377,6 @@ __device__ __forceinline__ void qu_softmax_warps(QuSmem<L>& sm, const QuParams& 
     for (int c = 0; c < kCg; ++c) l[c] = 0.f;
     const int nt = s.tiles();
     for (int t = 0; t < nt; ++t, ++n) {
-      at.step();  // V's slot
       if (kByTiles && (int)(n & 1u) != group) {
         at.step();
         continue;
@@ -442,8 +443,9 @@ __device__ __forceinline__ void qu_softmax_warps(QuSmem<L>& sm, const QuParams& 
         qu_lds(m, gm);
         qu_lds(mv, gmv);
         if (begun) {
-          // the sums of the group's tile before have to be complete: by tiles S of this one was issued behind them
-          if (!kByTiles && qu_meet_any<128>(bar, !um_wait(&sm.pv_done[buf ^ 1u], ((n - 1) >> 1) & 1u, &sm.abort_flag, p.status))) return give_up();
+          // the group's weighted sums so far have to be complete
+          const uint32_t done = kByTiles ? n - 2 : n - 1;
+          if (qu_meet_any<128>(bar, !um_wait(&sm.pv_done[done & 1u], (done >> 1) & 1u, &sm.abort_flag, p.status))) return give_up();
           tc_fence_after_sync();
 #pragma unroll
           for (int c = 0; c < kCg; ++c) l[c] *= sm.f[group][c];
@@ -497,6 +499,8 @@ __device__ __forceinline__ void qu_softmax_warps(QuSmem<L>& sm, const QuParams& 
               r[c + 3] = (r[c + 3] - b1.y) * 16.f;
             }
           }
+        // (the weights of tile n - 2, in the same place, have been used: almost always long ago; a wait that runs out shows at the next meeting)
+        if (n >= 2) um_wait(&sm.pv_done[buf], ((n >> 1) - 1) & 1u, &sm.abort_flag, p.status);
         const uint32_t w_row = smem_u32(sm.w[buf]) + key * 128;
 #pragma unroll
         for (int i = 0; i < kWords / 4; ++i)
@@ -504,9 +508,9 @@ __device__ __forceinline__ void qu_softmax_warps(QuSmem<L>& sm, const QuParams& 
       }
       // V rows of keys that are not there weigh nothing, but may hold anything: 0 x NaN is not 0
       if (t == nt - 1 && (kByTiles || group == 0) && ((cnt & 1) || (s.j0 + s.n == s.nb && (s.len & (kQuUnit - 1))))) {
-        if (qu_meet_any<128>(bar, !um_wait(&sm.full[at.at], at.phase, &sm.abort_flag, p.status))) return give_up();
+        if (qu_meet_any<128>(bar, !um_wait(&sm.v_full[at.at], at.phase, &sm.abort_flag, p.status))) return give_up();
         if (key < ((cnt + 1) / 2) * 32 && (at_key == 0x7fffffff || at_key >= s.len)) {
-          const uint32_t v_row = smem_u32(sm.slot[at.at]) + (key >> 3) * (8 * kDim) + (key & 7) * 128;
+          const uint32_t v_row = smem_u32(sm.v[at.at]) + (key >> 3) * (8 * kDim) + (key & 7) * 128;
 #pragma unroll
           for (int i = 0; i < kDim / 16; ++i) qu_sts4(v_row + (i >> 3) * 1024 + (i & 7) * 16, 0u, 0u, 0u, 0u);
         }
@@ -590,22 +594,21 @@ __device__ __forceinline__ void qu_softmax_warps(QuSmem<L>& sm, const QuParams& 
   }
 }
 
-// ---- warps 10 and 11: a segment's queries as e4m3 terms -----------------------------------------------------------------------
+// ---- warp 11: a segment's queries as e4m3 terms -----------------------------------------------------------------------
 template <class L, typename T, int kCg>
-__device__ __forceinline__ void qu_query_warps(QuSmem<L>& sm, const QuParams& a, const DecodeParams& p, int head, int ct, QuWalk walk, int tid) {
-  constexpr int kDim = L::kChunks * 128, kFly = L::kC / 2 < 4 ? L::kC / 2 : 4;  // columns of a warp in flight
-  const int half = tid >> 5, lane = tid & 31;
+__device__ __forceinline__ void qu_query_warp(QuSmem<L>& sm, const QuParams& a, const DecodeParams& p, int head, int ct, QuWalk walk, int lane) {
+  constexpr int kDim = L::kChunks * 128, kFly = 4;  // columns in flight
   const int d = 8 * lane;  // (head_dim 128: half of the lanes)
   QuSeg s;
   for (uint32_t seg = 0; walk.next(p, s); ++seg) {
     const long long token = a.query_start_loc ? (long long)a.query_start_loc[s.b] : (long long)s.b * a.width;
 #pragma unroll 1
-    for (int c0 = 0; c0 < L::kC; c0 += 2 * kFly) {
+    for (int c0 = 0; c0 < L::kC; c0 += kFly) {
       float x[kFly][8];
       int limit[kFly];
 #pragma unroll
       for (int i = 0; i < kFly; ++i) {
-        const int at = ct * L::kC + c0 + 2 * i + half;
+        const int at = ct * L::kC + c0 + i;
         limit[i] = 0;
 #pragma unroll
         for (int k = 0; k < 8; ++k) x[i][k] = 0.f;
@@ -620,7 +623,7 @@ __device__ __forceinline__ void qu_query_warps(QuSmem<L>& sm, const QuParams& a,
       if (c0 == 0 && seg > 1 && !um_wait(&sm.q_free[seg & 1u], ((seg >> 1) - 1) & 1u, &sm.abort_flag, p.status)) return;
 #pragma unroll
       for (int i = 0; i < kFly; ++i) {
-        const int c = c0 + 2 * i + half;
+        const int c = c0 + i;
         const int bits = __reduce_max_sync(kFullMask, __float_as_int(q_largest(0.f, x[i])));
         int e = (bits >> 23) - 127 - 7;  // largest = 2^(e + 7) * [1, 2)
         e = bits == 0 ? 0 : (e < -126 ? -126 : e);
@@ -672,12 +675,16 @@ quantized_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&k_map)) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&v_map)) : "memory");
     sm.start_b = p.batch; sm.start_j = 0; sm.abort_flag = 0;
-    for (int i = 0; i < L::kSlots; ++i) {
-      mbar_init(smem_u32(&sm.full[i]), 1);
-      mbar_init(smem_u32(&sm.empty[i]), 1);
+    for (int i = 0; i < L::kKSlots; ++i) {
+      mbar_init(smem_u32(&sm.k_full[i]), 1);
+      mbar_init(smem_u32(&sm.k_empty[i]), 1);
+    }
+    for (int i = 0; i < L::kVSlots; ++i) {
+      mbar_init(smem_u32(&sm.v_full[i]), 1);
+      mbar_init(smem_u32(&sm.v_empty[i]), 1);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(smem_u32(&sm.q_full[i]), 64);
+      mbar_init(smem_u32(&sm.q_full[i]), 32);
       mbar_init(smem_u32(&sm.q_free[i]), 1);
       mbar_init(smem_u32(&sm.s_full[i]), 1);
       mbar_init(smem_u32(&sm.p_full[i]), kByTiles ? 128 : 256);
@@ -754,13 +761,14 @@ quantized_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
   const uint32_t tmem = sm.tmem_base;
 
   if (warp < 8) qu_softmax_warps<L, kCg, kByTiles>(sm, a, p, tmem, head, hct, ct, walk, range, warp >> 2, warp & 3, lane);
-  else if (warp == 8) {
+  else if (warp == 8) qu_scores_warp<L>(sm, p, tmem, walk);
+  else if (warp == 9) {
     if (hct == 0 && lane == 0) a.cuts[range] = umma_cut(p, pt, range, walk.b, walk.j, walk.g);
     __syncwarp();
-    qu_mma_warp<L>(sm, p, tmem, walk);
+    qu_sums_warp<L>(sm, p, tmem, walk);
   }
-  else if (warp == 9) qu_producer<L>(&k_map, &v_map, a, p, sm, head, walk, lane);
-  else qu_query_warps<L, T, kCg>(sm, a, p, head, ct, walk, threadIdx.x - 320);
+  else if (warp == 10) qu_producer<L>(&k_map, &v_map, a, p, sm, head, walk, lane);
+  else qu_query_warp<L, T, kCg>(sm, a, p, head, ct, walk, lane);
 
   tc_fence_before_sync();
   __syncthreads();
