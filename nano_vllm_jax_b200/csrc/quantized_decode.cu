@@ -16,7 +16,7 @@
 //     two halves of the eight columns of one mma.sync, with more they are two of them;
 //   * the K scale of a block multiplies its scores, the V scale goes into the exponent of the weights: a running maximum of
 //     its own for the weighted sum keeps blocks of any scale apart from the sum of the weights.
-// Maxima are lazy: only a score that passes its column's maximum by 2^8 (one vote per tile) rescales the sums.
+// Maxima are lazy: one vote per tile says whether a score has left them behind, and only then the sums are rescaled.
 
 #include "cluster.cuh"
 #include "decode_parts.cuh"
@@ -46,7 +46,9 @@ struct QDecodeParams {
 
 constexpr int kQdWarps = 4, kQdThreads = 32 * kQdWarps;
 constexpr float kQdNone = -3e38f;  // a maximum that no score has touched
-constexpr float kQdSlack = 8.f;    // weights may reach 2^8 before the sums are rescaled
+// The reference of the sum of weights moves when a score passes it by 2^8; that of the weighted sum is set 2^7 below the largest weight and moves
+// when one would pass 2^15: f16 ends at 65504 above and at 2^-24 below, and a key 2^10 below the largest still has 22 bits in two terms.
+constexpr float kQdSlack = 8.f, kQdLift = 7.f;
 
 // Shared memory: the queries as f16 while the tiles are walked, then each warp's sums.
 // kTiles: mma column tiles of 8.  kPack: at most four columns, the low term of the weights in columns 4 - 7.  kF32: f32 queries.
@@ -275,7 +277,7 @@ __global__ void __launch_bounds__(kQdThreads, kPack && kD == 256 ? 3 : 1) quanti
         if constexpr (kF32 && kPack) s[j][k] += __shfl_xor_sync(kFullMask, s[j][k], 2);  // the low terms' columns are two lanes away
         const int i = k & 1, key = this_tile * 16 + g + 8 * (k >> 1);
         s[j][k] = key < limit[j][i] && usable ? s[j][k] * (factor[j][i] * k_unit) : -INFINITY;
-        over |= s[j][k] > m[j][i] + kQdSlack || s[j][k] + v_log > mv[j][i] + kQdSlack;
+        over |= s[j][k] > m[j][i] + kQdSlack || s[j][k] + v_log > mv[j][i] + (kQdSlack + kQdLift);
       }
     if (__any_sync(kFullMask, over)) {
 #pragma unroll
@@ -285,7 +287,7 @@ __global__ void __launch_bounds__(kQdThreads, kPack && kD == 256 ? 3 : 1) quanti
           float top = fmaxf(s[j][i], s[j][i + 2]);
 #pragma unroll
           for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, o));
-          const float now = fmaxf(m[j][i], top), now_v = fmaxf(mv[j][i], top + v_log);
+          const float now = fmaxf(m[j][i], top), now_v = fmaxf(mv[j][i], top + v_log - kQdLift);
           l[j][i] *= ex2_approx(m[j][i] - now);
           const float f = ex2_approx(mv[j][i] - now_v);
           m[j][i] = now;
@@ -526,13 +528,15 @@ static QuEncodeTiledFn qu_encode_fn() {
   }();
   return fn;
 }
-// A layer [token, kv head, head_dim] of bytes seen as {128 dims, token of a group of 8, 128-dim chunk, group, kv head}: a box is 16 keys of
-// one kv head and lands as [group][chunk][8 keys][128 B] with the 128-byte swizzle.  `extent` = (tokens << 12) | kv heads << 1 | head_dim 256.
+// A layer [token, kv head, head_dim] of bytes seen as {128 dims, token of a group of 8, 128-dim chunk, group, kv head}: a box is 16, 32 or 64 keys
+// of one kv head and lands as [group][chunk][8 keys][128 B] with the 128-byte swizzle.  (An SM takes in ~20 B per cycle through boxes of
+// 2 KiB, 16 keys of head_dim 128, and needs 23.)  `extent` = (tokens << 14) | log2(keys / 16) << 12 | kv heads << 1 | head_dim 256.
 static bool qu_make_map(CUtensorMap* map, const void* base, uint64_t extent) {
-  const cuuint64_t tokens = extent >> 12, heads = (extent >> 1) & 0x7ff, dim = extent & 1 ? 256 : 128;
+  const cuuint32_t unit = 16u << ((extent >> 12) & 3);
+  const cuuint64_t tokens = extent >> 14, heads = (extent >> 1) & 0x7ff, dim = extent & 1 ? 256 : 128;
   const cuuint64_t dims[5] = {128, 8, dim / 128, tokens / 8, heads};
   const cuuint64_t strides[4] = {heads * dim, 128, 8 * heads * dim, dim};
-  const cuuint32_t box[5] = {128, 8, (cuuint32_t)(dim / 128), 2, 1};
+  const cuuint32_t box[5] = {128, 8, (cuuint32_t)(dim / 128), unit / 8, 1};
   const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
   return qu_encode_fn()(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 5, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -609,8 +613,8 @@ __global__ void __launch_bounds__(256) quantized_umma_fold_kernel(QuParams a, in
   }
 }
 
-// What a row's end costs a CTA, in units of 16 keys (decode_parts.cuh).
-constexpr int kQuRowEndCost = 8;
+// What a row's end costs a CTA, in keys (decode_parts.cuh).
+constexpr int kQuRowEndCost = 128;
 
 static int run_quantized_umma(const QDecodeParams& q, int q_dtype, int head_dim, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
   const int sms = decode_wide_num_ctas();
@@ -621,7 +625,8 @@ static int run_quantized_umma(const QDecodeParams& q, int q_dtype, int head_dim,
   const QuPlan w = qu_plan(columns, q.num_kv_heads, head_dim, sms);
   if (!workspace || !aligned16(workspace) || workspace_bytes < w.bytes()) return NVJ_ERR_WORKSPACE;
   CUtensorMap k_map, v_map;
-  const uint64_t extent = (uint64_t)q.num_blocks * q.block_size << 12 | (uint64_t)q.num_kv_heads << 1 | (head_dim == 256 ? 1u : 0u);
+  const int unit_log2 = q.block_size % 64 == 0 ? 6 : q.block_size % 32 == 0 ? 5 : 4;
+  const uint64_t extent = (uint64_t)q.num_blocks * q.block_size << 14 | (uint64_t)(unit_log2 - 4) << 12 | (uint64_t)q.num_kv_heads << 1 | (head_dim == 256 ? 1u : 0u);
   if (!tensor_map_cached(&k_map, kQuMapKind, q.k_cache, extent, qu_make_map) || !tensor_map_cached(&v_map, kQuMapKind, q.v_cache, extent, qu_make_map))
     return NVJ_ERR_UNSUPPORTED;
   char* at = static_cast<char*>(workspace);
@@ -640,6 +645,8 @@ static int run_quantized_umma(const QDecodeParams& q, int q_dtype, int head_dim,
   a.groups = q.groups;
   a.num_q_heads = q.groups * q.num_kv_heads;
   a.num_kv_heads = q.num_kv_heads;
+  a.unit = 1 << unit_log2;
+  a.unit_log2 = unit_log2;
   a.column_tiles = w.column_tiles;
   a.tile_columns = w.tile_columns;
   a.hcts = w.hcts;
@@ -655,7 +662,7 @@ static int run_quantized_umma(const QDecodeParams& q, int q_dtype, int head_dim,
   p.batch = q.rows;
   p.table_width = q.table_width;
   p.block_size = q.block_size;
-  p.row_end_cost = kQuRowEndCost;
+  p.row_end_cost = kQuRowEndCost >> unit_log2;
   const auto launch = q_dtype == NVJ_BF16 ? launch_quantized_umma_bf16 : q_dtype == NVJ_F16 ? launch_quantized_umma_f16 : launch_quantized_umma_f32;
   const int rc = launch(k_map, v_map, a, p, head_dim, w.ranges, stream);
   if (rc != NVJ_OK || w.ranges < 2) return rc;

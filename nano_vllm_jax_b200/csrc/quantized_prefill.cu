@@ -95,7 +95,7 @@ struct QPrefillParams {
 // The numbers of a tile are fetched into registers while the tile in front is worked on, and become f16 in shared memory: every
 // warp reads them by ldmatrix.  Scores, both references of the maxima and both terms of the weights as in the decode kernel.
 constexpr int kQpWarps = 8, kQpThreads = 32 * kQpWarps, kQpRows = 16 * kQpWarps;
-constexpr float kQpNone = -3e38f, kQpSlack = 8.f;
+constexpr float kQpNone = -3e38f, kQpSlack = 8.f, kQpLift = 7.f;  // (the references are the decode kernel's)
 
 template <typename T, int kD>
 struct QpShape {
@@ -344,7 +344,8 @@ __global__ void __launch_bounds__(kQpThreads, 1) quantized_prefill_kernel(QPrefi
         top_v[i] = fmaxf(top_v[i], x + v);
       }
     }
-    const bool over = top[0] > m[0] + kQpSlack || top[1] > m[1] + kQpSlack || top_v[0] > mv[0] + kQpSlack || top_v[1] > mv[1] + kQpSlack;
+    const bool over = top[0] > m[0] + kQpSlack || top[1] > m[1] + kQpSlack || top_v[0] > mv[0] + (kQpSlack + kQpLift) ||
+                      top_v[1] > mv[1] + (kQpSlack + kQpLift);
     if (__any_sync(kFullMask, over)) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -353,7 +354,7 @@ __global__ void __launch_bounds__(kQpThreads, 1) quantized_prefill_kernel(QPrefi
           top[i] = fmaxf(top[i], __shfl_xor_sync(kFullMask, top[i], o));
           top_v[i] = fmaxf(top_v[i], __shfl_xor_sync(kFullMask, top_v[i], o));
         }
-        const float now = fmaxf(m[i], top[i]), now_v = fmaxf(mv[i], top_v[i]);
+        const float now = fmaxf(m[i], top[i]), now_v = fmaxf(mv[i], top_v[i] - kQpLift);
         l[i] *= ex2_approx(m[i] - now);
         const float f = ex2_approx(mv[i] - now_v);
         m[i] = now;

@@ -3,25 +3,26 @@
 //
 // e4m3 is an operand type of the tensor cores, so K and V need no conversion and go from memory to shared memory and no further; what
 // has to become e4m3 is the other side, and a number becomes a sum of e4m3 terms: t0 = rne(x), t1 = rne(16 (x - t0)), ..., each with
-// four bits of it.  bf16 queries (8 bits) are two terms exactly, f16 three, f32 five (2^-20); the weights of the softmax five (2^-20).  The
-// terms are columns of their own, added with their powers of 16 when a result is read:
+// four bits of it.  bf16 queries (8 bits) are two terms exactly, f16 three, f32 five (2^-20); the weights of the softmax five (2^-20, and
+// never closer than 2^-26, the last place of the fifth term: the largest weight is kept between 2^3 and 2^8, so that a key 2^8 below it
+// still has 2^-21).  The terms are columns of their own, added with their powers of 16 when a result is read:
 //   S^T = K Q^T    [128 keys x kQTerms * kC]            32 dims per MMA, K and Q from shared memory, K-major;
 //   O^T = V^T P^T  [kDim / 128 x 128 dims x 5 * kC]     32 keys per MMA, V and the weights from shared memory, MN-major.
 // A tile of 128 keys of one kv head is 64 KiB (head_dim 256), 1.4 us of an SM's share of the memory; its products take a fraction of
 // that, and its softmax (thread = key) ~ 150 instructions per warp for four columns, where the mma.sync form, which converts every
 // number in registers, spends 5500 on the same bytes.
 //
-// Work split: CTA = (range, kv head and column tile).  The 16-key units of all rows form one sequence that is cut into equal ranges
+// Work split: CTA = (range, kv head and column tile).  The units of 16 to 64 keys of all rows form one sequence that is cut into equal ranges
 // (decode_parts.cuh); rows cut over ranges leave partials, folded by a second small launch.
 //   warps 0 - 7   softmax, thread = key, in two groups of four warps.  Up to eight columns the groups take the tiles in turn, each with
 //                 references, sums and accumulators of its own (a tile's chain of waits, from its scores to its weights, is longer than
 //                 its bytes: one group alone took 1.85 us per tile of 64 KiB); with 16 or 24 they take half of the columns each.
 //                 Scores from tensor memory, times the K scale of the key's block; weights exp2(s + log2 V scale - reference) as
-//                 e4m3 terms into shared memory; their sum without the V scale under a reference of its own.  A reference is set 2^4 above
-//                 the largest score and moves when a score passes it by 2^8 (weights up to 2^8 <= 448).  Thread = dim when a
+//                 e4m3 terms into shared memory; their sum without the V scale under a reference of its own.
+//                 Thread = dim when a
 //                 row's segment ends.
 //   warps 8, 9    MMA issue: the scores (up to two tiles ahead), the weighted sums.
-//   warp 10       TMA producer: 16-key boxes [8-key group][128-byte chunk][8 keys][128 B], 128-byte swizzle, into rings of tiles of K
+//   warp 10       TMA producer: boxes of a unit's keys [8-key group][128-byte chunk][8 keys][128 B], 128-byte swizzle, into rings of tiles of K
 //                 and of V (160 KiB), and with K the scales of its blocks.
 //   warp 11       the queries, up to two segments ahead: scaled to 2^7 - 2^8 by a power of two per column, split into terms.
 // Every wait is bounded; after a timeout (NVJ_DEV_TIMEOUT) the kernel stops issuing, lets copies land and frees its tensor
@@ -38,11 +39,12 @@
 namespace nvj {
 
 constexpr int kQuTile = 128;    // keys per tile
-constexpr int kQuUnit = 16;     // keys per box
-constexpr int kQuUnits = kQuTile / kQuUnit;
+constexpr int kQuUnits = 8;     // boxes per tile, at most: a box is a unit of 16, 32 or 64 keys of one block (QuParams::unit)
 constexpr int kQuPTerms = 5;
 constexpr int kQuThreads = 384;
-constexpr float kQuNone = -3e38f, kQuSlack = 8.f, kQuHead = 4.f;
+// References: of the weighted sum, set 2^3 below its largest weight and moved when one would pass 2^8 (e4m3 ends at 448); of the sum of the
+// weights, set 2^4 above and moved when a score passes it by 2^8.
+constexpr float kQuNone = -3e38f, kQuSlack = 8.f, kQuHead = 4.f, kQuLift = 3.f;
 
 template <typename T>
 constexpr int quq_terms() {
@@ -64,7 +66,6 @@ struct QuLayout {
   static constexpr int kSets = kByTiles ? (kSets0 < 4 ? 2 : 4) : (kSets0 < 2 ? 1 : 2);
   static constexpr int kColO = 2 * kNS;                                 // S twice, then the sets
   static constexpr int kTileBytes = kQuTile * kDim;                     // of K (or V)
-  static constexpr int kUnitBytes = kQuUnit * kDim;
   static constexpr int kQChunk = kNS * 128;                             // bytes of a chunk of the query terms
   static constexpr int kQBytes = kChunks * kQChunk, kWBytes = kQuTile * 128;
   static constexpr int kFit = (232448 - 1024 - 6144 - 2 * kQBytes - 2 * kWBytes) / kTileBytes;
@@ -184,29 +185,45 @@ struct QuRing {
     if (++at == kSlots) { at = 0; phase ^= 1u; reuse = true; }
   }
 };
-// The CTA's segments: 16-key units [j0, j0 + n) of row b, which has nb of them and len keys.
+// The CTA's segments: units [j0, j0 + n) of row b, which has nb of them and len keys.  A tile is `per` units.
 struct QuSeg {
   int b, j0, n, nb, len;
-  __device__ __forceinline__ int tiles() const { return (n + kQuUnits - 1) / kQuUnits; }
-  __device__ __forceinline__ int tile_units(int t) const { return min(n - t * kQuUnits, kQuUnits); }
+  __device__ __forceinline__ int tiles(int per) const { return (n + per - 1) / per; }
+  __device__ __forceinline__ int tile_units(int t, int per) const { return min(n - t * per, per); }
   __device__ __forceinline__ bool whole() const { return n == nb; }
 };
-struct QuWalk {
+__device__ __forceinline__ int qu_row_units(const QuParams& a, int len) { return (len + a.unit - 1) >> a.unit_log2; }
+struct QuWalk {  // (next_seg of decode_parts.cuh, over units)
   int b, j;
   long long g, g1;
-  __device__ __forceinline__ bool next(const DecodeParams& p, QuSeg& s) {
-    Seg r;
-    if (!next_seg(p, b, j, g, g1, r)) return false;
-    s = QuSeg{r.b, r.j0, r.j1 - r.j0, r.nb, r.len};
-    return true;
+  __device__ __forceinline__ bool next(const QuParams& a, const DecodeParams& p, QuSeg& s) {
+    while (g < g1 && b < p.batch) {
+      const int len = decode_row_len(p, b), nb = qu_row_units(a, len), all = blocks_in_sequence(p, nb);
+      if (j >= all) { ++b; j = 0; continue; }
+      const int take = (long long)(all - j) < g1 - g ? all - j : (int)(g1 - g);
+      const int j0 = j, j1 = min(j + take, nb), row = b;
+      g += take; ++b; j = 0;  // either the row is finished or the range is
+      if (j1 <= j0) continue;  // only the row's end lies here
+      s = QuSeg{row, j0, j1 - j0, nb, len};
+      return true;
+    }
+    return false;
   }
 };
+// What the range that begins at position j of row b, and at g0 of the sequence, tells the fold (umma_cut of decode_parts.cuh).
+__device__ __forceinline__ UmmaCut qu_cut(const QuParams& a, const DecodeParams& p, const Partition& pt, int range, int b, int j, long long g0) {
+  const int nb = qu_row_units(a, decode_row_len(p, b));
+  const int first = pt.cta_of(g0 - j);
+  if (j == 0 || j >= nb || first != range - 1) return kNoCut;
+  return UmmaCut{b, first, pt.cta_of(g0 - j + nb - 1), 0};
+}
 
 // ---- warp 10: TMA loads ------------------------------------------------------------------------------------------------------------
 template <class L>
 __device__ __forceinline__ void qu_producer(const CUtensorMap* k_map, const CUtensorMap* v_map, const QuParams& a, const DecodeParams& p, QuSmem<L>& sm,
                                             int head, QuWalk walk, int lane) {
-  const int per_block = p.block_size / kQuUnit;
+  const int per = kQuTile / a.unit, per_block = p.block_size / a.unit;
+  const uint32_t unit_bytes = (uint32_t)a.unit * L::kChunks * 128;
   const int oob = (int)(p.num_blocks * (p.block_size / 8));  // a box that starts here is filled with zeros
   uint64_t policy;  // every block is read once
   asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
@@ -217,19 +234,19 @@ __device__ __forceinline__ void qu_producer(const CUtensorMap* k_map, const CUte
   QuRing<L::kVSlots> v_at;
   uint32_t tile = 0;
   QuSeg s, nxt;
-  bool have = walk.next(p, s);
+  bool have = walk.next(a, p, s);
   int ids = have ? ids_at(s, 0) : 0;
   while (have) {
     bool more = false;
     int next_first = 0;
-    for (int i0 = 0; i0 < s.n; i0 += 32) {  // 32 units = 4 tiles at a time
+    for (int i0 = 0; i0 < s.n; i0 += 32) {  // 32 units = 4 tiles or more at a time
       const int ahead = ids_at(s, i0 + 32);
       const int n = min(s.n - i0, 32);
       const bool bad = lane < n && (ids < 0 || ids >= p.num_blocks);
       if (bad) atomicOr(p.status, NVJ_DEV_BAD_BLOCK_ID);
-      const int group = bad || lane >= n ? oob : ids * (p.block_size / 8) + (s.j0 + i0 + lane) % per_block * 2;
-      for (int i = 0; i < n; i += kQuUnits) {
-        const int cnt = min(n - i, kQuUnits), mine = __shfl_sync(kFullMask, group, (i + lane) & 31);  // a lane per unit
+      const int group = bad || lane >= n ? oob : ids * (p.block_size / 8) + (s.j0 + i0 + lane) % per_block * (a.unit / 8);
+      for (int i = 0; i < n; i += per) {
+        const int cnt = min(n - i, per), mine = __shfl_sync(kFullMask, group, (i + lane) & 31);  // a lane per unit
         const int id = __shfl_sync(kFullMask, bad ? -1 : ids, (i + lane) & 31);
         {
           if (k_at.reuse && !um_wait(&sm.k_empty[k_at.at], k_at.phase ^ 1u, &sm.abort_flag, p.status)) return;
@@ -250,18 +267,18 @@ __device__ __forceinline__ void qu_producer(const CUtensorMap* k_map, const CUte
             }
           }
           __syncwarp();
-          if (lane == 0) mbar_arrive_expect_tx(full, (uint32_t)cnt * L::kUnitBytes);
+          if (lane == 0) mbar_arrive_expect_tx(full, (uint32_t)cnt * unit_bytes);
           __syncwarp();
-          if (lane < cnt) qu_load(smem_u32(sm.k[k_at.at]) + lane * L::kUnitBytes, k_map, mine, head, full, policy);
+          if (lane < cnt) qu_load(smem_u32(sm.k[k_at.at]) + lane * unit_bytes, k_map, mine, head, full, policy);
           __syncwarp();
           k_at.step();
         }
         {
           if (v_at.reuse && !um_wait(&sm.v_empty[v_at.at], v_at.phase ^ 1u, &sm.abort_flag, p.status)) return;
           const uint32_t full = smem_u32(&sm.v_full[v_at.at]);
-          if (lane == 0) mbar_arrive_expect_tx(full, (uint32_t)cnt * L::kUnitBytes);
+          if (lane == 0) mbar_arrive_expect_tx(full, (uint32_t)cnt * unit_bytes);
           __syncwarp();
-          if (lane < cnt) qu_load(smem_u32(sm.v[v_at.at]) + lane * L::kUnitBytes, v_map, mine, head, full, policy);
+          if (lane < cnt) qu_load(smem_u32(sm.v[v_at.at]) + lane * unit_bytes, v_map, mine, head, full, policy);
           __syncwarp();
           v_at.step();
         }
@@ -269,7 +286,7 @@ __device__ __forceinline__ void qu_producer(const CUtensorMap* k_map, const CUte
       }
       ids = ahead;
       if (i0 == 0) {  // the row behind this one, once the first copies are on their way
-        more = walk.next(p, nxt);
+        more = walk.next(a, p, nxt);
         if (more) next_first = ids_at(nxt, 0);
       }
     }
@@ -283,16 +300,17 @@ __device__ __forceinline__ void qu_producer(const CUtensorMap* k_map, const CUte
 // A warp for either product: a tile's ~ 500 cycles of waits, descriptors and commits on each side would otherwise add up to more than its
 // bytes take (head_dim 128).  S(n) takes the place of S(n - 2), which has been read when that tile's weights are there.
 template <class L>
-__device__ __forceinline__ void qu_scores_warp(QuSmem<L>& sm, const DecodeParams& p, uint32_t tmem, QuWalk walk) {
+__device__ __forceinline__ void qu_scores_warp(QuSmem<L>& sm, const QuParams& a, const DecodeParams& p, uint32_t tmem, QuWalk walk) {
   constexpr uint32_t idesc = qu_idesc(L::kNS, false, false);
   const uint64_t k_desc0 = umma_desc(smem_u32(sm.k[0]), 16, L::kChunks * 1024);  // keys are rows: groups of 8
   const uint64_t q_desc0 = umma_desc(smem_u32(sm.q[0][0]), 16, 1024);
   QuRing<L::kKSlots> at;
   QuSeg s;
+  const int per = kQuTile / a.unit;
   uint32_t n = 0;
-  for (uint32_t seg = 0; walk.next(p, s); ++seg) {
+  for (uint32_t seg = 0; walk.next(a, p, s); ++seg) {
     const uint32_t qb = seg & 1u;
-    const int nt = s.tiles();
+    const int nt = s.tiles(per);
     for (int t = 0; t < nt; ++t, ++n) {
       if (t == 0 && !um_wait(&sm.q_full[qb], (seg >> 1) & 1u, &sm.abort_flag, p.status)) return;
       if (!um_wait(&sm.k_full[at.at], at.phase, &sm.abort_flag, p.status)) return;
@@ -315,15 +333,16 @@ __device__ __forceinline__ void qu_scores_warp(QuSmem<L>& sm, const DecodeParams
   }
 }
 template <class L>
-__device__ __forceinline__ void qu_sums_warp(QuSmem<L>& sm, const DecodeParams& p, uint32_t tmem, QuWalk walk) {
+__device__ __forceinline__ void qu_sums_warp(QuSmem<L>& sm, const QuParams& a, const DecodeParams& p, uint32_t tmem, QuWalk walk) {
   constexpr uint32_t idesc = qu_idesc(L::kNO, true, true);
   const uint64_t v_desc0 = umma_desc(smem_u32(sm.v[0]), 1024, L::kChunks * 1024);  // dims are rows, a chunk at a time; keys in groups of 8
   const uint64_t w_desc0 = umma_desc(smem_u32(sm.w[0]), 1024, 1024);
   QuRing<L::kVSlots> at;
   QuSeg s;
+  const int per = kQuTile / a.unit;
   uint32_t n = 0;
-  for (uint32_t seg = 0; walk.next(p, s); ++seg) {
-    const int nt = s.tiles();
+  for (uint32_t seg = 0; walk.next(a, p, s); ++seg) {
+    const int nt = s.tiles(per);
     const uint32_t n0 = n;
     for (int t = 0; t < nt; ++t, ++n) {
       if (!um_wait(&sm.v_full[at.at], at.phase, &sm.abort_flag, p.status)) return;
@@ -332,12 +351,12 @@ __device__ __forceinline__ void qu_sums_warp(QuSmem<L>& sm, const DecodeParams& 
       if (t == 0 && seg > 0 && !um_wait(&sm.o_free, (seg - 1) & 1u, &sm.abort_flag, p.status)) return;
       tc_fence_after_sync();
       if (um_elect_one()) {
-        const int steps = (s.tile_units(t) + 1) / 2;
+        const int steps = (s.tile_units(t, per) * a.unit + 31) / 32;
         const uint32_t o = tmem + L::kColO + ((n0 & 1u) + t) % L::kSets * (L::kChunks * L::kNO);
         const uint64_t v_desc = v_desc0 + (uint64_t)((at.at * L::kTileBytes) >> 4), w_desc = w_desc0 + (uint64_t)(((n & 1u) * L::kWBytes) >> 4);
         for (int i = 0; i < steps; ++i) {  // 32 keys, four groups of 8
           const uint32_t accumulate = (t >= L::kSets || i > 0) ? 1u : 0u;
-          const uint64_t wd = w_desc + (uint64_t)((i * 32 * 128) >> 4), vd = v_desc + (uint64_t)((i * 2 * L::kUnitBytes) >> 4);
+          const uint64_t wd = w_desc + (uint64_t)((i * 32 * 128) >> 4), vd = v_desc + (uint64_t)((i * 32 * L::kChunks * 128) >> 4);
 #pragma unroll
           for (int h = 0; h < L::kChunks; ++h) qu_mma(o + h * L::kNO, vd + (uint64_t)((h * 1024) >> 4), wd, idesc, accumulate);
         }
@@ -366,8 +385,9 @@ __device__ __forceinline__ void qu_softmax_warps(QuSmem<L>& sm, const QuParams& 
   float(&gmv)[12] = sm.mv[group];
   QuRing<L::kVSlots> at;  // V's slot of the tile at hand
   QuSeg s;
+  const int per = kQuTile / a.unit, my_unit = key >> a.unit_log2;
   uint32_t n = 0;
-  for (uint32_t seg = 0; walk.next(p, s); ++seg) {
+  for (uint32_t seg = 0; walk.next(a, p, s); ++seg) {
     const float* factor = sm.factor[seg & 3u] + first_col;
     const int* limit = sm.limit[seg & 3u] + first_col;
     const uint32_t n0 = n;
@@ -375,19 +395,19 @@ __device__ __forceinline__ void qu_softmax_warps(QuSmem<L>& sm, const QuParams& 
     float l[kCg];
 #pragma unroll
     for (int c = 0; c < kCg; ++c) l[c] = 0.f;
-    const int nt = s.tiles();
+    const int nt = s.tiles(per);
     for (int t = 0; t < nt; ++t, ++n) {
       if (kByTiles && (int)(n & 1u) != group) {
         at.step();
         continue;
       }
-      const int cnt = s.tile_units(t);
+      const int cnt = s.tile_units(t, per);
       const uint32_t buf = n & 1u, phase = (n >> 1) & 1u;
       // this thread's key; one that the tile does not have is behind everybody's last one
-      const int at_key = (key >> 4) < cnt ? (s.j0 + t * kQuUnits) * kQuUnit + key : 0x7fffffff;
+      const int at_key = my_unit < cnt ? (s.j0 + t * per) * a.unit + key : 0x7fffffff;
       const bool ok = um_wait(&sm.s_full[buf], phase, &sm.abort_flag, p.status);
       tc_fence_after_sync();
-      const float k_unit = sm.k_unit[n & 7u][key >> 4], v_unit = sm.v_unit[n & 7u][key >> 4];
+      const float k_unit = sm.k_unit[n & 7u][my_unit], v_unit = sm.v_unit[n & 7u][my_unit];
       float sc[kCg];
       {
         float x[kSRead][8];
@@ -433,7 +453,7 @@ __device__ __forceinline__ void qu_softmax_warps(QuSmem<L>& sm, const QuParams& 
           const float old = begun ? gm[key] : kQuNone, old_v = begun ? gmv[key] : kQuNone;
           // (a column whose scores stay under its reference keeps it)
           const float now = !begun || x > old + kQuSlack ? fmaxf(old, x + kQuHead) : old;
-          const float now_v = !begun || y > old_v + kQuSlack ? fmaxf(old_v, y + kQuHead) : old_v;
+          const float now_v = !begun || y > old_v + kQuSlack ? fmaxf(old_v, y - kQuLift) : old_v;
           sm.f[group][key] = ex2_approx(old - now);
           sm.fv[group][key] = ex2_approx(old_v - now_v);
           gm[key] = now;
@@ -507,9 +527,9 @@ __device__ __forceinline__ void qu_softmax_warps(QuSmem<L>& sm, const QuParams& 
           qu_sts4(w_row + (((region * (kWords / 4) + i) ^ (key & 7)) << 4), bytes[4 * i], bytes[4 * i + 1], bytes[4 * i + 2], bytes[4 * i + 3]);
       }
       // V rows of keys that are not there weigh nothing, but may hold anything: 0 x NaN is not 0
-      if (t == nt - 1 && (kByTiles || group == 0) && ((cnt & 1) || (s.j0 + s.n == s.nb && (s.len & (kQuUnit - 1))))) {
+      if (t == nt - 1 && (kByTiles || group == 0) && ((cnt * a.unit & 31) || (s.j0 + s.n == s.nb && (s.len & (a.unit - 1))))) {
         if (qu_meet_any<128>(bar, !um_wait(&sm.v_full[at.at], at.phase, &sm.abort_flag, p.status))) return give_up();
-        if (key < ((cnt + 1) / 2) * 32 && (at_key == 0x7fffffff || at_key >= s.len)) {
+        if (key < (cnt * a.unit + 31) / 32 * 32 && (at_key == 0x7fffffff || at_key >= s.len)) {
           const uint32_t v_row = smem_u32(sm.v[at.at]) + (key >> 3) * (8 * kDim) + (key & 7) * 128;
 #pragma unroll
           for (int i = 0; i < kDim / 16; ++i) qu_sts4(v_row + (i >> 3) * 1024 + (i & 7) * 16, 0u, 0u, 0u, 0u);
@@ -597,24 +617,23 @@ __device__ __forceinline__ void qu_softmax_warps(QuSmem<L>& sm, const QuParams& 
 // ---- warp 11: a segment's queries as e4m3 terms -----------------------------------------------------------------------
 template <class L, typename T, int kCg>
 __device__ __forceinline__ void qu_query_warp(QuSmem<L>& sm, const QuParams& a, const DecodeParams& p, int head, int ct, QuWalk walk, int lane) {
-  constexpr int kDim = L::kChunks * 128, kFly = 4;  // columns in flight
+  constexpr int kDim = L::kChunks * 128, kMost = sizeof(T) == 4 ? 6 : 12, kFly = L::kC < kMost ? L::kC : L::kC % kMost == 0 ? kMost : 4;  // columns in flight
   const int d = 8 * lane;  // (head_dim 128: half of the lanes)
   QuSeg s;
-  for (uint32_t seg = 0; walk.next(p, s); ++seg) {
+  for (uint32_t seg = 0; walk.next(a, p, s); ++seg) {
     const long long token = a.query_start_loc ? (long long)a.query_start_loc[s.b] : (long long)s.b * a.width;
 #pragma unroll 1
     for (int c0 = 0; c0 < L::kC; c0 += kFly) {
-      float x[kFly][8];
+      QRaw<T> raw[kFly];
       int limit[kFly];
 #pragma unroll
       for (int i = 0; i < kFly; ++i) {
         const int at = ct * L::kC + c0 + i;
         limit[i] = 0;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) x[i][k] = 0.f;
+        raw[i] = QRaw<T>{};
         if (at < a.columns) {
           const long long row = token + at / a.groups;
-          if (d < kDim) q_floats(q_load8(static_cast<const T*>(a.q) + (row * a.num_q_heads + head * a.groups + at % a.groups) * kDim + d), x[i]);
+          if (d < kDim) raw[i] = q_load8(static_cast<const T*>(a.q) + (row * a.num_q_heads + head * a.groups + at % a.groups) * kDim + d);
           const int last = a.positions ? a.positions[row] : 0x7ffffffe;
           limit[i] = last < s.len ? last + 1 : s.len;
         }
@@ -624,15 +643,17 @@ __device__ __forceinline__ void qu_query_warp(QuSmem<L>& sm, const QuParams& a, 
 #pragma unroll
       for (int i = 0; i < kFly; ++i) {
         const int c = c0 + i;
-        const int bits = __reduce_max_sync(kFullMask, __float_as_int(q_largest(0.f, x[i])));
+        float x[8];
+        q_floats(raw[i], x);
+        const int bits = __reduce_max_sync(kFullMask, __float_as_int(q_largest(0.f, x)));
         int e = (bits >> 23) - 127 - 7;  // largest = 2^(e + 7) * [1, 2)
         e = bits == 0 ? 0 : (e < -126 ? -126 : e);
         const float down = q_pow2(-e);
         bool odd = false;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          odd |= !(x[i][k] - x[i][k] == 0.f);  // an infinity or NaN: the column's scores are NaN
-          x[i][k] *= down;
+          odd |= !(x[k] - x[k] == 0.f);  // an infinity or NaN: the column's scores are NaN
+          x[k] *= down;
         }
         odd = __any_sync(kFullMask, odd);
         if (lane == 0) {
@@ -644,10 +665,10 @@ __device__ __forceinline__ void qu_query_warp(QuSmem<L>& sm, const QuParams& a, 
           uint32_t b[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            b[k] = q_pack2(x[i][2 * k], x[i][2 * k + 1]);
+            b[k] = q_pack2(x[2 * k], x[2 * k + 1]);
             const float2 y = q_float2(q_half2(b[k]));
-            x[i][2 * k] = (x[i][2 * k] - y.x) * 16.f;
-            x[i][2 * k + 1] = (x[i][2 * k + 1] - y.y) * 16.f;
+            x[2 * k] = (x[2 * k] - y.x) * 16.f;
+            x[2 * k + 1] = (x[2 * k + 1] - y.y) * 16.f;
           }
           const int row = c / kCg * L::kSRegion + j * kCg + c % kCg;
           if (d < kDim)
@@ -709,7 +730,7 @@ quantized_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
     const int b = base + threadIdx.x;
     int len = 0;
     if (b < p.batch) len = decode_row_len(p, b);
-    const int n = blocks_in_sequence(p, (len + kBlk - 1) / kBlk);
+    const int n = blocks_in_sequence(p, qu_row_units(a, len));
     if (base == 0) first_n = n;
     mine += n;
     const bool ours = b < p.batch && len <= 0 && b % ranges == range &&
@@ -743,7 +764,7 @@ quantized_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
   for (int base = 0; base < p.batch && carry <= g0; base += kQuThreads) {
     const int b = base + threadIdx.x;
     int n = 0;
-    if (b < p.batch) n = blocks_in_sequence(p, (decode_row_len(p, b) + kBlk - 1) / kBlk);
+    if (b < p.batch) n = blocks_in_sequence(p, qu_row_units(a, decode_row_len(p, b)));
     int chunk_total = 0;
     const long long excl = carry + qu_inclusive_scan(n, sm.scan, chunk_total) - n;
     if (n > 0 && excl <= g0 && g0 < excl + n) { sm.start_b = b; sm.start_j = (int)(g0 - excl); }
@@ -761,11 +782,11 @@ quantized_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
   const uint32_t tmem = sm.tmem_base;
 
   if (warp < 8) qu_softmax_warps<L, kCg, kByTiles>(sm, a, p, tmem, head, hct, ct, walk, range, warp >> 2, warp & 3, lane);
-  else if (warp == 8) qu_scores_warp<L>(sm, p, tmem, walk);
+  else if (warp == 8) qu_scores_warp<L>(sm, a, p, tmem, walk);
   else if (warp == 9) {
-    if (hct == 0 && lane == 0) a.cuts[range] = umma_cut(p, pt, range, walk.b, walk.j, walk.g);
+    if (hct == 0 && lane == 0) a.cuts[range] = qu_cut(a, p, pt, range, walk.b, walk.j, walk.g);
     __syncwarp();
-    qu_sums_warp<L>(sm, p, tmem, walk);
+    qu_sums_warp<L>(sm, a, p, tmem, walk);
   }
   else if (warp == 10) qu_producer<L>(&k_map, &v_map, a, p, sm, head, walk, lane);
   else qu_query_warp<L, T, kCg>(sm, a, p, head, ct, walk, lane);

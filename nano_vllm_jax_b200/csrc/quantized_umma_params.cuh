@@ -22,6 +22,7 @@ struct QuParams {
   float* part_ml;   // [2 * ranges][hcts][tile_columns][2]
   UmmaCut* cuts;    // [ranges]
   int width, columns, groups, num_q_heads, num_kv_heads;
+  int unit, unit_log2;  // keys per box: the largest of 16, 32 and 64 that divides a block
   int column_tiles, tile_columns, hcts;  // hcts = num_kv_heads * column_tiles
   float scale_log2;
 };

@@ -86,7 +86,8 @@ def tolerance(q, k, v, scale, term_bits=22):
     * a score is a sum of d products that are exact in f32, taken 16 at a time: every step may cut a last place (2^-23) of a partial sum of
       at most S = scale * max sum |q k|, and the two factors behind the sum round twice: an absolute error of (d / 16 + 2) 2^-23 S;
     * a weight's relative error is that times 1 (d exp(s) = exp(s) ds), 2^-22 each of the exponent's two roundings (times |s| <= S) and of
-      ex2.approx, and 2^-term_bits of its two 16-bit terms; in numerator and denominator;
+      ex2.approx, and 2^-term_bits of its terms (two of f16: 22, two of bf16: 16, five of e4m3: 20); in numerator and denominator;
+    * (f32 queries as five e4m3 terms, 2^-20: inside the same, S / 2^20 < (d / 16 + 2) S / 2^23 for d >= 128)
     * the weighted sum takes two products (high and low term) per 16 keys, 2^-23 of a partial sum cut each time, the sum of
       the weights one addition per key: (n / 8 + n) 2^-23; merging warps and CTAs adds a few.
     All of it relative to the largest |v|, which bounds the weighted mean."""

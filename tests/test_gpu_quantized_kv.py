@@ -208,6 +208,9 @@ def _check(out, q, state, tables, lens, limits, scale, term_bits=22):
         assert np.isfinite(out[r]).all() and off <= R.tolerance(q[r], k, v, scale, term_bits), (r, n, off)
 
 
+TERM_BITS = {1: 22, 2: 20}  # of a form's softmax weights
+
+
 def _forms(shape):
     return FORMS if shape[2] >= 128 else (1,)
 
@@ -233,11 +236,11 @@ def test_decode(shape, dtype):
     for form in _forms(shape):
         out = Q.paged_decode_attention_quantized(q, k, v, ks, vs, _i32(tables), _i32(LENGTHS), d ** -0.5, form=form)
         assert out.dtype == F32 and out.shape == q.shape
-        _check(_f64(out)[:, None], q64[:, None], state, tables, LENGTHS, [[n] for n in LENGTHS], d ** -0.5)
+        _check(_f64(out)[:, None], q64[:, None], state, tables, LENGTHS, [[n] for n in LENGTHS], d ** -0.5, TERM_BITS[form])
         # the same rows one at a time (clusters of other sizes, other ranges)
         for r in (1, 9, 15):
             one = Q.paged_decode_attention_quantized(q[r: r + 1], k, v, ks, vs, _i32(tables[r: r + 1]), _i32(LENGTHS[r: r + 1]), d ** -0.5, form=form)
-            _check(_f64(one)[:, None], q64[r: r + 1, None], state, tables[r: r + 1], LENGTHS[r: r + 1], [LENGTHS[r: r + 1]], d ** -0.5)
+            _check(_f64(one)[:, None], q64[r: r + 1, None], state, tables[r: r + 1], LENGTHS[r: r + 1], [LENGTHS[r: r + 1]], d ** -0.5, TERM_BITS[form])
 
 
 @pytest.mark.parametrize("width", [2, 3, 5, 9, 17])
@@ -257,9 +260,9 @@ def test_rows_of_several_tokens(shape, dtype, width):
     for form in _forms(shape):
         out = Q.paged_decode_attention_quantized(*args, positions=_i32(limits - 1), form=form)
         assert out.shape == (len(lens), width, hq * d)
-        _check(_f64(out).reshape(q64.shape), q64, state, tables, lens, limits, d ** -0.5)
+        _check(_f64(out).reshape(q64.shape), q64, state, tables, lens, limits, d ** -0.5, TERM_BITS[form])
         free = Q.paged_decode_attention_quantized(*args, form=form)
-        _check(_f64(free).reshape(q64.shape), q64, state, tables, lens, [[n] * width for n in lens], d ** -0.5)
+        _check(_f64(free).reshape(q64.shape), q64, state, tables, lens, [[n] * width for n in lens], d ** -0.5, TERM_BITS[form])
 
 
 @pytest.mark.parametrize("form", FORMS)
@@ -275,7 +278,7 @@ def test_any_scale_of_the_scores(scale, dtype, form):
     q, q64 = _queries(rng, (3, hq, d), dtype)
     (k, ks), (v, vs) = (_gpu(*s) for s in state)
     out = Q.paged_decode_attention_quantized(q, k, v, ks, vs, _i32(tables), _i32(lens), scale, form=form)
-    _check(_f64(out)[:, None], q64[:, None], state, tables, lens, [[n] for n in lens], scale)
+    _check(_f64(out)[:, None], q64[:, None], state, tables, lens, [[n] for n in lens], scale, TERM_BITS[form])
 
 
 @pytest.mark.parametrize("route", [1, 2, "prefill"])
@@ -311,8 +314,35 @@ def test_blocks_of_very_different_scales(route):
         want = R.attend(q64[r: r + 1], kk, vv, np.ones((1, n), bool), d ** -0.5)[0]
         # relative to the values that the softmax is about: the quiet ones in rows 0 and 2
         loudest = np.abs(vv).max() if r == 1 else np.abs(vv[np.abs(vv).max((1, 2)) < 1]).max()
-        within = R.tolerance(q64[r: r + 1], kk, vv, d ** -0.5) / np.abs(vv).max() * loudest
+        within = R.tolerance(q64[r: r + 1], kk, vv, d ** -0.5, TERM_BITS.get(route, 22)) / np.abs(vv).max() * loudest
         assert np.abs(out[r] - want).max() <= within
+
+
+@pytest.mark.parametrize("route", [1, 2, "prefill"])
+def test_one_loud_key_over_many_quiet_ones(route):
+    # one key's weight is 2^10 of each of the 8000 others', which together decide: they must keep their bits
+    hq, hkv, d, bs = shape = SHAPES[1]
+    rng = np.random.default_rng(25)
+    n = 8000
+    tables = rng.permutation(n // bs)[None]
+    state = [_pool(rng, n // bs, shape, spread=1) for _ in range(2)]
+    state[0][0][:], state[0][1][:] = 0x38, 1.0  # keys of ones; one of twos
+    state[0][0][tables[0, 130], 3] = 0x40
+    state[1][1][:] = 2.0 ** -8
+    q = np.full((1, hq, d), 10 * np.log(2) / d * 8)
+    qg = torch.from_numpy(q).to(F16).cuda()
+    q64 = _f64(qg)
+    (k, ks), (v, vs) = (_gpu(*s) for s in state)
+    args = (k, v, ks, vs, _i32(tables), _i32([n]))
+    if route == "prefill":
+        out = Q.packed_paged_prefill_attention_quantized(qg[None], *args, _i32([[n - 1]]), _i32([0, 1]), bs, 1 / 8, hq // hkv, num_decode_rows=0)
+    else:
+        out = Q.paged_decode_attention_quantized(qg, *args, 1 / 8, form=route)
+    kk, vv = (R.gather(codes, s, tables[0], n) for codes, s in state)
+    want = R.attend(q64, kk, vv, np.ones((1, n), bool), 1 / 8)[0]
+    off = _f64(out).reshape(hq, d) - want
+    # a weight is at least 2^-18 of itself right (above), the sums cut 2^-23 of their size n / 8 times in the mean half a place
+    assert np.linalg.norm(off) <= 1e-5 * np.linalg.norm(want)
 
 
 @pytest.mark.parametrize("form", FORMS)
@@ -328,7 +358,7 @@ def test_queries_of_any_size(queries, form):
     for dtype in (BF16, F32):
         q = torch.from_numpy(rng.standard_normal((2, hq, d)) * queries).to(dtype).cuda()
         out = Q.paged_decode_attention_quantized(q, k, v, ks, vs, _i32(tables), _i32(lens), 1 / 16, form=form)
-        _check(_f64(out)[:, None], _f64(q)[:, None], state, tables, lens, [[n] for n in lens], 1 / 16)
+        _check(_f64(out)[:, None], _f64(q)[:, None], state, tables, lens, [[n] for n in lens], 1 / 16, TERM_BITS[form])
 
 
 @pytest.mark.parametrize("form", FORMS)
@@ -365,7 +395,7 @@ def test_what_lies_outside_the_pool_or_the_table_is_flagged(monkeypatch):
         for r, good in ((0, [0, 2]), (1, [0, 1])):  # the other blocks' keys alone
             kk, vv = (R.gather(codes, s, tables[r][good], 32) for codes, s in state)
             want = R.attend(q64[r: r + 1], kk, vv, np.ones((1, 32), bool), d ** -0.5)[0]
-            assert np.abs(_f64(out[r]) - want).max() <= R.tolerance(q64[r: r + 1], kk, vv, d ** -0.5)
+            assert np.abs(_f64(out[r]) - want).max() <= R.tolerance(q64[r: r + 1], kk, vv, d ** -0.5, TERM_BITS.get(form, 22))
         with pytest.raises(K.DeviceStatusError, match="device status 2 "):
             K.check_device_status()
     for form in FORMS:
@@ -399,7 +429,7 @@ def test_blocks_beyond_four_gigabytes():
     q, q64 = _queries(rng, (2, hq, d), BF16)
     for form in FORMS:
         out = Q.paged_decode_attention_quantized(q, big[0][0], big[1][0], big[0][1], big[1][1], _i32(far[local]), _i32([41, 48]), 1 / 16, form=form)
-        _check(_f64(out)[:, None], q64[:, None], state, local, [41, 48], [[41], [48]], 1 / 16)
+        _check(_f64(out)[:, None], q64[:, None], state, local, [41, 48], [[41], [48]], 1 / 16, TERM_BITS[form])
     for dtype in (BF16, F32):
         out = Q.packed_paged_prefill_attention_quantized(q.to(dtype)[None], big[0][0], big[1][0], big[0][1], big[1][1], _i32(far[local]), _i32([41, 48]),
                                                          _i32([[40, 47]]), _i32([0, 1, 2]), bs, 1 / 16, 4, num_decode_rows=0)
@@ -418,7 +448,7 @@ def test_more_rows_than_a_grid_dimension_holds(shape, form):
     out = Q.paged_decode_attention_quantized(q, k, v, ks, vs, _i32(tables), _i32(lens), d ** -0.5, form=form)
     assert torch.isfinite(out).all()
     pick = [0, 1, 40000, 65534, 65535, 65536, rows - 1]
-    _check(_f64(out[pick])[:, None], _f64(q[pick])[:, None], state, tables[pick], lens[pick], [[n] for n in lens[pick]], d ** -0.5)
+    _check(_f64(out[pick])[:, None], _f64(q[pick])[:, None], state, tables[pick], lens[pick], [[n] for n in lens[pick]], d ** -0.5, TERM_BITS[form])
 
 
 # ------------------------------------------------------------------------------------------------ packed prefill
@@ -631,4 +661,4 @@ def test_rows_cut_over_many_ranges_of_the_tcgen05_tiles(shape, dtype, rows, hi):
     q, q64 = _queries(rng, (rows, hq, d), dtype)
     (k, ks), (v, vs) = (_gpu(*s) for s in state)
     out = Q.paged_decode_attention_quantized(q, k, v, ks, vs, _i32(tables), _i32(lens), d ** -0.5, form=2)
-    _check(_f64(out)[:, None], q64[:, None], state, tables, lens, [[n] for n in lens], d ** -0.5)
+    _check(_f64(out)[:, None], q64[:, None], state, tables, lens, [[n] for n in lens], d ** -0.5, TERM_BITS[2])
