@@ -17,10 +17,9 @@
 //   warps 0 - 7   softmax, thread = key, in two groups of four warps.  Up to eight columns the groups take the tiles in turn, each with
 //                 references, sums and accumulators of its own (a tile's chain of waits, from its scores to its weights, is longer than
 //                 its bytes: one group alone took 1.85 us per tile of 64 KiB); with 16 or 24 they take half of the columns each.
-//                 Scores from tensor memory, times the K scale of the key's block; weights exp2(s + log2 V scale - reference) as
-//                 e4m3 terms into shared memory; their sum without the V scale under a reference of its own.
-//                 Thread = dim when a
-//                 row's segment ends.
+//                 Scores from tensor memory, times the K scale of the key's block, plus the log2 of its V scale; weights exp2(that -
+//                 reference) as e4m3 terms into shared memory; their sum with the V scale divided out again (relative to the first
+//                 tile's largest).  Thread = dim when a row's segment ends.
 //   warps 8, 9    MMA issue: the scores (up to two tiles ahead), the weighted sums.
 //   warp 10       TMA producer: boxes of a unit's keys [8-key group][128-byte chunk][8 keys][128 B], 128-byte swizzle, into rings of tiles of K
 //                 and of V (160 KiB), and with K the scales of its blocks.
@@ -42,9 +41,10 @@ constexpr int kQuTile = 128;    // keys per tile
 constexpr int kQuUnits = 8;     // boxes per tile, at most: a box is a unit of 16, 32 or 64 keys of one block (QuParams::unit)
 constexpr int kQuPTerms = 5;
 constexpr int kQuThreads = 384;
-// References: of the weighted sum, set 2^3 below its largest weight and moved when one would pass 2^8 (e4m3 ends at 448); of the sum of the
-// weights, set 2^4 above and moved when a score passes it by 2^8.
-constexpr float kQuNone = -3e38f, kQuSlack = 8.f, kQuHead = 4.f, kQuLift = 3.f;
+// The reference of a column's weights is set 2^3 below its largest weight and moved when one would pass 2^8 (e4m3 ends at 448).
+constexpr float kQuNone = -3e38f, kQuSlack = 8.f, kQuLift = 3.f;
+constexpr float kQuMostInverse = 100.f;  // log2 of what a weight is multiplied by, at most, to take the V scale out of it again
+constexpr int kQuLens = kQuThreads;      // rows whose lengths a CTA keeps in shared memory
 
 template <typename T>
 constexpr int quq_terms() {
@@ -86,11 +86,14 @@ struct QuSmem {
   alignas(16) float k_unit[8][kQuUnits], v_unit[8][kQuUnits];  // by tile: the scales of its units' blocks; V's -1: no such block
   alignas(16) float factor[4][L::kC];  // by segment: what a column's products are multiplied by, and the keys it may see
   alignas(16) int limit[4][L::kC];
-  alignas(16) float red[2][4][12], red_v[2][4][12];  // per group and warp
-  alignas(16) float m[2][12], mv[2][12], f[2][12], fv[2][12];
+  alignas(16) float red[2][4][12];  // per group and warp
+  float red_v[2][4];
+  float m[2][12], mv[2][12];  // at the end: references of the sum of the weights, and of the weighted sums
+  int col_row[L::kC], col_token[L::kC];  // of a column: its row of the row's queries (and of its output), its token
+  int lens[kQuLens];  // of rows lens_from ..
   alignas(16) float out_f[2][L::kC];  // what a group's sums are multiplied by at the end
   int scan[16];
-  int start_b, start_j, abort_flag;
+  int start_b, start_j, lens_from, abort_flag;
   uint32_t tmem_base;
 };
 
@@ -196,9 +199,11 @@ __device__ __forceinline__ int qu_row_units(const QuParams& a, int len) { return
 struct QuWalk {  // (next_seg of decode_parts.cuh, over units)
   int b, j;
   long long g, g1;
+  const int* lens;  // in shared memory: an access to global memory takes up to 2 us here while the copies are under way
+  int lens_from;
   __device__ __forceinline__ bool next(const QuParams& a, const DecodeParams& p, QuSeg& s) {
     while (g < g1 && b < p.batch) {
-      const int len = decode_row_len(p, b), nb = qu_row_units(a, len), all = blocks_in_sequence(p, nb);
+      const int len = b - lens_from < kQuLens ? lens[b - lens_from] : decode_row_len(p, b), nb = qu_row_units(a, len), all = blocks_in_sequence(p, nb);
       if (j >= all) { ++b; j = 0; continue; }
       const int take = (long long)(all - j) < g1 - g ? all - j : (int)(g1 - g);
       const int j0 = j, j1 = min(j + take, nb), row = b;
@@ -381,8 +386,6 @@ __device__ __forceinline__ void qu_softmax_warps(QuSmem<L>& sm, const QuParams& 
   tmem += (uint32_t)(warp * 32) << 16;
   // a group that leaves early meets the other one, which waits at a segment's end or leaves as well
   auto give_up = [] { qu_meet_any<256>(3, true); };
-  float(&gm)[12] = sm.m[group];
-  float(&gmv)[12] = sm.mv[group];
   QuRing<L::kVSlots> at;  // V's slot of the tile at hand
   QuSeg s;
   const int per = kQuTile / a.unit, my_unit = key >> a.unit_log2;
@@ -392,9 +395,12 @@ __device__ __forceinline__ void qu_softmax_warps(QuSmem<L>& sm, const QuParams& 
     const int* limit = sm.limit[seg & 3u] + first_col;
     const uint32_t n0 = n;
     bool begun = false;  // the group has had a tile of this segment
-    float l[kCg];
+    float l[kCg], m[kCg], v_first = 0.f;
 #pragma unroll
-    for (int c = 0; c < kCg; ++c) l[c] = 0.f;
+    for (int c = 0; c < kCg; ++c) {
+      l[c] = 0.f;
+      m[c] = kQuNone;
+    }
     const int nt = s.tiles(per);
     for (int t = 0; t < nt; ++t, ++n) {
       if (kByTiles && (int)(n & 1u) != group) {
@@ -407,7 +413,8 @@ __device__ __forceinline__ void qu_softmax_warps(QuSmem<L>& sm, const QuParams& 
       const int at_key = my_unit < cnt ? (s.j0 + t * per) * a.unit + key : 0x7fffffff;
       const bool ok = um_wait(&sm.s_full[buf], phase, &sm.abort_flag, p.status);
       tc_fence_after_sync();
-      const float k_unit = sm.k_unit[n & 7u][my_unit], v_unit = sm.v_unit[n & 7u][my_unit];
+      const float k_unit = sm.k_unit[n & 7u][my_unit], v_unit = my_unit < cnt ? sm.v_unit[n & 7u][my_unit] : -1.f;
+      const float v_log = v_unit >= 0.f ? __log2f(v_unit) : 0.f;
       float sc[kCg];
       {
         float x[kSRead][8];
@@ -426,49 +433,52 @@ __device__ __forceinline__ void qu_softmax_warps(QuSmem<L>& sm, const QuParams& 
           float y = x[((L::kQTerms - 1) * kCg + c) / 8][((L::kQTerms - 1) * kCg + c) % 8];
 #pragma unroll
           for (int j = L::kQTerms - 2; j >= 0; --j) y = fmaf(y, 0.0625f, x[(j * kCg + c) / 8][(j * kCg + c) % 8]);
-          sc[c] = there && at_key < seen[c] ? y * (by[c] * k_unit) : -INFINITY;
+          sc[c] = there && at_key < seen[c] ? fmaf(y, by[c] * k_unit, v_log) : -INFINITY;
         }
       }
-      const float v_log = v_unit >= 0.f ? __log2f(v_unit) : 0.f;
-      float m[kCg], mv[kCg];
-      qu_lds(m, gm);
-      qu_lds(mv, gmv);
       bool above = !begun;
 #pragma unroll
-      for (int c = 0; c < kCg; ++c) above |= sc[c] > m[c] + kQuSlack || sc[c] + v_log > mv[c] + kQuSlack;
+      for (int c = 0; c < kCg; ++c) above |= sc[c] > m[c] + kQuSlack;
       if (qu_meet_any<128>(bar, !ok || above)) {
-        // the first tile, or rarely a later one: the tile's maxima; what has been summed so far is brought to the new references
+        // the first tile, or rarely a later one: the tile's maxima; what has been summed so far is brought to the new references, which every
+        // thread finds for itself
 #pragma unroll
         for (int c = 0; c < kCg; ++c) {
-          const float x = qu_warp_max(sc[c]), y = qu_warp_max(sc[c] + v_log);
-          if (lane == 0) {
-            sm.red[group][warp][c] = x;
-            sm.red_v[group][warp][c] = y;
+          const float x = qu_warp_max(sc[c]);
+          if (lane == 0) sm.red[group][warp][c] = x;
+        }
+        if (!begun) {
+          const float x = qu_warp_max(v_unit >= 0.f ? v_log : -INFINITY);
+          if (lane == 0) sm.red_v[group][warp] = x;
+        }
+        // (the group's weighted sums so far have to be complete)
+        const uint32_t done = kByTiles ? n - 2 : n - 1;
+        const bool complete = !begun || um_wait(&sm.pv_done[done & 1u], (done >> 1) & 1u, &sm.abort_flag, p.status);
+        if (qu_meet_any<128>(bar, !ok || !complete)) return give_up();
+        float f[kCg];
+#pragma unroll
+        for (int c = 0; c < kCg; c += 4) {
+          float x[4], y[4];
+          qu_lds(x, &sm.red[group][0][c]);
+#pragma unroll
+          for (int w = 1; w < 4; ++w) {
+            qu_lds(y, &sm.red[group][w][c]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = fmaxf(x[e], y[e]);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float now = x[e] > m[c + e] + kQuSlack ? x[e] - kQuLift : m[c + e];  // (one whose scores stay under it keeps its reference)
+            f[c + e] = ex2_approx(m[c + e] - now);
+            l[c + e] *= f[c + e];
+            m[c + e] = now;
           }
         }
-        if (qu_meet_any<128>(bar, !ok)) return give_up();
-        if (key < kCg) {
-          const float x = fmaxf(fmaxf(sm.red[group][0][key], sm.red[group][1][key]), fmaxf(sm.red[group][2][key], sm.red[group][3][key]));
-          const float y = fmaxf(fmaxf(sm.red_v[group][0][key], sm.red_v[group][1][key]), fmaxf(sm.red_v[group][2][key], sm.red_v[group][3][key]));
-          const float old = begun ? gm[key] : kQuNone, old_v = begun ? gmv[key] : kQuNone;
-          // (a column whose scores stay under its reference keeps it)
-          const float now = !begun || x > old + kQuSlack ? fmaxf(old, x + kQuHead) : old;
-          const float now_v = !begun || y > old_v + kQuSlack ? fmaxf(old_v, y - kQuLift) : old_v;
-          sm.f[group][key] = ex2_approx(old - now);
-          sm.fv[group][key] = ex2_approx(old_v - now_v);
-          gm[key] = now;
-          gmv[key] = now_v;
-        }
-        qu_meet_any<128>(bar, false);
-        qu_lds(m, gm);
-        qu_lds(mv, gmv);
-        if (begun) {
-          // the group's weighted sums so far have to be complete
-          const uint32_t done = kByTiles ? n - 2 : n - 1;
-          if (qu_meet_any<128>(bar, !um_wait(&sm.pv_done[done & 1u], (done >> 1) & 1u, &sm.abort_flag, p.status))) return give_up();
+        if (!begun) {
+          v_first = fmaxf(fmaxf(sm.red_v[group][0], sm.red_v[group][1]), fmaxf(sm.red_v[group][2], sm.red_v[group][3]));
+          v_first = v_first == -INFINITY ? 0.f : v_first;
+        } else {
           tc_fence_after_sync();
-#pragma unroll
-          for (int c = 0; c < kCg; ++c) l[c] *= sm.f[group][c];
 #pragma unroll 1
           for (int k = 0; k < L::kSets; ++k) {
             const int since = (k - (int)(n0 & 1u) + L::kSets) % L::kSets;  // the set's first tile in this segment
@@ -485,7 +495,7 @@ __device__ __forceinline__ void qu_softmax_warps(QuSmem<L>& sm, const QuParams& 
                 tmem_loaded(o[i]);
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                  if (8 * i + e < kQuPTerms * kCg) o[i][e] *= sm.fv[group][(8 * i + e) % kCg];
+                  if (8 * i + e < kQuPTerms * kCg) o[i][e] *= f[(8 * i + e) % kCg];
                 qu_tmem_st8(from + 8 * i, o[i]);
               }
             }
@@ -497,10 +507,11 @@ __device__ __forceinline__ void qu_softmax_warps(QuSmem<L>& sm, const QuParams& 
       // weights as e4m3 terms: byte term * kCg + column of the group's region of the key's row
       {
         float r[kCg];
+        const float inverse = ex2_approx(fminf(v_first - v_log, kQuMostInverse));
 #pragma unroll
         for (int c = 0; c < kCg; ++c) {
-          l[c] += ex2_approx(sc[c] - m[c]);
-          r[c] = ex2_approx(sc[c] + v_log - mv[c]);
+          r[c] = ex2_approx(sc[c] - m[c]);
+          l[c] = fmaf(r[c], inverse, l[c]);
         }
         uint32_t bytes[kWords];
 #pragma unroll
@@ -547,7 +558,13 @@ __device__ __forceinline__ void qu_softmax_warps(QuSmem<L>& sm, const QuParams& 
       for (int o = 16; o > 0; o >>= 1) l[c] += __shfl_xor_sync(kFullMask, l[c], o);
       if (lane == 0) sm.red[group][warp][c] = l[c];
     }
-    if (!begun && key < kCg) gm[key] = gmv[key] = kQuNone;
+    if (key == 0) {
+#pragma unroll
+      for (int c = 0; c < kCg; ++c) {
+        sm.mv[group][c] = m[c];
+        sm.m[group][c] = m[c] - v_first;
+      }
+    }
     if (qu_meet_any<256>(3, !um_wait(&sm.o_full, seg & 1u, &sm.abort_flag, p.status))) return;
     const bool final_row = s.whole();
     const long long slot = (long long)partial_slot(range, s.j0 == 0) * a.hcts + hct;
@@ -603,9 +620,7 @@ __device__ __forceinline__ void qu_softmax_warps(QuSmem<L>& sm, const QuParams& 
       for (int c = 0; c < kCg; ++c) {
         const int col = r * kCg + c;
         if (col >= columns || (L::kChunks == 1 && L::kRegions == 1 && c / (kCg / 2) != group)) continue;
-        const int at_col = ct * L::kC + col;
-        float* to = final_row ? a.out + ((token + at_col / a.groups) * a.num_q_heads + head * a.groups + at_col % a.groups) * kDim
-                              : a.part_acc + (slot * L::kC + col) * kDim;
+        float* to = final_row ? a.out + (token * a.num_q_heads + sm.col_row[col]) * kDim : a.part_acc + (slot * L::kC + col) * kDim;
         to[h * 128 + key] = y[c];
       }
     }
@@ -625,52 +640,59 @@ __device__ __forceinline__ void qu_query_warp(QuSmem<L>& sm, const QuParams& a, 
 #pragma unroll 1
     for (int c0 = 0; c0 < L::kC; c0 += kFly) {
       QRaw<T> raw[kFly];
-      int limit[kFly];
+      int limit[kFly], bits[kFly];
 #pragma unroll
       for (int i = 0; i < kFly; ++i) {
-        const int at = ct * L::kC + c0 + i;
-        limit[i] = 0;
         raw[i] = QRaw<T>{};
-        if (at < a.columns) {
-          const long long row = token + at / a.groups;
-          if (d < kDim) raw[i] = q_load8(static_cast<const T*>(a.q) + (row * a.num_q_heads + head * a.groups + at % a.groups) * kDim + d);
-          const int last = a.positions ? a.positions[row] : 0x7ffffffe;
+        limit[i] = 0;
+        if (ct * L::kC + c0 + i < a.columns) {
+          if (d < kDim) raw[i] = q_load8(static_cast<const T*>(a.q) + (token * a.num_q_heads + sm.col_row[c0 + i]) * kDim + d);
+          const int last = a.positions ? a.positions[token + sm.col_token[c0 + i]] : 0x7ffffffe;
           limit[i] = last < s.len ? last + 1 : s.len;
         }
       }
+      // (column by column each step waited for the one before: 300 cycles per column)
+#pragma unroll
+      for (int i = 0; i < kFly; ++i) {
+        float x[8];
+        q_floats(raw[i], x);
+        bits[i] = 0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) bits[i] = max(bits[i], __float_as_int(x[k]) & 0x7fffffff);
+      }
+#pragma unroll
+      for (int i = 0; i < kFly; ++i) bits[i] = __reduce_max_sync(kFullMask, bits[i]);
       // the scores of the segment two before have been computed
       if (c0 == 0 && seg > 1 && !um_wait(&sm.q_free[seg & 1u], ((seg >> 1) - 1) & 1u, &sm.abort_flag, p.status)) return;
 #pragma unroll
       for (int i = 0; i < kFly; ++i) {
         const int c = c0 + i;
-        float x[8];
-        q_floats(raw[i], x);
-        const int bits = __reduce_max_sync(kFullMask, __float_as_int(q_largest(0.f, x)));
-        int e = (bits >> 23) - 127 - 7;  // largest = 2^(e + 7) * [1, 2)
-        e = bits == 0 ? 0 : (e < -126 ? -126 : e);
+        const bool odd = bits[i] >= 0x7f800000;  // an infinity or NaN: the column's scores are NaN
+        int e = (bits[i] >> 23) - 127 - 7;       // largest = 2^(e + 7) * [1, 2)
+        e = bits[i] == 0 || odd ? 0 : (e < -126 ? -126 : e);
         const float down = q_pow2(-e);
-        bool odd = false;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          odd |= !(x[k] - x[k] == 0.f);  // an infinity or NaN: the column's scores are NaN
-          x[k] *= down;
-        }
-        odd = __any_sync(kFullMask, odd);
         if (lane == 0) {
           sm.factor[seg & 3u][c] = odd ? __int_as_float(0x7fffffff) : q_pow2(e) * a.scale_log2;
           sm.limit[seg & 3u][c] = limit[i];
         }
+        float x[8];
+        q_floats(raw[i], x);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] *= down;
+        const int row0 = c / kCg * L::kSRegion + c % kCg;
 #pragma unroll
         for (int j = 0; j < L::kQTerms; ++j) {
           uint32_t b[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             b[k] = q_pack2(x[2 * k], x[2 * k + 1]);
-            const float2 y = q_float2(q_half2(b[k]));
-            x[2 * k] = (x[2 * k] - y.x) * 16.f;
-            x[2 * k + 1] = (x[2 * k + 1] - y.y) * 16.f;
+            if (j + 1 < L::kQTerms) {
+              const float2 y = q_float2(q_half2(b[k]));
+              x[2 * k] = (x[2 * k] - y.x) * 16.f;
+              x[2 * k + 1] = (x[2 * k + 1] - y.y) * 16.f;
+            }
           }
-          const int row = c / kCg * L::kSRegion + j * kCg + c % kCg;
+          const int row = row0 + j * kCg;
           if (d < kDim)
             *reinterpret_cast<uint2*>(sm.q[seg & 1u][d / 128] + row * 128 + (((d % 128 / 16) ^ (row & 7)) << 4) + (d & 8)) =
                 make_uint2(b[0] | b[1] << 16, b[2] | b[3] << 16);
@@ -695,7 +717,7 @@ quantized_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
   if (threadIdx.x == 0) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&k_map)) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&v_map)) : "memory");
-    sm.start_b = p.batch; sm.start_j = 0; sm.abort_flag = 0;
+    sm.start_b = p.batch; sm.start_j = 0; sm.lens_from = 0; sm.abort_flag = 0;
     for (int i = 0; i < L::kKSlots; ++i) {
       mbar_init(smem_u32(&sm.k_full[i]), 1);
       mbar_init(smem_u32(&sm.k_empty[i]), 1);
@@ -715,6 +737,11 @@ quantized_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
     mbar_init(smem_u32(&sm.o_free), 256);
     mbar_fence_init();
   }
+  if (threadIdx.x < L::kC) {
+    const int at = ct * L::kC + threadIdx.x;
+    sm.col_token[threadIdx.x] = at / a.groups;
+    sm.col_row[threadIdx.x] = at / a.groups * a.num_q_heads + head * a.groups + at % a.groups;
+  }
   // (rows of the query terms that no column fills: finite, and never read)
   for (int i = threadIdx.x; i < (int)sizeof(sm.q) / 16; i += kQuThreads) reinterpret_cast<uint4*>(sm.q)[i] = make_uint4(0, 0, 0, 0);
   fence_proxy_async_smem();
@@ -731,7 +758,10 @@ quantized_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
     int len = 0;
     if (b < p.batch) len = decode_row_len(p, b);
     const int n = blocks_in_sequence(p, qu_row_units(a, len));
-    if (base == 0) first_n = n;
+    if (base == 0) {
+      first_n = n;
+      sm.lens[threadIdx.x] = len;
+    }
     mine += n;
     const bool ours = b < p.batch && len <= 0 && b % ranges == range &&
                       (!p.query_start_loc || p.query_start_loc[b + 1] - p.query_start_loc[b] == 1);
@@ -771,7 +801,13 @@ quantized_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
     carry += chunk_total;
   }
   __syncthreads();
-  const QuWalk walk{sm.start_b, sm.start_j, g0, g1};
+  if (p.batch > kQuThreads) {  // (else pass 1 has left all lengths)
+    const int b = sm.start_b + threadIdx.x;
+    sm.lens[threadIdx.x] = b < p.batch ? decode_row_len(p, b) : 0;
+    if (threadIdx.x == 0) sm.lens_from = sm.start_b;
+    __syncthreads();
+  }
+  const QuWalk walk{sm.start_b, sm.start_j, g0, g1, sm.lens, sm.lens_from};
   if (warp == 8) {  // tensor memory between the wait and the release (umma.cuh)
     tmem_alloc(smem_u32(&sm.tmem_base), 512);
     if (lane == 0) pdl_release();
