@@ -629,77 +629,83 @@ __device__ __forceinline__ void qu_softmax_warps(QuSmem<L>& sm, const QuParams& 
   }
 }
 
-// ---- warp 11: a segment's queries as e4m3 terms -----------------------------------------------------------------------
+// ---- queries as e4m3 terms: a column per warp at a time ---------------------------------------------------------------------------
+// (Loops that are rolled up: twelve columns unrolled were 20 KB of code that a CTA runs through once or twice, and waits for: 13 us in front
+// of the first scores of rows of five tokens.)
+template <class L, typename T>
+struct QuColumn {  // lane l's dims 8 l ..
+  QRaw<T> raw;
+  int limit;
+  __device__ __forceinline__ void load(const QuSmem<L>& sm, const QuParams& a, const QuSeg& s, long long token, int ct, int c, int lane) {
+    raw = QRaw<T>{};
+    limit = 0;
+    if (ct * L::kC + c < a.columns) {
+      if (8 * lane < L::kChunks * 128) raw = q_load8(static_cast<const T*>(a.q) + (token * a.num_q_heads + sm.col_row[c]) * (L::kChunks * 128) + 8 * lane);
+      const int last = a.positions ? a.positions[token + sm.col_token[c]] : 0x7ffffffe;
+      limit = last < s.len ? last + 1 : s.len;
+    }
+  }
+  template <int kCg>
+  __device__ __forceinline__ void store(QuSmem<L>& sm, const QuParams& a, uint32_t seg, int c, int lane) const {
+    const int d = 8 * lane;
+    float x[8];
+    q_floats(raw, x);
+    int bits = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) bits = max(bits, __float_as_int(x[k]) & 0x7fffffff);
+    bits = __reduce_max_sync(kFullMask, bits);
+    const bool odd = bits >= 0x7f800000;  // an infinity or NaN: the column's scores are NaN
+    int e = (bits >> 23) - 127 - 7;       // largest = 2^(e + 7) * [1, 2)
+    e = bits == 0 || odd ? 0 : (e < -126 ? -126 : e);
+    const float down = q_pow2(-e);
+    if (lane == 0) {
+      sm.factor[seg & 3u][c] = odd ? __int_as_float(0x7fffffff) : q_pow2(e) * a.scale_log2;
+      sm.limit[seg & 3u][c] = limit;
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] *= down;
+    const int row0 = c / kCg * L::kSRegion + c % kCg;
+#pragma unroll
+    for (int j = 0; j < L::kQTerms; ++j) {
+      uint32_t b[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        b[k] = q_pack2(x[2 * k], x[2 * k + 1]);
+        if (j + 1 < L::kQTerms) {
+          const float2 y = q_float2(q_half2(b[k]));
+          x[2 * k] = (x[2 * k] - y.x) * 16.f;
+          x[2 * k + 1] = (x[2 * k + 1] - y.y) * 16.f;
+        }
+      }
+      const int row = row0 + j * kCg;
+      if (d < L::kChunks * 128)
+        *reinterpret_cast<uint2*>(sm.q[seg & 1u][d / 128] + row * 128 + (((d % 128 / 16) ^ (row & 7)) << 4) + (d & 8)) =
+            make_uint2(b[0] | b[1] << 16, b[2] | b[3] << 16);
+    }
+  }
+};
+__device__ __forceinline__ long long qu_first_token(const QuParams& a, int b) {
+  return a.query_start_loc ? (long long)a.query_start_loc[b] : (long long)b * a.width;
+}
+// Warp 11: the segments behind the first, whose queries all warps have brought in before.
 template <class L, typename T, int kCg>
-__device__ __forceinline__ void qu_query_warp(QuSmem<L>& sm, const QuParams& a, const DecodeParams& p, int head, int ct, QuWalk walk, int lane) {
-  constexpr int kDim = L::kChunks * 128, kMost = sizeof(T) == 4 ? 6 : 12, kFly = L::kC < kMost ? L::kC : L::kC % kMost == 0 ? kMost : 4;  // columns in flight
-  const int d = 8 * lane;  // (head_dim 128: half of the lanes)
+__device__ __forceinline__ void qu_query_warp(QuSmem<L>& sm, const QuParams& a, const DecodeParams& p, int ct, QuWalk walk, int lane) {
   QuSeg s;
   for (uint32_t seg = 0; walk.next(a, p, s); ++seg) {
-    const long long token = a.query_start_loc ? (long long)a.query_start_loc[s.b] : (long long)s.b * a.width;
-#pragma unroll 1
-    for (int c0 = 0; c0 < L::kC; c0 += kFly) {
-      QRaw<T> raw[kFly];
-      int limit[kFly], bits[kFly];
-#pragma unroll
-      for (int i = 0; i < kFly; ++i) {
-        raw[i] = QRaw<T>{};
-        limit[i] = 0;
-        if (ct * L::kC + c0 + i < a.columns) {
-          if (d < kDim) raw[i] = q_load8(static_cast<const T*>(a.q) + (token * a.num_q_heads + sm.col_row[c0 + i]) * kDim + d);
-          const int last = a.positions ? a.positions[token + sm.col_token[c0 + i]] : 0x7ffffffe;
-          limit[i] = last < s.len ? last + 1 : s.len;
-        }
-      }
-      // (column by column each step waited for the one before: 300 cycles per column)
-#pragma unroll
-      for (int i = 0; i < kFly; ++i) {
-        float x[8];
-        q_floats(raw[i], x);
-        bits[i] = 0;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) bits[i] = max(bits[i], __float_as_int(x[k]) & 0x7fffffff);
-      }
-#pragma unroll
-      for (int i = 0; i < kFly; ++i) bits[i] = __reduce_max_sync(kFullMask, bits[i]);
+    if (seg > 0) {
+      const long long token = qu_first_token(a, s.b);
+      QuColumn<L, T> now, next;
+      now.load(sm, a, s, token, ct, 0, lane);
       // the scores of the segment two before have been computed
-      if (c0 == 0 && seg > 1 && !um_wait(&sm.q_free[seg & 1u], ((seg >> 1) - 1) & 1u, &sm.abort_flag, p.status)) return;
-#pragma unroll
-      for (int i = 0; i < kFly; ++i) {
-        const int c = c0 + i;
-        const bool odd = bits[i] >= 0x7f800000;  // an infinity or NaN: the column's scores are NaN
-        int e = (bits[i] >> 23) - 127 - 7;       // largest = 2^(e + 7) * [1, 2)
-        e = bits[i] == 0 || odd ? 0 : (e < -126 ? -126 : e);
-        const float down = q_pow2(-e);
-        if (lane == 0) {
-          sm.factor[seg & 3u][c] = odd ? __int_as_float(0x7fffffff) : q_pow2(e) * a.scale_log2;
-          sm.limit[seg & 3u][c] = limit[i];
-        }
-        float x[8];
-        q_floats(raw[i], x);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) x[k] *= down;
-        const int row0 = c / kCg * L::kSRegion + c % kCg;
-#pragma unroll
-        for (int j = 0; j < L::kQTerms; ++j) {
-          uint32_t b[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            b[k] = q_pack2(x[2 * k], x[2 * k + 1]);
-            if (j + 1 < L::kQTerms) {
-              const float2 y = q_float2(q_half2(b[k]));
-              x[2 * k] = (x[2 * k] - y.x) * 16.f;
-              x[2 * k + 1] = (x[2 * k + 1] - y.y) * 16.f;
-            }
-          }
-          const int row = row0 + j * kCg;
-          if (d < kDim)
-            *reinterpret_cast<uint2*>(sm.q[seg & 1u][d / 128] + row * 128 + (((d % 128 / 16) ^ (row & 7)) << 4) + (d & 8)) =
-                make_uint2(b[0] | b[1] << 16, b[2] | b[3] << 16);
-        }
+      if (seg > 1 && !um_wait(&sm.q_free[seg & 1u], ((seg >> 1) - 1) & 1u, &sm.abort_flag, p.status)) return;
+#pragma unroll 1
+      for (int c = 0; c < L::kC; ++c) {
+        if (c + 1 < L::kC) next.load(sm, a, s, token, ct, c + 1, lane);
+        now.template store<kCg>(sm, a, seg, c, lane);
+        now = next;
       }
+      fence_proxy_async_smem();
     }
-    fence_proxy_async_smem();
     mbar_arrive(smem_u32(&sm.q_full[seg & 1u]));
   }
 }
@@ -808,24 +814,40 @@ quantized_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
     __syncthreads();
   }
   const QuWalk walk{sm.start_b, sm.start_j, g0, g1, sm.lens, sm.lens_from};
-  if (warp == 8) {  // tensor memory between the wait and the release (umma.cuh)
-    tmem_alloc(smem_u32(&sm.tmem_base), 512);
-    if (lane == 0) pdl_release();
-  }
-  tc_fence_before_sync();
-  __syncthreads();
-  tc_fence_after_sync();
-  const uint32_t tmem = sm.tmem_base;
+  if (warp == 10) {  // needs neither queries nor tensor memory
+    qu_producer<L>(&k_map, &v_map, a, p, sm, head, walk, lane);
+  } else {
+    if (warp == 8) {  // tensor memory between the wait and the release (umma.cuh)
+      tmem_alloc(smem_u32(&sm.tmem_base), 512);
+      if (lane == 0) pdl_release();
+    }
+    {  // the first segment's queries
+      QuSeg s;
+      QuWalk first = walk;
+      const bool have = first.next(a, p, s);
+      const long long token = have ? qu_first_token(a, s.b) : 0;
+#pragma unroll 1
+      for (int c = warp - (warp > 10); have && c < L::kC; c += kQuThreads / 32 - 1) {
+        QuColumn<L, T> column;
+        column.load(sm, a, s, token, ct, c, lane);
+        column.template store<kCg>(sm, a, 0u, c, lane);
+      }
+      fence_proxy_async_smem();
+    }
+    tc_fence_before_sync();
+    named_bar_sync(4, kQuThreads - 32);
+    tc_fence_after_sync();
+    const uint32_t tmem = sm.tmem_base;
 
-  if (warp < 8) qu_softmax_warps<L, kCg, kByTiles>(sm, a, p, tmem, head, hct, ct, walk, range, warp >> 2, warp & 3, lane);
-  else if (warp == 8) qu_scores_warp<L>(sm, a, p, tmem, walk);
-  else if (warp == 9) {
-    if (hct == 0 && lane == 0) a.cuts[range] = qu_cut(a, p, pt, range, walk.b, walk.j, walk.g);
-    __syncwarp();
-    qu_sums_warp<L>(sm, a, p, tmem, walk);
+    if (warp < 8) qu_softmax_warps<L, kCg, kByTiles>(sm, a, p, tmem, head, hct, ct, walk, range, warp >> 2, warp & 3, lane);
+    else if (warp == 8) qu_scores_warp<L>(sm, a, p, tmem, walk);
+    else if (warp == 9) {
+      if (hct == 0 && lane == 0) a.cuts[range] = qu_cut(a, p, pt, range, walk.b, walk.j, walk.g);
+      __syncwarp();
+      qu_sums_warp<L>(sm, a, p, tmem, walk);
+    }
+    else qu_query_warp<L, T, kCg>(sm, a, p, ct, walk, lane);
   }
-  else if (warp == 10) qu_producer<L>(&k_map, &v_map, a, p, sm, head, walk, lane);
-  else qu_query_warp<L, T, kCg>(sm, a, p, head, ct, walk, lane);
 
   tc_fence_before_sync();
   __syncthreads();
@@ -834,7 +856,7 @@ quantized_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
     while (global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
     __syncthreads();
   }
-  if (warp == 8) tmem_dealloc(tmem, 512);
+  if (warp == 8) tmem_dealloc(sm.tmem_base, 512);
 }
 
 template <typename T, int kDim, int kCg, bool kByTiles>
