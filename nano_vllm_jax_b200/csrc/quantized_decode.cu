@@ -563,41 +563,44 @@ static QuPlan qu_plan(int columns, int num_kv_heads, int head_dim, int sms) {
   return w;
 }
 
-// One CTA per (boundary between two ranges, kv head and column tile): the first boundary that cuts a row folds the row's columns from the
-// ranges' partials.  Thread = (column, 4 dims) in turn.
+// The first boundary that cuts a row folds the row's columns from the ranges' partials.  Grid: boundary, kv head and column tile, 256 pieces of
+// (column, 4 dims); a thread a piece.  Behind boundary c lies a row that begins in range c and goes on in c + 1, if any does: those two
+// parts are asked for together with what was cut.  (A CTA for all columns, that asked first and loaded then: 11 us behind rows of five tokens.)
 __global__ void __launch_bounds__(256) quantized_umma_fold_kernel(QuParams a, int head_dim) {
-  const int hct = blockIdx.y, head = hct / a.column_tiles, ct = hct % a.column_tiles;
+  const int hct = blockIdx.y, head = hct / a.column_tiles, ct = hct % a.column_tiles, pieces = head_dim / 4;
+  const int item = blockIdx.z * 256 + threadIdx.x, c = item / pieces, d = item % pieces * 4, at = ct * a.tile_columns + c;
+  const int out_row = at / a.groups * a.num_q_heads + head * a.groups + at % a.groups;
+  const bool mine = c < min(a.columns - ct * a.tile_columns, a.tile_columns);
+  const int first = blockIdx.x;
   pdl_wait();
   pdl_release();
-  const UmmaCut cut = a.cuts[blockIdx.x + 1];
-  if (cut.b < 0) return;
-  const int parts = cut.last - cut.first + 1, pieces = head_dim / 4;
-  const int columns = min(a.columns - ct * a.tile_columns, a.tile_columns);
-  const long long token = a.query_start_loc ? (long long)a.query_start_loc[cut.b] : (long long)cut.b * a.width;
-  for (int i = threadIdx.x; i < columns * pieces; i += 256) {
-    const int c = i / pieces, d = i % pieces * 4;
-    float top = -3e38f, sum = 0.f;
-    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int k0 = 0; k0 < parts; k0 += 8) {  // eight parts in flight
-      float2 e[8];
-      float4 x[8];
+  if (!mine) return;
+  auto slot_of = [&](int part) { return ((long long)partial_slot(part, part == first) * a.hcts + hct) * a.tile_columns + c; };
+  auto load = [&](int part, float2& e, float4& x) {
+    e = __ldcg(reinterpret_cast<const float2*>(a.part_ml + slot_of(part) * 2));
+    x = __ldcg(reinterpret_cast<const float4*>(a.part_acc + slot_of(part) * head_dim + d));
+  };
+  float2 e[8];
+  float4 x[8];
+  load(first, e[0], x[0]);
+  load(first + 1, e[1], x[1]);
+  const int4 cut = __ldcg(reinterpret_cast<const int4*>(a.cuts + first + 1));  // row, its first and last range
+  if (cut.x < 0) return;
+  float top = -3e38f, sum = 0.f;
+  float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int from = first;;) {
+    const int n = from == first ? 2 : min(cut.z + 1 - from, 8);
+    float now = top;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int part = cut.first + (k0 + k < parts ? k0 + k : 0);
-        const long long slot = ((long long)partial_slot(part, part == cut.first) * a.hcts + hct) * a.tile_columns + c;
-        e[k] = __ldcg(reinterpret_cast<const float2*>(a.part_ml + slot * 2));
-        x[k] = __ldcg(reinterpret_cast<const float4*>(a.part_acc + slot * head_dim + d));
-        if (k0 + k >= parts) e[k] = make_float2(-3e38f, 0.f), x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-      }
-      float now = top;
+    for (int k = 0; k < 8; ++k)
+      if (k < n) now = fmaxf(now, e[k].x);
+    const float f = ex2_approx(top - now);
+    sum *= f;
+    y = make_float4(y.x * f, y.y * f, y.z * f, y.w * f);
+    top = now;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) now = fmaxf(now, e[k].x);
-      const float f = ex2_approx(top - now);
-      sum *= f;
-      y = make_float4(y.x * f, y.y * f, y.z * f, y.w * f);
-      top = now;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
+    for (int k = 0; k < 8; ++k)
+      if (k < n) {
         const float w = ex2_approx(e[k].x - top);
         sum = fmaf(e[k].y, w, sum);
         y.x = fmaf(x[k].x, w, y.x);
@@ -605,16 +608,21 @@ __global__ void __launch_bounds__(256) quantized_umma_fold_kernel(QuParams a, in
         y.z = fmaf(x[k].z, w, y.z);
         y.w = fmaf(x[k].w, w, y.w);
       }
-    }
-    const float inverse = sum == 0.f ? 0.f : 1.f / sum;
-    const int at = ct * a.tile_columns + c;
-    *reinterpret_cast<float4*>(a.out + ((token + at / a.groups) * a.num_q_heads + head * a.groups + at % a.groups) * head_dim + d) =
-        make_float4(y.x * inverse, y.y * inverse, y.z * inverse, y.w * inverse);
+    from += n;
+    if (from > cut.z) break;
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (from + k <= cut.z) load(from + k, e[k], x[k]);
   }
+  const float inverse = sum == 0.f ? 0.f : 1.f / sum;
+  const long long token = a.query_start_loc ? (long long)a.query_start_loc[cut.x] : (long long)cut.x * a.width;
+  *reinterpret_cast<float4*>(a.out + (token * a.num_q_heads + out_row) * head_dim + d) =
+      make_float4(y.x * inverse, y.y * inverse, y.z * inverse, y.w * inverse);
 }
 
-// What a row's end costs a CTA, in keys (decode_parts.cuh).
-constexpr int kQuRowEndCost = 128;
+// What a row's end costs a CTA, in keys (decode_parts.cuh), up to eight columns and beyond.  256 rows of 1024 - 4096 keys 107.4 us with 64, 107.2 with
+// 128, 106.5 with 192, 106.8 with 256, 107.1 with 384; 48 rows of 8 heads 39.2, 38.5, 38.4, 38.1, 38.5; 64 rows of 5 tokens 58.4, 56.7, 55.8, 55.2, 53.6.
+constexpr int kQuRowEndCost = 256, kQuWideRowEndCost = 384;
 
 static int run_quantized_umma(const QDecodeParams& q, int q_dtype, int head_dim, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
   const int sms = decode_wide_num_ctas();
@@ -662,11 +670,11 @@ static int run_quantized_umma(const QDecodeParams& q, int q_dtype, int head_dim,
   p.batch = q.rows;
   p.table_width = q.table_width;
   p.block_size = q.block_size;
-  p.row_end_cost = kQuRowEndCost >> unit_log2;
+  p.row_end_cost = (w.tile_columns <= 8 ? kQuRowEndCost : kQuWideRowEndCost) >> unit_log2;
   const auto launch = q_dtype == NVJ_BF16 ? launch_quantized_umma_bf16 : q_dtype == NVJ_F16 ? launch_quantized_umma_f16 : launch_quantized_umma_f32;
   const int rc = launch(k_map, v_map, a, p, head_dim, w.ranges, stream);
   if (rc != NVJ_OK || w.ranges < 2) return rc;
-  return launch_after(quantized_umma_fold_kernel, dim3(w.ranges - 1, w.hcts), dim3(256), 0, stream, a, head_dim) == cudaSuccess ? NVJ_OK : NVJ_ERR_LAUNCH;
+  return launch_after(quantized_umma_fold_kernel, dim3(w.ranges - 1, w.hcts, (w.tile_columns * head_dim / 4 + 255) / 256), dim3(256), 0, stream, a, head_dim) == cudaSuccess ? NVJ_OK : NVJ_ERR_LAUNCH;
 }
 
 // Whether a call goes to the tcgen05 form.
