@@ -15,6 +15,7 @@
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <cuda_runtime_api.h>
 #include <dlfcn.h>
@@ -46,6 +47,12 @@ struct Library {
   decltype(&nvj_stage_in) stage_in;
   decltype(&nvj_hybrid_snapshot_host_slots) snapshot;
   decltype(&nvj_hybrid_restore_host_slots) restore;
+  decltype(&nvj_kv_append_quantized) quantized_append;
+  decltype(&nvj_paged_decode_quantized) quantized_decode;
+  decltype(&nvj_paged_decode_quantized_workspace_bytes) quantized_decode_bytes;
+  decltype(&nvj_paged_prefill_quantized) quantized_prefill;
+  decltype(&nvj_paged_prefill_quantized_workspace_bytes) quantized_prefill_bytes;
+  decltype(&nvj_build_packed_layout) packed_layout;
 };
 Library lib;
 PyObject* cb_workspace;  // (device index, rows): makes Python create the workspace and hand it over
@@ -399,6 +406,178 @@ PyObject* packed_prefill(PyObject* const* a, Py_ssize_t n) {
                            wb, variant, tiles_only ? 3 : 0, (int)counted, stream));
   if (!finished(rc, "nvj_paged_prefill_packed", l.device, stream, ws != nullptr, true)) return nullptr;
   return THPVariable_Wrap(std::move(out));
+}
+
+// ---- the 8-bit cache ----------------------------------------------------------------------------------------------
+// One layer [NB, bs, Hkv, D] e4m3 with scales [NB, Hkv] f32.
+struct QuantizedLayer {
+  bool ok = false;
+  int device, block_size, hkv, d;
+  long long blocks;
+  void *k, *v;
+  float *ks, *vs;
+};
+bool aligned(const at::Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0; }
+QuantizedLayer quantized_layer(PyObject* const* a) {  // k, v, k_scale, v_scale
+  QuantizedLayer l;
+  const at::Tensor *k = tensor(a[0]), *v = tensor(a[1]), *ks = tensor(a[2]), *vs = tensor(a[3]);
+  if (!k || !v || !ks || !vs || !k->is_cuda() || k->dim() != 4 || v->sizes() != k->sizes() || k->scalar_type() != at::kFloat8_e4m3fn ||
+      v->scalar_type() != at::kFloat8_e4m3fn || ks->scalar_type() != at::kFloat || vs->scalar_type() != at::kFloat || ks->dim() != 2 ||
+      vs->sizes() != ks->sizes() || ks->size(0) != k->size(0) || ks->size(1) != k->size(2))
+    return l;
+  l.device = k->get_device();
+  if (!on(*v, l.device) || !on(*ks, l.device) || !on(*vs, l.device) || !k->is_contiguous() || !v->is_contiguous() || !ks->is_contiguous() ||
+      !vs->is_contiguous() || !aligned(*k) || !aligned(*v))
+    return l;
+  l.blocks = k->size(0);
+  l.block_size = (int)k->size(1);
+  l.hkv = (int)k->size(2);
+  l.d = (int)k->size(3);
+  l.k = k->data_ptr();
+  l.v = v->data_ptr();
+  l.ks = static_cast<float*>(ks->data_ptr());
+  l.vs = static_cast<float*>(vs->data_ptr());
+  const bool dims = l.d == 64 || l.d == 128 || l.d == 256, block = l.block_size == 16 || l.block_size == 32 || l.block_size == 48 || l.block_size == 64;
+  l.ok = dims && block;
+  return l;
+}
+bool plain_rows(const at::Tensor& t, int device) { return on(t, device) && dtype_code(t) >= 0 && t.is_contiguous() && aligned(t); }
+
+// quantized_append(new_k, new_v, k, v, k_scale, v_scale, positions, block_table, query_start_loc | None, token_row_ids | None,
+//                  seq_lens | None) -> True
+PyObject* quantized_append(PyObject* const* a, Py_ssize_t n) {
+  if (!args_are(n, 11)) return nullptr;
+  const at::Tensor *nk = tensor(a[0]), *nv = tensor(a[1]), *pos = tensor(a[6]), *tab = tensor(a[7]);
+  const at::Tensor* extra[3];  // query_start_loc, token_row_ids, seq_lens
+  const QuantizedLayer l = quantized_layer(a + 2);
+  if (!l.ok || !nk || !nv || !pos || !tab) NVJ_NONE();
+  for (int i = 0; i < 3; ++i) {
+    extra[i] = a[8 + i] == Py_None ? nullptr : tensor(a[8 + i]);
+    if (a[8 + i] != Py_None && (!extra[i] || !meta(*extra[i], l.device))) NVJ_NONE();
+  }
+  if (nk->dim() != 4 || nk->sizes() != nv->sizes() || nk->size(2) != l.hkv || nk->size(3) != l.d || nk->dtype() != nv->dtype() ||
+      !plain_rows(*nk, l.device) || !plain_rows(*nv, l.device) || !meta(*pos, l.device) || !meta(*tab, l.device))
+    NVJ_NONE();
+  const long long rows = nk->size(0), cols = nk->size(1);
+  const bool packed = extra[1] != nullptr;
+  if (rows * cols == 0 || pos->dim() != 2 || pos->size(0) != rows || pos->size(1) != cols || tab->dim() != 2 || tab->numel() == 0 || l.blocks == 0 ||
+      (packed ? rows != 1 || extra[1]->sizes() != pos->sizes() : rows > tab->size(0)) ||
+      (extra[0] && (extra[0]->dim() != 1 || extra[0]->numel() < 1)) || (extra[2] && (extra[2]->dim() != 1 || extra[2]->size(0) != tab->size(0))))
+    NVJ_NONE();
+  const c10::cuda::OptionalCUDAGuard guard(c10::Device(c10::kCUDA, (c10::DeviceIndex)l.device));
+  void* stream = stream_of(l.device);
+  int32_t* st = status_for(l.device, stream);
+  if (!st) return nullptr;
+  auto given = [&](int i) { return extra[i] ? i32(*extra[i]) : nullptr; };
+  int rc;
+  NVJ_CALL(rc, lib.quantized_append(nk->data_ptr(), nv->data_ptr(), dtype_code(*nk), i32(*pos), i32(*tab), given(1), (int)tab->size(0),
+                                    (int)tab->size(1), given(0), extra[0] ? (int)extra[0]->numel() - 1 : 0, given(2), (int)rows, (int)cols, l.k, l.v,
+                                    l.ks, l.vs, l.blocks, l.block_size, l.hkv, l.d, st, stream));
+  if (!finished(rc, "nvj_kv_append_quantized", l.device, stream, false, true)) return nullptr;
+  Py_RETURN_TRUE;
+}
+
+// quantized_decode(q, k, v, k_scale, v_scale, block_table, seq_lens, scale, positions | None, form) -> out as q [B, Hq, D], or [B, T, Hq * D]
+PyObject* quantized_decode(PyObject* const* a, Py_ssize_t n) {
+  if (!args_are(n, 10)) return nullptr;
+  const at::Tensor *q = tensor(a[0]), *tab = tensor(a[5]), *len = tensor(a[6]), *pos = a[8] == Py_None ? nullptr : tensor(a[8]);
+  const double scale = PyFloat_AsDouble(a[7]);
+  const long long form = PyLong_AsLongLong(a[9]);
+  if (PyErr_Occurred()) { PyErr_Clear(); NVJ_NONE(); }
+  const QuantizedLayer l = quantized_layer(a + 1);
+  if (!l.ok || !q || !tab || !len || (!pos && a[8] != Py_None) || (q->dim() != 3 && q->dim() != 4)) NVJ_NONE();
+  const bool wide = q->dim() == 4;
+  const long long batch = q->size(0), width = wide ? q->size(1) : 1, hq = q->size(-2);
+  if (batch * width * hq == 0 || q->size(-1) != l.d || hq % l.hkv != 0 || !plain_rows(*q, l.device) || !meta(*tab, l.device) || !meta(*len, l.device) ||
+      tab->dim() != 2 || tab->size(0) != batch || len->dim() != 1 || len->size(0) != batch ||
+      (pos && (!meta(*pos, l.device) || pos->numel() != batch * width)) || batch * width > 0x7fffffffLL)
+    NVJ_NONE();
+  const c10::cuda::OptionalCUDAGuard guard(c10::Device(c10::kCUDA, (c10::DeviceIndex)l.device));
+  void* stream = stream_of(l.device);
+  int32_t* st = status_for(l.device, stream);
+  if (!st) return nullptr;
+  at::Tensor out = wide ? output({batch, width, hq * l.d}, l.device) : output({batch, hq, l.d}, l.device);
+  const size_t bytes = lib.quantized_decode_bytes((int)batch, (int)width, (int)tab->size(1), l.block_size, l.hkv, l.d, (int)hq, (int)form);
+  at::Tensor scratch;
+  if (bytes) scratch = empty({(long long)bytes}, at::kByte, l.device);
+  int rc;
+  NVJ_CALL(rc, lib.quantized_decode(q->data_ptr(), dtype_code(*q), l.k, l.v, l.ks, l.vs, l.blocks, l.block_size, l.hkv, l.d, (int)hq, i32(*tab),
+                                    (int)tab->size(1), i32(*len), pos ? i32(*pos) : nullptr, nullptr, (int)batch, (int)width, (float)scale,
+                                    static_cast<float*>(out.data_ptr()), st, bytes ? scratch.data_ptr() : nullptr, bytes, (int)form, stream));
+  if (!finished(rc, "nvj_paged_decode_quantized", l.device, stream, false, true)) return nullptr;
+  return THPVariable_Wrap(std::move(out));
+}
+
+// quantized_prefill(query [1, T, Hq, D], k, v, k_scale, v_scale, block_table, kv_lens, positions, query_start_loc, block_size, scale, groups,
+//                   decode_rows | None, tile_pairs | None) -> out [1, T, Hq * D] float32
+PyObject* quantized_prefill(PyObject* const* a, Py_ssize_t n) {
+  if (!args_are(n, 14)) return nullptr;
+  const at::Tensor *q = tensor(a[0]), *tab = tensor(a[5]), *len = tensor(a[6]), *pos = tensor(a[7]), *qsl = tensor(a[8]);
+  const long long bs = PyLong_AsLongLong(a[9]), groups = PyLong_AsLongLong(a[11]);
+  const double scale = PyFloat_AsDouble(a[10]);
+  const long long singles = a[12] == Py_None ? -1 : PyLong_AsLongLong(a[12]), pairs = a[13] == Py_None ? -1 : PyLong_AsLongLong(a[13]);
+  if (PyErr_Occurred()) { PyErr_Clear(); NVJ_NONE(); }
+  const QuantizedLayer l = quantized_layer(a + 1);
+  if (!l.ok || !q || !tab || !len || !pos || !qsl || q->dim() != 4 || q->size(0) != 1) NVJ_NONE();
+  const long long tokens = q->size(1), hq = q->size(2);
+  if (tokens * hq == 0 || q->size(3) != l.d || bs != l.block_size || hq != l.hkv * groups || !plain_rows(*q, l.device) || !meta(*tab, l.device) ||
+      !meta(*len, l.device) || !meta(*pos, l.device) || !meta(*qsl, l.device) || tab->dim() != 2 || pos->dim() != 2 || pos->size(0) != 1 ||
+      pos->size(1) != tokens || len->dim() != 1 || len->size(0) != tab->size(0) || qsl->dim() != 1 || qsl->size(0) != tab->size(0) + 1)
+    NVJ_NONE();
+  const int rows = (int)tab->size(0), width = (int)tab->size(1), dt = dtype_code(*q);
+  const c10::cuda::OptionalCUDAGuard guard(c10::Device(c10::kCUDA, (c10::DeviceIndex)l.device));
+  void* stream = stream_of(l.device);
+  int32_t* st = status_for(l.device, stream);
+  if (!st) return nullptr;
+  at::Tensor out = output({1, tokens, hq * l.d}, l.device);
+  const size_t bytes = lib.quantized_prefill_bytes(dt, rows, width, l.block_size, l.hkv, l.d, (int)hq, (float)scale, (int)singles);
+  at::Tensor scratch;
+  if (bytes) scratch = empty({(long long)bytes}, at::kByte, l.device);
+  int rc;
+  NVJ_CALL(rc, lib.quantized_prefill(q->data_ptr(), dt, l.k, l.v, l.ks, l.vs, l.blocks, l.block_size, l.hkv, l.d, (int)hq, i32(*tab), width, i32(*len),
+                                     i32(*pos), i32(*qsl), rows, (int)tokens, (float)scale, static_cast<float*>(out.data_ptr()), st,
+                                     bytes ? scratch.data_ptr() : nullptr, bytes, (int)singles, (int)pairs, stream));
+  if (!finished(rc, "nvj_paged_prefill_quantized", l.device, stream, false, true)) return nullptr;
+  return THPVariable_Wrap(std::move(out));
+}
+
+// packed_layout(cached_lens, new_lens, block_tables, free_blocks, free_head, block_size, token_bucket) -> (positions, token_row_ids,
+// slot_mapping [1, T], query_start_loc, seq_lens, free_head)
+PyObject* packed_layout(PyObject* const* a, Py_ssize_t n) {
+  if (!args_are(n, 7)) return nullptr;
+  const at::Tensor* t[5];
+  for (int i = 0; i < 5; ++i)
+    if (!(t[i] = tensor(a[i])) || !t[i]->is_cuda()) NVJ_NONE();
+  const int device = t[2]->get_device();
+  for (const at::Tensor* x : t)
+    if (!meta(*x, device)) NVJ_NONE();
+  const long long bs = PyLong_AsLongLong(a[5]), bucket = PyLong_AsLongLong(a[6]);
+  if (PyErr_Occurred()) { PyErr_Clear(); NVJ_NONE(); }
+  const at::Tensor &cached = *t[0], &fresh = *t[1], &tab = *t[2], &list = *t[3], &head = *t[4];
+  if (tab.dim() != 2 || cached.dim() != 1 || cached.size(0) != tab.size(0) || fresh.sizes() != cached.sizes() || list.dim() != 1 || head.dim() != 1 ||
+      head.size(0) != 1 || bs < 1 || bs > 0x7fffffff || bucket < 0 || bucket > 0x3fffffff)
+    NVJ_NONE();
+  const long long rows = tab.size(0);
+  const c10::cuda::OptionalCUDAGuard guard(c10::Device(c10::kCUDA, (c10::DeviceIndex)device));
+  void* stream = stream_of(device);
+  int32_t* st = status_for(device, stream);
+  if (!st) return nullptr;
+  // one allocation: the token arrays, each from a 16-byte boundary on, then head, lengths and query_start_loc
+  const long long pitch = (bucket + 3) / 4 * 4, rest = 3 * pitch;
+  const at::Tensor flat = empty({rest + 2 * rows + 2}, at::kInt, device);
+  at::Tensor out[6] = {flat.as_strided({1, bucket}, {bucket, 1}, 0), flat.as_strided({1, bucket}, {bucket, 1}, pitch),
+                       flat.as_strided({1, bucket}, {bucket, 1}, 2 * pitch), flat.as_strided({rows + 1}, {1}, rest + 1 + rows),
+                       flat.as_strided({rows}, {1}, rest + 1), flat.as_strided({1}, {1}, rest)};
+  int32_t* at = static_cast<int32_t*>(flat.data_ptr());
+  int rc;
+  NVJ_CALL(rc, lib.packed_layout(i32(cached), i32(fresh), (int)rows, static_cast<int32_t*>(tab.data_ptr()), (int)tab.size(1), (int)bs, i32(list),
+                                 (int)list.numel(), i32(head), (int)bucket, at, at + pitch, at + 2 * pitch, at + rest + 1 + rows,
+                                 at + rest + 1, at + rest, st, stream));
+  if (!finished(rc, "nvj_build_packed_layout", device, stream, false, true)) return nullptr;
+  PyObject* r = PyTuple_New(6);
+  if (!r) return nullptr;
+  for (int i = 0; i < 6; ++i) PyTuple_SET_ITEM(r, i, THPVariable_Wrap(std::move(out[i])));
+  return r;
 }
 
 // norm_rope(query, k, v, q_weight, k_weight, positions, slot_mapping, k_layer, v_layer, query_start_loc | None, packed, eps,
@@ -1100,6 +1279,12 @@ PyObject* init(PyObject*, PyObject* args) {
   get(lib.copy_blocks, "nvj_copy_blocks");
   get(lib.snapshot, "nvj_hybrid_snapshot_host_slots");
   get(lib.restore, "nvj_hybrid_restore_host_slots");
+  get(lib.quantized_append, "nvj_kv_append_quantized");
+  get(lib.quantized_decode, "nvj_paged_decode_quantized");
+  get(lib.quantized_decode_bytes, "nvj_paged_decode_quantized_workspace_bytes");
+  get(lib.quantized_prefill, "nvj_paged_prefill_quantized");
+  get(lib.quantized_prefill_bytes, "nvj_paged_prefill_quantized_workspace_bytes");
+  get(lib.packed_layout, "nvj_build_packed_layout");
   if (missing) {
     PyErr_Format(PyExc_ImportError, "libnvj_b200.so does not export %s", missing);
     return nullptr;
@@ -1166,6 +1351,10 @@ PyMethodDef methods[] = {
     NVJ_FAST(pack_batch, "a batch's lists on the device"),
     NVJ_FAST(slot_mapping, "flat cache slots of positions, or None"),
     NVJ_FAST(prefill_slots, "flat cache slots of a prefill batch and its shape, or None"),
+    NVJ_FAST(quantized_append, "append to the 8-bit cache, or None"),
+    NVJ_FAST(quantized_decode, "decode attention over the 8-bit cache, or None"),
+    NVJ_FAST(quantized_prefill, "ragged packed attention over the 8-bit cache, or None"),
+    NVJ_FAST(packed_layout, "a packed step's arrays from its rows' lengths, or None"),
     {"init", init, METH_VARARGS, "resolve the library's entry points and keep the callbacks"},
     {"set_workspace", set_workspace, METH_VARARGS, "hand over a (device, stream)'s workspace"},
     {"set_status_word", set_status_word, METH_VARARGS, "hand over a (device, stream)'s status word"},

@@ -5,12 +5,12 @@
 //   first[r] = head + need[0] + .. + need[r - 1]          block_tables[r][ceil(cached[r] / bs) + j] = free_blocks[first[r] + j]
 //   qsl[r]   = new[0] + .. + new[r - 1]                   token qsl[r] + t: position cached[r] + t, slot from the table entry
 //
-// One launch.  Every CTA adds up the lengths itself (thread i the rows 32 at a time of its share, then a scan over the threads'
-// sums), which costs a CTA one trip to memory for up to a few thousand rows and spares a grid-wide wait, and keeps both
-// prefixes in shared memory; then it writes its share of the tokens and of the rows.  A token's row is found by bisection there.
+// One launch.  Every CTA adds up the lengths itself (a thread consecutive rows, then a scan over the threads' sums), which costs
+// one trip to memory for up to a few thousand rows and spares a grid-wide wait, and keeps both prefixes in shared memory; then it writes
+// its share of the tokens and of the rows.  A thread writes four tokens in a row: it finds the first one's row by bisection and walks on.
 // A slot comes from the free list or from the old part of the table, never from an entry that another CTA is writing, so no
 // order between CTAs is needed.
-// The kernel is bound by latency (two dependent trips) up to ~10^5 tokens; 12 bytes per token are written.
+// Bound by latency: the trip for the lengths, the scan, the trip for the table entries, the stores (12 bytes per token).
 
 #include "nvj_common.cuh"
 
@@ -33,39 +33,82 @@ struct LayoutParams {
 };
 
 constexpr int kLayoutThreads = 512;
+constexpr int kLayoutHeld = 8;  // rows that a thread keeps in registers between the two looks at them
 
-// Row r's cached and new tokens; a row that its table has no room for, or a negative length, is flagged and gets nothing.
-__device__ __forceinline__ int2 layout_row(const LayoutParams& p, int r, int* bad) {
-  int c = p.cached_lens[r], n = p.new_lens[r];
-  if (c < 0 || n < 0 || (long long)c + n > (long long)p.table_width * p.block_size) {
+__device__ __forceinline__ int layout_blocks(int tokens, int bs) { return (int)(((long long)tokens + bs - 1) / bs); }
+// A row's cached and new tokens; a row that its table has no room for, or a negative length, is flagged and gets nothing.
+__device__ __forceinline__ int2 layout_row(const LayoutParams& p, int c, int n, int* bad) {
+  const long long most = (long long)p.table_width * p.block_size;
+  if (c < 0 || n < 0 || (long long)c + n > most) {
     *bad = 1;
     n = 0;
-    const long long most = (long long)p.table_width * p.block_size;
     c = c < 0 ? 0 : (c > most ? (int)most : c);
   }
   return make_int2(c, n);
 }
-__device__ __forceinline__ int layout_blocks(int tokens, int bs) { return (int)(((long long)tokens + bs - 1) / bs); }
+// The last i < n with from[i] <= x.
+__device__ __forceinline__ int layout_find(const int* from, int n, int x) {
+  int lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (from[mid] <= x) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
 
 __global__ void __launch_bounds__(kLayoutThreads) packed_layout_kernel(LayoutParams p) {
-  pdl_wait();
-  pdl_release();
   extern __shared__ int layout_smem[];
-  int* qsl = layout_smem;               // [rows + 1]
-  int* first = layout_smem + p.rows + 1;  // [rows + 1], from 0
+  int* qsl = layout_smem;           // [rows + 1]
+  int* first = qsl + p.rows + 1;    // [rows + 1], from 0
+  int* cached = first + p.rows + 1;  // [rows]
   __shared__ int2 sums[kLayoutThreads / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  pdl_wait();
+  pdl_release();
   const int head = *p.free_head;
-  const int per = (p.rows + kLayoutThreads - 1) / kLayoutThreads;  // consecutive rows of a thread
+  int per = (p.rows + kLayoutThreads - 1) / kLayoutThreads;  // consecutive rows of a thread
+  const bool wide = per > 1 && ((reinterpret_cast<uintptr_t>(p.cached_lens) | reinterpret_cast<uintptr_t>(p.new_lens)) & 15) == 0;
+  if (wide) per = (per + 3) & ~3;  // four rows per load
+  int c[kLayoutHeld], n[kLayoutHeld];
   int bad = 0;
-  int2 mine = make_int2(0, 0);
-  for (int k = 0; k < per; ++k) {
-    const int r = tid * per + k;
-    if (r < p.rows) {
-      const int2 cn = layout_row(p, r, &bad);
-      mine.x += cn.y;
-      mine.y += layout_blocks(cn.x + cn.y, p.block_size) - layout_blocks(cn.x, p.block_size);
+  if (wide) {
+#pragma unroll
+    for (int k = 0; k < kLayoutHeld; k += 4) {
+      const int r = tid * per + k;
+      if (k < per && r + 4 <= p.rows) {
+        const int4 x = *reinterpret_cast<const int4*>(p.cached_lens + r), y = *reinterpret_cast<const int4*>(p.new_lens + r);
+        c[k] = x.x; c[k + 1] = x.y; c[k + 2] = x.z; c[k + 3] = x.w;
+        n[k] = y.x; n[k + 1] = y.y; n[k + 2] = y.z; n[k + 3] = y.w;
+      } else {
+#pragma unroll
+        for (int e = k; e < k + 4; ++e) {
+          const bool there = e < per && tid * per + e < p.rows;
+          c[e] = there ? p.cached_lens[tid * per + e] : 0;
+          n[e] = there ? p.new_lens[tid * per + e] : 0;
+        }
+      }
     }
+  } else {
+#pragma unroll
+    for (int k = 0; k < kLayoutHeld; ++k) {
+      const bool there = k < per && tid * per + k < p.rows;
+      c[k] = there ? p.cached_lens[tid * per + k] : 0;
+      n[k] = there ? p.new_lens[tid * per + k] : 0;
+    }
+  }
+  auto fresh_blocks = [&](int2 cn) { return layout_blocks(cn.x + cn.y, p.block_size) - layout_blocks(cn.x, p.block_size); };
+  int2 mine = make_int2(0, 0);
+#pragma unroll
+  for (int k = 0; k < kLayoutHeld; ++k) {
+    const int2 cn = layout_row(p, c[k], n[k], &bad);
+    mine.x += cn.y;
+    mine.y += fresh_blocks(cn);
+  }
+  for (int k = kLayoutHeld; k < per && tid * per + k < p.rows; ++k) {
+    const int2 cn = layout_row(p, p.cached_lens[tid * per + k], p.new_lens[tid * per + k], &bad);
+    mine.x += cn.y;
+    mine.y += fresh_blocks(cn);
   }
   int2 upto = mine;  // inclusive over the warp
 #pragma unroll
@@ -75,23 +118,27 @@ __global__ void __launch_bounds__(kLayoutThreads) packed_layout_kernel(LayoutPar
   }
   if (lane == 31) sums[warp] = upto;
   __syncthreads();
-  if (p.rows == 0 && tid == 0) qsl[0] = first[0] = 0;
   int2 at = make_int2(upto.x - mine.x, upto.y - mine.y);
-  for (int w = 0; w < warp; ++w) at.x += sums[w].x, at.y += sums[w].y;
-  for (int k = 0; k < per; ++k) {
-    const int r = tid * per + k;
-    if (r < p.rows) {
-      int unused = 0;
-      const int2 cn = layout_row(p, r, &unused);
-      qsl[r] = at.x;
-      first[r] = at.y;
-      at.x += cn.y;
-      at.y += layout_blocks(cn.x + cn.y, p.block_size) - layout_blocks(cn.x, p.block_size);
-    }
+#pragma unroll
+  for (int w = 0; w < kLayoutThreads / 32; ++w)
+    if (w < warp) at.x += sums[w].x, at.y += sums[w].y;
+  if (p.rows == 0 && tid == 0) qsl[0] = first[0] = 0;
+  auto leave = [&](int r, int2 cn) {
+    qsl[r] = at.x;
+    first[r] = at.y;
+    cached[r] = cn.x;
+    at.x += cn.y;
+    at.y += fresh_blocks(cn);
     if (r == p.rows - 1) qsl[p.rows] = at.x, first[p.rows] = at.y;
-  }
+  };
+  int unused = 0;
+#pragma unroll
+  for (int k = 0; k < kLayoutHeld; ++k)
+    if (k < per && tid * per + k < p.rows) leave(tid * per + k, layout_row(p, c[k], n[k], &unused));
+  for (int k = kLayoutHeld; k < per && tid * per + k < p.rows; ++k)
+    leave(tid * per + k, layout_row(p, p.cached_lens[tid * per + k], p.new_lens[tid * per + k], &unused));
   __syncthreads();
-  const int total = qsl[p.rows];
+  const int total = qsl[p.rows], blocks = first[p.rows];
   const long long threads = (long long)gridDim.x * kLayoutThreads, me = (long long)blockIdx.x * kLayoutThreads + tid;
   // An id from the list, -1 past its end (a slot or table entry that the kernels downstream flag and skip).
   auto taken = [&](long long k) {
@@ -99,55 +146,66 @@ __global__ void __launch_bounds__(kLayoutThreads) packed_layout_kernel(LayoutPar
     return i >= 0 && i < p.free_count ? p.free_blocks[i] : -1;
   };
   if (blockIdx.x == 0) {
-    for (int r = tid; r <= p.rows; r += kLayoutThreads) p.query_start_loc[r] = qsl[r];
     if (tid == 0) {
-      *p.free_head_out = head + first[p.rows];
+      *p.free_head_out = head + blocks;
       if (total > p.token_bucket) bad = 1;
-      if (first[p.rows] > 0 && (head < 0 || (long long)head + first[p.rows] > p.free_count)) atomicOr(p.status, NVJ_DEV_BAD_BLOCK_ID);
+      if (blocks > 0 && (head < 0 || (long long)head + blocks > p.free_count)) atomicOr(p.status, NVJ_DEV_BAD_BLOCK_ID);
     }
     if (bad) atomicOr(p.status, NVJ_DEV_BAD_LENGTH);
   }
-  for (long long i = me; i < p.token_bucket; i += threads) {
-    int row = 0, position = 0, slot = -1;
-    if (i < total) {
-      int lo = 0, hi = p.rows - 1;  // the last row with qsl[row] <= i
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (qsl[mid] <= i) lo = mid;
-        else hi = mid - 1;
+  const bool vector = ((reinterpret_cast<uintptr_t>(p.positions) | reinterpret_cast<uintptr_t>(p.token_row_ids) |
+                        reinterpret_cast<uintptr_t>(p.slot_mapping)) & 15) == 0;
+  for (long long i0 = 4 * me; i0 < p.token_bucket; i0 += 4 * threads) {
+    int position[4], row[4], slot[4];
+    int r = i0 < total ? layout_find(qsl, p.rows, (int)i0) : 0, held = 0, block = -1, id = -1;  // of the token in front
+    bool begun = false;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const long long i = i0 + e;
+      position[e] = row[e] = 0;
+      slot[e] = -1;
+      if (i < total) {
+        bool moved = !begun;
+        while (i >= qsl[r + 1]) ++r, moved = true;
+        if (moved) held = layout_blocks(cached[r], p.block_size), block = -1;
+        begun = true;
+        row[e] = r;
+        position[e] = cached[r] + (int)(i - qsl[r]);
+        const int b = position[e] / p.block_size;
+        if (b != block) {
+          block = b;
+          id = b < held ? p.block_tables[(long long)r * p.table_width + b] : taken(first[r] + (b - held));
+        }
+        if (id >= 0) slot[e] = id * p.block_size + (position[e] - b * p.block_size);
       }
-      row = lo;
-      int unused = 0;
-      const int c = layout_row(p, row, &unused).x, held = layout_blocks(c, p.block_size);
-      position = c + (int)(i - qsl[row]);
-      const int b = position / p.block_size;
-      const int id = b < held ? p.block_tables[(long long)row * p.table_width + b] : taken(first[row] + (b - held));
-      slot = id < 0 ? -1 : id * p.block_size + (position - b * p.block_size);
     }
-    p.positions[i] = position;
-    p.token_row_ids[i] = row;
-    p.slot_mapping[i] = slot;
-  }
-  for (long long r = me; r < p.rows; r += threads) {
-    int unused = 0;
-    const int2 cn = layout_row(p, (int)r, &unused);
-    p.seq_lens[r] = cn.x + cn.y;
-  }
-  // the new table entries, one per thread: entry k of all of them belongs to the last row with first[row] <= k
-  for (long long k = me; k < first[p.rows]; k += threads) {
-    int lo = 0, hi = p.rows - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (first[mid] <= k) lo = mid;
-      else hi = mid - 1;
+    if (vector && i0 + 4 <= p.token_bucket) {
+      *reinterpret_cast<int4*>(p.positions + i0) = make_int4(position[0], position[1], position[2], position[3]);
+      *reinterpret_cast<int4*>(p.token_row_ids + i0) = make_int4(row[0], row[1], row[2], row[3]);
+      *reinterpret_cast<int4*>(p.slot_mapping + i0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (i0 + e < p.token_bucket) {
+          p.positions[i0 + e] = position[e];
+          p.token_row_ids[i0 + e] = row[e];
+          p.slot_mapping[i0 + e] = slot[e];
+        }
     }
-    int unused = 0;
-    const int held = layout_blocks(layout_row(p, lo, &unused).x, p.block_size);
-    p.block_tables[(long long)lo * p.table_width + held + (int)(k - first[lo])] = taken(k);
+  }
+  for (long long r = me; r <= p.rows; r += threads) {
+    p.query_start_loc[r] = qsl[r];
+    if (r < p.rows) p.seq_lens[r] = cached[r] + (qsl[r + 1] - qsl[r]);
+  }
+  // the new table entries: entry k of all of them belongs to the last row with first[row] <= k
+  for (long long k = me; k < blocks; k += threads) {
+    const int r = layout_find(first, p.rows, (int)k);
+    p.block_tables[(long long)r * p.table_width + layout_blocks(cached[r], p.block_size) + (int)(k - first[r])] = taken(k);
   }
 }
 
-constexpr int kLayoutMaxRows = 16384;  // two prefixes of so many rows in shared memory
+constexpr int kLayoutMaxRows = 16384;  // two prefixes and a length of so many rows in shared memory
+constexpr int layout_smem_bytes(int rows) { return (3 * rows + 2) * (int)sizeof(int); }
 
 }  // namespace nvj
 
@@ -165,19 +223,18 @@ extern "C" int nvj_build_packed_layout(const int32_t* cached_lens, const int32_t
   if (rows > 0 && (!cached_lens || !new_lens || !seq_lens || (table_width > 0 && !block_tables))) return NVJ_ERR_INVALID_ARGUMENT;
   if (free_count > 0 && !free_blocks) return NVJ_ERR_INVALID_ARGUMENT;
   if (token_bucket > 0 && (!positions || !token_row_ids || !slot_mapping)) return NVJ_ERR_INVALID_ARGUMENT;
-  const int smem = 2 * (rows + 1) * (int)sizeof(int);
   static PerDeviceFlags ready;
   if (!once_per_device(ready, [&](int) {
         return cudaFuncSetAttribute(packed_layout_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    2 * (kLayoutMaxRows + 1) * (int)sizeof(int)) == cudaSuccess;
+                                    layout_smem_bytes(kLayoutMaxRows)) == cudaSuccess;
       }))
     return NVJ_ERR_LAUNCH;
   LayoutParams p{cached_lens, new_lens, block_tables, free_blocks, free_head, positions, token_row_ids, slot_mapping, query_start_loc,
                  seq_lens, free_head_out, status, rows, table_width, block_size, free_count, token_bucket};
-  const long long work = token_bucket > rows ? token_bucket : rows;
+  const long long work = token_bucket / 4 > rows ? token_bucket / 4 : rows;
   long long ctas = (work + kLayoutThreads - 1) / kLayoutThreads;
   ctas = ctas < 1 ? 1 : (ctas > 148 ? 148 : ctas);
-  return launch_after(packed_layout_kernel, dim3((unsigned)ctas), dim3(kLayoutThreads), (size_t)smem, static_cast<cudaStream_t>(stream), p) ==
+  return launch_after(packed_layout_kernel, dim3((unsigned)ctas), dim3(kLayoutThreads), (size_t)layout_smem_bytes(rows), static_cast<cudaStream_t>(stream), p) ==
                  cudaSuccess
              ? NVJ_OK
              : NVJ_ERR_LAUNCH;

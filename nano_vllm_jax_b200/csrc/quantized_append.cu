@@ -132,27 +132,25 @@ __device__ void q_append_run(const QAppendParams& p, int first, int n, long long
     if (s * kRows + sub < n) store(s * kRows + sub, q_load8(src + (long long)(s * kRows + sub) * token_stride));
 }
 
-// Grid x: windows of `window` tokens; grid y: 2 * num_kv_heads (K, V of each head).  A window's warps take the runs that begin in it
-// in turn.
+// Grid x: windows of `window` tokens; grid y: the (K or V, head) pairs, a warp each.  A warp takes the runs that begin in its window one
+// behind the other.
 constexpr int kQAppendWarps = 4;
 template <typename T, int kD>
 __global__ void __launch_bounds__(32 * kQAppendWarps) quantized_append_kernel(QAppendParams p, int window) {
   pdl_wait();
   pdl_release();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int task = window == 1 ? blockIdx.x * kQAppendWarps + warp : blockIdx.x;
-  const int base = task * window;  // first token of the window
-  if (base >= p.n_tokens) return;
-  const int head = blockIdx.y >> 1;
-  const bool is_v = blockIdx.y & 1;
+  const int lane = threadIdx.x & 31, part = blockIdx.y * kQAppendWarps + (threadIdx.x >> 5);
+  const int base = blockIdx.x * window;  // first token of the window
+  const int head = part >> 1;
+  const bool is_v = part & 1;
+  if (head >= p.num_kv_heads) return;
   // lane l looks at token base - 1 + l: the one in front tells whether the window's first token begins a run
   const QToken t = q_token(p, base - 1 + lane);
   const long long in_front = __shfl_up_sync(kFullMask, t.entry, 1);
   const bool same = lane > 0 && t.entry >= 0 && t.entry == in_front;
   const unsigned chain = __ballot_sync(kFullMask, same);
   unsigned starts = __ballot_sync(kFullMask, lane > 0 && lane <= window && t.entry >= 0 && !same);
-  for (int k = 0; starts; ++k, starts &= starts - 1) {
-    if (window > 1 && k % kQAppendWarps != warp) continue;
+  for (; starts; starts &= starts - 1) {
     const int at = __ffs(starts) - 1;  // lane of the run's first token
     const long long entry = __shfl_sync(kFullMask, t.entry, at);
     const int first = base - 1 + at;
@@ -173,10 +171,11 @@ __global__ void __launch_bounds__(32 * kQAppendWarps) quantized_append_kernel(QA
 
 template <typename T>
 static int launch_quantized_append(const QAppendParams& p, int head_dim, cudaStream_t stream) {
-  // A token per warp while the warps find a place at once, 16 tokens per CTA beyond: see the launch below.
-  const int window = (long long)p.n_tokens * p.num_kv_heads * 2 <= 148LL * 64 ? 1 : 16;
-  const int per = window == 1 ? kQAppendWarps : window;
-  const dim3 grid((p.n_tokens + per - 1) / per, 2 * p.num_kv_heads);
+  // Batches of a few tokens per row: a run per window.  Prompts: windows of 16 tokens, in which one run begins, mostly (a window per token: 37 us
+  // for 16384 tokens, most of it warps that find nothing to do).
+  const long long rows = p.packed ? p.qsl_rows : (p.n_tokens + p.n_cols - 1) / p.n_cols;
+  const int window = p.n_tokens <= 4 * (rows > 0 ? rows : 1) ? 1 : 16;
+  const dim3 grid((p.n_tokens + window - 1) / window, (2 * p.num_kv_heads + kQAppendWarps - 1) / kQAppendWarps);
   auto go = [&](auto* kernel) {
     return launch_after(kernel, grid, dim3(32 * kQAppendWarps), 0, stream, p, window) == cudaSuccess ? NVJ_OK : NVJ_ERR_LAUNCH;
   };

@@ -438,13 +438,24 @@ constexpr long long kQMostPages = 32768;  // (rows among them: the grid's y)
 
 }  // namespace nvj
 
-extern "C" size_t nvj_paged_prefill_quantized_workspace_bytes(int q_dtype, int rows, int table_width, int block_size, int num_kv_heads,
-                                                              int head_dim, int num_q_heads, float scale) {
-  using namespace nvj;
-  if (rows <= 0 || table_width <= 0 || !quantized_unpacks(q_dtype, block_size, num_kv_heads, head_dim, num_q_heads, scale)) return 0;
+namespace nvj {
+// Bytes of a batch's pages, 0 where there are none.
+static size_t quantized_page_bytes(int q_dtype, int rows, int table_width, int block_size, int num_kv_heads, int head_dim, int num_q_heads, float scale) {
   const long long pages = (long long)rows * table_width;
-  if (pages > kQMostPages) return 0;
+  if (pages <= 0 || pages > kQMostPages || !quantized_unpacks(q_dtype, block_size, num_kv_heads, head_dim, num_q_heads, scale)) return 0;
   return (size_t)(pages * 2 * block_size * num_kv_heads * head_dim * 2 + (pages * 4 + 255) / 256 * 256);
+}
+}  // namespace nvj
+
+// The scratch serves the decode kernel's partials and then the pages, one launch behind the other.
+extern "C" size_t nvj_paged_prefill_quantized_workspace_bytes(int q_dtype, int rows, int table_width, int block_size, int num_kv_heads,
+                                                              int head_dim, int num_q_heads, float scale, int single_rows) {
+  using namespace nvj;
+  if (rows <= 0 || table_width <= 0) return 0;
+  const size_t pages = quantized_page_bytes(q_dtype, rows, table_width, block_size, num_kv_heads, head_dim, num_q_heads, scale);
+  const size_t partials =
+      single_rows == 0 ? 0 : nvj_paged_decode_quantized_workspace_bytes(rows, 1, table_width, block_size, num_kv_heads, head_dim, num_q_heads, 0);
+  return pages > partials ? pages : partials;
 }
 
 extern "C" int nvj_paged_prefill_quantized(const void* q, int q_dtype, const void* k_cache_layer, const void* v_cache_layer,
@@ -466,15 +477,13 @@ extern "C" int nvj_paged_prefill_quantized(const void* q, int q_dtype, const voi
     return NVJ_ERR_TOO_LARGE;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int skip_single = single_rows != 0;
-  // the workspace is used twice, one launch behind the other: by the decode kernel's partials and then for the pages
   if (skip_single && rows > 0) {
     const int rc = nvj_paged_decode_quantized(q, q_dtype, k_cache_layer, v_cache_layer, k_scale, v_scale, num_blocks, block_size, num_kv_heads,
                                               head_dim, num_q_heads, block_tables, table_width, kv_lens, positions, query_start_loc, rows, 1,
                                               scale, out, status, workspace, workspace_bytes, 0, stream);
     if (rc != NVJ_OK) return rc;
   }
-  const size_t needed =
-      nvj_paged_prefill_quantized_workspace_bytes(q_dtype, rows, table_width, block_size, num_kv_heads, head_dim, num_q_heads, scale);
+  const size_t needed = quantized_page_bytes(q_dtype, rows, table_width, block_size, num_kv_heads, head_dim, num_q_heads, scale);
   if (needed > 0 && workspace && workspace_bytes >= needed && aligned16(workspace)) {
     const long long pages = (long long)rows * table_width, page_bytes = 2LL * block_size * num_kv_heads * head_dim;
     QUnpackParams u{};

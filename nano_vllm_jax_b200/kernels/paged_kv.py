@@ -275,6 +275,9 @@ def build_packed_layout(cached_lens, new_lens, block_tables, free_blocks, free_h
     list suffices, and a list that ends too early, a row without room or a bucket too small is flagged on the device
     (`check_device_status`).
     """
+    made = host().packed_layout(cached_lens, new_lens, block_tables, free_blocks, free_head, block_size, token_bucket)
+    if made is not None:
+        return PackedLayout._make(made)
     named = (("cached_lens", cached_lens), ("new_lens", new_lens), ("block_tables", block_tables), ("free_blocks", free_blocks),
              ("free_head", free_head))
     for name, t in named:
@@ -291,10 +294,11 @@ def build_packed_layout(cached_lens, new_lens, block_tables, free_blocks, free_h
         raise ValueError("block_size must be positive and token_bucket not negative")
     rows, width = block_tables.shape
     device = block_tables.device
-    # one allocation: the three token arrays, then head, lengths and query_start_loc
-    flat = torch.empty(3 * bucket + 2 * rows + 2, dtype=torch.int32, device=device)
-    positions, ids, slots, rest = flat.split((bucket, bucket, bucket, 2 * rows + 2))
-    head, lens, qsl = rest.split((1, rows, rows + 1))
+    # one allocation: the token arrays, each from a 16-byte boundary on, then head, lengths and query_start_loc
+    pitch = -(-bucket // 4) * 4
+    flat = torch.empty(3 * pitch + 2 * rows + 2, dtype=torch.int32, device=device)
+    positions, ids, slots, head, lens, qsl = flat.split((pitch, pitch, pitch, 1, rows, rows + 1))
+    positions, ids, slots = positions[:bucket], ids[:bucket], slots[:bucket]
     with torch.cuda.device(device):
         st = _status_word(device)
         check(_lib.load().nvj_build_packed_layout(

@@ -84,6 +84,9 @@ def kv_append_quantized(new_k, new_v, k_cache_layer, v_cache_layer, k_scale, v_s
     `paged_kv.kv_append_slots`; rows with `seq_lens` <= 0, where given, are left alone.  The tokens that fall into one block
     stand together in the batch, as a row's consecutive positions do.
     """
+    if _k.host().quantized_append(new_k, new_v, k_cache_layer, v_cache_layer, k_scale, v_scale, positions, block_table, query_start_loc,
+                                  token_row_ids, seq_lens):
+        return k_cache_layer, v_cache_layer, k_scale, v_scale
     pages, page_size, hkv, d = _cache(k_cache_layer, v_cache_layer, k_scale, v_scale)
     device = k_cache_layer.device
     if new_k.ndim != 4 or new_k.shape != new_v.shape or tuple(new_k.shape[2:]) != (hkv, d):
@@ -136,6 +139,9 @@ def paged_decode_attention_quantized(q, k_cache_layer, v_cache_layer, k_scale, v
     with `positions` `[B, T]`, p <= positions[b, t]; one that sees none gives zeros.  `form`: 0 automatic, 1 mma.sync tiles on
     thread-block clusters, 2 tcgen05 tiles (head_dim 128 or 256).
     """
+    out = _k.host().quantized_decode(q, k_cache_layer, v_cache_layer, k_scale, v_scale, block_table, seq_lens, scale, positions, form)
+    if out is not None:
+        return out
     pages, page_size, hkv, d = _cache(k_cache_layer, v_cache_layer, k_scale, v_scale)
     device = k_cache_layer.device
     if q.ndim not in (3, 4):
@@ -185,6 +191,10 @@ def packed_paged_prefill_attention_quantized(query, k_cache_layer, v_cache_layer
     rows) as in `paged_kv.packed_paged_prefill_attention`.  bfloat16 queries of the model's shape run on the tcgen05 tiles over bf16
     pages written for the call (exact; up to 1 GiB, from torch's allocator), others on mma.sync tiles over the 8-bit blocks.
     """
+    out = _k.host().quantized_prefill(query, k_cache_layer, v_cache_layer, k_scale, v_scale, block_table, kv_lens, positions, query_start_loc,
+                                      block_size, scale, num_key_value_groups, num_decode_rows, query_tile_pairs)
+    if out is not None:
+        return out
     pages, page_size, hkv, d = _cache(k_cache_layer, v_cache_layer, k_scale, v_scale)
     device = k_cache_layer.device
     if query.ndim != 4 or query.shape[0] != 1:
@@ -213,7 +223,7 @@ def packed_paged_prefill_attention_quantized(query, k_cache_layer, v_cache_layer
     singles = -1 if num_decode_rows is None else int(num_decode_rows)
     pairs = -1 if query_tile_pairs is None else int(query_tile_pairs)
     with _on(device):
-        nbytes = lib.nvj_paged_prefill_quantized_workspace_bytes(_k._dt(query), rows, width, page_size, hkv, d, hq, float(scale))
+        nbytes = lib.nvj_paged_prefill_quantized_workspace_bytes(_k._dt(query), rows, width, page_size, hkv, d, hq, float(scale), singles)
         scratch = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
         st = _k._status_word(device)
         check(lib.nvj_paged_prefill_quantized(

@@ -85,10 +85,10 @@ def test_calls_with_nothing_to_do_launch_nothing():
 def test_scratch_of_a_prefill():
     size = _lib.load().nvj_paged_prefill_quantized_workspace_bytes
     page = 16 * 2 * 256 * 2
-    assert size(0, 3, 100, 16, 2, 256, 8, 0.1) == 300 * 2 * page + 1280
-    assert size(0, 1, 32768, 16, 2, 256, 8, 0.1) > 0 and size(0, 1, 32769, 16, 2, 256, 8, 0.1) == 0  # at most 1 GiB
+    assert size(0, 3, 100, 16, 2, 256, 8, 0.1, 0) == 300 * 2 * page + 1280
+    assert size(0, 1, 32768, 16, 2, 256, 8, 0.1, 0) > 0 and size(0, 1, 32769, 16, 2, 256, 8, 0.1, 0) == 0  # at most 1 GiB
     for other in ((1, 16, 2, 256, 8, 0.1), (2, 16, 2, 256, 8, 0.1), (0, 32, 2, 256, 8, 0.1), (0, 16, 2, 128, 8, 0.1), (0, 16, 2, 256, 8, 0.0)):
-        assert size(other[0], 3, 100, *other[1:]) == 0
+        assert size(other[0], 3, 100, *other[1:], 0) == 0
 
 
 def test_wrappers_refuse_tensors_that_are_not_on_a_gpu():
