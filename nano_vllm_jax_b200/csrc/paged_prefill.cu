@@ -20,7 +20,7 @@ int launch_prefill_umma2(const void* q, int q_dtype, const char* k_cache, const 
                          const int32_t* kv_lens, const int32_t* positions, const int32_t* query_start_loc,
                          int rows, int token_bucket, float scale, float* out, int32_t* status,
                          int skip_single, int split_p, int tile_pairs, bool may_split, int32_t* beside,
-                         cudaStream_t stream);
+                         bool flush, cudaStream_t stream);
 bool prefill_umma2_usable(float scale, long long num_blocks);
 int launch_prefill_umma(const void* q, int q_dtype, const char* k_cache, const char* v_cache,
                         long long num_blocks, const int32_t* block_tables, int table_width,
@@ -40,6 +40,7 @@ struct PackedArgs {
   int rows, token_bucket; float scale; float* out; int32_t* status;
   void* workspace; size_t workspace_bytes; int variant;
   int tile_pairs = -1;  // what the caller counted on the host (-1: not told)
+  bool flush = false;   // empty the tiles' accumulators every 8192 keys (paged_prefill_umma2.cu)
 };
 
 static int check_packed(const PackedArgs& a, bool* tile_ok) {
@@ -137,7 +138,7 @@ static int run_tiles(const PackedArgs& a, int skip_single, bool may_split, int32
   if (variant == 0 || variant == 4 || variant == 5) {
     const int rc = launch_prefill_umma2(a.q, a.q_dtype, kc, vc, a.num_blocks, a.block_tables, a.table_width, a.kv_lens, a.positions,
                                         a.query_start_loc, a.rows, a.token_bucket, a.scale, a.out, a.status, skip_single,
-                                        variant == 5 ? 0 : 1, a.tile_pairs, may_split, beside, s);
+                                        variant == 5 ? 0 : 1, a.tile_pairs, may_split, beside, a.flush, s);
     if (rc != NVJ_ERR_UNSUPPORTED || variant != 0) return rc;
   }
   if (variant == 0 || variant == 3) {
@@ -231,6 +232,17 @@ static int run_packed(const PackedArgs& a, int part, int cta_limit, cudaStream_t
   return run_tiles(a, skip_single, !skip_single, nullptr, s);
 }
 
+}  // namespace nvj
+
+namespace nvj {
+// The query tiles over the bf16 pages of an 8-bit cache (quantized_prefill.cu): part 2 or 3 of a batch on CTA pairs.
+int prefill_over_pages(const void* q, const void* k_pages, const void* v_pages, long long pages, const int32_t* page_tables, int table_width,
+                       const int32_t* kv_lens, const int32_t* positions, const int32_t* query_start_loc, int rows, int token_bucket, float scale,
+                       float* out, int32_t* status, void* workspace, size_t workspace_bytes, int part, int tile_pairs, cudaStream_t stream) {
+  return run_packed(PackedArgs{q, NVJ_BF16, k_pages, v_pages, NVJ_BF16, pages, kBlk, kHkv, kD, kHq, page_tables, table_width, kv_lens, positions,
+                               query_start_loc, rows, token_bucket, scale, out, status, workspace, workspace_bytes, 4, tile_pairs, true},
+                    part, 0, stream);
+}
 }  // namespace nvj
 
 #define NVJ_PACKED_PARAMS                                                                                                   \

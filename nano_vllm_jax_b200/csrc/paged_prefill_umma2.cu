@@ -84,6 +84,12 @@ struct Umma2Params {
   int pair_slots;  // CTA pairs that run at once
 };
 
+// With kFlush (the pages of an 8-bit cache): tiles of 64 keys after which the output accumulators are emptied into the
+// output rows.  The tensor cores cut the last place of what they add to: 1.2e-5 of a sum over 16384 keys left alone,
+// 9.4e-6 emptied each 128 tiles, 6.6e-6 each 64, 5.8e-6 each 32, for 1140, 1192, 1213 and 1541 us.  Even: the same
+// softmax group empties every time.
+constexpr int kU2FlushTiles = 64;
+
 struct Umma2Smem {
   alignas(1024) char k[kU2Stages][2][8192];  // [stage][this CTA's two blocks][8-key group][64-d chunk][8 keys][128 B]
   alignas(1024) char v[kU2Stages][4][4096];  // [stage][block][8-key group][this CTA's two 64-d chunks][8 keys][128 B]
@@ -98,6 +104,7 @@ struct Umma2Smem {
   // of token t stored at (piece ^ (t & 7)) so that both the row-wise fill and the token-wise read are conflict-free
   alignas(16) char qstage[kU2Tokens * kG * kD * 2];
   float2 own_ml[kU2Rows];  // this split's (max, sum) per row, for the fold
+  float m_flushed[kU2Rows];  // the reference of what has been emptied into the output row
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -260,9 +267,10 @@ __device__ __forceinline__ void u2_mma_warp(Umma2Smem& sm, const Umma2Params& p,
 // 2050 cycles per tile.)  What stays in turn is the row's reference (the running maximum, moved only when a tile exceeds it
 // by 2^kU2RescaleGap): a group settles its tile's reference behind the other's, before its exponentials.  False when a
 // wait ran out (the caller still joins its barriers).
+template <bool kFlush>
 __device__ __forceinline__ bool u2_softmax_tiles(Umma2Smem& sm, const Umma2Params& p, uint32_t my_tmem, int tok0, int ntok,
                                                  int kv_len, int tile0, int n_tiles, int group, int r, int token, float& m_row,
-                                                 float& l_row) {
+                                                 float& l_row, float* flush_row) {
   const int my_pos = token < ntok ? p.positions[tok0 + token] : -1;
   const int last_key = my_pos < kv_len - 1 ? my_pos : kv_len - 1;
   const float scale_log2 = p.scale * kU2Log2e;
@@ -290,7 +298,38 @@ __device__ __forceinline__ bool u2_softmax_tiles(Umma2Smem& sm, const Umma2Param
     if (t > 0) {
       if (!um_wait(&sm.m_full[quarter][group ^ 1], before, &sm.abort_flag, p.status)) return false;
       m_new = sm.m_row[group ^ 1][r];
-      if (__any_sync(0xffffffffu, tmax > m_new + kU2RescaleGap)) {
+      bool flushed = false;
+      if constexpr (kFlush) {
+        if (flush_row && t % kU2FlushTiles == 0) {  // the sums so far to the output row, and the accumulators to zero
+          if (!um_wait(&sm.pv_done[group ^ 1][1], before, &sm.abort_flag, p.status)) return false;
+          tc_fence_after_sync();
+          flushed = true;
+          const float back = t > kU2FlushTiles && m_new != -INFINITY ? ex2_approx(sm.m_flushed[r] - m_new) : 0.f;
+          sm.m_flushed[r] = m_new;
+          float4* to = reinterpret_cast<float4*>(flush_row);
+#pragma unroll 1
+          for (int cc = 0; cc < kD / 32; ++cc) {
+            float o[32];
+            tmem_ld32(my_tmem + kU2ColO + cc * 32, o);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              if (token < ntok) {
+                float4 x = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                if (back != 0.f) {
+                  const float4 y = to[cc * 8 + i];
+                  x = make_float4(fmaf(y.x, back, x.x), fmaf(y.y, back, x.y), fmaf(y.z, back, x.z), fmaf(y.w, back, x.w));
+                }
+                to[cc * 8 + i] = x;
+              }
+            }
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = 0.f;
+            tmem_st32(my_tmem + kU2ColO + cc * 32, o);
+          }
+          m_new = fmaxf(m_new, tmax);
+        }
+      }
+      if (!flushed && __any_sync(0xffffffffu, tmax > m_new + kU2RescaleGap)) {
         if (!um_wait(&sm.pv_done[group ^ 1][1], before, &sm.abort_flag, p.status)) return false;
         tc_fence_after_sync();
         const float m_old = m_new;
@@ -363,6 +402,7 @@ __device__ __forceinline__ void u2_request_q(const Umma2Params& p, int tok0, int
 __device__ __forceinline__ int u2_piece(int r, int c) { return r * kD + (((c & ~7) | ((c ^ r) & 7)) << 2); }
 
 // ---- warps 2-9 of both CTAs: Q staging, softmax, epilogue for this CTA's 128 rows -------------
+template <bool kFlush>
 __device__ __forceinline__ void u2_softmax_warps(Umma2Smem& sm, const Umma2Params& p, uint32_t tmem, int tok0, int ntok,
                                                  int kvh, int kv_len, int tile0, int n_tiles, int splits, int warp, int lane,
                                                  const uint4 (&u)[4][4]) {
@@ -424,7 +464,9 @@ __device__ __forceinline__ void u2_softmax_warps(Umma2Smem& sm, const Umma2Param
     NVJ_U2_PHASE(2);
   }
   float m_row = -INFINITY, l_row = 0.f;
-  bool alive = u2_softmax_tiles(sm, p, my_tmem, tok0, ntok, kv_len, tile0, n_tiles, half, r, token, m_row, l_row);
+  // (split key ranges are short, and their output rows not this CTA's alone)
+  float* out_row = kFlush && splits == 1 && n_tiles > kU2FlushTiles ? p.out + ((long long)(tok0 + token) * kHq + kvh * kG + hl) * kD : nullptr;
+  bool alive = u2_softmax_tiles<kFlush>(sm, p, my_tmem, tok0, ntok, kv_len, tile0, n_tiles, half, r, token, m_row, l_row, out_row);
   // ---- epilogue.  From here on the softmax threads meet at CTA-wide named barriers, so a thread whose wait ran out
   // does not leave: it skips the work and everybody returns together once the barrier has made the flag visible.
   NVJ_U2_PHASE(4);
@@ -454,6 +496,19 @@ __device__ __forceinline__ void u2_softmax_warps(Umma2Smem& sm, const Umma2Param
     float o[32];
     tmem_ld32(my_tmem + kU2ColO + half * (kD / 2) + cc * 32, o);
     const int c0 = (half * (kD / 2) + cc * 32) >> 2;  // first 16-byte piece of these 32 floats within the row
+    if constexpr (kFlush) {
+      if (out_row && token < ntok) {
+        const float back = m_row == -INFINITY ? 0.f : ex2_approx(sm.m_flushed[r] - m_row);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float4 y = reinterpret_cast<const float4*>(out_row)[c0 + i];
+          o[4 * i] = fmaf(y.x, back, o[4 * i]);
+          o[4 * i + 1] = fmaf(y.y, back, o[4 * i + 1]);
+          o[4 * i + 2] = fmaf(y.z, back, o[4 * i + 2]);
+          o[4 * i + 3] = fmaf(y.w, back, o[4 * i + 3]);
+        }
+      }
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       *reinterpret_cast<float4*>(stage + r * kD + ((c0 + (i ^ (r & 7))) << 2)) =
@@ -617,6 +672,7 @@ __device__ __forceinline__ int u2_split_count(const Umma2Params& p, int n_tiles,
   return splits > 1 ? splits : 1;
 }
 
+template <bool kFlush>
 __global__ void __launch_bounds__(kU2Threads, 1)
 prefill_umma2_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
                      const Umma2Params p) {
@@ -753,7 +809,7 @@ prefill_umma2_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
 
   if (warp == 0) u2_producer(&k_map, &v_map, p, sm, row, kvh, kv_len, tile0, my_tiles, rank, lane, first_ids);
   else if (warp == 1) { if (rank == 0) u2_mma_warp(sm, p, tmem, my_tiles); }
-  else u2_softmax_warps(sm, p, tmem, tok0, ntok, kvh, kv_len, tile0, my_tiles, splits, warp, lane, qv);
+  else u2_softmax_warps<kFlush>(sm, p, tmem, tok0, ntok, kvh, kv_len, tile0, my_tiles, splits, warp, lane, qv);
 
   tc_fence_before_sync();
   __syncthreads();
@@ -808,10 +864,10 @@ static cudaLaunchConfig_t u2_config(dim3 grid, cudaStream_t stream, cudaLaunchAt
   cfg.numAttrs = 2;
   return cfg;
 }
-static cudaError_t u2_launch(dim3 grid, cudaStream_t stream, const CUtensorMap& k_map, const CUtensorMap& v_map, const Umma2Params& p) {
+static cudaError_t u2_launch(dim3 grid, cudaStream_t stream, const CUtensorMap& k_map, const CUtensorMap& v_map, const Umma2Params& p, bool flush) {
   cudaLaunchAttribute attr[2];
   const cudaLaunchConfig_t cfg = u2_config(grid, stream, attr);
-  return cudaLaunchKernelEx(&cfg, prefill_umma2_kernel, k_map, v_map, p);
+  return flush ? cudaLaunchKernelEx(&cfg, prefill_umma2_kernel<true>, k_map, v_map, p) : cudaLaunchKernelEx(&cfg, prefill_umma2_kernel<false>, k_map, v_map, p);
 }
 // Clusters of `splits` pairs that the current device holds at once (asked for once per device; 0 when it does not say).
 static int u2_clusters_at_once(int splits) {
@@ -824,7 +880,7 @@ static int u2_clusters_at_once(int splits) {
     cudaLaunchConfig_t cfg = u2_config(dim3(2 * 74, kHkv, splits), nullptr, attr);
     cfg.numAttrs = 1;
     int clusters = 0;
-    if (cudaOccupancyMaxActiveClusters(&clusters, prefill_umma2_kernel, &cfg) != cudaSuccess) {
+    if (cudaOccupancyMaxActiveClusters(&clusters, prefill_umma2_kernel<false>, &cfg) != cudaSuccess) {
       cudaGetLastError();
       clusters = 0;
     }
@@ -842,11 +898,12 @@ int launch_prefill_umma2(const void* q, int q_dtype, const char* k_cache, const 
                          long long num_blocks, const int32_t* block_tables, int table_width,
                          const int32_t* kv_lens, const int32_t* positions, const int32_t* query_start_loc,
                          int rows, int token_bucket, float scale, float* out, int32_t* status,
-                         int skip_single, int split_p, int tile_pairs, bool may_split, int32_t* beside, cudaStream_t stream) {
+                         int skip_single, int split_p, int tile_pairs, bool may_split, int32_t* beside, bool flush, cudaStream_t stream) {
   static PerDeviceFlags opted_in;
   if (!(scale > 0.f) || num_blocks < 1 || !tensor_maps_available()) return NVJ_ERR_UNSUPPORTED;
   if (!once_per_device(opted_in, [](int) {
-        return cudaFuncSetAttribute(prefill_umma2_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kU2SmemBytes) == cudaSuccess;
+        return cudaFuncSetAttribute(prefill_umma2_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kU2SmemBytes) == cudaSuccess &&
+               cudaFuncSetAttribute(prefill_umma2_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kU2SmemBytes) == cudaSuccess;
       }))
     return NVJ_ERR_LAUNCH;
   CUtensorMap k_map, v_map;
@@ -877,7 +934,7 @@ int launch_prefill_umma2(const void* q, int q_dtype, const char* k_cache, const 
     for (int s = 2; s <= kU2MaxSplits && s * pairs * kHkv <= p.pair_slots; ++s)
       if ((pairs - 1) * kHkv <= u2_clusters_at_once(s)) splits = s;  // (one pair per head, if not more, is idle and leaves at once)
   }
-  return u2_launch(dim3(2 * pairs, kHkv, splits), stream, k_map, v_map, p) == cudaSuccess ? NVJ_OK : NVJ_ERR_LAUNCH;
+  return u2_launch(dim3(2 * pairs, kHkv, splits), stream, k_map, v_map, p, flush) == cudaSuccess ? NVJ_OK : NVJ_ERR_LAUNCH;
 }
 
 }  // namespace nvj

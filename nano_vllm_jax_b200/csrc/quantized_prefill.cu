@@ -12,6 +12,10 @@
 
 namespace nvj {
 
+int prefill_over_pages(const void* q, const void* k_pages, const void* v_pages, long long pages, const int32_t* page_tables, int table_width,
+                       const int32_t* kv_lens, const int32_t* positions, const int32_t* query_start_loc, int rows, int token_bucket, float scale,
+                       float* out, int32_t* status, void* workspace, size_t workspace_bytes, int part, int tile_pairs, cudaStream_t stream);
+
 // ---- pages of a scratch bf16 cache ----------------------------------------------------------------------------------------------
 struct QUnpackParams {
   const uint8_t* k_cache;
@@ -26,49 +30,55 @@ struct QUnpackParams {
   int32_t* page_tables;
   int32_t* status;
   long long num_blocks;
-  int rows, table_width, block_size, num_kv_heads, head_dim, skip_single;
+  int rows, table_width, skip_single;
 };
 
-// Grid (x: blocks of a row in strides, y: rows).  A block whose id is outside the pool becomes a page of zeros, as the other kernels take it.
+// Grid (x: blocks of a row in strides, y: rows); the model's shape, 16 tokens of 2 heads of 256: a thread four pieces of 16 numbers, two of K and two
+// of V, of one head.  The block's id is asked for together with the row's length: two trips to memory in a row.  A block whose id is outside
+// the pool becomes a page of zeros, as the other kernels take it, and so do the rows behind the last key, which hold anything.
 __global__ void __launch_bounds__(256) quantized_unpack_kernel(QUnpackParams p) {
+  constexpr int kRow = 512, kBlock = 16 * kRow;  // bytes of a token, and of a block
   pdl_wait();
   pdl_release();
   const int row = blockIdx.y;
-  const int len = p.kv_lens[row];
-  const int tokens = p.query_start_loc[row + 1] - p.query_start_loc[row];
-  const bool skip = tokens <= 0 || (p.skip_single && tokens == 1);
-  const int all = (int)(((long long)(len > 0 ? len : 0) + p.block_size - 1) / p.block_size);
-  const int blocks = skip ? 0 : (all < p.table_width ? all : p.table_width);
-  const int row_elems = p.num_kv_heads * p.head_dim, block_elems = p.block_size * row_elems;
+  const int len = p.kv_lens[row], from = p.query_start_loc[row], to = p.query_start_loc[row + 1];
+  const bool skip = to <= from || (p.skip_single && to - from == 1);
+  const int head = (threadIdx.x * 16 % kRow) / 256, token = threadIdx.x * 16 / kRow;  // of the first piece; the second is eight tokens on
   for (int b = blockIdx.x; b < p.table_width; b += gridDim.x) {
     const long long page = (long long)row * p.table_width + b;
-    if (threadIdx.x == 0) p.page_tables[page] = (int)page;
-    if (b >= blocks) continue;
     const int id = p.block_tables[page];
+    if (threadIdx.x == 0) p.page_tables[page] = (int)page;
+    const int left = len - b * 16;  // tokens of the row from this block on
+    if (skip || left <= 0) continue;
     const bool ok = id >= 0 && id < p.num_blocks;
     if (!ok && threadIdx.x == 0) atomicOr(p.status, NVJ_DEV_BAD_BLOCK_ID);
-    const long long from = ok ? (long long)id * block_elems : 0;
-    for (int e = threadIdx.x * 16; e < 2 * block_elems; e += blockDim.x * 16) {
-      const bool is_v = e >= block_elems;
-      const int at = is_v ? e - block_elems : e;
-      uint4 w = make_uint4(0, 0, 0, 0);
-      float unit = 0.f;
-      if (ok && (long long)b * p.block_size + at / row_elems < len) {  // rows behind the last key hold anything
-        w = ld_stream_u4((is_v ? p.v_cache : p.k_cache) + from + at);
-        unit = (is_v ? p.v_scale : p.k_scale)[(long long)id * p.num_kv_heads + at % row_elems / p.head_dim];
-      }
-      const uint32_t in[4] = {w.x, w.y, w.z, w.w};
+    uint4 w[4];
+    float unit[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w[i] = make_uint4(0, 0, 0, 0);
+      if (ok && token + 8 * (i & 1) < left)
+        w[i] = ld_stream_u4((i < 2 ? p.k_cache : p.v_cache) + (long long)id * kBlock + (i & 1) * (kBlock / 2) + threadIdx.x * 16);
+    }
+    if (ok) {
+      unit[0] = p.k_scale[(long long)id * 2 + head];
+      unit[1] = p.v_scale[(long long)id * 2 + head];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t in[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+      const float u = unit[i >> 1];
       uint32_t out[8];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 a = q_float2(q_half2(in[i])), c = q_float2(q_half2_high(in[i]));
-        const __nv_bfloat162 x = __floats2bfloat162_rn(a.x * unit, a.y * unit), y = __floats2bfloat162_rn(c.x * unit, c.y * unit);
-        out[2 * i] = *reinterpret_cast<const uint32_t*>(&x);
-        out[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&y);
+      for (int k = 0; k < 4; ++k) {
+        const float2 x = q_float2(q_half2(in[k])), y = q_float2(q_half2_high(in[k]));
+        const __nv_bfloat162 lo = __floats2bfloat162_rn(x.x * u, x.y * u), hi = __floats2bfloat162_rn(y.x * u, y.y * u);
+        out[2 * k] = *reinterpret_cast<const uint32_t*>(&lo);
+        out[2 * k + 1] = *reinterpret_cast<const uint32_t*>(&hi);
       }
-      uint4* to = reinterpret_cast<uint4*>((is_v ? p.v_pages : p.k_pages) + (page * block_elems + at) * 2);
-      to[0] = make_uint4(out[0], out[1], out[2], out[3]);
-      to[1] = make_uint4(out[4], out[5], out[6], out[7]);
+      uint4* at = reinterpret_cast<uint4*>((i < 2 ? p.k_pages : p.v_pages) + 2 * (page * kBlock + (i & 1) * (kBlock / 2) + threadIdx.x * 16));
+      at[0] = make_uint4(out[0], out[1], out[2], out[3]);
+      at[1] = make_uint4(out[4], out[5], out[6], out[7]);
     }
   }
 }
@@ -366,34 +376,44 @@ __global__ void __launch_bounds__(kQpThreads, 1) quantized_prefill_kernel(QPrefi
         }
       }
     }
+    uint32_t high[kNT / 2][4], low[kNT / 2][4];  // the weights' pairs are the operand of the second product
 #pragma unroll
-    for (int j = 0; j < kNT; j += 2) {  // 16 keys: the weights' pairs are the operand of the second product
-      uint32_t high[4], low[4];
+    for (int j = 0; j < kNT; ++j) {
+      const float2 vl = *reinterpret_cast<const float2*>(&qp_v_log[buf][8 * j + 2 * t]);
+      float w[4];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const float2 vl = *reinterpret_cast<const float2*>(&qp_v_log[buf][8 * (j + u) + 2 * t]);
-        float w[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int i = k >> 1;
-          const float v = k & 1 ? vl.y : vl.x;
-          l[i] += ex2_approx(s[j + u][k] - m[i]);
-          w[k] = ex2_approx(s[j + u][k] + v - mv[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          high[2 * u + i] = q_pair(w[2 * i], w[2 * i + 1]);
-          low[2 * u + i] = q_pair_rest(w[2 * i], w[2 * i + 1], high[2 * u + i]);
-        }
+      for (int k = 0; k < 4; ++k) {
+        const int i = k >> 1;
+        l[i] += ex2_approx(s[j][k] - m[i]);
+        w[k] = ex2_approx(s[j][k] + (k & 1 ? vl.y : vl.x) - mv[i]);
       }
 #pragma unroll
-      for (int d = 0; d < kOT; d += 2) {
+      for (int i = 0; i < 2; ++i) {
+        uint32_t& h = high[j / 2][2 * (j & 1) + i];
+        h = q_pair(w[2 * i], w[2 * i + 1]);
+        low[j / 2][2 * (j & 1) + i] = q_pair_rest(w[2 * i], w[2 * i + 1], h);
+      }
+    }
+    // A tile's weighted sum is taken from zero and added in f32: the tensor cores cut the last place of what they add to, and 1000 steps on one sum
+    // cost 3e-5 of it (8000 keys).
+#pragma unroll
+    for (int d = 0; d < kOT; d += 2) {
+      float part[2][4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) part[0][k] = part[1][k] = 0.f;
+#pragma unroll
+      for (int j = 0; j < kNT / 2; ++j) {
         uint32_t b[4];
-        qp_ldsm4_t(v_at + (j * 8 * kPitch + d * 8) * 2, b);
-        q_mma(acc[d], high[0], high[1], high[2], high[3], b[0], b[1]);
-        q_mma(acc[d + 1], high[0], high[1], high[2], high[3], b[2], b[3]);
-        q_mma(acc[d], low[0], low[1], low[2], low[3], b[0], b[1]);
-        q_mma(acc[d + 1], low[0], low[1], low[2], low[3], b[2], b[3]);
+        qp_ldsm4_t(v_at + (j * 16 * kPitch + d * 8) * 2, b);
+        q_mma(part[0], low[j][0], low[j][1], low[j][2], low[j][3], b[0], b[1]);
+        q_mma(part[1], low[j][0], low[j][1], low[j][2], low[j][3], b[2], b[3]);
+        q_mma(part[0], high[j][0], high[j][1], high[j][2], high[j][3], b[0], b[1]);
+        q_mma(part[1], high[j][0], high[j][1], high[j][2], high[j][3], b[2], b[3]);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        acc[d][k] += part[0][k];
+        acc[d + 1][k] += part[1][k];
       }
     }
   }
@@ -501,18 +521,14 @@ extern "C" int nvj_paged_prefill_quantized(const void* q, int q_dtype, const voi
     u.num_blocks = num_blocks;
     u.rows = rows;
     u.table_width = table_width;
-    u.block_size = block_size;
-    u.num_kv_heads = num_kv_heads;
-    u.head_dim = head_dim;
     u.skip_single = skip_single;
     const int across = (148 * 8 + rows - 1) / rows;
     if (launch_after(quantized_unpack_kernel, dim3(across < table_width ? across : table_width, rows), dim3(256), 0, s, u) != cudaSuccess)
       return NVJ_ERR_LAUNCH;
     // (with no rows of one token the key ranges may be split; part 3 asks for that by a workspace, and writes nothing there)
-    const int rc = nvj_paged_prefill_packed_counted(q, q_dtype, u.k_pages, u.v_pages, NVJ_BF16, pages, block_size, num_kv_heads, head_dim,
-                                                    num_q_heads, u.page_tables, table_width, kv_lens, positions, query_start_loc, rows,
-                                                    token_bucket, scale, out, status, skip_single ? nullptr : workspace,
-                                                    skip_single ? 0 : workspace_bytes, 4, skip_single ? 2 : 3, tile_pairs, stream);
+    const int rc = prefill_over_pages(q, u.k_pages, u.v_pages, pages, u.page_tables, table_width, kv_lens, positions, query_start_loc, rows, token_bucket,
+                                      scale, out, status, skip_single ? nullptr : workspace, skip_single ? 0 : workspace_bytes, skip_single ? 2 : 3,
+                                      tile_pairs, s);
     if (rc != NVJ_ERR_UNSUPPORTED) return rc;  // (without a tensor-map encoder)
   }
   QPrefillParams p{};

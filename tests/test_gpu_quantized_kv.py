@@ -518,7 +518,7 @@ def test_a_table_too_wide_for_the_pages_goes_to_the_other_tiles():
     _check([got[:100], got[100:]], [q64[0, :100], q64[0, 100:]], state, narrow, lens, [1 + np.arange(n) for n in lens], 1 / 16)
 
 
-@pytest.mark.parametrize("keys,tokens", [(9000, 200)])
+@pytest.mark.parametrize("keys,tokens", [(9000, 5000), (25000, 4700), (16449, 5100)])  # (no split of the key ranges: accumulators are emptied once, or three times)
 def test_packed_prefill_over_many_keys(keys, tokens):
     hq, hkv, d, bs = shape = SHAPES[0]
     rng = np.random.default_rng(21)
@@ -530,7 +530,7 @@ def test_packed_prefill_over_many_keys(keys, tokens):
     positions = np.arange(keys - tokens, keys)[None]
     out = _f64(Q.packed_paged_prefill_attention_quantized(q, k, v, ks, vs, _i32(tables), _i32([keys]), _i32(positions), _i32([0, tokens]), bs, 1 / 16, 4,
                                                           num_decode_rows=0)).reshape(tokens, hq, d)
-    pick = [0, 63, 64, tokens - 1]
+    pick = [0, 63, 64, 100, tokens // 2 + 1, tokens - 1]
     _check([out[pick]], [q64[0, pick]], state, tables, [keys], [positions[0, pick] + 1], 1 / 16, 16)
 
 
