@@ -629,36 +629,44 @@ __device__ __forceinline__ void qu_softmax_warps(QuSmem<L>& sm, const QuParams& 
   }
 }
 
-// ---- queries as e4m3 terms: a column per warp at a time ---------------------------------------------------------------------------
+// ---- queries as e4m3 terms: a column (head_dim 128: two) per warp at a time ---------------------------------------------------------------------------
 // (Loops that are rolled up: twelve columns unrolled were 20 KB of code that a CTA runs through once or twice, and waits for: 13 us in front
 // of the first scores of rows of five tokens.)
 template <class L, typename T>
-struct QuColumn {  // lane l's dims 8 l ..
+struct QuColumn {  // from column c on: column c + l / kLanes, dims 8 (l % kLanes) .. in lane l
+  static constexpr int kLanes = L::kChunks * 16, kCount = 32 / kLanes;
   QRaw<T> raw;
   int limit;
   __device__ __forceinline__ void load(const QuSmem<L>& sm, const QuParams& a, const QuSeg& s, long long token, int ct, int c, int lane) {
     raw = QRaw<T>{};
     limit = 0;
+    c += lane / kLanes;
     if (ct * L::kC + c < a.columns) {
-      if (8 * lane < L::kChunks * 128) raw = q_load8(static_cast<const T*>(a.q) + (token * a.num_q_heads + sm.col_row[c]) * (L::kChunks * 128) + 8 * lane);
+      raw = q_load8(static_cast<const T*>(a.q) + (token * a.num_q_heads + sm.col_row[c]) * (L::kChunks * 128) + 8 * (lane % kLanes));
       const int last = a.positions ? a.positions[token + sm.col_token[c]] : 0x7ffffffe;
       limit = last < s.len ? last + 1 : s.len;
     }
   }
   template <int kCg>
   __device__ __forceinline__ void store(QuSmem<L>& sm, const QuParams& a, uint32_t seg, int c, int lane) const {
-    const int d = 8 * lane;
+    const int d = 8 * (lane % kLanes);
+    c += lane / kLanes;
     float x[8];
     q_floats(raw, x);
     int bits = 0;
 #pragma unroll
     for (int k = 0; k < 8; ++k) bits = max(bits, __float_as_int(x[k]) & 0x7fffffff);
-    bits = __reduce_max_sync(kFullMask, bits);
+    if constexpr (kCount == 1) {
+      bits = __reduce_max_sync(kFullMask, bits);
+    } else {
+#pragma unroll
+      for (int o = kLanes / 2; o > 0; o >>= 1) bits = max(bits, __shfl_xor_sync(kFullMask, bits, o));
+    }
     const bool odd = bits >= 0x7f800000;  // an infinity or NaN: the column's scores are NaN
     int e = (bits >> 23) - 127 - 7;       // largest = 2^(e + 7) * [1, 2)
     e = bits == 0 || odd ? 0 : (e < -126 ? -126 : e);
     const float down = q_pow2(-e);
-    if (lane == 0) {
+    if (lane % kLanes == 0) {
       sm.factor[seg & 3u][c] = odd ? __int_as_float(0x7fffffff) : q_pow2(e) * a.scale_log2;
       sm.limit[seg & 3u][c] = limit;
     }
@@ -678,9 +686,8 @@ struct QuColumn {  // lane l's dims 8 l ..
         }
       }
       const int row = row0 + j * kCg;
-      if (d < L::kChunks * 128)
-        *reinterpret_cast<uint2*>(sm.q[seg & 1u][d / 128] + row * 128 + (((d % 128 / 16) ^ (row & 7)) << 4) + (d & 8)) =
-            make_uint2(b[0] | b[1] << 16, b[2] | b[3] << 16);
+      *reinterpret_cast<uint2*>(sm.q[seg & 1u][d / 128] + row * 128 + (((d % 128 / 16) ^ (row & 7)) << 4) + (d & 8)) =
+          make_uint2(b[0] | b[1] << 16, b[2] | b[3] << 16);
     }
   }
 };
@@ -694,15 +701,22 @@ __device__ __forceinline__ void qu_query_warp(QuSmem<L>& sm, const QuParams& a, 
   for (uint32_t seg = 0; walk.next(a, p, s); ++seg) {
     if (seg > 0) {
       const long long token = qu_first_token(a, s.b);
-      QuColumn<L, T> now, next;
-      now.load(sm, a, s, token, ct, 0, lane);
+      // a few columns are on their way at a time
+      using Column = QuColumn<L, T>;
+      constexpr int kAhead = L::kC < 4 * Column::kCount ? L::kC / Column::kCount : 4, kAll = kAhead * Column::kCount;
+      static_assert(L::kC % kAll == 0);
+      Column column[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) column[i].load(sm, a, s, token, ct, i * Column::kCount, lane);
       // the scores of the segment two before have been computed
       if (seg > 1 && !um_wait(&sm.q_free[seg & 1u], ((seg >> 1) - 1) & 1u, &sm.abort_flag, p.status)) return;
 #pragma unroll 1
-      for (int c = 0; c < L::kC; ++c) {
-        if (c + 1 < L::kC) next.load(sm, a, s, token, ct, c + 1, lane);
-        now.template store<kCg>(sm, a, seg, c, lane);
-        now = next;
+      for (int c = 0; c < L::kC; c += kAll) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          column[i].template store<kCg>(sm, a, seg, c + i * Column::kCount, lane);
+          if (c + kAll < L::kC) column[i].load(sm, a, s, token, ct, c + kAll + i * Column::kCount, lane);
+        }
       }
       fence_proxy_async_smem();
     }
@@ -827,7 +841,7 @@ quantized_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
       const bool have = first.next(a, p, s);
       const long long token = have ? qu_first_token(a, s.b) : 0;
 #pragma unroll 1
-      for (int c = warp - (warp > 10); have && c < L::kC; c += kQuThreads / 32 - 1) {
+      for (int c = (warp - (warp > 10)) * QuColumn<L, T>::kCount; have && c < L::kC; c += (kQuThreads / 32 - 1) * QuColumn<L, T>::kCount) {
         QuColumn<L, T> column;
         column.load(sm, a, s, token, ct, c, lane);
         column.template store<kCg>(sm, a, 0u, c, lane);
