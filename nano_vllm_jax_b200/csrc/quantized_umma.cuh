@@ -40,28 +40,28 @@ namespace nvj {
 constexpr int kQuTile = 128;    // keys per tile
 constexpr int kQuUnits = 8;     // boxes per tile, at most: a box is a unit of 16, 32 or 64 keys of one block (QuParams::unit)
 constexpr int kQuPTerms = 5;
-constexpr int kQuThreads = 384;
 // The reference of a column's weights is set 2^3 below its largest weight and moved when one would pass 2^8 (e4m3 ends at 448).
 constexpr float kQuNone = -3e38f, kQuSlack = 8.f, kQuLift = 3.f;
 constexpr float kQuMostInverse = 100.f;  // log2 of what a weight is multiplied by, at most, to take the V scale out of it again
-constexpr int kQuLens = kQuThreads;      // rows whose lengths a CTA keeps in shared memory
 
 template <typename T>
 constexpr int quq_terms() {
   return sizeof(T) == 4 ? 5 : std::is_same<T, __half>::value ? 3 : 2;
 }
 
-// kCg: columns of a softmax thread; kByTiles: the two groups take the tiles in turn, else half of the columns each.
-template <typename T, int kDim, int kCg, bool kByTiles>
+// kCg: columns of a softmax thread; kSharing: groups that share a tile, a region of the columns each.  One: two groups take the tiles in turn.
+template <typename T, int kDim, int kCg, int kSharing>
 struct QuLayout {
-  static constexpr int kC = kByTiles ? kCg : 2 * kCg;  // columns of the CTA
-  static constexpr int kRegions = kByTiles ? 1 : 2;    // of a row of query terms or weights: one per group that shares a tile
+  static constexpr bool kByTiles = kSharing == 1;
+  static constexpr int kGroups = kByTiles ? 2 : kSharing, kSoftmaxThreads = 128 * kGroups, kThreads = kSoftmaxThreads + 128;
+  static constexpr int kC = kCg * kSharing;  // columns of the CTA
+  static constexpr int kRegions = kSharing;  // of a row of query terms or weights
   static constexpr int kQTerms = quq_terms<T>();
   static constexpr int kChunks = kDim / 128;
   static constexpr int kSRegion = kQTerms * kCg;                        // columns of S: [region][term][kCg]
-  static constexpr int kORegion = (kQuPTerms * kCg + 15) / 16 * 16;     // columns of O: [region][term][kCg], padded
+  static constexpr int kORegion = kQuPTerms * kCg;                      // columns of O: [region][term][kCg]
   static constexpr int kNS = (kRegions * kSRegion + 15) / 16 * 16;      // (N of an MMA: multiples of 16)
-  static constexpr int kNO = kRegions * kORegion;
+  static constexpr int kNO = (kRegions * kORegion + 15) / 16 * 16;
   static constexpr int kSets0 = (512 - 2 * kNS) / (kNO * kChunks);      // accumulators that take the tiles in turn: shorter sums
   static constexpr int kSets = kByTiles ? (kSets0 < 4 ? 2 : 4) : (kSets0 < 2 ? 1 : 2);
   static constexpr int kColO = 2 * kNS;                                 // S twice, then the sets
@@ -86,11 +86,11 @@ struct QuSmem {
   alignas(16) float k_unit[8][kQuUnits], v_unit[8][kQuUnits];  // by tile: the scales of its units' blocks; V's -1: no such block
   alignas(16) float factor[4][L::kC];  // by segment: what a column's products are multiplied by, and the keys it may see
   alignas(16) int limit[4][L::kC];
-  alignas(16) float red[2][4][12];  // per group and warp
-  float red_v[2][4];
-  float m[2][12], mv[2][12];  // at the end: references of the sum of the weights, and of the weighted sums
+  alignas(16) float red[L::kGroups][4][8];  // per group and warp
+  float red_v[L::kGroups][4];
+  float m[L::kGroups][8], mv[L::kGroups][8];  // at the end: references of the sum of the weights, and of the weighted sums
   int col_row[L::kC], col_token[L::kC];  // of a column: its row of the row's queries (and of its output), its token
-  int lens[kQuLens];  // of rows lens_from ..
+  int lens[L::kThreads];  // of rows lens_from ..
   alignas(16) float out_f[2][L::kC];  // what a group's sums are multiplied by at the end
   int scan[16];
   int start_b, start_j, lens_from, abort_flag;
@@ -123,6 +123,10 @@ __device__ __forceinline__ void qu_tmem_st8(uint32_t taddr, const float (&v)[8])
 __device__ __forceinline__ void qu_sts4(uint32_t at, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
+__device__ __forceinline__ void qu_sts2(uint32_t at, uint32_t x, uint32_t y) {
+  asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void qu_sts1(uint32_t at, uint32_t x) { asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(x) : "memory"); }
 // N (a multiple of 4) numbers from a 16-byte boundary in shared memory on.
 template <int N>
 __device__ __forceinline__ void qu_lds(float (&v)[N], const float* from) {
@@ -156,6 +160,7 @@ __device__ __forceinline__ float qu_warp_max(float x) {
   return __int_as_float(k ^ ((k >> 31) & 0x7fffffff));
 }
 // Inclusive scan of one int per thread over the CTA.
+template <int kThreads>
 __device__ __forceinline__ int qu_inclusive_scan(int v, int* warp_sums, int& total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
@@ -168,7 +173,7 @@ __device__ __forceinline__ int qu_inclusive_scan(int v, int* warp_sums, int& tot
   __syncthreads();
   int before = 0, all = 0;
 #pragma unroll
-  for (int w = 0; w < kQuThreads / 32; ++w) {
+  for (int w = 0; w < kThreads / 32; ++w) {
     const int x = warp_sums[w];
     if (w < warp) before += x;
     all += x;
@@ -200,10 +205,10 @@ struct QuWalk {  // (next_seg of decode_parts.cuh, over units)
   int b, j;
   long long g, g1;
   const int* lens;  // in shared memory: an access to global memory takes up to 2 us here while the copies are under way
-  int lens_from;
+  int lens_from, lens_count;
   __device__ __forceinline__ bool next(const QuParams& a, const DecodeParams& p, QuSeg& s) {
     while (g < g1 && b < p.batch) {
-      const int len = b - lens_from < kQuLens ? lens[b - lens_from] : decode_row_len(p, b), nb = qu_row_units(a, len), all = blocks_in_sequence(p, nb);
+      const int len = b - lens_from < lens_count ? lens[b - lens_from] : decode_row_len(p, b), nb = qu_row_units(a, len), all = blocks_in_sequence(p, nb);
       if (j >= all) { ++b; j = 0; continue; }
       const int take = (long long)(all - j) < g1 - g ? all - j : (int)(g1 - g);
       const int j0 = j, j1 = min(j + take, nb), row = b;
@@ -377,15 +382,16 @@ __device__ __forceinline__ void qu_sums_warp(QuSmem<L>& sm, const QuParams& a, c
 
 // ---- warps 0 - 7: softmax and output.  Thread = key of the tile, then dim of the output ---------------------------------------
 // (A wait that runs out does so for one warp and perhaps not for the next: a group's warps leave together, behind a meeting.)
-template <class L, int kCg, bool kByTiles>
+template <class L, int kCg>
 __device__ __forceinline__ void qu_softmax_warps(QuSmem<L>& sm, const QuParams& a, const DecodeParams& p, uint32_t tmem, int head, int hct, int ct,
                                                  QuWalk walk, int range, int group, int warp, int lane) {
   constexpr int kSRead = (L::kSRegion + 7) / 8, kORead = (kQuPTerms * kCg + 7) / 8;  // pieces of 8 columns
+  constexpr bool kByTiles = L::kByTiles;
   constexpr int kDim = L::kChunks * 128, kWords = L::kORegion / 4;
   const int key = warp * 32 + lane, region = kByTiles ? 0 : group, first_col = kByTiles ? 0 : group * kCg, bar = 1 + group;
   tmem += (uint32_t)(warp * 32) << 16;
   // a group that leaves early meets the other one, which waits at a segment's end or leaves as well
-  auto give_up = [] { qu_meet_any<256>(3, true); };
+  auto give_up = [] { qu_meet_any<L::kSoftmaxThreads>(3, true); };
   QuRing<L::kVSlots> at;  // V's slot of the tile at hand
   QuSeg s;
   const int per = kQuTile / a.unit, my_unit = key >> a.unit_log2;
@@ -515,8 +521,6 @@ __device__ __forceinline__ void qu_softmax_warps(QuSmem<L>& sm, const QuParams& 
         }
         uint32_t bytes[kWords];
 #pragma unroll
-        for (int i = kQuPTerms * kCg / 4; i < kWords; ++i) bytes[i] = 0u;
-#pragma unroll
         for (int j = 0; j < kQuPTerms; ++j)
 #pragma unroll
           for (int c = 0; c < kCg; c += 4) {
@@ -533,9 +537,18 @@ __device__ __forceinline__ void qu_softmax_warps(QuSmem<L>& sm, const QuParams& 
         // (the weights of tile n - 2, in the same place, have been used: almost always long ago; a wait that runs out shows at the next meeting)
         if (n >= 2) um_wait(&sm.pv_done[buf], ((n >> 1) - 1) & 1u, &sm.abort_flag, p.status);
         const uint32_t w_row = smem_u32(sm.w[buf]) + key * 128;
+        // (bytes of the row behind the last region hold anything: they only reach columns of O that nothing reads)
+        const int piece = region * (kWords / 2);  // of 8 bytes: a region is 2.5 or 5 of the swizzle's 16
+        if constexpr (kWords % 4 == 1) {
 #pragma unroll
-        for (int i = 0; i < kWords / 4; ++i)
-          qu_sts4(w_row + (((region * (kWords / 4) + i) ^ (key & 7)) << 4), bytes[4 * i], bytes[4 * i + 1], bytes[4 * i + 2], bytes[4 * i + 3]);
+          for (int i = 0; i < kWords / 4; ++i)
+            qu_sts4(w_row + ((i ^ (key & 7)) << 4), bytes[4 * i], bytes[4 * i + 1], bytes[4 * i + 2], bytes[4 * i + 3]);
+          qu_sts1(w_row + (((kWords / 4) ^ (key & 7)) << 4), bytes[kWords - 1]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < kWords / 2; ++i)
+            qu_sts2(w_row + ((((piece + i) >> 1) ^ (key & 7)) << 4) + ((piece + i) & 1) * 8, bytes[2 * i], bytes[2 * i + 1]);
+        }
       }
       // V rows of keys that are not there weigh nothing, but may hold anything: 0 x NaN is not 0
       if (t == nt - 1 && (kByTiles || group == 0) && ((cnt * a.unit & 31) || (s.j0 + s.n == s.nb && (s.len & (a.unit - 1))))) {
@@ -565,7 +578,7 @@ __device__ __forceinline__ void qu_softmax_warps(QuSmem<L>& sm, const QuParams& 
         sm.m[group][c] = m[c] - v_first;
       }
     }
-    if (qu_meet_any<256>(3, !um_wait(&sm.o_full, seg & 1u, &sm.abort_flag, p.status))) return;
+    if (qu_meet_any<L::kSoftmaxThreads>(3, !um_wait(&sm.o_full, seg & 1u, &sm.abort_flag, p.status))) return;
     const bool final_row = s.whole();
     const long long slot = (long long)partial_slot(range, s.j0 == 0) * a.hcts + hct;
     const int tid = group * 128 + key;
@@ -585,15 +598,15 @@ __device__ __forceinline__ void qu_softmax_warps(QuSmem<L>& sm, const QuParams& 
         if (!final_row) *reinterpret_cast<float2*>(a.part_ml + (slot * L::kC + tid) * 2) = make_float2(sm.m[g][c], sum);
       }
     }
-    qu_meet_any<256>(3, false);
+    qu_meet_any<L::kSoftmaxThreads>(3, false);
     tc_fence_after_sync();
     const int columns = min(a.columns - ct * L::kC, L::kC);
     const long long token = a.query_start_loc ? (long long)a.query_start_loc[s.b] : (long long)s.b * a.width;
-    // head_dim 256: a group a chunk of the dims; 128: half of the columns
-    const int h = L::kChunks == 2 ? group : 0;
+    // a piece of the output is a chunk of the dims of a region; the single one of head_dim 128 and up to 8 columns is shared
+    constexpr bool kShared = L::kChunks * L::kRegions == 1;
 #pragma unroll 1
-    for (int r = 0; r < L::kRegions; ++r) {
-      if (L::kChunks == 1 && L::kRegions == 2 && r != group) continue;
+    for (int piece = kShared ? 0 : group; piece < L::kChunks * L::kRegions; piece += L::kGroups) {
+      const int h = piece % L::kChunks, r = piece / L::kChunks;
       float y[kCg];
 #pragma unroll
       for (int c = 0; c < kCg; ++c) y[c] = 0.f;
@@ -619,7 +632,7 @@ __device__ __forceinline__ void qu_softmax_warps(QuSmem<L>& sm, const QuParams& 
 #pragma unroll
       for (int c = 0; c < kCg; ++c) {
         const int col = r * kCg + c;
-        if (col >= columns || (L::kChunks == 1 && L::kRegions == 1 && c / (kCg / 2) != group)) continue;
+        if (col >= columns || (kShared && c / (kCg / 2) != group)) continue;
         float* to = final_row ? a.out + (token * a.num_q_heads + sm.col_row[col]) * kDim : a.part_acc + (slot * L::kC + col) * kDim;
         to[h * 128 + key] = y[c];
       }
@@ -724,10 +737,11 @@ __device__ __forceinline__ void qu_query_warp(QuSmem<L>& sm, const QuParams& a, 
   }
 }
 
-template <typename T, int kDim, int kCg, bool kByTiles>
-__global__ void __launch_bounds__(kQuThreads, 1)
+template <typename T, int kDim, int kCg, int kSharing>
+__global__ void __launch_bounds__(QuLayout<T, kDim, kCg, kSharing>::kThreads, 1)
 quantized_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const QuParams a, const DecodeParams p) {
-  using L = QuLayout<T, kDim, kCg, kByTiles>;
+  using L = QuLayout<T, kDim, kCg, kSharing>;
+  constexpr int kThreads = L::kThreads, kScoresWarp = 4 * L::kGroups, kSumsWarp = kScoresWarp + 1, kTmaWarp = kScoresWarp + 2;
   extern __shared__ unsigned char qu_smem_raw[];
   QuSmem<L>& sm = *reinterpret_cast<QuSmem<L>*>((reinterpret_cast<uintptr_t>(qu_smem_raw) + 1023) & ~(uintptr_t)1023);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -750,11 +764,11 @@ quantized_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
       mbar_init(smem_u32(&sm.q_full[i]), 32);
       mbar_init(smem_u32(&sm.q_free[i]), 1);
       mbar_init(smem_u32(&sm.s_full[i]), 1);
-      mbar_init(smem_u32(&sm.p_full[i]), kByTiles ? 128 : 256);
+      mbar_init(smem_u32(&sm.p_full[i]), 128 * kSharing);
       mbar_init(smem_u32(&sm.pv_done[i]), 1);
     }
     mbar_init(smem_u32(&sm.o_full), 1);
-    mbar_init(smem_u32(&sm.o_free), 256);
+    mbar_init(smem_u32(&sm.o_free), L::kSoftmaxThreads);
     mbar_fence_init();
   }
   if (threadIdx.x < L::kC) {
@@ -763,17 +777,17 @@ quantized_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
     sm.col_row[threadIdx.x] = at / a.groups * a.num_q_heads + head * a.groups + at % a.groups;
   }
   // (rows of the query terms that no column fills: finite, and never read)
-  for (int i = threadIdx.x; i < (int)sizeof(sm.q) / 16; i += kQuThreads) reinterpret_cast<uint4*>(sm.q)[i] = make_uint4(0, 0, 0, 0);
+  for (int i = threadIdx.x; i < (int)sizeof(sm.q) / 16; i += kThreads) reinterpret_cast<uint4*>(sm.q)[i] = make_uint4(0, 0, 0, 0);
   fence_proxy_async_smem();
   pdl_wait();
   {  // this CTA's share of the block tables into the L2, while the lengths are on their way
     const long long lines = ((long long)p.batch * p.table_width * (long long)sizeof(int32_t) + 127) / 128;
-    const long long line = (long long)blockIdx.x * kQuThreads + threadIdx.x;
+    const long long line = (long long)blockIdx.x * kThreads + threadIdx.x;
     if (line < lines) asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const char*>(p.block_tables) + line * 128));
   }
   // ---- pass 1: total number of units; zero the output of rows without keys
   int mine = 0, first_n = 0;
-  for (int base = 0; base < p.batch; base += kQuThreads) {
+  for (int base = 0; base < p.batch; base += kThreads) {
     const int b = base + threadIdx.x;
     int len = 0;
     if (b < p.batch) len = decode_row_len(p, b);
@@ -797,7 +811,7 @@ quantized_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
     }
   }
   int total = 0;
-  const int incl = qu_inclusive_scan(mine, sm.scan, total);
+  const int incl = qu_inclusive_scan<kThreads>(mine, sm.scan, total);
   const Partition pt = make_partition(total > 0 ? total : 1, ranges);
   const long long g0 = pt.start(range), g1 = pt.start(range + 1);
   if (total == 0 || range >= pt.n || g0 == g1) {  // nothing for this CTA
@@ -806,32 +820,32 @@ quantized_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
   }
   // ---- pass 2: locate (row, unit) of g0
   long long carry = 0;
-  if (p.batch <= kQuThreads) {  // one row per thread: the scan of pass 1 has the answer already
+  if (p.batch <= kThreads) {  // one row per thread: the scan of pass 1 has the answer already
     const long long excl = incl - first_n;
     if (first_n > 0 && excl <= g0 && g0 < excl + first_n) { sm.start_b = threadIdx.x; sm.start_j = (int)(g0 - excl); }
     carry = g0 + 1;  // skips the loop below
   }
-  for (int base = 0; base < p.batch && carry <= g0; base += kQuThreads) {
+  for (int base = 0; base < p.batch && carry <= g0; base += kThreads) {
     const int b = base + threadIdx.x;
     int n = 0;
     if (b < p.batch) n = blocks_in_sequence(p, qu_row_units(a, decode_row_len(p, b)));
     int chunk_total = 0;
-    const long long excl = carry + qu_inclusive_scan(n, sm.scan, chunk_total) - n;
+    const long long excl = carry + qu_inclusive_scan<kThreads>(n, sm.scan, chunk_total) - n;
     if (n > 0 && excl <= g0 && g0 < excl + n) { sm.start_b = b; sm.start_j = (int)(g0 - excl); }
     carry += chunk_total;
   }
   __syncthreads();
-  if (p.batch > kQuThreads) {  // (else pass 1 has left all lengths)
+  if (p.batch > kThreads) {  // (else pass 1 has left all lengths)
     const int b = sm.start_b + threadIdx.x;
     sm.lens[threadIdx.x] = b < p.batch ? decode_row_len(p, b) : 0;
     if (threadIdx.x == 0) sm.lens_from = sm.start_b;
     __syncthreads();
   }
-  const QuWalk walk{sm.start_b, sm.start_j, g0, g1, sm.lens, sm.lens_from};
-  if (warp == 10) {  // needs neither queries nor tensor memory
+  const QuWalk walk{sm.start_b, sm.start_j, g0, g1, sm.lens, sm.lens_from, kThreads};
+  if (warp == kTmaWarp) {  // needs neither queries nor tensor memory
     qu_producer<L>(&k_map, &v_map, a, p, sm, head, walk, lane);
   } else {
-    if (warp == 8) {  // tensor memory between the wait and the release (umma.cuh)
+    if (warp == kScoresWarp) {  // tensor memory between the wait and the release (umma.cuh)
       tmem_alloc(smem_u32(&sm.tmem_base), 512);
       if (lane == 0) pdl_release();
     }
@@ -841,7 +855,7 @@ quantized_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
       const bool have = first.next(a, p, s);
       const long long token = have ? qu_first_token(a, s.b) : 0;
 #pragma unroll 1
-      for (int c = (warp - (warp > 10)) * QuColumn<L, T>::kCount; have && c < L::kC; c += (kQuThreads / 32 - 1) * QuColumn<L, T>::kCount) {
+      for (int c = (warp - (warp > kTmaWarp)) * QuColumn<L, T>::kCount; have && c < L::kC; c += (kThreads / 32 - 1) * QuColumn<L, T>::kCount) {
         QuColumn<L, T> column;
         column.load(sm, a, s, token, ct, c, lane);
         column.template store<kCg>(sm, a, 0u, c, lane);
@@ -849,13 +863,13 @@ quantized_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
       fence_proxy_async_smem();
     }
     tc_fence_before_sync();
-    named_bar_sync(4, kQuThreads - 32);
+    named_bar_sync(4, kThreads - 32);
     tc_fence_after_sync();
     const uint32_t tmem = sm.tmem_base;
 
-    if (warp < 8) qu_softmax_warps<L, kCg, kByTiles>(sm, a, p, tmem, head, hct, ct, walk, range, warp >> 2, warp & 3, lane);
-    else if (warp == 8) qu_scores_warp<L>(sm, a, p, tmem, walk);
-    else if (warp == 9) {
+    if (warp < kScoresWarp) qu_softmax_warps<L, kCg>(sm, a, p, tmem, head, hct, ct, walk, range, warp >> 2, warp & 3, lane);
+    else if (warp == kScoresWarp) qu_scores_warp<L>(sm, a, p, tmem, walk);
+    else if (warp == kSumsWarp) {
       if (hct == 0 && lane == 0) a.cuts[range] = qu_cut(a, p, pt, range, walk.b, walk.j, walk.g);
       __syncwarp();
       qu_sums_warp<L>(sm, a, p, tmem, walk);
@@ -870,19 +884,20 @@ quantized_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
     while (global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
     __syncthreads();
   }
-  if (warp == 8) tmem_dealloc(sm.tmem_base, 512);
+  if (warp == kScoresWarp) tmem_dealloc(sm.tmem_base, 512);
 }
 
-template <typename T, int kDim, int kCg, bool kByTiles>
+template <typename T, int kDim, int kCg, int kSharing>
 static int launch_quantized_umma(const CUtensorMap& k_map, const CUtensorMap& v_map, const QuParams& a, const DecodeParams& p, int ranges,
                                  cudaStream_t stream) {
-  constexpr int bytes = (int)sizeof(QuSmem<QuLayout<T, kDim, kCg, kByTiles>>) + 1024;
+  using L = QuLayout<T, kDim, kCg, kSharing>;
+  constexpr int bytes = (int)sizeof(QuSmem<L>) + 1024;
   static_assert(bytes <= 232448, "the ring exceeds the shared memory of one CTA");
-  auto* kernel = quantized_umma_kernel<T, kDim, kCg, kByTiles>;
+  auto* kernel = quantized_umma_kernel<T, kDim, kCg, kSharing>;
   static PerDeviceFlags ready;
   if (!once_per_device(ready, [&](int) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess; }))
     return NVJ_ERR_LAUNCH;
-  return launch_after(kernel, dim3((unsigned)(ranges * a.hcts)), dim3(kQuThreads), bytes, stream, k_map, v_map, a, p) == cudaSuccess ? NVJ_OK
+  return launch_after(kernel, dim3((unsigned)(ranges * a.hcts)), dim3(L::kThreads), bytes, stream, k_map, v_map, a, p) == cudaSuccess ? NVJ_OK
                                                                                                                              : NVJ_ERR_LAUNCH;
 }
 template <typename T>
@@ -891,10 +906,10 @@ static int launch_quantized_umma_shape(const CUtensorMap& k_map, const CUtensorM
   auto columns = [&](auto dim) {
     constexpr int kDim = decltype(dim)::value;
     switch (a.tile_columns) {
-      case 4: return launch_quantized_umma<T, kDim, 4, true>(k_map, v_map, a, p, ranges, stream);
-      case 8: return launch_quantized_umma<T, kDim, 8, true>(k_map, v_map, a, p, ranges, stream);
-      case 16: return launch_quantized_umma<T, kDim, 8, false>(k_map, v_map, a, p, ranges, stream);
-      default: return launch_quantized_umma<T, kDim, 12, false>(k_map, v_map, a, p, ranges, stream);
+      case 4: return launch_quantized_umma<T, kDim, 4, 1>(k_map, v_map, a, p, ranges, stream);
+      case 8: return launch_quantized_umma<T, kDim, 8, 1>(k_map, v_map, a, p, ranges, stream);
+      case 16: return launch_quantized_umma<T, kDim, 8, 2>(k_map, v_map, a, p, ranges, stream);
+      default: return launch_quantized_umma<T, kDim, 8, 3>(k_map, v_map, a, p, ranges, stream);
     }
   };
   return head_dim == 256 ? columns(std::integral_constant<int, 256>{}) : columns(std::integral_constant<int, 128>{});
