@@ -677,9 +677,14 @@ static int run_quantized_umma(const QDecodeParams& q, int q_dtype, int head_dim,
   return launch_after(quantized_umma_fold_kernel, dim3(w.ranges - 1, w.hcts, (w.tile_columns * head_dim / 4 + 255) / 256), dim3(256), 0, stream, a, head_dim) == cudaSuccess ? NVJ_OK : NVJ_ERR_LAUNCH;
 }
 
-// Whether a call goes to the tcgen05 form.
+// Whether a call goes to the tcgen05 form: by the room of its tables, since the lengths are on the GPU.  That form starts and folds 5 us later, and
+// takes 3 - 8 us for a row and head even if they have few keys, but 0.4 - 1.2 us per 128 keys behind them where this file's takes up to 2.8 (head_dim
+// 256).  Over 272 batches of 1 - 512 rows, 64 - 65536 keys, 4 - 80 columns and four head layouts the rule costs 1.5% against the better of both,
+// 30% at most (always this file's form: 23%, always the other: 19%).  Either side of it, us: 64 rows of 64 - 128 keys, 2 heads of 256 and 4
+// columns 10.2 against 14.9, 64 of 1024 - 2048 keys 45 against 27; one row of 4096 keys 11.7 against 15.1, one of 32768 45.9 against 22.6.
 static bool quantized_umma_pays(int rows, int width, int table_width, int block_size, int num_kv_heads, int head_dim, int groups) {
-  return head_dim >= 128 && (long long)rows * table_width * block_size / 16 * num_kv_heads * head_dim >= 1024LL * 512;
+  const long long room = (long long)table_width * block_size, columns = ((long long)width * groups + 3) / 4;
+  return head_dim >= 128 && room >= 320 && (double)rows * room * num_kv_heads * head_dim * columns >= 6 * 1048576.;
 }
 
 }  // namespace nvj
