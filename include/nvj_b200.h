@@ -497,13 +497,14 @@ int nvj_paged_decode_quantized(const void* q, int q_dtype, const void* k_cache_l
  *
  *   single_rows  0: no row holds a single query token; otherwise such rows, if there are any, are served by the decode kernel
  *   tile_pairs   as for nvj_paged_prefill_packed_counted (-1: not counted)
- *   workspace    nullable scratch of nvj_paged_prefill_quantized_workspace_bytes(...): with it, bf16 queries of the model's
- *                shape go to the tcgen05 tiles over bf16 pages that are written there; everything else, and a
- *                call without it, to mma.sync tiles over the 8-bit blocks.  Rows of a single token use it for the decode kernel's
- *                partials.  The size is 0 for calls that have no use for one.
+ *   workspace    nullable scratch of nvj_paged_prefill_quantized_workspace_bytes(...), 16-byte aligned, nothing kept in it between calls:
+ *                with it, bf16 queries of the model's shape go to the tcgen05 tiles over bf16 pages that are written there, up to 1 GiB of
+ *                them; elsewhere the sums of long rows (a call without it is as right, and rounds them a little more).  Rows of a
+ *                single token use it for the decode kernel's partials.
+ *                The size is 0 for calls that have no use for one.
  */
 size_t nvj_paged_prefill_quantized_workspace_bytes(int q_dtype, int rows, int table_width, int block_size, int num_kv_heads,
-                                                   int head_dim, int num_q_heads, float scale, int single_rows);
+                                                   int head_dim, int num_q_heads, float scale, int single_rows, int token_bucket, int tile_pairs);
 int nvj_paged_prefill_quantized(const void* q, int q_dtype, const void* k_cache_layer, const void* v_cache_layer,
                                 const float* k_scale, const float* v_scale, int64_t num_blocks, int block_size,
                                 int num_kv_heads, int head_dim, int num_q_heads, const int32_t* block_tables, int table_width,

@@ -84,7 +84,7 @@ SIGNATURES = {
                                            c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_float, c_void_p,
                                            c_void_p, c_void_p, c_size_t, c_int, c_void_p]),
     "nvj_paged_decode_quantized_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
-    "nvj_paged_prefill_quantized_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int]),
+    "nvj_paged_prefill_quantized_workspace_bytes": (c_size_t, [c_int] * 7 + [c_float] + [c_int] * 3),
     "nvj_paged_prefill_quantized": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_int,
                                             c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_float, c_void_p,
                                             c_void_p, c_void_p, c_size_t, c_int, c_int, c_void_p]),

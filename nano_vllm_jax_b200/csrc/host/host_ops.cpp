@@ -530,7 +530,7 @@ PyObject* quantized_prefill(PyObject* const* a, Py_ssize_t n) {
   int32_t* st = status_for(l.device, stream);
   if (!st) return nullptr;
   at::Tensor out = output({1, tokens, hq * l.d}, l.device);
-  const size_t bytes = lib.quantized_prefill_bytes(dt, rows, width, l.block_size, l.hkv, l.d, (int)hq, (float)scale, (int)singles);
+  const size_t bytes = lib.quantized_prefill_bytes(dt, rows, width, l.block_size, l.hkv, l.d, (int)hq, (float)scale, (int)singles, (int)tokens, (int)pairs);
   at::Tensor scratch;
   if (bytes) scratch = empty({(long long)bytes}, at::kByte, l.device);
   int rc;

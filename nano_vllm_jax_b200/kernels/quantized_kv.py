@@ -189,7 +189,7 @@ def packed_paged_prefill_attention_quantized(query, k_cache_layer, v_cache_layer
 
     Masks and the two counts (`num_decode_rows`: rows of a single query token, `query_tile_pairs`: 64-token tiles of the other
     rows) as in `paged_kv.packed_paged_prefill_attention`.  bfloat16 queries of the model's shape run on the tcgen05 tiles over bf16
-    pages written for the call (exact; up to 1 GiB, from torch's allocator), others on mma.sync tiles over the 8-bit blocks.
+    pages written for the call (exact; up to 1 GiB, from torch's allocator), others on tcgen05 tiles over the 8-bit blocks.
     """
     out = _k.host().quantized_prefill(query, k_cache_layer, v_cache_layer, k_scale, v_scale, block_table, kv_lens, positions, query_start_loc,
                                       block_size, scale, num_key_value_groups, num_decode_rows, query_tile_pairs)
@@ -223,7 +223,7 @@ def packed_paged_prefill_attention_quantized(query, k_cache_layer, v_cache_layer
     singles = -1 if num_decode_rows is None else int(num_decode_rows)
     pairs = -1 if query_tile_pairs is None else int(query_tile_pairs)
     with _on(device):
-        nbytes = lib.nvj_paged_prefill_quantized_workspace_bytes(_k._dt(query), rows, width, page_size, hkv, d, hq, float(scale), singles)
+        nbytes = lib.nvj_paged_prefill_quantized_workspace_bytes(_k._dt(query), rows, width, page_size, hkv, d, hq, float(scale), singles, tokens, pairs)
         scratch = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
         st = _k._status_word(device)
         check(lib.nvj_paged_prefill_quantized(

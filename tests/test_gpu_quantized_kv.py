@@ -534,6 +534,50 @@ def test_packed_prefill_over_many_keys(keys, tokens):
     _check([out[pick]], [q64[0, pick]], state, tables, [keys], [positions[0, pick] + 1], 1 / 16, 16)
 
 
+def _long_prefill(shape, dtype, rows, counts, term_bits, seed, spread=1):
+    """`rows` of (new, cached) tokens, checked at some of their tokens."""
+    hq, hkv, d, bs = shape
+    rng = np.random.default_rng(seed)
+    lens = [n + c for n, c in rows]
+    blocks = sum(-(-n // bs) for n in lens)
+    order, tables, at = rng.permutation(blocks), np.zeros((len(rows), max(-(-n // bs) for n in lens)), np.int64), 0
+    for r, n in enumerate(lens):
+        tables[r, : -(-n // bs)] = order[at: at + -(-n // bs)]
+        at += -(-n // bs)
+    state = [_pool(rng, blocks, shape, spread=spread) for _ in range(2)]
+    _poison_behind(state, tables, lens, bs)
+    (k, ks), (v, vs) = (_gpu(*x) for x in state)
+    total = sum(n for n, _ in rows)
+    q, q64 = _queries(rng, (1, total, hq, d), dtype)
+    positions, qsl = np.concatenate([np.arange(c, c + n) for n, c in rows])[None], np.cumsum([0] + [n for n, _ in rows])
+    out = _f64(Q.packed_paged_prefill_attention_quantized(q, k, v, ks, vs, _i32(tables), _i32(lens), _i32(positions), _i32(qsl), bs, d ** -0.5, hq // hkv,
+                                                          **counts)).reshape(total, hq, d)
+    for r, (n, c) in enumerate(rows):
+        pick = sorted({0, n // 3, 2 * n // 3, n - 1})
+        at = [qsl[r] + i for i in pick]
+        _check([out[at]], [q64[0, at]], state, tables[r: r + 1], lens[r: r + 1], [[c + 1 + i for i in pick]], d ** -0.5, term_bits)
+
+
+# few query tokens: clusters share a tile's keys; at 40000 keys and more each CTA empties its sums into scratch
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("shape", [(32, 8, 128, 16), (16, 1, 256, 16), (24, 2, 128, 64), (6, 6, 64, 48), (8, 2, 256, 32)])
+@pytest.mark.parametrize("rows", [[(2, 700)], [(20, 3000), (3, 17), (5, 0)], [(9, 45000)], [(17, 33000), (2, 70)]])
+def test_prefill_of_few_tokens_over_many_keys(shape, dtype, rows):
+    _long_prefill(shape, dtype, rows, dict(num_decode_rows=0, query_tile_pairs=len(rows)), 22, 31)
+
+
+# tiles enough for every SM: a CTA takes all keys of its rows, and empties its sums into the output every 4096 of them
+@pytest.mark.parametrize("shape,dtype", [((32, 8, 128, 16), F16), ((16, 1, 256, 16), F32), ((16, 8, 64, 32), BF16)])
+def test_prefill_of_many_tokens_over_many_keys(shape, dtype):
+    _long_prefill(shape, dtype, [(610, 8500), (700, 3487)], dict(num_decode_rows=0), 22, 32)
+
+
+# the caller's count of tiles only sets how many CTAs share one: too small, too large or nothing
+@pytest.mark.parametrize("tiles", [None, 0, 1, 10 ** 6])
+def test_prefill_with_any_count_of_tiles(tiles):
+    _long_prefill((32, 8, 128, 16), BF16, [(150, 900), (70, 0), (2, 333)], dict(num_decode_rows=0, query_tile_pairs=tiles), 22, 33)
+
+
 # ------------------------------------------------------------------------------------------------ refusals
 
 def test_wrappers_refuse_what_does_not_fit_together():

@@ -84,11 +84,18 @@ def test_calls_with_nothing_to_do_launch_nothing():
 
 def test_scratch_of_a_prefill():
     size = _lib.load().nvj_paged_prefill_quantized_workspace_bytes
+    # (q type, rows, table width, block size, kv heads, head_dim, query heads, scale, single rows, tokens, 64-token tiles)
     page = 16 * 2 * 256 * 2
-    assert size(0, 3, 100, 16, 2, 256, 8, 0.1, 0) == 300 * 2 * page + 1280
-    assert size(0, 1, 32768, 16, 2, 256, 8, 0.1, 0) > 0 and size(0, 1, 32769, 16, 2, 256, 8, 0.1, 0) == 0  # at most 1 GiB
-    for other in ((1, 16, 2, 256, 8, 0.1), (2, 16, 2, 256, 8, 0.1), (0, 32, 2, 256, 8, 0.1), (0, 16, 2, 128, 8, 0.1), (0, 16, 2, 256, 8, 0.0)):
-        assert size(other[0], 3, 100, *other[1:], 0) == 0
+    assert size(0, 3, 100, 16, 2, 256, 8, 0.1, 0, 64, -1) == 300 * 2 * page + 1280
+    sums = 4 * 8 * 2 * 128 * 256 * 4  # long rows of few tokens: what a cluster's CTAs have summed
+    assert size(0, 1, 32768, 16, 2, 256, 8, 0.1, 0, 64, -1) > sums and size(0, 1, 32769, 16, 2, 256, 8, 0.1, 0, 64, -1) == sums  # at most 1 GiB
+    assert size(1, 1, 1024, 16, 2, 256, 8, 0.1, 0, 64, -1) == sums == size(1, 1, 1024, 16, 2, 256, 8, 0.1, 0, 64, 1)
+    assert size(0, 1, 1024, 16, 2, 256, 8, 0.0, 0, 64, -1) == sums
+    assert size(1, 1, 512, 16, 2, 256, 8, 0.1, 0, 64, -1) == 0  # not long enough
+    assert size(1, 1, 1024, 16, 2, 256, 8, 0.1, 0, 8192, -1) == 0  # tiles enough without clusters
+    assert size(1, 1, 1024, 16, 2, 100, 8, 0.1, 0, 64, -1) == 0 and size(1, 0, 1024, 16, 2, 256, 8, 0.1, 0, 64, -1) == 0
+    decode = _lib.load().nvj_paged_decode_quantized_workspace_bytes(64, 1, 256, 16, 2, 256, 8, 0)  # (0 without a GPU)
+    assert size(1, 64, 256, 16, 2, 256, 8, 0.1, 5, 64, -1) >= decode
 
 
 def test_wrappers_refuse_tensors_that_are_not_on_a_gpu():
