@@ -9,8 +9,9 @@
 // A tile of 64 keys takes 4 * 128 * 64 * head_dim flops for S and twice that for O's two terms: 2200 cycles of an SM at head_dim 256.  What
 // bounds the kernel is the conversion: a loader's 16 pieces of a tile 1700 cycles (13 per pair of numbers), with their addresses, copies and
 // waits 3400.  Against the tiles of mma.sync that stood here before: 1984 f16 tokens behind 727, 32 heads of 128 over 8, 452 -> 185 us;
-// 1018 tokens of four rows behind 1232 each 165 -> 75; 55 f32 tokens of two rows behind 1214 (8 heads of 256 over 2) 160 -> 30; 54 tokens
-// behind 1398 (16 heads of 64 over 2) 62 -> 15; the smallest calls of head_dim 256 4 us slower (17.7 -> 21.7).
+// 1018 tokens of four rows behind 1232 each 165 -> 76; 55 f32 tokens of two rows behind 1214 (8 heads of 256 over 2) 160 -> 29; 54 tokens
+// behind 1398 (16 heads of 64 over 2) 62 -> 16; the smallest calls as long as they took (20 tokens, heads of 256: 17.7 -> 17.4).  A
+// small call at head_dim 256 is start and end: row and lengths 2.4 us, queries 3.6, a tile 2, rows staged 3, folded over DSMEM 5.
 //
 // CTA: 128 query rows (token major, a kv head's `groups` heads minor) of one table row and kv head.  While that gives fewer tiles than the GPU
 // has room for, a tile's keys are split over a cluster of up to eight CTAs, which fold their rows through each other's shared memory.
@@ -185,6 +186,45 @@ __device__ __forceinline__ void qt_loaders(QtSmem<T, kD>& sm, const QtParams& p,
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
+
+// ---- queries: 8 dims a lane, so many rows of a warp at a time -----------------------------------------------------------------------------
+template <typename T, int kD>
+struct QtQueries {
+  static constexpr int kWarps = 10, kLanes = kD / 8, kAtOnce = 32 / kLanes;
+  static constexpr int kAll = (kQtRows + kWarps * kAtOnce - 1) / (kWarps * kAtOnce);  // passes of a warp
+  static constexpr int kMost = sizeof(T) == 4 ? 4 : 7, kRounds = kAll < kMost ? kAll : kMost;  // of them on their way at a time
+  static __device__ __forceinline__ int row_of(int round, int warp, int lane) { return (round * kWarps + warp) * kAtOnce + lane / kLanes; }
+  // Times a power of two per row that makes the largest 2^14 - 2^15.
+  static __device__ __forceinline__ void store(QtSmem<T, kD>& sm, const QRaw<T>& raw, int r, int lane, float scale_log2) {
+    float x[8];
+    q_floats(raw, x);
+    int bits = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) bits = max(bits, __float_as_int(x[k]) & 0x7fffffff);
+    if constexpr (kLanes == 32) {
+      bits = __reduce_max_sync(kFullMask, bits);
+    } else {
+#pragma unroll
+      for (int o = kLanes / 2; o > 0; o >>= 1) bits = max(bits, __shfl_xor_sync(kFullMask, bits, o));
+    }
+    const bool odd = bits >= 0x7f800000;  // an infinity or NaN: the row's scores are NaN
+    int e = (bits >> 23) - 127 - 14;
+    e = bits == 0 || odd ? 0 : (e < -126 ? -126 : e);
+    const float down = q_pow2(-e);
+    if (r >= kQtRows) return;
+    if (lane % kLanes == 0) sm.factor[r] = odd ? __int_as_float(0x7fffffff) : q_pow2(e) * scale_log2;
+    uint32_t w[4], low[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float a = x[2 * k] * down, b = x[2 * k + 1] * down;
+      w[k] = q_pair(a, b);
+      low[k] = q_pair_rest(a, b, w[k]);
+    }
+    const int d = 8 * (lane % kLanes), at = r * 128 + (((d % 64 / 8) ^ (r & 7)) << 4);
+    *reinterpret_cast<uint4*>(sm.q[0][d / 64] + at) = make_uint4(w[0], w[1], w[2], w[3]);
+    if constexpr (QtSmem<T, kD>::kQTerms == 2) *reinterpret_cast<uint4*>(sm.q[1][d / 64] + at) = make_uint4(low[0], low[1], low[2], low[3]);
+  }
+};
 
 // ---- warps 8 and 9 --------------------------------------------------------------------------------------------------------------
 template <typename T, int kD>
@@ -460,6 +500,20 @@ __global__ void __launch_bounds__(kQtThreads, 1) quantized_prefill_umma_kernel(c
     if (tid == 0) atomicOr(p.status, NVJ_DEV_BAD_LENGTH);
     len = p.table_width * p.block_size;
   }
+  // queries on their way before anything else is asked for
+  using Q = QtQueries<T, kD>;
+  auto query = [&](int r) {
+    const int at = first_row + r;
+    QRaw<T> raw{};
+    if (r < kQtRows && at < query_rows)
+      raw = q_load8(static_cast<const T*>(p.q) + ((long long)(token0 + at / p.groups) * hq + head * p.groups + at % p.groups) * kD + 8 * (lane % Q::kLanes));
+    return raw;
+  };
+  QRaw<T> queries[Q::kRounds];
+  if (warp < 10) {
+#pragma unroll
+    for (int u = 0; u < Q::kRounds; ++u) queries[u] = query(Q::row_of(u, warp, lane));
+  }
   if (tid < kQtRows) {  // how many keys the tile's rows see
     const int at = first_row + tid;
     int limit = 0;
@@ -484,47 +538,13 @@ __global__ void __launch_bounds__(kQtThreads, 1) quantized_prefill_umma_kernel(c
     if (tiles > 0 && warp >= 12) qt_loaders<true>(sm, p, row, head, len, tile0, tiles, tid - 384);
     else if (tiles > 0) qt_loaders<false>(sm, p, row, head, len, tile0, tiles, tid - 320);
   } else {
-    // queries: 8 dims a lane, so many rows of a warp at a time, times a power of two per row that makes the largest 2^14 - 2^15
-    constexpr int kLanes = kD / 8, kAtOnce = 32 / kLanes;
-    constexpr int kRounds = sizeof(T) == 4 ? 2 : 4;  // on their way at a time
-#pragma unroll 1
-    for (int i0 = warp * kAtOnce; tiles > 0 && i0 < kQtRows; i0 += 10 * kAtOnce * kRounds) {
-      QRaw<T> raw[kRounds];
+    for (int i0 = 0; tiles > 0; ) {
 #pragma unroll
-      for (int u = 0; u < kRounds; ++u) {
-        const int r = i0 + u * 10 * kAtOnce + lane / kLanes, at = first_row + r;
-        raw[u] = QRaw<T>{};
-        if (r < kQtRows && at < query_rows)
-          raw[u] = q_load8(static_cast<const T*>(p.q) + ((long long)(token0 + at / p.groups) * hq + head * p.groups + at % p.groups) * kD + 8 * (lane % kLanes));
-      }
+      for (int u = 0; u < Q::kRounds; ++u) Q::store(sm, queries[u], Q::row_of(i0 + u, warp, lane), lane, p.scale_log2);
+      i0 += Q::kRounds;
+      if (i0 >= Q::kAll) break;
 #pragma unroll
-      for (int u = 0; u < kRounds; ++u) {
-        const int r = i0 + u * 10 * kAtOnce + lane / kLanes;
-        float x[8];
-        q_floats(raw[u], x);
-        int bits = 0;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) bits = max(bits, __float_as_int(x[k]) & 0x7fffffff);
-#pragma unroll
-        for (int o = kLanes / 2; o > 0; o >>= 1) bits = max(bits, __shfl_xor_sync(kFullMask, bits, o));
-        const bool odd = bits >= 0x7f800000;  // an infinity or NaN: the row's scores are NaN
-        int e = (bits >> 23) - 127 - 14;
-        e = bits == 0 || odd ? 0 : (e < -126 ? -126 : e);
-        const float down = q_pow2(-e);
-        if (r < kQtRows) {
-          if (lane % kLanes == 0) sm.factor[r] = odd ? __int_as_float(0x7fffffff) : q_pow2(e) * p.scale_log2;
-          uint32_t w[4], low[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float a = x[2 * k] * down, b = x[2 * k + 1] * down;
-            w[k] = q_pair(a, b);
-            low[k] = q_pair_rest(a, b, w[k]);
-          }
-          const int d = 8 * (lane % kLanes), at = r * 128 + (((d % 64 / 8) ^ (r & 7)) << 4);
-          *reinterpret_cast<uint4*>(sm.q[0][d / 64] + at) = make_uint4(w[0], w[1], w[2], w[3]);
-          if constexpr (L::kQTerms == 2) *reinterpret_cast<uint4*>(sm.q[1][d / 64] + at) = make_uint4(low[0], low[1], low[2], low[3]);
-        }
-      }
+      for (int u = 0; u < Q::kRounds; ++u) queries[u] = query(Q::row_of(i0 + u, warp, lane));
     }
     fence_proxy_async_smem();
     named_bar_sync(5, kQtSoftmax + 64);
@@ -540,7 +560,7 @@ __global__ void __launch_bounds__(kQtThreads, 1) quantized_prefill_umma_kernel(c
       QtRow o;
       const bool alive = qt_softmax(sm, p, my_tmem, tile0, tiles, r, half, warp & 3, flush_row, flush, o);
       // (the staged rows take the place of the queries, keys and values of all rows: every product has to be over)
-      if (splits > 1) named_bar_sync(6, kQtSoftmax);
+      named_bar_sync(6, kQtSoftmax);
       if (alive) {
         const float sums_log = o.m - o.v_first;  // what the row's sum is relative to
         const float f = splits > 1 ? 1.f : o.l == 0.f ? 0.f : ex2_approx(o.v_first) / o.l;
@@ -566,7 +586,7 @@ __global__ void __launch_bounds__(kQtThreads, 1) quantized_prefill_umma_kernel(c
               }
               z = make_float4(z.x * f, z.y * f, z.z * f, z.w * f);
             }
-            *reinterpret_cast<float4*>(splits > 1 ? stage + qt_piece<kD>(r, c / 4 + j) : out_row + c + 4 * j) = z;
+            *reinterpret_cast<float4*>(stage + qt_piece<kD>(r, c / 4 + j)) = z;
           }
         }
       } else if (splits > 1) {  // (the others fold without it; the status says so)
@@ -580,19 +600,32 @@ __global__ void __launch_bounds__(kQtThreads, 1) quantized_prefill_umma_kernel(c
   tc_fence_before_sync();
   __syncthreads();
   bool odd = false;
-  if (splits > 1) {
+  constexpr int kLanes = kD / 4 < 32 ? kD / 4 : 32, kHalves = kD / 4 / kLanes;  // of a warp, a piece of the row each; head_dim 256: two
+  constexpr int kWarps = kQtThreads / 32;
+  auto out_of = [&](int r) {
+    const int at = first_row + r;
+    return reinterpret_cast<float4*>(p.out + ((long long)(token0 + at / p.groups) * hq + head * p.groups + at % p.groups) * kD);
+  };
+  const int last_row = min(query_rows - first_row, kQtRows);
+  if (splits == 1) {
+    if (lane < kLanes && !sm.abort_flag) {
+#pragma unroll 4
+      for (int i = warp; i < last_row * kHalves; i += kWarps) {
+        const int piece = i % kHalves * kLanes + lane;
+        out_of(i / kHalves)[piece] = *reinterpret_cast<const float4*>(stage + qt_piece<kD>(i / kHalves, piece));
+      }
+    }
+  } else {
     cl_sync();  // every CTA's rows are staged
-    const int row0 = rank * kQtRows / splits, row1 = (rank + 1) * kQtRows / splits;
-    constexpr int kLanes = kD / 4 < 32 ? kD / 4 : 32;  // of a warp, a piece of the row each; head_dim 256: two
-    for (int r = row0 + warp; r < row1; r += kQtThreads / 32) {
-      const int at = first_row + r;
-      if (at >= query_rows) continue;
-      // lane s: CTA s's weight in this row
+    const int row0 = rank * kQtRows / splits, row1 = min((rank + 1) * kQtRows / splits, last_row);
+    // four rows of a warp at a time: lane 8 i + s has CTA s's reference, sum and, in the end, weight in row i of them
+    for (int first = row0 + 4 * warp; first < row1; first += 4 * kWarps) {
+      const int mine = first + lane / kQtMostSplits, s = lane % kQtMostSplits;
       float2 e = make_float2(kQtNone, 0.f);
       float mv = kQtNone;
-      if (lane < parts) {
-        e = cl_ld2(cl_map(&ml[r], lane));
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(mv) : "r"(cl_map(&mv_of[r], lane)) : "memory");
+      if (s < parts && mine < row1) {
+        e = cl_ld2(cl_map(&ml[mine], s));
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(mv) : "r"(cl_map(&mv_of[mine], s)) : "memory");
       }
       const bool none = e.y == 0.f;
       float top = none ? kQtNone : e.x;
@@ -602,26 +635,34 @@ __global__ void __launch_bounds__(kQtThreads, 1) quantized_prefill_umma_kernel(c
 #pragma unroll
       for (int o = 1; o < kQtMostSplits; o <<= 1) sum += __shfl_xor_sync(kFullMask, sum, o);
       const float f = none ? 0.f : ex2_approx(mv - top) / sum;
-      const unsigned real = __ballot_sync(kFullMask, !none) & ((1u << kQtMostSplits) - 1);
-      float* to = p.out + ((long long)(token0 + at / p.groups) * hq + head * p.groups + at % p.groups) * kD;
-#pragma unroll 1
-      for (int h = 0; h < kD / 4; h += kLanes) {
-        float4 x[kQtMostSplits];
-#pragma unroll
-        for (int s = 0; s < kQtMostSplits; ++s) {
-          x[s] = make_float4(0.f, 0.f, 0.f, 0.f);
-          if ((real >> s & 1) && lane < kLanes) x[s] = cl_ld4(cl_map(stage + qt_piece<kD>(r, h + lane), s));
-        }
-        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int s = 0; s < kQtMostSplits; ++s) {
-          const float g = __shfl_sync(kFullMask, f, s);
-          if (real >> s & 1) y = make_float4(fmaf(x[s].x, g, y.x), fmaf(x[s].y, g, y.y), fmaf(x[s].z, g, y.z), fmaf(x[s].w, g, y.w));
-        }
-        odd |= cl_not_finite(y);
-        if (lane < kLanes) reinterpret_cast<float4*>(to)[h + lane] = y;
-      }
+      const unsigned real = __ballot_sync(kFullMask, !none);
       odd |= !(f <= 1.f) || !(mv <= 3e38f);
+      const int items = min(4, row1 - first) * kHalves;
+#pragma unroll 1
+      for (int i = 0; i < items; i += 2) {  // two pieces' loads at a time
+        float4 x[2][kQtMostSplits];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int k = (i + u) / kHalves, piece = (i + u) % kHalves * kLanes + lane;
+#pragma unroll
+          for (int c = 0; c < kQtMostSplits; ++c) {
+            x[u][c] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (i + u < items && (real >> (k * kQtMostSplits + c) & 1) && lane < kLanes) x[u][c] = cl_ld4(cl_map(stage + qt_piece<kD>(first + k, piece), c));
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int k = min((i + u) / kHalves, 3);
+          float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int c = 0; c < kQtMostSplits; ++c) {
+            const float g = __shfl_sync(kFullMask, f, k * kQtMostSplits + c);
+            if (real >> (k * kQtMostSplits + c) & 1) y = make_float4(fmaf(x[u][c].x, g, y.x), fmaf(x[u][c].y, g, y.y), fmaf(x[u][c].z, g, y.z), fmaf(x[u][c].w, g, y.w));
+          }
+          odd |= cl_not_finite(y);
+          if (i + u < items && lane < kLanes) out_of(first + k)[(i + u) % kHalves * kLanes + lane] = y;
+        }
+      }
     }
   }
   if (sm.abort_flag) {  // give MMAs in flight time to land before the CTA's memory is released
