@@ -1,11 +1,13 @@
 // Append of new K/V rows to the 8-bit paged cache (quantized_kv.cuh).
 //
 // A block's tokens share a scale per kv head, so the unit of work is not a token but a run: the tokens of one call that stand
-// together in the batch and fall into one block.  One warp takes a run's rows of K, or of V, of one kv head: it finds their largest
-// magnitude in registers, settles the block's scale, rescales the rows that were there if the scale has to grow, and stores the new
-// ones.  K and V, and the heads, are warps of their own; nothing is shared between warps, so there are no atomics and no
-// second pass over memory.  bytes = tokens * kv_heads * head_dim * 2 * (source size + 1), bound by HBM for prompts, by the chain
-// positions -> block id -> scale -> store for a decode step.
+// together in the batch and fall into one block.  A run's rows of K, or of V, of one kv head are taken by one warp (batches of a few tokens per
+// row) or by a CTA of four (prompts): their largest magnitude, found in registers, settles the block's scale; the rows that were there are
+// rescaled if it has to grow, and the new ones stored.  K and V, the heads and the runs have nothing in common, so there are no
+// atomics and no second pass over memory.
+// bytes = tokens * kv_heads * head_dim * 2 * (source size + 1).  Prompts are bound by HBM and, in front of it, by the chain positions -> block id ->
+// scale -> stores: 16384 bf16 tokens of 2 heads of 256 14.7 us (50 MB: 7.7 us); with a warp per run, 126 registers of held rows and so half
+// of the CTAs in a second wave, 18.4.  A decode step is launch and chain: 256 tokens 3.5 us.
 
 #include "quantized_kv.cuh"
 
@@ -38,7 +40,7 @@ __device__ __forceinline__ QToken q_token(const QAppendParams& p, int i) {
   QToken t{-1, 0};
   if (i < 0 || i >= p.n_tokens) return t;
   const int pos = p.positions[i];
-  int row = p.packed ? p.token_row_ids[i] : i / p.n_cols;
+  const int row = p.packed ? p.token_row_ids[i] : i / p.n_cols;
   if (p.query_start_loc) {
     if (p.packed) {
       if (i >= p.query_start_loc[p.qsl_rows]) return t;
@@ -60,22 +62,25 @@ __device__ __forceinline__ QToken q_token(const QAppendParams& p, int i) {
   return t;
 }
 
-// One run: `n` tokens from `first` on, offsets[] as q_token gives them.  kLanes lanes hold a row of 8 * kLanes elements.
-template <typename T, int kD>
-__device__ void q_append_run(const QAppendParams& p, int first, int n, long long entry, int head, bool is_v, int lane) {
+// One run: `n` tokens from `first` on, of table entry `entry`, by kShare warps that meet at the CTA's barrier.  kLanes lanes hold a row of
+// 8 * kLanes elements; a warp takes every kShare-th step of its rows.
+template <typename T, int kD, int kShare>
+__device__ void q_append_run(const QAppendParams& p, int first, int n, long long entry, int head, bool is_v, int warp, int lane) {
   constexpr int kLanes = kD / 8, kRows = 32 / kLanes;  // lanes of a row, rows of a step
-  constexpr int kHold = sizeof(T) == 4 ? 8 : 16;       // steps whose rows stay in registers between the two looks at them
-  const int col = (lane % kLanes) * 8, sub = lane / kLanes;
+  constexpr int kHold = 4;                             // steps whose rows stay in registers between the two looks at them
+  __shared__ float largest_of[kShare];
+  const int col = (lane % kLanes) * 8, sub = warp * kRows + lane / kLanes;
+  constexpr int kNext = kShare * kRows;  // rows from one step to the next
   const long long token_stride = (long long)p.num_kv_heads * kD;
   const T* src = static_cast<const T*>(is_v ? p.new_v : p.new_k) + (long long)first * token_stride + (long long)head * kD + col;
   const int id = p.block_tables[entry];
-  const int steps = (n + kRows - 1) / kRows;
+  const int steps = (n + kNext - 1) / kNext;
   QRaw<T> held[kHold];
 #pragma unroll
   for (int s = 0; s < kHold; ++s)
-    if (s < steps && s * kRows + sub < n) held[s] = q_load8(src + (long long)(s * kRows + sub) * token_stride);
+    if (s * kNext + sub < n) held[s] = q_load8(src + (long long)(s * kNext + sub) * token_stride);
   if (id < 0 || id >= p.num_blocks) {
-    if (lane == 0) atomicOr(p.status, NVJ_DEV_BAD_BLOCK_ID);
+    if (warp == 0 && lane == 0) atomicOr(p.status, NVJ_DEV_BAD_BLOCK_ID);
     return;
   }
   float* scale_at = (is_v ? p.v_scale : p.k_scale) + (long long)id * p.num_kv_heads + head;
@@ -83,8 +88,10 @@ __device__ void q_append_run(const QAppendParams& p, int first, int n, long long
   // the offsets of up to 32 tokens at a time, one per lane; whether the block begins here, and which of its rows are new
   bool begins = false;
   unsigned fresh[2] = {0u, 0u};  // offsets 0 - 31 and 32 - 63
+  int my_offset = 0;             // of token first + lane
   for (int c = 0; c < n; c += 32) {
     const int o = c + lane < n ? p.positions[first + c + lane] % p.block_size : -1;
+    if (c == 0) my_offset = o;
     begins |= __any_sync(kFullMask, o == 0);
     fresh[0] |= __reduce_or_sync(kFullMask, o >= 0 && o < 32 ? 1u << o : 0u);
     fresh[1] |= __reduce_or_sync(kFullMask, o >= 32 ? 1u << (o - 32) : 0u);
@@ -92,23 +99,30 @@ __device__ void q_append_run(const QAppendParams& p, int first, int n, long long
   float largest = 0.f, x[8];
 #pragma unroll
   for (int s = 0; s < kHold; ++s)
-    if (s < steps && s * kRows + sub < n) {
+    if (s * kNext + sub < n) {
       q_floats(held[s], x);
       largest = q_largest(largest, x);
     }
   for (int s = kHold; s < steps; ++s)
-    if (s * kRows + sub < n) {
-      q_floats(q_load8(src + (long long)(s * kRows + sub) * token_stride), x);
+    if (s * kNext + sub < n) {
+      q_floats(q_load8(src + (long long)(s * kNext + sub) * token_stride), x);
       largest = q_largest(largest, x);
     }
   largest = __int_as_float(__reduce_max_sync(kFullMask, __float_as_int(largest)));
+  if constexpr (kShare > 1) {
+    if (lane == 0) largest_of[warp] = largest;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kShare; ++w) largest = fmaxf(largest, largest_of[w]);
+    __syncthreads();  // (before the next run's)
+  }
   const float wanted = q_scale_for(largest);
   const float scale = begins ? wanted : fmaxf(wanted, before);
   uint8_t* base = (is_v ? p.v_cache : p.k_cache) + ((long long)id * p.block_size * p.num_kv_heads + head) * kD + col;
-  if (scale != before && lane == 0) *scale_at = scale;
+  if (scale != before && warp == 0 && lane == 0) *scale_at = scale;
   if (!begins && scale > before) {  // the rows that were there, in the new unit
     const float ratio = before / scale;
-    for (int o = sub; o < p.block_size; o += kRows) {
+    for (int o = sub; o < p.block_size; o += kNext) {
       if (fresh[o >> 5] >> (o & 31) & 1) continue;
       uint2* at = reinterpret_cast<uint2*>(base + (long long)o * token_stride);
       const uint2 w = *at;
@@ -118,32 +132,44 @@ __device__ void q_append_run(const QAppendParams& p, int first, int n, long long
     }
   }
   const float inverse = 1.f / scale;
-  auto store = [&](int r, const QRaw<T>& raw) {
+  auto store = [&](int o, const QRaw<T>& raw) {
     q_floats(raw, x);
-    const int o = p.positions[first + r] % p.block_size;
     *reinterpret_cast<uint2*>(base + (long long)o * token_stride) =
         make_uint2(q_pack2(x[0] * inverse, x[1] * inverse) | q_pack2(x[2] * inverse, x[3] * inverse) << 16,
                    q_pack2(x[4] * inverse, x[5] * inverse) | q_pack2(x[6] * inverse, x[7] * inverse) << 16);
   };
 #pragma unroll
-  for (int s = 0; s < kHold; ++s)
-    if (s < steps && s * kRows + sub < n) store(s * kRows + sub, held[s]);
-  for (int s = kHold; s < steps; ++s)
-    if (s * kRows + sub < n) store(s * kRows + sub, q_load8(src + (long long)(s * kRows + sub) * token_stride));
+  for (int s = 0; s < kHold; ++s) {
+    const int r = s * kNext + sub, o = __shfl_sync(kFullMask, my_offset, r & 31);
+    if (r < n) store(r < 32 ? o : p.positions[first + r] % p.block_size, held[s]);
+  }
+  for (int s = kHold; s < steps; ++s) {
+    const int r = s * kNext + sub;
+    if (r < n) store(p.positions[first + r] % p.block_size, q_load8(src + (long long)r * token_stride));
+  }
 }
 
-// Grid x: windows of `window` tokens; grid y: the (K or V, head) pairs, a warp each.  A warp takes the runs that begin in its window one
-// behind the other.
+// Grid x: windows of `window` tokens; the CTA takes the runs that begin in its window one behind the other.  kShare 1: a warp for each (K or V,
+// head), grid y counts them in fours; 4: the CTA's warps share the runs of one.
 constexpr int kQAppendWarps = 4;
-template <typename T, int kD>
+template <typename T, int kD, int kShare>
 __global__ void __launch_bounds__(32 * kQAppendWarps) quantized_append_kernel(QAppendParams p, int window) {
   pdl_wait();
   pdl_release();
-  const int lane = threadIdx.x & 31, part = blockIdx.y * kQAppendWarps + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = kShare > 1 ? (int)blockIdx.y : (int)blockIdx.y * kQAppendWarps + warp;
   const int base = blockIdx.x * window;  // first token of the window
   const int head = part >> 1;
   const bool is_v = part & 1;
   if (head >= p.num_kv_heads) return;
+  if constexpr (kShare > 1) {  // a prompt: the window's rows on their way to the L2 while their places are looked up
+    constexpr int kLines = kD * (int)sizeof(T) / 128;
+    const char* from = static_cast<const char*>(is_v ? p.new_v : p.new_k);
+    for (int i = threadIdx.x; i < window * kLines; i += 32 * kQAppendWarps) {
+      const long long token = base + i / kLines;
+      if (token < p.n_tokens)
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(from + (token * p.num_kv_heads + head) * kD * (long long)sizeof(T) + i % kLines * 128));
+    }
+  }
   // lane l looks at token base - 1 + l: the one in front tells whether the window's first token begins a run
   const QToken t = q_token(p, base - 1 + lane);
   const long long in_front = __shfl_up_sync(kFullMask, t.entry, 1);
@@ -165,23 +191,28 @@ __global__ void __launch_bounds__(32 * kQAppendWarps) quantized_append_kernel(QA
         if (add < 32) break;
       }
     }
-    q_append_run<T, kD>(p, first, n, entry, head, is_v, lane);
+    q_append_run<T, kD, kShare>(p, first, n, entry, head, is_v, kShare > 1 ? warp : 0, lane);
   }
 }
 
 template <typename T>
 static int launch_quantized_append(const QAppendParams& p, int head_dim, cudaStream_t stream) {
   // Batches of a few tokens per row: a run per window.  Prompts: windows of 16 tokens, in which one run begins, mostly (a window per token: 37 us
-  // for 16384 tokens, most of it warps that find nothing to do).
+  // for 16384 tokens, most of it warps that find nothing to do; windows of 31: 16.5 against 14.7).
   const long long rows = p.packed ? p.qsl_rows : (p.n_tokens + p.n_cols - 1) / p.n_cols;
-  const int window = p.n_tokens <= 4 * (rows > 0 ? rows : 1) ? 1 : 16;
-  const dim3 grid((p.n_tokens + window - 1) / window, (2 * p.num_kv_heads + kQAppendWarps - 1) / kQAppendWarps);
+  const bool prompt = p.n_tokens > 4 * (rows > 0 ? rows : 1);
+  const int window = prompt ? 16 : 1, parts = 2 * p.num_kv_heads;
+  const dim3 grid((p.n_tokens + window - 1) / window, prompt ? parts : (parts + kQAppendWarps - 1) / kQAppendWarps);
   auto go = [&](auto* kernel) {
     return launch_after(kernel, grid, dim3(32 * kQAppendWarps), 0, stream, p, window) == cudaSuccess ? NVJ_OK : NVJ_ERR_LAUNCH;
   };
-  if (head_dim == 256) return go(quantized_append_kernel<T, 256>);
-  if (head_dim == 128) return go(quantized_append_kernel<T, 128>);
-  return go(quantized_append_kernel<T, 64>);
+  auto dims = [&](auto share) {
+    constexpr int kShare = decltype(share)::value;
+    if (head_dim == 256) return go(quantized_append_kernel<T, 256, kShare>);
+    if (head_dim == 128) return go(quantized_append_kernel<T, 128, kShare>);
+    return go(quantized_append_kernel<T, 64, kShare>);
+  };
+  return prompt ? dims(std::integral_constant<int, kQAppendWarps>{}) : dims(std::integral_constant<int, 1>{});
 }
 
 }  // namespace nvj
