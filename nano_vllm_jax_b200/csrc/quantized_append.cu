@@ -30,14 +30,53 @@ struct QAppendParams {
   int qsl_rows, packed, n_tokens, n_cols, table_rows, table_width, block_size, num_kv_heads;
 };
 
+// Block and offset of a position, for the block sizes that there are (a division by a number that is not known: ~25 instructions of a kernel that
+// is bound by them).
+__device__ __forceinline__ int q_block_of(int pos, int block_size) {
+  return block_size == 48 ? (int)__umulhi((unsigned)pos >> 4, 0x55555556u) : (int)((unsigned)pos >> (31 - __clz(block_size)));
+}
+__device__ __forceinline__ int q_offset_of(int pos, int block_size) { return pos - q_block_of(pos, block_size) * block_size; }
+
+// The largest magnitude of raw rows, two numbers an instruction; NaN does not count, infinity does (and is looked for then).
+template <typename T>
+struct QMost {
+  __nv_bfloat162 m = __floats2bfloat162_rn(0.f, 0.f);
+  __device__ __forceinline__ void add(const QRaw<T>& r) {
+    const uint32_t w[4] = {r.v.x, r.v.y, r.v.z, r.v.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) m = __hmax2(m, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[k])));
+  }
+  __device__ __forceinline__ float value() const { return fmaxf(__low2float(m), __high2float(m)); }
+};
+template <>
+struct QMost<__half> {
+  __half2 m = __floats2half2_rn(0.f, 0.f);
+  __device__ __forceinline__ void add(const QRaw<__half>& r) {
+    const uint32_t w[4] = {r.v.x, r.v.y, r.v.z, r.v.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) m = __hmax2(m, __habs2(*reinterpret_cast<const __half2*>(&w[k])));
+  }
+  __device__ __forceinline__ float value() const { return fmaxf(__low2float(m), __high2float(m)); }
+};
+template <>
+struct QMost<float> {
+  float m = 0.f;
+  __device__ __forceinline__ void add(const QRaw<float>& r) {
+    float x[8];
+    q_floats(r, x);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) m = fmaxf(m, fabsf(x[k]));
+  }
+  __device__ __forceinline__ float value() const { return m; }
+};
+
 // What a lane knows about one token of the batch: its row's place in the block table, or -1 for a token that is not written.
 struct QToken {
   long long entry;  // row * table_width + block of the row
-  int offset;       // within the block
 };
 
 __device__ __forceinline__ QToken q_token(const QAppendParams& p, int i) {
-  QToken t{-1, 0};
+  QToken t{-1};
   if (i < 0 || i >= p.n_tokens) return t;
   const int pos = p.positions[i];
   const int row = p.packed ? p.token_row_ids[i] : i / p.n_cols;
@@ -53,12 +92,12 @@ __device__ __forceinline__ QToken q_token(const QAppendParams& p, int i) {
     return t;
   }
   if (p.seq_lens && p.seq_lens[row] <= 0) return t;
-  if (pos < 0 || pos / p.block_size >= p.table_width) {
+  const int block = q_block_of(pos, p.block_size);
+  if (pos < 0 || block >= p.table_width) {
     atomicOr(p.status, NVJ_DEV_BAD_LENGTH);
     return t;
   }
-  t.entry = (long long)row * p.table_width + pos / p.block_size;
-  t.offset = pos % p.block_size;
+  t.entry = (long long)row * p.table_width + block;
   return t;
 }
 
@@ -90,31 +129,40 @@ __device__ void q_append_run(const QAppendParams& p, int first, int n, long long
   unsigned fresh[2] = {0u, 0u};  // offsets 0 - 31 and 32 - 63
   int my_offset = 0;             // of token first + lane
   for (int c = 0; c < n; c += 32) {
-    const int o = c + lane < n ? p.positions[first + c + lane] % p.block_size : -1;
+    const int o = c + lane < n ? q_offset_of(p.positions[first + c + lane], p.block_size) : -1;
     if (c == 0) my_offset = o;
     begins |= __any_sync(kFullMask, o == 0);
     fresh[0] |= __reduce_or_sync(kFullMask, o >= 0 && o < 32 ? 1u << o : 0u);
     fresh[1] |= __reduce_or_sync(kFullMask, o >= 32 ? 1u << (o - 32) : 0u);
   }
-  float largest = 0.f, x[8];
+  float x[8];
+  auto over_all = [&](float mine) {  // the largest of the run's
+    mine = __int_as_float(__reduce_max_sync(kFullMask, __float_as_int(mine)));
+    if constexpr (kShare > 1) {
+      if (lane == 0) largest_of[warp] = mine;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < kShare; ++w) mine = fmaxf(mine, largest_of[w]);
+      __syncthreads();  // (before it is written again)
+    }
+    return mine;
+  };
+  QMost<T> most;
 #pragma unroll
   for (int s = 0; s < kHold; ++s)
-    if (s * kNext + sub < n) {
-      q_floats(held[s], x);
-      largest = q_largest(largest, x);
-    }
+    if (s * kNext + sub < n) most.add(held[s]);
   for (int s = kHold; s < steps; ++s)
-    if (s * kNext + sub < n) {
-      q_floats(q_load8(src + (long long)(s * kNext + sub) * token_stride), x);
-      largest = q_largest(largest, x);
-    }
-  largest = __int_as_float(__reduce_max_sync(kFullMask, __float_as_int(largest)));
-  if constexpr (kShare > 1) {
-    if (lane == 0) largest_of[warp] = largest;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kShare; ++w) largest = fmaxf(largest, largest_of[w]);
-    __syncthreads();  // (before the next run's)
+    if (s * kNext + sub < n) most.add(q_load8(src + (long long)(s * kNext + sub) * token_stride));
+  float largest = over_all(most.value());
+  if (largest == INFINITY) {  // rarely: the finite ones
+    float finite = 0.f;
+#pragma unroll 1
+    for (int s = 0; s < steps; ++s)
+      if (s * kNext + sub < n) {
+        q_floats(q_load8(src + (long long)(s * kNext + sub) * token_stride), x);
+        finite = q_largest(finite, x);
+      }
+    largest = over_all(finite);
   }
   const float wanted = q_scale_for(largest);
   const float scale = begins ? wanted : fmaxf(wanted, before);
@@ -141,11 +189,11 @@ __device__ void q_append_run(const QAppendParams& p, int first, int n, long long
 #pragma unroll
   for (int s = 0; s < kHold; ++s) {
     const int r = s * kNext + sub, o = __shfl_sync(kFullMask, my_offset, r & 31);
-    if (r < n) store(r < 32 ? o : p.positions[first + r] % p.block_size, held[s]);
+    if (r < n) store(r < 32 ? o : q_offset_of(p.positions[first + r], p.block_size), held[s]);
   }
   for (int s = kHold; s < steps; ++s) {
     const int r = s * kNext + sub;
-    if (r < n) store(p.positions[first + r] % p.block_size, q_load8(src + (long long)r * token_stride));
+    if (r < n) store(q_offset_of(p.positions[first + r], p.block_size), q_load8(src + (long long)r * token_stride));
   }
 }
 
