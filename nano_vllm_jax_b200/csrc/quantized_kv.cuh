@@ -16,7 +16,6 @@
 
 namespace nvj {
 
-constexpr float kQLargest = 448.f;  // of e4m3
 constexpr int kQLowExp = -117, kQHighExp = 119;
 
 // Head layouts and block sizes that the kernels take: rows of 64, 128 or 256 elements, blocks of 16, 32, 48 or 64 tokens (a key tile of 16

@@ -7,8 +7,9 @@
 //                numbers below 2^-31 of their row's largest), f32 ones two f16 terms (2^-22);
 //   O = P V      [128 query rows x head_dim]  16 keys per MMA; P from tensor memory, as two f16 terms (2^-22 of a weight).
 // A tile of 64 keys takes 4 * 128 * 64 * head_dim flops for S and twice that for O's two terms: 2200 cycles of an SM at head_dim 256.  What
-// bounds the kernel is the conversion: a loader's 16 pieces of a tile 1700 cycles (13 per pair of numbers), with their addresses, copies and
-// waits 3400.  Against the tiles of mma.sync that stood here before: 1984 f16 tokens behind 727, 32 heads of 128 over 8, 452 -> 185 us;
+// bounds the kernel are the loaders: 3400 cycles for a tile, half of them for the conversion of 16 pieces per thread, at 6 - 9 cycles per
+// instruction of a warp whatever it is (e4m3 to f16 by integer instructions, four for one: 234 us instead of 185 in the first of these).
+// Against the tiles of mma.sync that stood here before: 1984 f16 tokens behind 727, 32 heads of 128 over 8, 452 -> 185 us;
 // 1018 tokens of four rows behind 1232 each 165 -> 76; 55 f32 tokens of two rows behind 1214 (8 heads of 256 over 2) 160 -> 29; 54 tokens
 // behind 1398 (16 heads of 64 over 2) 62 -> 16; the smallest calls as long as they took (20 tokens, heads of 256: 17.7 -> 17.4).  A
 // small call at head_dim 256 is start and end: row and lengths 2.4 us, queries 3.6, a tile 2, rows staged 3, folded over DSMEM 5.
