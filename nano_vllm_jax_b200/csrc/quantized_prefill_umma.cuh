@@ -19,8 +19,8 @@
 //   warps 0 - 7    softmax, thread = (query row, half of the tile's keys); a row's two halves are a pair of warps
 //   warps 8, 9     MMA issue: scores (up to two tiles ahead), weighted sums
 //   warps 10 - 13  keys, values: 16-byte pieces of the blocks to shared memory, one tile ahead, and from there as f16 to their tiles
-// The weights of a row are exp2(score - reference) times the V scale; the reference is set 2^7 above its first largest weight's exponent
-// and moved when one would pass 2^15 (f16 ends at 2^16), which a later tile rarely does.  Their sum is taken in f32 with the V scale
+// The weights of a row are exp2(score - reference) times the V scale; the reference is set so that the largest weight is 2^7,
+// and moved when a later one would pass 2^15 (f16 ends at 2^16), which is rare.  Their sum is taken in f32 with the V scale
 // divided out again, relative to the first tile's largest.
 // The tensor cores cut the last place of what they add to: 1.2e-5 of a sum over 16384 keys.  After kQtFlush tiles the sums are
 // emptied into the output row (clusters: into scratch) and begun again.

@@ -879,7 +879,9 @@ def qk_norm_rope_kv_append(query, k, v, q_norm_weight, k_norm_weight, positions,
 # --------------------------------------------------------------------------- copies / tokens
 
 def copy_blocks(k_cache, v_cache, src_ids, dst_ids):
-    """cache[:, dst] = cache[:, src] on the 5-D caches, in place (src and dst sets disjoint)."""
+    """cache[:, dst] = cache[:, src] on the 5-D caches, in place (src and dst sets disjoint; no 8-bit caches, whose blocks' scales lie elsewhere)."""
+    if k_cache.dtype == torch.float8_e4m3fn:
+        raise ValueError("copy_blocks does not take 8-bit caches: their blocks' scales lie in tensors of their own")
     if host().copy_blocks(k_cache, v_cache, src_ids, dst_ids):
         return k_cache, v_cache
     lib = _lib.load()

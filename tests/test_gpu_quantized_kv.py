@@ -580,6 +580,25 @@ def test_prefill_with_any_count_of_tiles(tiles):
 
 # ------------------------------------------------------------------------------------------------ refusals
 
+def test_the_other_entry_points_refuse_8_bit_caches():
+    hq, hkv, d, bs = SHAPES[0]
+    k5 = torch.zeros(1, 4, bs, hkv, d, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+    k, v = k5[0], k5[0].clone()
+    tables, lens, q = _i32([[0, 1], [2, 3]]), _i32([3, 4]), torch.zeros(2, 1, hq, d, device="cuda", dtype=BF16)
+    new, pos = torch.zeros(2, 1, hkv, d, device="cuda", dtype=BF16), _i32([[2], [3]])
+    calls = [lambda: K.paged_decode_attention(q, k, v, tables, lens, 0.1),
+             lambda: K.paged_decode_attention_wide(q, k, v, tables, lens, pos, 0.1),
+             lambda: K.paged_decode_attention_with_kv_append(q, new, new, k5, k5.clone(), tables, lens, pos, 0, bs, 0.1, hq // hkv),
+             lambda: K.packed_paged_prefill_attention(q.reshape(1, 2, hq, d), k, v, tables, lens, pos.reshape(1, 2), _i32([0, 1, 2]), bs, 0.1, hq // hkv),
+             lambda: K.kv_append_slots(new, new, _i32([[2], [35]]), k, v),
+             lambda: K.copy_blocks(k5, k5.clone(), _i32([0]), _i32([1]))]
+    for call in calls:
+        with pytest.raises((ValueError, TypeError, RuntimeError)):
+            call()
+    torch.cuda.synchronize()
+    assert not k5.view(torch.uint8).any() and not v.view(torch.uint8).any()
+
+
 def test_wrappers_refuse_what_does_not_fit_together():
     hq, hkv, d, bs = SHAPES[0]
     k = torch.zeros(4, bs, hkv, d, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
