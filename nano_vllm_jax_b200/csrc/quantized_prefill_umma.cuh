@@ -6,19 +6,19 @@
 //   S = Q K^T    [128 query rows x 64 keys]   16 dims per MMA; bf16 and f16 queries are f16 times a power of two per row (exact, but for bf16
 //                numbers below 2^-31 of their row's largest), f32 ones two f16 terms (2^-22);
 //   O = P V      [128 query rows x head_dim]  16 keys per MMA; P from tensor memory, as two f16 terms (2^-22 of a weight).
-// A tile of 64 keys takes 4 * 128 * 64 * head_dim flops for S and twice that for O's two terms: 2200 cycles of an SM at head_dim 256.  What
-// bounds the kernel are the loaders: 3400 cycles for a tile, half of them for the conversion of 16 pieces per thread, at 6 - 9 cycles per
-// instruction of a warp whatever it is (e4m3 to f16 by integer instructions, four for one: 234 us instead of 185 in the first of these).
-// Against the tiles of mma.sync that stood here before: 1984 f16 tokens behind 727, 32 heads of 128 over 8, 452 -> 185 us;
-// 1018 tokens of four rows behind 1232 each 165 -> 76; 55 f32 tokens of two rows behind 1214 (8 heads of 256 over 2) 160 -> 29; 54 tokens
-// behind 1398 (16 heads of 64 over 2) 62 -> 16; the smallest calls as long as they took (20 tokens, heads of 256: 17.7 -> 17.4).  A
-// small call at head_dim 256 is start and end: row and lengths 2.4 us, queries 3.6, a tile 2, rows staged 3, folded over DSMEM 5.
+// A tile of 64 keys takes 4 * 128 * 64 * head_dim flops for S and twice that for O's two terms: 2200 cycles of an SM at head_dim 256.  A softmax
+// thread's way from a tile's scores to its weights takes as long: scores out of tensor memory 400, the pair's meeting 500, exponentials and terms
+// 700, back 250.  head_dim 64 takes just that, 128 2500, 256 3400, where queries, keys and values move 220 KB through shared memory per tile.
+// Against the tiles of mma.sync that stood here before: 1984 f16 tokens behind 727, 32 heads of 128 over 8, 452 -> 186 us; 1018 tokens of
+// four rows behind 1232 each 165 -> 74; 55 f32 tokens of two rows behind 1214 (8 heads of 256 over 2) 160 -> 27; 54 tokens behind 1398 (16
+// heads of 64 over 2) 62 -> 16; the smallest calls as long as they took (20 tokens, heads of 256: 17.7 -> 17).  A small call at head_dim
+// 256 is start and end: row and lengths 2.4 us, queries 3, a tile 2, rows staged 3, folded over DSMEM 5.
 //
 // CTA: 128 query rows (token major, a kv head's `groups` heads minor) of one table row and kv head.  While that gives fewer tiles than the GPU
 // has room for, a tile's keys are split over a cluster of up to eight CTAs, which fold their rows through each other's shared memory.
 //   warps 0 - 7    softmax, thread = (query row, half of the tile's keys); a row's two halves are a pair of warps
-//   warps 8, 9     MMA issue: scores (up to two tiles ahead), weighted sums
-//   warps 10 - 13  keys, values: 16-byte pieces of the blocks to shared memory, one tile ahead, and from there as f16 to their tiles
+//   warps 8 - 11   keys: 16-byte pieces of the blocks to registers, one tile ahead, and from there as f16 to their tiles
+//   warps 12 - 15  values, in the same way; the first issues the weighted sums' MMAs, the second the scores', a tile ahead
 // The weights of a row are exp2(score - reference) times the V scale; the reference is set so that the largest weight is 2^7,
 // and moved when a later one would pass 2^15 (f16 ends at 2^16), which is rare.  Their sum is taken in f32 with the V scale
 // divided out again, relative to the first tile's largest.
@@ -34,7 +34,7 @@
 
 namespace nvj {
 
-constexpr int kQtRows = 128, kQtKeys = 64, kQtThreads = 448, kQtSoftmax = 256, kQtLoaders = 64;
+constexpr int kQtRows = 128, kQtKeys = 64, kQtThreads = 512, kQtSoftmax = 256, kQtLoaders = 128;
 constexpr int kQtColS = 256, kQtColP = 384;  // of tensor memory: O from 0, S twice, P twice (two terms of 32 columns)
 constexpr float kQtNone = -3e38f, kQtSlack = 8.f, kQtLift = 7.f, kQtMostInverse = 100.f;
 
@@ -43,15 +43,15 @@ struct QtSmem {
   static constexpr int kQTerms = std::is_same<T, float>::value ? 2 : 1;
   static constexpr int kChunks = kD / 64;                 // of 64 dims: 128 bytes of f16
   static constexpr int kTileBytes = kQtKeys * kD * 2;
-  static constexpr int kRawBytes = kTileBytes;            // a tile of K and one of V as they lie in the cache
-  static constexpr int kFit = (232448 - 1024 - 2048 - kQTerms * kChunks * 16384 - kRawBytes) / kTileBytes;
+  static constexpr int kFit = (232448 - 1024 - 2048 - kQTerms * kChunks * 16384) / kTileBytes;
   static constexpr int kKSlots = kFit >= 3 ? 2 : 1, kVSlots = kFit >= 4 ? 2 : 1;
   alignas(1024) char q[kQTerms][kChunks][kQtRows * 128];  // [chunk][row][128 B]
   alignas(1024) char k[kKSlots][kTileBytes];              // [8-key group][chunk][8 keys][128 B]
   alignas(1024) char v[kVSlots][kTileBytes];
-  alignas(1024) char raw[2][kRawBytes / 2];  // [K, V][piece][thread][16 B]: a loader's own bytes
   alignas(8) unsigned long long k_full[kKSlots], k_empty[kKSlots], v_full[kVSlots], v_empty[kVSlots], s_full[2], p_full[2], pv_done[2];
-  alignas(16) float k_unit[4][4], v_unit[4][4];  // by tile and 16 keys: the block's scales; V's -1: no such block
+  // by tile and 16 keys: the block's scales; V's -1: no such block.  Those of tile n + 1 are asked for when S(n - 2) is complete, hence when the weights
+  // of n - 4 are there: eight places, so that n - 7's have been read.
+  alignas(16) float k_unit[8][4], v_unit[8][4];
   float factor[kQtRows];
   int limit[kQtRows];
   float red[kQtRows];  // between the two threads of a row
@@ -75,11 +75,61 @@ __device__ __forceinline__ constexpr uint32_t qt_idesc(int n, bool b_mn) {
 template <int kD>
 __device__ __forceinline__ int qt_piece(int r, int piece) { return r * kD + ((piece ^ (r & 15)) << 2); }
 
-// ---- warps 10 - 13 -------------------------------------------------------------------------------------------------------------
-template <bool kV, typename T, int kD>
-__device__ __forceinline__ void qt_loaders(QtSmem<T, kD>& sm, const QtParams& p, int row, int head, int len, int tile0, int tiles, int tid) {
+// ---- MMA issue ------------------------------------------------------------------------------------------------------------------------
+// S of tile n takes the place of S of n - 2, which has been read when that tile's weights are there.
+template <typename T, int kD>
+__device__ __forceinline__ bool qt_issue_scores(QtSmem<T, kD>& sm, const QtParams& p, uint32_t tmem, int n) {
   using L = QtSmem<T, kD>;
-  constexpr int kPieces = kD / 16, kStep = kQtLoaders / (kD / 16);  // pieces per thread; keys between them (4, 8 or 16)
+  constexpr uint32_t idesc = qt_idesc(kQtKeys, false);
+  const int slot = n % L::kKSlots;
+  if (!um_wait(&sm.k_full[slot], (n / L::kKSlots) & 1u, &sm.abort_flag, p.status)) return false;
+  if (n >= 2 && !um_wait(&sm.p_full[n & 1], ((n >> 1) - 1) & 1u, &sm.abort_flag, p.status)) return false;
+  tc_fence_after_sync();
+  if (um_elect_one()) {
+    const uint64_t q_desc = umma_desc(smem_u32(sm.q[0][0]), 16, 1024), k_desc = umma_desc(smem_u32(sm.k[slot]), 16, L::kChunks * 1024);
+#pragma unroll
+    for (int term = L::kQTerms - 1; term >= 0; --term)
+#pragma unroll
+      for (int ks = 0; ks < kD / 16; ++ks)
+        umma_bf16_ss(tmem + kQtColS + (n & 1) * kQtKeys,
+                     q_desc + (uint64_t)((((term * L::kChunks + (ks >> 2)) * kQtRows * 128) + (ks & 3) * 32) >> 4),
+                     k_desc + (uint64_t)(((ks >> 2) * 1024 + (ks & 3) * 32) >> 4), idesc, ks > 0 || term < L::kQTerms - 1 ? 1u : 0u);
+    umma_commit(smem_u32(&sm.s_full[n & 1]));
+    umma_commit(smem_u32(&sm.k_empty[slot]));
+  }
+  __syncwarp();
+  return true;
+}
+template <typename T, int kD>
+__device__ __forceinline__ bool qt_issue_sums(QtSmem<T, kD>& sm, const QtParams& p, uint32_t tmem, int n, bool flush) {
+  using L = QtSmem<T, kD>;
+  constexpr uint32_t idesc = qt_idesc(kD, true);
+  const int slot = n % L::kVSlots;
+  if (!um_wait(&sm.v_full[slot], (n / L::kVSlots) & 1u, &sm.abort_flag, p.status)) return false;
+  if (!um_wait(&sm.p_full[n & 1], (n >> 1) & 1u, &sm.abort_flag, p.status)) return false;
+  tc_fence_after_sync();
+  if (um_elect_one()) {
+    const uint64_t v_desc = umma_desc(smem_u32(sm.v[slot]), 1024, L::kChunks * 1024);  // chunks of 64 dims, groups of 8 keys
+    const bool anew = flush ? n % kQtFlush == 0 : n == 0;
+#pragma unroll
+    for (int ks = 0; ks < kQtKeys / 16; ++ks)
+#pragma unroll
+      for (int term = 1; term >= 0; --term)
+        umma_bf16_ts(tmem, tmem + kQtColP + (n & 1) * 64 + term * 32 + ks * 8, v_desc + (uint64_t)((ks * 2 * L::kChunks * 1024) >> 4), idesc,
+                     anew && ks == 0 && term == 1 ? 0u : 1u);
+    umma_commit(smem_u32(&sm.pv_done[n & 1]));
+    umma_commit(smem_u32(&sm.v_empty[slot]));
+  }
+  __syncwarp();
+  return true;
+}
+
+// ---- warps 8 - 15 -------------------------------------------------------------------------------------------------------------
+template <bool kV, typename T, int kD>
+__device__ __forceinline__ void qt_loaders(QtSmem<T, kD>& sm, const QtParams& p, uint32_t tmem, bool flush, int row, int head, int len, int tile0,
+                                           int tiles, int tid) {
+  using L = QtSmem<T, kD>;
+  constexpr int kPieces = kD / 32, kStep = kQtLoaders / (kD / 16);  // pieces per thread; keys between them (8, 16 or 32)
   const int32_t* table = p.block_tables + (long long)row * p.table_width;
   // Of the tile's first kStep keys: the thread's key, 64 dims and 16 bytes of them.  (Eight lanes of a store: four pieces each of an even and an
   // odd key, which the swizzle puts into different banks.)
@@ -105,7 +155,7 @@ __device__ __forceinline__ void qt_loaders(QtSmem<T, kD>& sm, const QtParams& p,
   auto locate = [&](int tile) {
     whole = (tile + 1) * kQtKeys <= len;
     if (!kV && tid < 4) {  // the scales, counted with K
-      const int i = tid == 0 ? id[0] : tid == 1 ? id[1] : tid == 2 ? id[2] : id[3], slot = (tile - tile0) & 3;
+      const int i = tid == 0 ? id[0] : tid == 1 ? id[1] : tid == 2 ? id[2] : id[3], slot = (tile - tile0) & 7;
       if ((unsigned)i < ids_end) {
         const long long entry = (long long)i * p.num_kv_heads + head;
         asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(&sm.k_unit[slot][tid])), "l"(p.k_scale + entry) : "memory");
@@ -129,41 +179,41 @@ __device__ __forceinline__ void qt_loaders(QtSmem<T, kD>& sm, const QtParams& p,
       }
     }
   };
-  // Through shared memory of its own a thread's pieces need no registers.  (In registers, with addresses found piece by piece and all four warps at
-  // both K and V: 6200 cycles per tile of 64 keys of 256; so 4700 with the pieces in shared memory, 3600 with addresses found once per 16 keys.)
-  const uint32_t raw = smem_u32(sm.raw[kV]) + tid * 16;
+  // (Four warps for K and V, and two that only issued MMAs: up to 20% slower with f32 queries, 5% with heads of 128, 5 - 7% faster on 4096 tokens of
+  // heads of 64, or of 256 in f16.  The pieces by way of shared memory instead of registers: 0 - 5% slower.)
   const uint8_t* cache = kV ? p.v_cache : p.k_cache;
+  uint4 held[kPieces];
   auto fetch = [&](int tile) {
-    auto copy = [&](int i, long long from, int bytes) {
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(raw + i * (kQtLoaders * 16)), "l"(cache + from), "r"(bytes) : "memory");
-    };
     const int step_bytes = kStep * row_bytes;
     if (whole) {
 #pragma unroll
-      for (int i = 0; i < kPieces; ++i) copy(i, at[i * kStep / 16] + i * kStep % 16 / kStep * step_bytes, 16);
-    } else {  // keys behind the row's last one become zeros, which as values weigh nothing
-#pragma unroll 1
       for (int i = 0; i < kPieces; ++i) {
-        const int key = key_of + i * kStep, j = key >> 4;
-        const long long base = j == 0 ? at[0] : j == 1 ? at[1] : j == 2 ? at[2] : at[3];
-        const bool there = base >= 0 && tile * kQtKeys + key < len;
-        copy(i, there ? base + i * kStep % 16 / kStep * step_bytes : 0ll, there ? 16 : 0);
+        if constexpr (kStep == 32) held[i] = ld_stream_u4(cache + (key_of >= 16 ? at[2 * i + 1] : at[2 * i]));
+        else held[i] = ld_stream_u4(cache + (at[i * kStep / 16] + i * kStep % 16 / kStep * step_bytes));
+      }
+    } else {  // keys behind the row's last one become zeros, which as values weigh nothing
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        const int key = key_of + i * kStep;
+        long long from;
+        if constexpr (kStep == 32) from = key_of >= 16 ? at[2 * i + 1] : at[2 * i];
+        else from = at[i * kStep / 16];
+        held[i] = make_uint4(0, 0, 0, 0);
+        if (from >= 0 && tile * kQtKeys + key < len) held[i] = ld_stream_u4(cache + from + (kStep < 16 ? i * kStep % 16 / kStep * step_bytes : 0));
       }
     }
   };
   const uint32_t dst = (key_of >> 3) * (L::kChunks * 1024) + chunk * 1024 + (key_of & 7) * 128 + ((((tid & 3) * 2) ^ (key_of & 7)) << 4);
   auto store = [&](char* tile) {
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    // (kStep 4: every other piece is of a key four rows on in the group of eight, which the swizzle has 64 bytes off)
-    const uint32_t to = smem_u32(tile) + dst, to_4 = to ^ 64u;
+    if (!kV && tid < 4) asm volatile("cp.async.wait_all;" ::: "memory");
+    const uint32_t to = smem_u32(tile) + dst;
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
-      uint32_t w[4];
-      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(raw + i * (kQtLoaders * 16)) : "memory");
+      const uint32_t w[4] = {held[i].x, held[i].y, held[i].z, held[i].w};
 #pragma unroll
       for (int h = 0; h < 2; ++h)
         asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};"
-                     ::"r"(((kStep == 4 && i % 2 == 1 ? to_4 : to) ^ (h ? 16u : 0u)) + i * kStep / 8 * (L::kChunks * 1024) + i * kStep % 8 * 128), "r"(q_half2(w[2 * h])), "r"(q_half2_high(w[2 * h])),
+                     ::"r"((h ? to ^ 16u : to) + i * (kStep / 8 * L::kChunks * 1024)), "r"(q_half2(w[2 * h])), "r"(q_half2_high(w[2 * h])),
                        "r"(q_half2(w[2 * h + 1])), "r"(q_half2_high(w[2 * h + 1])) : "memory");
     }
   };
@@ -172,10 +222,20 @@ __device__ __forceinline__ void qt_loaders(QtSmem<T, kD>& sm, const QtParams& p,
   locate(tile0);
   fetch(tile0);
   ids_of(tile0 + 1);
+  // The values' first two warps issue the MMAs: one the weighted sums, one the scores, a tile ahead.  (By the first warps of the keys and of the values,
+  // each issuing what its own tiles are for, 3700 cycles per tile of 64 keys of 256: the keys' warp had the scales to bring as well.)
+  const bool sums = kV && tid < 32, scores = kV && tid >= 32 && tid < 64;
+  bool alive = true;
+  if (scores) {
+    named_bar_sync(5, kQtSoftmax + 32);  // the queries are there
+    alive = qt_issue_scores(sm, p, tmem, 0);
+  }
 #pragma unroll 1
-  for (int n = 0; n < tiles; ++n) {
+  for (int n = 0; alive && n < tiles; ++n) {
     const int slot = n % kSlots;
-    if (n >= kSlots && !um_wait(kV ? &sm.v_empty[slot] : &sm.k_empty[slot], (n / kSlots - 1) & 1u, &sm.abort_flag, p.status)) break;
+    if (scores && n + 1 < tiles && !(alive = qt_issue_scores(sm, p, tmem, n + 1))) break;
+    if (sums && n > 0 && !(alive = qt_issue_sums(sm, p, tmem, n - 1, flush))) break;
+    if (n >= kSlots && !(alive = um_wait(kV ? &sm.v_empty[slot] : &sm.k_empty[slot], (n / kSlots - 1) & 1u, &sm.abort_flag, p.status))) break;
     store(kV ? sm.v[slot] : sm.k[slot]);
     fence_proxy_async_smem();
     mbar_arrive(smem_u32(kV ? &sm.v_full[slot] : &sm.k_full[slot]));
@@ -185,15 +245,16 @@ __device__ __forceinline__ void qt_loaders(QtSmem<T, kD>& sm, const QtParams& p,
       ids_of(tile0 + n + 2);
     }
   }
+  if (sums && alive) qt_issue_sums(sm, p, tmem, tiles - 1, flush);
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 // ---- queries: 8 dims a lane, so many rows of a warp at a time -----------------------------------------------------------------------------
 template <typename T, int kD>
 struct QtQueries {
-  static constexpr int kWarps = 10, kLanes = kD / 8, kAtOnce = 32 / kLanes;
+  static constexpr int kWarps = 8, kLanes = kD / 8, kAtOnce = 32 / kLanes;
   static constexpr int kAll = (kQtRows + kWarps * kAtOnce - 1) / (kWarps * kAtOnce);  // passes of a warp
-  static constexpr int kMost = sizeof(T) == 4 ? 4 : 7, kRounds = kAll < kMost ? kAll : kMost;  // of them on their way at a time
+  static constexpr int kMost = sizeof(T) == 4 ? 4 : 8, kRounds = kAll < kMost ? kAll : kMost;  // of them on their way at a time
   static __device__ __forceinline__ int row_of(int round, int warp, int lane) { return (round * kWarps + warp) * kAtOnce + lane / kLanes; }
   // Times a power of two per row that makes the largest 2^14 - 2^15.
   static __device__ __forceinline__ void store(QtSmem<T, kD>& sm, const QRaw<T>& raw, int r, int lane, float scale_log2) {
@@ -227,59 +288,6 @@ struct QtQueries {
   }
 };
 
-// ---- warps 8 and 9 --------------------------------------------------------------------------------------------------------------
-template <typename T, int kD>
-__device__ __forceinline__ void qt_scores_warp(QtSmem<T, kD>& sm, const QtParams& p, uint32_t tmem, int tiles) {
-  using L = QtSmem<T, kD>;
-  constexpr uint32_t idesc = qt_idesc(kQtKeys, false);
-  const uint64_t q_desc0 = umma_desc(smem_u32(sm.q[0][0]), 16, 1024);
-  const uint64_t k_desc0 = umma_desc(smem_u32(sm.k[0]), 16, L::kChunks * 1024);
-  for (int n = 0; n < tiles; ++n) {
-    const int slot = n % L::kKSlots;
-    if (!um_wait(&sm.k_full[slot], (n / L::kKSlots) & 1u, &sm.abort_flag, p.status)) return;
-    if (n >= 2 && !um_wait(&sm.p_full[n & 1], ((n >> 1) - 1) & 1u, &sm.abort_flag, p.status)) return;  // S(n - 2) has been read
-    tc_fence_after_sync();
-    if (um_elect_one()) {
-      const uint64_t k_desc = k_desc0 + (uint64_t)((slot * L::kTileBytes) >> 4);
-#pragma unroll
-      for (int term = L::kQTerms - 1; term >= 0; --term)
-#pragma unroll
-        for (int ks = 0; ks < kD / 16; ++ks)
-          umma_bf16_ss(tmem + kQtColS + (n & 1) * kQtKeys,
-                       q_desc0 + (uint64_t)((((term * L::kChunks + (ks >> 2)) * kQtRows * 128) + (ks & 3) * 32) >> 4),
-                       k_desc + (uint64_t)(((ks >> 2) * 1024 + (ks & 3) * 32) >> 4), idesc, ks > 0 || term < L::kQTerms - 1 ? 1u : 0u);
-      umma_commit(smem_u32(&sm.s_full[n & 1]));
-      umma_commit(smem_u32(&sm.k_empty[slot]));
-    }
-    __syncwarp();
-  }
-}
-template <typename T, int kD>
-__device__ __forceinline__ void qt_sums_warp(QtSmem<T, kD>& sm, const QtParams& p, uint32_t tmem, int tiles, bool flush) {
-  using L = QtSmem<T, kD>;
-  constexpr uint32_t idesc = qt_idesc(kD, true);
-  const uint64_t v_desc0 = umma_desc(smem_u32(sm.v[0]), 1024, L::kChunks * 1024);  // chunks of 64 dims, groups of 8 keys
-  for (int n = 0; n < tiles; ++n) {
-    const int slot = n % L::kVSlots;
-    if (!um_wait(&sm.v_full[slot], (n / L::kVSlots) & 1u, &sm.abort_flag, p.status)) return;
-    if (!um_wait(&sm.p_full[n & 1], (n >> 1) & 1u, &sm.abort_flag, p.status)) return;
-    tc_fence_after_sync();
-    if (um_elect_one()) {
-      const uint64_t v_desc = v_desc0 + (uint64_t)((slot * L::kTileBytes) >> 4);
-      const bool anew = flush ? n % kQtFlush == 0 : n == 0;
-#pragma unroll
-      for (int ks = 0; ks < kQtKeys / 16; ++ks)
-#pragma unroll
-        for (int term = 1; term >= 0; --term)
-          umma_bf16_ts(tmem, tmem + kQtColP + (n & 1) * 64 + term * 32 + ks * 8, v_desc + (uint64_t)((ks * 2 * L::kChunks * 1024) >> 4), idesc,
-                       anew && ks == 0 && term == 1 ? 0u : 1u);
-      umma_commit(smem_u32(&sm.pv_done[n & 1]));
-      umma_commit(smem_u32(&sm.v_empty[slot]));
-    }
-    __syncwarp();
-  }
-}
-
 // ---- warps 0 - 7 ----------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ float qt_log(float v_unit) { return v_unit < 0.f ? -INFINITY : __log2f(v_unit); }
 struct QtRow {  // what a softmax thread knows of its row at the end
@@ -303,7 +311,7 @@ __device__ __forceinline__ bool qt_softmax(QtSmem<T, kD>& sm, const QtParams& p,
     tc_fence_after_sync();
     float x[32];
     tmem_ld32(tmem + kQtColS + buf * kQtKeys + half * 32, x);
-    const float2 unit = *reinterpret_cast<const float2*>(&sm.k_unit[n & 3][2 * half]), v_unit = *reinterpret_cast<const float2*>(&sm.v_unit[n & 3][2 * half]);
+    const float2 unit = *reinterpret_cast<const float2*>(&sm.k_unit[n & 7][2 * half]), v_unit = *reinterpret_cast<const float2*>(&sm.v_unit[n & 7][2 * half]);
     const int key0 = (tile0 + n) * kQtKeys + half * 32;
     const float by[2] = {factor * unit.x, factor * unit.y}, plus[2] = {qt_log(v_unit.x), qt_log(v_unit.y)};
     // exponents of the weights will be x * mul + add - reference
@@ -343,7 +351,7 @@ __device__ __forceinline__ bool qt_softmax(QtSmem<T, kD>& sm, const QtParams& p,
       o.l *= f;
       o.m = now;
       if (!begun) {
-        const float* all = sm.v_unit[n & 3];
+        const float* all = sm.v_unit[n & 7];
         const float big = qt_log(fmaxf(fmaxf(all[0], all[1]), fmaxf(all[2], all[3])));
         o.v_first = big == -INFINITY ? 0.f : big;
       } else {
@@ -477,10 +485,10 @@ __global__ void __launch_bounds__(kQtThreads, 1) quantized_prefill_umma_kernel(c
     tmem_alloc(smem_u32(&sm.tmem_base), 512);  // (between the wait and the release: umma.cuh)
     if (lane == 0) pdl_release();
     tc_fence_before_sync();
-  } else if (warp >= 10) {  // padding behind the last row's tokens
+  } else if (warp >= 12) {  // padding behind the last row's tokens
     const int end = p.query_start_loc[p.rows], from = end > 0 ? end : 0;
     const long long per_token = (long long)p.groups * (kD / 4), pad = from < p.token_bucket ? (long long)(p.token_bucket - from) * per_token : 0;
-    for (long long i = (long long)blockIdx.x * 2 * kQtLoaders + tid - 320; i < pad; i += (long long)gridDim.x * 2 * kQtLoaders) {
+    for (long long i = (long long)blockIdx.x * kQtLoaders + tid - 384; i < pad; i += (long long)gridDim.x * kQtLoaders) {
       const long long token = from + i / per_token;
       reinterpret_cast<float4*>(p.out + (token * hq + head * p.groups) * kD)[i % per_token] = make_float4(0.f, 0.f, 0.f, 0.f);
     }
@@ -511,7 +519,7 @@ __global__ void __launch_bounds__(kQtThreads, 1) quantized_prefill_umma_kernel(c
     return raw;
   };
   QRaw<T> queries[Q::kRounds];
-  if (warp < 10) {
+  if (warp < 8) {
 #pragma unroll
     for (int u = 0; u < Q::kRounds; ++u) queries[u] = query(Q::row_of(u, warp, lane));
   }
@@ -535,9 +543,9 @@ __global__ void __launch_bounds__(kQtThreads, 1) quantized_prefill_umma_kernel(c
   float* scratch = splits == 1 ? nullptr : p.flush;
   const bool flush = tiles > kQtFlush && (splits == 1 || scratch);
 
-  if (warp >= 10) {
-    if (tiles > 0 && warp >= 12) qt_loaders<true>(sm, p, row, head, len, tile0, tiles, tid - 384);
-    else if (tiles > 0) qt_loaders<false>(sm, p, row, head, len, tile0, tiles, tid - 320);
+  if (warp >= 8) {
+    if (tiles > 0 && warp >= 12) qt_loaders<true>(sm, p, tmem, flush, row, head, len, tile0, tiles, tid - 384);
+    else if (tiles > 0) qt_loaders<false>(sm, p, tmem, flush, row, head, len, tile0, tiles, tid - 256);
   } else {
     for (int i0 = 0; tiles > 0; ) {
 #pragma unroll
@@ -548,12 +556,8 @@ __global__ void __launch_bounds__(kQtThreads, 1) quantized_prefill_umma_kernel(c
       for (int u = 0; u < Q::kRounds; ++u) queries[u] = query(Q::row_of(i0 + u, warp, lane));
     }
     fence_proxy_async_smem();
-    named_bar_sync(5, kQtSoftmax + 64);
-    if (warp == 8) {
-      qt_scores_warp(sm, p, tmem, tiles);
-    } else if (warp == 9) {
-      qt_sums_warp(sm, p, tmem, tiles, flush);
-    } else {
+    if (tiles > 0) named_bar_sync(5, kQtSoftmax + 32);
+    {
       const int r = (warp & 3) * 32 + lane, half = warp >> 2, at = first_row + r;
       const uint32_t my_tmem = tmem + ((uint32_t)((warp & 3) * 32) << 16);
       float* out_row = at < query_rows ? p.out + ((long long)(token0 + at / p.groups) * hq + head * p.groups + at % p.groups) * kD : nullptr;
