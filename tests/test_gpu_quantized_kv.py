@@ -578,6 +578,87 @@ def test_prefill_with_any_count_of_tiles(tiles):
     _long_prefill((32, 8, 128, 16), BF16, [(150, 900), (70, 0), (2, 333)], dict(num_decode_rows=0, query_tile_pairs=tiles), 22, 33)
 
 
+TILES = [((32, 8, 128, 16), F16), ((16, 1, 256, 16), BF16), ((8, 2, 256, 16), F32), ((16, 2, 64, 32), BF16)]  # shapes of the 8-bit tiles
+
+
+def _prefill(q, state_gpu, tables, lens, rows, shape, scale):
+    (k, ks), (v, vs) = state_gpu
+    positions, qsl = np.concatenate([np.arange(c, c + n) for n, c in rows])[None], np.cumsum([0] + [n for n, _ in rows])
+    return Q.packed_paged_prefill_attention_quantized(q, k, v, ks, vs, _i32(tables), _i32(lens), _i32(positions), _i32(qsl), shape[3], scale,
+                                                      shape[0] // shape[1], num_decode_rows=0)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.07, 1.5])
+@pytest.mark.parametrize("shape,dtype", TILES)
+def test_prefill_tiles_with_any_scale_of_the_scores_and_queries_of_any_size(shape, dtype, scale):
+    hq, hkv, d, bs = shape
+    rng = np.random.default_rng(34)
+    rows = [(70, 200), (3, 61)]
+    lens = [n + c for n, c in rows]
+    tables = _tables(rng, lens, bs, 60)
+    for size in (1.0, 2.0 ** 12, 2.0 ** -12):
+        state = [_pool(rng, 60, shape, spread=1) for _ in range(2)]
+        state[0][1][:] /= size
+        q = torch.from_numpy(rng.standard_normal((1, 73, hq, d)) * size).to(dtype).cuda()
+        out = _f64(_prefill(q, [_gpu(*x) for x in state], tables, lens, rows, shape, scale)).reshape(73, hq, d)
+        q64 = _f64(q)[0]
+        _check([out[:70], out[70:]], [q64[:70], q64[70:]], state, tables, lens, [c + 1 + np.arange(n) for n, c in rows], scale)
+
+
+@pytest.mark.parametrize("shape,dtype", TILES)
+def test_prefill_tiles_keep_nan_and_infinite_queries_in_their_row_and_head_and_nan_values_visible(shape, dtype):
+    hq, hkv, d, bs = shape
+    rng = np.random.default_rng(35)
+    rows = [(40, 300), (9, 0)]
+    lens = [n + c for n, c in rows]
+    tables = _tables(rng, lens, bs, 60)
+    state = [_pool(rng, 60, shape) for _ in range(2)]
+    gpu = [_gpu(*x) for x in state]
+    q = torch.from_numpy(rng.standard_normal((1, 49, hq, d))).to(dtype).cuda()
+    clean = _prefill(q, gpu, tables, lens, rows, shape, d ** -0.5).view(49, hq, d)
+    odd = q.clone()
+    odd[0, 5, 3, 7], odd[0, 44, 0, 0] = float("nan"), float("-inf")
+    out = _prefill(odd, gpu, tables, lens, rows, shape, d ** -0.5).view(49, hq, d)
+    assert torch.isnan(out[5, 3]).all() and torch.isnan(out[44, 0]).all()
+    out[5, 3], out[44, 0] = clean[5, 3], clean[44, 0]
+    assert torch.equal(out, clean)
+    gpu[1][0].view(torch.uint8)[tables[0, 1], 2, hkv - 1, 9] = 127  # a value that all of row 0's tokens see
+    out = _prefill(q, gpu, tables, lens, rows, shape, d ** -0.5).view(49, hq, d)
+    heads = slice((hkv - 1) * (hq // hkv), hq)
+    assert torch.isnan(out[:40, heads, 9]).all()
+    out[:40, heads, 9] = clean[:40, heads, 9]
+    assert torch.equal(out, clean)
+
+
+@pytest.mark.parametrize("shape,dtype", TILES)
+def test_prefill_tiles_from_a_graph_on_another_stream_and_bit_for_bit(shape, dtype):
+    hq, hkv, d, bs = shape
+    rng = np.random.default_rng(36)
+    rows = [(30, 500), (100, 7)]
+    lens = [n + c for n, c in rows]
+    tables = _tables(rng, lens, bs, 80)
+    gpu = [_gpu(*_pool(rng, 80, shape)) for _ in range(2)]
+    q = torch.from_numpy(rng.standard_normal((1, 130, hq, d))).to(dtype).cuda()
+    want = _prefill(q, gpu, tables, lens, rows, shape, d ** -0.5)
+    (k, ks), (v, vs) = gpu
+    positions, qsl = np.concatenate([np.arange(c, c + n) for n, c in rows])[None], np.cumsum([0] + [n for n, _ in rows])
+    args = [_i32(x) for x in (tables, lens, positions, qsl)]
+    from nano_vllm_jax_b200.engine.resident_decode import CapturedStep
+    steps = [CapturedStep(lambda: Q.packed_paged_prefill_attention_quantized(q, k, v, ks, vs, *args, bs, d ** -0.5, hq // hkv, num_decode_rows=0)) for _ in range(2)]
+    for step in steps:
+        step.capture()
+    streams = [torch.cuda.Stream() for _ in steps]
+    for _ in range(3):
+        for step in steps:
+            step.result.fill_(float("nan"))
+        torch.cuda.synchronize()
+        for step, stream in zip(steps, streams):
+            with torch.cuda.stream(stream):
+                step.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(step.result, want) for step in steps)
+
+
 # ------------------------------------------------------------------------------------------------ refusals
 
 def test_the_other_entry_points_refuse_8_bit_caches():
