@@ -64,8 +64,12 @@ struct QdShape {
   static constexpr int kBytes = kQBytes > kAccBytes ? kQBytes : kAccBytes;
 };
 
+// CTAs that an SM is to hold at least.  head_dim 64: a warp has half or a quarter of the bytes of the other forms under way, so more warps have to be
+// there (126 rows of 4850 - 9700 keys, 4 heads of 64: 180 us with what 98 registers leave room for, 160 with five; six, at 80 registers, 152
+// and small calls 7% slower; 64 rows of 4 tokens, 16 heads over 2, 43 -> 34 with four).
+constexpr int qd_resident(int dim, int tiles, bool pack) { return dim == 64 ? (tiles > 1 ? 4 : pack ? 5 : 1) : pack && dim == 256 ? 3 : 1; }
 template <typename T, int kD, int kTiles, bool kPack>
-__global__ void __launch_bounds__(kQdThreads, kPack && kD == 256 ? 3 : 1) quantized_decode_kernel(QDecodeParams p, int ctas) {
+__global__ void __launch_bounds__(kQdThreads, qd_resident(kD, kTiles, kPack)) quantized_decode_kernel(QDecodeParams p, int ctas) {
   constexpr bool kF32 = std::is_same<T, float>::value;
   using S = QdShape<kD, kTiles, kPack, kF32>;
   constexpr int kCols = S::kCols, kParts = kD / 64;  // parts of 64 dims: one 16-byte piece per lane and key row
