@@ -65,7 +65,7 @@ struct QdShape {
 };
 
 // CTAs that an SM is to hold at least.  head_dim 64: a warp has half or a quarter of the bytes of the other forms under way, so more warps have to be
-// there (126 rows of 4850 - 9700 keys, 4 heads of 64: 180 us with what 98 registers leave room for, 160 with five; six, at 80 registers, 152
+// there (126 rows of 4850 - 9700 keys, 4 heads of 64: 180 us with as few as there were, 160 with five; six, at 80 registers, 152
 // and small calls 7% slower; 64 rows of 4 tokens, 16 heads over 2, 43 -> 34 with four).
 constexpr int qd_resident(int dim, int tiles, bool pack) { return dim == 64 ? (tiles > 1 ? 4 : pack ? 5 : 1) : pack && dim == 256 ? 3 : 1; }
 template <typename T, int kD, int kTiles, bool kPack>
@@ -73,6 +73,9 @@ __global__ void __launch_bounds__(kQdThreads, qd_resident(kD, kTiles, kPack)) qu
   constexpr bool kF32 = std::is_same<T, float>::value;
   using S = QdShape<kD, kTiles, kPack, kF32>;
   constexpr int kCols = S::kCols, kParts = kD / 64;  // parts of 64 dims: one 16-byte piece per lane and key row
+  // Tiles that a warp has under way; one of 64 dims is 2 KiB (with one of them 126 rows of 4850 - 9700 keys, 4 heads, 160 us instead of 154, 16 heads
+  // over 2 104 instead of 94).
+  constexpr int kAhead = kD == 64 && kTiles == 1 ? 2 : 1;
   constexpr int kVHalves = kD >= 128 ? kD / 128 : 1;  // parts of 128 dims of V (64: 8-byte pieces)
   constexpr int kVWords = kD >= 128 ? 4 : 2;          // words of a V piece
   constexpr int kMTiles = kD / 16;
@@ -109,6 +112,15 @@ __global__ void __launch_bounds__(kQdThreads, qd_resident(kD, kTiles, kPack)) qu
     return b < p.table_width ? table[b] : -1;
   };
   int id = fetch_id(tile);
+  // (the 32 tiles behind them, if registers run two tiles ahead: one outside the pool is flagged with its scales)
+  int next_ids = -1;
+  auto fetch_next_ids = [&](int first) {
+    if constexpr (kAhead > 1) {
+      next_ids = fetch_id(first + 32 * step);
+      if (next_ids >= p.num_blocks) next_ids = -1;
+    }
+  };
+  fetch_next_ids(tile);
   if (!live) len = 0;
   if (len > p.table_width * (long long)p.block_size) {
     if (threadIdx.x == 0 && rank == 0) atomicOr(p.status, NVJ_DEV_BAD_LENGTH);
@@ -128,9 +140,9 @@ __global__ void __launch_bounds__(kQdThreads, qd_resident(kD, kTiles, kPack)) qu
     }
   };
   const long long key_stride = (long long)p.num_kv_heads * kD;
-  uint4 kr[kParts][2];                // keys g and g + 8: dims 64 part + 16 t ..
-  uint4 vr[kVHalves][4];              // keys 2t, 2t + 1, 2t + 8, 2t + 9: dims 128 half + 16 g .. (64 dims: 8 g ..)
-  auto load_k = [&](int tile_id, int which) {
+  uint4 k_held[kAhead][kParts][2];    // keys g and g + 8: dims 64 part + 16 t ..
+  uint4 v_held[kAhead][kVHalves][4];  // keys 2t, 2t + 1, 2t + 8, 2t + 9: dims 128 half + 16 g .. (64 dims: 8 g ..)
+  auto load_k = [&](uint4 (&kr)[kParts][2], int tile_id, int which) {
     if (tile_id < 0) {
 #pragma unroll
       for (int s = 0; s < kParts; ++s) kr[s][0] = kr[s][1] = make_uint4(0, 0, 0, 0);
@@ -143,7 +155,7 @@ __global__ void __launch_bounds__(kQdThreads, qd_resident(kD, kTiles, kPack)) qu
       kr[s][1] = ld_stream_u4(at + 8 * key_stride + 64 * s);
     }
   };
-  auto load_v = [&](int tile_id, int which) {
+  auto load_v = [&](uint4 (&vr)[kVHalves][4], int tile_id, int which) {
     const int first = which * 16 + 2 * t;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -170,9 +182,14 @@ __global__ void __launch_bounds__(kQdThreads, qd_resident(kD, kTiles, kPack)) qu
   int slot = 0;  // lane that holds the current tile's id and scales
   if (tile < tiles) {
     fetch_scales(tile);
-    const int first_id = __shfl_sync(kFullMask, id, 0);
-    load_k(first_id, tile);
-    load_v(first_id, tile);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int first_id = __shfl_sync(kFullMask, id, u);
+      if (tile + u * step < tiles) {
+        load_k(k_held[u], first_id, tile + u * step);
+        load_v(v_held[u], first_id, tile + u * step);
+      }
+    }
   }
 
   // queries into shared memory: a warp a column at a time, lane l the dims 8 l .. (f16 after a power of two that brings the largest
@@ -234,7 +251,7 @@ __global__ void __launch_bounds__(kQdThreads, qd_resident(kD, kTiles, kPack)) qu
 #pragma unroll
       for (int k = 0; k < 4; ++k) acc[j][i][k] = 0.f;
 
-  while (tile < tiles) {
+  auto work_on = [&](uint4 (&kr)[kParts][2], uint4 (&vr)[kVHalves][4]) {
     const float k_unit = __shfl_sync(kFullMask, ks, slot), v_log = __log2f(__shfl_sync(kFullMask, lv, slot));
     const bool usable = __shfl_sync(kFullMask, id, slot) >= 0;
     // S^T = K Q^T: rows keys, columns queries
@@ -259,18 +276,24 @@ __global__ void __launch_bounds__(kQdThreads, qd_resident(kD, kTiles, kPack)) qu
             q_mma(s[j], q_half2(lo[k]), q_half2(hi[k]), q_half2_high(lo[k]), q_half2_high(hi[k]), b[2 * k], b[2 * k + 1]);
         }
     }
-    // the next tile's K rows
+    // the K rows of the tile that is to take these registers
     const int this_tile = tile;
     tile += step;
+    const int next = tile + (kAhead - 1) * step;
     if (++slot == 32) {
       slot = 0;
       if (tile < tiles) {
-        id = fetch_id(tile);
+        id = kAhead > 1 ? next_ids : fetch_id(tile);
         fetch_scales(tile);
+        fetch_next_ids(tile);
       }
     }
-    const int next_id = __shfl_sync(kFullMask, id, slot);
-    if (tile < tiles) load_k(next_id, tile);
+    int next_id = __shfl_sync(kFullMask, id, (slot + kAhead - 1) & 31);
+    if constexpr (kAhead > 1) {
+      const int behind = __shfl_sync(kFullMask, next_ids, (slot + kAhead - 1) & 31);
+      if (slot + kAhead - 1 >= 32) next_id = behind;
+    }
+    if (next < tiles) load_k(kr, next_id, next);
 
     // scores in log2 units; whether one passes its maximum by more than the slack
     bool over = false;
@@ -346,7 +369,12 @@ __global__ void __launch_bounds__(kQdThreads, qd_resident(kD, kTiles, kPack)) qu
         }
       }
     }
-    if (tile < tiles) load_v(next_id, tile);
+    if (next < tiles) load_v(vr, next_id, next);
+  };
+  while (tile < tiles) {
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (tile < tiles) work_on(k_held[u], v_held[u]);
   }
 
   // the warps' sums into shared memory (the queries are no longer needed)
