@@ -578,6 +578,35 @@ def test_prefill_with_any_count_of_tiles(tiles):
     _long_prefill((32, 8, 128, 16), BF16, [(150, 900), (70, 0), (2, 333)], dict(num_decode_rows=0, query_tile_pairs=tiles), 22, 33)
 
 
+# rows of several windows of 32 tiles per warp; a block outside the pool in a later window
+@pytest.mark.parametrize("shape,dtype", [((6, 6, 64, 48), BF16), ((16, 2, 64, 32), F16), ((32, 8, 64, 16), F32), ((4, 1, 128, 16), BF16)])
+def test_long_rows_on_the_mma_sync_tiles(shape, dtype, monkeypatch):
+    hq, hkv, d, bs = shape
+    rng = np.random.default_rng(37)
+    rows, width = 130, 20000 // bs
+    lens = rng.integers(1, width * bs + 1, rows)
+    lens[:4] = [width * bs, 8193, 16400, 1]
+    tables = rng.integers(0, 90, (rows, width))  # (rows share blocks)
+    state = [_pool(rng, 90, shape, spread=1) for _ in range(2)]
+    (k, ks), (v, vs) = (_gpu(*x) for x in state)
+    q, q64 = _queries(rng, (rows, hq, d), dtype)
+    out = Q.paged_decode_attention_quantized(q, k, v, ks, vs, _i32(tables), _i32(lens), d ** -0.5, form=1)
+    pick = [0, 1, 2, 3, 77, 129]
+    _check(_f64(out[pick])[:, None], q64[pick][:, None], state, tables[pick], lens[pick], [[n] for n in lens[pick]], d ** -0.5)
+    monkeypatch.setenv("NVJ_CHECK_STATUS", "0")
+    for bad in (90, -3, 1 << 30):
+        broken = tables.copy()
+        broken[0, 12000 // bs] = bad
+        got = Q.paged_decode_attention_quantized(q, k, v, ks, vs, _i32(broken), _i32(lens), d ** -0.5, form=1)
+        with pytest.raises(K.DeviceStatusError, match="device status 2 "):
+            K.check_device_status()
+        seen = np.arange(lens[0]) // bs != 12000 // bs
+        kk, vv = (R.gather(codes, x, tables[0], lens[0]) for codes, x in state)
+        want = R.attend(q64[:1], kk[seen], vv[seen], np.ones((1, seen.sum()), bool), d ** -0.5)[0]
+        assert np.abs(_f64(got[0]) - want).max() <= R.tolerance(q64[:1], kk, vv, d ** -0.5)
+        assert torch.equal(got[1:], out[1:])
+
+
 TILES = [((32, 8, 128, 16), F16), ((16, 1, 256, 16), BF16), ((8, 2, 256, 16), F32), ((16, 2, 64, 32), BF16)]  # shapes of the 8-bit tiles
 
 
