@@ -17,6 +17,8 @@
 //   * the K scale of a block multiplies its scores, the V scale goes into the exponent of the weights: a running maximum of
 //     its own for the weighted sum keeps blocks of any scale apart from the sum of the weights.
 // Maxima are lazy: one vote per tile says whether a score has left them behind, and only then the sums are rescaled.
+// Measured: four rows of 64 - 512 keys, 8 heads of 256 over 2, 7.3 us, which is launch, trips and merge; 126 rows of 4850 - 9700 keys, 4 heads of 64, 154 us
+// (47% of the copy rate), 16 over 2 94 us (38%): instructions.
 
 #include "cluster.cuh"
 #include "decode_parts.cuh"

@@ -14,16 +14,20 @@
 //
 // Work split: CTA = (range, kv head and column tile).  The units of 16 to 64 keys of all rows form one sequence that is cut into equal ranges
 // (decode_parts.cuh); rows cut over ranges leave partials, folded by a second small launch.
-//   warps 0 - 7   softmax, thread = key, in two groups of four warps.  Up to eight columns the groups take the tiles in turn, each with
-//                 references, sums and accumulators of its own (a tile's chain of waits, from its scores to its weights, is longer than
-//                 its bytes: one group alone took 1.85 us per tile of 64 KiB); with 16 or 24 they take half of the columns each.
-//                 Scores from tensor memory, times the K scale of the key's block, plus the log2 of its V scale; weights exp2(that -
-//                 reference) as e4m3 terms into shared memory; their sum with the V scale divided out again (relative to the first
-//                 tile's largest).  Thread = dim when a row's segment ends.
-//   warps 8, 9    MMA issue: the scores (up to two tiles ahead), the weighted sums.
-//   warp 10       TMA producer: boxes of a unit's keys [8-key group][128-byte chunk][8 keys][128 B], 128-byte swizzle, into rings of tiles of K
-//                 and of V (160 KiB), and with K the scales of its blocks.
-//   warp 11       the queries, up to two segments ahead: scaled to 2^7 - 2^8 by a power of two per column, split into terms.
+//   softmax    thread = key, in groups of four warps.  Up to eight columns two groups take the tiles in turn, each with
+//              references, sums and accumulators of its own (a tile's chain of waits, from its scores to its weights, is longer than
+//              its bytes: one group alone took 1.85 us per tile of 64 KiB); of 16 or 24 two or three groups take eight each (two of twelve:
+//              64 rows of 5 tokens 50.4 us, three of eight 47.6).
+//              Scores from tensor memory, times the K scale of the key's block, plus the log2 of its V scale; weights exp2(that -
+//              reference) as e4m3 terms into shared memory; their sum with the V scale divided out again (relative to the first
+//              tile's largest).  Thread = dim when a row's segment ends.
+//   2 warps    MMA issue: the scores (up to two tiles ahead), the weighted sums.
+//   1 warp     TMA producer: boxes of a unit's keys [8-key group][128-byte chunk][8 keys][128 B], 128-byte swizzle, into rings of tiles of K
+//              and of V (160 KiB), and with K the scales of its blocks.
+//   1 warp     the queries, up to two segments ahead: scaled to 2^7 - 2^8 by a power of two per column, split into terms.
+// Measured, 8 bf16 heads of 256 over 2: 256 rows of 1024 - 4096 keys 107 us (6.3 TB/s, 96% of the copy rate), 64 of 8192 - 32768 200 us (103%), 64 of
+// 1024 - 4096 with 5 tokens each 47.5 us (55%: bound by a tile's way from scores to weights, 1.75 us where its bytes take 1.4); 48 f16 rows of 200 - 3000
+// keys, 32 heads of 128 over 8, 37.7 us (64%: 5 us until the first scores, 5 for the fold).
 // Every wait is bounded; after a timeout (NVJ_DEV_TIMEOUT) the kernel stops issuing, lets copies land and frees its tensor
 // memory.  A block id outside the pool is flagged, fetched from beyond the tensor (zeros) and its keys are left out.
 #pragma once
@@ -228,7 +232,7 @@ __device__ __forceinline__ UmmaCut qu_cut(const QuParams& a, const DecodeParams&
   return UmmaCut{b, first, pt.cta_of(g0 - j + nb - 1), 0};
 }
 
-// ---- warp 10: TMA loads ------------------------------------------------------------------------------------------------------------
+// ---- TMA loads ------------------------------------------------------------------------------------------------------------
 template <class L>
 __device__ __forceinline__ void qu_producer(const CUtensorMap* k_map, const CUtensorMap* v_map, const QuParams& a, const DecodeParams& p, QuSmem<L>& sm,
                                             int head, QuWalk walk, int lane) {
@@ -306,7 +310,7 @@ __device__ __forceinline__ void qu_producer(const CUtensorMap* k_map, const CUte
   }
 }
 
-// ---- warps 8 and 9: MMA issue -------------------------------------------------------------------------------------------------
+// ---- MMA issue -------------------------------------------------------------------------------------------------
 // A warp for either product: a tile's ~ 500 cycles of waits, descriptors and commits on each side would otherwise add up to more than its
 // bytes take (head_dim 128).  S(n) takes the place of S(n - 2), which has been read when that tile's weights are there.
 template <class L>
@@ -380,7 +384,7 @@ __device__ __forceinline__ void qu_sums_warp(QuSmem<L>& sm, const QuParams& a, c
   }
 }
 
-// ---- warps 0 - 7: softmax and output.  Thread = key of the tile, then dim of the output ---------------------------------------
+// ---- softmax and output.  Thread = key of the tile, then dim of the output ---------------------------------------
 // (A wait that runs out does so for one warp and perhaps not for the next: a group's warps leave together, behind a meeting.)
 template <class L, int kCg>
 __device__ __forceinline__ void qu_softmax_warps(QuSmem<L>& sm, const QuParams& a, const DecodeParams& p, uint32_t tmem, int head, int hct, int ct,
@@ -707,7 +711,7 @@ struct QuColumn {  // from column c on: column c + l / kLanes, dims 8 (l % kLane
 __device__ __forceinline__ long long qu_first_token(const QuParams& a, int b) {
   return a.query_start_loc ? (long long)a.query_start_loc[b] : (long long)b * a.width;
 }
-// Warp 11: the segments behind the first, whose queries all warps have brought in before.
+// The query warp: the segments behind the first, whose queries all warps have brought in before.
 template <class L, typename T, int kCg>
 __device__ __forceinline__ void qu_query_warp(QuSmem<L>& sm, const QuParams& a, const DecodeParams& p, int ct, QuWalk walk, int lane) {
   QuSeg s;
