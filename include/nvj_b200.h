@@ -479,7 +479,8 @@ int nvj_kv_append_quantized(const void* new_k, const void* new_v, int src_dtype,
  * A length beyond the block table is flagged and clipped, a block id outside the pool flagged and its keys left out.
  *
  *   form       0 automatic, 1 mma.sync tiles on thread-block clusters (width * num_q_heads / num_kv_heads <= 16 columns per pass over a
- *              row's keys), 2 tcgen05 tiles (24 columns; head_dim 128 or 256, else NVJ_ERR_UNSUPPORTED)
+ *              row's keys), 2 tcgen05 tiles (24 columns; head_dim 128 or 256, else NVJ_ERR_UNSUPPORTED; a row's V scales may be any, but what
+ *              lies 2^90 below its largest values is only right to 2^-90 of those)
  *   workspace  nullable scratch of nvj_paged_decode_quantized_workspace_bytes(..., form) bytes (0: the call has no use for one), 16-byte
  *              aligned, nothing kept in it between calls; without one the automatic choice is form 1
  */

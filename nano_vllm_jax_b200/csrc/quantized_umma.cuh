@@ -19,8 +19,8 @@
 //              its bytes: one group alone took 1.85 us per tile of 64 KiB); of 16 or 24 two or three groups take eight each (two of twelve:
 //              64 rows of 5 tokens 50.4 us, three of eight 47.6).
 //              Scores from tensor memory, times the K scale of the key's block, plus the log2 of its V scale; weights exp2(that -
-//              reference) as e4m3 terms into shared memory; their sum with the V scale divided out again (relative to the first
-//              tile's largest).  Thread = dim when a row's segment ends.
+//              reference) as e4m3 terms into shared memory; their sum with the V scale divided out again, relative to the largest so far.
+//              Thread = dim when a row's segment ends.
 //   2 warps    MMA issue: the scores (up to two tiles ahead), the weighted sums.
 //   1 warp     TMA producer: boxes of a unit's keys [8-key group][128-byte chunk][8 keys][128 B], 128-byte swizzle, into rings of tiles of K
 //              and of V (160 KiB), and with K the scales of its blocks.
@@ -46,7 +46,12 @@ constexpr int kQuUnits = 8;     // boxes per tile, at most: a box is a unit of 1
 constexpr int kQuPTerms = 5;
 // The reference of a column's weights is set 2^3 below its largest weight and moved when one would pass 2^8 (e4m3 ends at 448).
 constexpr float kQuNone = -3e38f, kQuSlack = 8.f, kQuLift = 3.f;
-constexpr float kQuMostInverse = 100.f;  // log2 of what a weight is multiplied by, at most, to take the V scale out of it again
+// V scales reach from 2^-117 (the append's for a block of zeros) to 2^119.  A sum of weights is of exp2(score - (reference - v_top)), v_top the
+// log2 of the group's largest V scale so far, but for kQuFar; the weight of a key whose block is 2^kQuFar quieter may be zero and says nothing of that
+// any more, so that such keys take an exponential of their own (for all keys: 64 rows of 5 tokens 48.6 -> 53 us).  Next to a loud block
+// their share may be as large as 2^(score's lead): it ends at 2^kQuMost, where a row's loud keys weigh 2^-kQuMost and less.  So what a
+// row's output owes to values 2^-90 of the largest of its blocks and smaller may be off, by 2^-90 of that largest one at most.
+constexpr float kQuFar = 40.f, kQuMost = 106.f, kQuMostSum = 0x1p108f;  // (10^6 keys of 2^kQuMost are an f32 number)
 
 template <typename T>
 constexpr int quq_terms() {
@@ -405,7 +410,7 @@ __device__ __forceinline__ void qu_softmax_warps(QuSmem<L>& sm, const QuParams& 
     const int* limit = sm.limit[seg & 3u] + first_col;
     const uint32_t n0 = n;
     bool begun = false;  // the group has had a tile of this segment
-    float l[kCg], m[kCg], v_first = 0.f;
+    float l[kCg], m[kCg], v_top = kQuNone;
 #pragma unroll
     for (int c = 0; c < kCg; ++c) {
       l[c] = 0.f;
@@ -424,7 +429,7 @@ __device__ __forceinline__ void qu_softmax_warps(QuSmem<L>& sm, const QuParams& 
       const bool ok = um_wait(&sm.s_full[buf], phase, &sm.abort_flag, p.status);
       tc_fence_after_sync();
       const float k_unit = sm.k_unit[n & 7u][my_unit], v_unit = my_unit < cnt ? sm.v_unit[n & 7u][my_unit] : -1.f;
-      const float v_log = v_unit >= 0.f ? __log2f(v_unit) : 0.f;
+      const float v_log = v_unit >= 0.f ? __log2f(fmaxf(v_unit, 0x1p-126f)) : v_top;
       float sc[kCg];
       {
         float x[kSRead][8];
@@ -446,7 +451,7 @@ __device__ __forceinline__ void qu_softmax_warps(QuSmem<L>& sm, const QuParams& 
           sc[c] = there && at_key < seen[c] ? fmaf(y, by[c] * k_unit, v_log) : -INFINITY;
         }
       }
-      bool above = !begun;
+      bool above = v_log > v_top + kQuFar || !begun;
 #pragma unroll
       for (int c = 0; c < kCg; ++c) above |= sc[c] > m[c] + kQuSlack;
       if (qu_meet_any<128>(bar, !ok || above)) {
@@ -457,8 +462,8 @@ __device__ __forceinline__ void qu_softmax_warps(QuSmem<L>& sm, const QuParams& 
           const float x = qu_warp_max(sc[c]);
           if (lane == 0) sm.red[group][warp][c] = x;
         }
-        if (!begun) {
-          const float x = qu_warp_max(v_unit >= 0.f ? v_log : -INFINITY);
+        {
+          const float x = qu_warp_max(v_unit >= 0.f ? v_log : kQuNone);
           if (lane == 0) sm.red_v[group][warp] = x;
         }
         // (the group's weighted sums so far have to be complete)
@@ -466,6 +471,9 @@ __device__ __forceinline__ void qu_softmax_warps(QuSmem<L>& sm, const QuParams& 
         const bool complete = !begun || um_wait(&sm.pv_done[done & 1u], (done >> 1) & 1u, &sm.abort_flag, p.status);
         if (qu_meet_any<128>(bar, !ok || !complete)) return give_up();
         float f[kCg];
+        const float v_most = fmaxf(fmaxf(sm.red_v[group][0], sm.red_v[group][1]), fmaxf(sm.red_v[group][2], sm.red_v[group][3]));
+        const float v_now = v_most > v_top + kQuFar ? v_most : v_top, raised = v_now - v_top;
+        v_top = v_now;
 #pragma unroll
         for (int c = 0; c < kCg; c += 4) {
           float x[4], y[4];
@@ -480,14 +488,12 @@ __device__ __forceinline__ void qu_softmax_warps(QuSmem<L>& sm, const QuParams& 
           for (int e = 0; e < 4; ++e) {
             const float now = x[e] > m[c + e] + kQuSlack ? x[e] - kQuLift : m[c + e];  // (one whose scores stay under it keeps its reference)
             f[c + e] = ex2_approx(m[c + e] - now);
-            l[c + e] *= f[c + e];
+            l[c + e] *= ex2_approx(fminf((m[c + e] - now) + raised, 126.f));
+            l[c + e] = l[c + e] > kQuMostSum ? kQuMostSum : l[c + e];
             m[c + e] = now;
           }
         }
-        if (!begun) {
-          v_first = fmaxf(fmaxf(sm.red_v[group][0], sm.red_v[group][1]), fmaxf(sm.red_v[group][2], sm.red_v[group][3]));
-          v_first = v_first == -INFINITY ? 0.f : v_first;
-        } else {
+        if (begun) {
           tc_fence_after_sync();
 #pragma unroll 1
           for (int k = 0; k < L::kSets; ++k) {
@@ -517,11 +523,17 @@ __device__ __forceinline__ void qu_softmax_warps(QuSmem<L>& sm, const QuParams& 
       // weights as e4m3 terms: byte term * kCg + column of the group's region of the key's row
       {
         float r[kCg];
-        const float inverse = ex2_approx(fminf(v_first - v_log, kQuMostInverse));
+        const float back = v_top - v_log;
+        const bool far = back > kQuFar;
+        const float inverse = far ? 0.f : ex2_approx(back);
 #pragma unroll
         for (int c = 0; c < kCg; ++c) {
           r[c] = ex2_approx(sc[c] - m[c]);
           l[c] = fmaf(r[c], inverse, l[c]);
+        }
+        if (__builtin_expect(far, 0)) {
+#pragma unroll
+          for (int c = 0; c < kCg; ++c) l[c] += ex2_approx(fminf((sc[c] - m[c]) + back, kQuMost));
         }
         uint32_t bytes[kWords];
 #pragma unroll
@@ -579,7 +591,7 @@ __device__ __forceinline__ void qu_softmax_warps(QuSmem<L>& sm, const QuParams& 
 #pragma unroll
       for (int c = 0; c < kCg; ++c) {
         sm.mv[group][c] = m[c];
-        sm.m[group][c] = m[c] - v_first;
+        sm.m[group][c] = m[c] > kQuNone ? m[c] - v_top : kQuNone;
       }
     }
     if (qu_meet_any<L::kSoftmaxThreads>(3, !um_wait(&sm.o_full, seg & 1u, &sm.abort_flag, p.status))) return;

@@ -1,0 +1,135 @@
+"""Attention over the 8-bit cache where scales, masks, tables and batches have edges, against 64-bit sums (test_gpu_quantized_kv.py has the ordinary cases)."""
+
+import numpy as np
+import pytest
+import torch
+
+import quantized_reference as R
+from nano_vllm_jax_b200.kernels import paged_kv as K
+from nano_vllm_jax_b200.kernels import quantized_kv as Q
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+MODEL = (8, 2, 256, 16)  # query heads, kv heads, head_dim, block size
+
+
+def _i32(x):
+    return torch.from_numpy(np.ascontiguousarray(x, dtype=np.int32)).cuda()
+
+
+def _f64(t):
+    return t.double().cpu().numpy()
+
+
+def _gpu(codes, scale):
+    return torch.from_numpy(codes.copy()).cuda().view(torch.float8_e4m3fn), torch.from_numpy(scale.astype(np.float32)).cuda()
+
+
+def _rows(rng, lens, shape):
+    """A pool without spare blocks: tables, and [(bytes, scales)] of K and of V, values about 1."""
+    _, hkv, d, bs = shape
+    need = [-(-n // bs) for n in lens]
+    ids, tables, at = rng.permutation(sum(need)), np.zeros((len(lens), max(need)), np.int64), 0
+    for r, n in enumerate(need):
+        tables[r, :n] = ids[at: at + n]
+        at += n
+    state = []
+    for _ in range(2):
+        codes = rng.integers(0, 256, (sum(need), bs, hkv, d)).astype(np.uint8)
+        codes[(codes & 127) == 127] = 1
+        state.append((codes, np.full((sum(need), hkv), 2.0 ** -8)))
+    return tables, state
+
+
+def _attend(route, q, state, tables, lens, limits, shape, scale):
+    """q [rows, tokens, hq, d]; token t of row r sees keys below limits[r][t].  Routes: the decode forms 1 and 2, and "prefill"."""
+    hq, hkv, d, bs = shape
+    (k, ks), (v, vs) = (_gpu(*s) for s in state)
+    args = (k, v, ks, vs, _i32(tables), _i32(lens))
+    rows, tokens = q.shape[:2]
+    if route == "prefill":
+        out = Q.packed_paged_prefill_attention_quantized(q.reshape(1, rows * tokens, hq, d), *args, _i32(np.asarray(limits).reshape(1, -1) - 1),
+                                                         _i32(np.arange(rows + 1) * tokens), bs, scale, hq // hkv, num_decode_rows=0)
+    else:
+        out = Q.paged_decode_attention_quantized(q, *args, scale, positions=_i32(np.asarray(limits) - 1), form=route)
+    return _f64(out).reshape(q.shape)
+
+
+TERM_BITS = {1: 22, 2: 20, "prefill": 22}  # of a route's softmax weights
+
+
+def _check(out, q, state, tables, lens, limits, scale, term_bits):
+    q = _f64(q)
+    for r, n in enumerate(lens):
+        k, v = (R.gather(codes, s, tables[r], n) for codes, s in state)
+        want = R.attend(q[r], k, v, np.arange(n)[None] < np.minimum(limits[r], n)[:, None], scale)
+        off = np.abs(out[r] - want).max()
+        assert np.isfinite(out[r]).all() and off <= R.tolerance(q[r], k, v, scale, term_bits), (r, n, off)
+
+
+# ------------------------------------------------------------------------------------------------ scales far apart
+
+def _quiet(pattern, blocks):
+    """Which of a row's blocks are the quiet ones."""
+    b = np.arange(blocks)
+    return {"first": b == 0, "last": b == blocks - 1, "front": b < blocks // 2, "back": b >= blocks // 2, "every other": b % 2 == 0, "all but one": b != blocks // 3}[pattern]
+
+
+PATTERNS = ("first", "last", "front", "back", "every other", "all but one")
+DECODES = [(MODEL, 1, BF16), ((32, 8, 128, 16), 1, F16), ((32, 8, 128, 32), 2, F32), ((24, 2, 128, 64), 1, BF16), (MODEL, 5, BF16), (MODEL, 4, F32), ((6, 6, 64, 48), 1, BF16)]
+
+
+# Exponents of the V scales of a row's quiet and other blocks.  The append gives a block of zeros 2^-117, and values about 1 2^-8.  Scores are alike
+# on both sides, so that the keys of the quiet blocks, which add next to nothing to the weighted sum, are half of the sum of the weights.
+@pytest.mark.parametrize("quiet,loud", [(-117, -8), (-117, 30), (-100, 60), (-60, 30)])
+@pytest.mark.parametrize("shape,tokens,dtype", DECODES)
+@pytest.mark.parametrize("form", [1, 2])
+def test_decode_over_blocks_whose_scales_lie_far_apart(form, shape, tokens, dtype, quiet, loud):
+    hq, hkv, d, bs = shape
+    if form == 2 and d < 128:
+        pytest.skip("the tcgen05 form is for head_dim 128 and 256")
+    rng = np.random.default_rng(50)
+    lens = [160 + 7 * i for i in range(len(PATTERNS))] + [3000 + 11 * i for i in range(len(PATTERNS))]
+    tables, state = _rows(rng, lens, shape)
+    for r, n in enumerate(lens):
+        blocks = -(-n // bs)
+        still = _quiet(PATTERNS[r % len(PATTERNS)], blocks)
+        state[1][1][tables[r, :blocks]] = np.where(still, 2.0 ** quiet, 2.0 ** loud)[:, None]
+        if quiet == -117:
+            state[1][0][tables[r, :blocks][still]] = 0
+    state[1][1][tables[0, :10], 0] = 2.0 ** -8  # (a head of its own: nothing far apart there)
+    q = torch.from_numpy(rng.standard_normal((len(lens), tokens, hq, d))).to(dtype).cuda()
+    limits = np.array(lens)[:, None] - tokens + 1 + np.arange(tokens)[None]
+    out = _attend(form, q, state, tables, lens, limits, shape, d ** -0.5)
+    _check(out, q, state, tables, lens, limits, d ** -0.5, TERM_BITS[form])
+
+
+@pytest.mark.parametrize("power", [-117, 100])
+@pytest.mark.parametrize("form", [1, 2])
+def test_decode_over_values_of_extreme_scales(form, power):
+    hq, hkv, d, bs = MODEL
+    rng = np.random.default_rng(51)
+    lens = [40, 2500, 300]
+    tables, state = _rows(rng, lens, MODEL)
+    state[1][1][:] = 2.0 ** power
+    q = torch.from_numpy(rng.standard_normal((3, 1, hq, d))).to(BF16).cuda()
+    limits = np.array(lens)[:, None]
+    _check(_attend(form, q, state, tables, lens, limits, MODEL, 1 / 16), q, state, tables, lens, limits, 1 / 16, TERM_BITS[form])
+
+
+# A row's last block is 2^80 as loud as the others and only its last token sees it: what the other tokens see is summed as well as in a row without it.
+@pytest.mark.parametrize("length", [96, 144, 1000 * 16])
+@pytest.mark.parametrize("form", [1, 2])
+def test_decode_of_tokens_that_do_not_see_the_loud_block(form, length):
+    hq, hkv, d, bs = MODEL
+    rng = np.random.default_rng(52)
+    lens = [length + bs]
+    tables, state = _rows(rng, lens, MODEL)
+    state[1][1][:] = 2.0 ** -60
+    state[1][1][tables[0, -1]] = 2.0 ** 20
+    q = torch.from_numpy(rng.standard_normal((1, 3, hq, d))).to(BF16).cuda()
+    limits = np.array([[length - 5, length, length + bs]])
+    out = _attend(form, q, state, tables, lens, limits, MODEL, 1 / 16)
+    for t, n in enumerate(limits[0]):
+        _check(out[:, t: t + 1], q[:, t: t + 1], state, tables, [n], limits[:, t: t + 1], 1 / 16, TERM_BITS[form])
