@@ -20,8 +20,9 @@
 //   warps 8 - 11   keys: 16-byte pieces of the blocks to registers, one tile ahead, and from there as f16 to their tiles
 //   warps 12 - 15  values, in the same way; the first issues the weighted sums' MMAs, the second the scores', a tile ahead
 // The weights of a row are exp2(score - reference) times the V scale; the reference is set so that the largest weight is 2^7,
-// and moved when a later one would pass 2^15 (f16 ends at 2^16), which is rare.  Their sum is taken in f32 with the V scale
-// divided out again, relative to the first tile's largest.
+// and moved when a later one would pass 2^15 (f16 ends at 2^16), which is rare.  Their sum is taken in f32, relative to the largest score's: the
+// weights of 16 keys of one block with the block's V scale divided out again, or, where a block is so quiet that its weights may be
+// zero although its keys count in that sum (the append gives a block of zeros 2^-117), exponentials of their own.
 // The tensor cores cut the last place of what they add to: 1.2e-5 of a sum over 16384 keys.  After kQtFlush tiles the sums are
 // emptied into the output row (clusters: into scratch) and begun again.
 // Every wait is bounded; after a timeout (NVJ_DEV_TIMEOUT) the kernel stops issuing, lets MMAs land and frees its tensor memory.
@@ -36,14 +37,15 @@ namespace nvj {
 
 constexpr int kQtRows = 128, kQtKeys = 64, kQtThreads = 512, kQtSoftmax = 256, kQtLoaders = 128;
 constexpr int kQtColS = 256, kQtColP = 384;  // of tensor memory: O from 0, S twice, P twice (two terms of 32 columns)
-constexpr float kQtNone = -3e38f, kQtSlack = 8.f, kQtLift = 7.f, kQtMostInverse = 100.f;
+constexpr float kQtNone = -3e38f, kQtSlack = 8.f, kQtLift = 7.f;
+constexpr float kQtFar = 40.f;  // log2 of what weights are multiplied by, at most, on their way into their sum
 
 template <typename T, int kD>
 struct QtSmem {
   static constexpr int kQTerms = std::is_same<T, float>::value ? 2 : 1;
   static constexpr int kChunks = kD / 64;                 // of 64 dims: 128 bytes of f16
   static constexpr int kTileBytes = kQtKeys * kD * 2;
-  static constexpr int kFit = (232448 - 1024 - 2048 - kQTerms * kChunks * 16384) / kTileBytes;
+  static constexpr int kFit = (232448 - 1024 - 3072 - kQTerms * kChunks * 16384) / kTileBytes;
   static constexpr int kKSlots = kFit >= 3 ? 2 : 1, kVSlots = kFit >= 4 ? 2 : 1;
   alignas(1024) char q[kQTerms][kChunks][kQtRows * 128];  // [chunk][row][128 B]
   alignas(1024) char k[kKSlots][kTileBytes];              // [8-key group][chunk][8 keys][128 B]
@@ -54,7 +56,7 @@ struct QtSmem {
   alignas(16) float k_unit[8][4], v_unit[8][4];
   float factor[kQtRows];
   int limit[kQtRows];
-  float red[kQtRows];  // between the two threads of a row
+  float2 red[kQtRows];  // between the two threads of a row
   int found[3], most, abort_flag;
   uint32_t tmem_base;
 };
@@ -289,9 +291,10 @@ struct QtQueries {
 };
 
 // ---- warps 0 - 7 ----------------------------------------------------------------------------------------------------------------
-__device__ __forceinline__ float qt_log(float v_unit) { return v_unit < 0.f ? -INFINITY : __log2f(v_unit); }
-struct QtRow {  // what a softmax thread knows of its row at the end
-  float m, l, v_first, m_flushed;
+// (A scale of zero is as good as the smallest there is.)
+__device__ __forceinline__ float qt_log(float v_unit) { return v_unit < 0.f ? -INFINITY : __log2f(fmaxf(v_unit, 0x1p-126f)); }
+struct QtRow {  // what a softmax thread knows of its row at the end: references of the weighted sums and of the sum l of the weights
+  float m, top, l, m_flushed;
 };
 template <typename T, int kD>
 __device__ __forceinline__ bool qt_softmax(QtSmem<T, kD>& sm, const QtParams& p, uint32_t tmem, int tile0, int tiles, int r, int half, int pair, float* flush_row,
@@ -300,9 +303,8 @@ __device__ __forceinline__ bool qt_softmax(QtSmem<T, kD>& sm, const QtParams& p,
   const float factor = sm.factor[r];
   const int limit = sm.limit[r];
   const int fewest = __reduce_min_sync(kFullMask, limit);
-  o.m = kQtNone;
+  o.m = o.top = kQtNone;
   o.l = 0.f;
-  o.v_first = 0.f;
   o.m_flushed = 0.f;
   bool begun = false;
   for (int n = 0; n < tiles; ++n) {
@@ -314,47 +316,43 @@ __device__ __forceinline__ bool qt_softmax(QtSmem<T, kD>& sm, const QtParams& p,
     const float2 unit = *reinterpret_cast<const float2*>(&sm.k_unit[n & 7][2 * half]), v_unit = *reinterpret_cast<const float2*>(&sm.v_unit[n & 7][2 * half]);
     const int key0 = (tile0 + n) * kQtKeys + half * 32;
     const float by[2] = {factor * unit.x, factor * unit.y}, plus[2] = {qt_log(v_unit.x), qt_log(v_unit.y)};
-    // exponents of the weights will be x * mul + add - reference
-    float top, mul[2], add[2];
+    // scores are x * mul; the exponents of the weights that and add - reference
+    float top, most, mul[2], add[2] = {plus[0], plus[1]};  // the largest score, and the largest with its V scale
     if (key0 + 32 > fewest || plus[0] == -INFINITY || plus[1] == -INFINITY || !(p.scale_log2 > 0.f)) {
-      top = -INFINITY;
+      float big[2] = {-INFINITY, -INFINITY};
 #pragma unroll
       for (int j = 0; j < 32; ++j) {
-        const float y = fmaf(x[j], by[j >> 4], plus[j >> 4]);
-        x[j] = key0 + j < limit && plus[j >> 4] != -INFINITY ? y : -INFINITY;
-        top = fmaxf(top, x[j]);
+        x[j] = key0 + j < limit && plus[j >> 4] != -INFINITY ? x[j] * by[j >> 4] : -INFINITY;
+        big[j >> 4] = fmaxf(big[j >> 4], x[j]);
       }
+      most = fmaxf(big[0], big[1]);
+      top = fmaxf(big[0] + plus[0], big[1] + plus[1]);
       mul[0] = mul[1] = 1.f;
-      add[0] = add[1] = 0.f;
     } else {  // the largest score of 16 keys of one block is the largest product's
       float big[2] = {x[0], x[16]};
 #pragma unroll
       for (int j = 0; j < 32; ++j) big[j >> 4] = fmaxf(big[j >> 4], x[j]);
+      most = fmaxf(big[0] * by[0], big[1] * by[1]);
       top = fmaxf(fmaf(big[0], by[0], plus[0]), fmaf(big[1], by[1], plus[1]));
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        mul[h] = by[h];
-        add[h] = plus[h];
-      }
+      mul[0] = by[0];
+      mul[1] = by[1];
     }
-    if (qt_pair_any(1 + pair, !ok || !begun || top > o.m + kQtSlack)) {
-      if (half == 0) sm.red[r] = top;
+    if (qt_pair_any(1 + pair, !ok || !begun || top > o.m + kQtSlack || most > o.top + kQtSlack)) {
+      if (half == 0) sm.red[r] = make_float2(top, most);
       const bool complete = !begun || um_wait(&sm.pv_done[buf ^ 1], ((n - 1) >> 1) & 1u, &sm.abort_flag, p.status);
       if (qt_pair_any(1 + pair, !ok || !complete)) return false;
       tc_fence_after_sync();
-      float both = top;
-      if (half == 1) sm.red[r] = both = fmaxf(top, sm.red[r]);
+      float2 both = make_float2(top, most);
+      if (half == 1) sm.red[r] = both = make_float2(fmaxf(top, sm.red[r].x), fmaxf(most, sm.red[r].y));
       qt_pair_any(1 + pair, false);
       if (half == 0) both = sm.red[r];
-      const float now = both > o.m + kQtSlack ? both - kQtLift : o.m;  // (a row whose scores stay under it keeps its reference)
+      const float now = both.x > o.m + kQtSlack ? both.x - kQtLift : o.m;  // (a row whose scores stay under it keeps its reference)
+      const float now_top = both.y > o.top + kQtSlack ? both.y : o.top;
       const float f = ex2_approx(o.m - now);
-      o.l *= f;
+      o.l *= ex2_approx(o.top - now_top);
       o.m = now;
-      if (!begun) {
-        const float* all = sm.v_unit[n & 7];
-        const float big = qt_log(fmaxf(fmaxf(all[0], all[1]), fmaxf(all[2], all[3])));
-        o.v_first = big == -INFINITY ? 0.f : big;
-      } else {
+      o.top = now_top;
+      if (begun) {
 #pragma unroll 1
         for (int c = half * kHalf; c < (half + 1) * kHalf; c += 32) {
           float y[32];
@@ -396,9 +394,16 @@ __device__ __forceinline__ bool qt_softmax(QtSmem<T, kD>& sm, const QtParams& p,
       high[j] = q_pair(a, b);
       low[j] = q_pair_rest(a, b, high[j]);
     }
-    // (a block that is not there has no weights, and no scale to divide by)
-    o.l = fmaf(sum[0], ex2_approx(fminf(o.v_first - plus[0], kQtMostInverse)), o.l);
-    o.l = fmaf(sum[1], ex2_approx(fminf(o.v_first - plus[1], kQtMostInverse)), o.l);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float back = (o.m - o.top) - plus[h];
+      if (back > kQtFar) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o.l += ex2_approx(fmaf(x[16 * h + j], mul[h], -o.top));
+      } else {
+        o.l = fmaf(sum[h], ex2_approx(back), o.l);
+      }
+    }
     // (the weights of tile n - 2, in the same place, have been used: almost always long ago; a wait that runs out shows at the next meeting)
     if (n >= 2) um_wait(&sm.pv_done[buf], ((n >> 1) - 1) & 1u, &sm.abort_flag, p.status);
     tc_fence_after_sync();
@@ -411,11 +416,11 @@ __device__ __forceinline__ bool qt_softmax(QtSmem<T, kD>& sm, const QtParams& p,
   // all sums are there
   if (tiles > 0 && qt_pair_any(1 + pair, !um_wait(&sm.pv_done[(tiles - 1) & 1], ((tiles - 1) >> 1) & 1u, &sm.abort_flag, p.status))) return false;
   tc_fence_after_sync();
-  if (half == 1) sm.red[r] = o.l;
+  if (half == 1) sm.red[r].x = o.l;
   qt_pair_any(1 + pair, false);
-  if (half == 0) sm.red[r] = o.l = o.l + sm.red[r];
+  if (half == 0) sm.red[r].x = o.l = o.l + sm.red[r].x;
   qt_pair_any(1 + pair, false);
-  o.l = sm.red[r];
+  o.l = sm.red[r].x;
   return true;
 }
 
@@ -567,11 +572,10 @@ __global__ void __launch_bounds__(kQtThreads, 1) quantized_prefill_umma_kernel(c
       // (the staged rows take the place of the queries, keys and values of all rows: every product has to be over)
       named_bar_sync(6, kQtSoftmax);
       if (alive) {
-        const float sums_log = o.m - o.v_first;  // what the row's sum is relative to
-        const float f = splits > 1 ? 1.f : o.l == 0.f ? 0.f : ex2_approx(o.v_first) / o.l;
+        const float f = splits > 1 ? 1.f : o.l == 0.f ? 0.f : ex2_approx(o.m - o.top) / o.l;
         const float back = flush ? ex2_approx(o.m_flushed - o.m) : 0.f;
         if (splits > 1 && half == 0) {
-          ml[r] = make_float2(sums_log, o.l);
+          ml[r] = make_float2(o.top, o.l);
           mv_of[r] = o.m;
         }
 #pragma unroll 1
@@ -684,7 +688,7 @@ static int launch_quantized_prefill_umma(QtParams p, int tiles, int most_tiles, 
   using L = QtSmem<T, kD>;
   constexpr int need = (int)sizeof(L) + 1024, bytes = need < 120 * 1024 ? 120 * 1024 : need;  // (one CTA per SM: all of its tensor memory)
   static_assert(need <= 232448, "shared memory of one CTA");
-  static_assert((int)sizeof(L) - (int)offsetof(L, k_full) <= 2048 && offsetof(L, k_full) >= kQtRows * (kD * 4 + 12), "tiles, and staged rows in their place");
+  static_assert((int)sizeof(L) - (int)offsetof(L, k_full) <= 3072 && offsetof(L, k_full) >= kQtRows * (kD * 4 + 12), "tiles, and staged rows in their place");
   auto* kernel = quantized_prefill_umma_kernel<T, kD>;
   static PerDeviceFlags ready, clusters[kQtMostSplits + 1];
   if (!once_per_device(ready, [&](int) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess; }))

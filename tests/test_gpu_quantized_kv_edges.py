@@ -133,3 +133,57 @@ def test_decode_of_tokens_that_do_not_see_the_loud_block(form, length):
     out = _attend(form, q, state, tables, lens, limits, MODEL, 1 / 16)
     for t, n in enumerate(limits[0]):
         _check(out[:, t: t + 1], q[:, t: t + 1], state, tables, [n], limits[:, t: t + 1], 1 / 16, TERM_BITS[form])
+
+
+# (shape and query type; few rows of few tokens, whose keys clusters of CTAs share, or tokens enough for a CTA per tile)
+TILES = [((32, 8, 128, 16), F16), ((16, 1, 256, 16), BF16), (MODEL, F32), ((16, 2, 64, 32), BF16), (MODEL, BF16)]  # (the last: pages and their tiles)
+
+
+@pytest.mark.parametrize("quiet,loud", [(-117, -8), (-117, 30), (-100, 60), (-60, 30)])
+@pytest.mark.parametrize("shape,dtype", TILES)
+@pytest.mark.parametrize("tokens", [3, 130])
+def test_prefill_over_blocks_whose_scales_lie_far_apart(tokens, shape, dtype, quiet, loud):
+    hq, hkv, d, bs = shape
+    rng = np.random.default_rng(53)
+    lens = [160 + 7 * i for i in range(len(PATTERNS))] + ([3000 + 11 * i for i in range(len(PATTERNS))] if tokens < 100 else [])
+    tables, state = _rows(rng, lens, shape)
+    for r, n in enumerate(lens):
+        blocks = -(-n // bs)
+        still = _quiet(PATTERNS[r % len(PATTERNS)], blocks)
+        state[1][1][tables[r, :blocks]] = np.where(still, 2.0 ** quiet, 2.0 ** loud)[:, None]
+        if quiet == -117:
+            state[1][0][tables[r, :blocks][still]] = 0
+    state[1][1][tables[0, :160 // bs], 0] = 2.0 ** -8  # (a head of its own: nothing far apart there)
+    q = torch.from_numpy(rng.standard_normal((len(lens), tokens, hq, d))).to(dtype).cuda()
+    limits = np.array(lens)[:, None] - tokens + 1 + np.arange(tokens)[None]
+    out = _attend("prefill", q, state, tables, lens, limits, shape, d ** -0.5)
+    _check(out, q, state, tables, lens, limits, d ** -0.5, 16 if shape == MODEL and dtype == BF16 else 22)
+
+
+@pytest.mark.parametrize("power", [-117, 100])
+@pytest.mark.parametrize("shape,dtype", TILES[:4])
+def test_prefill_over_values_of_extreme_scales(shape, dtype, power):
+    hq, hkv, d, bs = shape
+    rng = np.random.default_rng(54)
+    lens = [40, 2500, 300]
+    tables, state = _rows(rng, lens, shape)
+    state[1][1][:] = 2.0 ** power
+    q = torch.from_numpy(rng.standard_normal((3, 2, hq, d))).to(dtype).cuda()
+    limits = np.array(lens)[:, None] - 1 + np.arange(2)[None]
+    _check(_attend("prefill", q, state, tables, lens, limits, shape, d ** -0.5), q, state, tables, lens, limits, d ** -0.5, 22)
+
+
+@pytest.mark.parametrize("length", [96, 144, 5000 * 16])
+@pytest.mark.parametrize("shape,dtype", TILES[:3])
+def test_prefill_of_tokens_that_do_not_see_the_loud_block(shape, dtype, length):
+    hq, hkv, d, bs = shape
+    rng = np.random.default_rng(55)
+    lens = [length + bs]
+    tables, state = _rows(rng, lens, shape)
+    state[1][1][:] = 2.0 ** -100
+    state[1][1][tables[0, -1]] = 2.0 ** 60
+    q = torch.from_numpy(rng.standard_normal((1, 3, hq, d))).to(dtype).cuda()
+    limits = np.array([[length - 5, length, length + bs]])
+    out = _attend("prefill", q, state, tables, lens, limits, shape, d ** -0.5)
+    for t, n in enumerate(limits[0]):
+        _check(out[:, t: t + 1], q[:, t: t + 1], state, tables, [n], limits[:, t: t + 1], d ** -0.5, 22)
