@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(kQdThreads, qd_resident(kD, kTiles, kPack)) qu
       m[j][i] = mv[j][i] = kQdNone;
       l[j][i] = 0.f;
       limit[j][i] = len;
-      if (p.positions && at < columns) {
+      if (p.positions && at < columns && live) {  // (a row that is not ours may begin behind the last token)
         const int last = p.positions[token + at / p.groups];
         limit[j][i] = last < len ? last + 1 : len;
       }

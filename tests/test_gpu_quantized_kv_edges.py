@@ -187,3 +187,34 @@ def test_prefill_of_tokens_that_do_not_see_the_loud_block(shape, dtype, length):
     out = _attend("prefill", q, state, tables, lens, limits, shape, d ** -0.5)
     for t, n in enumerate(limits[0]):
         _check(out[:, t: t + 1], q[:, t: t + 1], state, tables, [n], limits[:, t: t + 1], d ** -0.5, 22)
+
+
+# ------------------------------------------------------------------------------------------------ packed batches
+
+def _packed(rng, rows, shape, dtype):
+    """Rows [(new, cached)] in a bucket without padding, as the call takes them, and what to check them with."""
+    hq, hkv, d, bs = shape
+    lens = [n + c for n, c in rows]
+    tables, state = _rows(rng, lens, shape)
+    total = sum(n for n, _ in rows)
+    q = torch.from_numpy(rng.standard_normal((1, total, hq, d))).to(dtype).cuda()
+    positions, qsl = np.concatenate([np.arange(c, c + n) for n, c in rows])[None], np.cumsum([0] + [n for n, _ in rows])
+    return q, tables, state, lens, positions, qsl
+
+
+@pytest.mark.parametrize("shape,dtype,cached", [((16, 2, 64, 32), F16, 60), (MODEL, BF16, 30), (MODEL, BF16, 2000), ((32, 8, 128, 16), F32, 900)])
+def test_rows_without_tokens_behind_a_full_bucket(shape, dtype, cached):
+    # (the batch is padded to its rows, not to its tokens: query_start_loc of the last rows is the bucket)
+    hq, hkv, d, bs = shape
+    rng = np.random.default_rng(58)
+    rows = [(1, cached + i) for i in range(40)] + [(0, 5)] + [(3, cached)] + [(1, 7)] + [(0, cached)] * 85
+    q, tables, state, lens, positions, qsl = _packed(rng, rows, shape, dtype)
+    around = _i32(np.concatenate([np.full(4, 1 << 30), positions[0], np.full(4, 1 << 30)]))  # nobody's numbers on either side
+    (k, ks), (v, vs) = (_gpu(*s) for s in state)
+    tokens = positions.shape[1]
+    out = _f64(Q.packed_paged_prefill_attention_quantized(q, k, v, ks, vs, _i32(tables), _i32(lens), around[4: 4 + tokens][None], _i32(qsl), bs, d ** -0.5,
+                                                          hq // hkv)).reshape(tokens, hq, d)
+    for r, (n, c) in enumerate(rows):
+        at = slice(qsl[r], qsl[r + 1])
+        if n:
+            _check(out[None, at], q[:, at], state, tables[r: r + 1], [lens[r]], [c + 1 + np.arange(n)], d ** -0.5, 16 if shape == MODEL and n > 1 else 20)
