@@ -475,7 +475,8 @@ int nvj_kv_append_quantized(const void* new_k, const void* new_v, int src_dtype,
  * Attention for rows of `width` query tokens over the 8-bit cache: q [rows, width, num_q_heads, head_dim] bf16, f16 or f32; token t of row b
  * attends keys p < seq_lens[b] and, with positions given ([rows, width]), p <= positions[b, t].  out as q, float32; a token that
  * sees no key gets zeros.  Meant for few query tokens per row; any width is taken.  query_start_loc given (width 1): q, positions and out are those of a packed batch, and
- * the rows that hold exactly one token are served, nothing else is written.  The scale may be any number.
+ * the rows that hold exactly one token are served, nothing else is written; the call is not told how many tokens those hold, so that all of
+ * query_start_loc has to lie within (nvj_paged_prefill_quantized knows its bucket).  The scale may be any number.
  * A length beyond the block table is flagged and clipped, a block id outside the pool flagged and its keys left out.
  *
  *   form       0 automatic, 1 mma.sync tiles on thread-block clusters (width * num_q_heads / num_kv_heads <= 16 columns per pass over a
@@ -494,7 +495,8 @@ int nvj_paged_decode_quantized(const void* q, int q_dtype, const void* k_cache_l
                                size_t workspace_bytes, int form, nvj_stream_t stream);
 
 /*
- * Ragged packed prefill attention over the 8-bit cache: masks, layout and padding as nvj_paged_prefill_packed.
+ * Ragged packed prefill attention over the 8-bit cache: masks, layout and padding as nvj_paged_prefill_packed.  Tokens that query_start_loc
+ * counts beyond the bucket are left out.
  *
  *   single_rows  0: no row holds a single query token; otherwise such rows, if there are any, are served by the decode kernel
  *   tile_pairs   as for nvj_paged_prefill_packed_counted (-1: not counted)

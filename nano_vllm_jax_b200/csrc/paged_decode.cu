@@ -317,7 +317,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) decode_pipelined_kernel(Dec
     mine += blocks_in_sequence(p, (len + kBlk - 1) / kBlk);
     // rows without keys get zeros; in a packed batch only the rows this pass owns (one query token) are touched
     const bool mine_to_zero = b < p.batch && len <= 0 && (b % grid) == (int)blockIdx.x &&
-                              (!p.packed_rows || p.query_start_loc[b + 1] - p.query_start_loc[b] == 1);
+                              (!p.packed_rows || packed_row_served(p, b));
     const unsigned idle = __ballot_sync(kFullMask, mine_to_zero);
     for (unsigned m = idle; m; m &= m - 1) {
       const int bb = base + (warp << 5) + (__ffs(m) - 1);

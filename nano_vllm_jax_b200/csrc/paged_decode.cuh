@@ -41,8 +41,8 @@ struct DecodeParams {
   const int32_t* query_start_loc;
   const int32_t* query_positions;
   int qsl_rows;
-  // packed_rows != 0 (pipelined kernel inside a packed batch): `batch` counts table rows; a row
-  // takes part only if it holds exactly one query token, i = query_start_loc[b]; it reads q[i],
+  // packed_rows != 0 (a kernel inside a packed batch of so many tokens): `batch` counts table rows; a row
+  // takes part only if it holds exactly one query token, i = query_start_loc[b], one of the batch's; it reads q[i],
   // writes out[i] and attends min(seq_lens[b], query_positions[i] + 1) keys.  Other rows are left
   // alone (no zero fill): the prefill kernel owns them.
   int packed_rows;
@@ -96,6 +96,12 @@ inline bool wide_takes_mma_sync(const DecodeParams& p) {
   return p.width <= 4 && (long long)p.batch * p.table_width > (p.width == 2 ? 4096 : 12288);
 }
 
+// Whether a packed batch's row b is this pass's: one query token, one of the batch's.
+__device__ __forceinline__ bool packed_row_served(const DecodeParams& p, int b) {
+  const int i = p.query_start_loc[b];
+  return p.query_start_loc[b + 1] - i == 1 && i >= 0 && i < p.packed_rows;
+}
+
 // Keys row b attends: seq_lens[b], clipped to what its page list can hold.  kWindow: the call may limit them further (a kernel
 // without a spare register pays 1% for code that a decode step never reaches).
 template <bool kWindow = true>
@@ -110,8 +116,8 @@ __device__ __forceinline__ int decode_row_len(const DecodeParams& p, int b) {
     }
   }
   if (p.packed_rows) {
+    if (!packed_row_served(p, b)) return 0;
     const int i = p.query_start_loc[b];
-    if (p.query_start_loc[b + 1] - i != 1) return 0;
     const int cap = p.query_positions[i] + 1;
     len = len < cap ? len : cap;
   }

@@ -171,7 +171,7 @@ __global__ void __launch_bounds__(kClThreads, 2) decode_cluster_kernel(DecodePar
   int ids = unit_id(lane);
   const int len = decode_row_len(p, b);  // the same in every thread of the cluster
   const long long qi = decode_query_index(p, b);
-  if (p.packed_rows && p.query_start_loc[b + 1] - p.query_start_loc[b] != 1) return;  // not this pass's row (the whole cluster leaves)
+  if (p.packed_rows && !packed_row_served(p, b)) return;  // not this pass's row (the whole cluster leaves)
   constexpr bool kFull = sizeof(T) == 4;
   const int d0 = lane * (kFull ? 4 : 8), d1 = kFull ? kD / 2 + lane * 4 : lane * 8 + 4;  // this lane's dims: four from each
   // query heads in slot order (slot h of a lane holds head h ^ hperm), times scale * log2(e)
@@ -447,7 +447,7 @@ __global__ void __launch_bounds__(kCmThreads, 3) decode_cluster_mma_kernel(Decod
   int ids = block_id(lane);
   const int len = decode_row_len(p, b);
   const long long qi = decode_query_index(p, b);
-  if (p.packed_rows && p.query_start_loc[b + 1] - p.query_start_loc[b] != 1) {  // not this pass's row (the whole cluster leaves)
+  if (p.packed_rows && !packed_row_served(p, b)) {  // not this pass's row (the whole cluster leaves)
     cl_end_beside(p);
     return;
   }

@@ -384,7 +384,7 @@ decode_stream_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
     mine += blocks_in_sequence(p, (len + kBlk - 1) / kBlk);
     // rows without keys get zeros; in a packed batch only the rows this pass owns (one query token) are touched
     const bool mine_to_zero = b < p.batch && len <= 0 && (b % grid) == (int)blockIdx.x &&
-                              (!p.packed_rows || p.query_start_loc[b + 1] - p.query_start_loc[b] == 1);
+                              (!p.packed_rows || packed_row_served(p, b));
     const unsigned idle = __ballot_sync(kFullMask, mine_to_zero);
     for (unsigned m = idle; m; m &= m - 1) {
       const int bb = base + (warp << 5) + (__ffs(m) - 1);

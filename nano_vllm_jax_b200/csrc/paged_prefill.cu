@@ -83,7 +83,7 @@ static int run_single_token_rows(const PackedArgs& a, int cta_limit, int32_t* be
   d.query_start_loc = a.query_start_loc;
   d.query_positions = a.positions;
   d.qsl_rows = a.rows;
-  d.packed_rows = 1;
+  d.packed_rows = a.token_bucket;
   d.out = a.out;
   d.num_blocks = a.num_blocks;
   d.table_width = a.table_width;

@@ -37,11 +37,11 @@ struct QDecodeParams {
   const int32_t* block_tables;
   const int32_t* seq_lens;
   const int32_t* positions;        // nullable: [rows, width], packed: per token
-  const int32_t* query_start_loc;  // packed: the rows of one query token are served, the others left alone
+  const int32_t* query_start_loc;  // packed: the rows of one query token, one of `tokens`, are served, the others left alone
   float* out;
   int32_t* status;
   long long num_blocks;
-  int rows, width, table_width, block_size, num_kv_heads, groups;
+  int rows, width, tokens, table_width, block_size, num_kv_heads, groups;
   int column_tiles;  // tiles of query columns of a row and kv head
   float scale_log2;  // scale * log2(e)
 };
@@ -100,7 +100,7 @@ __global__ void __launch_bounds__(kQdThreads, qd_resident(kD, kTiles, kPack)) qu
   if (p.query_start_loc) {
     token = p.query_start_loc[row];
     width = 1;
-    live = p.query_start_loc[row + 1] - token == 1;
+    live = p.query_start_loc[row + 1] - token == 1 && token >= 0 && token < p.tokens;
   }
   const int columns = width * p.groups;  // of the row and kv head: column c = (token c / groups, head c % groups)
   int len = p.seq_lens[row];
@@ -698,7 +698,7 @@ static int run_quantized_umma(const QDecodeParams& q, int q_dtype, int head_dim,
   p.seq_lens = q.seq_lens;
   p.query_start_loc = q.query_start_loc;
   p.query_positions = q.positions;
-  p.packed_rows = q.query_start_loc != nullptr;
+  p.packed_rows = q.query_start_loc ? q.tokens : 0;
   p.status = q.status;
   p.num_blocks = q.num_blocks;
   p.batch = q.rows;
@@ -735,13 +735,13 @@ extern "C" size_t nvj_paged_decode_quantized_workspace_bytes(int rows, int width
   return qu_plan(width * groups, num_kv_heads, head_dim, sms).bytes();
 }
 
-extern "C" int nvj_paged_decode_quantized(const void* q, int q_dtype, const void* k_cache_layer, const void* v_cache_layer,
-                                          const float* k_scale, const float* v_scale, int64_t num_blocks, int block_size,
-                                          int num_kv_heads, int head_dim, int num_q_heads, const int32_t* block_tables, int table_width,
-                                          const int32_t* seq_lens, const int32_t* positions, const int32_t* query_start_loc, int rows,
-                                          int width, float scale, float* out, int32_t* status, void* workspace,
-                                          size_t workspace_bytes, int form, nvj_stream_t stream) {
-  using namespace nvj;
+namespace nvj {
+// `tokens`: how many a packed batch's q, positions and out hold; rows whose token lies elsewhere are not served.
+int paged_decode_quantized(const void* q, int q_dtype, const void* k_cache_layer, const void* v_cache_layer, const float* k_scale, const float* v_scale,
+                           int64_t num_blocks, int block_size, int num_kv_heads, int head_dim, int num_q_heads, const int32_t* block_tables,
+                           int table_width, const int32_t* seq_lens, const int32_t* positions, const int32_t* query_start_loc, int rows, int width,
+                           int tokens, float scale, float* out, int32_t* status, void* workspace, size_t workspace_bytes, int form,
+                           nvj_stream_t stream) {
   if (form < 0 || form > 2) return NVJ_ERR_INVALID_ARGUMENT;
   if (rows < 0 || width < 0 || table_width < 0 || num_blocks < 0) return NVJ_ERR_INVALID_ARGUMENT;
   if (q_dtype < NVJ_BF16 || q_dtype > NVJ_F32 || !quantized_cache_shape_ok(block_size, num_kv_heads, head_dim)) return NVJ_ERR_UNSUPPORTED;
@@ -768,6 +768,7 @@ extern "C" int nvj_paged_decode_quantized(const void* q, int q_dtype, const void
   p.num_blocks = num_blocks;
   p.rows = rows;
   p.width = width;
+  p.tokens = tokens;
   p.table_width = table_width;
   p.block_size = block_size;
   p.num_kv_heads = num_kv_heads;
@@ -781,4 +782,16 @@ extern "C" int nvj_paged_decode_quantized(const void* q, int q_dtype, const void
   if (q_dtype == NVJ_BF16) return launch_quantized_decode_dims<__nv_bfloat16>(p, head_dim, s);
   if (q_dtype == NVJ_F16) return launch_quantized_decode_dims<__half>(p, head_dim, s);
   return launch_quantized_decode_dims<float>(p, head_dim, s);
+}
+}  // namespace nvj
+
+extern "C" int nvj_paged_decode_quantized(const void* q, int q_dtype, const void* k_cache_layer, const void* v_cache_layer,
+                                          const float* k_scale, const float* v_scale, int64_t num_blocks, int block_size,
+                                          int num_kv_heads, int head_dim, int num_q_heads, const int32_t* block_tables, int table_width,
+                                          const int32_t* seq_lens, const int32_t* positions, const int32_t* query_start_loc, int rows,
+                                          int width, float scale, float* out, int32_t* status, void* workspace,
+                                          size_t workspace_bytes, int form, nvj_stream_t stream) {
+  return nvj::paged_decode_quantized(q, q_dtype, k_cache_layer, v_cache_layer, k_scale, v_scale, num_blocks, block_size, num_kv_heads, head_dim,
+                                     num_q_heads, block_tables, table_width, seq_lens, positions, query_start_loc, rows, width, 0x7fffffff, scale, out,
+                                     status, workspace, workspace_bytes, form, stream);
 }

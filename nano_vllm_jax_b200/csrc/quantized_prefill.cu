@@ -17,6 +17,12 @@ int prefill_over_pages(const void* q, const void* k_pages, const void* v_pages, 
                        const int32_t* kv_lens, const int32_t* positions, const int32_t* query_start_loc, int rows, int token_bucket, float scale,
                        float* out, int32_t* status, void* workspace, size_t workspace_bytes, int part, int tile_pairs, cudaStream_t stream);
 
+int paged_decode_quantized(const void* q, int q_dtype, const void* k_cache_layer, const void* v_cache_layer, const float* k_scale, const float* v_scale,
+                           int64_t num_blocks, int block_size, int num_kv_heads, int head_dim, int num_q_heads, const int32_t* block_tables,
+                           int table_width, const int32_t* seq_lens, const int32_t* positions, const int32_t* query_start_loc, int rows, int width,
+                           int tokens, float scale, float* out, int32_t* status, void* workspace, size_t workspace_bytes, int form,
+                           nvj_stream_t stream);
+
 // ---- pages of a scratch bf16 cache ----------------------------------------------------------------------------------------------
 struct QUnpackParams {
   const uint8_t* k_cache;
@@ -151,9 +157,9 @@ extern "C" int nvj_paged_prefill_quantized(const void* q, int q_dtype, const voi
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int skip_single = single_rows != 0;
   if (skip_single && rows > 0) {
-    const int rc = nvj_paged_decode_quantized(q, q_dtype, k_cache_layer, v_cache_layer, k_scale, v_scale, num_blocks, block_size, num_kv_heads,
-                                              head_dim, num_q_heads, block_tables, table_width, kv_lens, positions, query_start_loc, rows, 1,
-                                              scale, out, status, workspace, workspace_bytes, 0, stream);
+    const int rc = paged_decode_quantized(q, q_dtype, k_cache_layer, v_cache_layer, k_scale, v_scale, num_blocks, block_size, num_kv_heads, head_dim,
+                                          num_q_heads, block_tables, table_width, kv_lens, positions, query_start_loc, rows, 1, token_bucket, scale, out,
+                                          status, workspace, workspace_bytes, 0, stream);
     if (rc != NVJ_OK) return rc;
   }
   const size_t needed = quantized_page_bytes(q_dtype, rows, table_width, block_size, num_kv_heads, head_dim, num_q_heads, scale);

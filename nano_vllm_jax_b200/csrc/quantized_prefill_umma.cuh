@@ -461,8 +461,10 @@ __global__ void __launch_bounds__(kQtThreads, 1) quantized_prefill_umma_kernel(c
   const int tile_at = (int)blockIdx.x / splits;
   if (warp == 0) {
     auto tiles_of = [&](int r) {
-      const int n = p.query_start_loc[r + 1] - p.query_start_loc[r];
-      return n <= 0 || (p.skip_single && n == 1) ? 0 : (int)(((long long)n * p.groups + kQtRows - 1) / kQtRows);
+      const int from = p.query_start_loc[r], to = p.query_start_loc[r + 1];
+      if (from < 0 || (p.skip_single && to - from == 1)) return 0;
+      const int n = min(to, p.token_bucket) - from;
+      return n <= 0 ? 0 : (int)(((long long)n * p.groups + kQtRows - 1) / kQtRows);
     };
     const int first_tiles = lane < p.rows ? tiles_of(lane) : 0;
     int total = first_tiles;

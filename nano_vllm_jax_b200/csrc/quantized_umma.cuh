@@ -814,7 +814,7 @@ quantized_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
     }
     mine += n;
     const bool ours = b < p.batch && len <= 0 && b % ranges == range &&
-                      (!p.query_start_loc || p.query_start_loc[b + 1] - p.query_start_loc[b] == 1);
+                      (!p.packed_rows || packed_row_served(p, b));
     for (unsigned todo = __ballot_sync(kFullMask, ours); todo; todo &= todo - 1) {
       const int bb = base + (warp << 5) + (__ffs(todo) - 1);
       const long long token = a.query_start_loc ? (long long)a.query_start_loc[bb] : (long long)bb * a.width;

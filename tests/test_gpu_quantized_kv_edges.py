@@ -218,3 +218,78 @@ def test_rows_without_tokens_behind_a_full_bucket(shape, dtype, cached):
         at = slice(qsl[r], qsl[r + 1])
         if n:
             _check(out[None, at], q[:, at], state, tables[r: r + 1], [lens[r]], [c + 1 + np.arange(n)], d ** -0.5, 16 if shape == MODEL and n > 1 else 20)
+
+
+# A bucket that is too small for its rows, as a layout that was flagged hands it on: tokens beyond it are neither read nor written.  The arrays of the
+# call lie inside larger ones, so that the test sees what lands behind them.
+def _too_small(call, q, positions, qsl, bucket, out_shape):
+    (tokens, hq, d) = q.shape
+    out = torch.full((tokens, hq, d), 7.0, device="cuda")
+    call(q[:bucket][None], _i32(positions)[:bucket][None], _i32(qsl), out[:bucket])
+    torch.cuda.synchronize()
+    assert bool((out[bucket:] == 7.0).all())
+    return _f64(out[:bucket])
+
+
+@pytest.mark.parametrize("shape,dtype,cached", [((16, 2, 64, 32), F16, 60), (MODEL, BF16, 30), (MODEL, BF16, 2000), ((32, 8, 128, 16), F32, 900)])
+@pytest.mark.parametrize("rows,bucket", [([(1, 1)] * 30, 20), ([(1, 1)] * 9 + [(70, 3)] + [(1, 1)] * 9, 50), ([(200, 0), (1, 5), (1, 5)], 200), ([(5, 9)] * 7, 8)])
+def test_tokens_beyond_the_bucket_are_left_out(shape, dtype, cached, rows, bucket):
+    from nano_vllm_jax_b200 import _lib
+    hq, hkv, d, bs = shape
+    rng = np.random.default_rng(59)
+    rows = [(n, c * cached) for n, c in rows]
+    q, tables, state, lens, positions, qsl = _packed(rng, rows, shape, dtype)
+    (k, ks), (v, vs) = (_gpu(*s) for s in state)
+    t, l, lib = _i32(tables), _i32(lens), _lib.load()
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+
+    def call(q, positions, qsl, out):
+        args = (K._dt(q), len(rows), tables.shape[1], bs, hkv, d, hq, d ** -0.5, -1, bucket, -1)
+        scratch = torch.empty(lib.nvj_paged_prefill_quantized_workspace_bytes(*args), dtype=torch.uint8, device="cuda")
+        _lib.check(lib.nvj_paged_prefill_quantized(
+            q.data_ptr(), K._dt(q), k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), k.shape[0], bs, hkv, d, hq, t.data_ptr(), tables.shape[1],
+            l.data_ptr(), positions.data_ptr(), qsl.data_ptr(), len(rows), bucket, d ** -0.5, out.data_ptr(), status.data_ptr(), scratch.data_ptr(),
+            scratch.numel(), -1, -1, torch.cuda.current_stream().cuda_stream), "prefill")
+
+    out = _too_small(call, q[0], positions[0], qsl, bucket, q.shape[1:])
+    for r, (n, c) in enumerate(rows):
+        at = slice(min(qsl[r], bucket), min(qsl[r + 1], bucket))
+        if at.stop > at.start:
+            _check(out[None, at], q[:, at], state, tables[r: r + 1], [lens[r]], [c + 1 + np.arange(at.stop - at.start)], d ** -0.5, 16 if shape == MODEL else 20)
+
+
+@pytest.mark.parametrize("cached", [30, 3000])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_tokens_beyond_the_bucket_of_a_bf16_cache_are_left_out(dtype, cached):
+    from nano_vllm_jax_b200 import _lib
+    hq, hkv, d, bs = MODEL
+    rng = np.random.default_rng(60)
+    lib = _lib.load()
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for rows, bucket in (([(1, cached)] * 30, 20), ([(1, cached)] * 9 + [(70, 3)] + [(1, cached)] * 9, 50), ([(1, cached)] * 300, 280)):
+        lens = [n + c for n, c in rows]
+        width = -(-max(lens) // bs)
+        tables = rng.integers(0, 200, (len(rows), width))  # (rows share blocks)
+        k, v = (torch.from_numpy(rng.standard_normal((200, bs, hkv, d))).to(BF16).cuda() for _ in range(2))
+        total = sum(n for n, _ in rows)
+        q = torch.from_numpy(rng.standard_normal((total, hq, d))).to(dtype).cuda()
+        positions, qsl = np.concatenate([np.arange(c, c + n) for n, c in rows]), np.cumsum([0] + [n for n, _ in rows])
+        t, l = _i32(tables), _i32(lens)
+        scratch = K._workspace(q.device, len(rows)).buf
+
+        def call(q, positions, qsl, out):
+            _lib.check(lib.nvj_paged_prefill_packed(
+                q.data_ptr(), K._dt(q), k.data_ptr(), v.data_ptr(), K._dt(k), k.shape[0], bs, hkv, d, hq, t.data_ptr(), width, l.data_ptr(), positions.data_ptr(),
+                qsl.data_ptr(), len(rows), bucket, d ** -0.5, out.data_ptr(), status.data_ptr(), scratch.data_ptr(), scratch.numel(), 0,
+                torch.cuda.current_stream().cuda_stream), "prefill")
+
+        out = _too_small(call, q, positions, qsl, bucket, q.shape[1:])
+        kk, vv = _f64(k), _f64(v)
+        for r in sorted({0, 3, len(rows) // 2, len(rows) - 1}):
+            n, c = rows[r]
+            at = slice(min(qsl[r], bucket), min(qsl[r + 1], bucket))
+            if at.stop > at.start:
+                x, y = (a[tables[r]].reshape(-1, hkv, d)[:lens[r]] for a in (kk, vv))
+                seen = np.arange(lens[r])[None] < c + 1 + np.arange(at.stop - at.start)[:, None]
+                want = R.attend(_f64(q[at]), x, y, seen, d ** -0.5)
+                assert np.abs(out[at] - want).max() <= R.tolerance(_f64(q[at]), x, y, d ** -0.5, 8), r  # (weights rounded to bf16)
