@@ -44,6 +44,9 @@ namespace nvj {
 constexpr int kQuTile = 128;    // keys per tile
 constexpr int kQuUnits = 8;     // boxes per tile, at most: a box is a unit of 16, 32 or 64 keys of one block (QuParams::unit)
 constexpr int kQuPTerms = 5;
+// Named barriers (0 is __syncthreads'): a softmax group's, from this one on; all groups'; everybody's but the producer's.  None has two meanings: after a
+// wait that ran out a group may meet the others where another one still votes, with another number of threads.
+constexpr int kQuBarGroup = 1, kQuBarAll = 4, kQuBarQueries = 5;
 // The reference of a column's weights is set 2^3 below its largest weight and moved when one would pass 2^8 (e4m3 ends at 448).
 constexpr float kQuNone = -3e38f, kQuSlack = 8.f, kQuLift = 3.f;
 // V scales reach from 2^-117 (the append's for a block of zeros) to 2^119.  A sum of weights is of exp2(score - (reference - v_top)), v_top the
@@ -80,6 +83,7 @@ struct QuLayout {
   static constexpr int kFit = (232448 - 1024 - 6144 - 2 * kQBytes - 2 * kWBytes) / kTileBytes;
   static constexpr int kSlots = kFit < 160 * 1024 / kTileBytes ? kFit : 160 * 1024 / kTileBytes;
   static constexpr int kKSlots = kSlots / 2, kVSlots = kSlots - kKSlots;  // a ring of tiles of K, one of V (which waits for its weights)
+  static_assert(kQuBarGroup + kGroups <= kQuBarAll && kQuBarAll != kQuBarQueries, "a barrier of its own for every meeting");
   static_assert(kNO <= 128 && kNS <= 256, "a row of weights is 128 bytes");
   static_assert(kColO + kSets * kChunks * kNO <= 512, "tensor memory");
   static_assert(kKSlots >= 1 && kVSlots >= 2, "the rings");
@@ -397,10 +401,10 @@ __device__ __forceinline__ void qu_softmax_warps(QuSmem<L>& sm, const QuParams& 
   constexpr int kSRead = (L::kSRegion + 7) / 8, kORead = (kQuPTerms * kCg + 7) / 8;  // pieces of 8 columns
   constexpr bool kByTiles = L::kByTiles;
   constexpr int kDim = L::kChunks * 128, kWords = L::kORegion / 4;
-  const int key = warp * 32 + lane, region = kByTiles ? 0 : group, first_col = kByTiles ? 0 : group * kCg, bar = 1 + group;
+  const int key = warp * 32 + lane, region = kByTiles ? 0 : group, first_col = kByTiles ? 0 : group * kCg, bar = kQuBarGroup + group;
   tmem += (uint32_t)(warp * 32) << 16;
   // a group that leaves early meets the other one, which waits at a segment's end or leaves as well
-  auto give_up = [] { qu_meet_any<L::kSoftmaxThreads>(3, true); };
+  auto give_up = [] { qu_meet_any<L::kSoftmaxThreads>(kQuBarAll, true); };
   QuRing<L::kVSlots> at;  // V's slot of the tile at hand
   QuSeg s;
   const int per = kQuTile / a.unit, my_unit = key >> a.unit_log2;
@@ -594,7 +598,7 @@ __device__ __forceinline__ void qu_softmax_warps(QuSmem<L>& sm, const QuParams& 
         sm.m[group][c] = m[c] > kQuNone ? m[c] - v_top : kQuNone;
       }
     }
-    if (qu_meet_any<L::kSoftmaxThreads>(3, !um_wait(&sm.o_full, seg & 1u, &sm.abort_flag, p.status))) return;
+    if (qu_meet_any<L::kSoftmaxThreads>(kQuBarAll, !um_wait(&sm.o_full, seg & 1u, &sm.abort_flag, p.status))) return;
     const bool final_row = s.whole();
     const long long slot = (long long)partial_slot(range, s.j0 == 0) * a.hcts + hct;
     const int tid = group * 128 + key;
@@ -614,7 +618,7 @@ __device__ __forceinline__ void qu_softmax_warps(QuSmem<L>& sm, const QuParams& 
         if (!final_row) *reinterpret_cast<float2*>(a.part_ml + (slot * L::kC + tid) * 2) = make_float2(sm.m[g][c], sum);
       }
     }
-    qu_meet_any<L::kSoftmaxThreads>(3, false);
+    qu_meet_any<L::kSoftmaxThreads>(kQuBarAll, false);
     tc_fence_after_sync();
     const int columns = min(a.columns - ct * L::kC, L::kC);
     const long long token = a.query_start_loc ? (long long)a.query_start_loc[s.b] : (long long)s.b * a.width;
@@ -879,7 +883,7 @@ quantized_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
       fence_proxy_async_smem();
     }
     tc_fence_before_sync();
-    named_bar_sync(4, kThreads - 32);
+    named_bar_sync(kQuBarQueries, kThreads - 32);
     tc_fence_after_sync();
     const uint32_t tmem = sm.tmem_base;
 

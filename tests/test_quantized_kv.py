@@ -141,3 +141,18 @@ def test_the_reference_rounds_as_the_format_does():
                                            (3.38e38, 2.0 ** 119), (1.0, 2.0 ** -8)])
 def test_scales_of_the_reference(largest, scale):
     assert R.scale_for(largest) == scale
+
+
+def test_every_named_barrier_of_the_tcgen05_decode_kernel_has_one_meaning():
+    # three groups of 128 threads with a barrier each, one of all groups, one of all warps but the producer's: a barrier that two of them used, with
+    # different numbers of threads, would hang after a wait that ran out
+    import re
+    from pathlib import Path
+    text = re.sub(r"//[^\n]*", "", (Path(Q.__file__).parents[1] / "csrc" / "quantized_umma.cuh").read_text())
+    ids = {name: int(n) for name, n in re.findall(r"\b(kQuBar\w+) = (\d+)", text)}
+    groups = max(int(n) for n in re.findall(r"launch_quantized_umma<T, kDim, \d+, (\d+)>", text))
+    used = [ids["kQuBarGroup"] + g for g in range(max(groups, 2))] + [ids["kQuBarAll"], ids["kQuBarQueries"]]
+    assert len(set(used)) == len(used) and 0 not in used and max(used) < 16
+    meetings = set(re.findall(r"qu_meet_any<([^>]*)>\((\w+),", text)) | set(re.findall(r"(named_bar_sync)\((\w+),", text))
+    assert meetings == {("128", "bar"), ("L::kSoftmaxThreads", "kQuBarAll"), ("named_bar_sync", "kQuBarQueries")}
+    assert re.search(r"\bbar = kQuBarGroup \+ group;", text)
