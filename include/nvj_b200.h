@@ -474,7 +474,7 @@ int nvj_kv_append_quantized(const void* new_k, const void* new_v, int src_dtype,
 /*
  * Attention for rows of `width` query tokens over the 8-bit cache: q [rows, width, num_q_heads, head_dim] bf16, f16 or f32; token t of row b
  * attends keys p < seq_lens[b] and, with positions given ([rows, width]), p <= positions[b, t].  out as q, float32; a token that
- * sees no key gets zeros.  Meant for few query tokens per row; any width is taken.  query_start_loc given (width 1): q, positions and out are those of a packed batch, and
+ * sees no key gets zeros.  Keys that no token of a row sees may hold anything, NaN included.  Meant for few query tokens per row; any width is taken.  query_start_loc given (width 1): q, positions and out are those of a packed batch, and
  * the rows that hold exactly one token are served, nothing else is written; the call is not told how many tokens those hold, so that all of
  * query_start_loc has to lie within (nvj_paged_prefill_quantized knows its bucket).  The scale may be any number.
  * A length beyond the block table is flagged and clipped, a block id outside the pool flagged and its keys left out.

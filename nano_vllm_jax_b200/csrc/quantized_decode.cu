@@ -123,11 +123,18 @@ __global__ void __launch_bounds__(kQdThreads, qd_resident(kD, kTiles, kPack)) qu
     }
   };
   fetch_next_ids(tile);
+  int last = 0x7fffffff;  // position of the last key that a token of the row sees
+  if (p.positions && live) {
+    last = lane < width ? p.positions[token + lane] : -1;
+    for (int i = lane + 32; i < width; i += 32) last = max(last, p.positions[token + i]);
+    last = __reduce_max_sync(kFullMask, last);
+  }
   if (!live) len = 0;
   if (len > p.table_width * (long long)p.block_size) {
     if (threadIdx.x == 0 && rank == 0) atomicOr(p.status, NVJ_DEV_BAD_LENGTH);
     len = p.table_width * p.block_size;
   }
+  len = min(len - 1, last) + 1;  // (keys that none of them sees may hold anything, as those behind the row's last one)
   const int tiles = (len + 15) >> 4;
   float ks = 0.f, lv = 0.f;  // scales of this lane's tile: of K, and log2 of V's
   auto fetch_scales = [&](int first) {

@@ -31,25 +31,38 @@ struct QUnpackParams {
   const float* v_scale;
   const int32_t* block_tables;
   const int32_t* kv_lens;
+  const int32_t* positions;
   const int32_t* query_start_loc;
   char* k_pages;  // page row * table_width + b: block b of the row
   char* v_pages;
   int32_t* page_tables;
   int32_t* status;
   long long num_blocks;
-  int rows, table_width, skip_single;
+  int rows, table_width, skip_single, token_bucket;
 };
 
 // Grid (x: blocks of a row in strides, y: rows); the model's shape, 16 tokens of 2 heads of 256: a thread four pieces of 16 numbers, two of K and two
 // of V, of one head.  The block's id is asked for together with the row's length: two trips to memory in a row.  A block whose id is outside
-// the pool becomes a page of zeros, as the other kernels take it, and so do the rows behind the last key, which hold anything.
+// the pool becomes a page of zeros, as the other kernels take it, and so do the rows behind the last key that a token sees, which hold anything.
 __global__ void __launch_bounds__(256) quantized_unpack_kernel(QUnpackParams p) {
   constexpr int kRow = 512, kBlock = 16 * kRow;  // bytes of a token, and of a block
   pdl_wait();
   pdl_release();
   const int row = blockIdx.y;
-  const int len = p.kv_lens[row], from = p.query_start_loc[row], to = p.query_start_loc[row + 1];
-  const bool skip = to <= from || (p.skip_single && to - from == 1);
+  const int len = p.kv_lens[row], from = p.query_start_loc[row], end = p.query_start_loc[row + 1], to = end < p.token_bucket ? end : p.token_bucket;
+  const bool skip = to <= from || from < 0 || (p.skip_single && end - from == 1);
+  // Keys that a token sees: all of the row's where its last token stands at their end, as nearly always; else the tokens are looked at.
+  int seen = len;
+  if (!skip && p.positions[to - 1] + 1 < len) {
+    __shared__ int most;
+    if (threadIdx.x == 0) most = 0;
+    __syncthreads();
+    int mine = 0;
+    for (int i = from + threadIdx.x; i < to; i += 256) mine = max(mine, p.positions[i] < len ? p.positions[i] + 1 : len);
+    atomicMax(&most, __reduce_max_sync(kFullMask, mine));
+    __syncthreads();
+    seen = most;
+  }
   const int head = (threadIdx.x * 16 % kRow) / 256, token = threadIdx.x * 16 / kRow;  // of the first piece; the second is eight tokens on
   for (int b = blockIdx.x; b < p.table_width; b += gridDim.x) {
     const long long page = (long long)row * p.table_width + b;
@@ -60,6 +73,7 @@ __global__ void __launch_bounds__(256) quantized_unpack_kernel(QUnpackParams p) 
     const bool ok = id >= 0 && id < p.num_blocks;
     if (!ok && threadIdx.x == 0) atomicOr(p.status, NVJ_DEV_BAD_BLOCK_ID);
     uint4 w[4];
+    const int left_seen = seen - b * 16;
     float unit[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -73,6 +87,7 @@ __global__ void __launch_bounds__(256) quantized_unpack_kernel(QUnpackParams p) 
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
+      if (token + 8 * (i & 1) >= left_seen) w[i] = make_uint4(0, 0, 0, 0);
       const uint32_t in[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
       const float u = unit[i >> 1];
       uint32_t out[8];
@@ -172,6 +187,7 @@ extern "C" int nvj_paged_prefill_quantized(const void* q, int q_dtype, const voi
     u.v_scale = v_scale;
     u.block_tables = block_tables;
     u.kv_lens = kv_lens;
+    u.positions = positions;
     u.query_start_loc = query_start_loc;
     u.k_pages = static_cast<char*>(workspace);
     u.v_pages = u.k_pages + pages * page_bytes;
@@ -181,6 +197,7 @@ extern "C" int nvj_paged_prefill_quantized(const void* q, int q_dtype, const voi
     u.rows = rows;
     u.table_width = table_width;
     u.skip_single = skip_single;
+    u.token_bucket = token_bucket;
     const int across = (148 * 8 + rows - 1) / rows;
     if (launch_after(quantized_unpack_kernel, dim3(across < table_width ? across : table_width, rows), dim3(256), 0, s, u) != cudaSuccess)
       return NVJ_ERR_LAUNCH;

@@ -542,7 +542,8 @@ __global__ void __launch_bounds__(kQtThreads, 1) quantized_prefill_umma_kernel(c
     if (lane == 0) atomicMax(&sm.most, most);
   }
   __syncthreads();
-  const int all_tiles = (sm.most + kQtKeys - 1) / kQtKeys;
+  len = sm.most;  // (keys that none of the rows sees may hold anything, as those behind the table row's last one)
+  const int all_tiles = (len + kQtKeys - 1) / kQtKeys;
   const int parts = splits == 1 ? 1 : min(splits, max(1, all_tiles / kQtSplitTiles));
   const int tile0 = rank < parts ? (int)((long long)all_tiles * rank / parts) : 0;
   const int tiles = rank < parts ? (int)((long long)all_tiles * (rank + 1) / parts) - tile0 : 0;

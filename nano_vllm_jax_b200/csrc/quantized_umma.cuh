@@ -99,6 +99,7 @@ struct QuSmem {
   alignas(16) float k_unit[8][kQuUnits], v_unit[8][kQuUnits];  // by tile: the scales of its units' blocks; V's -1: no such block
   alignas(16) float factor[4][L::kC];  // by segment: what a column's products are multiplied by, and the keys it may see
   alignas(16) int limit[4][L::kC];
+  int seen[4];  // by segment: the largest limit, hence the keys that any column sees
   alignas(16) float red[L::kGroups][4][8];  // per group and warp
   float red_v[L::kGroups][4];
   float m[L::kGroups][8], mv[L::kGroups][8];  // at the end: references of the sum of the weights, and of the weighted sums
@@ -570,10 +571,11 @@ __device__ __forceinline__ void qu_softmax_warps(QuSmem<L>& sm, const QuParams& 
             qu_sts2(w_row + ((((piece + i) >> 1) ^ (key & 7)) << 4) + ((piece + i) & 1) * 8, bytes[2 * i], bytes[2 * i + 1]);
         }
       }
-      // V rows of keys that are not there weigh nothing, but may hold anything: 0 x NaN is not 0
-      if (t == nt - 1 && (kByTiles || group == 0) && ((cnt * a.unit & 31) || (s.j0 + s.n == s.nb && (s.len & (a.unit - 1))))) {
+      // V rows of keys that are not there, or that no column sees, weigh nothing, but may hold anything: 0 x NaN is not 0
+      const int seen = sm.seen[seg & 3u];
+      if ((kByTiles || group == 0) && ((cnt * a.unit & 31) || (s.j0 + t * per + cnt) * a.unit > seen)) {
         if (qu_meet_any<128>(bar, !um_wait(&sm.v_full[at.at], at.phase, &sm.abort_flag, p.status))) return give_up();
-        if (key < (cnt * a.unit + 31) / 32 * 32 && (at_key == 0x7fffffff || at_key >= s.len)) {
+        if (key < (cnt * a.unit + 31) / 32 * 32 && at_key >= seen) {
           const uint32_t v_row = smem_u32(sm.v[at.at]) + (key >> 3) * (8 * kDim) + (key & 7) * 128;
 #pragma unroll
           for (int i = 0; i < kDim / 16; ++i) qu_sts4(v_row + (i >> 3) * 1024 + (i & 7) * 16, 0u, 0u, 0u, 0u);
@@ -741,6 +743,7 @@ __device__ __forceinline__ void qu_query_warp(QuSmem<L>& sm, const QuParams& a, 
       Column column[kAhead];
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) column[i].load(sm, a, s, token, ct, i * Column::kCount, lane);
+      int seen = 0;
       // the scores of the segment two before have been computed
       if (seg > 1 && !um_wait(&sm.q_free[seg & 1u], ((seg >> 1) - 1) & 1u, &sm.abort_flag, p.status)) return;
 #pragma unroll 1
@@ -748,9 +751,12 @@ __device__ __forceinline__ void qu_query_warp(QuSmem<L>& sm, const QuParams& a, 
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
           column[i].template store<kCg>(sm, a, seg, c + i * Column::kCount, lane);
+          seen = max(seen, column[i].limit);
           if (c + kAll < L::kC) column[i].load(sm, a, s, token, ct, c + kAll + i * Column::kCount, lane);
         }
       }
+      seen = __reduce_max_sync(kFullMask, seen);
+      if (lane == 0) sm.seen[seg & 3u] = seen;
       fence_proxy_async_smem();
     }
     mbar_arrive(smem_u32(&sm.q_full[seg & 1u]));
@@ -771,7 +777,7 @@ quantized_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
   if (threadIdx.x == 0) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&k_map)) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&v_map)) : "memory");
-    sm.start_b = p.batch; sm.start_j = 0; sm.lens_from = 0; sm.abort_flag = 0;
+    sm.start_b = p.batch; sm.start_j = 0; sm.lens_from = 0; sm.abort_flag = 0; sm.seen[0] = 0;
     for (int i = 0; i < L::kKSlots; ++i) {
       mbar_init(smem_u32(&sm.k_full[i]), 1);
       mbar_init(smem_u32(&sm.k_empty[i]), 1);
@@ -879,6 +885,8 @@ quantized_umma_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_co
         QuColumn<L, T> column;
         column.load(sm, a, s, token, ct, c, lane);
         column.template store<kCg>(sm, a, 0u, c, lane);
+        const int seen = __reduce_max_sync(kFullMask, column.limit);
+        if (lane == 0) atomicMax(&sm.seen[0], seen);
       }
       fence_proxy_async_smem();
     }

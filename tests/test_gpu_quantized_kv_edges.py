@@ -189,6 +189,28 @@ def test_prefill_of_tokens_that_do_not_see_the_loud_block(shape, dtype, length):
         _check(out[:, t: t + 1], q[:, t: t + 1], state, tables, [n], limits[:, t: t + 1], d ** -0.5, 22)
 
 
+# ------------------------------------------------------------------------------------------------ masks and tables
+
+@pytest.mark.parametrize("route,shape,dtype", [(1, MODEL, BF16), (1, (6, 6, 64, 48), F32), (2, MODEL, BF16), (2, (32, 8, 128, 32), F16)] + [("prefill", *t) for t in TILES])
+def test_keys_that_no_token_of_the_row_sees_may_hold_anything(route, shape, dtype):
+    hq, hkv, d, bs = shape
+    rng = np.random.default_rng(56)
+    lens = [200, 64, 1000, 90]
+    seen = [[130, 131], [0, 0], [990, 700], [65, 64]]  # keys that a row's two tokens see
+    tables, state = _rows(rng, lens, shape)
+    for codes, _ in state:
+        for r, limits in enumerate(seen):
+            for key in range(max(limits), lens[r]):
+                codes[tables[r, key // bs], key % bs] = 127
+    q = torch.from_numpy(rng.standard_normal((4, 2, hq, d))).to(dtype).cuda()
+    out = _attend(route, q, state, tables, lens, np.array(seen), shape, d ** -0.5)
+    assert not out[1].any()
+    if route != "prefill":  # (a decode row may as well name the largest position there is)
+        free = _attend(route, q[3:], state, tables[3:], [64], np.full((1, 2), 1 << 31), shape, d ** -0.5)
+        _check(free, q[3:], state, tables[3:], [64], np.full((1, 2), 64), d ** -0.5, TERM_BITS[route])
+    _check(out, q, state, tables, [max(s) for s in seen], np.array(seen), d ** -0.5, 16 if route == "prefill" and shape == MODEL and dtype == BF16 else TERM_BITS[route])
+
+
 # ------------------------------------------------------------------------------------------------ packed batches
 
 def _packed(rng, rows, shape, dtype):
