@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(kLayoutThreads) packed_layout_kernel(LayoutPar
   __syncthreads();
   const int total = qsl[p.rows], blocks = first[p.rows];
   const long long threads = (long long)gridDim.x * kLayoutThreads, me = (long long)blockIdx.x * kLayoutThreads + tid;
-  // An id from the list, -1 past its end (a slot or table entry that the kernels downstream flag and skip).
+  // An id from the list, -1 past its end (a slot or table entry that the kernels downstream flag and skip, as a negative id in it is).
   auto taken = [&](long long k) {
     const long long i = (long long)head + k;
     return i >= 0 && i < p.free_count ? p.free_blocks[i] : -1;
@@ -157,7 +157,6 @@ __global__ void __launch_bounds__(kLayoutThreads) packed_layout_kernel(LayoutPar
     if (tid == 0) {
       *p.free_head_out = head + blocks;
       if (total > p.token_bucket) bad = 1;
-      if (blocks > 0 && (head < 0 || (long long)head + blocks > p.free_count)) atomicOr(p.status, NVJ_DEV_BAD_BLOCK_ID);
     }
     if (bad) atomicOr(p.status, NVJ_DEV_BAD_LENGTH);
   }
@@ -207,8 +206,9 @@ __global__ void __launch_bounds__(kLayoutThreads) packed_layout_kernel(LayoutPar
   }
   // the new table entries: entry k of all of them belongs to the last row with first[row] <= k
   for (long long k = me; k < blocks; k += threads) {
-    const int r = layout_find(first, p.rows, (int)k);
-    p.block_tables[(long long)r * p.table_width + layout_blocks(p, cached[r]) + (int)(k - first[r])] = taken(k);
+    const int r = layout_find(first, p.rows, (int)k), id = taken(k);
+    if (id < 0) atomicOr(p.status, NVJ_DEV_BAD_BLOCK_ID);
+    p.block_tables[(long long)r * p.table_width + layout_blocks(p, cached[r]) + (int)(k - first[r])] = id;
   }
 }
 

@@ -114,7 +114,7 @@ class ResidentDecodeMetadata:
 
     def reserve(self, pool) -> None:
         """Room for the next token of every active row out of a `device_blocks.DeviceBlockPool`: what `set_block` does for the rows that
-        reach a new block, without the host knowing which."""
+        reach a new block, without the host knowing which.  May be captured together with the step that follows it."""
         pool.extend(self.block_tables, self.seq_lens, (self.seq_lens > 0).to(torch.int32), self.rows)
 
     def advance(self) -> None:

@@ -144,6 +144,61 @@ def test_resident_rows_take_their_next_blocks_from_the_pool():
     assert pool.free_head.tolist() == [0]
 
 
+def test_captured_decode_steps_take_new_blocks_at_every_replay():
+    bs = 4
+    lens = np.array([5, 8, 0, 1, 16])
+    meta = ResidentDecodeMetadata(5, 8, bs)
+    tables = np.zeros((5, 8), np.int64)
+    for r, n in enumerate(lens):
+        tables[r, : -(-n // bs)] = 100 + 10 * r + np.arange(-(-n // bs))
+    meta.load(tables, lens)
+    pool = DeviceBlockPool(range(40, 60), bs)
+    ids = iter(range(40, 60))
+
+    def step():
+        meta.reserve(pool)
+        meta.advance()
+
+    def walk(ids):
+        for r in range(5):
+            if lens[r] > 0:
+                if lens[r] % bs == 0:
+                    tables[r, lens[r] // bs] = next(ids)
+                lens[r] += 1
+
+    def same():
+        return np.array_equal(meta.seq_lens.cpu().numpy(), lens) and np.array_equal(meta.block_tables.cpu().numpy(), tables)
+
+    captured = CapturedStep(step)
+    captured.capture()  # (runs it once)
+    walk(ids)
+    for _ in range(6):
+        captured.replay()
+        walk(ids)
+    assert same() and pool.free_head.tolist() == [next(ids) - 40]
+    pool.reset([70, 71, 72, 73, 74])  # the ids that are free now, into the list that the step was captured with
+    ids = iter([70, 71, 72, 73, 74])
+    for _ in range(4):
+        captured.replay()
+        walk(ids)
+    assert same()
+    K.check_device_status()
+
+
+def test_a_pool_s_list_that_is_shorter_than_it_was_ends_where_it_ends(monkeypatch):
+    monkeypatch.setenv("NVJ_CHECK_STATUS", "0")
+    pool = DeviceBlockPool(range(10), 16)
+    pool.reset([3, 4])
+    tables = _i32(np.zeros((3, 2)))
+    lay = pool.extend(tables, _i32([0, 0, 0]), _i32([1, 1, 1]), 3)
+    assert tables.tolist() == [[3, 0], [4, 0], [-1, 0]] and lay.slot_mapping.tolist() == [[48, 64, -1]] and pool.free_head.tolist() == [3]
+    with pytest.raises(K.DeviceStatusError, match="device status 2 "):
+        K.check_device_status()
+    pool.reset(list(range(20, 40)))  # more than there ever were
+    assert pool.extend(tables, _i32([0, 0, 0]), _i32([1, 1, 1]), 3).slot_mapping.tolist() == [[320, 336, 352]]
+    K.check_device_status()
+
+
 # ------------------------------------------------------------------------------------------------ the operators in a run
 
 @pytest.mark.parametrize("heads", [(8, 2, 256, 16), (8, 4, 64, 32)])
