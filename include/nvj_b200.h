@@ -83,8 +83,9 @@ int nvj_compute_slot_mapping(const int32_t* positions, const int32_t* block_tabl
  *   the last row's get position 0, row 0 and slot -1.
  * A row with a negative length, or more tokens than its table has room for, is flagged NVJ_DEV_BAD_LENGTH and gets no new tokens; tokens
  * beyond the bucket are flagged the same way and left out (query_start_loc counts them).  Entries beyond the end of the free list
- * become -1, and their tokens' slots, flagged NVJ_DEV_BAD_BLOCK_ID, and so are negative ids in the list.  free_head_out may not be free_head.  At most 16384 rows, and
- * rows * table_width * block_size below 2^31; NVJ_ERR_TOO_LARGE beyond.
+ * become -1, and their tokens' slots, flagged NVJ_DEV_BAD_BLOCK_ID, and so are negative ids in the list.
+ * free_head_out may not be free_head, nor seq_lens one of the lengths.  At most 16384 rows, and rows * table_width * block_size below
+ * 2^31; NVJ_ERR_TOO_LARGE beyond.
  */
 int nvj_build_packed_layout(const int32_t* cached_lens, const int32_t* new_lens, int rows, int32_t* block_tables,
                             int table_width, int block_size, const int32_t* free_blocks, int free_count,

@@ -229,6 +229,7 @@ extern "C" int nvj_build_packed_layout(const int32_t* cached_lens, const int32_t
   if ((long long)table_width * block_size * (rows > 0 ? rows : 1) > 0x7fffffffLL) return NVJ_ERR_TOO_LARGE;
   if (!free_head || !free_head_out || !query_start_loc || !status || free_head == free_head_out) return NVJ_ERR_INVALID_ARGUMENT;
   if (rows > 0 && (!cached_lens || !new_lens || !seq_lens || (table_width > 0 && !block_tables))) return NVJ_ERR_INVALID_ARGUMENT;
+  if (rows > 0 && (seq_lens == cached_lens || seq_lens == new_lens)) return NVJ_ERR_INVALID_ARGUMENT;  // (a CTA reads them while another writes)
   if (free_count > 0 && !free_blocks) return NVJ_ERR_INVALID_ARGUMENT;
   if (token_bucket > 0 && (!positions || !token_row_ids || !slot_mapping)) return NVJ_ERR_INVALID_ARGUMENT;
   static PerDeviceFlags ready;

@@ -156,3 +156,8 @@ def test_every_named_barrier_of_the_tcgen05_decode_kernel_has_one_meaning():
     meetings = set(re.findall(r"qu_meet_any<([^>]*)>\((\w+),", text)) | set(re.findall(r"(named_bar_sync)\((\w+),", text))
     assert meetings == {("128", "bar"), ("L::kSoftmaxThreads", "kQuBarAll"), ("named_bar_sync", "kQuBarQueries")}
     assert re.search(r"\bbar = kQuBarGroup \+ group;", text)
+
+
+def test_a_layout_does_not_write_its_lengths_over_those_that_it_reads():
+    apart = dict(cached=P, new=P + 4096, tables=P + 8192, lens=P + 12288)
+    assert _layout(**apart | {"lens": P}) == INVALID and _layout(**apart | {"lens": P + 4096}) == INVALID
