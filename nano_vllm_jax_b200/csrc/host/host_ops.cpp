@@ -439,7 +439,7 @@ QuantizedLayer quantized_layer(PyObject* const* a) {  // k, v, k_scale, v_scale
   l.ks = static_cast<float*>(ks->data_ptr());
   l.vs = static_cast<float*>(vs->data_ptr());
   const bool dims = l.d == 64 || l.d == 128 || l.d == 256, block = l.block_size == 16 || l.block_size == 32 || l.block_size == 48 || l.block_size == 64;
-  l.ok = dims && block;
+  l.ok = dims && block && l.hkv >= 1;
   return l;
 }
 bool plain_rows(const at::Tensor& t, int device) { return on(t, device) && dtype_code(t) >= 0 && t.is_contiguous() && aligned(t); }

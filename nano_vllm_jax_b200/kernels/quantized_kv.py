@@ -44,6 +44,8 @@ def _cache(k, v, k_scale, v_scale):
     pages, page_size, hkv, d = k.shape
     if not quantized_cache_supported(page_size, d):
         raise ValueError(f"an 8-bit cache has head_dim in {HEAD_DIMS} and page_size in {PAGE_SIZES}, not {d} and {page_size}")
+    if hkv < 1:
+        raise ValueError("an 8-bit cache has at least one kv head")
     for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
         if t.dtype != torch.float32 or t.shape != (pages, hkv):
             raise ValueError(f"{name} must be float32 [num_pages, num_kv_heads]")

@@ -315,3 +315,14 @@ def test_tokens_beyond_the_bucket_of_a_bf16_cache_are_left_out(dtype, cached):
                 seen = np.arange(lens[r])[None] < c + 1 + np.arange(at.stop - at.start)[:, None]
                 want = R.attend(_f64(q[at]), x, y, seen, d ** -0.5)
                 assert np.abs(out[at] - want).max() <= R.tolerance(_f64(q[at]), x, y, d ** -0.5, 8), r  # (weights rounded to bf16)
+
+
+def test_a_cache_without_heads_is_refused():
+    k = torch.zeros(4, 16, 0, 256, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+    s = torch.ones(4, 0, device="cuda")
+    q, tables, lens = torch.zeros(2, 8, 256, device="cuda"), _i32([[0, 1], [2, 3]]), _i32([3, 4])
+    for call in (lambda: Q.paged_decode_attention_quantized(q, k, k, s, s, tables, lens, 1.0),
+                 lambda: Q.packed_paged_prefill_attention_quantized(q[None], k, k, s, s, tables, lens, _i32([[0, 1]]), _i32([0, 1, 2]), 16, 1.0, 4),
+                 lambda: Q.kv_append_quantized(q[:, None, :0], q[:, None, :0], k, k, s, s, _i32([[0], [0]]), tables)):
+        with pytest.raises(ValueError, match="kv head"):
+            call()
