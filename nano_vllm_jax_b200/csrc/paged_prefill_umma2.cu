@@ -267,8 +267,10 @@ __device__ __forceinline__ void u2_mma_warp(Umma2Smem& sm, const Umma2Params& p,
 // 2050 cycles per tile.)  What stays in turn is the row's reference (the running maximum, moved only when a tile exceeds it
 // by 2^kU2RescaleGap): a group settles its tile's reference behind the other's, before its exponentials.  False when a
 // wait ran out (the caller still joins its barriers).
-template <bool kFlush>
-__device__ __forceinline__ bool u2_softmax_tiles(Umma2Smem& sm, const Umma2Params& p, uint32_t my_tmem, int tok0, int ntok,
+// kMissing: some of an 8-bit cache's blocks were outside the pool, so that they have no page: their keys are left out.  (A walk of its own, since to look
+// for them in every tile costs 16384 tokens of a prompt 1540 us instead of 1365: registers.)
+template <bool kFlush, bool kMissing>
+__device__ __forceinline__ bool u2_softmax_tiles(Umma2Smem& sm, const Umma2Params& p, uint32_t my_tmem, int row, int tok0, int ntok,
                                                  int kv_len, int tile0, int n_tiles, int group, int r, int token, float& m_row,
                                                  float& l_row, float* flush_row) {
   const int my_pos = token < ntok ? p.positions[tok0 + token] : -1;
@@ -286,6 +288,12 @@ __device__ __forceinline__ bool u2_softmax_tiles(Umma2Smem& sm, const Umma2Param
     u2_arrive_warp(smem_u32(&sm.s_read));
     const int lim = last_key - (tile0 + t) * kU2Keys;
     float tmax = -INFINITY;
+    if constexpr (kMissing) {
+      const int at = (tile0 + t) * (kU2Keys / kBlk) + (r & 3);
+      const unsigned gone = __ballot_sync(0xffffffffu, at < p.table_width && p.block_tables[(long long)row * p.table_width + at] < 0);
+#pragma unroll
+      for (int i = 0; i < kU2Keys; ++i) s[i] = gone >> i / kBlk & 1u ? -INFINITY : s[i];
+    }
     if (lim >= kU2Keys - 1) {
 #pragma unroll
       for (int i = 0; i < kU2Keys; i += 2) tmax = fmaxf(tmax, fmaxf(s[i], s[i + 1]));
@@ -403,9 +411,9 @@ __device__ __forceinline__ int u2_piece(int r, int c) { return r * kD + (((c & ~
 
 // ---- warps 2-9 of both CTAs: Q staging, softmax, epilogue for this CTA's 128 rows -------------
 template <bool kFlush>
-__device__ __forceinline__ void u2_softmax_warps(Umma2Smem& sm, const Umma2Params& p, uint32_t tmem, int tok0, int ntok,
+__device__ __forceinline__ void u2_softmax_warps(Umma2Smem& sm, const Umma2Params& p, uint32_t tmem, int row, int tok0, int ntok,
                                                  int kvh, int kv_len, int tile0, int n_tiles, int splits, int warp, int lane,
-                                                 const uint4 (&u)[4][4]) {
+                                                 const uint4 (&u)[4][4], bool missing) {
   const int quarter = warp & 3, half = (warp - 2) >> 2;
   const int r = quarter * 32 + lane, token = lane, hl = quarter;
   const uint32_t my_tmem = tmem + ((uint32_t)(quarter * 32) << 16);
@@ -466,7 +474,8 @@ __device__ __forceinline__ void u2_softmax_warps(Umma2Smem& sm, const Umma2Param
   float m_row = -INFINITY, l_row = 0.f;
   // (split key ranges are short, and their output rows not this CTA's alone)
   float* out_row = kFlush && splits == 1 && n_tiles > kU2FlushTiles ? p.out + ((long long)(tok0 + token) * kHq + kvh * kG + hl) * kD : nullptr;
-  bool alive = u2_softmax_tiles<kFlush>(sm, p, my_tmem, tok0, ntok, kv_len, tile0, n_tiles, half, r, token, m_row, l_row, out_row);
+  bool alive = missing ? u2_softmax_tiles<kFlush, kFlush>(sm, p, my_tmem, row, tok0, ntok, kv_len, tile0, n_tiles, half, r, token, m_row, l_row, out_row)
+                       : u2_softmax_tiles<kFlush, false>(sm, p, my_tmem, row, tok0, ntok, kv_len, tile0, n_tiles, half, r, token, m_row, l_row, out_row);
   // ---- epilogue.  From here on the softmax threads meet at CTA-wide named barriers, so a thread whose wait ran out
   // does not leave: it skips the work and everybody returns together once the barrier has made the flag visible.
   NVJ_U2_PHASE(4);
@@ -720,6 +729,8 @@ prefill_umma2_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
       pdl_release();
     }
   }
+  // (pages that are missing have been flagged by the kernel that wrote the others)
+  const bool missing = kFlush && (*reinterpret_cast<volatile int32_t*>(p.status) & NVJ_DEV_BAD_BLOCK_ID) != 0;
   auto leave = [&] {  // the whole cluster leaves without having touched its tensor memory
     cl_sync();
     if (warp == 1) tmem2_dealloc(sm.tmem_base, kU2TmemCols);
@@ -809,7 +820,7 @@ prefill_umma2_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_con
 
   if (warp == 0) u2_producer(&k_map, &v_map, p, sm, row, kvh, kv_len, tile0, my_tiles, rank, lane, first_ids);
   else if (warp == 1) { if (rank == 0) u2_mma_warp(sm, p, tmem, my_tiles); }
-  else u2_softmax_warps<kFlush>(sm, p, tmem, tok0, ntok, kvh, kv_len, tile0, my_tiles, splits, warp, lane, qv);
+  else u2_softmax_warps<kFlush>(sm, p, tmem, row, tok0, ntok, kvh, kv_len, tile0, my_tiles, splits, warp, lane, qv, missing);
 
   tc_fence_before_sync();
   __syncthreads();

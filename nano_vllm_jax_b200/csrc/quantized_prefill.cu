@@ -43,7 +43,7 @@ struct QUnpackParams {
 
 // Grid (x: blocks of a row in strides, y: rows); the model's shape, 16 tokens of 2 heads of 256: a thread four pieces of 16 numbers, two of K and two
 // of V, of one head.  The block's id is asked for together with the row's length: two trips to memory in a row.  A block whose id is outside
-// the pool becomes a page of zeros, as the other kernels take it, and so do the rows behind the last key that a token sees, which hold anything.
+// the pool has no page, and the tiles leave its keys out; the rows behind the last key that a token sees, which hold anything, become zeros.
 __global__ void __launch_bounds__(256) quantized_unpack_kernel(QUnpackParams p) {
   constexpr int kRow = 512, kBlock = 16 * kRow;  // bytes of a token, and of a block
   pdl_wait();
@@ -71,7 +71,10 @@ __global__ void __launch_bounds__(256) quantized_unpack_kernel(QUnpackParams p) 
     const int left = len - b * 16;  // tokens of the row from this block on
     if (skip || left <= 0) continue;
     const bool ok = id >= 0 && id < p.num_blocks;
-    if (!ok && threadIdx.x == 0) atomicOr(p.status, NVJ_DEV_BAD_BLOCK_ID);
+    if (!ok && threadIdx.x == 0) {
+      atomicOr(p.status, NVJ_DEV_BAD_BLOCK_ID);
+      p.page_tables[page] = -1;
+    }
     uint4 w[4];
     const int left_seen = seen - b * 16;
     float unit[2] = {0.f, 0.f};

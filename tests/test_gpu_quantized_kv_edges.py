@@ -211,6 +211,30 @@ def test_keys_that_no_token_of_the_row_sees_may_hold_anything(route, shape, dtyp
     _check(out, q, state, tables, [max(s) for s in seen], np.array(seen), d ** -0.5, 16 if route == "prefill" and shape == MODEL and dtype == BF16 else TERM_BITS[route])
 
 
+@pytest.mark.parametrize("route,shape,dtype", [(1, MODEL, BF16), (2, MODEL, BF16)] + [("prefill", *t) for t in TILES])
+def test_blocks_outside_the_pool_reach_nothing(route, shape, dtype, monkeypatch):
+    hq, hkv, d, bs = shape
+    rng = np.random.default_rng(57)
+    lens = [200, 2000, 70, bs]
+    tables, state = _rows(rng, lens, shape)
+    q = torch.from_numpy(rng.standard_normal((4, 3, hq, d))).to(dtype).cuda()
+    limits = np.array(lens)[:, None] - 2 + np.arange(3)[None]
+    monkeypatch.setenv("NVJ_CHECK_STATUS", "0")
+    broken = tables.copy()
+    pool = len(state[0][0])
+    broken[0, 0], broken[0, 100 // bs], broken[1, 1000 // bs], broken[1, 1984 // bs], broken[3, 0] = pool, -1, 1 << 30, pool, -(1 << 31)
+    out = _attend(route, q, state, broken, lens, limits, shape, d ** -0.5)
+    with pytest.raises(K.DeviceStatusError, match="device status 2 "):
+        K.check_device_status()
+    q = _f64(q)
+    for r, n in enumerate(lens):
+        good = np.repeat(broken[r, : -(-n // bs)] == tables[r, : -(-n // bs)], bs)[:n]
+        k, v = (R.gather(codes, s, tables[r], n) for codes, s in state)
+        want = R.attend(q[r], k, v, (np.arange(n)[None] < limits[r][:, None]) & good[None], d ** -0.5)
+        term_bits = 16 if route == "prefill" and shape == MODEL and dtype == BF16 else TERM_BITS[route]
+        assert np.abs(out[r] - want).max() <= R.tolerance(q[r], k, v, d ** -0.5, term_bits), r
+
+
 # ------------------------------------------------------------------------------------------------ packed batches
 
 def _packed(rng, rows, shape, dtype):
