@@ -183,7 +183,8 @@ __global__ void __launch_bounds__(kLayoutThreads) packed_layout_kernel(LayoutPar
           block = b;
           id = b < held ? p.block_tables[(long long)r * p.table_width + b] : taken(first[r] + (b - held));
         }
-        if (id >= 0) slot[e] = id * p.block_size + (position[e] - b * p.block_size);
+        const long long at = (long long)id * p.block_size + (position[e] - b * p.block_size);
+        if (id >= 0 && at <= 0x7fffffffLL) slot[e] = (int)at;  // (an id whose slots no int32 names belongs to no pool)
       }
     }
     if (vector && i0 + 4 <= p.token_bucket) {

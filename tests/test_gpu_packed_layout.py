@@ -106,6 +106,13 @@ def test_what_does_not_fit_is_flagged_and_left_out(monkeypatch):
     assert got.query_start_loc.tolist() == [0, 3, 7] and got.slot_mapping.tolist() == [[128, 129, 130, 144, 145]]
 
 
+def test_ids_whose_slots_pass_32_bits_have_none():
+    # (1 << 28) * 16 is 0 in 32 bits: the slot of another row's token
+    tables = _i32([[1 << 28, 0], [7, 0], [(1 << 27) - 1, 0]])
+    got = K.build_packed_layout(_i32([5, 16, 14]), _i32([2, 1, 2]), tables, _i32([(1 << 31) - 1]), _i32([0]), 16, 5)
+    assert got.slot_mapping.tolist() == [[-1, -1, -1, (1 << 31) - 2, (1 << 31) - 1]] and tables[1, 1].item() == (1 << 31) - 1
+
+
 def test_wrapper_refuses_what_does_not_fit_together():
     good = dict(cached_lens=_i32([1, 2]), new_lens=_i32([1, 1]), block_tables=_i32([[0], [1]]), free_blocks=_i32([4]), free_head=_i32([0]), block_size=16,
                 token_bucket=4)
