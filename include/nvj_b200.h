@@ -459,7 +459,7 @@ int nvj_paged_prefill_packed_counted(const void* q, int q_dtype,
  *
  * The tokens of a call that fall into one block have to stand together in the batch (any order among them); a row's
  * consecutive positions do.  A block that two runs of tokens write in one call (two rows that share it) ends as either leaves it, or
- * as a mixture.  For each run and kv head, K and V apart: a = the largest finite magnitude, e = the least integer with
+ * as a mixture, and so does a position that two tokens name.  For each run and kv head, K and V apart: a = the largest finite magnitude, e = the least integer with
  * a <= 448 * 2^e.  If one of the tokens is the block's first (offset 0) the block begins anew with scale 2^e; otherwise its scale
  * becomes max(scale, 2^e), and if it grows the numbers of the block's other rows are rescaled, rounded to nearest even.  New
  * numbers are value / scale rounded to nearest even; magnitudes over 448 * scale (infinities among them) are held there, NaN is kept.

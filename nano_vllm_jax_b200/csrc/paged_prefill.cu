@@ -40,7 +40,7 @@ struct PackedArgs {
   int rows, token_bucket; float scale; float* out; int32_t* status;
   void* workspace; size_t workspace_bytes; int variant;
   int tile_pairs = -1;  // what the caller counted on the host (-1: not told)
-  bool flush = false;   // empty the tiles' accumulators every 8192 keys (paged_prefill_umma2.cu)
+  bool flush = false;   // the pages of an 8-bit cache: empty the tiles' accumulators every 4096 keys, leave out missing ones (paged_prefill_umma2.cu)
 };
 
 static int check_packed(const PackedArgs& a, bool* tile_ok) {

@@ -84,7 +84,7 @@ struct Umma2Params {
   int pair_slots;  // CTA pairs that run at once
 };
 
-// With kFlush (the pages of an 8-bit cache): tiles of 64 keys after which the output accumulators are emptied into the
+// With kFlush (the pages of an 8-bit cache; missing ones are -1 in the tables): tiles of 64 keys after which the output accumulators are emptied into the
 // output rows.  The tensor cores cut the last place of what they add to: 1.2e-5 of a sum over 16384 keys left alone,
 // 9.4e-6 emptied each 128 tiles, 6.6e-6 each 64, 5.8e-6 each 32, for 1140, 1192, 1213 and 1541 us.  Even: the same
 // softmax group empties every time.

@@ -6,8 +6,8 @@
 // rescaled if it has to grow, and the new ones stored.  K and V, the heads and the runs have nothing in common, so there are no
 // atomics and no second pass over memory.
 // bytes = tokens * kv_heads * head_dim * 2 * (source size + 1).  Prompts are bound by HBM and, in front of it, by the chain positions -> block id ->
-// scale -> stores: 16384 bf16 tokens of 2 heads of 256 14.7 us (50 MB: 7.7 us); with a warp per run, 126 registers of held rows and so half
-// of the CTAs in a second wave, 18.4.  A decode step is launch and chain: 256 tokens 3.5 us.
+// scale -> stores: 16384 bf16 tokens of 2 heads of 256 11.0 us (50 MB: 7.7 us), 13 with cold caches; with a warp per run, 126 registers of held rows and so
+// half of the CTAs in a second wave, a quarter more.  A decode step is launch and chain: 256 tokens 3.3 - 3.5 us.
 
 #include "quantized_kv.cuh"
 
@@ -245,8 +245,8 @@ __global__ void __launch_bounds__(32 * kQAppendWarps) quantized_append_kernel(QA
 
 template <typename T>
 static int launch_quantized_append(const QAppendParams& p, int head_dim, cudaStream_t stream) {
-  // Batches of a few tokens per row: a run per window.  Prompts: windows of 16 tokens, in which one run begins, mostly (a window per token: 37 us
-  // for 16384 tokens, most of it warps that find nothing to do; windows of 31: 16.5 against 14.7).
+  // Batches of a few tokens per row: a run per window.  Prompts: windows of 16 tokens, in which one run begins, mostly (16384 tokens when they took 14.7 us,
+  // before the divisions went: a window per token 37, most of it warps that find nothing to do; windows of 31 16.5).
   const long long rows = p.packed ? p.qsl_rows : (p.n_tokens + p.n_cols - 1) / p.n_cols;
   const bool prompt = p.n_tokens > 4 * (rows > 0 ? rows : 1);
   const int window = prompt ? 16 : 1, parts = 2 * p.num_kv_heads;

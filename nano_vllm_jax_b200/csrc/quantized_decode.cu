@@ -17,8 +17,8 @@
 //   * the K scale of a block multiplies its scores, the V scale goes into the exponent of the weights: a running maximum of
 //     its own for the weighted sum keeps blocks of any scale apart from the sum of the weights.
 // Maxima are lazy: one vote per tile says whether a score has left them behind, and only then the sums are rescaled.
-// Measured: four rows of 64 - 512 keys, 8 heads of 256 over 2, 7.3 us, which is launch, trips and merge; 126 rows of 4850 - 9700 keys, 4 heads of 64, 154 us
-// (47% of the copy rate), 16 over 2 94 us (38%): instructions.
+// Measured: four rows of 64 - 512 keys, 8 heads of 256 over 2, 6.9 - 7.5 us, which is launch, trips and merge; 126 rows of 4850 - 9700 keys, 4 heads of 64, 157
+// us (46% of the copy rate), 16 over 2 94 us (38%): instructions.
 
 #include "cluster.cuh"
 #include "decode_parts.cuh"
@@ -720,8 +720,8 @@ static int run_quantized_umma(const QDecodeParams& q, int q_dtype, int head_dim,
 
 // Whether a call goes to the tcgen05 form: by the room of its tables, since the lengths are on the GPU.  That form starts and folds 5 us later, and
 // takes 3 - 8 us for a row and head even if they have few keys, but 0.4 - 1.2 us per 128 keys behind them where this file's takes up to 2.8 (head_dim
-// 256).  Over 272 batches of 1 - 512 rows, 64 - 65536 keys, 4 - 80 columns and four head layouts the rule costs 1.5% against the better of both,
-// 30% at most (always this file's form: 23%, always the other: 19%).  Either side of it, us: 64 rows of 64 - 128 keys, 2 heads of 256 and 4
+// 256).  Over 272 batches of 1 - 512 rows, 64 - 65536 keys, 4 - 80 columns and four head layouts (drawn once, their times are not kept) the rule cost
+// 1.5% against the better of both, 30% at most (always this file's form: 23%, always the other: 19%).  Either side of it, us: 64 rows of 64 - 128 keys, 2 heads of 256 and 4
 // columns 10.2 against 14.9, 64 of 1024 - 2048 keys 45 against 27; one row of 4096 keys 11.7 against 15.1, one of 32768 45.9 against 22.6.
 static bool quantized_umma_pays(int rows, int width, int table_width, int block_size, int num_kv_heads, int head_dim, int groups) {
   const long long room = (long long)table_width * block_size, columns = ((long long)width * groups + 3) / 4;

@@ -5,8 +5,8 @@
 //     pages of a scratch cache, and the tcgen05 tiles of the bf16 cache run over it (paged_prefill_umma2.cu).  Writing out moves 5 bytes
 //     per number, once per call: 6 us for 3.6k keys, 1% of a prompt's time.
 //   * Every other head layout, block size and query type: quantized_prefill_umma.cuh, which converts the numbers on their way into shared memory,
-//     for every 128 query rows anew (the pages' batches would take it 30.6 us instead of 28.7 for 512 tokens of three rows behind 1024, 134
-//     instead of 105 for a prompt of 4096; 42 instead of 44 for 256 tokens behind 4000).
+//     for every 128 query rows anew (the pages' batches would take it 29.7 us instead of 28.7 for 512 tokens of three rows behind 1024, 135
+//     instead of 108 for a prompt of 4096; 41.5 instead of 45.6 for 256 tokens behind 4000).
 
 #include "quantized_kv.cuh"
 #include "quantized_prefill_params.cuh"

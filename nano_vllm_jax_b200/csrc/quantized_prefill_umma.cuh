@@ -9,7 +9,7 @@
 // A tile of 64 keys takes 4 * 128 * 64 * head_dim flops for S and twice that for O's two terms: 2200 cycles of an SM at head_dim 256.  A softmax
 // thread's way from a tile's scores to its weights takes as long: scores out of tensor memory 400, the pair's meeting 500, exponentials and terms
 // 700, back 250.  head_dim 64 takes just that, 128 2500, 256 3400, where queries, keys and values move 220 KB through shared memory per tile.
-// Against the tiles of mma.sync that stood here before: 1984 f16 tokens behind 727, 32 heads of 128 over 8, 452 -> 186 us; 1018 tokens of
+// Against the tiles of mma.sync that stood here before: 1984 f16 tokens behind 727, 32 heads of 128 over 8, 452 -> 187 us; 1018 tokens of
 // four rows behind 1232 each 165 -> 74; 55 f32 tokens of two rows behind 1214 (8 heads of 256 over 2) 160 -> 27; 54 tokens behind 1398 (16
 // heads of 64 over 2) 62 -> 16; the smallest calls as long as they took (20 tokens, heads of 256: 17.7 -> 17).  A small call at head_dim
 // 256 is start and end: row and lengths 2.4 us, queries 3, a tile 2, rows staged 3, folded over DSMEM 5.

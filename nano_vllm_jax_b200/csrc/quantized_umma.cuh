@@ -3,9 +3,12 @@
 //
 // e4m3 is an operand type of the tensor cores, so K and V need no conversion and go from memory to shared memory and no further; what
 // has to become e4m3 is the other side, and a number becomes a sum of e4m3 terms: t0 = rne(x), t1 = rne(16 (x - t0)), ..., each with
-// four bits of it.  bf16 queries (8 bits) are two terms exactly, f16 three, f32 five (2^-20); the weights of the softmax five (2^-20, and
+// four bits of it.  bf16 queries (8 bits) are two terms, f16 three, f32 five (2^-20); the weights of the softmax five (2^-20, and
 // never closer than 2^-26, the last place of the fifth term: the largest weight is kept between 2^3 and 2^8, so that a key 2^8 below it
-// still has 2^-21).  The terms are columns of their own, added with their powers of 16 when a result is read:
+// still has 2^-21).  The last term's last place bounds small numbers, too: two terms are exact down to 2^-13 of a column's largest query number and
+// round smaller ones to 2^-22 of it, three (f16) 2^-14 and 2^-26, five to 2^-34.  (256 dims of which one is 2^8 / 2^12 times the others, and the others
+// decide: 5.5e-6 / 3.4e-4 of the result in bf16, 4.6e-7 / 1.5e-5 in f16, 4e-7 in f32; a third term for bf16 would cost 64 rows of 5 tokens 2.8 us.)
+// The terms are columns of their own, added with their powers of 16 when a result is read:
 //   S^T = K Q^T    [128 keys x kQTerms * kC]            32 dims per MMA, K and Q from shared memory, K-major;
 //   O^T = V^T P^T  [kDim / 128 x 128 dims x 5 * kC]     32 keys per MMA, V and the weights from shared memory, MN-major.
 // A tile of 128 keys of one kv head is 64 KiB (head_dim 256), 1.4 us of an SM's share of the memory; its products take a fraction of
@@ -16,8 +19,8 @@
 // (decode_parts.cuh); rows cut over ranges leave partials, folded by a second small launch.
 //   softmax    thread = key, in groups of four warps.  Up to eight columns two groups take the tiles in turn, each with
 //              references, sums and accumulators of its own (a tile's chain of waits, from its scores to its weights, is longer than
-//              its bytes: one group alone took 1.85 us per tile of 64 KiB); of 16 or 24 two or three groups take eight each (two of twelve:
-//              64 rows of 5 tokens 50.4 us, three of eight 47.6).
+//              its bytes: one group alone took 1.85 us per tile of 64 KiB); of 16 or 24 two or three groups take eight each (two of twelve
+//              columns 2.8 us slower on 64 rows of 5 tokens).
 //              Scores from tensor memory, times the K scale of the key's block, plus the log2 of its V scale; weights exp2(that -
 //              reference) as e4m3 terms into shared memory; their sum with the V scale divided out again, relative to the largest so far.
 //              Thread = dim when a row's segment ends.
@@ -25,9 +28,9 @@
 //   1 warp     TMA producer: boxes of a unit's keys [8-key group][128-byte chunk][8 keys][128 B], 128-byte swizzle, into rings of tiles of K
 //              and of V (160 KiB), and with K the scales of its blocks.
 //   1 warp     the queries, up to two segments ahead: scaled to 2^7 - 2^8 by a power of two per column, split into terms.
-// Measured, 8 bf16 heads of 256 over 2: 256 rows of 1024 - 4096 keys 107 us (6.3 TB/s, 96% of the copy rate), 64 of 8192 - 32768 200 us (103%), 64 of
-// 1024 - 4096 with 5 tokens each 47.5 us (55%: bound by a tile's way from scores to weights, 1.75 us where its bytes take 1.4); 48 f16 rows of 200 - 3000
-// keys, 32 heads of 128 over 8, 37.7 us (64%: 5 us until the first scores, 5 for the fold).
+// Measured on several GPUs, 8 bf16 heads of 256 over 2: 256 rows of 1024 - 4096 keys 107 - 113 us (92 - 96% of the copy rate), 64 of 8192 - 32768 200 - 208
+// us (99 - 103%), 64 of 1024 - 4096 with 5 tokens each 48 - 50 us (53 - 55%: bound by a tile's way from scores to weights, 1.75 us where its bytes take
+// 1.4); 48 f16 rows of 200 - 3000 keys, 32 heads of 128 over 8, 38.1 us (64%: 5 us until the first scores, 5 for the fold).
 // Every wait is bounded; after a timeout (NVJ_DEV_TIMEOUT) the kernel stops issuing, lets copies land and frees its tensor
 // memory.  A block id outside the pool is flagged, fetched from beyond the tensor (zeros) and its keys are left out.
 #pragma once

@@ -138,7 +138,7 @@ def paged_decode_attention_quantized(q, k_cache_layer, v_cache_layer, k_scale, v
     """Decode attention over one layer of the 8-bit cache, for rows of one query token or a few.
 
     q `[B, Hq, D]` -> float32 `[B, Hq, D]`, or `[B, T, Hq, D]` -> `[B, T, Hq * D]`.  Token t of row b sees the keys p < seq_lens[b] and,
-    with `positions` `[B, T]`, p <= positions[b, t]; one that sees none gives zeros.  `form`: 0 automatic, 1 mma.sync tiles on
+    with `positions` `[B, T]`, p <= positions[b, t]; one that sees none gives zeros.  Keys that no token of a row sees may hold anything.  `form`: 0 automatic, 1 mma.sync tiles on
     thread-block clusters, 2 tcgen05 tiles (head_dim 128 or 256).
     """
     out = _k.host().quantized_decode(q, k_cache_layer, v_cache_layer, k_scale, v_scale, block_table, seq_lens, scale, positions, form)
@@ -190,7 +190,8 @@ def packed_paged_prefill_attention_quantized(query, k_cache_layer, v_cache_layer
     """Ragged packed prefill over one layer of the 8-bit cache: query `[1, T, Hq, D]` -> float32 `[1, T, Hq * D]`, padded tokens 0.
 
     Masks and the two counts (`num_decode_rows`: rows of a single query token, `query_tile_pairs`: 64-token tiles of the other
-    rows) as in `paged_kv.packed_paged_prefill_attention`.  bfloat16 queries of the model's shape run on the tcgen05 tiles over bf16
+    rows) as in `paged_kv.packed_paged_prefill_attention`; tokens that `query_start_loc`
+    counts beyond the bucket are left out.  bfloat16 queries of the model's shape run on the tcgen05 tiles over bf16
     pages written for the call (exact; up to 1 GiB, from torch's allocator), others on tcgen05 tiles over the 8-bit blocks.
     """
     out = _k.host().quantized_prefill(query, k_cache_layer, v_cache_layer, k_scale, v_scale, block_table, kv_lens, positions, query_start_loc,
