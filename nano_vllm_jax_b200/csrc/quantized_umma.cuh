@@ -2,13 +2,13 @@
 // rows of few query tokens.  Included by one file per type of query (quantized_umma_*.cu).
 //
 // e4m3 is an operand type of the tensor cores, so K and V need no conversion and go from memory to shared memory and no further; what
-// has to become e4m3 is the other side, and a number becomes a sum of e4m3 terms: t0 = rne(x), t1 = rne(16 (x - t0)), ..., each with
-// four bits of it.  bf16 queries (8 bits) are two terms, f16 three, f32 five (2^-20); the weights of the softmax five (2^-20, and
-// never closer than 2^-26, the last place of the fifth term: the largest weight is kept between 2^3 and 2^8, so that a key 2^8 below it
-// still has 2^-21).  The last term's last place bounds small numbers, too: two terms are exact down to 2^-13 of a column's largest query number and
-// round smaller ones to 2^-22 of it, three (f16) 2^-14 and 2^-26, five to 2^-34.  (256 dims of which one is 2^8 / 2^12 times the others, and the others
-// decide: 5.5e-6 / 3.4e-4 of the result in bf16, 4.6e-7 / 1.5e-5 in f16, 4e-7 in f32; a third term for bf16 would cost 64 rows of 5 tokens 2.8 us.)
-// The terms are columns of their own, added with their powers of 16 when a result is read:
+// has to become e4m3 is the other side, and a number becomes a sum of e4m3 terms: t0 = rne(x), t1 = rne(u (x - t0)), ..., each with
+// four bits of it; u = 32 for queries, 16 for weights.  bf16 queries are three terms, or two where a CTA has more than eight columns, f16 three, f32
+// five (2^-20); the weights of the softmax five (2^-20, and never closer than 2^-26, the last place of the fifth term: the largest weight is kept between
+// 2^3 and 2^8, so that a key 2^8 below it still has 2^-21).  The last term's last place bounds a query's small numbers, too: they are right to 2^-23, 2^-28
+// or 2^-38 of the row's largest number, with two, three or five terms (exact, in bf16, from 2^-15 of it on with two, in f16 from 2^-17 on).  One of 256 dims
+// 2^12 times the others, which decide: 1.2e-6 of the result in bf16 and one token (with two terms and u = 16 it was 3.4e-4), 2.2e-6 in f16, 4e-7 in f32.
+// The terms are columns of their own, added with their powers of u when a result is read:
 //   S^T = K Q^T    [128 keys x kQTerms * kC]            32 dims per MMA, K and Q from shared memory, K-major;
 //   O^T = V^T P^T  [kDim / 128 x 128 dims x 5 * kC]     32 keys per MMA, V and the weights from shared memory, MN-major.
 // A tile of 128 keys of one kv head is 64 KiB (head_dim 256), 1.4 us of an SM's share of the memory; its products take a fraction of
@@ -59,9 +59,9 @@ constexpr float kQuNone = -3e38f, kQuSlack = 8.f, kQuLift = 3.f;
 // row's output owes to values 2^-90 of the largest of its blocks and smaller may be off, by 2^-90 of that largest one at most.
 constexpr float kQuFar = 40.f, kQuMost = 106.f, kQuMostSum = 0x1p108f;  // (10^6 keys of 2^kQuMost are an f32 number)
 
-template <typename T>
-constexpr int quq_terms() {
-  return sizeof(T) == 4 ? 5 : std::is_same<T, __half>::value ? 3 : 2;
+template <typename T, int kSharing>
+constexpr int quq_terms() {  // (a third one of bf16 is free up to eight columns; with 20 it takes 64 rows 2.8 us of 49)
+  return sizeof(T) == 4 ? 5 : std::is_same<T, __half>::value || kSharing == 1 ? 3 : 2;
 }
 
 // kCg: columns of a softmax thread; kSharing: groups that share a tile, a region of the columns each.  One: two groups take the tiles in turn.
@@ -71,7 +71,7 @@ struct QuLayout {
   static constexpr int kGroups = kByTiles ? 2 : kSharing, kSoftmaxThreads = 128 * kGroups, kThreads = kSoftmaxThreads + 128;
   static constexpr int kC = kCg * kSharing;  // columns of the CTA
   static constexpr int kRegions = kSharing;  // of a row of query terms or weights
-  static constexpr int kQTerms = quq_terms<T>();
+  static constexpr int kQTerms = quq_terms<T, kSharing>();
   static constexpr int kChunks = kDim / 128;
   static constexpr int kSRegion = kQTerms * kCg;                        // columns of S: [region][term][kCg]
   static constexpr int kORegion = kQuPTerms * kCg;                      // columns of O: [region][term][kCg]
@@ -455,7 +455,7 @@ __device__ __forceinline__ void qu_softmax_warps(QuSmem<L>& sm, const QuParams& 
         for (int c = 0; c < kCg; ++c) {
           float y = x[((L::kQTerms - 1) * kCg + c) / 8][((L::kQTerms - 1) * kCg + c) % 8];
 #pragma unroll
-          for (int j = L::kQTerms - 2; j >= 0; --j) y = fmaf(y, 0.0625f, x[(j * kCg + c) / 8][(j * kCg + c) % 8]);
+          for (int j = L::kQTerms - 2; j >= 0; --j) y = fmaf(y, 0.03125f, x[(j * kCg + c) / 8][(j * kCg + c) % 8]);
           sc[c] = there && at_key < seen[c] ? fmaf(y, by[c] * k_unit, v_log) : -INFINITY;
         }
       }
@@ -719,8 +719,8 @@ struct QuColumn {  // from column c on: column c + l / kLanes, dims 8 (l % kLane
         b[k] = q_pack2(x[2 * k], x[2 * k + 1]);
         if (j + 1 < L::kQTerms) {
           const float2 y = q_float2(q_half2(b[k]));
-          x[2 * k] = (x[2 * k] - y.x) * 16.f;
-          x[2 * k + 1] = (x[2 * k + 1] - y.y) * 16.f;
+          x[2 * k] = (x[2 * k] - y.x) * 32.f;  // (a term is at most 2^8, what its rounding leaves 2^3)
+          x[2 * k + 1] = (x[2 * k + 1] - y.y) * 32.f;
         }
       }
       const int row = row0 + j * kCg;

@@ -350,3 +350,21 @@ def test_a_cache_without_heads_is_refused():
                  lambda: Q.kv_append_quantized(q[:, None, :0], q[:, None, :0], k, k, s, s, _i32([[0], [0]]), tables)):
         with pytest.raises(ValueError, match="kv head"):
             call()
+
+
+# One number of a query 2^power times the others, and keys that are small there, so that the others decide: they keep their bits.
+@pytest.mark.parametrize("route,tokens,power", [(1, 1, 14), (2, 1, 8), (2, 1, 14), (2, 2, 14), (1, 5, 12), (2, 5, 8), (2, 5, 12), ("prefill", 3, 14)])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_queries_with_one_large_number(route, tokens, power, dtype):
+    hq, hkv, d, bs = MODEL
+    rng = np.random.default_rng(61)
+    lens = [300, 2100]
+    tables, state = _rows(rng, lens, MODEL)
+    state[0][0][..., 7] &= 0x87  # (2^-6 at most, times the scale)
+    down = 64.0 if dtype == F16 else 1.0  # (f16 ends at 65504)
+    q = rng.standard_normal((2, tokens, hq, d)) / down
+    q[..., 7] *= 2.0 ** power
+    q = torch.from_numpy(q).to(dtype).cuda()
+    limits = np.array(lens)[:, None] - tokens + 1 + np.arange(tokens)[None]
+    out = _attend(route, q, state, tables, lens, limits, MODEL, down / 16)
+    _check(out, q, state, tables, lens, limits, down / 16, 16 if route == "prefill" and dtype == BF16 else TERM_BITS[route])
