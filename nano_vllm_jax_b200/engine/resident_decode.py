@@ -143,6 +143,8 @@ class DecodeStepGraph:
         (each step's launch collects the step before), and `flush()` brings it up to date."""
         if k_cache.ndim != 5:
             raise ValueError("k_cache must be the 5-D cache [L, NB, bs, Hkv, D]")
+        if k_cache.dtype == torch.float8_e4m3fn:
+            raise ValueError("DecodeStepGraph does not take 8-bit caches (capture their append and decode in a CapturedStep)")
         self.meta, self.k_cache, self.v_cache = meta, k_cache, v_cache
         self.layer_id, self.scale, self.groups = int(layer_id), float(scale), int(num_key_value_groups)
         _, _, bs, hkv, d = k_cache.shape

@@ -82,6 +82,8 @@ class HostDecodePipeline:
             raise ValueError("depth must be at least 1")
         if not isinstance(backend, B200Backend):
             raise TypeError("backend must be a B200Backend")
+        if cache.k_cache.dtype == torch.float8_e4m3fn:
+            raise ValueError("HostDecodePipeline does not take 8-bit caches")
         dev = cache.k_cache.device
         _, _, _, hkv, d = cache.k_cache.shape
         hq = hkv * num_key_value_groups

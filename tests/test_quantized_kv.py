@@ -161,3 +161,13 @@ def test_every_named_barrier_of_the_tcgen05_decode_kernel_has_one_meaning():
 def test_a_layout_does_not_write_its_lengths_over_those_that_it_reads():
     apart = dict(cached=P, new=P + 4096, tables=P + 8192, lens=P + 12288)
     assert _layout(**apart | {"lens": P}) == INVALID and _layout(**apart | {"lens": P + 4096}) == INVALID
+
+
+def test_the_pipeline_and_the_step_graph_refuse_an_8_bit_cache_at_once():
+    from nano_vllm_jax_b200.engine.resident_decode import DecodeStepGraph, ResidentDecodeMetadata
+    from nano_vllm_jax_b200.host_pipeline import HostDecodePipeline
+    cache = B200Backend(device="cpu").allocate_kv_cache(kvc.KVCacheSpec(1, 4, 16, 2, 256, torch.float8_e4m3fn), 2, 2)
+    with pytest.raises(ValueError, match="8-bit"):
+        HostDecodePipeline(B200Backend(device="cpu"), cache, 2, 2, 16, 0.1, 4)
+    with pytest.raises(ValueError, match="8-bit"):
+        DecodeStepGraph(ResidentDecodeMetadata(2, 2, 16, device="cpu"), cache.k_cache, cache.v_cache, 0, 0.1, 4)
