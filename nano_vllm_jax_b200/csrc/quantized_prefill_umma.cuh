@@ -45,7 +45,7 @@ struct QtSmem {
   static constexpr int kQTerms = std::is_same<T, float>::value ? 2 : 1;
   static constexpr int kChunks = kD / 64;                 // of 64 dims: 128 bytes of f16
   static constexpr int kTileBytes = kQtKeys * kD * 2;
-  static constexpr int kFit = (232448 - 1024 - 3072 - kQTerms * kChunks * 16384) / kTileBytes;
+  static constexpr int kFit = (232448 - 1024 - 4096 - kQTerms * kChunks * 16384) / kTileBytes;
   static constexpr int kKSlots = kFit >= 3 ? 2 : 1, kVSlots = kFit >= 4 ? 2 : 1;
   alignas(1024) char q[kQTerms][kChunks][kQtRows * 128];  // [chunk][row][128 B]
   alignas(1024) char k[kKSlots][kTileBytes];              // [8-key group][chunk][8 keys][128 B]
@@ -317,7 +317,7 @@ __device__ __forceinline__ bool qt_softmax(QtSmem<T, kD>& sm, const QtParams& p,
     const int key0 = (tile0 + n) * kQtKeys + half * 32;
     const float by[2] = {factor * unit.x, factor * unit.y}, plus[2] = {qt_log(v_unit.x), qt_log(v_unit.y)};
     // scores are x * mul; the exponents of the weights that and add - reference
-    float top, most, mul[2], add[2] = {plus[0], plus[1]};  // the largest score, and the largest with its V scale
+    float top, most, mul[2], add[2] = {plus[0], plus[1]};  // the largest score with its V scale, and the largest without
     if (key0 + 32 > fewest || plus[0] == -INFINITY || plus[1] == -INFINITY || !(p.scale_log2 > 0.f)) {
       float big[2] = {-INFINITY, -INFINITY};
 #pragma unroll
@@ -691,7 +691,7 @@ static int launch_quantized_prefill_umma(QtParams p, int tiles, int most_tiles, 
   using L = QtSmem<T, kD>;
   constexpr int need = (int)sizeof(L) + 1024, bytes = need < 120 * 1024 ? 120 * 1024 : need;  // (one CTA per SM: all of its tensor memory)
   static_assert(need <= 232448, "shared memory of one CTA");
-  static_assert((int)sizeof(L) - (int)offsetof(L, k_full) <= 3072 && offsetof(L, k_full) >= kQtRows * (kD * 4 + 12), "tiles, and staged rows in their place");
+  static_assert((int)sizeof(L) - (int)offsetof(L, k_full) <= 4096 && offsetof(L, k_full) >= kQtRows * (kD * 4 + 12), "tiles, and staged rows in their place");
   auto* kernel = quantized_prefill_umma_kernel<T, kD>;
   static PerDeviceFlags ready, clusters[kQtMostSplits + 1];
   if (!once_per_device(ready, [&](int) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess; }))
