@@ -115,6 +115,8 @@ class ResidentDecodeMetadata:
     def reserve(self, pool) -> None:
         """Room for the next token of every active row out of a `device_blocks.DeviceBlockPool`: what `set_block` does for the rows that
         reach a new block, without the host knowing which.  May be captured together with the step that follows it."""
+        if pool.block_size != self.block_size:
+            raise ValueError("the pool's block size differs from the metadata's")
         pool.extend(self.block_tables, self.seq_lens, (self.seq_lens > 0).to(torch.int32), self.rows)
 
     def advance(self) -> None:

@@ -171,3 +171,10 @@ def test_the_pipeline_and_the_step_graph_refuse_an_8_bit_cache_at_once():
         HostDecodePipeline(B200Backend(device="cpu"), cache, 2, 2, 16, 0.1, 4)
     with pytest.raises(ValueError, match="8-bit"):
         DecodeStepGraph(ResidentDecodeMetadata(2, 2, 16, device="cpu"), cache.k_cache, cache.v_cache, 0, 0.1, 4)
+
+
+def test_rows_do_not_take_blocks_of_another_size():
+    from nano_vllm_jax_b200.engine.device_blocks import DeviceBlockPool
+    from nano_vllm_jax_b200.engine.resident_decode import ResidentDecodeMetadata
+    with pytest.raises(ValueError, match="block size"):
+        ResidentDecodeMetadata(2, 4, 16, device="cpu").reserve(DeviceBlockPool([1, 2], 32, device="cpu"))
