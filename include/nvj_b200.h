@@ -516,6 +516,62 @@ int nvj_paged_prefill_quantized(const void* q, int q_dtype, const void* k_cache_
                                 int token_bucket, float scale, float* out, int32_t* status, void* workspace,
                                 size_t workspace_bytes, int single_rows, int tile_pairs, nvj_stream_t stream);
 
+/* ------------------------------------------------- attention over selected blocks */
+
+/*
+ * A cache of bf16, f16 or f32 pages [num_blocks, block_size, num_kv_heads, head_dim] with the bounds of every block's keys beside it, in the
+ * cache's type: [num_blocks, num_kv_heads, 2, head_dim], the smallest number of each dim in front of the largest (no counterpart in the
+ * reference).  head_dim a multiple of 8 up to 256, otherwise NVJ_ERR_UNSUPPORTED; data pointers 16-byte aligned.
+ */
+
+/*
+ * Append of new K/V rows with the position rotation on the way: k [tokens, num_kv_heads, head_dim] of act_dtype, and q [tokens, num_q_heads,
+ * head_dim] where given, have the pairs (x[i], x[i + rotary_dim / 2]), or (x[2 i], x[2 i + 1]) if `interleaved`, turned by the angle
+ * positions[token] * inv_freq[i], i < rotary_dim / 2 (a product in 64 bits; cosine, sine and products in f32; rounded once).  Keys and
+ * v go to their place in the cache, in cache_dtype, queries to q_out [tokens, num_q_heads, head_dim] in act_dtype.  rotary_dim 0: no rotation.
+ * Strides count elements, are multiples of 16 bytes, and the head's dims are contiguous.
+ *
+ * Which tokens count and where they stand: as in nvj_kv_append_quantized (q is turned for every token).  The tokens of a call that fall into one block have to stand
+ * together in the batch; a block that two runs of tokens write in one call ends with the bounds of either, or a mixture.  k_bounds given: a block whose first token
+ * (offset 0) is among the call's begins anew, another's bounds widen; they are those of the keys as stored, NaN stays NaN.  k_bounds NULL: a plain append.
+ * A position outside the block table is flagged NVJ_DEV_BAD_LENGTH, a block id or table row outside its range NVJ_DEV_BAD_BLOCK_ID, and skipped.
+ */
+int nvj_rope_kv_append(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k, int64_t k_token_stride,
+                       int64_t k_head_stride, const void* v, int64_t v_token_stride, int64_t v_head_stride, int act_dtype,
+                       const float* inv_freq, int rotary_dim, int interleaved, const int32_t* positions,
+                       const int32_t* block_tables, const int32_t* token_row_ids, int table_rows, int table_width,
+                       const int32_t* query_start_loc, int qsl_rows, const int32_t* seq_lens, int n_rows, int n_cols,
+                       void* k_cache_layer, void* v_cache_layer, void* k_bounds, int cache_dtype, int64_t num_blocks,
+                       int block_size, int num_q_heads, int num_kv_heads, int head_dim, void* q_out, int32_t* status,
+                       nvj_stream_t stream);
+
+/*
+ * The blocks that each query token is to read: q [rows, width, num_q_heads, head_dim]; token t of row b sees the blocks with keys p < seq_lens[b]
+ * and, with positions given ([rows, width]), p <= positions[b, t].  A block's score for a kv head is the largest, over the group's query heads, of
+ *     sum_d max(q_d, 0) high_d + min(q_d, 0) low_d
+ * (with a positive scale an upper bound of its keys' scores).  Chosen are the `first` first and the `last` last blocks (first + last <= budget)
+ * and of the others those of the highest scores, ties by the lowest column, as sums in 64 bits rank them.  A score that is NaN (as with any bound that is not finite) or beyond f32 ranks as infinity; a block id outside the pool is flagged and
+ * its block ranks last.  A length beyond the block table is flagged and clipped.
+ *   selected [rows, width, num_kv_heads, budget] int32: columns of the row's block table, ascending, -1 behind them.
+ * table_width up to 49152, otherwise NVJ_ERR_TOO_LARGE.
+ */
+int nvj_select_blocks(const void* q, int q_dtype, const void* k_bounds, int cache_dtype, int64_t num_blocks, int block_size,
+                      int num_kv_heads, int head_dim, int num_q_heads, const int32_t* block_tables, int table_width,
+                      const int32_t* seq_lens, const int32_t* positions, int rows, int width, int budget, int first, int last,
+                      int32_t* selected, int32_t* status, nvj_stream_t stream);
+
+/*
+ * Attention of each query token over listed blocks: masks as above, keys those of the blocks in selected [rows, width, num_kv_heads, entries].
+ * An entry below 0, or of a block that the token does not see, adds nothing; every other counts, also one that is listed twice.
+ * out [rows, width, num_q_heads, head_dim] float32; a token without keys gets zeros.  Keys behind the last one that a token
+ * sees may hold anything.  A block id outside the pool is flagged and its keys left out.  The scale may be any number.
+ */
+int nvj_paged_decode_selected(const void* q, int q_dtype, const void* k_cache_layer, const void* v_cache_layer, int cache_dtype,
+                              int64_t num_blocks, int block_size, int num_kv_heads, int head_dim, int num_q_heads,
+                              const int32_t* block_tables, int table_width, const int32_t* seq_lens, const int32_t* positions,
+                              const int32_t* selected, int entries, int rows, int width, float scale, float* out,
+                              int32_t* status, nvj_stream_t stream);
+
 /* ------------------------------------------------------------------ copies */
 
 /*

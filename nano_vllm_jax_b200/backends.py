@@ -25,7 +25,8 @@ import torch
 from . import kv_cache as kvc
 from .kernels import paged_kv as _k
 from .kernels import quantized_kv as _q
-from .kv_cache import AttentionMetadata, KVCacheSpec, KVCacheStorage, QuantizedKVCacheStorage
+from .kernels import selective_kv as _s
+from .kv_cache import AttentionMetadata, KVCacheSpec, KVCacheStorage, QuantizedKVCacheStorage, SelectiveKVCacheStorage
 
 B200_IMPL = "b200"
 
@@ -83,6 +84,11 @@ class B200Backend:
     def allocate_kv_cache(self, spec: KVCacheSpec, max_seqs: int, max_blocks_per_seq: int) -> KVCacheStorage:
         dtype = full_attention_kv_cache_dtype(spec.dtype, self.config)
         capped = replace(spec, dtype=dtype)
+        # not in the reference: decode reads this many blocks of a row (config.full_attention_selected_blocks; 0 or None: all of them)
+        budget = getattr(self.config, "full_attention_selected_blocks", None)
+        if budget:
+            first, last = (getattr(self.config, f"full_attention_selected_{end}", 1) for end in ("first", "last"))
+            return kvc.init_selective_kv_cache(capped, budget, first, last, device=self.device)
         if dtype == torch.float8_e4m3fn:
             return kvc.init_quantized_kv_cache(capped, device=self.device)
         capped = replace(capped, num_blocks=kvc.cap_num_kv_cache_blocks(capped))
@@ -197,6 +203,8 @@ class B200Backend:
     def write_kv(self, layer_id, k, v, cache: KVCacheStorage, metadata: AttentionMetadata) -> KVCacheStorage:
         if type(cache) is QuantizedKVCacheStorage:
             return self._write_quantized(layer_id, k, v, cache, metadata)
+        if type(cache) is SelectiveKVCacheStorage:
+            return self._write_selective(layer_id, k, v, cache, metadata)
         unread = metadata.__dict__["slot_mapping"]
         if type(unread) is kvc.SlotsFromTables:
             done = _k.host().append(k, v, cache.k_cache, cache.v_cache, layer_id, None, unread.positions, unread.block_tables,
@@ -219,6 +227,8 @@ class B200Backend:
                   scale, num_key_value_groups, is_prefill):
         if type(cache) is QuantizedKVCacheStorage:
             return self._attend_quantized(layer_id, query, cache, metadata, block_size, scale, num_key_value_groups, is_prefill)
+        if type(cache) is SelectiveKVCacheStorage and not is_prefill and metadata.block_tables.shape[1] > cache.budget:
+            return self._attend_selected(layer_id, query, cache, metadata, block_size, scale, num_key_value_groups)
         f32 = torch.float32
         if is_prefill:
             if metadata.token_row_ids is not None:
@@ -260,6 +270,9 @@ class B200Backend:
         if type(cache) is QuantizedKVCacheStorage:
             self._write_quantized(layer_id, k, v, cache, metadata)
             return cache, self._attend_quantized(layer_id, query, cache, metadata, block_size, scale, num_key_value_groups, is_prefill)
+        if type(cache) is SelectiveKVCacheStorage:
+            self._write_selective(layer_id, k, v, cache, metadata)
+            return cache, self.attention(layer_id, query, cache, metadata, block_size, scale, num_key_value_groups, is_prefill)
         if not is_prefill and metadata.positions is not None:  # one token per row on the 5-D cache; anything else comes back as None
             out = _k.host().fused_decode(query, k, v, cache.k_cache, cache.v_cache, metadata.block_tables, metadata.seq_lens,
                                          metadata.positions, layer_id, block_size, scale, num_key_value_groups, 0, None, None)
@@ -314,6 +327,37 @@ class B200Backend:
                 num_key_value_groups, num_decode_rows=0)
             return out.reshape(batch, width, -1)
         return _q.paged_decode_attention_quantized(query, *layer, tables, lens, scale, positions=positions)
+
+
+    # ---- over a cache with key bounds (kernels/selective_kv.py): the append keeps them, decode reads the blocks that they select
+    def _write_selective(self, layer_id, k, v, cache: SelectiveKVCacheStorage, metadata: AttentionMetadata) -> SelectiveKVCacheStorage:
+        if metadata.positions is None:
+            raise ValueError("metadata.positions is required for an append to a selective cache")
+        i32 = torch.int32
+        ids = None if metadata.token_row_ids is None else metadata.token_row_ids.to(i32)
+        k_layer, v_layer, bounds = cache.layer(layer_id)
+        _s.rope_kv_append(None, k, v, k_layer, v_layer, metadata.positions.to(i32), metadata.block_tables.to(i32), None, k_bounds=bounds,
+                          query_start_loc=metadata.query_start_loc.to(i32), token_row_ids=ids, seq_lens=metadata.seq_lens.to(i32))
+        return cache
+
+    def _attend_selected(self, layer_id, query, cache: SelectiveKVCacheStorage, metadata: AttentionMetadata, block_size, scale,
+                         num_key_value_groups):
+        if metadata.positions is None:
+            raise ValueError("metadata.positions is required for decode attention")
+        if scale <= 0:
+            raise ValueError("a selective cache's scores are upper bounds for a positive scale only")
+        i32 = torch.int32
+        k_layer, v_layer, bounds = cache.layer(layer_id)
+        tables, lens, positions = metadata.block_tables.to(i32), metadata.seq_lens.to(i32), metadata.positions.to(i32)
+        if block_size != k_layer.shape[1] or query.shape[2] != k_layer.shape[2] * num_key_value_groups:
+            raise ValueError("query / cache shapes do not agree")
+        if positions.shape[0] != tables.shape[0]:
+            raise ValueError("positions and block_tables batch dimensions must match")
+        if metadata.max_kv_len is not None and metadata.max_kv_len < tables.shape[1] * block_size:
+            lens = lens.clamp(max=int(metadata.max_kv_len))
+        chosen = _s.select_blocks(query, bounds, tables, lens, block_size, cache.budget, positions=positions, first=cache.first,
+                                  last=cache.last)
+        return _s.paged_decode_attention_selected(query, k_layer, v_layer, tables, lens, chosen, scale, positions=positions)
 
 
 def select_backend(name: Optional[str] = None, config=None, device="cuda") -> B200Backend:

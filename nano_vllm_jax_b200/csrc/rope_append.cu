@@ -1,0 +1,426 @@
+// Append of new K/V rows to the paged cache with the position rotation on the way, and the bounds of every block's keys beside it.
+//
+//   (a, b) -> (a c - b s, b c + a s),  c = cos(pos * inv_freq[i]), s = sin(pos * inv_freq[i]),  i < rot / 2
+// for the pairs (x[i], x[i + rot/2]) of a query's or key's first `rot` dims, or (x[2i], x[2i + 1]) when they are interleaved.  The angle is a
+// product in 64 bits (31 bits of position x 24 of frequency), cosine and sine are good to fp32, the products are formed in fp32 and the
+// result is rounded once, to the type of the query or of the cache.
+// Bounds: per block and kv head the smallest and the largest stored number of each dim, low in front of high; a block that begins with
+// this call's tokens starts anew, another's widen.  NaN stays NaN.
+//
+// The unit of work for K and V is a run, as in the 8-bit append: tokens of the call that stand together and fall into one block; a warp
+// takes one run of one kv head, so that the bounds need no atomics.  Queries are dealt by token, so that a warp makes a token's cosines once for
+// several heads.  A row is held by 8, 16 or 32 lanes, 8 elements each; its pairs meet by a shuffle.  Cosines and sines go through 1 KiB of
+// shared memory per warp, each made once.
+
+#include "quantized_kv.cuh"
+#include "rotary.cuh"
+
+namespace nvj {
+
+struct RopeAppendParams {
+  const void* q;
+  const void* k;
+  const void* v;
+  long long q_token, q_head, k_token, k_head, v_token, v_head;  // strides in elements
+  void* q_out;                                                  // [tokens, hq, D]
+  void* k_cache;
+  void* v_cache;
+  void* bounds;  // nullable [num_blocks, hkv, 2, D]
+  const float* inv_freq;
+  const int32_t* positions;
+  const int32_t* block_tables;
+  const int32_t* token_row_ids;    // packed batches
+  const int32_t* query_start_loc;  // nullable
+  const int32_t* seq_lens;         // nullable: rows with seq_lens[r] <= 0 are left alone
+  int32_t* status;
+  long long num_blocks;
+  int rot, interleaved, hq, hkv, d, qsl_rows, packed, n_tokens, n_cols, table_rows, table_width, block_size;
+  int window, kv_ctas, q_ctas, item_heads;  // tokens of a CTA; grid y: CTAs of K and V runs, then of queries, `item_heads` heads of a token at a time
+};
+
+constexpr int kRaWarps = 4, kRaHold = 4;  // rows (steps of rows) that a warp has in flight
+
+__device__ __forceinline__ float ra_min(float a, float b) {
+  float y;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+__device__ __forceinline__ float ra_max(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+
+// Eight numbers in the type C, rounded to nearest even, and back.
+template <typename C>
+__device__ __forceinline__ QRaw<C> ra_pack(const float (&x)[8]) {
+  QRaw<C> r;
+  if constexpr (sizeof(C) == 4) {
+    r.v = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+    r.w = make_uint4(__float_as_uint(x[4]), __float_as_uint(x[5]), __float_as_uint(x[6]), __float_as_uint(x[7]));
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (std::is_same<C, __half>::value) {
+        w[i] = q_pair(x[2 * i], x[2 * i + 1]);
+      } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
+    r.v = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  return r;
+}
+template <typename C>
+__device__ __forceinline__ void ra_store(C* at, const QRaw<C>& r) {
+  *reinterpret_cast<uint4*>(at) = r.v;
+  if constexpr (sizeof(C) == 4) *reinterpret_cast<uint4*>(at + 4) = r.w;
+}
+
+// Cosines and sines of position `pos` by the kLanes lanes of a row, into their row's part of the warp's table.
+template <int kLanes>
+__device__ __forceinline__ void ra_angles(float2* cs, const float* inv_freq, int half, int pos, int lane) {
+  for (int f = lane % kLanes; f < half; f += kLanes) {
+    float c, s;
+    cos_sin((double)pos * (double)inv_freq[f], c, s);
+    cs[f] = make_float2(c, s);
+  }
+}
+
+// One row turned in place: x are this lane's elements col .. col + 7, `src` the row, cs its table.  All lanes of the warp are here.
+template <typename T, int kLanes>
+__device__ __forceinline__ void ra_turn(float (&x)[8], const T* src, const float2* cs, int rot, bool interleaved, int col, int lane, bool live) {
+  const int half = rot >> 1;
+  if (interleaved) {
+    if (col < rot) {
+#pragma unroll
+      for (int j = 0; j < 8; j += 2)
+        if (col + j < rot) {
+          const float2 t = cs[(col + j) >> 1];
+          const float a = x[j], b = x[j + 1];
+          x[j] = fmaf(a, t.x, -(b * t.y));
+          x[j + 1] = fmaf(b, t.x, a * t.y);
+        }
+    }
+    return;
+  }
+  float other[8];
+  if ((half & 7) == 0) {  // the partners are another lane's elements
+    const int from = (lane & ~(kLanes - 1)) + (col < half ? (col + half) >> 3 : col < rot ? (col - half) >> 3 : col >> 3);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) other[j] = __shfl_sync(kFullMask, x[j], from);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int i = col + j;
+      other[j] = live && i < rot ? (float)src[i < half ? i + half : i - half] : 0.f;
+    }
+  }
+  if (col < rot) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int i = col + j;
+      if (i < rot) {
+        const float2 t = cs[i < half ? i : i - half];
+        x[j] = fmaf(x[j], t.x, i < half ? -(other[j] * t.y) : other[j] * t.y);
+      }
+    }
+  }
+}
+
+// Table entry (row * table_width + block of the row) and block of a token, or -1 for a token that is not written.
+struct RaToken {
+  long long entry;
+  int block;
+};
+__device__ __forceinline__ RaToken ra_token(const RopeAppendParams& p, int i) {
+  RaToken t{-1, 0};
+  if (i < 0 || i >= p.n_tokens) return t;
+  const int pos = p.positions[i];
+  const int row = p.packed ? p.token_row_ids[i] : i / p.n_cols;
+  if (p.query_start_loc) {
+    if (p.packed) {
+      if (i >= p.query_start_loc[p.qsl_rows]) return t;
+    } else {
+      if (row >= p.qsl_rows || i - row * p.n_cols >= p.query_start_loc[row + 1] - p.query_start_loc[row]) return t;
+    }
+  }
+  if (row < 0 || row >= p.table_rows) {
+    atomicOr(p.status, NVJ_DEV_BAD_BLOCK_ID);
+    return t;
+  }
+  if (p.seq_lens && p.seq_lens[row] <= 0) return t;
+  const int block = pos / p.block_size;
+  if (pos < 0 || block >= p.table_width) {
+    atomicOr(p.status, NVJ_DEV_BAD_LENGTH);
+    return t;
+  }
+  t.entry = (long long)row * p.table_width + block;
+  t.block = block;
+  return t;
+}
+
+// One run of one kv head: `n` tokens from `first` on, of table entry `entry`.
+template <typename T, typename C, int kLanes>
+__device__ void ra_run(const RopeAppendParams& p, int first, int n, long long entry, int block, int head, bool is_v, float2* table, int lane) {
+  constexpr int kRows = 32 / kLanes;
+  const int sub = lane / kLanes, col = (lane % kLanes) * 8;
+  const bool inside = col < p.d;
+  const T* src = static_cast<const T*>(is_v ? p.v : p.k);
+  const long long token_stride = is_v ? p.v_token : p.k_token, at_head = head * (is_v ? p.v_head : p.k_head);
+  const int id = p.block_tables[entry];
+  const bool turned = !is_v && p.rot > 0;
+  const int half = p.rot >> 1;
+  float2* cs = table + sub * half;
+  const bool ok = id >= 0 && id < p.num_blocks;
+  if (!ok && lane == 0) atomicOr(p.status, NVJ_DEV_BAD_BLOCK_ID);
+  if (!ok) return;
+  C* base = static_cast<C*>(is_v ? p.v_cache : p.k_cache) + ((long long)id * p.block_size * p.hkv + head) * p.d + col;
+  const long long slot = (long long)p.hkv * p.d;
+  const bool bounded = !is_v && p.bounds;
+  float low[8], high[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) low[j] = INFINITY, high[j] = -INFINITY;
+  bool begins = false;
+  for (int at = 0; at < n; at += kRaHold * kRows) {
+    QRaw<T> raw[kRaHold];
+    int pos[kRaHold];
+#pragma unroll
+    for (int s = 0; s < kRaHold; ++s) {
+      const int r = at + s * kRows + sub;
+      pos[s] = 0;
+      if (r < n) {
+        pos[s] = p.positions[first + r];
+        if (inside) raw[s] = q_load8(src + (long long)(first + r) * token_stride + at_head + col);
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < kRaHold; ++s) {
+      if (at + s * kRows >= n) break;
+      const int r = at + s * kRows + sub;
+      const bool live = r < n && inside;
+      if (turned) {
+        __syncwarp();
+        if (r < n) ra_angles<kLanes>(cs, p.inv_freq, half, pos[s], lane);
+        __syncwarp();
+      }
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = 0.f;
+      if (live) q_floats(raw[s], x);
+      if (turned) ra_turn<T, kLanes>(x, src + (long long)(first + r) * token_stride + at_head, cs, p.rot, p.interleaved, col, lane, live);
+      if (live) {
+        const int o = pos[s] - block * p.block_size;
+        const QRaw<C> w = ra_pack<C>(x);
+        ra_store<C>(base + (long long)o * slot, w);
+        if (bounded) {
+          begins |= o == 0;
+          q_floats(w, x);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) low[j] = ra_min(low[j], x[j]), high[j] = ra_max(high[j], x[j]);
+        }
+      }
+    }
+  }
+  if (!bounded) return;
+  begins = __any_sync(kFullMask, begins);
+#pragma unroll
+  for (int o = kLanes; o < 32; o <<= 1)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      low[j] = ra_min(low[j], __shfl_xor_sync(kFullMask, low[j], o));
+      high[j] = ra_max(high[j], __shfl_xor_sync(kFullMask, high[j], o));
+    }
+  if (sub == 0 && inside) {
+    C* at = static_cast<C*>(p.bounds) + ((long long)id * p.hkv + head) * 2 * p.d + col;
+    if (!begins) {
+      float x[8];
+      q_floats(q_load8(at), x);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) low[j] = ra_min(low[j], x[j]);
+      q_floats(q_load8(at + p.d), x);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) high[j] = ra_max(high[j], x[j]);
+    }
+    ra_store<C>(at, ra_pack<C>(low));
+    ra_store<C>(at + p.d, ra_pack<C>(high));
+  }
+}
+
+template <typename T, typename C, int kLanes>
+__global__ void __launch_bounds__(32 * kRaWarps) rope_append_kernel(RopeAppendParams p) {
+  __shared__ float2 tables[kRaWarps][128];  // rows of a step x rot / 2 frequencies
+  constexpr int kRows = 32 / kLanes;
+  pdl_wait();
+  pdl_release();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long base = (long long)blockIdx.x * p.window;  // first token of the window
+  float2* table = tables[warp];
+  if ((int)blockIdx.y < p.kv_ctas) {
+    const int part = blockIdx.y * kRaWarps + warp, head = part >> 1;
+    if (head >= p.hkv) return;
+    // lane l looks at token base - 1 + l: the one in front tells whether the window's first token begins a run
+    const RaToken t = ra_token(p, (int)base - 1 + lane);
+    const long long in_front = __shfl_up_sync(kFullMask, t.entry, 1);
+    const bool same = lane > 0 && t.entry >= 0 && t.entry == in_front;
+    const unsigned chain = __ballot_sync(kFullMask, same);
+    unsigned starts = __ballot_sync(kFullMask, lane > 0 && lane <= p.window && t.entry >= 0 && !same);
+    for (; starts; starts &= starts - 1) {
+      const int at = __ffs(starts) - 1;  // lane of the run's first token
+      const long long entry = __shfl_sync(kFullMask, t.entry, at);
+      const int block = __shfl_sync(kFullMask, t.block, at);
+      const int first = (int)base - 1 + at;
+      const unsigned follow = at == 31 ? 0u : ~(chain >> (at + 1));  // bit j clear: token first + 1 + j is of the run
+      int n = 1 + (follow ? __ffs(follow) - 1 : 32);
+      if (at + n > 31) {  // the run may go on behind what the lanes have seen
+        n = 32 - at;
+        for (;;) {
+          const unsigned more = __ballot_sync(kFullMask, ra_token(p, first + n + lane).entry == entry);
+          const int add = more == kFullMask ? 32 : __ffs(~more) - 1;
+          n += add;
+          if (add < 32) break;
+        }
+      }
+      ra_run<T, C, kLanes>(p, first, n, entry, block, head, part & 1, table, lane);
+    }
+    return;
+  }
+  // queries: items of `item_heads` heads of a token
+  const int sub = lane / kLanes, col = (lane % kLanes) * 8, half = p.rot >> 1;
+  const bool inside = col < p.d;
+  const int chunks = (p.hq + p.item_heads - 1) / p.item_heads, items = p.window * chunks;
+  for (int item = ((int)blockIdx.y - p.kv_ctas) * kRaWarps + warp; item < items; item += p.q_ctas * kRaWarps) {
+    const long long token = base + item / chunks;
+    if (token >= p.n_tokens) break;
+    const int h0 = item % chunks * p.item_heads, h1 = min(p.hq, h0 + p.item_heads);
+    const T* src = static_cast<const T*>(p.q) + token * p.q_token;
+    T* dst = static_cast<T*>(p.q_out) + token * p.hq * p.d;
+    bool made = false;
+    for (int h = h0; h < h1; h += kRaHold * kRows) {
+      QRaw<T> raw[kRaHold];
+#pragma unroll
+      for (int s = 0; s < kRaHold; ++s) {
+        const int mine = h + s * kRows + sub;
+        if (mine < h1 && inside) raw[s] = q_load8(src + mine * p.q_head + col);
+      }
+      if (!made && half > 0) {
+        __syncwarp();
+        const int pos = p.positions[token];
+        for (int f = lane; f < half; f += 32) {
+          float c, s;
+          cos_sin((double)pos * (double)p.inv_freq[f], c, s);
+          table[f] = make_float2(c, s);
+        }
+        __syncwarp();
+        made = true;
+      }
+#pragma unroll
+      for (int s = 0; s < kRaHold; ++s) {
+        if (h + s * kRows >= h1) break;
+        const int mine = h + s * kRows + sub;
+        const bool live = mine < h1 && inside;
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = 0.f;
+        if (live) q_floats(raw[s], x);
+        if (half > 0) ra_turn<T, kLanes>(x, src + mine * p.q_head, table, p.rot, p.interleaved, col, lane, live);
+        if (live) ra_store<T>(dst + (long long)mine * p.d + col, ra_pack<T>(x));
+      }
+    }
+  }
+}
+
+template <typename T, typename C>
+static int launch_rope_append(RopeAppendParams p, cudaStream_t stream) {
+  // Batches of a few tokens per row: a token per CTA column, its heads dealt out.  Prompts: windows of 16 tokens, in which one run begins, mostly.
+  const long long rows = p.packed ? (p.query_start_loc ? p.qsl_rows : 1) : (p.n_tokens + p.n_cols - 1) / p.n_cols;
+  const bool prompt = p.n_tokens > 4 * (rows > 0 ? rows : 1);
+  const int lanes = p.d <= 64 ? 8 : p.d <= 128 ? 16 : 32;
+  p.window = prompt ? 16 : 1;
+  p.item_heads = prompt ? p.hq : 32 / lanes;
+  p.kv_ctas = (2 * p.hkv + kRaWarps - 1) / kRaWarps;
+  const int items = p.hq > 0 ? p.window * ((p.hq + p.item_heads - 1) / p.item_heads) : 0;
+  p.q_ctas = (items + kRaWarps - 1) / kRaWarps;
+  if (prompt && p.q_ctas > 2) p.q_ctas = 2;
+  const dim3 grid((unsigned)((p.n_tokens + p.window - 1LL) / p.window), p.kv_ctas + p.q_ctas);
+  auto go = [&](auto* kernel) { return launch_after(kernel, grid, dim3(32 * kRaWarps), 0, stream, p) == cudaSuccess ? NVJ_OK : NVJ_ERR_LAUNCH; };
+  if (lanes == 8) return go(rope_append_kernel<T, C, 8>);
+  if (lanes == 16) return go(rope_append_kernel<T, C, 16>);
+  return go(rope_append_kernel<T, C, 32>);
+}
+template <typename T>
+static int launch_rope_append_cache(const RopeAppendParams& p, int cache_dtype, cudaStream_t s) {
+  if (cache_dtype == NVJ_BF16) return launch_rope_append<T, __nv_bfloat16>(p, s);
+  if (cache_dtype == NVJ_F16) return launch_rope_append<T, __half>(p, s);
+  return launch_rope_append<T, float>(p, s);
+}
+
+}  // namespace nvj
+
+extern "C" int nvj_rope_kv_append(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k, int64_t k_token_stride,
+                                  int64_t k_head_stride, const void* v, int64_t v_token_stride, int64_t v_head_stride, int act_dtype,
+                                  const float* inv_freq, int rotary_dim, int interleaved, const int32_t* positions,
+                                  const int32_t* block_tables, const int32_t* token_row_ids, int table_rows, int table_width,
+                                  const int32_t* query_start_loc, int qsl_rows, const int32_t* seq_lens, int n_rows, int n_cols,
+                                  void* k_cache_layer, void* v_cache_layer, void* k_bounds, int cache_dtype, int64_t num_blocks,
+                                  int block_size, int num_q_heads, int num_kv_heads, int head_dim, void* q_out, int32_t* status,
+                                  nvj_stream_t stream) {
+  using namespace nvj;
+  if (n_rows < 0 || n_cols < 0 || table_rows < 0 || table_width < 0 || qsl_rows < 0 || num_blocks < 0 || num_q_heads < 0 || num_kv_heads < 1 ||
+      block_size < 1 || rotary_dim < 0 || rotary_dim > head_dim || (rotary_dim & 1))
+    return NVJ_ERR_INVALID_ARGUMENT;
+  if (act_dtype < NVJ_BF16 || act_dtype > NVJ_F32 || cache_dtype < NVJ_BF16 || cache_dtype > NVJ_F32 || head_dim < 8 || head_dim > 256 ||
+      head_dim % 8 != 0 || num_kv_heads > 1024 || num_q_heads > 65536)
+    return NVJ_ERR_UNSUPPORTED;
+  const long long n = (long long)n_rows * n_cols;
+  if (n == 0) return NVJ_OK;
+  if (n > 0x7fffffffLL - 64) return NVJ_ERR_TOO_LARGE;
+  if (!k || !v || !positions || !block_tables || !k_cache_layer || !v_cache_layer || !status || (q && !q_out) || (rotary_dim > 0 && !inv_freq))
+    return NVJ_ERR_INVALID_ARGUMENT;
+  if (table_rows == 0 || table_width == 0 || num_blocks == 0) return NVJ_ERR_INVALID_ARGUMENT;
+  if (token_row_ids && n_rows != 1) return NVJ_ERR_INVALID_ARGUMENT;
+  const bool placed = aligned16(q) && aligned16(k) && aligned16(v) && aligned16(k_cache_layer) && aligned16(v_cache_layer) && aligned16(k_bounds) &&
+                      aligned16(q_out);
+  const int64_t strides = q_token_stride | q_head_stride | k_token_stride | k_head_stride | v_token_stride | v_head_stride;
+  if (!placed || (strides & (act_dtype == NVJ_F32 ? 3 : 7)) != 0) return NVJ_ERR_INVALID_ARGUMENT;
+  RopeAppendParams p{};
+  p.q = q;
+  p.k = k;
+  p.v = v;
+  p.q_token = q_token_stride;
+  p.q_head = q_head_stride;
+  p.k_token = k_token_stride;
+  p.k_head = k_head_stride;
+  p.v_token = v_token_stride;
+  p.v_head = v_head_stride;
+  p.q_out = q_out;
+  p.k_cache = k_cache_layer;
+  p.v_cache = v_cache_layer;
+  p.bounds = k_bounds;
+  p.inv_freq = inv_freq;
+  p.positions = positions;
+  p.block_tables = block_tables;
+  p.token_row_ids = token_row_ids;
+  p.query_start_loc = query_start_loc;
+  p.seq_lens = seq_lens;
+  p.status = status;
+  p.num_blocks = num_blocks;
+  p.rot = rotary_dim;
+  p.interleaved = interleaved;
+  p.hq = q ? num_q_heads : 0;
+  p.hkv = num_kv_heads;
+  p.d = head_dim;
+  p.qsl_rows = qsl_rows;
+  p.packed = token_row_ids != nullptr;
+  p.n_tokens = (int)n;
+  p.n_cols = n_cols;
+  p.table_rows = table_rows;
+  p.table_width = table_width;
+  p.block_size = block_size;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (act_dtype == NVJ_BF16) return launch_rope_append_cache<__nv_bfloat16>(p, cache_dtype, s);
+  if (act_dtype == NVJ_F16) return launch_rope_append_cache<__half>(p, cache_dtype, s);
+  return launch_rope_append_cache<float>(p, cache_dtype, s);
+}

@@ -41,7 +41,7 @@ import torch
 from . import _lib
 from .backends import B200Backend
 from .kernels import paged_kv as _k
-from .kv_cache import KVCacheStorage
+from .kv_cache import KVCacheStorage, SelectiveKVCacheStorage
 
 
 @dataclass
@@ -84,6 +84,8 @@ class HostDecodePipeline:
             raise TypeError("backend must be a B200Backend")
         if cache.k_cache.dtype == torch.float8_e4m3fn:
             raise ValueError("HostDecodePipeline does not take 8-bit caches")
+        if isinstance(cache, SelectiveKVCacheStorage):
+            raise ValueError("HostDecodePipeline does not take selective caches (its append keeps no key bounds)")
         dev = cache.k_cache.device
         _, _, _, hkv, d = cache.k_cache.shape
         hq = hkv * num_key_value_groups

@@ -61,6 +61,30 @@ class QuantizedKVCacheStorage(KVCacheStorage):
 
 
 @dataclass
+class SelectiveKVCacheStorage(KVCacheStorage):
+    """A cache whose decode attention reads selected blocks (not in the reference): beside the pages `[num_layers, num_blocks, block_size,
+    num_kv_heads, head_dim]` the bounds of every block's keys `[num_layers, num_blocks, num_kv_heads, 2, head_dim]` (the smallest
+    number of each dimension, then the largest), kept by the append.  Of a row's blocks decode reads the `first` first, the `last`
+    last and those of the highest scores, `budget` in all (`kernels/selective_kv.py`); prefill reads all of them."""
+
+    k_bounds: torch.Tensor
+    budget: int
+    first: int = 1
+    last: int = 1
+
+    def layer(self, layer_id: int):
+        """(k, v, k_bounds) of one layer, as the kernels of `kernels/selective_kv.py` take them."""
+        if self.k_cache.ndim != 5:
+            raise ValueError("a selective cache has rank 5 [L, NB, bs, Hkv, D]")
+        return tuple(_resolve_kv_layer(t, layer_id)[0] for t in (self.k_cache, self.v_cache, self.k_bounds))
+
+    def copy_blocks(self, src_ids, dst_ids) -> None:
+        """Blocks `dst_ids` <- `src_ids` in every layer, their bounds with them (src and dst sets disjoint)."""
+        _k.copy_blocks(self.k_cache, self.v_cache, src_ids, dst_ids)
+        self.k_bounds[:, dst_ids.long()] = self.k_bounds[:, src_ids.long()]
+
+
+@dataclass
 class AttentionMetadata:
     """Per-step paged/ragged attention metadata (kv_cache.py:51-64).
 
@@ -223,6 +247,26 @@ def init_quantized_kv_cache(spec: KVCacheSpec, device="cuda") -> QuantizedKVCach
     scales = (spec.num_layers, nb, spec.num_kv_heads)
     numbers = [torch.zeros(shape, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn) for _ in range(2)]
     return QuantizedKVCacheStorage(*numbers, *[torch.full(scales, 2.0 ** -117, dtype=torch.float32, device=device) for _ in range(2)])
+
+
+def init_selective_kv_cache(spec: KVCacheSpec, budget: int, first: int = 1, last: int = 1, device="cuda") -> SelectiveKVCacheStorage:
+    """Zero-filled cache with key bounds of as many blocks as `spec` allows; decode reads `budget` blocks of a row."""
+    from .kernels.selective_kv import check_budget, selective_cache_supported
+    if not selective_cache_supported(spec.dtype, spec.head_dim):
+        raise ValueError(f"a selective cache has dtype bfloat16, float16 or float32 and a head_dim that is a multiple of 8 up to 256, not "
+                         f"{spec.dtype} and {spec.head_dim}")
+    check_budget(budget, first, last)
+    nb = spec.num_blocks
+    if spec.max_kv_cache_bytes is not None:
+        bounds = spec.num_layers * spec.num_kv_heads * 2 * spec.head_dim * _itemsize(spec.dtype)
+        per_block = estimate_kv_cache_bytes(replace(spec, num_blocks=1)) + bounds
+        if spec.max_kv_cache_bytes < per_block:
+            raise ValueError(f"max_kv_cache_bytes is too small for one KV block ({spec.max_kv_cache_bytes} < {per_block})")
+        nb = min(nb, spec.max_kv_cache_bytes // per_block)
+    shape = (spec.num_layers, nb, spec.block_size, spec.num_kv_heads, spec.head_dim)
+    pages = [torch.zeros(shape, dtype=spec.dtype, device=device) for _ in range(2)]
+    bounds = torch.zeros((spec.num_layers, nb, spec.num_kv_heads, 2, spec.head_dim), dtype=spec.dtype, device=device)
+    return SelectiveKVCacheStorage(*pages, bounds, int(budget), int(first), int(last))
 
 
 def init_hybrid_state(config, batch_size: int = 1, dtype=None, device="cuda") -> HybridLayerState:
