@@ -553,7 +553,7 @@ int nvj_rope_kv_append(const void* q, int64_t q_token_stride, int64_t q_head_str
  * and of the others those of the highest scores, ties by the lowest column, as sums in 64 bits rank them.  A score that is NaN (as with any bound that is not finite) or beyond f32 ranks as infinity; a block id outside the pool is flagged and
  * its block ranks last.  A length beyond the block table is flagged and clipped.
  *   selected [rows, width, num_kv_heads, budget] int32: columns of the row's block table, ascending, -1 behind them.
- * table_width up to 49152, otherwise NVJ_ERR_TOO_LARGE.
+ * table_width up to 45056, otherwise NVJ_ERR_TOO_LARGE.
  */
 int nvj_select_blocks(const void* q, int q_dtype, const void* k_bounds, int cache_dtype, int64_t num_blocks, int block_size,
                       int num_kv_heads, int head_dim, int num_q_heads, const int32_t* block_tables, int table_width,

@@ -15,6 +15,7 @@
 // No workspace, no second launch.  Bound by the bytes of the bounds, 2 head_dim numbers per block and kv head: 1/block_size of the cache.
 
 #include "cluster.cuh"
+#include "decode_cluster.cuh"
 #include "quantized_kv.cuh"
 
 namespace nvj {
@@ -34,7 +35,7 @@ struct SelectParams {
 
 constexpr int kBsWarps = 8, kBsThreads = 32 * kBsWarps;
 constexpr int kBsBins = 2048;
-constexpr int kBsMostColumns = 49152;  // of a row: their scores fit one SM's shared memory
+constexpr int kBsMostColumns = 45056;  // of a row: their scores fit one SM's shared memory, beside the queries
 constexpr int kBsMostCtas = 16;
 constexpr uint32_t kBsInfinity = 0xff800000u;  // bs_key(+infinity)
 
@@ -164,6 +165,13 @@ __device__ __forceinline__ void bs_rescore(const SelectParams& p, BsShared& s, c
   }
 }
 
+// The larger of two, NaN if either is.
+__device__ __forceinline__ float bs_larger(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+
 // Scores of up to 16 blocks by a warp, for any type and head_dim: a block at a time, the dims over the lanes.
 __device__ void bs_score_any(const SelectParams& p, long long q_at, const int32_t* table, int head, int c0, int n, uint32_t keys_at, float& most,
                              int lane) {
@@ -186,7 +194,7 @@ __device__ void bs_score_any(const SelectParams& p, long long q_at, const int32_
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kFullMask, sum, o);
-        if (!(sum <= best) && best == best) best = sum;  // (NaN stays)
+        best = bs_larger(best, sum);
       }
     }
 #pragma unroll
@@ -196,7 +204,151 @@ __device__ void bs_score_any(const SelectParams& p, long long q_at, const int32_
   }
 }
 
-__global__ void __launch_bounds__(kBsThreads) block_select_kernel(SelectParams p, int ctas) {
+// The same on tensor-core tiles, for head_dim 64, 128 and 256 and up to 16 query heads of a kv head: the blocks are the rows of an mma.sync tile, the heads its
+// columns, and the contraction runs over the 2 D bounds, the positive parts of the queries standing against the high ones, the negative parts against the low.
+// A lane's 16 bytes of a block's bounds are its operands as they come (selected_decode.cuh); 128 dims of 16 blocks are under way in
+// registers, and each piece is asked for again as soon as it has been used.
+template <typename C, int kD, int kTiles, int kTerms>
+struct BsTiles {
+  static constexpr int kPitch = kD + 8;
+  static constexpr int kHalves = kD > 128 ? kD / 128 : 1, kPieces = kD / 32 / kHalves;
+  static constexpr int kQBytes = kTerms * 2 * 8 * kTiles * kPitch * 2;  // [term][sign][column][pitch]
+
+  // The queries' parts into shared memory.
+  static __device__ void stage(const SelectParams& p, long long q_at, C* qs) {
+    for (int i = threadIdx.x; i < 8 * kTiles * kD; i += kBsThreads) {
+      const int col = i / kD, d = i % kD;
+      float x = col < p.groups ? bs_load(p.q, q_at + (long long)col * kD + d, p.q_dtype) : 0.f;
+      const bool negative = x < 0.f;
+#pragma unroll
+      for (int term = 0; term < kTerms; ++term) {
+        C h;
+        if constexpr (std::is_same<C, __half>::value) h = __float2half_rn(x);
+        else h = kTerms > 1 ? __float2bfloat16_rz(x) : __float2bfloat16_rn(x);  // (cut: the largest f32 numbers stay finite)
+        x -= (float)h;
+        qs[((term * 2 + (negative ? 1 : 0)) * 8 * kTiles + col) * kPitch + d] = h;
+        qs[((term * 2 + (negative ? 0 : 1)) * 8 * kTiles + col) * kPitch + d] = C(0.f);
+      }
+    }
+  }
+
+  uint4 held[kPieces][2][2];  // [piece][low, high][row g, row g + 8]
+  const C* at[2];             // bounds of rows g and g + 8, this lane's dims; null: no block there
+  int id;                     // of column tile + lane, the tile behind the one in the registers
+
+  __device__ void fetch_id(const int32_t* table, int c0, int n, int lane) { id = lane < 16 && c0 + lane < n ? table[c0 + lane] : -1; }
+  // places of the tile whose ids are there; flags those outside the pool
+  __device__ void take(const SelectParams& p, int head, int c0, int n, int lane) {
+    const bool used = lane < 16 && c0 + lane < n;
+    if (used && (id < 0 || id >= p.num_blocks)) {
+      atomicOr(p.status, NVJ_DEV_BAD_BLOCK_ID);
+      id = -1;
+    }
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int mine = __shfl_sync(kFullMask, id, (lane >> 2) + 8 * r);
+      at[r] = mine < 0 ? nullptr : static_cast<const C*>(p.bounds) + ((long long)mine * p.hkv + head) * 2 * kD + 8 * (lane & 3);
+    }
+  }
+  __device__ void ask(int piece, int half) {
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        held[piece][b][r] = make_uint4(0, 0, 0, 0);
+        if (at[r]) held[piece][b][r] = ld_stream_u4(at[r] + b * kD + 32 * (half * kPieces + piece));
+      }
+  }
+  static __device__ __forceinline__ void widen(uint32_t& m, const uint4& v) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (std::is_same<C, __half>::value) {
+        const __half2 x = __hmax2(*reinterpret_cast<const __half2*>(&m), __habs2(*reinterpret_cast<const __half2*>(&w[i])));
+        m = *reinterpret_cast<const uint32_t*>(&x);
+      } else {
+        const __nv_bfloat162 x = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&m), __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[i])));
+        m = *reinterpret_cast<const uint32_t*>(&x);
+      }
+    }
+  }
+  static __device__ __forceinline__ float larger(uint32_t m) {
+    float2 f;
+    if constexpr (std::is_same<C, __half>::value) f = q_float2(m);
+    else f = bf16x2_to_float2(m);
+    return fmaxf(f.x, f.y);
+  }
+
+  // All tiles from c0 on, `stride` columns apart.
+  __device__ void run(const SelectParams& p, const C* qs, const int32_t* table, int head, int c0, int stride, int n, uint32_t keys_at, float& most, int lane) {
+    const int g = lane >> 2, t = lane & 3;
+    float acc[kTiles][2][4];
+    uint32_t large[2];
+    bool there[2];
+    while (c0 < n) {
+      const int next = c0 + stride;
+#pragma unroll
+      for (int j = 0; j < kTiles; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[j][0][i] = acc[j][1][i] = 0.f;
+      large[0] = large[1] = 0u;
+      there[0] = at[0] != nullptr;
+      there[1] = at[1] != nullptr;
+#pragma unroll
+      for (int half = 0; half < kHalves; ++half) {
+        if (half == kHalves - 1) {  // what is asked for from here on is the next tile's
+          take(p, head, next, n, lane);
+          fetch_id(table, next + stride, n, lane);
+        }
+#pragma unroll
+        for (int piece = 0; piece < kPieces; ++piece) {
+          const uint4 low0 = held[piece][0][0], low1 = held[piece][0][1], high0 = held[piece][1][0], high1 = held[piece][1][1];
+          widen(large[0], low0);
+          widen(large[0], high0);
+          widen(large[1], low1);
+          widen(large[1], high1);
+#pragma unroll
+          for (int j = 0; j < kTiles; ++j)
+#pragma unroll
+            for (int term = 0; term < kTerms; ++term) {
+              const C* q = qs + ((term * 2 * kTiles + j) * 8 + g) * kPitch + 32 * (half * kPieces + piece) + 8 * t;
+              const uint4 up = *reinterpret_cast<const uint4*>(q), down = *reinterpret_cast<const uint4*>(q + 8 * kTiles * kPitch);
+              cm_mma<C>(acc[j][0], {high0.x, high1.x, high0.y, high1.y}, up.x, up.y);
+              cm_mma<C>(acc[j][1], {low0.x, low1.x, low0.y, low1.y}, down.x, down.y);
+              cm_mma<C>(acc[j][0], {high0.z, high1.z, high0.w, high1.w}, up.z, up.w);
+              cm_mma<C>(acc[j][1], {low0.z, low1.z, low0.w, low1.w}, down.z, down.w);
+            }
+          ask(piece, half == kHalves - 1 ? 0 : half + 1);
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float best = -INFINITY, m = larger(large[r]);
+#pragma unroll
+        for (int j = 0; j < kTiles; ++j)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            if (8 * j + 2 * t + i < p.groups) best = bs_larger(best, acc[j][0][2 * r + i] + acc[j][1][2 * r + i]);
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) {
+          best = bs_larger(best, __shfl_xor_sync(kFullMask, best, o));
+          m = fmaxf(m, __shfl_xor_sync(kFullMask, m, o));
+        }
+        if (!there[r]) best = -INFINITY;
+        if (best - best == 0.f) most = fmaxf(most, m);
+        const int c = c0 + g + 8 * r;
+        if (t == 0 && c < n) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(keys_at + 4 * c), "r"(bs_key(best)) : "memory");
+      }
+      c0 = next;
+    }
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) most = fmaxf(most, __shfl_xor_sync(kFullMask, most, o));
+  }
+};
+
+// kD 0: any type and layout.
+template <typename C, int kD, int kTiles, int kTerms>
+__global__ void __launch_bounds__(kBsThreads, 2) block_select_kernel(SelectParams p, int ctas) {
   extern __shared__ __align__(16) uint32_t keys[];
   __shared__ BsShared s;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -237,8 +389,22 @@ __global__ void __launch_bounds__(kBsThreads) block_select_kernel(SelectParams p
     if (lane == 0) s.norm[warp] = mine;
   }
   float most = 0.f;
-  for (int c = (rank * kBsWarps + warp) * 16; c < n; c += ctas * kBsWarps * 16)
-    bs_score_any(p, q_at, table, head, c, n, keys_at, most, lane);
+  const int c0 = (rank * kBsWarps + warp) * 16, stride = ctas * kBsWarps * 16;
+  if constexpr (kD > 0) {
+    using Tiles = BsTiles<C, kD, kTiles, kTerms>;
+    __shared__ __align__(16) C qs[Tiles::kQBytes / 2];
+    Tiles tiles;
+    tiles.fetch_id(table, c0, n, lane);
+    tiles.take(p, head, c0, n, lane);
+#pragma unroll
+    for (int piece = 0; piece < Tiles::kPieces; ++piece) tiles.ask(piece, 0);
+    tiles.fetch_id(table, c0 + stride, n, lane);
+    Tiles::stage(p, q_at, qs);
+    __syncthreads();
+    tiles.run(p, qs, table, head, c0, stride, n, keys_at, most, lane);
+  } else {
+    for (int c = c0; c < n; c += stride) bs_score_any(p, q_at, table, head, c, n, keys_at, most, lane);
+  }
   if (lane == 0) {
     const uint32_t at = (ctas > 1 ? cl_map(s.most, 0) : smem_u32(s.most)) + 4 * (rank * kBsWarps + warp);
     asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(most) : "memory");
@@ -264,8 +430,10 @@ __global__ void __launch_bounds__(kBsThreads) block_select_kernel(SelectParams p
       for (int w = 0; w < kBsWarps; ++w) norm = s.norm[w] > norm ? s.norm[w] : norm;
       for (int w = 0; w < ctas * kBsWarps; ++w) large = fmaxf(large, s.most[w]);
       // 2 D products, their sums in trees or rows of fp32: at most 2 D roundings of 2^-24 (chains of fused multiply-adds), or D / 8 steps of the
-      // tensor cores that cut 17 numbers at 2^-23 of the largest: 2.2 D * 2^-23
-      const double eps = p.d * (3.0 * 0x1p-23 * norm * (double)large + 0x1p-124);  // (and products below the normal numbers, taken for zero)
+      // tensor cores that cut 17 numbers at 2^-23 of the largest, 2.2 D * 2^-23, for each term of the queries; two terms leave 2^-16 of a query at most
+      constexpr double kSlip = kTerms > 1 ? 0x1p-16 : 0.0;
+      const double eps = (3.0 * kTerms * 0x1p-23 * p.d + kSlip) * norm * (double)large +
+                         0x1p-124 * (p.d + norm + p.d * (double)large);  // (and numbers below the normal ones, that may be taken for zero)
       const double low = (double)t - 2.0 * eps, high = (double)t + 2.0 * eps;
       // how many are in for sure, and how many stand between
       uint32_t in = 0, between = 0;
@@ -366,11 +534,12 @@ static int block_select_ctas(long long units, long long columns, int sms) {
   return (int)(c < 1 ? 1 : (c > 8 ? 8 : c));
 }
 
+template <typename C, int kD, int kTiles, int kTerms>
 static int launch_block_select(const SelectParams& p, cudaStream_t stream) {
+  auto* kernel = block_select_kernel<C, kD, kTiles, kTerms>;
   static PerDeviceFlags ready;
-  constexpr int kMostBytes = kBsMostColumns * 4;
-  if (!once_per_device(ready, [](int) {
-        return cudaFuncSetAttribute(block_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostBytes) == cudaSuccess;
+  if (!once_per_device(ready, [&](int) {
+        return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBsMostColumns * 4) == cudaSuccess;
       }))
     return NVJ_ERR_LAUNCH;
   const long long tokens = (long long)p.rows * p.width;
@@ -390,7 +559,27 @@ static int launch_block_select(const SelectParams& p, cudaStream_t stream) {
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = ctas > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, block_select_kernel, p, ctas) == cudaSuccess ? NVJ_OK : NVJ_ERR_LAUNCH;
+  return cudaLaunchKernelEx(&cfg, kernel, p, ctas) == cudaSuccess ? NVJ_OK : NVJ_ERR_LAUNCH;
+}
+template <typename C, int kD, int kTerms>
+static int launch_block_select_heads(const SelectParams& p, cudaStream_t stream) {
+  return p.groups <= 8 ? launch_block_select<C, kD, 1, kTerms>(p, stream) : launch_block_select<C, kD, 2, kTerms>(p, stream);
+}
+template <typename C, int kTerms>
+static int launch_block_select_dims(const SelectParams& p, cudaStream_t stream) {
+  if (p.d == 256) return launch_block_select_heads<C, 256, kTerms>(p, stream);
+  if (p.d == 128) return launch_block_select_heads<C, 128, kTerms>(p, stream);
+  return launch_block_select_heads<C, 64, kTerms>(p, stream);
+}
+// Tensor-core tiles where bounds and queries are exact in terms of the cache's type: all queries over bf16 bounds (f16's and f32's as two
+// terms), f16 ones over f16.
+static int launch_block_select_any(const SelectParams& p, cudaStream_t stream) {
+  if ((p.d == 64 || p.d == 128 || p.d == 256) && p.groups <= 16) {
+    if (p.cache_dtype == NVJ_BF16)
+      return p.q_dtype == NVJ_BF16 ? launch_block_select_dims<__nv_bfloat16, 1>(p, stream) : launch_block_select_dims<__nv_bfloat16, 2>(p, stream);
+    if (p.cache_dtype == NVJ_F16 && p.q_dtype == NVJ_F16) return launch_block_select_dims<__half, 1>(p, stream);
+  }
+  return launch_block_select<float, 0, 1, 1>(p, stream);
 }
 
 }  // namespace nvj
@@ -432,5 +621,5 @@ extern "C" int nvj_select_blocks(const void* q, int q_dtype, const void* k_bound
   p.budget = budget;
   p.first = first;
   p.last = last;
-  return launch_block_select(p, static_cast<cudaStream_t>(stream));
+  return launch_block_select_any(p, static_cast<cudaStream_t>(stream));
 }

@@ -1,27 +1,8 @@
-// Decode attention over selected blocks of a row.
-//
-//   out[t, h] = sum_p w_p v_p / sum_p w_p,  w_p = exp(scale * q[t, h] . k_p),  p in the blocks that selected[t, kv head] lists, p < len, p <= position[t]
-//
-// A list holds columns of the row's block table, -1 where it has ended; every entry counts, also one that is there twice.
+// Decode attention over selected blocks (selected_decode.cuh): the form for any type and head layout, and the C entry.
 
-#include "quantized_kv.cuh"
+#include "selected_decode.cuh"
 
 namespace nvj {
-
-struct SelectedParams {
-  const void* q;
-  const void* k_cache;
-  const void* v_cache;
-  const int32_t* block_tables;
-  const int32_t* seq_lens;
-  const int32_t* positions;  // nullable [rows, width]
-  const int32_t* selected;   // [rows, width, hkv, entries]
-  float* out;
-  int32_t* status;
-  long long num_blocks;
-  int q_dtype, rows, width, table_width, block_size, hkv, groups, d, entries;
-  float scale_log2;  // scale * log2(e)
-};
 
 __device__ __forceinline__ float sd_float(const void* p, long long i, int dtype) {
   if (dtype == NVJ_F32) return static_cast<const float*>(p)[i];
@@ -29,19 +10,8 @@ __device__ __forceinline__ float sd_float(const void* p, long long i, int dtype)
   return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
 }
 
-// Keys that a token of row `row` sees.
-__device__ __forceinline__ int sd_visible(const SelectedParams& p, int row, int token) {
-  int len = p.seq_lens[row];
-  if (len > (long long)p.table_width * p.block_size) {
-    if (threadIdx.x == 0) atomicOr(p.status, NVJ_DEV_BAD_LENGTH);
-    len = p.table_width * p.block_size;
-  }
-  return p.positions ? min(len - 1, p.positions[token]) + 1 : len;
-}
-
 // Any type and head layout: on the CUDA cores, a warp per entry and key, the dims over the lanes, four heads at a time.
 constexpr int kSgWarps = 4, kSgHeads = 4, kSgEach = 8;
-constexpr float kSdNone = -3e38f;  // a maximum that no score has touched
 template <typename C>
 __global__ void __launch_bounds__(32 * kSgWarps) selected_decode_generic_kernel(SelectedParams p) {
   __shared__ float sums[kSgWarps][kSgHeads][256];
@@ -176,6 +146,9 @@ extern "C" int nvj_paged_decode_selected(const void* q, int q_dtype, const void*
   p.entries = entries;
   p.scale_log2 = scale * 1.4426950408889634f;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool tiled = (head_dim == 64 || head_dim == 128 || head_dim == 256) && block_size % 16 == 0;
+  if (tiled && cache_dtype == NVJ_BF16) return launch_selected_bf16(p, s);
+  if (tiled && cache_dtype == NVJ_F16) return launch_selected_f16(p, s);
   if (cache_dtype == NVJ_BF16) return launch_selected_generic<__nv_bfloat16>(p, s);
   if (cache_dtype == NVJ_F16) return launch_selected_generic<__half>(p, s);
   return launch_selected_generic<float>(p, s);

@@ -21,7 +21,7 @@ from .._lib import check
 from . import paged_kv as _k
 from .quantized_kv import _ints, _on, _rows
 
-MOST_COLUMNS = 49152  # block-table columns that a selection takes (nvj_select_blocks)
+MOST_COLUMNS = 45056  # block-table columns that a selection takes (nvj_select_blocks)
 
 
 def selective_cache_supported(dtype, head_dim: int) -> bool:
