@@ -271,6 +271,12 @@ class B200Backend:
             self._write_quantized(layer_id, k, v, cache, metadata)
             return cache, self._attend_quantized(layer_id, query, cache, metadata, block_size, scale, num_key_value_groups, is_prefill)
         if type(cache) is SelectiveKVCacheStorage:
+            if not is_prefill and metadata.token_row_ids is None and metadata.positions is not None:
+                out = _k.host().selective_step(query, k, v, cache.k_cache, cache.v_cache, cache.k_bounds, layer_id, metadata.block_tables,
+                                               metadata.seq_lens, metadata.positions, metadata.query_start_loc, block_size, scale,
+                                               num_key_value_groups, cache.budget, cache.first, cache.last, metadata.max_kv_len)
+                if out is not None:
+                    return cache, out
             self._write_selective(layer_id, k, v, cache, metadata)
             return cache, self.attention(layer_id, query, cache, metadata, block_size, scale, num_key_value_groups, is_prefill)
         if not is_prefill and metadata.positions is not None:  # one token per row on the 5-D cache; anything else comes back as None

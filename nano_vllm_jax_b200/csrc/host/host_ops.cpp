@@ -54,6 +54,9 @@ struct Library {
   decltype(&nvj_paged_prefill_quantized) quantized_prefill;
   decltype(&nvj_paged_prefill_quantized_workspace_bytes) quantized_prefill_bytes;
   decltype(&nvj_build_packed_layout) packed_layout;
+  decltype(&nvj_rope_kv_append) rope_append;
+  decltype(&nvj_select_blocks) select_blocks;
+  decltype(&nvj_paged_decode_selected) selected_decode;
 };
 Library lib;
 PyObject* cb_workspace;  // (device index, rows): makes Python create the workspace and hand it over
@@ -741,6 +744,232 @@ PyObject* prefill_slots(PyObject* const* a, Py_ssize_t n) {
   return Py_BuildValue("NLL", THPVariable_Wrap(std::move(out)), (long long)pos->size(0), (long long)pos->size(1));
 }
 
+// ---- attention over selected blocks -----------------------------------------------------------------------------------
+// One layer [NB, bs, Hkv, D] of K and V in a 16- or 32-bit type, with bounds [NB, Hkv, 2, D] where they are given.
+struct SelectiveLayer {
+  bool ok = false;
+  int device, dtype, block_size, hkv, d;
+  long long blocks;
+  char *k, *v, *bounds = nullptr;
+};
+bool selective_dims(long long d) { return d >= 8 && d <= 256 && d % 8 == 0; }
+SelectiveLayer selective_layer(const at::Tensor* k, const at::Tensor* v) {
+  SelectiveLayer l;
+  if (!k || !v || !k->is_cuda() || k->dim() != 4 || v->sizes() != k->sizes() || v->dtype() != k->dtype() || !on(*v, k->get_device()) ||
+      !k->is_contiguous() || !v->is_contiguous() || !aligned(*k) || !aligned(*v) || !selective_dims(k->size(3)) || k->size(2) < 1 || k->size(1) < 1)
+    return l;
+  l.device = k->get_device();
+  l.dtype = dtype_code(*k);
+  l.blocks = k->size(0);
+  l.block_size = (int)k->size(1);
+  l.hkv = (int)k->size(2);
+  l.d = (int)k->size(3);
+  l.k = static_cast<char*>(k->data_ptr());
+  l.v = static_cast<char*>(v->data_ptr());
+  l.ok = l.dtype >= 0;
+  return l;
+}
+// Rows [rows, cols, heads, d] as the append reads them: evenly spaced tokens and heads, whole 16-byte pieces.
+struct RopeRows {
+  const void* data = nullptr;
+  long long token = 0, head = 0;
+};
+bool rope_rows(const at::Tensor& t, int device, RopeRows* r) {
+  const long long rows = t.size(0), cols = t.size(1), heads = t.size(2), d = t.size(3), unit = 16 / (long long)t.element_size();
+  if (!on(t, device) || !aligned(t) || t.stride(3) != 1 || (rows > 1 && cols > 1 && t.stride(0) != t.stride(1) * cols)) return false;
+  r->data = t.data_ptr();
+  r->token = cols > 1 ? t.stride(1) : rows > 1 ? t.stride(0) : heads * d;
+  r->head = heads > 1 ? t.stride(2) : d;
+  return r->token % unit == 0 && r->head % unit == 0 && r->token >= 0 && r->head >= 0;
+}
+// new rows against a layer: one shape and dtype, the layer's heads
+bool new_rows(const at::Tensor* k, const at::Tensor* v, const SelectiveLayer& l) {
+  return k && v && k->dim() == 4 && k->sizes() == v->sizes() && k->dtype() == v->dtype() && dtype_code(*k) >= 0 && k->size(2) == l.hkv &&
+         k->size(3) == l.d && k->size(0) * k->size(1) > 0;
+}
+
+// rope_append(query | None, k, v, k_layer, v_layer, positions, block_table, inv_freq | None, k_bounds | None, query_start_loc | None,
+//             token_row_ids | None, seq_lens | None, interleaved) -> the rotated queries, or True without queries
+PyObject* rope_append(PyObject* const* a, Py_ssize_t n) {
+  if (!args_are(n, 13)) return nullptr;
+  const at::Tensor *q = a[0] == Py_None ? nullptr : tensor(a[0]), *k = tensor(a[1]), *v = tensor(a[2]), *pos = tensor(a[5]), *tab = tensor(a[6]);
+  const at::Tensor *inv = a[7] == Py_None ? nullptr : tensor(a[7]), *bounds = a[8] == Py_None ? nullptr : tensor(a[8]);
+  const at::Tensor* extra[3];  // query_start_loc, token_row_ids, seq_lens
+  const SelectiveLayer l = selective_layer(tensor(a[3]), tensor(a[4]));
+  const int interleaved = PyObject_IsTrue(a[12]);
+  if (interleaved < 0) { PyErr_Clear(); NVJ_NONE(); }
+  if (!l.ok || !new_rows(k, v, l) || !pos || !tab || (!q && a[0] != Py_None) || (!inv && a[7] != Py_None) || (!bounds && a[8] != Py_None)) NVJ_NONE();
+  for (int i = 0; i < 3; ++i) {
+    extra[i] = a[9 + i] == Py_None ? nullptr : tensor(a[9 + i]);
+    if (a[9 + i] != Py_None && (!extra[i] || !meta(*extra[i], l.device))) NVJ_NONE();
+  }
+  const long long rows = k->size(0), cols = k->size(1);
+  const bool packed = extra[1] != nullptr;
+  RopeRows rq, rk, rv;
+  if (!rope_rows(*k, l.device, &rk) || !rope_rows(*v, l.device, &rv) || !meta(*pos, l.device) || !meta(*tab, l.device) || pos->dim() != 2 ||
+      pos->size(0) != rows || pos->size(1) != cols || tab->dim() != 2 || tab->numel() == 0 || l.blocks == 0 ||
+      (packed ? rows != 1 || extra[1]->sizes() != pos->sizes() : rows > tab->size(0)) ||
+      (extra[0] && (extra[0]->dim() != 1 || extra[0]->numel() < 1)) || (extra[2] && (extra[2]->dim() != 1 || extra[2]->size(0) != tab->size(0))))
+    NVJ_NONE();
+  if (q && (q->dim() != 4 || q->dtype() != k->dtype() || q->size(0) != rows || q->size(1) != cols || q->size(2) < 1 || q->size(3) != l.d ||
+            !rope_rows(*q, l.device, &rq)))
+    NVJ_NONE();
+  if (inv && (!on(*inv, l.device) || inv->scalar_type() != at::kFloat || inv->dim() != 1 || !inv->is_contiguous() || 2 * inv->numel() > l.d)) NVJ_NONE();
+  if (bounds && (!on(*bounds, l.device) || bounds->dtype() != tensor(a[3])->dtype() || bounds->dim() != 4 || bounds->size(0) != l.blocks ||
+                 bounds->size(1) != l.hkv || bounds->size(2) != 2 || bounds->size(3) != l.d || !bounds->is_contiguous() || !aligned(*bounds)))
+    NVJ_NONE();
+  const c10::cuda::OptionalCUDAGuard guard(c10::Device(c10::kCUDA, (c10::DeviceIndex)l.device));
+  void* stream = stream_of(l.device);
+  int32_t* st = status_for(l.device, stream);
+  if (!st) return nullptr;
+  at::Tensor out;
+  if (q) {
+    out = empty({rows, cols, q->size(2), l.d}, q->scalar_type(), l.device);
+    if (env_is("NVJ_POISON_OUTPUT", "1")) out.fill_(std::nan(""));
+  }
+  auto given = [&](int i) { return extra[i] ? i32(*extra[i]) : nullptr; };
+  int rc;
+  NVJ_CALL(rc, lib.rope_append(rq.data, rq.token, rq.head, rk.data, rk.token, rk.head, rv.data, rv.token, rv.head, dtype_code(*k),
+                               inv ? static_cast<const float*>(inv->data_ptr()) : nullptr, inv ? 2 * (int)inv->numel() : 0, interleaved, i32(*pos),
+                               i32(*tab), given(1), (int)tab->size(0), (int)tab->size(1), given(0), extra[0] ? (int)extra[0]->numel() - 1 : 0,
+                               given(2), (int)rows, (int)cols, l.k, l.v, bounds ? bounds->data_ptr() : nullptr, l.dtype, l.blocks, l.block_size,
+                               q ? (int)q->size(2) : 0, l.hkv, l.d, q ? out.data_ptr() : nullptr, st, stream));
+  if (!finished(rc, "nvj_rope_kv_append", l.device, stream, false, true)) return nullptr;
+  if (!q) Py_RETURN_TRUE;
+  return THPVariable_Wrap(std::move(out));
+}
+
+// Query rows [batch, heads, d] or [batch, tokens, heads, d] with their tables, lengths and positions.
+struct QueryRows {
+  bool ok = false, wide;
+  long long batch, width, hq;
+};
+QueryRows query_rows(const at::Tensor* q, const at::Tensor* tab, const at::Tensor* len, const at::Tensor* pos, int device, long long hkv, long long d) {
+  QueryRows r;
+  if (!q || !tab || !len || (q->dim() != 3 && q->dim() != 4) || !plain_rows(*q, device)) return r;
+  r.wide = q->dim() == 4;
+  r.batch = q->size(0);
+  r.width = r.wide ? q->size(1) : 1;
+  r.hq = q->size(-2);
+  r.ok = r.batch * r.width * r.hq > 0 && r.batch * r.width <= 0x7fffffffLL && q->size(-1) == d && r.hq % hkv == 0 && meta(*tab, device) &&
+         meta(*len, device) && tab->dim() == 2 && tab->size(0) == r.batch && len->dim() == 1 && len->size(0) == r.batch &&
+         (!pos || (meta(*pos, device) && pos->numel() == r.batch * r.width));
+  return r;
+}
+constexpr long long kMostColumns = 45056;  // block-table columns that a selection takes
+at::Tensor selection(const QueryRows& r, long long hkv, long long budget, int device) {
+  at::Tensor t = r.wide ? empty({r.batch, r.width, hkv, budget}, at::kInt, device) : empty({r.batch, hkv, budget}, at::kInt, device);
+  if (env_is("NVJ_POISON_OUTPUT", "1")) t.fill_(1 << 30);
+  return t;
+}
+
+// select_blocks(q, k_bounds, block_table, seq_lens, block_size, budget, positions | None, first, last) -> int32 columns
+PyObject* select_blocks(PyObject* const* a, Py_ssize_t n) {
+  if (!args_are(n, 9)) return nullptr;
+  const at::Tensor *q = tensor(a[0]), *b = tensor(a[1]), *tab = tensor(a[2]), *len = tensor(a[3]), *pos = a[6] == Py_None ? nullptr : tensor(a[6]);
+  const long long bs = PyLong_AsLongLong(a[4]), budget = PyLong_AsLongLong(a[5]), first = PyLong_AsLongLong(a[7]), last = PyLong_AsLongLong(a[8]);
+  if (PyErr_Occurred()) { PyErr_Clear(); NVJ_NONE(); }
+  if (!q || !b || (!pos && a[6] != Py_None) || !b->is_cuda() || b->dim() != 4 || b->size(2) != 2 || b->size(1) < 1 || !b->is_contiguous() ||
+      !aligned(*b) || dtype_code(*b) < 0 || !selective_dims(b->size(3)))
+    NVJ_NONE();
+  const int device = b->get_device(), hkv = (int)b->size(1), d = (int)b->size(3);
+  const QueryRows r = query_rows(q, tab, len, pos, device, hkv, d);
+  if (!r.ok || bs < 1 || bs > 65536 || budget < 1 || budget > 0x7fffffffLL || first < 0 || last < 0 || first + last > budget || tab->size(1) > kMostColumns) NVJ_NONE();
+  const c10::cuda::OptionalCUDAGuard guard(c10::Device(c10::kCUDA, (c10::DeviceIndex)device));
+  void* stream = stream_of(device);
+  int32_t* st = status_for(device, stream);
+  if (!st) return nullptr;
+  at::Tensor out = selection(r, hkv, budget, device);
+  int rc;
+  NVJ_CALL(rc, lib.select_blocks(q->data_ptr(), dtype_code(*q), b->data_ptr(), dtype_code(*b), b->size(0), (int)bs, hkv, d, (int)r.hq, i32(*tab),
+                                 (int)tab->size(1), i32(*len), pos ? i32(*pos) : nullptr, (int)r.batch, (int)r.width, (int)budget, (int)first,
+                                 (int)last, static_cast<int32_t*>(out.data_ptr()), st, stream));
+  if (!finished(rc, "nvj_select_blocks", device, stream, false, true)) return nullptr;
+  return THPVariable_Wrap(std::move(out));
+}
+
+// selected_decode(q, k_layer, v_layer, block_table, seq_lens, selected, scale, positions | None) -> out as q [B, Hq, D], or [B, T, Hq * D]
+PyObject* selected_decode(PyObject* const* a, Py_ssize_t n) {
+  if (!args_are(n, 8)) return nullptr;
+  const at::Tensor *q = tensor(a[0]), *tab = tensor(a[3]), *len = tensor(a[4]), *sel = tensor(a[5]), *pos = a[7] == Py_None ? nullptr : tensor(a[7]);
+  const double scale = PyFloat_AsDouble(a[6]);
+  if (PyErr_Occurred()) { PyErr_Clear(); NVJ_NONE(); }
+  const SelectiveLayer l = selective_layer(tensor(a[1]), tensor(a[2]));
+  if (!l.ok || !sel || (!pos && a[7] != Py_None)) NVJ_NONE();
+  const QueryRows r = query_rows(q, tab, len, pos, l.device, l.hkv, l.d);
+  if (!r.ok || !meta(*sel, l.device) || sel->dim() != q->dim() || sel->size(0) != r.batch || sel->size(-2) != l.hkv || (r.wide && sel->size(1) != r.width))
+    NVJ_NONE();
+  const c10::cuda::OptionalCUDAGuard guard(c10::Device(c10::kCUDA, (c10::DeviceIndex)l.device));
+  void* stream = stream_of(l.device);
+  int32_t* st = status_for(l.device, stream);
+  if (!st) return nullptr;
+  at::Tensor out = r.wide ? output({r.batch, r.width, r.hq * l.d}, l.device) : output({r.batch, r.hq, l.d}, l.device);
+  int rc;
+  NVJ_CALL(rc, lib.selected_decode(q->data_ptr(), dtype_code(*q), l.k, l.v, l.dtype, l.blocks, l.block_size, l.hkv, l.d, (int)r.hq, i32(*tab),
+                                   (int)tab->size(1), i32(*len), pos ? i32(*pos) : nullptr, i32(*sel), (int)sel->size(-1), (int)r.batch, (int)r.width,
+                                   (float)scale, static_cast<float*>(out.data_ptr()), st, stream));
+  if (!finished(rc, "nvj_paged_decode_selected", l.device, stream, false, true)) return nullptr;
+  return THPVariable_Wrap(std::move(out));
+}
+
+// selective_step(query [B, T, Hq, D], k, v, k_cache, v_cache, k_bounds (5-D), layer, block_tables, seq_lens, positions, query_start_loc, block_size, scale,
+//                groups, budget, first, last, max_kv_len | None) -> out [B, T, Hq * D]: a decode step's append, selection and attention
+PyObject* selective_step(PyObject* const* a, Py_ssize_t n) {
+  if (!args_are(n, 18)) return nullptr;
+  const at::Tensor *q = tensor(a[0]), *k = tensor(a[1]), *v = tensor(a[2]), *kc = tensor(a[3]), *b = tensor(a[5]), *tab = tensor(a[7]), *len = tensor(a[8]),
+                   *pos = tensor(a[9]), *qsl = tensor(a[10]);
+  const long long layer = PyLong_AsLongLong(a[6]), bs = PyLong_AsLongLong(a[11]), groups = PyLong_AsLongLong(a[13]), budget = PyLong_AsLongLong(a[14]),
+                  first = PyLong_AsLongLong(a[15]), last = PyLong_AsLongLong(a[16]);
+  const double scale = PyFloat_AsDouble(a[12]);
+  const long long max_len = a[17] == Py_None ? -1 : PyLong_AsLongLong(a[17]);
+  if (PyErr_Occurred()) { PyErr_Clear(); NVJ_NONE(); }
+  const Layer c = cache_layer(kc, tensor(a[4]), layer);
+  if (!c.ok || !q || !k || !v || !b || !tab || !len || !pos || !qsl || q->dim() != 4 || c.block_size != bs || !selective_dims(c.d) || c.hkv < 1 ||
+      ((reinterpret_cast<uintptr_t>(c.k) | reinterpret_cast<uintptr_t>(c.v)) & 15))
+    NVJ_NONE();
+  SelectiveLayer l;
+  l.ok = true;
+  l.device = c.device, l.dtype = c.dtype, l.block_size = c.block_size, l.hkv = c.hkv, l.d = c.d, l.blocks = c.blocks, l.k = c.k, l.v = c.v;
+  const QueryRows r = query_rows(q, tab, len, pos, l.device, l.hkv, l.d);
+  RopeRows rk, rv;
+  if (!r.ok || r.hq != l.hkv * groups || !new_rows(k, v, l) || k->size(0) != r.batch || k->size(1) != r.width || !rope_rows(*k, l.device, &rk) ||
+      !rope_rows(*v, l.device, &rv) || pos->dim() != 2 || pos->size(0) != r.batch || !meta(*qsl, l.device) || qsl->dim() != 1 || qsl->numel() < 1 ||
+      tab->numel() == 0 || l.blocks == 0 || tab->size(1) > kMostColumns || !(scale > 0) || budget < 1 || first < 0 || last < 0 || first + last > budget ||
+      tab->size(1) <= budget || (max_len >= 0 && max_len < tab->size(1) * bs))
+    NVJ_NONE();
+  if (!on(*b, l.device) || b->dtype() != kc->dtype() || b->dim() != 5 || b->size(0) != kc->size(0) || b->size(1) != l.blocks || b->size(2) != l.hkv ||
+      b->size(3) != 2 || b->size(4) != l.d || !b->is_contiguous())
+    NVJ_NONE();
+  l.bounds = static_cast<char*>(b->data_ptr()) + layer * l.blocks * l.hkv * 2 * l.d * (long long)b->element_size();
+  if (reinterpret_cast<uintptr_t>(l.bounds) & 15) NVJ_NONE();
+  const c10::cuda::OptionalCUDAGuard guard(c10::Device(c10::kCUDA, (c10::DeviceIndex)l.device));
+  void* stream = stream_of(l.device);
+  int32_t* st = status_for(l.device, stream);
+  if (!st) return nullptr;
+  at::Tensor out = output({r.batch, r.width, r.hq * l.d}, l.device), chosen = selection(r, l.hkv, budget, l.device);
+  const char* at = "nvj_rope_kv_append";
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = lib.rope_append(nullptr, 0, 0, rk.data, rk.token, rk.head, rv.data, rv.token, rv.head, dtype_code(*k), nullptr, 0, 0, i32(*pos), i32(*tab), nullptr,
+                       (int)r.batch, (int)tab->size(1), i32(*qsl), (int)qsl->numel() - 1, i32(*len), (int)r.batch, (int)r.width, l.k, l.v, l.bounds, l.dtype,
+                       l.blocks, l.block_size, 0, l.hkv, l.d, nullptr, st, stream);
+  if (rc == NVJ_OK) {
+    at = "nvj_select_blocks";
+    rc = lib.select_blocks(q->data_ptr(), dtype_code(*q), l.bounds, l.dtype, l.blocks, l.block_size, l.hkv, l.d, (int)r.hq, i32(*tab), (int)tab->size(1),
+                           i32(*len), i32(*pos), (int)r.batch, (int)r.width, (int)budget, (int)first, (int)last,
+                           static_cast<int32_t*>(chosen.data_ptr()), st, stream);
+  }
+  if (rc == NVJ_OK) {
+    at = "nvj_paged_decode_selected";
+    rc = lib.selected_decode(q->data_ptr(), dtype_code(*q), l.k, l.v, l.dtype, l.blocks, l.block_size, l.hkv, l.d, (int)r.hq, i32(*tab),
+                             (int)tab->size(1), i32(*len), i32(*pos), static_cast<const int32_t*>(chosen.data_ptr()), (int)budget, (int)r.batch,
+                             (int)r.width, (float)scale, static_cast<float*>(out.data_ptr()), st, stream);
+  }
+  Py_END_ALLOW_THREADS
+  if (!finished(rc, at, l.device, stream, false, true)) return nullptr;
+  return THPVariable_Wrap(std::move(out));
+}
+
 // ---- prefix hashes --------------------------------------------------------------------------------------------------
 
 // XXH64 (seed 0) over 64-bit words, after the published specification of the xxHash family: four lanes over stripes of four
@@ -1287,6 +1516,9 @@ PyObject* init(PyObject*, PyObject* args) {
   get(lib.quantized_prefill, "nvj_paged_prefill_quantized");
   get(lib.quantized_prefill_bytes, "nvj_paged_prefill_quantized_workspace_bytes");
   get(lib.packed_layout, "nvj_build_packed_layout");
+  get(lib.rope_append, "nvj_rope_kv_append");
+  get(lib.select_blocks, "nvj_select_blocks");
+  get(lib.selected_decode, "nvj_paged_decode_selected");
   if (missing) {
     PyErr_Format(PyExc_ImportError, "libnvj_b200.so does not export %s", missing);
     return nullptr;
@@ -1357,6 +1589,10 @@ PyMethodDef methods[] = {
     NVJ_FAST(quantized_decode, "decode attention over the 8-bit cache, or None"),
     NVJ_FAST(quantized_prefill, "ragged packed attention over the 8-bit cache, or None"),
     NVJ_FAST(packed_layout, "a packed step's arrays from its rows' lengths, or None"),
+    NVJ_FAST(rope_append, "rotation + append with key bounds, or None"),
+    NVJ_FAST(select_blocks, "the blocks that each query token is to read, or None"),
+    NVJ_FAST(selected_decode, "decode attention over selected blocks, or None"),
+    NVJ_FAST(selective_step, "append, selection and attention of a decode step, or None"),
     {"init", init, METH_VARARGS, "resolve the library's entry points and keep the callbacks"},
     {"set_workspace", set_workspace, METH_VARARGS, "hand over a (device, stream)'s workspace"},
     {"set_status_word", set_status_word, METH_VARARGS, "hand over a (device, stream)'s status word"},

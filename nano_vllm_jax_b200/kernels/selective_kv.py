@@ -92,6 +92,10 @@ def rope_kv_append(query, k, v, k_cache_layer, v_cache_layer, positions, block_t
     position * inv_freq[i].  Every query token is rotated.  `k_bounds`, where given, are brought up to date.  The tokens that fall into one block stand together in the
     batch, as a row's consecutive positions do.  Caches and bounds are updated in place.
     """
+    done = _k.host().rope_append(query, k, v, k_cache_layer, v_cache_layer, positions, block_table, inv_freq, k_bounds, query_start_loc,
+                                 token_row_ids, seq_lens, interleaved)
+    if done is not None:
+        return None if query is None else done
     _pages("k_cache", k_cache_layer)
     _pages("v_cache", v_cache_layer, k_cache_layer)
     device = k_cache_layer.device
@@ -192,6 +196,9 @@ def select_blocks(q, k_bounds, block_table, seq_lens, block_size, budget, *, pos
     `sum(max(q, 0) * high + min(q, 0) * low)`, the largest of the kv head's query heads, is highest (ties: the lowest column), an upper bound of
     their keys' scores under a positive scale.  A score that is not a number, or beyond float32, ranks as infinity.
     """
+    out = _k.host().select_blocks(q, k_bounds, block_table, seq_lens, block_size, budget, positions, first, last)
+    if out is not None:
+        return out
     if not isinstance(q, torch.Tensor):
         raise ValueError("q must be a CUDA tensor (there is no CPU path)")
     device = q.device
@@ -229,6 +236,9 @@ def paged_decode_attention_selected(q, k_cache_layer, v_cache_layer, block_table
     the listed blocks' keys, those with p < seq_lens[b] and, with `positions` `[B, T]`, p <= positions[b, t]; one that sees none gives zeros.  Entries
     below 0 and blocks that the token does not see add nothing; a block that is listed twice counts twice.
     """
+    out = _k.host().selected_decode(q, k_cache_layer, v_cache_layer, block_table, seq_lens, selected, scale, positions)
+    if out is not None:
+        return out
     _pages("k_cache", k_cache_layer)
     _pages("v_cache", v_cache_layer, k_cache_layer)
     device = k_cache_layer.device
