@@ -5,7 +5,7 @@
 // A list holds columns of the row's block table, -1 where it has ended; every entry counts, also one that is there twice.
 //
 // Bound by the bytes of K and V of the listed blocks, which lie scattered over the pool, block_size * head_dim numbers at a stretch if a block had
-// one kv head only.  selected_decode_kernel, for bf16 and f16 caches:
+// one kv head only.  selected_decode_kernel, for bf16 and f16 caches with blocks of whole 16-key tiles:
 //   * one thread-block cluster per (query token, kv head, tile of query columns); the list's 16-key tiles are dealt to the cluster's warps in
 //     turn, and warps and CTAs merge through shared and distributed shared memory: no workspace, no second launch;
 //   * K and V go from global memory to registers in 16-byte pieces and nowhere else: both products are taken transposed
@@ -59,7 +59,7 @@ template <int kD, int kTiles, bool kPack, int kTerms>
 struct SdShape {
   static constexpr int kCols = kPack ? 4 : 8 * kTiles;  // query columns
   static constexpr int kQCols = 8 * kTiles;             // columns of the operand
-  static constexpr int kQPitch = kD + 8;                // elements; two columns' pieces fall into different banks
+  static constexpr int kQPitch = kD + 32;               // elements; the eight columns' pieces of 16 bytes fall into different banks
   static constexpr int kQBytes = kTerms * kQCols * kQPitch * 2;
   static constexpr int kAccPitch = kD + 4;  // floats
   static constexpr int kAccBytes = kSdWarps * kCols * kAccPitch * 4;
@@ -80,7 +80,88 @@ __device__ __forceinline__ void sd_query8(const SelectedParams& p, long long at,
   else q_floats(q_load8(static_cast<const __nv_bfloat16*>(p.q) + at), x);
 }
 
-template <typename C, int kD, int kTiles, bool kPack, int kTerms>
+// The end of a kernel: the sums of the CTA's warps, kCols columns of `dims` numbers each relative to its reference, and those of the cluster's CTAs into one: the output
+// of the heads first_head .. of this kv head's group.
+template <int kCols, int kAccPitch>
+__device__ __forceinline__ void sd_merge(const SelectedParams& p, float* all, const float2 (&sd_ml)[kSdWarps][kCols], float2 (&sd_ML)[kCols], int token, int head,
+                                         int first_head, int dims, int ctas, int rank) {
+  const int quads = dims >> 2;
+  auto place = [&](int col, int d) {
+    return p.out + (((long long)token * p.hkv + head) * p.groups + first_head + col) * dims + d;
+  };
+  const int used = min(kCols, p.groups - first_head);
+  for (int i = threadIdx.x; i < used * quads; i += kSdThreads) {
+    const int col = i / quads, d = i % quads * 4;
+    float top = kSdNone, sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kSdWarps; ++w) top = fmaxf(top, sd_ml[w][col].x);
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kSdWarps; ++w) {
+      const float2 ml = sd_ml[w][col];
+      const float f = ex2_approx(ml.x - top);
+      sum = fmaf(ml.y, f, sum);
+      const float4 x = *reinterpret_cast<const float4*>(all + (w * kCols + col) * kAccPitch + d);
+      y.x = fmaf(x.x, f, y.x);
+      y.y = fmaf(x.y, f, y.y);
+      y.z = fmaf(x.z, f, y.z);
+      y.w = fmaf(x.w, f, y.w);
+    }
+    if (ctas == 1) {
+      const float inverse = sum == 0.f ? 0.f : 1.f / sum;
+      *reinterpret_cast<float4*>(place(col, d)) = make_float4(y.x * inverse, y.y * inverse, y.z * inverse, y.w * inverse);
+    } else {
+      *reinterpret_cast<float4*>(all + col * kAccPitch + d) = y;  // (read above by this thread alone)
+      if (d == 0) sd_ML[col] = make_float2(top, sum);
+    }
+  }
+  if (ctas == 1) return;
+  cl_sync();
+  bool odd = false;
+  const int pieces = used * quads, per = (pieces + ctas - 1) / ctas;
+  for (int i = threadIdx.x; i < per; i += kSdThreads) {
+    const int piece = rank * per + i;
+    if (piece >= pieces) break;
+    const int col = piece / quads, d = piece % quads * 4;
+    float top = kSdNone, sum = 0.f;
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int first = 0; first < ctas; first += 4) {  // four CTAs' shares in flight
+      float2 e[4];
+      float4 x[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int from = first + k < ctas ? first + k : first;
+        e[k] = cl_ld2(cl_map(&sd_ML[col], from));
+        x[k] = cl_ld4(cl_map(all + col * kAccPitch + d, from));
+        if (first + k >= ctas) e[k] = make_float2(kSdNone, 0.f), x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      float now = top;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) now = fmaxf(now, e[k].x);
+      const float f = ex2_approx(top - now);
+      sum *= f;
+      y = make_float4(y.x * f, y.y * f, y.z * f, y.w * f);
+      top = now;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float w = ex2_approx(e[k].x - top);
+        sum = fmaf(e[k].y, w, sum);
+        y.x = fmaf(x[k].x, w, y.x);
+        y.y = fmaf(x[k].y, w, y.y);
+        y.z = fmaf(x[k].z, w, y.z);
+        y.w = fmaf(x[k].w, w, y.w);
+      }
+    }
+    const float inverse = sum == 0.f ? 0.f : 1.f / sum;
+    y = make_float4(y.x * inverse, y.y * inverse, y.z * inverse, y.w * inverse);
+    odd |= cl_not_finite(y) || !(sum - sum == 0.f);
+    *reinterpret_cast<float4*>(place(col, d)) = y;
+  }
+  cl_sync_read(odd);  // no CTA goes while another reads its sums
+}
+
+// kRagged: a head_dim below kD, its missing dims zero.
+template <typename C, int kD, int kTiles, bool kPack, int kTerms, bool kRagged>
 __global__ void __launch_bounds__(kSdThreads) selected_decode_kernel(SelectedParams p, int ctas) {
   using S = SdShape<kD, kTiles, kPack, kTerms>;
   constexpr bool kF16 = std::is_same<C, __half>::value;
@@ -101,7 +182,7 @@ __global__ void __launch_bounds__(kSdThreads) selected_decode_kernel(SelectedPar
   const int rank = ctas > 1 ? (int)cl_rank() : 0;
   const int token = blockIdx.x / ctas, row = token / p.width;
   const int head = blockIdx.y / p.column_tiles, ct = blockIdx.y % p.column_tiles;
-  const int hq = p.hkv * p.groups;
+  const int hq = p.hkv * p.groups, dims = kRagged ? p.d : kD;
   pdl_wait();
   pdl_release();
   const int32_t* table = p.block_tables + (long long)row * p.table_width;
@@ -130,7 +211,7 @@ __global__ void __launch_bounds__(kSdThreads) selected_decode_kernel(SelectedPar
     there = __ballot_sync(kFullMask, id >= 0);
   };
   look();
-  const long long key_stride = (long long)p.hkv * kD;
+  const long long key_stride = (long long)p.hkv * dims;
   uint4 k_held[kAhead][kParts][2];   // keys g and g + 8: dims 32 part + 8 t ..
   uint4 v_held[kAhead][kVParts][4];  // keys 2t, 2t + 1, 2t + 8, 2t + 9: dims 64 part + 8 g ..
   int left[kAhead];                  // keys of the tile that are to be seen; 0: no tile
@@ -148,26 +229,36 @@ __global__ void __launch_bounds__(kSdThreads) selected_decode_kernel(SelectedPar
     there &= there - 1;
     const long long key = (long long)__shfl_sync(kFullMask, id, slot) * p.block_size + __shfl_sync(kFullMask, off, slot);
     left[u] = visible - __shfl_sync(kFullMask, base, slot);
-    const long long at = (key * p.hkv + head) * kD;
+    const long long at = (key * p.hkv + head) * dims;
     const C* kp = static_cast<const C*>(p.k_cache) + at + g * key_stride + 8 * t;
     next_v[u] = static_cast<const C*>(p.v_cache) + at;
 #pragma unroll
     for (int s = 0; s < kParts; ++s) {
-      k_held[u][s][0] = ld_stream_u4(kp + 32 * s);
-      k_held[u][s][1] = ld_stream_u4(kp + 8 * key_stride + 32 * s);
+      if (!kRagged || 32 * s + 8 * t < dims) {
+        k_held[u][s][0] = ld_stream_u4(kp + 32 * s);
+        k_held[u][s][1] = ld_stream_u4(kp + 8 * key_stride + 32 * s);
+      } else {
+        k_held[u][s][0] = k_held[u][s][1] = make_uint4(0, 0, 0, 0);
+      }
     }
   };
   auto ask_v = [&](int u) {
     if (left[u] <= 0) return;
+    const C* vp = next_v[u] + 2 * t * key_stride + 8 * g;
+    if (!kRagged && left[u] >= 16) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int key = 2 * t + (k & 1) + 8 * (k >> 1);
-      const C* vp = next_v[u] + key * key_stride + 8 * g;
-      const bool ok = key < left[u];  // keys behind the last one hold anything: they must not reach a product
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int h = 0; h < kVParts; ++h) v_held[u][h][k] = ld_stream_u4(vp + ((k & 1) + 8 * (k >> 1)) * key_stride + 64 * h);
+      return;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {  // keys behind the last one hold anything: they must not reach a product
+      const int key = (k & 1) + 8 * (k >> 1);
 #pragma unroll
       for (int h = 0; h < kVParts; ++h) {
         v_held[u][h][k] = make_uint4(0, 0, 0, 0);
-        if (ok) v_held[u][h][k] = ld_stream_u4(vp + 64 * h);
+        if (2 * t + key < left[u] && (!kRagged || 64 * h + 8 * g < dims)) v_held[u][h][k] = ld_stream_u4(vp + key * key_stride + 64 * h);
       }
     }
   };
@@ -184,7 +275,7 @@ __global__ void __launch_bounds__(kSdThreads) selected_decode_kernel(SelectedPar
     float x[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = 0.f;
-    if (at < p.groups && lane < kD / 8) sd_query8(p, ((long long)token * hq + head * p.groups + at) * kD + 8 * lane, x);
+    if (at < p.groups && lane < dims / 8) sd_query8(p, ((long long)token * hq + head * p.groups + at) * dims + 8 * lane, x);
     float factor = p.scale_log2;
     if constexpr (kF16 && kTerms > 1) {
       const int bits = __reduce_max_sync(kFullMask, __float_as_int(q_largest(0.f, x)));
@@ -367,107 +458,35 @@ __global__ void __launch_bounds__(kSdThreads) selected_decode_kernel(SelectedPar
     }
   }
   __syncthreads();
-  // ... and into one, relative to the largest reference: to the output, or in the first warp's place for the cluster
-  float* all = reinterpret_cast<float*>(sd_smem);
-  auto place = [&](int col, int d) { return p.out + ((long long)token * hq + head * p.groups + ct * kCols + col) * kD + d; };
-  const int used = min(kCols, p.groups - ct * kCols);
-  for (int i = threadIdx.x; i < used * (kD / 4); i += kSdThreads) {
-    const int col = i / (kD / 4), d = i % (kD / 4) * 4;
-    float top = kSdNone, sum = 0.f;
-#pragma unroll
-    for (int w = 0; w < kSdWarps; ++w) top = fmaxf(top, sd_ml[w][col].x);
-    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int w = 0; w < kSdWarps; ++w) {
-      const float2 ml = sd_ml[w][col];
-      const float f = ex2_approx(ml.x - top);
-      sum = fmaf(ml.y, f, sum);
-      const float4 x = *reinterpret_cast<const float4*>(all + (w * kCols + col) * S::kAccPitch + d);
-      y.x = fmaf(x.x, f, y.x);
-      y.y = fmaf(x.y, f, y.y);
-      y.z = fmaf(x.z, f, y.z);
-      y.w = fmaf(x.w, f, y.w);
-    }
-    if (ctas == 1) {
-      const float inverse = sum == 0.f ? 0.f : 1.f / sum;
-      *reinterpret_cast<float4*>(place(col, d)) = make_float4(y.x * inverse, y.y * inverse, y.z * inverse, y.w * inverse);
-    } else {
-      *reinterpret_cast<float4*>(all + col * S::kAccPitch + d) = y;  // (read above by this thread alone)
-      if (d == 0) sd_ML[col] = make_float2(top, sum);
-    }
-  }
-  if (ctas == 1) return;
-  cl_sync();
-  bool odd = false;
-  const int pieces = used * (kD / 4), per = (pieces + ctas - 1) / ctas;
-  for (int i = threadIdx.x; i < per; i += kSdThreads) {
-    const int piece = rank * per + i;
-    if (piece >= pieces) break;
-    const int col = piece / (kD / 4), d = piece % (kD / 4) * 4;
-    float top = kSdNone, sum = 0.f;
-    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int first = 0; first < ctas; first += 4) {  // four CTAs' shares in flight
-      float2 e[4];
-      float4 x[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int from = first + k < ctas ? first + k : first;
-        e[k] = cl_ld2(cl_map(&sd_ML[col], from));
-        x[k] = cl_ld4(cl_map(all + col * S::kAccPitch + d, from));
-        if (first + k >= ctas) e[k] = make_float2(kSdNone, 0.f), x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-      }
-      float now = top;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) now = fmaxf(now, e[k].x);
-      const float f = ex2_approx(top - now);
-      sum *= f;
-      y = make_float4(y.x * f, y.y * f, y.z * f, y.w * f);
-      top = now;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float w = ex2_approx(e[k].x - top);
-        sum = fmaf(e[k].y, w, sum);
-        y.x = fmaf(x[k].x, w, y.x);
-        y.y = fmaf(x[k].y, w, y.y);
-        y.z = fmaf(x[k].z, w, y.z);
-        y.w = fmaf(x[k].w, w, y.w);
-      }
-    }
-    const float inverse = sum == 0.f ? 0.f : 1.f / sum;
-    y = make_float4(y.x * inverse, y.y * inverse, y.z * inverse, y.w * inverse);
-    odd |= cl_not_finite(y) || !(sum - sum == 0.f);
-    *reinterpret_cast<float4*>(place(col, d)) = y;
-  }
-  cl_sync_read(odd);  // no CTA goes while another reads its sums
+  sd_merge<kCols, S::kAccPitch>(p, reinterpret_cast<float*>(sd_smem), sd_ml, sd_ML, token, head, ct * kCols, dims, ctas, rank);
 }
 
-// CTAs per cluster.
+// CTAs per cluster: as many as are resident at once, two to an SM, and no more than one per four tiles.  Lists are of one length, so that more of them gain nothing at
+// the end and cost their start (512 lists of 64 16-key tiles of 256 dims: one CTA each 89 us, two 105, four 122; 10 lists of 32: eight 7.1, four 8.6, one 15).
 static int selected_decode_ctas(long long units, long long tiles, int sms) {
-  long long c = (2LL * sms + units / 2) / units;
-  if (c < 4 && tiles > 32) c = 4;
+  long long c = 2LL * sms / units;
+  if (c < 1 && 2 * units < 5LL * sms) c = 2;  // (a round and a bit: halves; 320 lists of 64: one CTA 77, two 68; 384 of 96 tiles of 128 dims: 50, 55)
   const long long useful = (tiles + kSdWarps - 1) / kSdWarps;
   c = c < useful ? c : useful;
   return (int)(c < 1 ? 1 : (c > 16 ? 16 : c));
 }
 
-template <typename C, int kD, int kTiles, bool kPack, int kTerms>
-static int launch_selected(SelectedParams p, cudaStream_t stream) {
-  using S = SdShape<kD, kTiles, kPack, kTerms>;
-  auto* kernel = selected_decode_kernel<C, kD, kTiles, kPack, kTerms>;
-  static PerDeviceFlags ready;
+// A launch of `kernel`, whose CTAs take `columns` heads of a group and `keys` keys of a list at a time.
+inline int launch_selected_clusters(void (*kernel)(SelectedParams, int), PerDeviceFlags& ready, SelectedParams p, int columns, int keys, int smem,
+                                    cudaStream_t stream) {
   if (!once_per_device(ready, [&](int) {
-        return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes) == cudaSuccess &&
+        return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) == cudaSuccess &&
                cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess;
       }))
     return NVJ_ERR_LAUNCH;
-  p.column_tiles = (p.groups + S::kCols - 1) / S::kCols;
-  const long long tokens = (long long)p.rows * p.width;
-  const int ctas = selected_decode_ctas(tokens * p.hkv * p.column_tiles, (long long)p.entries * p.block_size / 16, 148);
+  p.column_tiles = (p.groups + columns - 1) / columns;
+  const long long tokens = (long long)p.rows * p.width, per_block = (p.block_size + keys - 1) / keys;
   if ((long long)p.hkv * p.column_tiles > 65535) return NVJ_ERR_TOO_LARGE;
+  const int ctas = selected_decode_ctas(tokens * p.hkv * p.column_tiles, p.entries * per_block, 148);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(ctas * tokens), p.hkv * p.column_tiles, 1);
   cfg.blockDim = dim3(kSdThreads, 1, 1);
-  cfg.dynamicSmemBytes = S::kBytes;
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -481,8 +500,16 @@ static int launch_selected(SelectedParams p, cudaStream_t stream) {
   return cudaLaunchKernelEx(&cfg, kernel, p, ctas) == cudaSuccess ? NVJ_OK : NVJ_ERR_LAUNCH;
 }
 
+template <typename C, int kD, int kTiles, bool kPack, int kTerms, bool kRagged = false>
+static int launch_selected(const SelectedParams& p, cudaStream_t stream) {
+  using S = SdShape<kD, kTiles, kPack, kTerms>;
+  static PerDeviceFlags ready;
+  return launch_selected_clusters(selected_decode_kernel<C, kD, kTiles, kPack, kTerms, kRagged>, ready, p, S::kCols, 16, S::kBytes, stream);
+}
+
 template <typename C, int kD>
 static int launch_selected_columns(const SelectedParams& p, bool same, cudaStream_t stream) {
+  if (p.d != kD) return launch_selected<C, kD, 1, false, 3, true>(p, stream);
   // (16 columns of 256 dims do not fit a thread's registers: two clusters read the blocks, the second mostly from the L2)
   if constexpr (kD < 256)
     if (p.groups > 8) return same ? launch_selected<C, kD, 2, false, 1>(p, stream) : launch_selected<C, kD, 2, false, 3>(p, stream);
@@ -490,11 +517,11 @@ static int launch_selected_columns(const SelectedParams& p, bool same, cudaStrea
   if (p.groups <= 4) return launch_selected<C, kD, 1, true, 1>(p, stream);
   return launch_selected<C, kD, 1, false, 1>(p, stream);
 }
-// A cache of type C, head_dim 64, 128 or 256 and blocks of whole 16-key tiles; `same`: the queries are of the cache's type.
+// A cache of type C and blocks of whole 16-key tiles; `same`: the queries are of the cache's type.
 template <typename C>
 static int launch_selected_dims(const SelectedParams& p, bool same, cudaStream_t stream) {
-  if (p.d == 256) return launch_selected_columns<C, 256>(p, same, stream);
-  if (p.d == 128) return launch_selected_columns<C, 128>(p, same, stream);
+  if (p.d > 128) return launch_selected_columns<C, 256>(p, same, stream);
+  if (p.d > 64) return launch_selected_columns<C, 128>(p, same, stream);
   return launch_selected_columns<C, 64>(p, same, stream);
 }
 // selected_decode_bf16.cu, selected_decode_f16.cu
