@@ -753,18 +753,25 @@ __global__ void __launch_bounds__(32 * kBsMostWarps, kD == 0 && kTiles > 1 ? 1 :
     }
 }
 
-// How a call is cut: CTAs per cluster and their warps.  A CTA has ~8 us beside its stream (ids, queries, border, output), which others hide: many rows go one to a
-// CTA of four warps, four to an SM (256 rows of 128 - 512 blocks, 2 heads of 256: 46 us, two CTAs each 52, four 57); few long ones are cut into as many as leave
-// two rounds of CTAs of eight warps, so that the longest are not left alone at the end (64 rows of 1024 - 4096 blocks: one CTA 97, two 96, three 89, four 87).
+// How a call is cut: CTAs per cluster and their warps.  A CTA has ~8 us beside its stream (ids, queries, border, output), which others hide.
+//   * Many rows, or short ones: four warps each, four CTAs to an SM (256 rows of 128 - 512 blocks, 2 heads of 256: 46 us, two CTAs each 52, four 57; 250
+//     rows of 190: 25, with eight warps 31).
+//   * Few long rows: eight warps, as many CTAs as are resident at once (64 rows of 1000: two 32, four 37; 32: four 22, eight 26), and twice as many where each would still
+//     have more than 1024 blocks, so that the longest rows are not left alone at the end (64 rows of 1024 - 4096: two 96, four 87).
+//   * At most a CTA per tile of its warps, or per two of them where the CTAs do not all have an SM of their own (16 rows of 1000: four 18.0, eight
+//     19.9; 8 rows: four 15.0, eight 13.9).
 struct BsPlan {
   int ctas, warps;
 };
 static BsPlan block_select_plan(long long units, long long columns, int sms) {
   const int warps = units > 2LL * sms || columns <= 512 ? 4 : 8;
-  long long c = (32LL / warps) * sms / units;
-  const long long useful = (columns + 16 * warps - 1) / (16 * warps);
-  c = c < useful ? c : useful;
-  return {(int)(c < 1 || units > 2LL * sms ? 1 : (c > kBsMostCtas ? kBsMostCtas : c)), warps};
+  long long c = units > 2LL * sms ? 1 : (16LL / warps) * sms / units;
+  if (columns > 1024 * c) c *= 2;
+  const long long tiles = (columns + 16 * warps - 1) / (16 * warps);
+  if (c > tiles) c = tiles;
+  if (c > kBsMostCtas) c = kBsMostCtas;
+  if (units * c > sms && c > (tiles + 1) / 2) c = (tiles + 1) / 2;
+  return {(int)(c < 1 ? 1 : c), warps};
 }
 
 template <typename C, int kD, int kTiles, int kTerms, bool kRagged = false>

@@ -9,11 +9,10 @@
 //
 // The unit of work for K and V is a run, as in the 8-bit append: tokens of the call that stand together and fall into one block; a warp
 // takes one run of one kv head, so that the bounds need no atomics.  Queries are dealt by token, so that a warp makes a token's cosines once for
-// several heads.  A row is held by 8, 16 or 32 lanes, 8 elements each; its pairs meet by a shuffle.  Cosines and sines go through 1 KiB of
-// shared memory per warp, each made once.
+// several heads.  A row is held by 8, 16 or 32 lanes, 8 elements each; its pairs meet by a shuffle of the loaded words.  Cosines and
+// sines go through shared memory, each made once.
 
 #include "quantized_kv.cuh"
-#include "rotary.cuh"
 
 namespace nvj {
 
@@ -35,7 +34,7 @@ struct RopeAppendParams {
   int32_t* status;
   long long num_blocks;
   int rot, interleaved, hq, hkv, d, qsl_rows, packed, n_tokens, n_cols, table_rows, table_width, block_size;
-  int window, kv_ctas, q_ctas, item_heads;  // tokens of a CTA; grid y: CTAs of K and V runs, then of queries, `item_heads` heads of a token at a time
+  int window, kv_ctas, kv_heads, q_ctas, item_heads;  // tokens of a CTA; grid y: CTAs of K and V runs of `kv_heads` heads, then of queries, `item_heads` heads of a token at a time
 };
 
 constexpr int kRaWarps = 4, kRaHold = 4;  // rows (steps of rows) that a warp has in flight
@@ -79,54 +78,105 @@ __device__ __forceinline__ void ra_store(C* at, const QRaw<C>& r) {
   if constexpr (sizeof(C) == 4) *reinterpret_cast<uint4*>(at + 4) = r.w;
 }
 
-// Cosines and sines of position `pos` by the kLanes lanes of a row, into their row's part of the warp's table.
+// How a row's pairs lie: `whole` where a lane's eight elements are turned or left together and their partners are another lane's eight, or their own neighbours.
+struct RaPairs {
+  int rot, half;
+  bool pairs, whole, turns;  // turns: this lane's elements are (where whole)
+  int from;                  // the lane that has the partners
+};
 template <int kLanes>
-__device__ __forceinline__ void ra_angles(float2* cs, const float* inv_freq, int half, int pos, int lane) {
-  for (int f = lane % kLanes; f < half; f += kLanes) {
-    float c, s;
-    cos_sin((double)pos * (double)inv_freq[f], c, s);
-    cs[f] = make_float2(c, s);
+__device__ __forceinline__ RaPairs ra_pairs(const RopeAppendParams& p, int lane) {
+  RaPairs r;
+  const int col = (lane % kLanes) * 8;
+  r.rot = p.rot;
+  r.half = p.rot >> 1;
+  r.pairs = p.interleaved;
+  r.whole = (p.rot & (r.pairs ? 7 : 15)) == 0;
+  r.turns = col < p.rot;
+  r.from = (lane & ~(kLanes - 1)) + (col < r.half ? (col + r.half) >> 3 : col < r.rot ? (col - r.half) >> 3 : col >> 3);
+  return r;
+}
+// Cosine and sine to a few units of 2^-24 of an angle up to 2^53: in units of half a turn, a rounding in 64 bits away (rotary.cuh keeps more next to the zeros).
+__device__ __forceinline__ float2 ra_cos_sin(double angle) {
+  const double turns = angle * 0x1.45f306dc9c883p-2;  // 1 / pi
+  const long long halves = __double2ll_rn(2.0 * turns);
+  float s, c;
+  sincospif((float)fma(-0.5, (double)halves, turns), &s, &c);
+  const int quarter = (int)halves & 3;
+  const float cq = (quarter & 1) ? s : c, sq = (quarter & 1) ? c : s;
+  return make_float2(quarter == 1 || quarter == 2 ? -cq : cq, quarter & 2 ? -sq : sq);
+}
+// Cosines and sines of a position, by the lanes `mine` of `lanes`.
+__device__ __forceinline__ void ra_angles(float2* cs, const float* inv_freq, int half, int pos, int mine, int lanes) {
+  for (int f = mine; f < half; f += lanes) cs[f] = ra_cos_sin((double)pos * (double)inv_freq[f]);
+}
+// What this lane's elements and their partners are multiplied by (whole rows).
+struct RaFactors {
+  float c[8], s[8];
+};
+__device__ __forceinline__ void ra_factors(RaFactors& f, const float2* cs, const RaPairs& r, int col) {
+  if (!r.turns) return;
+  if (r.pairs) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 t = cs[(col >> 1) + j];
+      f.c[2 * j] = f.c[2 * j + 1] = t.x;
+      f.s[2 * j] = -t.y;
+      f.s[2 * j + 1] = t.y;
+    }
+  } else {
+    const float2* at = cs + (col < r.half ? col : col - r.half);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float2 t = at[j];
+      f.c[j] = t.x;
+      f.s[j] = col < r.half ? -t.y : t.y;
+    }
   }
 }
-
-// One row turned in place: x are this lane's elements col .. col + 7, `src` the row, cs its table.  All lanes of the warp are here.
-template <typename T, int kLanes>
-__device__ __forceinline__ void ra_turn(float (&x)[8], const T* src, const float2* cs, int rot, bool interleaved, int col, int lane, bool live) {
-  const int half = rot >> 1;
-  if (interleaved) {
-    if (col < rot) {
+template <typename T>
+__device__ __forceinline__ QRaw<T> ra_shuffle(const QRaw<T>& r, int from) {
+  QRaw<T> o;
+  o.v = make_uint4(__shfl_sync(kFullMask, r.v.x, from), __shfl_sync(kFullMask, r.v.y, from), __shfl_sync(kFullMask, r.v.z, from),
+                   __shfl_sync(kFullMask, r.v.w, from));
+  if constexpr (sizeof(T) == 4)
+    o.w = make_uint4(__shfl_sync(kFullMask, r.w.x, from), __shfl_sync(kFullMask, r.w.y, from), __shfl_sync(kFullMask, r.w.z, from),
+                     __shfl_sync(kFullMask, r.w.w, from));
+  return o;
+}
+// One row turned: x from `raw`.  All lanes of the warp are here.
+template <typename T>
+__device__ __forceinline__ void ra_turn(float (&x)[8], const QRaw<T>& raw, const RaFactors& f, const RaPairs& r) {
+  q_floats(raw, x);
+  if (r.pairs) {
+    if (r.turns) {
 #pragma unroll
-      for (int j = 0; j < 8; j += 2)
-        if (col + j < rot) {
-          const float2 t = cs[(col + j) >> 1];
-          const float a = x[j], b = x[j + 1];
-          x[j] = fmaf(a, t.x, -(b * t.y));
-          x[j + 1] = fmaf(b, t.x, a * t.y);
-        }
+      for (int j = 0; j < 8; j += 2) {
+        const float a = x[j], b = x[j + 1];
+        x[j] = fmaf(a, f.c[j], b * f.s[j]);
+        x[j + 1] = fmaf(b, f.c[j + 1], a * f.s[j + 1]);
+      }
     }
     return;
   }
   float other[8];
-  if ((half & 7) == 0) {  // the partners are another lane's elements
-    const int from = (lane & ~(kLanes - 1)) + (col < half ? (col + half) >> 3 : col < rot ? (col - half) >> 3 : col >> 3);
+  q_floats(ra_shuffle(raw, r.from), other);
+  if (r.turns) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) other[j] = __shfl_sync(kFullMask, x[j], from);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int i = col + j;
-      other[j] = live && i < rot ? (float)src[i < half ? i + half : i - half] : 0.f;
-    }
+    for (int j = 0; j < 8; ++j) x[j] = fmaf(x[j], f.c[j], other[j] * f.s[j]);
   }
-  if (col < rot) {
+}
+// The same where a lane's elements differ: element by element, partners from memory.
+template <typename T>
+__device__ __forceinline__ void ra_turn_odd(float (&x)[8], const T* src, const float2* cs, const RaPairs& r, int col) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int i = col + j;
-      if (i < rot) {
-        const float2 t = cs[i < half ? i : i - half];
-        x[j] = fmaf(x[j], t.x, i < half ? -(other[j] * t.y) : other[j] * t.y);
-      }
-    }
+  for (int j = 0; j < 8; ++j) {
+    const int i = col + j;
+    if (i >= r.rot) continue;
+    const bool first = r.pairs ? !(i & 1) : i < r.half;
+    const float other = (float)src[r.pairs ? i ^ 1 : first ? i + r.half : i - r.half];
+    const float2 t = cs[r.pairs ? i >> 1 : first ? i : i - r.half];
+    x[j] = fmaf(x[j], t.x, first ? -(other * t.y) : other * t.y);
   }
 }
 
@@ -162,105 +212,154 @@ __device__ __forceinline__ RaToken ra_token(const RopeAppendParams& p, int i) {
   return t;
 }
 
-// One run of one kv head: `n` tokens from `first` on, of table entry `entry`.
-template <typename T, typename C, int kLanes>
-__device__ void ra_run(const RopeAppendParams& p, int first, int n, long long entry, int block, int head, bool is_v, float2* table, int lane) {
+constexpr int kRaTable = 512;  // cosines and sines that a warp's table holds
+
+// One run: `n` tokens from `first` on, of table entry `entry`, of the kv heads head0 .. head1, by kShare warps that meet at the CTA's barriers.
+template <typename T, typename C, int kLanes, int kShare>
+__device__ __forceinline__ void ra_run(const RopeAppendParams& p, int first, int n, long long entry, int block, int head0, int head1, bool is_v,
+                                       float2 (&tables)[kRaWarps][kRaTable], int warp, int lane) {
   constexpr int kRows = 32 / kLanes;
-  const int sub = lane / kLanes, col = (lane % kLanes) * 8;
+  const int lane_row = lane / kLanes, sub = (kShare > 1 ? warp * kRows : 0) + lane_row, col = (lane % kLanes) * 8;
+  constexpr int kStep = kShare * kRows;  // rows from one step to the next
+  float2* table = tables[warp];
   const bool inside = col < p.d;
   const T* src = static_cast<const T*>(is_v ? p.v : p.k);
-  const long long token_stride = is_v ? p.v_token : p.k_token, at_head = head * (is_v ? p.v_head : p.k_head);
+  const long long token_stride = is_v ? p.v_token : p.k_token, head_stride = is_v ? p.v_head : p.k_head;
   const int id = p.block_tables[entry];
   const bool turned = !is_v && p.rot > 0;
-  const int half = p.rot >> 1;
-  float2* cs = table + sub * half;
-  const bool ok = id >= 0 && id < p.num_blocks;
-  if (!ok && lane == 0) atomicOr(p.status, NVJ_DEV_BAD_BLOCK_ID);
-  if (!ok) return;
-  C* base = static_cast<C*>(is_v ? p.v_cache : p.k_cache) + ((long long)id * p.block_size * p.hkv + head) * p.d + col;
+  const RaPairs pairs = ra_pairs<kLanes>(p, lane);
   const long long slot = (long long)p.hkv * p.d;
   const bool bounded = !is_v && p.bounds;
-  float low[8], high[8];
+  const int steps = (n + kStep - 1) / kStep;
+  const bool kept = steps * kRows * pairs.half <= kRaTable;  // the table holds the angles of all rows of this warp, for all heads
+  bool made = false, begins = false;
+  for (int head = head0; head < head1; ++head) {
+    C* base = static_cast<C*>(is_v ? p.v_cache : p.k_cache) + (((long long)id * p.block_size - (long long)block * p.block_size) * p.hkv + head) * p.d + col;
+    float low[8], high[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) low[j] = INFINITY, high[j] = -INFINITY;
-  bool begins = false;
-  for (int at = 0; at < n; at += kRaHold * kRows) {
-    QRaw<T> raw[kRaHold];
-    int pos[kRaHold];
+    for (int j = 0; j < 8; ++j) low[j] = INFINITY, high[j] = -INFINITY;
+    for (int at = 0; at < n; at += kRaHold * kStep) {
+      QRaw<T> raw[kRaHold];
+      int pos[kRaHold];
 #pragma unroll
-    for (int s = 0; s < kRaHold; ++s) {
-      const int r = at + s * kRows + sub;
-      pos[s] = 0;
-      if (r < n) {
-        pos[s] = p.positions[first + r];
-        if (inside) raw[s] = q_load8(src + (long long)(first + r) * token_stride + at_head + col);
+      for (int s = 0; s < kRaHold; ++s) {
+        const int r = at + s * kStep + sub;
+        pos[s] = 0;
+        if (r < n) {
+          pos[s] = p.positions[first + r];
+          if (inside) raw[s] = q_load8(src + (long long)(first + r) * token_stride + head * head_stride + col);
+        }
       }
-    }
-#pragma unroll
-    for (int s = 0; s < kRaHold; ++s) {
-      if (at + s * kRows >= n) break;
-      const int r = at + s * kRows + sub;
-      const bool live = r < n && inside;
-      if (turned) {
+      if (id < 0 || id >= p.num_blocks) {  // (the rows have been asked for before the id is there)
+        if (lane == 0) atomicOr(p.status, NVJ_DEV_BAD_BLOCK_ID);
+        return;
+      }
+      if (turned && !made) {
         __syncwarp();
-        if (r < n) ra_angles<kLanes>(cs, p.inv_freq, half, pos[s], lane);
+        if (kept) {
+          for (int s = 0; s < steps; ++s)
+            if (s * kStep + sub < n)
+              ra_angles(table + (s * kRows + lane_row) * pairs.half, p.inv_freq, pairs.half, p.positions[first + s * kStep + sub], lane % kLanes, kLanes);
+          made = true;
+        } else {
+#pragma unroll
+          for (int s = 0; s < kRaHold; ++s)
+            if (at + s * kStep + sub < n) ra_angles(table + (s * kRows + lane_row) * pairs.half, p.inv_freq, pairs.half, pos[s], lane % kLanes, kLanes);
+        }
         __syncwarp();
       }
-      float x[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = 0.f;
-      if (live) q_floats(raw[s], x);
-      if (turned) ra_turn<T, kLanes>(x, src + (long long)(first + r) * token_stride + at_head, cs, p.rot, p.interleaved, col, lane, live);
-      if (live) {
-        const int o = pos[s] - block * p.block_size;
-        const QRaw<C> w = ra_pack<C>(x);
-        ra_store<C>(base + (long long)o * slot, w);
-        if (bounded) {
-          begins |= o == 0;
-          q_floats(w, x);
+      for (int s = 0; s < kRaHold; ++s) {
+        if (at + s * kStep + (kShare > 1 ? warp * kRows : 0) >= n) break;
+        const int r = at + s * kStep + sub;
+        const bool live = r < n && inside;
+        const float2* cs = table + ((kept ? at / kStep + s : s) * kRows + lane_row) * pairs.half;
+        float x[8];
+        if (turned && pairs.whole) {
+          RaFactors f;
+          ra_factors(f, cs, pairs, col);
+          ra_turn(x, raw[s], f, pairs);
+        } else {
+          q_floats(raw[s], x);
+          if (turned && live) ra_turn_odd(x, src + (long long)(first + r) * token_stride + head * head_stride, cs, pairs, col);
+        }
+        if (live) {
+          const QRaw<C> w = ra_pack<C>(x);
+          ra_store<C>(base + (long long)pos[s] * slot, w);
+          if (bounded) {
+            begins |= pos[s] == block * p.block_size;
+            q_floats(w, x);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) low[j] = ra_min(low[j], x[j]), high[j] = ra_max(high[j], x[j]);
+            for (int j = 0; j < 8; ++j) low[j] = ra_min(low[j], x[j]), high[j] = ra_max(high[j], x[j]);
+          }
         }
       }
     }
-  }
-  if (!bounded) return;
-  begins = __any_sync(kFullMask, begins);
+    if (!bounded) continue;
+    begins = __any_sync(kFullMask, begins);
 #pragma unroll
-  for (int o = kLanes; o < 32; o <<= 1)
+    for (int o = kLanes; o < 32; o <<= 1)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      low[j] = ra_min(low[j], __shfl_xor_sync(kFullMask, low[j], o));
-      high[j] = ra_max(high[j], __shfl_xor_sync(kFullMask, high[j], o));
+      for (int j = 0; j < 8; ++j) {
+        low[j] = ra_min(low[j], __shfl_xor_sync(kFullMask, low[j], o));
+        high[j] = ra_max(high[j], __shfl_xor_sync(kFullMask, high[j], o));
+      }
+    if constexpr (kShare > 1) {
+      __shared__ __align__(16) float ends[kRaWarps][512];
+      begins = __syncthreads_or(begins);  // (and the ends of the head before have been read)
+      if (lane_row == 0 && inside)
+#pragma unroll
+        for (int j = 0; j < 8; j += 4) {
+          *reinterpret_cast<float4*>(&ends[warp][col + j]) = make_float4(low[j], low[j + 1], low[j + 2], low[j + 3]);
+          *reinterpret_cast<float4*>(&ends[warp][256 + col + j]) = make_float4(high[j], high[j + 1], high[j + 2], high[j + 3]);
+        }
+      __syncthreads();
+      if ((head - head0) % kShare == warp && lane_row == 0 && inside)  // (the heads in turn)
+#pragma unroll
+        for (int w = 0; w < kShare; ++w)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) low[j] = ra_min(low[j], ends[w][col + j]), high[j] = ra_max(high[j], ends[w][256 + col + j]);
     }
-  if (sub == 0 && inside) {
-    C* at = static_cast<C*>(p.bounds) + ((long long)id * p.hkv + head) * 2 * p.d + col;
-    if (!begins) {
-      float x[8];
-      q_floats(q_load8(at), x);
+    if ((kShare == 1 || (head - head0) % kShare == warp) && lane_row == 0 && inside) {
+      C* at = static_cast<C*>(p.bounds) + ((long long)id * p.hkv + head) * 2 * p.d + col;
+      if (!begins) {
+        float x[8];
+        q_floats(q_load8(at), x);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) low[j] = ra_min(low[j], x[j]);
-      q_floats(q_load8(at + p.d), x);
+        for (int j = 0; j < 8; ++j) low[j] = ra_min(low[j], x[j]);
+        q_floats(q_load8(at + p.d), x);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) high[j] = ra_max(high[j], x[j]);
+        for (int j = 0; j < 8; ++j) high[j] = ra_max(high[j], x[j]);
+      }
+      ra_store<C>(at, ra_pack<C>(low));
+      ra_store<C>(at + p.d, ra_pack<C>(high));
     }
-    ra_store<C>(at, ra_pack<C>(low));
-    ra_store<C>(at + p.d, ra_pack<C>(high));
   }
 }
 
-template <typename T, typename C, int kLanes>
-__global__ void __launch_bounds__(32 * kRaWarps) rope_append_kernel(RopeAppendParams p) {
-  __shared__ float2 tables[kRaWarps][128];  // rows of a step x rot / 2 frequencies
+// kShare 1: a warp takes the runs of its part (K or V of a kv head); 4: the CTA's warps share them.
+template <typename T, typename C, int kLanes, int kShare>
+__global__ void __launch_bounds__(32 * kRaWarps, sizeof(T) == 4 ? 4 : 5) rope_append_kernel(RopeAppendParams p) {
+  __shared__ __align__(16) float2 tables[kRaWarps][kRaTable];  // rows x rot / 2 frequencies
   constexpr int kRows = 32 / kLanes;
   pdl_wait();
   pdl_release();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long base = (long long)blockIdx.x * p.window;  // first token of the window
-  float2* table = tables[warp];
   if ((int)blockIdx.y < p.kv_ctas) {
-    const int part = blockIdx.y * kRaWarps + warp, head = part >> 1;
+    const int part = kShare > 1 ? (int)blockIdx.y : (int)blockIdx.y * kRaWarps + warp, head = (part >> 1) * p.kv_heads;
     if (head >= p.hkv) return;
+    if constexpr (kShare > 1) {  // a prompt: the window's rows on their way to the L2 while their places are looked up
+      const int heads = min(p.kv_heads, p.hkv - head), lines = (p.d * (int)sizeof(T) + 127) / 128;
+      const char* from = static_cast<const char*>(part & 1 ? p.v : p.k);
+      const long long token_stride = (part & 1 ? p.v_token : p.k_token) * (long long)sizeof(T), head_stride = (part & 1 ? p.v_head : p.k_head) * (long long)sizeof(T);
+      for (int i = threadIdx.x; i < p.window * heads * lines; i += 32 * kRaWarps) {
+        const long long token = base + i / (heads * lines);
+        const int j = i % (heads * lines);
+        if (token < p.n_tokens)
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(from + token * token_stride + (head + j / lines) * head_stride + j % lines * 128));
+      }
+    }
     // lane l looks at token base - 1 + l: the one in front tells whether the window's first token begins a run
     const RaToken t = ra_token(p, (int)base - 1 + lane);
     const long long in_front = __shfl_up_sync(kFullMask, t.entry, 1);
@@ -283,51 +382,56 @@ __global__ void __launch_bounds__(32 * kRaWarps) rope_append_kernel(RopeAppendPa
           if (add < 32) break;
         }
       }
-      ra_run<T, C, kLanes>(p, first, n, entry, block, head, part & 1, table, lane);
+      ra_run<T, C, kLanes, kShare>(p, first, n, entry, block, head, min(p.hkv, head + p.kv_heads), part & 1, tables, warp, lane);
     }
     return;
   }
   // queries: items of `item_heads` heads of a token
-  const int sub = lane / kLanes, col = (lane % kLanes) * 8, half = p.rot >> 1;
+  constexpr int kHold = sizeof(T) == 4 ? 4 : 8;  // a token's rows of eight heads on their way before its angles are made
+  float2* table = tables[warp];
+  const int sub = lane / kLanes, col = (lane % kLanes) * 8;
   const bool inside = col < p.d;
+  const RaPairs pairs = ra_pairs<kLanes>(p, lane);
   const int chunks = (p.hq + p.item_heads - 1) / p.item_heads, items = p.window * chunks;
   for (int item = ((int)blockIdx.y - p.kv_ctas) * kRaWarps + warp; item < items; item += p.q_ctas * kRaWarps) {
     const long long token = base + item / chunks;
     if (token >= p.n_tokens) break;
     const int h0 = item % chunks * p.item_heads, h1 = min(p.hq, h0 + p.item_heads);
-    const T* src = static_cast<const T*>(p.q) + token * p.q_token;
-    T* dst = static_cast<T*>(p.q_out) + token * p.hq * p.d;
+    const T* src = static_cast<const T*>(p.q) + token * p.q_token + (h0 + sub) * p.q_head;
+    T* dst = static_cast<T*>(p.q_out) + (token * p.hq + h0 + sub) * p.d + col;
+    const long long step = kRows * p.q_head;
+    RaFactors f;
     bool made = false;
-    for (int h = h0; h < h1; h += kRaHold * kRows) {
-      QRaw<T> raw[kRaHold];
+    for (int h = h0; h < h1; h += kHold * kRows) {
+      QRaw<T> raw[kHold];
 #pragma unroll
-      for (int s = 0; s < kRaHold; ++s) {
+      for (int s = 0; s < kHold; ++s) {
         const int mine = h + s * kRows + sub;
-        if (mine < h1 && inside) raw[s] = q_load8(src + mine * p.q_head + col);
+        if (mine < h1 && inside) raw[s] = q_load8(src + s * step + col);
       }
-      if (!made && half > 0) {
+      if (!made && pairs.half > 0) {
         __syncwarp();
-        const int pos = p.positions[token];
-        for (int f = lane; f < half; f += 32) {
-          float c, s;
-          cos_sin((double)pos * (double)p.inv_freq[f], c, s);
-          table[f] = make_float2(c, s);
-        }
+        ra_angles(table, p.inv_freq, pairs.half, p.positions[token], lane, 32);
         __syncwarp();
+        if (pairs.whole) ra_factors(f, table, pairs, col);
         made = true;
       }
 #pragma unroll
-      for (int s = 0; s < kRaHold; ++s) {
+      for (int s = 0; s < kHold; ++s) {
         if (h + s * kRows >= h1) break;
         const int mine = h + s * kRows + sub;
         const bool live = mine < h1 && inside;
         float x[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = 0.f;
-        if (live) q_floats(raw[s], x);
-        if (half > 0) ra_turn<T, kLanes>(x, src + mine * p.q_head, table, p.rot, p.interleaved, col, lane, live);
-        if (live) ra_store<T>(dst + (long long)mine * p.d + col, ra_pack<T>(x));
+        if (pairs.half > 0 && pairs.whole) {
+          ra_turn(x, raw[s], f, pairs);
+        } else {
+          q_floats(raw[s], x);
+          if (pairs.half > 0 && live) ra_turn_odd(x, src + s * step, table, pairs, col);
+        }
+        if (live) ra_store<T>(dst + s * kRows * p.d, ra_pack<T>(x));
       }
+      src += kHold * step;
+      dst += kHold * kRows * p.d;
     }
   }
 }
@@ -337,18 +441,23 @@ static int launch_rope_append(RopeAppendParams p, cudaStream_t stream) {
   // Batches of a few tokens per row: a token per CTA column, its heads dealt out.  Prompts: windows of 16 tokens, in which one run begins, mostly.
   const long long rows = p.packed ? (p.query_start_loc ? p.qsl_rows : 1) : (p.n_tokens + p.n_cols - 1) / p.n_cols;
   const bool prompt = p.n_tokens > 4 * (rows > 0 ? rows : 1);
-  const int lanes = p.d <= 64 ? 8 : p.d <= 128 ? 16 : 32;
+  const int lanes = p.d <= 64 ? 8 : p.d <= 128 ? 16 : 32, at_once = 32 / lanes;
   p.window = prompt ? 16 : 1;
-  p.item_heads = prompt ? p.hq : 32 / lanes;
-  p.kv_ctas = (2 * p.hkv + kRaWarps - 1) / kRaWarps;
+  p.kv_heads = prompt ? 2 : 1;
+  const int parts = 2 * ((p.hkv + p.kv_heads - 1) / p.kv_heads);
+  p.kv_ctas = prompt ? parts : (parts + kRaWarps - 1) / kRaWarps;
+  p.item_heads = prompt ? 8 * at_once : at_once;
   const int items = p.hq > 0 ? p.window * ((p.hq + p.item_heads - 1) / p.item_heads) : 0;
-  p.q_ctas = (items + kRaWarps - 1) / kRaWarps;
-  if (prompt && p.q_ctas > 2) p.q_ctas = 2;
+  p.q_ctas = (items + kRaWarps * (prompt ? 2 : 1) - 1) / (kRaWarps * (prompt ? 2 : 1));
   const dim3 grid((unsigned)((p.n_tokens + p.window - 1LL) / p.window), p.kv_ctas + p.q_ctas);
   auto go = [&](auto* kernel) { return launch_after(kernel, grid, dim3(32 * kRaWarps), 0, stream, p) == cudaSuccess ? NVJ_OK : NVJ_ERR_LAUNCH; };
-  if (lanes == 8) return go(rope_append_kernel<T, C, 8>);
-  if (lanes == 16) return go(rope_append_kernel<T, C, 16>);
-  return go(rope_append_kernel<T, C, 32>);
+  auto shared = [&](auto width) {
+    constexpr int kLanes = decltype(width)::value;
+    return prompt ? go(rope_append_kernel<T, C, kLanes, kRaWarps>) : go(rope_append_kernel<T, C, kLanes, 1>);
+  };
+  if (lanes == 8) return shared(std::integral_constant<int, 8>{});
+  if (lanes == 16) return shared(std::integral_constant<int, 16>{});
+  return shared(std::integral_constant<int, 32>{});
 }
 template <typename T>
 static int launch_rope_append_cache(const RopeAppendParams& p, int cache_dtype, cudaStream_t s) {

@@ -461,14 +461,15 @@ __global__ void __launch_bounds__(kSdThreads) selected_decode_kernel(SelectedPar
   sd_merge<kCols, S::kAccPitch>(p, reinterpret_cast<float*>(sd_smem), sd_ml, sd_ML, token, head, ct * kCols, dims, ctas, rank);
 }
 
-// CTAs per cluster: as many as are resident at once, two to an SM, and no more than one per four tiles.  Lists are of one length, so that more of them gain nothing at
-// the end and cost their start (512 lists of 64 16-key tiles of 256 dims: one CTA each 89 us, two 105, four 122; 10 lists of 32: eight 7.1, four 8.6, one 15).
+// CTAs per cluster: as many as are resident at once, two to an SM less what clusters leave unused, up to 8 (16, which are placed one by one, for up to four lists), and no
+// more than one per four tiles.  Lists are of one length, so that more CTAs than that gain nothing at the end and cost their start.  64 16-key tiles of 256 dims:
+// 2 lists 16 CTAs 7.2 us, 8 8.4; 16 lists 8 10.9, 16 16.4; 64 lists 4 18.5, 6 27.8; 128 lists 2 28.3, 1 33.6; 512 lists 1 89, 2 105.
 static int selected_decode_ctas(long long units, long long tiles, int sms) {
-  long long c = 2LL * sms / units;
+  long long c = 7LL * sms / (4 * units);
   if (c < 1 && 2 * units < 5LL * sms) c = 2;  // (a round and a bit: halves; 320 lists of 64: one CTA 77, two 68; 384 of 96 tiles of 128 dims: 50, 55)
-  const long long useful = (tiles + kSdWarps - 1) / kSdWarps;
+  const long long useful = (tiles + kSdWarps - 1) / kSdWarps, most = units > 4 ? 8 : 16;
   c = c < useful ? c : useful;
-  return (int)(c < 1 ? 1 : (c > 16 ? 16 : c));
+  return (int)(c < 1 ? 1 : (c > most ? most : c));
 }
 
 // A launch of `kernel`, whose CTAs take `columns` heads of a group and `keys` keys of a list at a time.
