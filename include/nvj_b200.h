@@ -546,7 +546,7 @@ int nvj_rope_kv_append(const void* q, int64_t q_token_stride, int64_t q_head_str
                        nvj_stream_t stream);
 
 /*
- * The blocks that each query token is to read: q [rows, width, num_q_heads, head_dim]; token t of row b sees the blocks with keys p < seq_lens[b]
+ * The blocks that each query token is to read, by bounds with low <= high: q [rows, width, num_q_heads, head_dim]; token t of row b sees the blocks with keys p < seq_lens[b]
  * and, with positions given ([rows, width]), p <= positions[b, t].  A block's score for a kv head is the largest, over the group's query heads, of
  *     sum_d max(q_d, 0) high_d + min(q_d, 0) low_d
  * (with a positive scale an upper bound of its keys' scores).  Chosen are the `first` first and the `last` last blocks (first + last <= budget)

@@ -106,6 +106,21 @@ __device__ __forceinline__ uint32_t bs_scan(uint32_t x, BsShared& s, int& which,
   return front + y - x;
 }
 
+// Sum over the CTA of one number per thread.
+__device__ __forceinline__ uint32_t bs_total(uint32_t x, BsShared& s, int& which) {
+  const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  x = __reduce_add_sync(kFullMask, x);
+  uint32_t* scan = s.scan[which];
+  which ^= 1;
+  if ((threadIdx.x & 31) == 0) scan[warp] = x;
+  __syncthreads();
+  uint32_t total = 0;
+#pragma unroll
+  for (int w = 0; w < kBsMostWarps; ++w)
+    if (w < warps) total += scan[w];
+  return total;
+}
+
 // The `want`-th largest (from 1) of keys[begin .. end), which lie in [least, largest]; `above`: how many are larger.  Each step deals the keys of the
 // interval to bins of equal width and goes on in the one that holds it: scores of one size spread over the bins at once, where digits
 // of the numbers themselves would put them all into a few.  (Four bins a thread for short rows.)
@@ -375,7 +390,8 @@ struct BsLanes {
 // The same on tensor-core tiles, for bf16 and f16 bounds and up to 16 query heads of a kv head: the blocks are the rows of an mma.sync tile, the heads its
 // columns, and the contraction runs over the 2 D bounds, the positive parts of the queries standing against the high ones, the negative parts against the low.
 // A lane's 16 bytes of a block's bounds are its operands as they come (selected_decode.cuh); 128 dims of 16 blocks are under way in
-// registers, and each piece is asked for again as soon as it has been used.
+// registers and asked for again when all have been used.  (Each piece as soon as it has been used: 64 rows of 1024 - 4096 blocks 90 us instead of 83.  Through shared
+// memory, by 16-byte asynchronous copies into two stages per warp, 89; by bulk copies of 256 bytes 134, the copy engine's limit.)
 // kRagged: a head_dim below kD, its missing dims zero.
 template <typename C, int kD, int kTiles, int kTerms, bool kRagged>
 struct BsTiles {
@@ -461,14 +477,14 @@ struct BsTiles {
         if (!kRagged || dim + 8 * (lane & 3) < p.d) held[piece][b][r] = ld_stream_u4(at[r] + b * (kRagged ? p.d : kD) + dim);
         else held[piece][b][r] = make_uint4(0, 0, 0, 0);
   }
-  // The larger magnitudes of two words' numbers.
-  static __device__ __forceinline__ uint32_t size(uint32_t a, uint32_t b) {
+  // The larger magnitudes of two words' bounds: low <= high, so that it is that of high or of -low.
+  static __device__ __forceinline__ uint32_t size(uint32_t low, uint32_t high) {
     uint32_t y;
     if constexpr (std::is_same<C, __half>::value) {
-      const __half2 x = __hmax2(__habs2(*reinterpret_cast<const __half2*>(&a)), __habs2(*reinterpret_cast<const __half2*>(&b)));
+      const __half2 x = __hmax2(*reinterpret_cast<const __half2*>(&high), __hneg2(*reinterpret_cast<const __half2*>(&low)));
       y = *reinterpret_cast<const uint32_t*>(&x);
     } else {
-      const __nv_bfloat162 x = __hmax2(__habs2(*reinterpret_cast<const __nv_bfloat162*>(&a)), __habs2(*reinterpret_cast<const __nv_bfloat162*>(&b)));
+      const __nv_bfloat162 x = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&high), __hneg2(*reinterpret_cast<const __nv_bfloat162*>(&low)));
       y = *reinterpret_cast<const uint32_t*>(&x);
     }
     return y;
@@ -514,8 +530,9 @@ struct BsTiles {
 #pragma unroll
             for (int i = 0; i < 4; ++i) acc[j][i] += sum[i];
           }
-          ask(p, piece, half == kHalves - 1 ? 0 : half + 1, lane);
         }
+#pragma unroll
+        for (int piece = 0; piece < kPieces; ++piece) ask(p, piece, half == kHalves - 1 ? 0 : half + 1, lane);
       }
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
@@ -645,12 +662,12 @@ __global__ void __launch_bounds__(32 * kBsMostWarps, kD == 0 && kTiles > 1 ? 1 :
       const uint32_t low = max(bs_key(__double2float_ru((double)t - 2.0 * eps)), bs_key(-INFINITY) + 1u),
                      high = min(bs_key(__double2float_rd((double)t + 2.0 * eps)), kBsInfinity - 1u);
       // how many are in for sure (in the upper half of the sum), and how many stand between
-      uint32_t mine = 0, all;
+      uint32_t mine = 0;
       for (int i = begin + threadIdx.x; i < end; i += threads) {
         const uint32_t k = keys[i];
         mine += k > high ? 0x10000u : k >= low ? 1u : 0u;
       }
-      bs_scan(mine, s, which, all);
+      const uint32_t all = bs_total(mine, s, which);
       const uint32_t in = all >> 16, between = all & 0xffffu;
       if (in + between == want) {
         border = low;
@@ -695,10 +712,9 @@ __global__ void __launch_bounds__(32 * kBsMostWarps, kD == 0 && kTiles > 1 ? 1 :
           });
           border = bs_nth(keys, begin, end, want, 0u, 0xffffffffu, s, which, above);
           take_equal = want - above;
-          uint32_t equal = 0, all_equal;
+          uint32_t equal = 0;
           for (int i = begin + threadIdx.x; i < end; i += threads) equal += keys[i] == border;
-          bs_scan(equal, s, which, all_equal);
-          if (all_equal == take_equal) break;
+          if (bs_total(equal, s, which) == take_equal) break;
           // more of one key than there is room for: equal scores, or a window that is too wide for them
           double lowest = INFINITY, highest = -INFINITY;
           bs_rescore(p, s, keys, table, q_at, head, begin, end, border, [&](int, double x) {
