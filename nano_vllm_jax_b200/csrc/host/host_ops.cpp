@@ -857,6 +857,9 @@ QueryRows query_rows(const at::Tensor* q, const at::Tensor* tab, const at::Tenso
   return r;
 }
 constexpr long long kMostColumns = 45056;  // block-table columns that a selection takes
+bool budget_holds(long long budget, long long first, long long last) {
+  return budget >= 1 && budget <= 0x7fffffffLL && first >= 0 && last >= 0 && first <= budget && last <= budget - first;
+}
 at::Tensor selection(const QueryRows& r, long long hkv, long long budget, int device) {
   at::Tensor t = r.wide ? empty({r.batch, r.width, hkv, budget}, at::kInt, device) : empty({r.batch, hkv, budget}, at::kInt, device);
   if (env_is("NVJ_POISON_OUTPUT", "1")) t.fill_(1 << 30);
@@ -874,7 +877,7 @@ PyObject* select_blocks(PyObject* const* a, Py_ssize_t n) {
     NVJ_NONE();
   const int device = b->get_device(), hkv = (int)b->size(1), d = (int)b->size(3);
   const QueryRows r = query_rows(q, tab, len, pos, device, hkv, d);
-  if (!r.ok || bs < 1 || bs > 65536 || budget < 1 || budget > 0x7fffffffLL || first < 0 || last < 0 || first + last > budget || tab->size(1) > kMostColumns) NVJ_NONE();
+  if (!r.ok || bs < 1 || bs > 65536 || !budget_holds(budget, first, last) || tab->size(1) > kMostColumns) NVJ_NONE();
   const c10::cuda::OptionalCUDAGuard guard(c10::Device(c10::kCUDA, (c10::DeviceIndex)device));
   void* stream = stream_of(device);
   int32_t* st = status_for(device, stream);
@@ -934,7 +937,7 @@ PyObject* selective_step(PyObject* const* a, Py_ssize_t n) {
   RopeRows rk, rv;
   if (!r.ok || r.hq != l.hkv * groups || !new_rows(k, v, l) || k->size(0) != r.batch || k->size(1) != r.width || !rope_rows(*k, l.device, &rk) ||
       !rope_rows(*v, l.device, &rv) || pos->dim() != 2 || pos->size(0) != r.batch || !meta(*qsl, l.device) || qsl->dim() != 1 || qsl->numel() < 1 ||
-      tab->numel() == 0 || l.blocks == 0 || tab->size(1) > kMostColumns || !(scale > 0) || budget < 1 || first < 0 || last < 0 || first + last > budget ||
+      tab->numel() == 0 || l.blocks == 0 || tab->size(1) > kMostColumns || !(scale > 0) || !budget_holds(budget, first, last) ||
       tab->size(1) <= budget || (max_len >= 0 && max_len < tab->size(1) * bs))
     NVJ_NONE();
   if (!on(*b, l.device) || b->dtype() != kc->dtype() || b->dim() != 5 || b->size(0) != kc->size(0) || b->size(1) != l.blocks || b->size(2) != l.hkv ||

@@ -438,17 +438,24 @@ __global__ void __launch_bounds__(32 * kRaWarps, sizeof(T) == 4 ? 4 : 5) rope_ap
 
 template <typename T, typename C>
 static int launch_rope_append(RopeAppendParams p, cudaStream_t stream) {
-  // Batches of a few tokens per row: a token per CTA column, its heads dealt out.  Prompts: windows of 16 tokens, in which one run begins, mostly.
-  const long long rows = p.packed ? (p.query_start_loc ? p.qsl_rows : 1) : (p.n_tokens + p.n_cols - 1) / p.n_cols;
-  const bool prompt = p.n_tokens > 4 * (rows > 0 ? rows : 1);
+  // Batches of a few tokens per row: a token per CTA column, its parts and heads dealt to warps.  Prompts: windows of up to 16 tokens, a row's mean, so that one run begins in
+  // each, mostly (a window's runs come one behind the other: 8 rows of 5 tokens 18.7 us with windows of 16), shared by a CTA's warps.  The more tokens, the more heads a warp
+  // takes, so that cosines are made less often.
+  const long long n = p.n_tokens, rows = p.packed ? (p.query_start_loc ? p.qsl_rows : 1) : (n + p.n_cols - 1) / p.n_cols;
+  const long long mean = n / (rows > 0 ? rows : 1);
+  const bool prompt = mean > 4;
   const int lanes = p.d <= 64 ? 8 : p.d <= 128 ? 16 : 32, at_once = 32 / lanes;
-  p.window = prompt ? 16 : 1;
-  p.kv_heads = prompt ? 2 : 1;
+  p.window = prompt ? (int)(mean < 16 ? mean : 16) : 1;
+  const long long windows = (n + p.window - 1) / p.window;
+  auto within = [](long long x, long long low, long long high) { return (int)(x < low ? low : x > high ? high : x); };
+  p.kv_heads = prompt ? (windows * 2 * p.hkv > 20 * 148 ? 2 : 1) : within(n * 2 * p.hkv / (32 * 148), 1, 4);
   const int parts = 2 * ((p.hkv + p.kv_heads - 1) / p.kv_heads);
   p.kv_ctas = prompt ? parts : (parts + kRaWarps - 1) / kRaWarps;
-  p.item_heads = prompt ? 8 * at_once : at_once;
-  const int items = p.hq > 0 ? p.window * ((p.hq + p.item_heads - 1) / p.item_heads) : 0;
-  p.q_ctas = (items + kRaWarps * (prompt ? 2 : 1) - 1) / (kRaWarps * (prompt ? 2 : 1));
+  const int steps = (p.hq + at_once - 1) / at_once, each = within(n * steps / (20 * 148), 1, 16);  // of a token; of a warp
+  const int item = within(each, 1, steps < 8 ? (steps > 0 ? steps : 1) : 8);
+  p.item_heads = item * at_once;
+  const int items = p.hq > 0 ? p.window * ((p.hq + p.item_heads - 1) / p.item_heads) : 0, of_warp = prompt && each > item ? each / item : 1;
+  p.q_ctas = (items + kRaWarps * of_warp - 1) / (kRaWarps * of_warp);
   const dim3 grid((unsigned)((p.n_tokens + p.window - 1LL) / p.window), p.kv_ctas + p.q_ctas);
   auto go = [&](auto* kernel) { return launch_after(kernel, grid, dim3(32 * kRaWarps), 0, stream, p) == cudaSuccess ? NVJ_OK : NVJ_ERR_LAUNCH; };
   auto shared = [&](auto width) {

@@ -65,7 +65,8 @@ class SelectiveKVCacheStorage(KVCacheStorage):
     """A cache whose decode attention reads selected blocks (not in the reference): beside the pages `[num_layers, num_blocks, block_size,
     num_kv_heads, head_dim]` the bounds of every block's keys `[num_layers, num_blocks, num_kv_heads, 2, head_dim]` (the smallest
     number of each dimension, then the largest), kept by the append.  Of a row's blocks decode reads the `first` first, the `last`
-    last and those of the highest scores, `budget` in all (`kernels/selective_kv.py`); prefill reads all of them."""
+    last and those of the highest scores, `budget` in all (`kernels/selective_kv.py`); prefill reads all of them.  The backend's own appends keep
+    the bounds; kernels that write the pages alone (fused append and decode, a captured `DecodeStepGraph`) leave them behind."""
 
     k_bounds: torch.Tensor
     budget: int

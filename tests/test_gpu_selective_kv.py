@@ -392,3 +392,85 @@ def test_attention_flags_blocks_outside_the_pool():
             S.paged_decode_attention_selected(q, k, v, _i32([[0, bad, 2]]), _i32([48]), chosen, 0.1)
     with pytest.raises(K.DeviceStatusError, match="sequence length"):
         S.paged_decode_attention_selected(q, k, v, _i32([[0, 1, 2]]), _i32([49]), chosen, 0.1)
+
+
+# ------------------------------------------------------------------------------------------------ refusals and empty calls
+
+def _small():
+    g = _gen(20)
+    k, v = _normal(g, BF16, 6, 16, 2, 64), _normal(g, BF16, 6, 16, 2, 64)
+    return dict(k=k, v=v, b=torch.stack((k.amin(1), k.amax(1)), 2).contiguous(), q=_normal(g, BF16, 2, 1, 8, 64), kv=_normal(g, BF16, 2, 1, 2, 64),
+                pos=_i32([[3], [20]]), tab=_i32([[0, 1, 2], [3, 4, 5]]), lens=_i32([4, 21]), sel=_i32(np.zeros((2, 1, 2, 2))), freq=torch.ones(32, device="cuda"))
+
+
+def _bad(s, **change):
+    return dict(s, **{k: f(s[k]) for k, f in change.items()})
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(k=lambda t: t.half()), "one shape, dtype"), (dict(k=lambda t: t[:, :, :, :20].contiguous(), v=lambda t: t[:, :, :, :20].contiguous()), "multiple of 8"),
+    (dict(k=lambda t: t.transpose(1, 2)), "NHD"), (dict(kv=lambda t: t[..., :32]), "heads those of the cache"), (dict(q=lambda t: t.float()), "same dtype"),
+    (dict(q=lambda t: t[:1]), "query must have shape"), (dict(b=lambda t: t.float()), "cache's dtype"), (dict(b=lambda t: t[:5].contiguous()), "k_bounds"),
+    (dict(b=lambda t: t.transpose(0, 1)), "k_bounds must be contiguous"), (dict(pos=lambda t: t.long()), "int32"), (dict(pos=lambda t: t[:1]), "positions must have shape"),
+    (dict(tab=lambda t: t[:1]), "batch dimensions"), (dict(tab=lambda t: t[0]), "2D"), (dict(tab=lambda t: t[:, :0]), "not empty"), (dict(lens=lambda t: t[:1]), "seq_lens"),
+    (dict(freq=lambda t: t.double()), "inv_freq"), (dict(freq=lambda t: torch.ones(33, device="cuda")), "inv_freq")])
+def test_append_refusals(change, match):
+    s = _bad(_small(), **change)
+    with pytest.raises(ValueError, match=match):
+        S.rope_kv_append(s["q"], s["kv"], s["kv"], s["k"], s["v"], s["pos"], s["tab"], s["freq"], k_bounds=s["b"], seq_lens=s["lens"])
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(q=lambda t: t[..., :32]), "head_dim must match"), (dict(q=lambda t: t[:, :, :3]), "divisible"), (dict(q=lambda t: t.double()), "dtype"),
+    (dict(q=lambda t: t[0, 0]), "q must have shape"), (dict(b=lambda t: t[:, :, :1]), "k_bounds"), (dict(tab=lambda t: t[:1]), "block_table"),
+    (dict(lens=lambda t: t.long()), "int32"), (dict(pos=lambda t: t[:1]), "positions"),
+    (dict(tab=lambda t: torch.zeros(2, S.MOST_COLUMNS + 1, dtype=torch.int32, device="cuda")), "columns")])
+def test_selection_refusals(change, match):
+    s = _bad(_small(), **change)
+    with pytest.raises(ValueError, match=match):
+        S.select_blocks(s["q"], s["b"], s["tab"], s["lens"], 16, 2, positions=s["pos"])
+
+
+@pytest.mark.parametrize("budget,first,last,block", [(0, 0, 0, 16), (2, 2, 1, 16), (2, -1, 1, 16), (2, 1, 2 ** 62, 16), (2, 2 ** 62, 2 ** 62, 16), (2, 1, 1, 0)])
+def test_selection_refuses_budgets(budget, first, last, block):
+    s = _small()
+    with pytest.raises(ValueError, match="budget|block_size"):
+        S.select_blocks(s["q"], s["b"], s["tab"], s["lens"], block, budget, first=first, last=last)
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(sel=lambda t: t[:, 0]), "selected"), (dict(sel=lambda t: t[:1]), "selected"), (dict(sel=lambda t: t.long()), "int32"), (dict(k=lambda t: t.float()), "one shape"),
+    (dict(q=lambda t: t[..., :32]), "head_dim"), (dict(q=lambda t: t[:, :, :3]), "divisible"), (dict(lens=lambda t: t[:1]), "seq_lens")])
+def test_attention_refusals(change, match):
+    s = _bad(_small(), **change)
+    with pytest.raises(ValueError, match=match):
+        S.paged_decode_attention_selected(s["q"], s["k"], s["v"], s["tab"], s["lens"], s["sel"], 0.1)
+
+
+def test_empty_batches_and_lists():
+    s = _small()
+    none = _i32(np.zeros((0, 3)))
+    assert S.select_blocks(s["q"][:0], s["b"], none, s["lens"][:0], 16, 2).shape == (0, 1, 2, 2)
+    assert S.paged_decode_attention_selected(s["q"][:0], s["k"], s["v"], none, s["lens"][:0], s["sel"][:0], 0.1).shape == (0, 1, 512)
+    assert S.rope_kv_append(s["q"][:0], s["kv"][:0], s["kv"][:0], s["k"], s["v"], s["pos"][:0], s["tab"], s["freq"]).shape == (0, 1, 8, 64)
+    assert not S.paged_decode_attention_selected(s["q"], s["k"], s["v"], s["tab"], s["lens"], s["sel"][..., :0], 0.1).any()
+    assert not S.paged_decode_attention_selected(s["q"], s["k"], s["v"], s["tab"][:, :0], _i32([0, 0]), s["sel"], 0.1).any()
+    assert (S.select_blocks(s["q"], s["b"], s["tab"][:, :0], _i32([0, 0]), 16, 2) == -1).all()
+    before = s["b"].clone()
+    S.rope_kv_append(None, s["kv"], s["kv"], s["k"], s["v"], s["pos"], s["tab"], None, k_bounds=s["b"], seq_lens=_i32([0, -5]))
+    assert torch.equal(s["b"], before)
+
+
+def test_metadata_that_is_not_contiguous_is_read_as_it_is():
+    g = _gen(21)
+    s = _small()
+    wide = torch.zeros(2, 6, dtype=torch.int32, device="cuda")
+    wide[:, ::2] = s["tab"]
+    q = _normal(g, BF16, 2, 8, 2, 64).transpose(1, 2)  # [2, 2, 8, 64]
+    pos = _i32([[3, 3], [19, 20]])
+    a = S.select_blocks(q, s["b"], wide[:, ::2], s["lens"], 16, 1, positions=pos, first=0, last=0)
+    b = S.select_blocks(q.contiguous(), s["b"], s["tab"], s["lens"], 16, 1, positions=pos, first=0, last=0)
+    assert torch.equal(a, b)
+    x = S.paged_decode_attention_selected(q, s["k"], s["v"], wide[:, ::2], s["lens"], a, 0.1, positions=pos)
+    y = S.paged_decode_attention_selected(q.contiguous(), s["k"], s["v"], s["tab"], s["lens"], b, 0.1, positions=pos)
+    assert torch.equal(x, y)
