@@ -52,19 +52,6 @@ __device__ __forceinline__ uint32_t bs_key(float x) {
 }
 __device__ __forceinline__ float bs_float(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key); }
 
-__device__ __forceinline__ float bs_load(const void* p, long long i, int dtype) {
-  if (dtype == NVJ_F32) return static_cast<const float*>(p)[i];
-  if (dtype == NVJ_F16) return __half2float(static_cast<const __half*>(p)[i]);
-  return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
-}
-
-__device__ __forceinline__ float4 bs_load4(const void* p, long long i, int dtype) {
-  if (dtype == NVJ_F32) return *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
-  const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
-  const float2 a = dtype == NVJ_F16 ? q_float2(v.x) : bf16x2_to_float2(v.x), b = dtype == NVJ_F16 ? q_float2(v.y) : bf16x2_to_float2(v.y);
-  return make_float4(a.x, a.y, b.x, b.y);
-}
-
 // What a warp of the cluster leaves with the scores: the largest sum of magnitudes that it has met in a block of a finite score, and the ends of its keys.
 struct BsEnds {
   float most;
@@ -201,18 +188,33 @@ __device__ __forceinline__ uint32_t bs_nth(const uint32_t* keys, int begin, int 
   }
 }
 
+__device__ __forceinline__ float4 bs_load4(const void* p, long long i, int dtype) {
+  if (dtype == NVJ_F32) return *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+  const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
+  const float2 a = dtype == NVJ_F16 ? q_float2(v.x) : bf16x2_to_float2(v.x), b = dtype == NVJ_F16 ? q_float2(v.y) : bf16x2_to_float2(v.y);
+  return make_float4(a.x, a.y, b.x, b.y);
+}
+
 // Score of one block in 64 bits, by a warp; the same in every lane.
 static __device__ double bs_exact(const SelectParams& p, long long q_at, long long bounds_at, int lane) {
   double best = -INFINITY;
   for (int g0 = 0; g0 < p.groups; g0 += 4) {  // four heads' loads in flight
     double sum[4] = {0.0, 0.0, 0.0, 0.0};
-    for (int d = lane; d < p.d; d += 32) {
-      const float low = bs_load(p.bounds, bounds_at + d, p.cache_dtype), high = bs_load(p.bounds, bounds_at + p.d + d, p.cache_dtype);
-      float q[4];
 #pragma unroll
-      for (int g = 0; g < 4; ++g) q[g] = g0 + g < p.groups ? bs_load(p.q, q_at + (long long)(g0 + g) * p.d + d, p.q_dtype) : 0.f;
+    for (int i = 0; i < 2; ++i) {
+      const int d = 128 * i + 4 * lane;
+      if (d >= p.d) continue;
+      const float4 low = bs_load4(p.bounds, bounds_at + d, p.cache_dtype), high = bs_load4(p.bounds, bounds_at + p.d + d, p.cache_dtype);
+      float4 q[4];
 #pragma unroll
-      for (int g = 0; g < 4; ++g) sum[g] += (double)q[g] * (double)(q[g] > 0.f ? high : low);
+      for (int g = 0; g < 4; ++g) q[g] = g0 + g < p.groups ? bs_load4(p.q, q_at + (long long)(g0 + g) * p.d + d, p.q_dtype) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        sum[g] += (double)q[g].x * (double)(q[g].x > 0.f ? high.x : low.x);
+        sum[g] += (double)q[g].y * (double)(q[g].y > 0.f ? high.y : low.y);
+        sum[g] += (double)q[g].z * (double)(q[g].z > 0.f ? high.z : low.z);
+        sum[g] += (double)q[g].w * (double)(q[g].w > 0.f ? high.w : low.w);
+      }
     }
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
