@@ -227,7 +227,7 @@ class B200Backend:
                   scale, num_key_value_groups, is_prefill):
         if type(cache) is QuantizedKVCacheStorage:
             return self._attend_quantized(layer_id, query, cache, metadata, block_size, scale, num_key_value_groups, is_prefill)
-        if type(cache) is SelectiveKVCacheStorage and not is_prefill and metadata.block_tables.shape[1] > cache.budget:
+        if type(cache) is SelectiveKVCacheStorage and not is_prefill:
             return self._attend_selected(layer_id, query, cache, metadata, block_size, scale, num_key_value_groups)
         f32 = torch.float32
         if is_prefill:

@@ -938,7 +938,7 @@ PyObject* selective_step(PyObject* const* a, Py_ssize_t n) {
   if (!r.ok || r.hq != l.hkv * groups || !new_rows(k, v, l) || k->size(0) != r.batch || k->size(1) != r.width || !rope_rows(*k, l.device, &rk) ||
       !rope_rows(*v, l.device, &rv) || pos->dim() != 2 || pos->size(0) != r.batch || !meta(*qsl, l.device) || qsl->dim() != 1 || qsl->numel() < 1 ||
       tab->numel() == 0 || l.blocks == 0 || tab->size(1) > kMostColumns || !(scale > 0) || !budget_holds(budget, first, last) ||
-      tab->size(1) <= budget || (max_len >= 0 && max_len < tab->size(1) * bs))
+      (max_len >= 0 && max_len < tab->size(1) * bs))
     NVJ_NONE();
   if (!on(*b, l.device) || b->dtype() != kc->dtype() || b->dim() != 5 || b->size(0) != kc->size(0) || b->size(1) != l.blocks || b->size(2) != l.hkv ||
       b->size(3) != 2 || b->size(4) != l.d || !b->is_contiguous())

@@ -376,6 +376,36 @@ def test_attention_batches_of_all_sizes():
         _attention(rows, MODEL, (BF16, BF16), [17 * (i % 23) for i in range(rows)], None, 6)
 
 
+def test_attention_over_lists_longer_than_a_warp_looks_ahead():
+    """Lists of hundreds of tiles with one CTA for each, so that a warp fetches places several times; most rows see little of theirs."""
+    lens = [5 if i % 20 else 700 + i for i in range(160)]
+    for layout, types, entries in (((16, 2, 64, 16), (BF16, BF16), 300), ((8, 2, 128, 16), (F32, F32), 150), ((8, 2, 64, 32), (F16, F16), 170)):
+        _attention(6, layout, types, lens, None, entries)
+
+
+def test_blocks_beyond_offsets_of_32_bits():
+    """The last blocks of a pool of 2.46e9 numbers of K: appended, selected and attended as the first ones of a small pool."""
+    hq, hkv, d, bs, pool = 8, 2, 128, 16, 600_000
+    g = _gen(31)
+    small = [torch.zeros(40, bs, hkv, d, dtype=BF16, device="cuda") for _ in range(2)] + [torch.zeros(40, hkv, 2, d, dtype=BF16, device="cuda")]
+    large = [torch.empty(pool, bs, hkv, d, dtype=BF16, device="cuda") for _ in range(2)] + [torch.empty(pool, hkv, 2, d, dtype=BF16, device="cuda")]
+    for t in large:
+        t[-40:] = 0
+    n = 37 * bs + 5
+    q, nk, nv = (_normal(g, BF16, 1, n, h, d) for h in (hq, hkv, hkv))
+    one = _normal(g, BF16, 1, hq, d)
+    ids, freq = torch.zeros(1, n, dtype=torch.int32, device="cuda"), torch.from_numpy(_freq(32)).cuda()
+    outs = []
+    for (k, v, b), first in ((small, 0), (large, pool - 40)):
+        table = _i32([np.arange(40)[::-1] + first])
+        turned = S.rope_kv_append(q, nk, nv, k, v, _i32([np.arange(n)]), table, freq, k_bounds=b, token_row_ids=ids)
+        chosen = S.select_blocks(one, b, table, _i32([n]), bs, 9)
+        out = S.paged_decode_attention_selected(one, k, v, table, _i32([n]), chosen, d ** -0.5)
+        outs.append((turned, chosen, out, k[-40:], v[-40:], b[-40:]))
+    for x, y in zip(*outs):
+        assert torch.equal(x, y)
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.1, 3.0, 1e-4])
 def test_attention_scales(scale):
     for layout, types in ((MODEL, (BF16, BF16)), ((32, 8, 128, 32), (F16, F16)), ((6, 3, 96, 16), (F32, F32))):

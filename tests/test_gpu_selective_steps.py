@@ -116,7 +116,7 @@ def test_a_budget_that_covers_the_row_gives_full_attention():
     lens = np.array([250, 17, 96])
     tables = rng.permutation(400)[: 3 * 20].reshape(3, 20)
     outs = []
-    for budget in (16, 20, 100):  # fewer columns than the tables' 20, as many, more: the last two take the kernels that read every block
+    for budget in (16, 20, 100):  # as many as the longest row's blocks, as the tables' columns, more
         backend, cache = _backend(budget, layers=1)
         g.manual_seed(3)
         cache = _prefill(backend, cache, 0, tables, lens - 1, g)
