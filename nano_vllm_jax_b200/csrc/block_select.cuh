@@ -13,8 +13,9 @@
 // four rows, 12 - 19 for long ones.)
 //
 // One thread-block cluster per query token and kv head: its warps score 16 blocks at a time and leave the scores, as ordered
-// integers, in the first CTA's shared memory, which finds the border by a radix selection and writes the columns in ascending order.
-// No workspace, no second launch.  Bound by the bytes of the bounds, 2 head_dim numbers per block and kv head: 1/block_size of the cache.
+// integers, in the first CTA's shared memory, which finds the border by bins over the scores' range and writes the columns in ascending order.
+// No workspace, no second launch.  Bound by the bytes of the bounds, 2 head_dim numbers per block and kv head: 1/block_size of the cache: 64 rows of 1024 - 4096 blocks, 2 heads
+// of 256, 336 MB in 78 us (51 at the copy rate), 256 of 128 - 512 41 (26), 4 rows of 512 7.4.
 
 #pragma once
 
@@ -772,12 +773,12 @@ __global__ void __launch_bounds__(32 * kBsMostWarps, kD == 0 && kTiles > 1 ? 1 :
 }
 
 // How a call is cut: CTAs per cluster and their warps.  A CTA has ~8 us beside its stream (ids, queries, border, output), which others hide.
-//   * Many rows, or short ones: four warps each, four CTAs to an SM (256 rows of 128 - 512 blocks, 2 heads of 256: 46 us, two CTAs each 52, four 57; 250
-//     rows of 190: 25, with eight warps 31).
-//   * Few long rows: eight warps, as many CTAs as are resident at once (64 rows of 1000: two 32, four 37; 32: four 22, eight 26), and twice as many where each would still
-//     have more than 1024 blocks, so that the longest rows are not left alone at the end (64 rows of 1024 - 4096: two 96, four 87).
-//   * At most a CTA per tile of its warps, or per two of them where the CTAs do not all have an SM of their own (16 rows of 1000: four 18.0, eight
-//     19.9; 8 rows: four 15.0, eight 13.9).
+//   * Many rows, or short ones: four warps each, four CTAs to an SM (256 rows of 128 - 512 blocks, 2 heads of 256: 42 us, two CTAs each 46, four 52; 250
+//     rows of 190: 21, with eight warps 26).
+//   * Few long rows: eight warps, as many CTAs as are resident at once (64 rows of 1000: two 27, four 32; 32: four 19, eight 25), and twice as many where each would still
+//     have more than 1024 blocks, so that the longest rows are not left alone at the end (64 rows of 1024 - 4096: two 81, four 78).
+//   * At most a CTA per tile of its warps, or per two of them where the CTAs do not all have an SM of their own (16 rows of 1000: four 15.2, eight
+//     16.2; 8 rows: four 13.4, eight 12.5).
 struct BsPlan {
   int ctas, warps;
 };

@@ -12,10 +12,11 @@
 //     (S^T = K Q^T, O^T = V^T P^T), and since the order of a contraction is free, the 16 bytes that a lane holds of a row ARE its
 //     operands, permuted the same way on the other side; V takes one byte permute per word besides, which pairs its keys;
 //   * queries of another type than the cache's are sums of three terms of its type, 24 bits; weights of three bf16 or two f16 terms, 24 and 22 bits (two of
-//     bf16, 2^-17: 64 selected blocks of 256 rows 2.1e-6 from 64 bits, relative to the size of the result, instead of 4e-7).  With up to four columns
+//     bf16, 2^-17: 64 selected blocks of 256 rows 2.1e-6 from 64 bits, relative to the size of the result, instead of 4.5e-7).  With up to four columns
 //     two terms of the weights are the two halves of the eight columns of one mma.sync.  A tile's products are summed by themselves and added in fp32 (left in the
 //     tensor cores' sums, which cut their last place, 8192 keys 3e-6 - 9e-6 from 64 bits instead of 1e-7 - 5e-7; 2% of the time);
 //   * a warp walks only the tiles that are there: it holds the places of its next 32 in its lanes and takes the set bits of their vote.
+// 256 rows, 64 blocks of 16 keys, 8 heads over 2 of 256: 540 MB in 92 us, 90% of the copy rate; 48 rows, 32 heads over 8 of 128: 51 us, 91%.
 // Maxima are lazy: one vote per tile says whether a score has left them behind, and only then the sums are rescaled.
 #pragma once
 
@@ -469,10 +470,10 @@ __global__ void __launch_bounds__(kSdThreads) selected_decode_kernel(SelectedPar
 
 // CTAs per cluster: as many as are resident at once, two to an SM less what clusters leave unused, up to 8 (16, which are placed one by one, for up to four lists), and no
 // more than one per four tiles.  Lists are of one length, so that more CTAs than that gain nothing at the end and cost their start.  64 16-key tiles of 256 dims:
-// 2 lists 16 CTAs 7.2 us, 8 8.4; 16 lists 8 10.9, 16 16.4; 64 lists 4 18.5, 6 27.8; 128 lists 2 28.3, 1 33.6; 512 lists 1 89, 2 105.
+// 2 lists 16 CTAs 7.5 us, 8 8.8; 16 lists 8 11.6, 16 17.6; 64 lists 4 19.3, 6 29.4; 128 lists 2 29.2, 1 36.1; 512 lists 1 92, 2 108.
 static int selected_decode_ctas(long long units, long long tiles, int sms) {
   long long c = 7LL * sms / (4 * units);
-  if (c < 1 && 2 * units < 5LL * sms) c = 2;  // (a round and a bit: halves; 320 lists of 64: one CTA 77, two 68; 384 of 96 tiles of 128 dims: 50, 55)
+  if (c < 1 && 2 * units < 5LL * sms) c = 2;  // (a round and a bit: halves; 320 lists of 64: one CTA 84, two 78; 384 of 96 tiles of 128 dims: 52, 58)
   const long long useful = (tiles + kSdWarps - 1) / kSdWarps, most = units > 4 ? 8 : 16;
   c = c < useful ? c : useful;
   return (int)(c < 1 ? 1 : (c > most ? most : c));
