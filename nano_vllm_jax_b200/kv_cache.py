@@ -80,9 +80,9 @@ class SelectiveKVCacheStorage(KVCacheStorage):
         return tuple(_resolve_kv_layer(t, layer_id)[0] for t in (self.k_cache, self.v_cache, self.k_bounds))
 
     def copy_blocks(self, src_ids, dst_ids) -> None:
-        """Blocks `dst_ids` <- `src_ids` in every layer, their bounds with them (src and dst sets disjoint)."""
+        """Blocks `dst_ids` <- `src_ids` in every layer, their bounds with them (src and dst sets disjoint; ids outside the pool are flagged and skipped)."""
         _k.copy_blocks(self.k_cache, self.v_cache, src_ids, dst_ids)
-        self.k_bounds[:, dst_ids.long()] = self.k_bounds[:, src_ids.long()]
+        _k.copy_blocks(self.k_bounds, self.k_bounds, src_ids, dst_ids)  # (K and V's places both: the same numbers twice)
 
 
 @dataclass

@@ -156,6 +156,20 @@ def test_block_copies_take_the_bounds_along():
         assert torch.equal(t, want)
 
 
+def test_block_copies_flag_and_skip_blocks_outside_the_pool(monkeypatch):
+    monkeypatch.setenv("NVJ_CHECK_STATUS", "0")
+    backend, cache = _backend(4)
+    cache.k_cache.normal_(), cache.v_cache.normal_(), cache.k_bounds.normal_()
+    blocks = cache.k_cache.shape[1]
+    before = [t.clone() for t in (cache.k_cache, cache.v_cache, cache.k_bounds)]
+    cache.copy_blocks(_i32([3, blocks, 5, -1]), _i32([9, 10, blocks + 7, 12]))
+    with pytest.raises(K.DeviceStatusError, match="outside the pool"):
+        K.check_device_status()
+    for t, old in zip((cache.k_cache, cache.v_cache, cache.k_bounds), before):
+        old[:, 9] = old[:, 3]
+        assert torch.equal(t, old)
+
+
 def _rotated_step(g, state, q, k, v, pos, lens, freq, budget, layer=0):
     kc, vc, b = state
     turned = S.rope_kv_append(q, k, v, kc, vc, pos, g, freq, k_bounds=b, seq_lens=lens)
