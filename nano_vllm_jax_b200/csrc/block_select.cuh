@@ -150,7 +150,7 @@ __device__ __forceinline__ uint32_t bs_nth(const uint32_t* keys, int begin, int 
     for (int i = 4; i <= each; i += 4) *reinterpret_cast<uint4*>(&s.hist[top - i]) = make_uint4(0, 0, 0, 0);
     __syncthreads();
     above = s.above;
-    const uint32_t inside = s.inside, from = least + (s.pick << shift), to = min(largest, from + ((1u << shift) - 1u));
+    const uint32_t inside = s.inside, from = least + (s.pick << shift), to = from + min(largest - from, (1u << shift) - 1u);
     if (shift == 0) {
       __syncthreads();  // (s.pick is written again by the next selection)
       return from;
@@ -579,7 +579,7 @@ __global__ void __launch_bounds__(32 * kBsMostWarps, kD == 0 && kTiles > 1 ? 1 :
     for (int i = threadIdx.x; i < kBsBins; i += threads) s.hist[i] = 0;
   pdl_wait();
   pdl_release();
-  int len = p.seq_lens[row];
+  int len = max(p.seq_lens[row], 0);
   if (len > (long long)p.table_width * p.block_size) {
     if (threadIdx.x == 0 && rank == 0) atomicOr(p.status, NVJ_DEV_BAD_LENGTH);
     len = p.table_width * p.block_size;

@@ -44,7 +44,7 @@ struct SelectedParams {
 
 // Keys that a token of row `row` sees.
 __device__ __forceinline__ int sd_visible(const SelectedParams& p, int row, int token) {
-  int len = p.seq_lens[row];
+  int len = max(p.seq_lens[row], 0);
   if (len > (long long)p.table_width * p.block_size) {
     if (threadIdx.x == 0) atomicOr(p.status, NVJ_DEV_BAD_LENGTH);
     len = p.table_width * p.block_size;

@@ -325,6 +325,20 @@ def test_a_selection_flags_blocks_outside_the_pool_and_ranks_them_last():
         S.select_blocks(q, bounds, _i32(np.arange(40)[None]), _i32([641]), 16, 38)
 
 
+@pytest.mark.parametrize("types", [(BF16, BF16), (F32, F32)], ids=str)
+def test_rows_of_negative_lengths_see_nothing(types):
+    """Down to the smallest integer, whatever the position says."""
+    g = _gen(15)
+    k = _normal(g, types[1], 40, 16, 2, 128)
+    bounds = torch.stack((k.amin(1), k.amax(1)), 2).contiguous()
+    tables, lens, pos = _i32(np.tile(np.arange(40), (4, 1))), _i32([-1, -2 ** 31, 0, 600]), _i32([[7], [600], [0], [-2 ** 31]])
+    q = _normal(g, types[0], 4, 1, 8, 128)
+    chosen = S.select_blocks(q, bounds, tables, lens, 16, 5, positions=pos)
+    assert (chosen == -1).all()
+    everything = _i32(np.tile(np.arange(40), (4, 1, 2, 1)))
+    assert (S.paged_decode_attention_selected(q, k, k, tables, lens, everything, 0.1, positions=pos) == 0).all()
+
+
 # ------------------------------------------------------------------------------------------------ attention
 
 def _attention(seed, layout, types, lens, positions, entries, scale=None, spoil=True):
