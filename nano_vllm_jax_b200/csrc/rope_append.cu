@@ -75,6 +75,41 @@ __device__ __forceinline__ QRaw<C> ra_pack(const float (&x)[8]) {
   }
   return r;
 }
+// The smaller and the larger of two words of numbers of the type C, NaN where either is.
+template <typename C, bool kLarger>
+__device__ __forceinline__ uint32_t ra_end(uint32_t a, uint32_t b) {
+  if constexpr (sizeof(C) == 4) {
+    return __float_as_uint(kLarger ? ra_max(__uint_as_float(a), __uint_as_float(b)) : ra_min(__uint_as_float(a), __uint_as_float(b)));
+  } else {
+    using Pair = typename std::conditional<std::is_same<C, __half>::value, __half2, __nv_bfloat162>::type;
+    const Pair x = *reinterpret_cast<const Pair*>(&a), y = *reinterpret_cast<const Pair*>(&b), z = kLarger ? __hmax2_nan(x, y) : __hmin2_nan(x, y);
+    return *reinterpret_cast<const uint32_t*>(&z);
+  }
+}
+template <typename C, bool kLarger>
+__device__ __forceinline__ uint4 ra_ends4(const uint4& a, const uint4& b) {
+  return make_uint4(ra_end<C, kLarger>(a.x, b.x), ra_end<C, kLarger>(a.y, b.y), ra_end<C, kLarger>(a.z, b.z), ra_end<C, kLarger>(a.w, b.w));
+}
+// Bounds of eight dims, as they are stored.
+template <typename C>
+struct RaEnds {
+  QRaw<C> low, high;
+  __device__ __forceinline__ void clear() {
+    constexpr uint32_t up = sizeof(C) == 4 ? 0x7f800000u : std::is_same<C, __half>::value ? 0x7c007c00u : 0x7f807f80u;  // infinities
+    constexpr uint32_t down = up | (sizeof(C) == 4 ? 0x80000000u : 0x80008000u);
+    low.v = make_uint4(up, up, up, up);
+    high.v = make_uint4(down, down, down, down);
+    if constexpr (sizeof(C) == 4) low.w = low.v, high.w = high.v;
+  }
+  __device__ __forceinline__ void take(const QRaw<C>& smaller, const QRaw<C>& larger) {
+    low.v = ra_ends4<C, false>(low.v, smaller.v);
+    high.v = ra_ends4<C, true>(high.v, larger.v);
+    if constexpr (sizeof(C) == 4) {
+      low.w = ra_ends4<C, false>(low.w, smaller.w);
+      high.w = ra_ends4<C, true>(high.w, larger.w);
+    }
+  }
+};
 template <typename C>
 __device__ __forceinline__ void ra_store(C* at, const QRaw<C>& r) {
   *reinterpret_cast<uint4*>(at) = r.v;
@@ -239,9 +274,8 @@ __device__ __forceinline__ void ra_run(const RopeAppendParams& p, int first, int
   bool made = false, begins = false;
   for (int head = head0; head < head1; ++head) {
     C* base = static_cast<C*>(is_v ? p.v_cache : p.k_cache) + (((long long)id * p.block_size - (long long)block * p.block_size) * p.hkv + head) * p.d + col;
-    float low[8], high[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) low[j] = INFINITY, high[j] = -INFINITY;
+    RaEnds<C> ends;
+    ends.clear();
     for (int at = 0; at < n; at += kRaHold * kStep) {
       QRaw<T> raw[kRaHold];
       int pos[kRaHold];
@@ -292,9 +326,7 @@ __device__ __forceinline__ void ra_run(const RopeAppendParams& p, int first, int
           ra_store<C>(base + (long long)pos[s] * slot, w);
           if (bounded) {
             begins |= pos[s] == block * p.block_size;
-            q_floats(w, x);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) low[j] = ra_min(low[j], x[j]), high[j] = ra_max(high[j], x[j]);
+            ends.take(w, w);
           }
         }
       }
@@ -302,41 +334,21 @@ __device__ __forceinline__ void ra_run(const RopeAppendParams& p, int first, int
     if (!bounded) continue;
     begins = __any_sync(kFullMask, begins);
 #pragma unroll
-    for (int o = kLanes; o < 32; o <<= 1)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        low[j] = ra_min(low[j], __shfl_xor_sync(kFullMask, low[j], o));
-        high[j] = ra_max(high[j], __shfl_xor_sync(kFullMask, high[j], o));
-      }
+    for (int o = kLanes; o < 32; o <<= 1) ends.take(ra_shuffle(ends.low, lane ^ o), ra_shuffle(ends.high, lane ^ o));
     if constexpr (kShare > 1) {
-      __shared__ __align__(16) float ends[kRaWarps][512];
+      __shared__ __align__(16) QRaw<C> of_warps[kRaWarps][2][32];
       begins = __syncthreads_or(begins);  // (and the ends of the head before have been read)
-      if (lane_row == 0 && inside)
-#pragma unroll
-        for (int j = 0; j < 8; j += 4) {
-          *reinterpret_cast<float4*>(&ends[warp][col + j]) = make_float4(low[j], low[j + 1], low[j + 2], low[j + 3]);
-          *reinterpret_cast<float4*>(&ends[warp][256 + col + j]) = make_float4(high[j], high[j + 1], high[j + 2], high[j + 3]);
-        }
+      if (lane_row == 0 && inside) of_warps[warp][0][lane] = ends.low, of_warps[warp][1][lane] = ends.high;
       __syncthreads();
       if ((head - head0) % kShare == warp && lane_row == 0 && inside)  // (the heads in turn)
 #pragma unroll
-        for (int w = 0; w < kShare; ++w)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) low[j] = ra_min(low[j], ends[w][col + j]), high[j] = ra_max(high[j], ends[w][256 + col + j]);
+        for (int w = 0; w < kShare; ++w) ends.take(of_warps[w][0][lane], of_warps[w][1][lane]);
     }
     if ((kShare == 1 || (head - head0) % kShare == warp) && lane_row == 0 && inside) {
       C* at = static_cast<C*>(p.bounds) + ((long long)id * p.hkv + head) * 2 * p.d + col;
-      if (!begins) {
-        float x[8];
-        q_floats(q_load8(at), x);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) low[j] = ra_min(low[j], x[j]);
-        q_floats(q_load8(at + p.d), x);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) high[j] = ra_max(high[j], x[j]);
-      }
-      ra_store<C>(at, ra_pack<C>(low));
-      ra_store<C>(at + p.d, ra_pack<C>(high));
+      if (!begins) ends.take(q_load8(at), q_load8(at + p.d));
+      ra_store<C>(at, ends.low);
+      ra_store<C>(at + p.d, ends.high);
     }
   }
 }
