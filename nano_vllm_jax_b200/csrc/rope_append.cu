@@ -12,7 +12,7 @@
 // several heads.  A row is held by 8, 16 or 32 lanes, 8 elements each; its pairs meet by a shuffle of the loaded words.  Cosines and
 // sines go through shared memory, and serve all heads that the warp takes.
 // Bytes: tokens * head_dim * (2 hq + 2 hkv) * element.  Small calls are launch and the chain positions -> block id -> rows, old bounds -> stores: 256 tokens of 8 heads over 2 of 256,
-// one per row, 4.5 us.  Prompts: 16384 bf16 tokens, 64 dims rotated, 47.7 us (203 MB: 31 at the copy rate; without rotation 42), 777 f32 tokens of 32 heads over 8 of 128 12.7 (5.9): instructions, 150 for a row, and
+// one per row, 4.5 us.  Prompts: 16384 bf16 tokens, 64 dims rotated, 45.5 us (203 MB: 31 at the copy rate), 777 f32 tokens of 32 heads over 8 of 128 12.8 (5.9): instructions, some 140 for a row (bounds as they are stored, two numbers of 16 bits at a time, spared 2 us), and
 // the chain of a K or V CTA, of which five fit an SM.
 
 #include "quantized_kv.cuh"
