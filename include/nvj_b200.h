@@ -550,8 +550,8 @@ int nvj_rope_kv_append(const void* q, int64_t q_token_stride, int64_t q_head_str
  * and, with positions given ([rows, width]), p <= positions[b, t].  A block's score for a kv head is the largest, over the group's query heads, of
  *     sum_d max(q_d, 0) high_d + min(q_d, 0) low_d
  * (with a positive scale an upper bound of its keys' scores).  Chosen are the `first` first and the `last` last blocks (first + last <= budget)
- * and of the others those of the highest scores, ties by the lowest column, as sums in 64 bits rank them.  A score that is NaN (as with any bound that is not finite) or beyond f32 ranks as infinity; a block id outside the pool is flagged and
- * its block ranks last.  A length beyond the block table is flagged and clipped.
+ * and of the others those of the highest scores, ties by the lowest column, as sums in 64 bits rank them, whatever their size.  A score that is NaN (as with any bound that is not finite) ranks as infinity; a block id outside the pool is
+ * flagged and its block ranks behind all others.  A length beyond the block table is flagged and clipped.
  *   selected [rows, width, num_kv_heads, budget] int32: columns of the row's block table, ascending, -1 behind them.
  * table_width up to 45056, otherwise NVJ_ERR_TOO_LARGE.
  */

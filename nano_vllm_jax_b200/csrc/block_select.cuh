@@ -3,12 +3,13 @@
 //   score(b) = max over the heads g of the kv head's group of  sum_d max(q_gd, 0) high_bd + min(q_gd, 0) low_bd
 // which no key of block b exceeds: low and high are the bounds of its keys (rope_append.cu).  Chosen are the `first` first and the
 // `last` last blocks that the token sees and, of the others, those of the highest scores; ties go to the lowest column.  A score
-// that is NaN, or beyond fp32, ranks as infinity.
+// that is NaN ranks as infinity; blocks outside the pool rank behind all others.
 //
 // Columns are whole numbers, so the border between chosen and left has to lie where it lies in exact arithmetic.  The scores are
 // sums in fp32 whose error is bounded by eps = c * (the largest sum of the products' magnitudes of all blocks), c from the number of
 // roundings; with t the border's score, blocks above t + 2 eps are in and those below t - 2 eps are out whatever was rounded, and the
-// few between the two are scored again in 64 bits.  Usually that is the block at the border alone, and nothing is left to decide.  (With |q|_1 * (largest |bound|)
+// few between the two are scored again in 64 bits.  Usually that is the block at the border alone, and nothing is left to decide.  Scores that fp32 sums
+// did not hold are scored in 64 bits first, and if numbers are among them eps is infinite.  (With |q|_1 * (largest |bound|)
 // in place of that sum and the tensor cores' sums over all dims in one, 2 - 8 blocks stood between in nearly every selection: 5 us for
 // four rows, 12 - 19 for long ones.)
 //
@@ -18,6 +19,8 @@
 // of 256, 336 MB in 78 us (51 at the copy rate), 256 of 128 - 512 41 (26), 4 rows of 512 7.4.
 
 #pragma once
+
+#include <cfloat>
 
 #include "cluster.cuh"
 #include "decode_cluster.cuh"
@@ -44,6 +47,8 @@ constexpr int kBsMostColumns = 45056;  // of a row: their scores fit one SM's sh
 constexpr int kBsMostCtas = 8;
 constexpr int kBsFew = 32;                    // keys that a warp ranks at once
 constexpr uint32_t kBsInfinity = 0xff800000u;  // bs_key(+infinity)
+constexpr uint32_t kBsLowest = 0x007fffffu;    // bs_key(-infinity)
+constexpr uint32_t kBsMissing = 0u;            // a block outside the pool: below every score (kBsLowest at first)
 
 // Floats as integers of the same order; NaN as infinity.
 __device__ __forceinline__ uint32_t bs_key(float x) {
@@ -196,7 +201,9 @@ __device__ __forceinline__ float4 bs_load4(const void* p, long long i, int dtype
   return make_float4(a.x, a.y, b.x, b.y);
 }
 
-// Score of one block in 64 bits, by a warp; the same in every lane.
+// Score of one block in 64 bits, by a warp; the same in every lane.  kStrict: bounds and queries may be no numbers, and what they make is kept (a query of any sign
+// against a bound that is not finite on either side: NaN or infinity, as the formula has it).
+template <bool kStrict = false>
 static __device__ double bs_exact(const SelectParams& p, long long q_at, long long bounds_at, int lane) {
   double best = -INFINITY;
   for (int g0 = 0; g0 < p.groups; g0 += 4) {  // four heads' loads in flight
@@ -215,21 +222,28 @@ static __device__ double bs_exact(const SelectParams& p, long long q_at, long lo
         sum[g] += (double)q[g].y * (double)(q[g].y > 0.f ? high.y : low.y);
         sum[g] += (double)q[g].z * (double)(q[g].z > 0.f ? high.z : low.z);
         sum[g] += (double)q[g].w * (double)(q[g].w > 0.f ? high.w : low.w);
+        if constexpr (kStrict) {  // zero times the other bounds
+          sum[g] += 0.0 * (double)(q[g].x > 0.f ? low.x : high.x);
+          sum[g] += 0.0 * (double)(q[g].y > 0.f ? low.y : high.y);
+          sum[g] += 0.0 * (double)(q[g].z > 0.f ? low.z : high.z);
+          sum[g] += 0.0 * (double)(q[g].w > 0.f ? low.w : high.w);
+        }
       }
     }
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) sum[g] += __shfl_xor_sync(kFullMask, sum[g], o);
-      if (g0 + g < p.groups) best = sum[g] > best ? sum[g] : best;
+      if (g0 + g < p.groups) best = sum[g] > best || (kStrict && sum[g] != sum[g]) ? sum[g] : best;
     }
   }
   return best;
 }
 
-// `f(column, score in 64 bits)` by the warps of the CTA, for the columns whose key is `key`; in batches of what the list holds, which is left at zero.
-template <class F>
-__device__ __forceinline__ void bs_rescore(const SelectParams& p, BsShared& s, const uint32_t* keys, const int32_t* table, long long q_at, int head,
+// `f(column, score in 64 bits)` by the warps of the CTA, for the columns whose key is `key`; in batches of what the list holds, which is left at zero.  kStrict: for the columns whose keys are
+// no number's (from kBsInfinity on and round to kBsLowest), of blocks that may be outside the pool; those get kBsMissing.
+template <bool kStrict = false, class F>
+__device__ __forceinline__ void bs_rescore(const SelectParams& p, BsShared& s, uint32_t* keys, const int32_t* table, long long q_at, int head,
                                            int begin, int end, uint32_t key, F&& f) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, threads = blockDim.x;
   for (int base = begin; base < end; base += kBsBins) {
@@ -238,12 +252,16 @@ __device__ __forceinline__ void bs_rescore(const SelectParams& p, BsShared& s, c
     if (threadIdx.x == 0) s.count = 0;
     __syncthreads();
     for (int i = base + threadIdx.x; i < stop; i += threads)
-      if (keys[i] == key) s.hist[atomicAdd(&s.count, 1u)] = i;
+      if (kStrict ? keys[i] - key <= kBsLowest - kBsInfinity : keys[i] == key) s.hist[atomicAdd(&s.count, 1u)] = i;
     __syncthreads();
     const int m = (int)s.count;
     for (int j = warp; j < m; j += threads >> 5) {
-      const int i = (int)s.hist[j];
-      f(i, bs_exact(p, q_at, ((long long)table[i] * p.hkv + head) * 2 * p.d, lane));
+      const int i = (int)s.hist[j], id = table[i];
+      if (kStrict && (id < 0 || id >= p.num_blocks)) {
+        if (lane == 0) keys[i] = kBsMissing;
+        continue;
+      }
+      f(i, bs_exact<kStrict>(p, q_at, ((long long)id * p.hkv + head) * 2 * p.d, lane));
     }
     __syncthreads();
     for (int j = threadIdx.x; j < m; j += threads) s.hist[j] = 0;
@@ -650,6 +668,19 @@ __global__ void __launch_bounds__(32 * kBsMostWarps, kD == 0 && kTiles > 1 ? 1 :
     least = __reduce_min_sync(kFullMask, least);
     largest = __reduce_max_sync(kFullMask, largest);
     for (int w = 0; w < warps; ++w) reach = fmaxf(reach, s.reach[w]);
+    if (largest >= kBsInfinity || least <= kBsLowest) {
+      // Scores that an fp32 sum did not hold: of operands that are no numbers, or sums of numbers that left fp32, be it on the way to one that it holds.  In 64 bits
+      // no sum of numbers does; such a block's place is found below, among all others that are numbers (eps is infinite).
+      bool numbers = false;
+      bs_rescore<true>(p, s, keys, table, q_at, head, begin, end, kBsInfinity, [&](int i, double x) {
+        const bool number = fabs(x) < INFINITY;
+        numbers |= number;
+        if (lane == 0) keys[i] = number ? bs_key(fminf(fmaxf((float)x, -FLT_MAX), FLT_MAX)) : x < 0.0 ? kBsLowest : kBsInfinity;
+      });
+      if (__syncthreads_or(numbers)) most = 0x7f800000u;
+      least = kBsMissing;
+      largest = kBsInfinity;
+    }
     border = bs_nth(keys, begin, end, want, least, largest, s, which, above);
     take_equal = want - above;
     all_equal_in = false;
@@ -661,8 +692,8 @@ __global__ void __launch_bounds__(32 * kBsMostWarps, kD == 0 && kTiles > 1 ? 1 :
       constexpr double kCut = kD > 0 ? 68.0 * kTerms : 16.0, kSlip = kTerms > 1 ? 0x1p-16 : 0.0;
       const double eps = ((kCut + p.d / 16) * 0x1p-23 + kSlip) * 1.01 * (double)__uint_as_float(most) +
                          0x1p-124 * p.d * (1.0 + (double)reach);  // (and products and bounds below the normal numbers, that may be taken for zero)
-      // (blocks that are not there, and scores beyond fp32, stay what they are)
-      const uint32_t low = max(bs_key(__double2float_ru((double)t - 2.0 * eps)), bs_key(-INFINITY) + 1u),
+      // (blocks that are not there, and scores that are no numbers, stay what they are)
+      const uint32_t low = max(bs_key(__double2float_ru((double)t - 2.0 * eps)), kBsLowest + 1u),
                      high = min(bs_key(__double2float_rd((double)t + 2.0 * eps)), kBsInfinity - 1u);
       // how many are in for sure (in the upper half of the sum), and how many stand between
       uint32_t mine = 0;

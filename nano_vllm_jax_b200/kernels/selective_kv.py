@@ -194,7 +194,8 @@ def select_blocks(q, k_bounds, block_table, seq_lens, block_size, budget, *, pos
     q `[B, Hq, D]` -> `[B, Hkv, budget]`, or `[B, T, Hq, D]` -> `[B, T, Hkv, budget]`.  Token t of row b sees the keys p < seq_lens[b] and, with
     `positions` `[B, T]`, p <= positions[b, t].  Of the blocks that hold them the `first` first and the `last` last are taken, and of the others those whose
     `sum(max(q, 0) * high + min(q, 0) * low)`, the largest of the kv head's query heads, is highest (ties: the lowest column), an upper bound of
-    their keys' scores under a positive scale.  A score that is not a number, or beyond float32, ranks as infinity.
+    their keys' scores under a positive scale.  Scores rank as sums in 64 bits; one that is not a number ranks as infinity, and a block outside the pool
+    (flagged) behind all others.
     """
     out = _k.host().select_blocks(q, k_bounds, block_table, seq_lens, block_size, budget, positions, first, last)
     if out is not None:
