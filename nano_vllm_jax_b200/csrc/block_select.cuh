@@ -688,8 +688,9 @@ __global__ void __launch_bounds__(32 * kBsMostWarps, kD == 0 && kTiles > 1 ? 1 :
     if (t - t == 0.f) {
       // Products are exact on the tensor cores (in a chain of fused multiply-adds, too).  A sum of 32 dims is four steps for each term of the
       // queries, each cuts up to 17 numbers at 2^-23 of the largest: 68 * 2^-23 of the magnitudes for a term; D / 32 of them are added up in fp32.  Two
-      // terms leave 2^-16 of a query at most.  The magnitudes' own sum is off by a thousandth at most.
-      constexpr double kCut = kD > 0 ? 68.0 * kTerms : 16.0, kSlip = kTerms > 1 ? 0x1p-16 : 0.0;
+      // terms of eight bits, both cut, leave 2^-15 of a query at most (with the second one rounded 2^-16, and the compiler spills: 256 rows 51 us instead of
+      // 45).  The magnitudes' own sum is off by a thousandth at most.
+      constexpr double kCut = kD > 0 ? 68.0 * kTerms : 16.0, kSlip = kTerms > 1 ? 0x1p-15 : 0.0;
       const double eps = ((kCut + p.d / 16) * 0x1p-23 + kSlip) * 1.01 * (double)__uint_as_float(most) +
                          0x1p-124 * p.d * (1.0 + (double)reach);  // (and products and bounds below the normal numbers, that may be taken for zero)
       // (blocks that are not there, and scores that are no numbers, stay what they are)

@@ -1,4 +1,4 @@
-"""Selection of blocks where scores leave fp32, or blocks of a row are not in the pool."""
+"""Selection of blocks where scores leave fp32 or differ by less than it tells apart, or blocks of a row are not in the pool."""
 
 import numpy as np
 import pytest
@@ -94,3 +94,23 @@ def test_blocks_outside_the_pool_rank_behind_every_other(layout, types, below, u
                 assert np.array_equal(got[b, 0, h], R.choose(score, 40, budget, 1, 2)), (budget, b, h)
     with pytest.raises(K.DeviceStatusError, match="outside the pool|sequence length"):
         K.check_device_status()
+
+
+@pytest.mark.parametrize("layout", [(4, 2, 64, 16), (8, 2, 128, 16), MODEL, (12, 1, 96, 16)], ids=str)
+def test_queries_of_the_largest_rest_over_bf16_bounds(layout):
+    """Queries of which two cut terms leave the most, 255 * 2^-23 of them, in half of the dims, exact ones in the others; blocks whose scores differ by less."""
+    worst = torch.tensor([0x3F8080FF], dtype=torch.int32).view(F32).item()
+
+    def near(q, bounds, tables):
+        sign = torch.where(torch.rand_like(q) < 0.5, -1.0, 1.0)
+        q[:] = sign * worst
+        q[..., ::2] = sign[..., ::2]
+        of = torch.arange(len(bounds), device="cuda")
+        bounds[:] = 0.0
+        bounds[of, :, 0, :], bounds[of, :, 1, :] = -1.0, 1.0  # every block the same, then one unit moved between a dim with a rest and one without
+        where = 2 * (of % (layout[2] // 2))
+        bounds[of, :, 0, where], bounds[of, :, 1, where] = -1.0 - 2.0 ** -7, 1.0 + 2.0 ** -7
+        other = 2 * ((of // 7) % (layout[2] // 2)) + 1
+        bounds[of, :, 0, other], bounds[of, :, 1, other] = -1.0 + 2.0 ** -7, 1.0 - 2.0 ** -7
+    for budget in (5, 32, 100):
+        _selection(23, layout, (F32, BF16), [16 * 110, 16 * 700], None, budget, 1, 2, near)
