@@ -609,7 +609,7 @@ __global__ void __launch_bounds__(32 * kBsMostWarps, kD == 0 && kTiles > 1 ? 1 :
   if (ctas > 1) cl_wait();
   if (n <= p.budget) {  // all of them
     if (rank == 0)
-      for (int i = threadIdx.x; i < p.budget; i += threads) out[i] = i < n ? i : -1;
+      for (unsigned i = threadIdx.x; i < (unsigned)p.budget; i += threads) out[i] = i < (unsigned)n ? (int)i : -1;  // (the step behind the largest budget passes 2^31)
     return;
   }
   const int32_t* table = p.block_tables + (long long)row * p.table_width;

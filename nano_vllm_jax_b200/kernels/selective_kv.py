@@ -22,6 +22,8 @@ from . import paged_kv as _k
 from .quantized_kv import _ints, _on, _rows
 
 MOST_COLUMNS = 45056  # block-table columns that a selection takes (nvj_select_blocks)
+MOST_BUDGET = 2 ** 31 - 1
+MOST_BLOCK_SIZE = 65536
 
 
 def selective_cache_supported(dtype, head_dim: int) -> bool:
@@ -31,8 +33,8 @@ def selective_cache_supported(dtype, head_dim: int) -> bool:
 
 def check_budget(budget: int, first: int, last: int) -> None:
     """A budget of blocks, the first and last ones of a row among them."""
-    if budget < 1 or first < 0 or last < 0 or first + last > budget:
-        raise ValueError(f"budget must be positive and hold the first and last blocks, not {budget} with {first} and {last}")
+    if budget < 1 or first < 0 or last < 0 or first + last > budget or budget > MOST_BUDGET:
+        raise ValueError(f"budget must be positive, at most {MOST_BUDGET}, and hold the first and last blocks, not {budget} with {first} and {last}")
 
 
 def _pages(name, t, like=None):
@@ -209,8 +211,8 @@ def select_blocks(q, k_bounds, block_table, seq_lens, block_size, budget, *, pos
     q = _rows("q", q, device)
     budget, first, last, block_size = int(budget), int(first), int(last), int(block_size)
     check_budget(budget, first, last)
-    if block_size < 1:
-        raise ValueError("block_size must be positive")
+    if not 1 <= block_size <= MOST_BLOCK_SIZE:
+        raise ValueError(f"block_size must be positive and at most {MOST_BLOCK_SIZE}, not {block_size}")
     block_table, seq_lens, positions = _batch(block_table, seq_lens, positions, batch, width, device)
     if block_table.shape[1] > MOST_COLUMNS:
         raise ValueError(f"a selection takes block tables of up to {MOST_COLUMNS} columns, not {block_table.shape[1]}")

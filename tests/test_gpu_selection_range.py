@@ -114,3 +114,19 @@ def test_queries_of_the_largest_rest_over_bf16_bounds(layout):
         bounds[of, :, 0, other], bounds[of, :, 1, other] = -1.0 + 2.0 ** -7, 1.0 - 2.0 ** -7
     for budget in (5, 32, 100):
         _selection(23, layout, (F32, BF16), [16 * 110, 16 * 700], None, budget, 1, 2, near)
+
+
+def test_the_largest_budget_lists_every_block():
+    """2^31 - 1 places, 8.6 GB: the row's columns, then -1 to the last one."""
+    bounds = torch.zeros(5, 1, 2, 8, dtype=BF16, device="cuda")
+    out = S.select_blocks(torch.zeros(1, 1, 8, dtype=BF16, device="cuda"), bounds, _i32([[4, 0, 2, 1, 3]]), _i32([33]), 16, S.MOST_BUDGET)
+    assert out.shape == (1, 1, S.MOST_BUDGET) and out[0, 0, :3].tolist() == [0, 1, 2]
+    for part in out[0, 0, 3:].split(1 << 28):
+        assert (part == -1).all()
+
+
+@pytest.mark.parametrize("budget,block_size", [(2 ** 31, 16), (2 ** 32 + 4, 16), (4, 2 ** 16 + 1), (4, 2 ** 32 + 16)])
+def test_numbers_that_a_call_cannot_hold_are_refused(budget, block_size):
+    bounds = torch.zeros(5, 1, 2, 8, dtype=BF16, device="cuda")
+    with pytest.raises(ValueError, match="at most"):
+        S.select_blocks(torch.zeros(1, 1, 8, dtype=BF16, device="cuda"), bounds, _i32([[4, 0, 2, 1, 3]]), _i32([33]), block_size, budget)
