@@ -361,8 +361,8 @@ class B200Backend:
             raise ValueError("positions and block_tables batch dimensions must match")
         if metadata.max_kv_len is not None and metadata.max_kv_len < tables.shape[1] * block_size:
             lens = lens.clamp(max=int(metadata.max_kv_len))
-        chosen = _s.select_blocks(query, bounds, tables, lens, block_size, cache.budget, positions=positions, first=cache.first,
-                                  last=cache.last)
+        budget = min(cache.budget, max(tables.shape[1], cache.first + cache.last, 1))  # (no row has more blocks than its table has columns)
+        chosen = _s.select_blocks(query, bounds, tables, lens, block_size, budget, positions=positions, first=cache.first, last=cache.last)
         return _s.paged_decode_attention_selected(query, k_layer, v_layer, tables, lens, chosen, scale, positions=positions)
 
 

@@ -24,6 +24,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdlib>
 #include <cstring>
@@ -921,8 +922,9 @@ PyObject* selective_step(PyObject* const* a, Py_ssize_t n) {
   if (!args_are(n, 18)) return nullptr;
   const at::Tensor *q = tensor(a[0]), *k = tensor(a[1]), *v = tensor(a[2]), *kc = tensor(a[3]), *b = tensor(a[5]), *tab = tensor(a[7]), *len = tensor(a[8]),
                    *pos = tensor(a[9]), *qsl = tensor(a[10]);
-  const long long layer = PyLong_AsLongLong(a[6]), bs = PyLong_AsLongLong(a[11]), groups = PyLong_AsLongLong(a[13]), budget = PyLong_AsLongLong(a[14]),
-                  first = PyLong_AsLongLong(a[15]), last = PyLong_AsLongLong(a[16]);
+  const long long layer = PyLong_AsLongLong(a[6]), bs = PyLong_AsLongLong(a[11]), groups = PyLong_AsLongLong(a[13]), first = PyLong_AsLongLong(a[15]),
+                  last = PyLong_AsLongLong(a[16]);
+  long long budget = PyLong_AsLongLong(a[14]);
   const double scale = PyFloat_AsDouble(a[12]);
   const long long max_len = a[17] == Py_None ? -1 : PyLong_AsLongLong(a[17]);
   if (PyErr_Occurred()) { PyErr_Clear(); NVJ_NONE(); }
@@ -943,6 +945,7 @@ PyObject* selective_step(PyObject* const* a, Py_ssize_t n) {
   if (!on(*b, l.device) || b->dtype() != kc->dtype() || b->dim() != 5 || b->size(0) != kc->size(0) || b->size(1) != l.blocks || b->size(2) != l.hkv ||
       b->size(3) != 2 || b->size(4) != l.d || !b->is_contiguous())
     NVJ_NONE();
+  budget = std::min<long long>(budget, std::max<long long>(tab->size(1), first + last));  // (no row has more blocks than its table has columns)
   l.bounds = static_cast<char*>(b->data_ptr()) + layer * l.blocks * l.hkv * 2 * l.d * (long long)b->element_size();
   if (reinterpret_cast<uintptr_t>(l.bounds) & 15) NVJ_NONE();
   const c10::cuda::OptionalCUDAGuard guard(c10::Device(c10::kCUDA, (c10::DeviceIndex)l.device));
