@@ -87,6 +87,8 @@ class B200Backend:
         # not in the reference: decode reads this many blocks of a row (config.full_attention_selected_blocks; 0 or None: all of them)
         budget = getattr(self.config, "full_attention_selected_blocks", None)
         if budget:
+            if max_blocks_per_seq is not None and max_blocks_per_seq > _s.MOST_COLUMNS:  # decode would refuse them at its first step
+                raise ValueError(f"a selection takes block tables of up to {_s.MOST_COLUMNS} columns, not {max_blocks_per_seq}")
             first, last = (getattr(self.config, f"full_attention_selected_{end}", 1) for end in ("first", "last"))
             return kvc.init_selective_kv_cache(capped, budget, first, last, device=self.device)
         if dtype == torch.float8_e4m3fn:
