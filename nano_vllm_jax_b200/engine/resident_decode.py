@@ -147,6 +147,9 @@ class DecodeStepGraph:
             raise ValueError("k_cache must be the 5-D cache [L, NB, bs, Hkv, D]")
         if k_cache.dtype == torch.float8_e4m3fn:
             raise ValueError("DecodeStepGraph does not take 8-bit caches (capture their append and decode in a CapturedStep)")
+        if getattr(k_cache, "has_key_bounds", False) or getattr(v_cache, "has_key_bounds", False):
+            raise ValueError("DecodeStepGraph does not take the pages of a selective cache, whose key bounds its append would leave behind "
+                             "(capture the backend's step in a CapturedStep)")
         self.meta, self.k_cache, self.v_cache = meta, k_cache, v_cache
         self.layer_id, self.scale, self.groups = int(layer_id), float(scale), int(num_key_value_groups)
         _, _, bs, hkv, d = k_cache.shape

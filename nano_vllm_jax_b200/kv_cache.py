@@ -65,13 +65,20 @@ class SelectiveKVCacheStorage(KVCacheStorage):
     """A cache whose decode attention reads selected blocks (not in the reference): beside the pages `[num_layers, num_blocks, block_size,
     num_kv_heads, head_dim]` the bounds of every block's keys `[num_layers, num_blocks, num_kv_heads, 2, head_dim]` (the smallest
     number of each dimension, then the largest), kept by the append.  Of a row's blocks decode reads the `first` first, the `last`
-    last and those of the highest scores, `budget` in all (`kernels/selective_kv.py`); prefill reads all of them.  The backend's own appends keep
-    the bounds; kernels that write the pages alone (fused append and decode, a captured `DecodeStepGraph`) leave them behind."""
+    last and those of the highest scores, `budget` in all (`kernels/selective_kv.py`); prefill, with the decode rows of a
+    mixed batch, reads all of them.  The backend's own appends keep the bounds.  What writes the pages alone leaves them behind, and the next selection ranks by
+    numbers that are no longer those of the keys: `paged_kv.copy_blocks` (take `copy_blocks` below), `kv_append_slots`, `qk_norm_rope_kv_append` and
+    `paged_decode_attention_with_kv_append` are not for such a cache; `DecodeStepGraph` and `HostDecodePipeline` refuse it.  Bounds only widen until a block begins anew:
+    a token that is written again at a place behind the block's first, as after rejected speculation, leaves the old key within them.  Scores stay upper bounds, looser ones."""
 
     k_bounds: torch.Tensor
     budget: int
     first: int = 1
     last: int = 1
+
+    def __post_init__(self):
+        for pages in (self.k_cache, self.v_cache):  # for callers that are handed the pages alone
+            pages.has_key_bounds = True
 
     def layer(self, layer_id: int):
         """(k, v, k_bounds) of one layer, as the kernels of `kernels/selective_kv.py` take them."""
