@@ -102,3 +102,45 @@ def test_decode_rows_of_a_mixed_batch_read_every_key():
     assert type(cache) is kvc.SelectiveKVCacheStorage
     assert torch.equal(out, plain.attention(0, q, kvc.KVCacheStorage(cache.k_cache, cache.v_cache), md, bs, d ** -0.5, hq // hkv, True))
     _bounds_hold(cache, 0, tables, cached + new)
+
+
+def test_the_backend_step_replayed_from_a_graph(monkeypatch):
+    """Captured once, replayed with other tokens, positions and lengths: as a twin's steps made one by one."""
+    monkeypatch.setenv("NVJ_CHECK_STATUS", "0")  # (reading the status back is no part of a graph)
+    hq, hkv, d, bs = 6, 3, 96, 16
+    rows, backend, g = 5, B200Backend(_Config()), _gen(30)
+    caches = [backend.allocate_kv_cache(kvc.KVCacheSpec(1, 200, bs, hkv, d, BF16), rows, 40) for _ in range(2)]
+    for t in (caches[0].k_cache, caches[0].v_cache):
+        t.copy_(_normal(g, BF16, *t.shape))
+    caches[0].k_bounds.copy_(torch.stack((caches[0].k_cache.amin(2), caches[0].k_cache.amax(2)), 3))
+    for a, b in zip((caches[1].k_cache, caches[1].v_cache, caches[1].k_bounds), (caches[0].k_cache, caches[0].v_cache, caches[0].k_bounds)):
+        a.copy_(b)
+    q, k, v = (_normal(g, BF16, rows, 1, h, d) for h in (hq, hkv, hkv))
+    tables, pos, lens = _i32(np.arange(200).reshape(rows, 40)), _i32(np.zeros((rows, 1))), _i32(np.zeros(rows))
+    start = np.array([100, 15, 0, 600, 320])
+
+    def fill(step):
+        for t in (q, k, v):
+            t.copy_(_normal(g, BF16, *t.shape))
+        pos.copy_(_i32((start + step)[:, None]))
+        lens.copy_(_i32(start + step + 1))
+
+    def run(cache):
+        md = backend.build_attention_metadata(pos, tables, lens, bs, False)
+        return backend.write_kv_and_attention(0, q, k, v, cache, md, bs, d ** -0.5, hq // hkv, False)[1]
+    fill(0)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for cache in caches:  # (the twin's bounds widen by this step's keys too)
+            run(cache)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run(caches[0])
+    for step in range(20):
+        fill(step)
+        graph.replay()
+        assert torch.equal(out, run(caches[1]))
+    for a, b in zip((caches[0].k_cache, caches[0].v_cache, caches[0].k_bounds), (caches[1].k_cache, caches[1].v_cache, caches[1].k_bounds)):
+        assert torch.equal(a, b)
