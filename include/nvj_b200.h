@@ -564,7 +564,9 @@ int nvj_select_blocks(const void* q, int q_dtype, const void* k_bounds, int cach
  * Attention of each query token over listed blocks: masks as above, keys those of the blocks in selected [rows, width, num_kv_heads, entries].
  * An entry below 0, or of a block that the token does not see, adds nothing; every other counts, also one that is listed twice.
  * out [rows, width, num_q_heads, head_dim] float32; a token without keys gets zeros.  Keys behind the last one that a token
- * sees may hold anything.  A block id outside the pool is flagged and its keys left out.  The scale may be any number.
+ * sees may hold anything.  A number of K or V that a token does see and that is not finite makes the outputs that it reaches not finite: over 16-bit caches NaN
+ * also where an infinite V alone would make them infinite, since weights are sums of terms, of any sign or zero (as in the other decode kernels).  A block id outside the pool
+ * is flagged and its keys left out.  The scale may be any number.
  */
 int nvj_paged_decode_selected(const void* q, int q_dtype, const void* k_cache_layer, const void* v_cache_layer, int cache_dtype,
                               int64_t num_blocks, int block_size, int num_kv_heads, int head_dim, int num_q_heads,

@@ -12,8 +12,9 @@
 // several heads.  A row is held by 8, 16 or 32 lanes, 8 elements each; its pairs meet by a shuffle of the loaded words.  Cosines and
 // sines go through shared memory, and serve all heads that the warp takes.
 // Bytes: tokens * head_dim * (2 hq + 2 hkv) * element.  Small calls are launch and the chain positions -> block id -> rows, old bounds -> stores: 256 tokens of 8 heads over 2 of 256,
-// one per row, 4.5 us.  Prompts: 16384 bf16 tokens, 64 dims rotated, 45.5 us (203 MB: 31 at the copy rate), 777 f32 tokens of 32 heads over 8 of 128 12.8 (5.9): instructions, some 140 for a row (bounds as they are stored, two numbers of 16 bits at a time, spared 2 us), and
-// the chain of a K or V CTA, of which five fit an SM.
+// one per row, 4.6 us.  Prompts: 16384 bf16 tokens, 64 dims rotated, 45.5 us (203 MB: 31 at the copy rate), 777 f32 tokens of 32 heads over 8 of 128 12.9 (5.9).  Neither bytes (35% of the DRAM's
+// peak) nor issue slots (50%) are full: too few warps, 29% of an SM's (96 registers of a thread, f32 127), wait for results of their own, of memory and for code, some 140
+// instructions for a row in every form that a call may take.  (Bounds as they are stored, two numbers of 16 bits at a time, spared 2 us.)
 
 #include "quantized_kv.cuh"
 

@@ -16,7 +16,8 @@
 //     two terms of the weights are the two halves of the eight columns of one mma.sync.  A tile's products are summed by themselves and added in fp32 (left in the
 //     tensor cores' sums, which cut their last place, 8192 keys 3e-6 - 9e-6 from 64 bits instead of 1e-7 - 5e-7; 2% of the time);
 //   * a warp walks only the tiles that are there: it holds the places of its next 32 in its lanes and takes the set bits of their vote.
-// 256 rows, 64 blocks of 16 keys, 8 heads over 2 of 256: 540 MB in 92 us, 90% of the copy rate; 48 rows, 32 heads over 8 of 128: 51 us, 91%.
+// 256 rows, 64 blocks of 16 keys, 8 heads over 2 of 256: 540 MB in 90.5 us, 91% of the copy rate (f16 89; f32 queries 103); 48 rows, 32 heads over 8 of 128 49.7, 92%.  Other
+// head_dims take the form of three query terms and eight columns: 256 rows of 6 heads over 3 of 96 74.5 us, 62%.
 // Maxima are lazy: one vote per tile says whether a score has left them behind, and only then the sums are rescaled.
 #pragma once
 

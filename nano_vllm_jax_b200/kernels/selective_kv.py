@@ -237,7 +237,8 @@ def paged_decode_attention_selected(q, k_cache_layer, v_cache_layer, block_table
 
     q `[B, Hq, D]` with selected `[B, Hkv, n]` -> float32 `[B, Hq, D]`, or `[B, T, Hq, D]` with `[B, T, Hkv, n]` -> `[B, T, Hq * D]`.  Token t of row b sees, of
     the listed blocks' keys, those with p < seq_lens[b] and, with `positions` `[B, T]`, p <= positions[b, t]; one that sees none gives zeros.  Entries
-    below 0 and blocks that the token does not see add nothing; a block that is listed twice counts twice.
+    below 0 and blocks that the token does not see add nothing; a block that is listed twice counts twice.  Keys that it sees are finite numbers: another makes the
+    outputs that it reaches infinite or NaN.
     """
     out = _k.host().selected_decode(q, k_cache_layer, v_cache_layer, block_table, seq_lens, selected, scale, positions)
     if out is not None:
